@@ -178,8 +178,8 @@ def prepare(case: Case, seed: int) -> dict[str, Any]:
         valid = pos >= 0
         s: dict[str, Any] = {"case": c, "ring_pos": torch.where(valid, pos, torch.zeros_like(pos)), "ring_valid": valid, "pos": seen}
         for name in ("k", "v"):
-            codes, pair = _quantize(_rows(g, c, w))
-            at = valid[:, :, None, None]
+            codes, pair = _quantize(_rows(g, c, w).transpose(1, 2).contiguous())
+            at = valid[:, None, :, None]
             s[f"ring_{name}"] = torch.where(at, _pack(codes), torch.zeros((), dtype=torch.uint8, device="cuda"))
             s[f"ring_{name}_scale"] = torch.where(at, pair, torch.zeros((), dtype=t, device="cuda"))
             s[name] = _rows(g, c, 1)
@@ -191,8 +191,8 @@ def prepare(case: Case, seed: int) -> dict[str, Any]:
         start = torch.randint(0, 2 * w, (b, 1), generator=g, device="cuda")
         last = start + (n if lengths is None else lengths[:, None])
         asked = last - w + torch.arange(w, device="cuda")  # the window's positions in order, oldest first
-        zeros = [torch.zeros(b, w, c["hkv"], c["dk"] // 2, dtype=torch.uint8, device="cuda") for _ in range(2)]
-        pairs = [torch.zeros(b, w, c["hkv"], 2, dtype=t, device="cuda") for _ in range(2)]
+        zeros = [torch.zeros(b, c["hkv"], w, c["dk"] // 2, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        pairs = [torch.zeros(b, c["hkv"], w, 2, dtype=t, device="cuda") for _ in range(2)]
         return {"case": c, "k": _rows(g, c, n), "v": _rows(g, c, n), "pos": start + torch.arange(n, device="cuda"),
                 "lengths": lengths, "asked": asked, "ring_k": zeros[0], "ring_v": zeros[1], "ring_k_scale": pairs[0],
                 "ring_v_scale": pairs[1], "ring_pos": torch.zeros(b, w, dtype=torch.long, device="cuda"),
@@ -270,8 +270,8 @@ def _project_own(s: dict[str, Any], c: Case) -> Any:
 
 def _store(s: dict[str, Any], rows: Tensor, at: Tensor, pos: Tensor, k: Tensor, v: Tensor) -> None:
     """Tokens ``k``, ``v`` at positions ``pos`` quantised into slots ``at`` of the batch rows ``rows``."""
-    s["ring_k"][rows, at], s["ring_k_scale"][rows, at] = _packed(k)
-    s["ring_v"][rows, at], s["ring_v_scale"][rows, at] = _packed(v)
+    s["ring_k"][rows, :, at], s["ring_k_scale"][rows, :, at] = _packed(k)
+    s["ring_v"][rows, :, at], s["ring_v_scale"][rows, :, at] = _packed(v)
     s["ring_pos"][rows, at] = pos
     s["ring_valid"][rows, at] = True
 
@@ -282,8 +282,8 @@ def _attn(s: dict[str, Any], c: Case) -> Any:
     p = s["pos"]
     slot = torch.arange(w, device=p.device)
     seen = s["ring_valid"] & (s["ring_pos"] <= p) & (s["ring_pos"] > p - w) & (slot != p % w)
-    keys = _values(s["ring_k"], s["ring_k_scale"]).transpose(1, 2)  # [b, hkv, w, dk]
-    values = _values(s["ring_v"], s["ring_v_scale"]).transpose(1, 2).contiguous()
+    keys = _values(s["ring_k"], s["ring_k_scale"])  # [b, hkv, w, dk]
+    values = _values(s["ring_v"], s["ring_v_scale"])
     q = s["q"].float().view(b, hkv, group, dk)
     scores = torch.matmul(q, keys.transpose(2, 3).contiguous()) / math.sqrt(dk)
     scores = scores.masked_fill(~seen[:, None, None, :], -math.inf)
@@ -314,7 +314,7 @@ def _cache(s: dict[str, Any], c: Case) -> Any:
     row = torch.arange(c["b"], device=slot.device)[:, None]
     found = s["ring_valid"][row, slot] & (s["ring_pos"][row, slot] == s["asked"])
     top = torch.finfo(t).max
-    keys, values = ((_values(s[f"ring_{name}"][row, slot], s[f"ring_{name}_scale"][row, slot]).clamp(-top, top)
+    keys, values = ((_values(s[f"ring_{name}"][row, :, slot], s[f"ring_{name}_scale"][row, :, slot]).clamp(-top, top)
                      * found[:, :, None, None]).to(t) for name in ("k", "v"))
     return [keys, values, found, s["ring_pos"], s["ring_valid"]]
 
@@ -398,18 +398,18 @@ def _exact_attn(s: dict[str, Any], c: Case) -> Any:
         for kv in range(c["hkv"]):
             rows = []
             for name, pair in zip(("k", "v"), scales):
-                packed = s[f"ring_{name}"][i, use, kv].long()
+                packed = s[f"ring_{name}"][i, kv, use].long()
                 low_high = torch.empty(packed.shape[0], dk, dtype=torch.float64, device="cuda")
                 low_high[:, 0::2], low_high[:, 1::2] = (packed % 16).double(), (packed // 16).double()
-                x = low_high * pair[i, use, kv, 0:1] + pair[i, use, kv, 1:2]
+                x = low_high * pair[i, kv, use, 0:1] + pair[i, kv, use, 1:2]
                 rows.append(torch.cat([x, s[name][i, :, kv].double()]))  # and the new token
             heads = slice(kv * c["group"], (kv + 1) * c["group"])
             weights = torch.softmax(s["q"][i, 0, heads].double() @ rows[0].t() / math.sqrt(dk), -1)
             out[i, 0, heads] = weights @ rows[1]
         for name, pair in zip(("k", "v"), scales):
             x = s[name][i, 0].double()
-            pair[i, p % w, :, 0] = (x.amax(-1) - x.amin(-1)) / 15
-            pair[i, p % w, :, 1] = x.amin(-1)
+            pair[i, :, p % w, 0] = (x.amax(-1) - x.amin(-1)) / 15
+            pair[i, :, p % w, 1] = x.amin(-1)
     return [out, None, None, *scales, None, None]
 
 
