@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define VSP_ABI_VERSION 22
+#define VSP_ABI_VERSION 23
 
 /* Status codes. */
 #define VSP_OK 0
@@ -483,6 +483,53 @@ int vsp_residual_rows_where(const float* x1, const void* a, float* x, const uint
 int vsp_pass_end(int count, const void* const* src, void* const* dst, const size_t* row_bytes, const float* x1,
                  const void* a, float* x, const uint8_t* active, const uint8_t* exits, int* n_iters, uint8_t* next,
                  void* norm_out, int rows, int d, void* stream);
+
+/* ---- the KV ring in four bits -------------------------------------------------------------------
+ * The decoding ring of vsp_ring_attn_* with each row of D features (one token, one KV head) as D codes
+ * of four bits and a pair: lo the row's smallest feature, s = (largest - lo) / 15 rounded to the
+ * tokens' type, code = round((x - lo) / s) in 0..15, value = lo + s code (codes 0 where s is 0; a row
+ * with an infinity or a NaN is stored as s = lo = NaN).
+ *   ring_k, ring_v   uint8 [B, HKV, window, D / 2], feature 2 i in the low half of byte i
+ *   k_scale, v_scale bf16 / fp16 [B, HKV, window, 2]: s, lo
+ *   ring_pos int64, ring_valid uint8 [B, window]
+ * D a multiple of 8 up to 256; window * D / 2 under 2 GiB. q, k, v and outputs 16-byte aligned, the ring's
+ * tensors 4-byte aligned. */
+
+/* Tokens k, v [B, N, HKV, D] at positions pos [B, N] (nonnegative, up by one along a row) into slots
+ * pos % window: of each row its last `window` tokens. lengths (int64 [B], 0..N, or NULL for N): only a
+ * row's first lengths[b] tokens are taken. */
+int vsp_quant_ring_write_bf16(const void* k, const void* v, const int64_t* pos, const int64_t* lengths, void* ring_k,
+                              void* ring_v, void* k_scale, void* v_scale, int64_t* ring_pos, uint8_t* ring_valid,
+                              int B, int N, int HKV, int D, int window, void* stream);
+int vsp_quant_ring_write_f16(const void* k, const void* v, const int64_t* pos, const int64_t* lengths, void* ring_k,
+                             void* ring_v, void* k_scale, void* v_scale, int64_t* ring_pos, uint8_t* ring_valid,
+                             int B, int N, int HKV, int D, int window, void* stream);
+
+/* The tokens at positions pos [B, N] (any order) as k, v [B, N, HKV, D]; found [B, N] = 1 where the ring
+ * holds the position, else 0 and the rows zero. Values past the type's range by the scale's rounding
+ * are brought back to its largest number. */
+int vsp_quant_ring_read_bf16(const void* ring_k, const void* ring_v, const void* k_scale, const void* v_scale,
+                             const int64_t* ring_pos, const uint8_t* ring_valid, const int64_t* pos, void* k, void* v,
+                             uint8_t* found, int B, int N, int HKV, int D, int window, void* stream);
+int vsp_quant_ring_read_f16(const void* ring_k, const void* ring_v, const void* k_scale, const void* v_scale,
+                            const int64_t* ring_pos, const uint8_t* ring_valid, const int64_t* pos, void* k, void* v,
+                            uint8_t* found, int B, int N, int HKV, int D, int window, void* stream);
+
+/* One new token per row: q [B, H, D] over the slots that are valid, hold a position in (p - window, p] and
+ * are not slot p % window, and over the new token k, v [B, HKV, D] itself (unquantised); o [B, H, D].
+ * H / HKV at most 8. `active` uint8 [B] or NULL: an inactive row's output is 0. With write != 0 the token
+ * is then quantised into slot p % window. Where several workgroups share a window the workspace holds
+ * their softmax states (vsp_quant_ring_attn_workspace_bytes; no initial contents needed, not shared by
+ * calls that may overlap in time). */
+size_t vsp_quant_ring_attn_workspace_bytes(int B, int H, int HKV, int D, int window);
+int vsp_quant_ring_attn_bf16(const void* q, const void* k, const void* v, const int64_t* pos, void* ring_k,
+                             void* ring_v, void* k_scale, void* v_scale, int64_t* ring_pos, uint8_t* ring_valid,
+                             void* o, const uint8_t* active, void* workspace, size_t workspace_bytes, int B, int H,
+                             int HKV, int D, int window, float scale, int write, void* stream);
+int vsp_quant_ring_attn_f16(const void* q, const void* k, const void* v, const int64_t* pos, void* ring_k,
+                            void* ring_v, void* k_scale, void* v_scale, int64_t* ring_pos, uint8_t* ring_valid,
+                            void* o, const uint8_t* active, void* workspace, size_t workspace_bytes, int B, int H,
+                            int HKV, int D, int window, float scale, int write, void* stream);
 
 #ifdef __cplusplus
 }
