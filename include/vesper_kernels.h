@@ -531,6 +531,37 @@ int vsp_quant_ring_attn_f16(const void* q, const void* k, const void* v, const i
                             void* o, const uint8_t* active, void* workspace, size_t workspace_bytes, int B, int H,
                             int HKV, int D, int window, float scale, int write, void* stream);
 
+/* ---- projections in 8-bit integers ---------------------------------------------------------------
+ * RMSNorm of the rows s = x + residual (float32; residual may be NULL) with gain (float32 [d] or NULL),
+ * y = s / sqrt(mean(s^2) + 1e-6) * gain, as int8 codes [rows, d] and a float32 scale a row: scale = max |y| / 127,
+ * code = round(y / scale) (both 0 where max |y| < 2^-120; scale NaN and codes 0 for a row with an infinity or
+ * a NaN). sum_out (x's type, may be NULL) receives s and must not overlap x or the residual. d a multiple of
+ * 8 in 8..16384; x, residual, sum_out and gain 16-byte aligned, out 8-byte. The name says x's type and, where
+ * it differs, the residual's. */
+int vsp_rms_norm_int8_f32_bf16(const void* x, const void* residual, void* sum_out, const float* gain, int8_t* out,
+                               float* scale, int rows, int d, void* stream);
+int vsp_rms_norm_int8_f32_f16(const void* x, const void* residual, void* sum_out, const float* gain, int8_t* out,
+                              float* scale, int rows, int d, void* stream);
+int vsp_rms_norm_int8_bf16(const void* x, const void* residual, void* sum_out, const float* gain, int8_t* out,
+                           float* scale, int rows, int d, void* stream);
+int vsp_rms_norm_int8_f16(const void* x, const void* residual, void* sum_out, const float* gain, int8_t* out,
+                          float* scale, int rows, int d, void* stream);
+
+/* Every block of a stacked projection in one launch: out_j[m, c] = (sum_k z[m, k] weights[j, c, k]) *
+ * (z_scale[m] weights_scale[j, c]) for c < used_j, sums in int32, with block `sigmoid_block` (-1: none)
+ * through the logistic function. z int8 [M, d], weights int8 [nblk, cols, d] (nblk 1..4, blocks past it
+ * ignored), z_scale float32 [M], weights_scale float32 [nblk, cols]; d a multiple of 16 in 16..16384; z,
+ * weights and the outputs ([M, used_j] of the type the name ends in) 16-byte aligned. */
+int vsp_project_int8_bf16(const int8_t* z, const float* z_scale, const int8_t* weights, const float* weights_scale,
+                          int nblk, int cols, int d, int M, int used0, int used1, int used2, int used3, void* out0,
+                          void* out1, void* out2, void* out3, int sigmoid_block, void* stream);
+int vsp_project_int8_f16(const int8_t* z, const float* z_scale, const int8_t* weights, const float* weights_scale,
+                         int nblk, int cols, int d, int M, int used0, int used1, int used2, int used3, void* out0,
+                         void* out1, void* out2, void* out3, int sigmoid_block, void* stream);
+int vsp_project_int8_f32(const int8_t* z, const float* z_scale, const int8_t* weights, const float* weights_scale,
+                         int nblk, int cols, int d, int M, int used0, int used1, int used2, int used3, void* out0,
+                         void* out1, void* out2, void* out3, int sigmoid_block, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

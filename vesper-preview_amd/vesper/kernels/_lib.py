@@ -96,6 +96,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "vsp_quant_ring_attn_workspace_bytes": (Z, [I, I, I, I, I]),
     "vsp_quant_ring_attn_bf16": (I, [P, P, P, P, P, P, P, P, P, P, P, P, P, Z, I, I, I, I, I, F, I, P]),
     "vsp_quant_ring_attn_f16": (I, [P, P, P, P, P, P, P, P, P, P, P, P, P, Z, I, I, I, I, I, F, I, P]),
+    "vsp_rms_norm_int8_f32_bf16": (I, [P, P, P, P, P, P, I, I, P]),
+    "vsp_rms_norm_int8_f32_f16": (I, [P, P, P, P, P, P, I, I, P]),
+    "vsp_rms_norm_int8_bf16": (I, [P, P, P, P, P, P, I, I, P]),
+    "vsp_rms_norm_int8_f16": (I, [P, P, P, P, P, P, I, I, P]),
+    "vsp_project_int8_bf16": (I, [P, P, P, P, I, I, I, I, I, I, I, I, P, P, P, P, I, P]),
+    "vsp_project_int8_f16": (I, [P, P, P, P, I, I, I, I, I, I, I, I, P, P, P, P, I, P]),
+    "vsp_project_int8_f32": (I, [P, P, P, P, I, I, I, I, I, I, I, I, P, P, P, P, I, P]),
     "vsp_key_filter_backward_workspace_bytes": (Z, [I, I, I, I]),
     "vsp_key_filter_backward_bf16": (I, [P, P, P, P, P, P, P, P, Z, I, I, I, I, I, P]),
     "vsp_key_filter_backward_f16": (I, [P, P, P, P, P, P, P, P, Z, I, I, I, I, I, P]),

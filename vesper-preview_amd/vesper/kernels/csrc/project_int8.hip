@@ -1,0 +1,335 @@
+// The looped column's projections in 8-bit integers on CDNA4 (gfx950): every block of a pass's stacked
+// weight in one launch, with a scale for each token and each output channel.
+//
+//   y_j[m, c] = (sum_k z[m, k] w_j[c, k]) (a_m b_jc),  int32 sums (exact: at most 16384 * 127^2 < 2^31),
+//
+// z [M, d] int8 with scales a (norm_int8.hip), the weights stacked and transposed as the bf16
+// projection's (project.hip; vesper/column.py:192-260, vesper/attention.py:269-292), [p, cols, d] int8 with
+// scales b [p, cols]. The product of the two scales is rounded to float32, the sum is converted to it, and
+// their product is rounded once more to the output's type; the write strength's block may pass through
+// the logistic function first.
+//
+// Two kernels, by the number of tokens:
+//
+// tile (many tokens): 256 tokens x 256 columns a workgroup, eight waves of 64 x 128, both operands through
+// LDS in double-buffered stages of 128 inputs (the 128-byte rows of the bf16 projection's stages, its
+// XOR swizzle and its block order), 16x16x64 int8 MFMA formed transposed (weight rows as the A operand).
+//
+// few (up to 64 tokens, a decode step): bound by reading the weights once. A workgroup takes 16 columns and
+// all the tokens; its waves share the inputs, each reading whole 128-byte lines of 16 weight rows straight
+// into the MFMA operand's registers; the waves' int32 sums are joined through LDS.
+#include <type_traits>
+
+#include "common.h"
+#include "vesper_kernels.h"
+
+namespace vsp {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMaxBlocks = 4;
+constexpr int kBM = 256;  // tokens a workgroup of the tile kernel
+constexpr int kBN = 256;  // its output columns
+constexpr int kBK = 128;  // inputs a stage
+constexpr int kFewCols = 16;   // output columns a workgroup of the few-token kernel
+constexpr int kFewTokens = 64; // its most tokens
+
+struct Blocks {
+  int nblk;
+  int used[kMaxBlocks];       // columns written per block
+  int start[kMaxBlocks + 1];  // first column tile of each block
+  void* out[kMaxBlocks];      // [M, used] per block
+};
+
+struct Args {
+  const int8_t* z;
+  const float* z_scale;
+  const int8_t* wt;
+  const float* w_scale;
+  int M, d, cols, sig_block;
+};
+
+template <typename T>
+__device__ __forceinline__ T finish(int sum, float scale, bool sig) {
+  float y = (float)sum * scale;
+  if (sig) y = 1.f / (1.f + expf(-y));
+  return from_f32<T>(y);
+}
+
+__device__ __forceinline__ int block_of(const Blocks& blk, int tile) {
+  int nb = 0;
+#pragma unroll
+  for (int j = 1; j < kMaxBlocks; ++j)
+    if (j < blk.nblk && tile >= blk.start[j]) nb = j;
+  return nb;
+}
+
+// 16 bytes from a buffer (zeros past its range).
+__device__ __forceinline__ i32x4 load16(__amdgpu_buffer_rsrc_t r, unsigned off) {
+  return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+}
+
+constexpr unsigned kOutside = 0x80000000u;  // an offset past every resource's range (under 2 GiB)
+
+template <typename T>
+__global__ __launch_bounds__(512, 1) void project_int8_kernel(const Args a, const Blocks blk, int ctiles, int mtiles) {
+  __shared__ __align__(16) int8_t sZ0[kBM * kBK], sZ1[kBM * kBK];
+  __shared__ __align__(16) int8_t sW0[kBN * kBK], sW1[kBN * kBK];
+
+  const int lg = xcd_logical_block(blockIdx.x, gridDim.x);
+  const int mt = lg / ctiles, ct = lg - mt * ctiles;
+  if (mt >= mtiles) return;  // the grid is padded to whole XCD rounds; whole workgroups leave
+  const int nb = block_of(blk, ct);
+  const int c0 = (ct - blk.start[nb]) * kBN;
+  const int used = blk.used[nb], d = a.d;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, lq = l & 15, g = l >> 4;
+  const int wm = w & 3, wn = w >> 2;  // the wave's tokens 64 wm .. + 63 and columns 128 wn .. + 127
+  const bool live = c0 + 128 * wn < used;
+  const int stages = (d + kBK - 1) / kBK;
+
+  // resources of the tile's own rows (under 256 x 16384 bytes): rows past the operands' ends read zeros
+  const int zrows = min(kBM, a.M - mt * kBM), wrows = min(kBN, a.cols - c0);
+  const __amdgpu_buffer_rsrc_t rz = buffer_rsrc(a.z + (size_t)mt * kBM * d, (unsigned)zrows * (unsigned)d);
+  const __amdgpu_buffer_rsrc_t rw = buffer_rsrc(a.wt + ((size_t)nb * a.cols + c0) * d, (unsigned)wrows * (unsigned)d);
+  auto kswz = [](int row) { return 2 * ((row >> 1) & 3); };
+  // direct loads: instruction j of wave w fills rows 8 (w + 8 j) .. + 7 of a stage, 128 bytes each; lane l brings
+  // row l / 8's logical segment (l % 8) ^ kswz(row)
+  const int lrow = l >> 3, lseg = (l & 7) ^ kswz(lrow);
+  unsigned off[4];  // the scalar offset holds the stage only: it stays below every resource's size
+#pragma unroll
+  for (int j = 0; j < 4; ++j) off[j] = (unsigned)(8 * w + 64 * j + lrow) * (unsigned)d + 16u * (unsigned)lseg;
+  auto issue = [&](int st, int8_t* dz, int8_t* dw) {
+    // inputs past d (d is a multiple of 16, so whole segments) are zeros in z; the weights' are what follows
+    const bool in = st * kBK + 16 * lseg < d;
+    const unsigned so = (unsigned)(st * kBK);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      buffer_load_lds16(rz, dz + (w + 8 * j) * 1024, in ? off[j] : kOutside, so);
+      buffer_load_lds16(rw, dw + (w + 8 * j) * 1024, off[j], so);
+    }
+  };
+
+  i32x4 acc[8][4];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
+  auto compute = [&](const int8_t* sz, const int8_t* sw) {
+    if (!live) return;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      i32x4 zf[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 64 * wm + 16 * i + lq;
+        zf[i] = *reinterpret_cast<const i32x4*>(sz + row * kBK + 16 * ((4 * s + g) ^ kswz(row)));
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = 128 * wn + 16 * j + lq;
+        const i32x4 f = *reinterpret_cast<const i32x4*>(sw + row * kBK + 16 * ((4 * s + g) ^ kswz(row)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, zf[i], acc[j][i], 0, 0, 0);
+      }
+    }
+  };
+
+  issue(0, sZ0, sW0);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+  for (int st = 0; st < stages; st += 2) {
+    if (st + 1 < stages) issue(st + 1, sZ1, sW1);
+    compute(sZ0, sW0);
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+    if (st + 1 < stages) {
+      if (st + 2 < stages) issue(st + 2, sZ0, sW0);
+      compute(sZ1, sW1);
+      __builtin_amdgcn_s_waitcnt(0x0F70);
+      __syncthreads();
+    }
+  }
+  if (!live) return;
+
+  // lane (lq, g) holds columns 16 j + 4 g + r of token 16 i + lq
+  const int m0 = mt * kBM + 64 * wm, cw = c0 + 128 * wn;
+  const float* ws = a.w_scale + (size_t)nb * a.cols;
+  float zs[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) zs[i] = a.z_scale[min(m0 + 16 * i + lq, a.M - 1)];
+  T* out = static_cast<T*>(blk.out[nb]);
+  if constexpr (sizeof(T) == 2) {
+    // through LDS (free once the last stage's barrier has passed), so that whole rows leave: the wave's
+    // 64 x 128 tile, row r's 16-byte segment s at s ^ (r & 15), then 16 lanes a row, four rows an instruction
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    typedef T V8 __attribute__((ext_vector_type(8)));
+    int8_t* base = (w >> 1) == 0 ? sZ0 : (w >> 1) == 1 ? sZ1 : (w >> 1) == 2 ? sW0 : sW1;
+    T* stile = reinterpret_cast<T*>(base) + (w & 1) * 64 * 128;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = 16 * j + 4 * g;
+      float bs[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bs[r] = ws[min(cw + c + r, used - 1)];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * i + lq;
+        V4 y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[r], nb == a.sig_block);
+        *reinterpret_cast<V4*>(stile + row * 128 + 8 * ((c >> 3) ^ (row & 15)) + (c & 7)) = y;
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the tile is in LDS (only this wave reads it)
+    const int seg = l & 15, col = cw + 8 * seg;
+    const bool whole = (used & 7) == 0;
+#pragma unroll
+    for (int it = 0; it < 16; ++it) {
+      const int row = 4 * it + (l >> 4), m = m0 + row;
+      if (m >= a.M || col >= used) continue;
+      const V8 v = *reinterpret_cast<const V8*>(stile + row * 128 + 8 * (seg ^ (row & 15)));
+      T* orow = out + (size_t)m * used + col;
+      if (whole) {
+        *reinterpret_cast<V8*>(orow) = v;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (col + r < used) orow[r] = v[r];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int col = cw + 16 * j + 4 * g;
+      float bs[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bs[r] = ws[min(col + r, used - 1)];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = m0 + 16 * i + lq;
+        if (m >= a.M) continue;
+        float y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[r], nb == a.sig_block);
+        T* orow = out + (size_t)m * used + col;
+        if ((used & 3) == 0 && col < used) {
+          *reinterpret_cast<float4*>(orow) = make_float4(y[0], y[1], y[2], y[3]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (col + r < used) orow[r] = y[r];
+        }
+      }
+    }
+  }
+}
+
+// MT tiles of 16 tokens, NW waves sharing the inputs.
+template <typename T, int MT, int NW>
+__global__ __launch_bounds__(64 * NW) void project_int8_few_kernel(const Args a, const Blocks blk) {
+  __shared__ int part[NW][MT][16][17];  // [token][column], a column more against bank conflicts
+  const int nb = block_of(blk, blockIdx.x);
+  const int c0 = ((int)blockIdx.x - blk.start[nb]) * kFewCols;
+  const int used = blk.used[nb], d = a.d;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, lq = l & 15, g = l >> 4;
+  const __amdgpu_buffer_rsrc_t rz = buffer_rsrc(a.z, (unsigned)a.M * (unsigned)d);
+  const __amdgpu_buffer_rsrc_t rw =
+      buffer_rsrc(a.wt + ((size_t)nb * a.cols + c0) * d, (unsigned)min(kFewCols, a.cols - c0) * (unsigned)d);
+  i32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = i32x4{0, 0, 0, 0};
+  // a step: 128 inputs of 16 weight rows, lane (lq, g) the 32 bytes at 32 g of row lq
+  const unsigned row = (unsigned)lq * (unsigned)d + 32u * (unsigned)g;
+  for (int k = 128 * w; k < d; k += 128 * NW) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned o = (unsigned)k + 16u * h;
+      const i32x4 f = load16(rw, row + o);
+      const bool in = k + 32 * g + 16 * h < d;  // d is a multiple of 16
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const i32x4 zf = load16(rz, in ? (unsigned)(16 * i) * (unsigned)d + row + o : kOutside);
+        acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, zf, acc[i], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) part[w][i][lq][4 * g + r] = acc[i][r];
+  __syncthreads();
+  const float* ws = a.w_scale + (size_t)nb * a.cols;
+  T* out = static_cast<T*>(blk.out[nb]);
+  for (int i = threadIdx.x; i < 256 * MT; i += 64 * NW) {
+    const int c = i & 15, m = i >> 4;
+    if (m >= a.M || c0 + c >= used) continue;
+    int sum = 0;
+#pragma unroll
+    for (int u = 0; u < NW; ++u) sum += part[u][m >> 4][m & 15][c];
+    out[(size_t)m * used + c0 + c] = finish<T>(sum, a.z_scale[m] * ws[c0 + c], nb == a.sig_block);
+  }
+}
+
+template <typename T>
+int project_int8(const int8_t* z, const float* z_scale, const int8_t* wt, const float* w_scale, int nblk, int cols,
+                 int d, int M, const int (&used_in)[kMaxBlocks], void* const (&out_in)[kMaxBlocks], int sigmoid_block,
+                 void* stream, const char* who) {
+  if (nblk < 1 || nblk > kMaxBlocks) return fail(ERR_ARG, "%s: %d weight blocks (1..%d)", who, nblk, kMaxBlocks);
+  if (d < 16 || d > 16384 || d % 16 != 0)
+    return fail(ERR_ARG, "%s: width %d (a multiple of 16 in 16..16384)", who, d);
+  if (M < 0 || cols < 1) return fail(ERR_ARG, "%s: bad sizes M=%d cols=%d", who, M, cols);
+  if (sigmoid_block < -1 || sigmoid_block >= nblk) return fail(ERR_ARG, "%s: sigmoid block %d", who, sigmoid_block);
+  const bool few = M <= kFewTokens;
+  const int width = few ? kFewCols : kBN;
+  Blocks blk{};
+  blk.nblk = nblk;
+  int64_t tiles = 0;
+  for (int j = 0; j < kMaxBlocks; ++j) {
+    blk.start[j] = (int)tiles;
+    if (j >= nblk) continue;
+    if (used_in[j] < 1 || used_in[j] > cols)
+      return fail(ERR_ARG, "%s: block %d uses %d of its %d columns", who, j, used_in[j], cols);
+    if (M > 0 && out_in[j] == nullptr) return fail(ERR_ARG, "%s: null output for block %d", who, j);
+    if (reinterpret_cast<uintptr_t>(out_in[j]) & 15) return fail(ERR_ARG, "%s: output %d must be 16-byte aligned", who, j);
+    blk.used[j] = used_in[j];
+    blk.out[j] = out_in[j];
+    tiles += ((int64_t)used_in[j] + width - 1) / width;
+  }
+  blk.start[kMaxBlocks] = (int)tiles;
+  if (M == 0) return OK;
+  if (!z || !z_scale || !wt || !w_scale) return fail(ERR_ARG, "%s: null pointer", who);
+  if ((reinterpret_cast<uintptr_t>(z) | reinterpret_cast<uintptr_t>(wt)) & 15)
+    return fail(ERR_ARG, "%s: z and the weights must be 16-byte aligned", who);
+  const int mtiles = (int)(((int64_t)M + kBM - 1) / kBM);
+  const int64_t n = few ? tiles : (tiles * mtiles + 7) / 8 * 8;  // whole rounds over the 8 XCDs
+  if (n >= ((int64_t)1 << 31)) return fail(ERR_ARG, "%s: too many tiles", who);
+  const Args a{z, z_scale, wt, w_scale, M, d, cols, sigmoid_block};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (!few) {
+    hipLaunchKernelGGL(project_int8_kernel<T>, dim3((unsigned)n), dim3(512), 0, s, a, blk, (int)tiles, mtiles);
+    return check_launch(who);
+  }
+  auto go = [&](auto kern, int nw) { hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(64 * nw), 0, s, a, blk); };
+  if (M <= 16) go(project_int8_few_kernel<T, 1, 4>, 4);
+  else if (M <= 32) go(project_int8_few_kernel<T, 2, 4>, 4);
+  else go(project_int8_few_kernel<T, 4, 4>, 4);
+  return check_launch(who);
+}
+
+}  // namespace
+}  // namespace vsp
+
+#define VSP_PROJECT_INT8(SUFFIX, T)                                                                                    \
+  extern "C" int vsp_project_int8_##SUFFIX(const int8_t* z, const float* z_scale, const int8_t* weights,               \
+                                           const float* weights_scale, int nblk, int cols, int d, int M, int used0,    \
+                                           int used1, int used2, int used3, void* out0, void* out1, void* out2,        \
+                                           void* out3, int sigmoid_block, void* stream) {                              \
+    const int used[4] = {used0, used1, used2, used3};                                                                  \
+    void* const out[4] = {out0, out1, out2, out3};                                                                     \
+    return vsp::project_int8<T>(z, z_scale, weights, weights_scale, nblk, cols, d, M, used, out, sigmoid_block, stream, \
+                                "vsp_project_int8_" #SUFFIX);                                                          \
+  }
+VSP_PROJECT_INT8(bf16, __bf16)
+VSP_PROJECT_INT8(f16, _Float16)
+VSP_PROJECT_INT8(f32, float)

@@ -3,6 +3,8 @@
 ``rms_norm_bf16(x, gain)`` is ``RMSNorm.forward`` (``vesper/column.py:146-188``) on the float32
 residual stream, ``x / sqrt(mean(x^2) + 1e-6) * gain`` computed scale-safely as the reference does,
 returned in bfloat16 for the bf16 projection GEMMs (``vsp_rms_norm_bf16``, one launch).
+``rms_norm_int8`` returns it in 8-bit integers with a scale a row (``vsp_rms_norm_int8_*``), the operand
+of ``projection_int8`` (``vsp_project_int8_*``), whose weights ``quantize_weights`` lays out once.
 """
 
 from __future__ import annotations
@@ -206,4 +208,152 @@ def projection(z: Tensor, weights_t: Tensor, used: tuple[int, ...], *,
     with _lib.on_device(z.device):
         _lib.call("vsp_project_bf16", zc.data_ptr(), wc.data_ptr(), p, cols, d, m, *widths, *ptrs,
                   -1 if sigmoid_block is None else sigmoid_block, _lib.stream_of(z.device))
+    return outs
+
+
+_INT8_SUFFIX = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
+# x and residual dtypes of rms_norm_int8
+_NORM_INT8 = {(torch.float32, torch.bfloat16): "f32_bf16", (torch.float32, torch.float16): "f32_f16",
+              (torch.bfloat16, torch.bfloat16): "bf16", (torch.float16, torch.float16): "f16"}
+
+
+def _aligned(t: Tensor, nbytes: int = 16) -> Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % nbytes == 0 else t.clone()
+
+
+def _refuse_grad(name: str, *tensors: Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ContractError(f"{name} is forward only: call it under torch.no_grad()")
+
+
+def rms_norm_int8(x: Tensor, gain: Tensor | None = None, *, residual: Tensor | None = None,
+                  sum_out: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """``RMSNorm`` over the last axis of ``x [..., d]`` (plus ``residual``) in 8-bit integers, one scale a row:
+    ``(codes int8 [..., d], scale float32 [...])`` with the norm ``y`` held as ``codes * scale``, ``scale = max
+    |y| / 127`` and ``codes = round(y / scale)``, in one launch (``vsp_rms_norm_int8_*``).
+
+    Args:
+        x: float32, bfloat16 or float16, its last axis ``d`` a multiple of 8 in 8..16384.
+        gain: optional float32 ``[d]`` (the norm's weight; ones when omitted).
+        residual: optional tensor shaped like ``x``, bfloat16 or float16 with a float32 ``x`` and else of x's
+            dtype: the norm is of the float32 sum ``x + residual``.
+        sum_out: with ``residual``, an optional contiguous tensor of x's shape and dtype (not ``x`` itself)
+            that receives the sum, rounded to that dtype.
+
+    A row whose normalized values are all below ``2 ** -120`` has scale 0 and codes 0; a row with an infinity
+    or a NaN has scale NaN and codes 0.
+
+    Raises:
+        ContractError: on a dtype, width or device outside that contract, or a tensor that needs a gradient.
+    """
+    if x.device.type != "cuda":
+        raise ContractError(f"the norm kernel runs on CUDA only, x is on {x.device}")
+    if x.dim() < 1:
+        raise ContractError("x: needs at least one axis")
+    rdtype = (torch.bfloat16 if x.dtype == torch.float32 else x.dtype) if residual is None else residual.dtype
+    if (x.dtype, rdtype) not in _NORM_INT8:
+        raise ContractError(f"x: dtype must be float32 (residual bfloat16 or float16), bfloat16 or float16 (residual the same), "
+                            f"got {x.dtype} and {rdtype}")
+    d = x.shape[-1]
+    if d < 8 or d > 16384 or d % 8:
+        raise ContractError(f"x: last axis {d} is not a multiple of 8 in 8..16384")
+    _refuse_grad("rms_norm_int8", x, gain, residual)
+    if gain is not None:
+        if gain.shape != (d,) or gain.dtype != torch.float32 or gain.device != x.device:
+            raise ContractError(f"gain: must be float32 [{d}] on {x.device}, got {tuple(gain.shape)} {gain.dtype}")
+        gain = _aligned(gain)
+    if residual is not None:
+        if residual.shape != x.shape or residual.device != x.device:
+            raise ContractError(f"residual: {tuple(x.shape)} on {x.device}, got {tuple(residual.shape)} on {residual.device}")
+        residual = _aligned(residual)
+    xc = _aligned(x)
+    if sum_out is not None:
+        if residual is None:
+            raise ContractError("sum_out needs a residual")
+        if (sum_out.shape != x.shape or sum_out.dtype != x.dtype or sum_out.device != x.device
+                or not sum_out.is_contiguous() or sum_out.data_ptr() % 16):
+            raise ContractError(f"sum_out: contiguous, aligned {x.dtype} {tuple(x.shape)} on {x.device}")
+        if x.numel() and sum_out.data_ptr() in (xc.data_ptr(), residual.data_ptr()):
+            raise ContractError("sum_out must not be x or the residual")
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    with _lib.on_device(x.device):
+        _lib.call(f"vsp_rms_norm_int8_{_NORM_INT8[x.dtype, rdtype]}", xc.data_ptr(), _lib.ptr(residual),
+                  _lib.ptr(sum_out), _lib.ptr(gain), codes.data_ptr(), scale.data_ptr(), xc.numel() // d, d,
+                  _lib.stream_of(x.device))
+    return codes, scale
+
+
+def quantize_weights(weights_t: Tensor) -> tuple[Tensor, Tensor]:
+    """A stacked projection weight ``[p, cols, d]`` (each block transposed, one output channel a row) as the
+    operands of ``projection_int8``, made once: int8 ``[p, cols, d]`` and float32 scales ``[p, cols]``, each row
+    ``codes * scale`` with ``scale = max |w| / 127`` and ``codes = round(w / scale)`` (zeros for a row of zeros).
+
+    Raises:
+        ContractError: if ``weights_t`` is not a floating ``[p, cols, d]`` tensor of finite values.
+    """
+    if weights_t.dim() != 3 or not weights_t.is_floating_point():
+        raise ContractError(f"weights_t: floating [p, cols, d], got {tuple(weights_t.shape)} {weights_t.dtype}")
+    with torch.no_grad():
+        w = weights_t.float()
+        if not bool(torch.isfinite(w).all()):
+            raise ContractError("weights_t: every value must be finite")
+        scale = w.abs().amax(-1) / 127 if w.shape[-1] else w.new_zeros(w.shape[:-1])
+        codes = torch.where(scale[..., None] > 0, torch.round(w / scale[..., None]).clamp(-127, 127), torch.zeros_like(w))
+        return codes.to(torch.int8).contiguous(), scale.contiguous()
+
+
+def projection_int8(z: Tensor, z_scale: Tensor, weights_q: Tensor, weights_scale: Tensor, used: tuple[int, ...], *,
+                    sigmoid_block: int | None = None, dtype: torch.dtype = torch.bfloat16) -> list[Tensor]:
+    """A sublayer's projections in 8-bit integers (``vsp_project_int8_*``, one launch): for each block ``j`` of
+    the stacked weight the sums of ``z[m, k] * weights_q[j, c, k]`` in int32 (exact) times ``z_scale[m] *
+    weights_scale[j, c]``, over the columns it uses. The counterpart of ``projection`` and, with few tokens, of
+    ``decode_projection``.
+
+    Args:
+        z: int8 ``[M, d]`` (``rms_norm_int8``'s codes, one row a token), ``d`` a multiple of 16 in 16..16384.
+        z_scale: float32 ``[M]``.
+        weights_q: int8 ``[p, cols, d]``: ``quantize_weights`` of the stacked ``[p, d, cols]`` weight, each block
+            transposed.
+        weights_scale: float32 ``[p, cols]``.
+        used: the columns kept of each of the ``p`` (1..4) blocks.
+        sigmoid_block: the block whose outputs pass through the logistic function (the write strength).
+        dtype: the outputs' dtype: bfloat16, float16 or float32.
+
+    Returns:
+        one ``[M, used_j]`` tensor per block.
+
+    Raises:
+        ContractError: on shapes, dtypes or devices outside that contract, or a tensor that needs a gradient.
+    """
+    if z.dim() != 2 or z.dtype != torch.int8 or z.device.type != "cuda":
+        raise ContractError(f"z: int8 [M, d] on CUDA, got {tuple(z.shape)} {z.dtype} on {z.device}")
+    m, d = z.shape
+    if weights_q.dim() != 3 or weights_q.dtype != torch.int8 or weights_q.shape[2] != d:
+        raise ContractError(f"weights_q: int8 [p, cols, {d}], got {tuple(weights_q.shape)} {weights_q.dtype}")
+    p, cols = weights_q.shape[0], weights_q.shape[1]
+    for name, t, shape in (("z_scale", z_scale, (m,)), ("weights_scale", weights_scale, (p, cols))):
+        if t.shape != shape or t.dtype != torch.float32:
+            raise ContractError(f"{name}: float32 {shape}, got {tuple(t.shape)} {t.dtype}")
+    for name, t in (("z_scale", z_scale), ("weights_q", weights_q), ("weights_scale", weights_scale)):
+        if t.device != z.device:
+            raise ContractError(f"{name} is on {t.device}, z on {z.device}")
+    if len(used) != p or not 1 <= p <= 4 or any(not 1 <= u <= cols for u in used):
+        raise ContractError(f"used: {p} widths in 1..{cols}, got {tuple(used)}")
+    if d % 16 or not 16 <= d <= 16384:
+        raise ContractError(f"z: width {d} is not a multiple of 16 in 16..16384")
+    if sigmoid_block is not None and not 0 <= sigmoid_block < p:
+        raise ContractError(f"sigmoid_block {sigmoid_block} is not one of the {p} blocks")
+    if dtype not in _INT8_SUFFIX:
+        raise ContractError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
+    _refuse_grad("projection_int8", z_scale, weights_scale)
+    zc, wc, zs, ws = _aligned(z), _aligned(weights_q), z_scale.contiguous(), weights_scale.contiguous()
+    outs = [torch.empty(m, u, dtype=dtype, device=z.device) for u in used]
+    ptrs = [o.data_ptr() for o in outs] + [0] * (4 - p)
+    widths = list(used) + [1] * (4 - p)
+    with _lib.on_device(z.device):
+        _lib.call(f"vsp_project_int8_{_INT8_SUFFIX[dtype]}", zc.data_ptr(), zs.data_ptr(), wc.data_ptr(), ws.data_ptr(),
+                  p, cols, d, m, *widths, *ptrs, -1 if sigmoid_block is None else sigmoid_block,
+                  _lib.stream_of(z.device))
     return outs
