@@ -1,0 +1,180 @@
+"""What the few-bit operators refuse, on the CPU: shapes, dtypes, widths, devices and gradients, at the Python
+boundary and at the C ABI, before any launch; and the float64 quantiser of the tests."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+BF16 = torch.bfloat16
+
+
+def _ring(b=2, hkv=2, dk=16, w=8, dtype=BF16):
+    from vesper.kernels.ring_quant import quant_ring_empty
+
+    return quant_ring_empty(b, hkv, dk, w, dtype, torch.device("cpu"))
+
+
+def _token(b=2, h=2, dk=16, n=1, dtype=BF16):
+    return torch.zeros(b, n, h, dk, dtype=dtype)
+
+
+def test_an_empty_ring():
+    ring = _ring(3, 2, 24, 7)
+    assert ring.k.shape == (3, 2, 7, 12) and ring.k_scale.shape == (3, 2, 7, 2) and ring.pos.shape == (3, 7)
+    assert not any(bool(t.any()) for t in ring.tensors())
+
+
+@pytest.mark.parametrize(("kwargs", "error", "match"), [
+    ({"w": 0}, ValueError, "window"),
+    ({"dk": 12}, ValueError, "head dimension 12"),
+    ({"dk": 264}, ValueError, "head dimension 264"),
+    ({"dk": 0}, ValueError, "head dimension 0"),
+    ({"dtype": torch.float32}, ValueError, "dtype"),
+])
+def test_rings_outside_the_contract(kwargs, error, match):
+    with pytest.raises(error, match=match):
+        _ring(**kwargs)
+
+
+def test_the_write_refuses():
+    from vesper.contracts import ContractError
+    from vesper.kernels.ring_quant import quant_ring_write
+
+    k, pos, ring = _token(n=3), torch.arange(3).expand(2, 3), _ring()
+    for bad, match in (((k[:, :2], k, pos, ring), "axis 1"), ((k, k.half(), pos, ring), "dtype"),
+                       ((k, k, pos.int(), ring), "dtype"), ((k, k, pos, _ring(hkv=1)), "hkv"),
+                       ((k, k, pos, _ring(dk=24)), "features"), ((k, k, pos, _ring(dtype=torch.float16)), "dtype"),
+                       ((k, k, pos, _ring(b=3)), "'b'"), ((k, k, pos, ring), "CUDA only")):
+        with pytest.raises(ContractError, match=match):
+            quant_ring_write(*bad)
+
+
+def test_the_read_refuses():
+    from vesper.contracts import ContractError
+    from vesper.kernels.ring_quant import QuantRingKVCache, quant_ring_read
+
+    ring = _ring()
+    with pytest.raises(ContractError, match="dtype"):
+        quant_ring_read(ring, torch.zeros(2, 3, dtype=torch.int32))
+    with pytest.raises(ContractError, match="'b'"):
+        quant_ring_read(ring, torch.zeros(3, 3, dtype=torch.long))
+    with pytest.raises(ContractError, match="CUDA only"):
+        quant_ring_read(ring, torch.zeros(2, 3, dtype=torch.long))
+    with pytest.raises(ContractError, match="'w'"):
+        quant_ring_read(QuantRingKVCache(*ring.tensors(), 9), torch.zeros(2, 3, dtype=torch.long))
+    with pytest.raises(ContractError, match="dtype"):
+        quant_ring_read(QuantRingKVCache(ring.k.char(), *ring.tensors()[1:], 8), torch.zeros(2, 3, dtype=torch.long))
+
+
+def test_the_attention_refuses():
+    from vesper.contracts import ContractError
+    from vesper.kernels.ring_quant import quant_ring_attention
+
+    q, k, pos, ring = _token(h=4), _token(), torch.zeros(2, 1, dtype=torch.long), _ring()
+    for bad, match in (((_token(n=2), k, k, pos, ring), "axis 1"), ((q.half(), k, k, pos, ring), "dtype"),
+                       ((q, k, k, pos, _ring(dtype=torch.float16)), "dtype"), ((q, k, k, pos.int(), ring), "dtype"),
+                       ((q, k, k, pos, ring), "CUDA only")):
+        with pytest.raises(ContractError, match=match):
+            quant_ring_attention(*bad)
+
+
+def test_the_norm_and_the_projection_refuse():
+    from vesper.contracts import ContractError
+    from vesper.kernels.norm import projection_int8, quantize_weights, rms_norm_int8
+
+    with pytest.raises(ContractError, match="CUDA only"):
+        rms_norm_int8(torch.zeros(2, 64))
+    z, w = torch.zeros(2, 64, dtype=torch.int8), torch.zeros(1, 8, 64, dtype=torch.int8)
+    with pytest.raises(ContractError, match="CUDA"):
+        projection_int8(z, torch.ones(2), w, torch.ones(1, 8), (8,))
+    with pytest.raises(ContractError, match="floating"):
+        quantize_weights(torch.zeros(2, 8, dtype=torch.float32))
+    with pytest.raises(ContractError, match="floating"):
+        quantize_weights(w)
+    with pytest.raises(ContractError, match="finite"):
+        quantize_weights(torch.full((1, 2, 16), math.nan))
+
+
+def test_the_column_refuses_other_forms():
+    from vesper.contracts import ContractError
+    from vesper.decode import cold_states, per_pass
+    from vesper.loop import LoopedColumn
+
+    with pytest.raises(ValueError, match="projections"):
+        LoopedColumn.random(32, 2, 1, 16, 4, 1, 0, torch.device("cpu"), projections="int4")
+    with pytest.raises(ValueError, match="multiple of 16"):
+        LoopedColumn.random(24, 3, 3, 8, 4, 1, 0, torch.device("cpu"), projections="int8")
+    assert per_pass() == 6 and per_pass(4) == 8
+    column = LoopedColumn.random(32, 2, 1, 16, 4, 2, 0, torch.device("cpu"), projections="int8")
+    with pytest.raises(ContractError, match="ring_bits"):
+        cold_states(column, 1, torch.device("cpu"), 8)
+    flat = cold_states(column, 3, torch.device("cpu"), 4)
+    assert len(flat) == 16 and flat[2].shape == (3, 1, 4, 8) and flat[4].shape == (3, 1, 4, 2)
+    (codes, scale), _ = column.int8_weights(1)
+    assert codes.shape == (4, 32, 32) and scale.shape == (4, 32)
+
+
+def test_the_c_entries_refuse_before_any_launch():
+    from vesper.kernels import _lib
+
+    lib = _lib.library()
+    none8, err = [None] * 10, lambda: lib.vsp_last_error().decode()  # noqa: E731
+    one = 0x1000  # never read: the call is refused first
+    write, read, attn = lib.vsp_quant_ring_write_bf16, lib.vsp_quant_ring_read_bf16, lib.vsp_quant_ring_attn_bf16
+    assert write(*none8, 1, 1, 1, 12, 4, None) != 0 and "head dimension 12" in err()
+    assert write(*none8, 1, -1, 1, 16, 4, None) != 0 and "N=-1" in err()
+    assert write(*none8, 1, 1, 1, 16, 0, None) != 0 and "W=0" in err()
+    assert write(*none8, 1, 1, 1, 16, 4, None) != 0 and "null" in err()
+    assert write(*none8, 1, 1, 1, 256, 1 << 24, None) != 0 and "2 GiB" in err()
+    assert write(one + 8, *[one] * 9, 1, 1, 1, 16, 4, None) != 0 and "16-byte" in err()
+    assert write(one, one, one, None, one + 2, *[one] * 5, 1, 1, 1, 16, 4, None) != 0 and "4-byte" in err()
+    assert write(*none8, 0, 1, 1, 16, 4, None) == 0 and write(*none8, 1, 0, 1, 16, 4, None) == 0
+    assert read(*none8, 1, 1, 0, 16, 4, None) != 0 and "HKV=0" in err()
+    assert read(*none8, 1, 1, 1, 16, 4, None) != 0 and "null" in err()
+    assert read(*none8, 1, 0, 1, 16, 4, None) == 0
+    call = lambda ptrs, b, h, hkv, d, w, ws=0: attn(*ptrs, ws, b, h, hkv, d, w, 1.0, 1, None)  # noqa: E731
+    assert call([None] * 13, 1, 3, 2, 16, 4) != 0 and "multiple of 2" in err()
+    assert call([None] * 13, 1, 9, 1, 16, 4) != 0 and "at most 8" in err()
+    assert call([None] * 13, 1, 1, 1, 264, 4) != 0 and "264" in err()
+    assert call([None] * 13, 1, 1, 1, 16, 4) != 0 and "null" in err()
+    assert call([None] * 13, 0, 1, 1, 16, 4) == 0
+    need = lib.vsp_quant_ring_attn_workspace_bytes(1, 2, 1, 64, 4096)
+    assert need > 0
+    assert call([one] * 13, 1, 2, 1, 64, 4096, need - 1) != 0 and "workspace" in err()
+    assert lib.vsp_quant_ring_attn_workspace_bytes(0, 2, 1, 64, 4096) == 0
+    norm = lib.vsp_rms_norm_int8_f32_bf16
+    assert norm(None, None, None, None, None, None, 1, 12, None) != 0 and "width 12" in err()
+    assert norm(None, None, None, None, None, None, 1, 16392, None) != 0 and "16392" in err()
+    assert norm(None, None, None, None, None, None, 1, 16, None) != 0 and "null" in err()
+    assert norm(one, None, one, None, one, one, 1, 16, None) != 0 and "residual" in err()
+    assert norm(one + 4, None, None, None, one, one, 1, 16, None) != 0 and "16-byte" in err()
+    assert norm(None, None, None, None, None, None, 0, 16, None) == 0
+    project = lib.vsp_project_int8_bf16
+    args = lambda p=1, cols=8, d=64, m=4, used=(8, 1, 1, 1), outs=(None,) * 4, sig=-1: project(  # noqa: E731
+        None, None, None, None, p, cols, d, m, *used, *outs, sig, None)
+    assert args(p=5) != 0 and "weight blocks" in err()
+    assert args(d=24) != 0 and "width 24" in err()
+    assert args(d=16400) != 0 and "16400" in err()
+    assert args(m=-1) != 0 and "M=-1" in err()
+    assert args(sig=1) != 0 and "sigmoid" in err()
+    assert args(used=(9, 1, 1, 1)) != 0 and "9 of its 8" in err()
+    assert args() != 0 and "null output" in err()
+    assert args(outs=(one + 8, None, None, None)) != 0 and "16-byte" in err()
+    assert args(outs=(one, None, None, None)) != 0 and "null pointer" in err()
+    assert args(m=0) == 0
+
+
+def test_the_oracles_quantiser_on_a_row_done_by_hand():
+    """[-1, 0.5, 2, 14]: scale 15 / 15 = 1, codes 0, 2 (1.5 to even), 3, 15."""
+    from oracle.quant import quantize_rows, ring_values, row_values, unpack_rows
+
+    x = torch.tensor([[-1.0, 0.5, 2.0, 14.0]], dtype=BF16)
+    codes, scale, lo, t = quantize_rows(x)
+    assert codes.tolist() == [[0, 2, 3, 15]] and scale.item() == 1 and lo.item() == -1 and t.tolist() == [[0, 1.5, 3, 15]]
+    assert row_values(codes, scale, lo).tolist() == [[-1, 1, 2, 14]]
+    packed = torch.tensor([[0x20, 0xF3]], dtype=torch.uint8)
+    assert torch.equal(unpack_rows(packed), codes)
+    assert ring_values(packed, torch.tensor([[1.0, -1.0]])).tolist() == [[-1, 1, 2, 14]]

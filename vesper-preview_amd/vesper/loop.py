@@ -27,7 +27,9 @@ reference's ``where`` merges; ``copy_forward="where"`` runs those merges as torc
 
 All passes run even when no token is active any more. The FFN is not part of the mixer path and
 is left out. The residual stream stays in float32 (autocast's convention); matmuls and mixers run
-in bfloat16 with the scan state in float32. Forward only.
+in bfloat16 with the scan state in float32. With ``projections="int8"`` the sublayers' norms are
+written in 8-bit integers with a scale a token and projected with weights in 8-bit integers with a
+scale a channel (``vsp_rms_norm_int8_*``, ``vsp_project_int8_*``); all else is the same. Forward only.
 """
 
 from __future__ import annotations
@@ -44,10 +46,11 @@ from vesper.contracts import ContractError, Dims, check_shape
 from vesper.kernels.carry import end_pass, halt_step, residual_rows_where
 from vesper.kernels.delta_scan import delta_scan_fused
 from vesper.kernels.keys import fused_keys
-from vesper.kernels.norm import projection, rms_norm_bf16
+from vesper.kernels.norm import projection, projection_int8, quantize_weights, rms_norm_bf16, rms_norm_int8
 from vesper.kernels.window_attn import window_attention
 
 BF16 = torch.bfloat16
+Normed = Tensor | tuple[Tensor, Tensor]  # a norm in bf16, or its 8-bit codes and their scales
 
 
 _ONES: dict[tuple[int, torch.device], Tensor] = {}
@@ -103,11 +106,12 @@ class LoopedColumn:
     Weights are ``[d, out]`` bfloat16 tensors per pass (``x @ w``): ``wq, wk, wv [d, h*dk]``,
     ``wb [d, h]``, ``waq [d, h*dk]``, ``wak, wav [d, hkv*dk]``; optional ``taps`` are the key
     filter's ``[K, h*dk]`` float32 taps per pass (``wk`` then gives the filter's input).
+    ``projections`` is "bf16" or "int8" (``h * dk`` a multiple of 16): the type the norms are projected in.
     """
 
     def __init__(self, weights: dict[str, Sequence[Tensor]], heads: int, kv_heads: int, head_dim: int,
                  window: int, taps: Sequence[Tensor] | None = None, copy_forward: str = "fused",
-                 rotary_base: float | None = 10000.0) -> None:
+                 rotary_base: float | None = 10000.0, projections: str = "bf16") -> None:
         names = ("wq", "wk", "wv", "wb", "waq", "wak", "wav")
         missing = [n for n in names if n not in weights]
         if missing:
@@ -123,6 +127,11 @@ class LoopedColumn:
         if copy_forward not in ("fused", "where"):
             raise ValueError(f"copy_forward is 'fused' or 'where', got {copy_forward!r}")
         self.copy_forward = copy_forward
+        if projections not in ("bf16", "int8"):
+            raise ValueError(f"projections are 'bf16' or 'int8', got {projections!r}")
+        if projections == "int8" and heads * head_dim % 16:
+            raise ValueError(f"int8 projections need a width that is a multiple of 16, got {heads * head_dim}")
+        self.projections = projections
         self.rotary_base = rotary_base
         self._positions: dict[tuple[int, int, torch.device], Tensor] = {}
         # Each sublayer's projections stacked into one [p, d, h*dk] weight per pass (narrower ones
@@ -136,22 +145,37 @@ class LoopedColumn:
         self.w_rec = [torch.stack([padded(self.w[n][t]) for n in ("wq", "wk", "wv", "wb")]) for t in range(self.passes)]
         self.w_attn = [torch.stack([padded(self.w[n][t]) for n in ("waq", "wak", "wav")]) for t in range(self.passes)]
         self._decode_w: dict[int, tuple[Tensor, Tensor]] = {}
+        # the int8 weights are made here: quantising reads a flag back, which a graph capture cannot
+        self._int8_w = [(quantize_weights(rec.transpose(1, 2)), quantize_weights(attn.transpose(1, 2)))
+                        for rec, attn in zip(self.w_rec, self.w_attn)] if projections == "int8" else []
 
-    def project_rec(self, t: int, xb: Tensor) -> tuple[Tensor, Tensor, Tensor, Tensor]:
-        """Pass ``t``'s recurrent projections of ``xb [b, n, d]`` (bf16), one launch:
+    def norm(self, x: Tensor, residual: Tensor | None = None, sum_out: Tensor | None = None) -> Normed:
+        """The norm of ``x`` (plus ``residual``) as this column projects it: bf16, or 8-bit codes and scales."""
+        if self.projections == "int8":
+            return rms_norm_int8(x, residual=residual, sum_out=sum_out)
+        return rms_norm_bf16(x, residual=residual, sum_out=sum_out)
+
+    def project_rec(self, t: int, xb: Normed) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+        """Pass ``t``'s recurrent projections of ``xb [b, n, d]`` (``norm``'s), one launch:
         ``q_in [b, n, h*dk]`` (before normalization), ``z [b, n, h*dk]`` (the key input),
         ``v [b, n, h, dk]``, ``beta = sigmoid [b, n, h]``."""
-        b, n, d = xb.shape
+        b, n, _ = xb.shape if isinstance(xb, Tensor) else xb[0].shape
         h, dk = self.heads, self.head_dim
         hd = h * dk
-        q_in, z, v, beta = self._project(xb.reshape(b * n, d), t, 0, (hd, hd, hd, h), sigmoid_block=3)
+        q_in, z, v, beta = self._project(xb, t, 0, (hd, hd, hd, h), sigmoid_block=3)
         return q_in.view(b, n, hd), z.view(b, n, hd), v.view(b, n, h, dk), beta.view(b, n, h)
 
-    def _project(self, xb: Tensor, t: int, which: int, used: tuple[int, ...],
+    def _project(self, xb: Normed, t: int, which: int, used: tuple[int, ...],
                  sigmoid_block: int | None = None) -> list[Tensor]:
         """The blocks of pass ``t``'s stacked weight (``which``: 0 recurrent, 1 attention) applied
-        to ``xb [M, d]``, each as its own ``[M, used_j]`` tensor: one ``vsp_project_bf16`` launch
-        when ``d`` is a multiple of 64, else the batched library GEMM over the padded stack."""
+        to ``xb [..., d]``, each as its own ``[M, used_j]`` tensor: one ``vsp_project_int8_bf16`` launch for
+        8-bit codes; for bf16 one ``vsp_project_bf16`` launch when ``d`` is a multiple of 64, else the
+        batched library GEMM over the padded stack."""
+        if not isinstance(xb, Tensor):
+            codes, scale = xb
+            return projection_int8(codes.reshape(-1, codes.shape[-1]), scale.reshape(-1), *self.int8_weights(t)[which], used,
+                                   sigmoid_block=sigmoid_block)
+        xb = xb.reshape(-1, xb.shape[-1])
         if xb.shape[1] % 64 == 0:
             return projection(xb, self.decode_weights(t)[which], used, sigmoid_block=sigmoid_block)
         y = torch.matmul(xb, (self.w_rec if which == 0 else self.w_attn)[t])
@@ -168,20 +192,26 @@ class LoopedColumn:
                                  self.w_attn[t].transpose(1, 2).contiguous())
         return self._decode_w[t]
 
-    def project_attn(self, t: int, xb: Tensor, pos: Tensor | None = None) -> tuple[Tensor, Tensor, Tensor]:
-        """Pass ``t``'s attention projections of ``xb [b, n, d]`` (bf16), one launch, with the
+    def int8_weights(self, t: int) -> tuple[tuple[Tensor, Tensor], tuple[Tensor, Tensor]]:
+        """Pass ``t``'s stacked recurrent and attention weights in 8-bit integers with a scale an output
+        channel (``quantize_weights`` of ``decode_weights``' layout); made with the column."""
+        return self._int8_w[t]
+
+    def project_attn(self, t: int, xb: Normed, pos: Tensor | None = None) -> tuple[Tensor, Tensor, Tensor]:
+        """Pass ``t``'s attention projections of ``xb [b, n, d]`` (``norm``'s), one launch, with the
         queries and keys rotated at positions ``pos [b, n]`` (default ``0..n-1``) in one launch
         when the column has a rotary base (``WindowedAttention.project``, ``attention.py:269-292``)."""
-        b, n, d = xb.shape
+        first = xb if isinstance(xb, Tensor) else xb[0]
+        b, n, _ = first.shape
         h, hkv, dk = self.heads, self.kv_heads, self.head_dim
-        yq, yk, yv = self._project(xb.reshape(b * n, d), t, 1, (h * dk, hkv * dk, hkv * dk))
+        yq, yk, yv = self._project(xb, t, 1, (h * dk, hkv * dk, hkv * dk))
         aq, ak = yq.view(b, n, h, dk), yk.view(b, n, hkv, dk)
         if self.rotary_base is not None:
             if pos is None:
-                key = (b, n, xb.device)
+                key = (b, n, first.device)
                 pos = self._positions.get(key)
                 if pos is None:
-                    pos = torch.arange(n, device=xb.device).expand(b, n).contiguous()
+                    pos = torch.arange(n, device=first.device).expand(b, n).contiguous()
                     self._positions[key] = pos
             aq, ak = rotary_qk(aq, ak, pos, self.rotary_base)
         return aq, ak, yv.view(b, n, hkv, dk)
@@ -194,7 +224,7 @@ class LoopedColumn:
     @classmethod
     def random(cls, d: int, heads: int, kv_heads: int, head_dim: int, window: int, passes: int, seed: int,
                device: torch.device, key_conv: int = 0, copy_forward: str = "fused",
-               rotary_base: float | None = 10000.0) -> LoopedColumn:
+               rotary_base: float | None = 10000.0, projections: str = "bf16") -> LoopedColumn:
         """Fixed random weights ~ N(0, 1/d) from a CPU generator (the same values on any device);
         with ``key_conv`` a filter of that width, taps ~ U(-1/sqrt(K), 1/sqrt(K)) as the
         reference draws them (``column.py:231-233``)."""
@@ -210,7 +240,7 @@ class LoopedColumn:
             bound = 1.0 / key_conv**0.5
             taps = [(torch.rand(key_conv, heads * head_dim, generator=g) * (2 * bound) - bound).to(device)
                     for _ in range(passes)]
-        return cls(weights, heads, kv_heads, head_dim, window, taps, copy_forward, rotary_base)
+        return cls(weights, heads, kv_heads, head_dim, window, taps, copy_forward, rotary_base, projections)
 
     def keys(self, t: int, z: Tensor, history: Tensor | None, active: Tensor | None = None,
              carried_z: Tensor | None = None) -> tuple[Tensor, Tensor | None]:
@@ -222,7 +252,7 @@ class LoopedColumn:
         assert history is not None
         return recurrent_keys(z, history, self.taps[t], self.heads, active=active, carried_z=carried_z)
 
-    def _step(self, x: Tensor, xb: Tensor, t: int, state: Tensor, history: Tensor | None, active: Tensor | None,
+    def _step(self, x: Tensor, xb: Normed, t: int, state: Tensor, history: Tensor | None, active: Tensor | None,
               carried: Written | None) -> tuple[tuple[Tensor, Tensor], Tensor, Tensor | None, Written]:
         """One pass over ``x`` (``xb``: its norm); returns ``(x1, a)`` (the hidden state after the recurrent sublayer
         and the attention's output: the pass's output is ``x1 + a``), the new state and history, and
@@ -250,7 +280,7 @@ class LoopedColumn:
             r, new_state = delta_scan_fused(q, k, v, beta, state, active=active)
         # x1 = x + r (float32, promoted in the add) and its norm, in one launch
         x1 = torch.empty_like(x)
-        aq, ak, av = self.project_attn(t, rms_norm_bf16(x, residual=r.reshape(b, n, h * dk), sum_out=x1))
+        aq, ak, av = self.project_attn(t, self.norm(x, r.reshape(b, n, h * dk), x1))
         if where and carried is not None and active is not None:
             ak = _where_tokens(active, ak, carried.attn_k)
             av = _where_tokens(active, av, carried.attn_v)
@@ -296,14 +326,14 @@ class LoopedColumn:
             x = x0
             new_states = list(states)
             new_histories: list[Tensor | None] = list(histories) if histories is not None else [None] * self.passes
-            xb: Tensor | None = None  # the norm of x, where the previous pass's end has written it
+            xb: Tensor | None = None  # the bf16 norm of x, where the previous pass's end has written it
             for t in range(self.passes):
                 last = t == self.passes - 1
                 # pass 0 runs with every token active: the unmasked kernels, as the reference's
                 # carry-free first pass
                 mask = None if carried is None else active
                 (x1, a), new_states[t], new_histories[t], written = self._step(
-                    x, rms_norm_bf16(x) if xb is None else xb, t, new_states[t], new_histories[t], mask, carried)
+                    x, self.norm(x) if xb is None else xb, t, new_states[t], new_histories[t], mask, carried)
                 if self.copy_forward == "where":
                     # halts = active & exit (all active on the last pass), n_iters += active, and the
                     # next pass's active & ~halts: one launch
@@ -332,7 +362,7 @@ class LoopedColumn:
                         if written.z is not None and carried.z is not None:
                             freeze.append((written.z, carried.z))
                     next_active, xb = end_pass(x1, a, x, active, None if last else exits[t], n_iters, freeze,
-                                               norm=not last)
+                                               norm=not last and self.projections == "bf16")
                 active = next_active
         hist_out = tuple(t for t in new_histories if t is not None) if self.taps is not None else None
         return LoopResult(y=x, states=tuple(new_states), n_iters=n_iters, histories=hist_out)
