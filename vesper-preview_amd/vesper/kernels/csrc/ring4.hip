@@ -35,7 +35,7 @@ namespace {
 
 constexpr int kQuantMaxGroup = 8;
 constexpr int kTile = 32;       // tokens a wave takes at a time
-constexpr int kAttnWaves = 4;   // waves a workgroup
+constexpr int kMaxSplits = 256;  // workgroups that share a window (one thread each in the join)
 constexpr float kRaise = 8.f;   // log2: how far a tile's maximum may exceed the running one
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -120,15 +120,28 @@ __global__ __launch_bounds__(256) void quant_read_kernel(const uint32_t* __restr
 }
 
 // ---- attention ----------------------------------------------------------------------------------
+// The mask and the exponent bits that turn codes into elements, in registers that the compiler cannot see
+// through: the and and the or then are one instruction (as literals they would be two, each with its own).
+struct CodeBits {
+  uint32_t mask, one;
+  __device__ __forceinline__ explicit CodeBits(uint32_t exponent) : mask(0x000f000fu), one(exponent) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm("" : "+s"(mask));
+    asm("" : "+v"(one));
+#endif
+  }
+  __device__ __forceinline__ uint32_t two(uint32_t w, int nibble) const { return ((w >> (4 * nibble)) & mask) | one; }
+};
 // The codes of a dword as eight elements, in the order 0 4 1 5 2 6 3 7 of the features.
 template <typename T> struct Codes;
 template <> struct Codes<__bf16> {
-  static constexpr float kBias = 128.f;  // 0x4300 | c is 128 + c
+  static constexpr float kBias = 128.f;
+  static constexpr uint32_t kOne = 0x43004300u;  // 0x4300 | c is 128 + c
   typedef bf16x8 V8;
-  __device__ __forceinline__ static V8 unpack(uint32_t w) {
+  __device__ __forceinline__ static V8 unpack(uint32_t w, const CodeBits& bits) {
     u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    for (int i = 0; i < 4; ++i) r[i] = bits.two(w, i);
     return __builtin_bit_cast(V8, r);
   }
   __device__ __forceinline__ static f32x4 mma(V8 a, V8 b, f32x4 c) {
@@ -137,13 +150,14 @@ template <> struct Codes<__bf16> {
 };
 template <> struct Codes<_Float16> {
   static constexpr float kBias = 0.f;
+  static constexpr uint32_t kOne = 0x64006400u;  // 0x6400 | c is 1024 + c
   typedef f16x8 V8;
-  __device__ __forceinline__ static V8 unpack(uint32_t w) {
+  __device__ __forceinline__ static V8 unpack(uint32_t w, const CodeBits& bits) {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const f16x2 x = __builtin_bit_cast(f16x2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u);  // 1024 + c
+      const f16x2 x = __builtin_bit_cast(f16x2, bits.two(w, i));
       r[i] = __builtin_bit_cast(uint32_t, x - f16x2{(_Float16)1024.f, (_Float16)1024.f});
     }
     return __builtin_bit_cast(V8, r);
@@ -155,39 +169,52 @@ template <> struct Codes<_Float16> {
 // the k-th feature of a dword's eight in Codes<T>'s order
 __device__ __forceinline__ constexpr int code_feature(int k) { return (k >> 1) + 4 * (k & 1); }
 
-// Buffer loads of 1 to 16 bytes a lane; past the resource's range they give zeros.
-__device__ __forceinline__ uint32_t load_b8(__amdgpu_buffer_rsrc_t r, unsigned off) {
-  return (uint32_t)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)off, 0, 0);
+// Buffer loads of 1 to 16 bytes a lane at a lane's offset and a scalar one; past the resource's range they give zeros.
+__device__ __forceinline__ uint32_t load_b8(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned base) {
+  return (uint32_t)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)off, (int)base, 0);
 }
-__device__ __forceinline__ uint32_t load_b16(__amdgpu_buffer_rsrc_t r, unsigned off) {
-  return (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)off, 0, 0);
+__device__ __forceinline__ uint32_t load_b16(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned base) {
+  return (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)off, (int)base, 0);
+}
+__device__ __forceinline__ u32x2 load_b64(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned base) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, (int)base, 0));
 }
 // WHOLE: every piece of N dwords that starts in the range ends in it; else dword by dword.
 template <int N, bool WHOLE>
-__device__ __forceinline__ void load_dwords(__amdgpu_buffer_rsrc_t r, unsigned off, uint32_t (&out)[N]) {
+__device__ __forceinline__ void load_dwords(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned base, uint32_t (&out)[N]) {
   if constexpr (N == 1 || !WHOLE) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)(off + 4 * i), 0, 0);
+    for (int i = 0; i < N; ++i)
+      out[i] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)(off + 4 * i), (int)base, 0);
   } else if constexpr (N == 2) {
-    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
+    const u32x2 x = load_b64(r, off, base);
     out[0] = x[0];
     out[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(off + 4 * i), 0, 0));
+      const u32x4 x =
+          __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(off + 4 * i), (int)base, 0));
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[i + e] = x[e];
     }
   }
 }
 
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r = x;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));  // without fmaxf's quieting of its inputs
+#endif
+  return r;
+}
+
 // The largest of x over the lanes l, l ^ 16, l ^ 32, l ^ 48 (a column of an MFMA result).
 __device__ __forceinline__ float max_over_rows(float x) {
   const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __builtin_fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  x = max3(__uint_as_float(p[0]), __uint_as_float(p[1]), __uint_as_float(p[1]));
   const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __builtin_fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+  return max3(__uint_as_float(q[0]), __uint_as_float(q[1]), __uint_as_float(q[1]));
 }
 
 struct QuantAttnArgs {
@@ -200,42 +227,114 @@ struct QuantAttnArgs {
   uint8_t* ring_valid;
   const uint8_t* active;
   float* partial;  // [B, H, splits, 2 + dk] softmax states, with more than one split
-  int B, H, HKV, dk, W, splits, write;
+  int B, H, HKV, dk, W, splits, per, heads;  // per: tiles a split; heads: B HKV
   float scale_log2;
 };
 
+// The new tokens into their slots, which no workgroup attends (a reader of their codes drops them): L lanes
+// a row, keys then values, in workgroups behind the attention's.
+template <typename T, int L>
+__device__ __forceinline__ void write_tokens(const T* knew, const T* vnew, const QuantAttnArgs& a, int block, int threads) {
+  const int64_t r = ((int64_t)block * threads + threadIdx.x) / L;
+  const int part = threadIdx.x % L;
+  if (r >= 2 * (int64_t)a.heads) return;  // whole rows of lanes
+  const bool values = r >= a.heads;
+  const size_t head = (size_t)(values ? r - a.heads : r);
+  const int b = (int)(head / a.HKV), kvh = (int)(head - (size_t)b * a.HKV);
+  const int64_t p = a.pos[b];
+  if (p < 0) return;
+  const int slot = (int)(p % a.W);
+  const bool live = 8 * part < a.dk;
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  if (live) load8_f32((values ? vnew : knew) + head * a.dk + 8 * part, x);
+  uint32_t pair;
+  const uint32_t codes = quantize_row8<T, L>(x, live, pair);
+  const size_t row = head * a.W + slot;
+  if (live) (values ? a.ring_v : a.ring_k)[row * (size_t)(a.dk / 8) + part] = codes;
+  if (part == 0) {
+    (values ? a.v_scale : a.k_scale)[row] = pair;
+    if (!values && kvh == 0) {
+      a.ring_pos[(size_t)b * a.W + slot] = p;
+      a.ring_valid[(size_t)b * a.W + slot] = 1;
+    }
+  }
+}
+
+// One tile's loads: a token's pair, position and flag a lane (lanes 0..31 the keys' pairs, 32..63 the values'),
+// and the codes of both products.
+template <int NS>
+struct QuantTile {
+  static constexpr int VD = NS <= 4 ? 1 : NS / 4;  // dwords of a lane's piece of a V row
+  uint32_t pair;
+  int64_t pos;
+  uint32_t flag;
+  uint32_t k[2][NS], v[8][VD];
+};
+
 // One workgroup: the query heads of one KV head of one row over one of `splits` runs of tiles of 32
-// slots, its waves taking the tiles in turn. NS: the head width in units of 32, rounded up to a power of two.
+// slots, its NW waves taking the tiles in turn, each with the next tile's loads in flight while it works on
+// one. NS: the head width in units of 32, rounded up to a power of two.
 // Lane (c, g) = (l % 16, l / 16). K tile: lane holds dwords g NS .. + NS of the codes of tokens c and
 // 16 + c. V tile: lane holds features c M .. + M of tokens 4 g + i and 16 + 4 g + i (i = 0..3), M = 2 NS,
 // which are the tokens whose scores it holds; its M accumulators hold features (4 g + r) M + e, r = 0..3.
 // Features past dk: K's meet zeros of q, V's are not stored; both lie inside the ring or read as zero.
 // WHOLE: dk is a whole number of lanes' pieces (NS dwords), so no piece reaches past the ring's end.
-template <typename T, int NS, bool WHOLE>
-__global__ __launch_bounds__(64 * kAttnWaves) void quant_attn_kernel(const T* __restrict__ q, const T* __restrict__ knew,
-                                                                     const T* __restrict__ vnew, T* __restrict__ o,
-                                                                     const QuantAttnArgs a) {
+// (At least two waves a SIMD: the accumulators then stay in the registers that the rescaling reads.)
+template <typename T, int NS, bool WHOLE, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_kernel(
+    const T* __restrict__ q, const T* __restrict__ knew, const T* __restrict__ vnew, T* __restrict__ o,
+    const QuantAttnArgs a) {
   constexpr int DP = 32 * NS, M = 2 * NS;
-  constexpr int NW = kAttnWaves;
-  constexpr int VD = M <= 8 ? 1 : M / 8;  // dwords of a lane's piece of a V row
   using C = Codes<T>;
   typedef T V8 __attribute__((ext_vector_type(8)));
   __shared__ __align__(16) float2 stage[NW][2][kTile];  // the tile's pairs as the products take them
   __shared__ float smerge[NW][kQuantMaxGroup][2 + DP];
+  __shared__ float sfresh[kQuantMaxGroup];
 
-  const int lg = xcd_logical_block(blockIdx.x, gridDim.x);
+  const int grid = a.heads * a.splits;
+  if ((int)blockIdx.x >= grid) {
+    write_tokens<T, DP / 8>(knew, vnew, a, (int)blockIdx.x - grid, 64 * NW);
+    return;
+  }
+  const int lg = xcd_logical_block(blockIdx.x, grid);
   const int kvh = lg % a.HKV, rest = lg / a.HKV;
   const int b = rest / a.splits, split = rest - b * a.splits;
   const int G = a.H / a.HKV, dk = a.dk, W = a.W;
   const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = l & 15, g = l >> 4;
-  const int64_t p = a.pos[b];
-  const int slot = p < 0 ? -1 : (int)(p % W);
   const size_t head = (size_t)b * a.HKV + kvh;
   const unsigned rb = (unsigned)dk / 2;  // bytes a row
   const __amdgpu_buffer_rsrc_t rk = buffer_rsrc(a.ring_k + head * W * (dk / 8), (unsigned)W * rb);
   const __amdgpu_buffer_rsrc_t rv = buffer_rsrc(a.ring_v + head * W * (dk / 8), (unsigned)W * rb);
   const uint32_t* pairs = (l < 32 ? a.k_scale : a.v_scale) + head * W;
+  const __amdgpu_buffer_rsrc_t rp = buffer_rsrc(a.ring_pos + (size_t)b * W, 8u * (unsigned)W);
+  const __amdgpu_buffer_rsrc_t rf = buffer_rsrc(a.ring_valid + (size_t)b * W, (unsigned)W);
 
+  // A tile's loads; its first slot is below W, so that the scalar offsets stay below the resources' sizes.
+  const unsigned koff = (unsigned)c * rb + 4u * NS * (unsigned)g, voff = 4u * (unsigned)g * rb + (unsigned)(c * NS);
+  auto fetch = [&](int t, QuantTile<NS>& x) {
+    const unsigned j0 = (unsigned)(kTile * t), base = j0 * rb, js = (unsigned)(l & 31);
+    x.pos = __builtin_bit_cast(int64_t, load_b64(rp, 8u * js, 8u * j0));
+    x.flag = load_b8(rf, js, j0);
+    x.pair = pairs[min((int)(j0 + js), W - 1)];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load_dwords<NS, WHOLE>(rk, koff + 16u * u * rb, base, x.k[u]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned off = voff + (unsigned)((i & 3) + 16 * (i >> 2)) * rb;
+      if constexpr (M == 2) x.v[i][0] = load_b8(rv, off, base);
+      else if constexpr (M == 4) x.v[i][0] = load_b16(rv, off, base);
+      else load_dwords<QuantTile<NS>::VD, WHOLE>(rv, off, base, x.v[i]);
+    }
+  };
+  const int first = split * a.per, last = min(first + a.per, (W + kTile - 1) / kTile);
+  int t = first + w;
+  QuantTile<NS> even, odd;
+  if (t < last) fetch(t, even);
+
+  const int64_t p = a.pos[b];
+  const int slot = p < 0 ? -1 : (int)(p % W);
   // the group's queries: column c holds head c % 8 (columns of heads past G are zero and never stored)
   const int hd = c & 7;
   const bool has = hd < G;
@@ -260,125 +359,106 @@ __global__ __launch_bounds__(64 * kAttnWaves) void quant_attn_kernel(const T* __
     }
   }
   qsum = sum_over_rows(qsum);
-  fresh = sum_over_rows(fresh) * a.scale_log2;
+  if (w == 0) {
+    fresh = sum_over_rows(fresh) * a.scale_log2;
+    if (l < kQuantMaxGroup) sfresh[l] = fresh;
+  }
 
   float m = -1e30f, lsum = 0.f, low = 0.f;  // the running maximum, the lane's sums of P and of P m'
   f32x4 acc[M], bias = zero4();
 #pragma unroll
   for (int e = 0; e < M; ++e) acc[e] = zero4();
-  if (split == 0 && w == 0) {  // the new token starts the first wave's state
-    m = fresh;
-    lsum = g == 0 ? 1.f : 0.f;
-    if (c < 8) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int e = 0; e < M; ++e) {
-          const int f = (4 * g + r) * M + e;
-          if (f < dk) acc[e][r] = to_f32(vnew[head * dk + f]);
-        }
-    }
-  }
   const float second = c < 8 ? 0.f : 1.f;
   bf16x8 ones;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = (__bf16)128.f;
 
-  const int tiles = (W + kTile - 1) / kTile;
-  const int first = (int)((int64_t)tiles * split / a.splits), last = (int)((int64_t)tiles * (split + 1) / a.splits);
-  for (int t = first + w; t < last; t += NW) {
-    const int j0 = kTile * t;
-    // the tile's loads
-    const int js = j0 + (l & 31), jc = min(js, W - 1);
-    const uint32_t pair = pairs[jc];
-    const int64_t rp = a.ring_pos[(size_t)b * W + jc];
-    const uint8_t flag = a.ring_valid[(size_t)b * W + jc];
-    uint32_t kc[2][NS], vc[8][VD];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) load_dwords<NS, WHOLE>(rk, (unsigned)(j0 + 16 * u + c) * rb + 4u * NS * (unsigned)g, kc[u]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned off = (unsigned)(j0 + 4 * g + (i & 3) + 16 * (i >> 2)) * rb + (unsigned)(c * NS);
-      if constexpr (M == 2) vc[i][0] = load_b8(rv, off);
-      else if constexpr (M == 4) vc[i][0] = load_b16(rv, off);
-      else load_dwords<VD, WHOLE>(rv, off, vc[i]);
-    }
-    // which tokens are seen, and their pairs: lanes 0..31 the keys', 32..63 the values'
-    const bool seen = js < W && flag != 0 && rp <= p && rp > p - W && js != slot && p >= 0;
+  const CodeBits kbits(C::kOne), vbits(Codes<__bf16>::kOne);
+  const int64_t oldest = p < 0 ? INT64_MAX : p - W;  // positions past it and up to p are seen
+  auto work = [&](int t, const QuantTile<NS>& tile) {
+    // which tokens are seen (slots past W read flag 0), and their pairs
+    const bool seen = tile.flag != 0 && tile.pos <= p && tile.pos > oldest && kTile * t + (l & 31) != slot;
     const uint32_t mask = (uint32_t)__ballot(seen);
-    if (mask == 0) continue;
-    const float ps = pair_scale<T>(pair), pl = pair_low<T>(pair);
-    float2 st;
-    if (l < 32) st = make_float2(ps * a.scale_log2, (pl - C::kBias * ps) * a.scale_log2);
-    else st = seen ? make_float2(ps, pl) : make_float2(0.f, 0.f);  // no NaN of an unseen slot meets a zero weight
-    __builtin_amdgcn_wave_barrier();
-    stage[w][l >> 5][l & 31] = st;
-    __builtin_amdgcn_wave_barrier();
-    // scores of the lane's eight tokens: 4 g + i in the first tile of 16, then 16 + 4 g + i
-    float sc[8];
+    if (mask != 0) {
+      const float ps = pair_scale<T>(tile.pair), pl = pair_low<T>(tile.pair);
+      float2 st;
+      if (l < 32) st = make_float2(ps * a.scale_log2, (pl - C::kBias * ps) * a.scale_log2);
+      else st = seen ? make_float2(ps, pl) : make_float2(0.f, 0.f);  // no NaN of an unseen slot meets a zero weight
+      __builtin_amdgcn_wave_barrier();
+      stage[w][l >> 5][l & 31] = st;
+      __builtin_amdgcn_wave_barrier();
+      // scores of the lane's eight tokens: 4 g + i in the first tile of 16, then 16 + 4 g + i
+      float sc[8];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      f32x4 d = zero4();
+      for (int u = 0; u < 2; ++u) {
+        f32x4 d = zero4();
 #pragma unroll
-      for (int s = 0; s < NS; ++s) d = C::mma(C::unpack(kc[u][s]), qf[s], d);
+        for (int s = 0; s < NS; ++s) d = C::mma(C::unpack(tile.k[u][s], kbits), qf[s], d);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 ab = stage[w][0][16 * u + 4 * g + i];
-        sc[4 * u + i] = ab.x * d[i] + ab.y * qsum;
+        for (int i = 0; i < 4; ++i) {
+          const float2 ab = stage[w][0][16 * u + 4 * g + i];
+          sc[4 * u + i] = ab.x * d[i] + ab.y * qsum;
+        }
+      }
+      if (mask != 0xffffffffu) {
+        const uint32_t mine = mask >> (4 * g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (((mine >> ((i & 3) + 16 * (i >> 2))) & 1u) == 0) sc[i] = -kInf;
+      }
+      const float top = max_over_rows(max3(max3(sc[0], sc[1], sc[2]), max3(sc[3], sc[4], sc[5]), max3(sc[6], sc[7], sc[7])));
+      if (__ballot(top > m + kRaise) != 0) {
+        const float mn = __builtin_fmaxf(m, top);
+        const float f = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        lsum *= f;
+        low *= f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          bias[r] *= f;
+#pragma unroll
+          for (int e = 0; e < M; ++e) acc[e][r] *= f;
+        }
+      }
+      // weights, and the weights times the values' scales as two bf16 parts over the column halves
+      bf16x8 pv;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 ab = stage[w][1][16 * (i >> 2) + 4 * g + (i & 3)];
+        const float pj = __builtin_amdgcn_exp2f(sc[i] - m);
+        lsum += pj;
+        low = __builtin_fmaf(pj, ab.y, low);
+        const float x = pj * ab.x;
+        pv[i] = (__bf16)__builtin_fmaf(-second, (float)(__bf16)x, x);
+      }
+      bias = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pv, bias, 0, 0, 0);
+      // pairs of tokens' codes of one feature: 16 bits a token and four features
+      constexpr int PIECES = M <= 4 ? 1 : M / 4, PER = M <= 4 ? M : 4;
+#pragma unroll
+      for (int h = 0; h < PIECES; ++h) {
+        uint32_t two[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x = tile.v[2 * i][h / 2], y = tile.v[2 * i + 1][h / 2];
+          two[i] = M <= 4 ? (x | (y << 16)) : (h & 1) == 0 ? ((x & 0xffffu) | (y << 16)) : ((x >> 16) | (y & 0xffff0000u));
+        }
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          u32x4 r;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r[i] = vbits.two(two[i], e);
+          acc[4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, r), pv, acc[4 * h + e], 0, 0, 0);
+        }
       }
     }
-    if (mask != 0xffffffffu) {
-      const uint32_t mine = mask >> (4 * g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (((mine >> ((i & 3) + 16 * (i >> 2))) & 1u) == 0) sc[i] = -kInf;
-    }
-    float top = sc[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, sc[i]);
-    top = max_over_rows(top);
-    if (__ballot(top > m + kRaise) != 0) {
-      const float mn = __builtin_fmaxf(m, top);
-      const float f = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      lsum *= f;
-      low *= f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        bias[r] *= f;
-#pragma unroll
-        for (int e = 0; e < M; ++e) acc[e][r] *= f;
-      }
-    }
-    // weights, and the weights times the values' scales as two bf16 parts over the column halves
-    bf16x8 pv;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 ab = stage[w][1][16 * (i >> 2) + 4 * g + (i & 3)];
-      const float pj = __builtin_amdgcn_exp2f(sc[i] - m);
-      lsum += pj;
-      low = __builtin_fmaf(pj, ab.y, low);
-      const float x = pj * ab.x;
-      pv[i] = (__bf16)__builtin_fmaf(-second, (float)(__bf16)x, x);
-    }
-    bias = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pv, bias, 0, 0, 0);
-    // pairs of tokens' codes of one feature: 16 bits a token and four features
-    constexpr int PIECES = M <= 4 ? 1 : M / 4, PER = M <= 4 ? M : 4;
-#pragma unroll
-    for (int h = 0; h < PIECES; ++h) {
-      uint32_t two[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t x = vc[2 * i][h / 2], y = vc[2 * i + 1][h / 2];
-        two[i] = M <= 4 ? (x | (y << 16)) : (h & 1) == 0 ? ((x & 0xffffu) | (y << 16)) : ((x >> 16) | (y & 0xffff0000u));
-      }
-#pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        u32x4 r;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = ((two[i] >> (4 * e)) & 0x000f000fu) | 0x43004300u;
-        acc[4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, r), pv, acc[4 * h + e], 0, 0, 0);
-      }
+  };
+  // two tiles a turn, each in registers of its own: a tile's loads are issued before the other's work
+  for (; t < last; t += 2 * NW) {
+    if (t + NW < last) fetch(t + NW, odd);
+    work(t, even);
+    if (t + NW < last) {
+      if (t + 2 * NW < last) fetch(t + 2 * NW, even);
+      work(t + NW, odd);
     }
   }
 
@@ -391,20 +471,25 @@ __global__ __launch_bounds__(64 * kAttnWaves) void quant_attn_kernel(const T* __
     for (int e = 0; e < M; ++e) {
       float x = acc[e][r] - bias[r];
       x += dpp_f32<0x128>(x);  // row_ror:8
-      if (c < G && (4 * g + r) * M + e < dk) smerge[w][c][2 + (4 * g + r) * M + e] = x + low;
+      if (c < G) smerge[w][c][2 + (4 * g + r) * M + e] = x + low;
     }
   if (g == 0 && c < G) {
     smerge[w][c][0] = m;
     smerge[w][c][1] = lsum;
   }
   __syncthreads();
+  // the waves' states, and in the first split the new token's (weight 1 at its score), joined
   const bool on = a.active == nullptr || a.active[b] != 0;
   for (int i = tid; i < G * dk; i += 64 * NW) {
     const int gi = i / dk, d = i - gi * dk;
-    float mx = smerge[0][gi][0];
+    float mx = split == 0 ? sfresh[gi] : -1e30f;
 #pragma unroll
-    for (int u = 1; u < NW; ++u) mx = __builtin_fmaxf(mx, smerge[u][gi][0]);
+    for (int u = 0; u < NW; ++u) mx = __builtin_fmaxf(mx, smerge[u][gi][0]);
     float ls = 0.f, num = 0.f;
+    if (split == 0) {
+      ls = __builtin_amdgcn_exp2f(sfresh[gi] - mx);
+      num = ls * to_f32(vnew[head * dk + d]);
+    }
 #pragma unroll
     for (int u = 0; u < NW; ++u) {
       const float f = __builtin_amdgcn_exp2f(smerge[u][gi][0] - mx);
@@ -423,48 +508,43 @@ __global__ __launch_bounds__(64 * kAttnWaves) void quant_attn_kernel(const T* __
       }
     }
   }
-
-  // The new token into its slot, which no workgroup attends (a reader of its codes drops them).
-  if (!a.write || split != 0 || p < 0) return;
-  constexpr int L = DP / 8;
-  if (w < 2 && l < L) {
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.f;
-    const bool live = 8 * l < dk;
-    if (live) load8_f32((w == 0 ? knew : vnew) + head * dk + 8 * l, x);
-    uint32_t pr;
-    const uint32_t codes = quantize_row8<T, L>(x, live, pr);
-    const size_t row = head * W + slot;
-    if (live) (w == 0 ? a.ring_k : a.ring_v)[row * (size_t)(dk / 8) + l] = codes;
-    if (l == 0) {
-      (w == 0 ? a.k_scale : a.v_scale)[row] = pr;
-      if (w == 0 && kvh == 0) {
-        a.ring_pos[(size_t)b * W + slot] = p;
-        a.ring_valid[(size_t)b * W + slot] = 1;
-      }
-    }
-  }
 }
 
-// The splits' softmax states of one query head joined, in the splits' order.
+// The splits' softmax states of one query head joined: their weights first, one split a thread, then groups of
+// dk threads take the splits in turn and the groups' sums are added in order.
 template <typename T>
-__global__ __launch_bounds__(256) void quant_join_kernel(const float* __restrict__ partial, T* __restrict__ o,
-                                                         const uint8_t* __restrict__ active, int H, int dk, int splits) {
+__global__ __launch_bounds__(1024) void quant_join_kernel(const float* __restrict__ partial, T* __restrict__ o,
+                                                          const uint8_t* __restrict__ active, int H, int dk,
+                                                          int splits) {
+  __shared__ float weight[kMaxSplits], sums[1024], red[2][16];
   const size_t row = blockIdx.x;
-  const float* part = partial + row * splits * (size_t)(2 + dk);
-  const bool on = active == nullptr || active[row / H] != 0;
-  float mx = part[0];
-  for (int s = 1; s < splits; ++s) mx = __builtin_fmaxf(mx, part[(size_t)s * (2 + dk)]);
-  for (int d = threadIdx.x; d < dk; d += 256) {
-    float ls = 0.f, num = 0.f;
-    for (int s = 0; s < splits; ++s) {
-      const float* x = part + (size_t)s * (2 + dk);
-      const float f = __builtin_amdgcn_exp2f(x[0] - mx);
-      ls += x[1] * f;
-      num += x[2 + d] * f;
-    }
-    o[row * dk + d] = from_f32<T>(on ? num / ls : 0.f);
+  const int pitch = 2 + dk;
+  const float* part = partial + row * splits * (size_t)pitch;
+  const int t = threadIdx.x, w = t >> 6, nw = blockDim.x >> 6;
+  const float m = t < splits ? part[(size_t)t * pitch] : -1e30f, l = t < splits ? part[(size_t)t * pitch + 1] : 0.f;
+  float mx = group_max<64>(m);
+  if ((t & 63) == 0) red[0][w] = mx;
+  __syncthreads();
+  for (int u = 0; u < nw; ++u) mx = __builtin_fmaxf(mx, red[0][u]);
+  const float f = __builtin_amdgcn_exp2f(m - mx);
+  if (t < splits) weight[t] = f;
+  const float ls = group_sum<64>(t < splits ? l * f : 0.f);
+  if ((t & 63) == 0) red[1][w] = ls;
+  __syncthreads();
+  const int groups = (int)blockDim.x / dk, grp = t / dk, d = t - grp * dk;
+  float num = 0.f;
+  if (grp < groups) {
+#pragma unroll 8
+    for (int s = grp; s < splits; s += groups) num += part[(size_t)s * pitch + 2 + d] * weight[s];
+  }
+  sums[t] = num;
+  __syncthreads();
+  if (t < dk) {
+    float total = 0.f, sum = 0.f;
+    for (int u = 0; u < nw; ++u) total += red[1][u];
+    for (int u = 0; u < groups; ++u) sum += sums[u * dk + t];
+    const bool on = active == nullptr || active[row / H] != 0;
+    o[row * dk + t] = from_f32<T>(on ? sum / total : 0.f);
   }
 }
 
@@ -547,17 +627,32 @@ int quant_read(const void* ring_k, const void* ring_v, const void* k_scale, cons
   return check_launch(who);
 }
 
-// How many workgroups share a head's window: enough that the card's 256 CUs have four each, and no more
-// than there are tiles for their waves.
-int attn_splits(int B, int HKV, int W) {
-  const int64_t heads = (int64_t)B * HKV;
-  const int tiles = (W + kTile - 1) / kTile, most = (tiles + kAttnWaves - 1) / kAttnWaves;
-  const int64_t want = heads >= 1024 ? 1 : (1024 + heads - 1) / heads;
-  return (int)(want < most ? want : most);
+// How a head's window is shared: waves a workgroup, workgroups (splits) a head and tiles a split.
+//
+// A workgroup costs about 2 us before and after its tiles, a tile 0.35 to 0.8 us of a wave, and a second split
+// the launch that joins them, 3.2 to 5 us. So, with tiles for 512 workgroups of four waves and eight tiles
+// each, or 256 heads: four waves, as many splits as make 512 workgroups (64 heads of 8191 slots at dk 64: 18.0 us
+// with 512, 22.4 with 256, 19.0 with 1024; 512 heads of 512 slots: 9.4 us, with eight waves 9.9, in two splits 15.2).
+// Else the workgroup is as wide as its registers allow, 16 waves up to dk 64 and eight beyond, and a window of up
+// to 64 tiles stays whole (8 heads of 512 slots at dk 64: 6.7 us, four splits of four waves 8.0; 128 heads with four
+// query heads each: 7.1 us, four waves in two splits 9.7); longer ones are split by 32 tiles, wider heads by 16
+// (one head of 65536 slots at dk 128: 64 splits 11.0 us, 128 8.3; 32 heads of 4096 at dk 256: four splits 16.2, eight 13.7).
+constexpr int kManyGroups = 512;
+struct AttnShape {
+  int waves, splits, per;
+};
+AttnShape attn_shape(int B, int HKV, int D, int W) {
+  const int64_t heads = (int64_t)B * HKV, tiles = ((int64_t)W + kTile - 1) / kTile;
+  const int64_t runs = tiles / (D <= 64 ? 32 : 16), most = runs < 1 ? 1 : runs > kMaxSplits ? kMaxSplits : runs;
+  const int64_t share = heads >= kManyGroups ? 1 : (kManyGroups + heads - 1) / heads;
+  const bool many = heads >= 256 || heads * most >= kManyGroups;
+  const int64_t splits = !many && tiles <= 64 ? 1 : share < most ? share : most;
+  const int64_t per = (tiles + splits - 1) / splits;
+  return {many ? 4 : D <= 64 ? 16 : 8, (int)((tiles + per - 1) / per), (int)per};
 }
 
 size_t attn_workspace(int B, int H, int HKV, int D, int W) {
-  const int splits = attn_splits(B, HKV, W);
+  const int splits = attn_shape(B, HKV, D, W).splits;
   return splits == 1 ? 0 : (size_t)B * H * splits * (2 + D) * sizeof(float);
 }
 
@@ -578,28 +673,35 @@ int quant_attn(const T* q, const T* knew, const T* vnew, const int64_t* pos, voi
     return fail(ERR_ARG, "%s: q, k and v must be 16-byte aligned", who);
   if (!aligned(ring_k, 4) || !aligned(ring_v, 4) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
     return fail(ERR_ARG, "%s: the ring's tensors must be 4-byte aligned", who);
-  const int splits = attn_splits(B, HKV, W);
+  const AttnShape shape = attn_shape(B, HKV, D, W);
+  const int splits = shape.splits;
   const size_t need = attn_workspace(B, H, HKV, D, W);
   if (need > 0 && (workspace == nullptr || ws_bytes < need || !aligned(workspace, 4)))
     return fail(ERR_ARG, "%s: workspace of %zu bytes given, %zu needed", who, workspace ? ws_bytes : (size_t)0, need);
-  const int64_t grid = (int64_t)B * HKV * splits;
+  const int threads = 64 * shape.waves, lanes = D <= 32 ? 4 : lanes_of(D);
+  const int64_t grid = (int64_t)B * HKV * splits + (write ? ((int64_t)B * HKV * 2 * lanes + threads - 1) / threads : 0);
   if (grid >= ((int64_t)1 << 31) || (int64_t)B * H >= ((int64_t)1 << 31))
     return fail(ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
   const QuantAttnArgs a{pos, static_cast<uint32_t*>(ring_k), static_cast<uint32_t*>(ring_v),
                         static_cast<uint32_t*>(k_scale), static_cast<uint32_t*>(v_scale), ring_pos, ring_valid, active,
-                        static_cast<float*>(workspace), B, H, HKV, D, W, splits, write,
-                        scale * 1.4426950408889634f};
+                        static_cast<float*>(workspace), B, H, HKV, D, W, splits, shape.per,
+                        B * HKV, scale * 1.4426950408889634f};
   auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kAttnWaves), 0, stream, q, knew, vnew, o, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(threads), 0, stream, q, knew, vnew, o, a);
   };
-  if (D <= 32) go(quant_attn_kernel<T, 1, true>);
-  else if (D <= 64) D % 16 == 0 ? go(quant_attn_kernel<T, 2, true>) : go(quant_attn_kernel<T, 2, false>);
-  else if (D <= 128) D % 32 == 0 ? go(quant_attn_kernel<T, 4, true>) : go(quant_attn_kernel<T, 4, false>);
-  else D % 64 == 0 ? go(quant_attn_kernel<T, 8, true>) : go(quant_attn_kernel<T, 8, false>);
+  auto by_width = [&](auto nw) {  // four waves, or the most that the width's registers allow (0)
+    constexpr int NW = decltype(nw)::value, N64 = NW == 0 ? 16 : NW, N256 = NW == 0 ? 8 : NW;
+    if (D <= 32) go(quant_attn_kernel<T, 1, true, N64>);
+    else if (D <= 64) D % 16 == 0 ? go(quant_attn_kernel<T, 2, true, N64>) : go(quant_attn_kernel<T, 2, false, N64>);
+    else if (D <= 128) D % 32 == 0 ? go(quant_attn_kernel<T, 4, true, N256>) : go(quant_attn_kernel<T, 4, false, N256>);
+    else D % 64 == 0 ? go(quant_attn_kernel<T, 8, true, N256>) : go(quant_attn_kernel<T, 8, false, N256>);
+  };
+  if (shape.waves == 4) by_width(std::integral_constant<int, 4>{});
+  else by_width(std::integral_constant<int, 0>{});
   if (splits > 1)
-    hipLaunchKernelGGL(quant_join_kernel<T>, dim3((unsigned)(B * H)), dim3(256), 0, stream,
-                       static_cast<const float*>(workspace), o, active, H, D, splits);
+    hipLaunchKernelGGL(quant_join_kernel<T>, dim3((unsigned)(B * H)), dim3(splits <= 8 ? 256 : 1024), 0,
+                       stream, static_cast<const float*>(workspace), o, active, H, D, splits);
   return check_launch(who);
 }
 
