@@ -35,31 +35,50 @@ __device__ __forceinline__ float pair_low(uint32_t pair) {
   return to_f32(__builtin_bit_cast(T, (uint16_t)(pair >> 16)));
 }
 
+// The least and the greatest of three, without fminf's and fmaxf's quieting of their inputs.
+__device__ __forceinline__ float min3(float x, float y, float z) {
+  float r = x;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+#endif
+  return r;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r = x;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+#endif
+  return r;
+}
+
 // Eight features of a row held by L adjacent lanes (lanes past the row's width are not live): the
 // lane's dword of codes, and the row's pair in every lane.
 template <typename T, int L>
 __device__ __forceinline__ uint32_t quantize_row8(const float (&x)[8], bool live, uint32_t& pair) {
-  float lo = kInf, hi = -kInf, bad = 0.f;
+  float lo = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), min3(x[6], x[7], x[7]));
+  float hi = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7]));
+  float bad = 0.f;  // NaN where the row holds a NaN or an infinity (which times 0 is one)
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float f = 0.5f * x[e];
-    if (live) {
-      lo = __builtin_fminf(lo, f);
-      hi = __builtin_fmaxf(hi, f);
-      if (!(__builtin_fabsf(x[e]) < kInf)) bad = 1.f;
-    }
-  }
-  lo = -group_max<L>(-lo);
-  hi = group_max<L>(hi);
-  bad = group_max<L>(bad);
+  for (int e = 0; e < 8; ++e) bad = __builtin_fmaf(x[e], 0.f, bad);
+  lo = 0.5f * -group_max<L>(live ? -lo : -kInf);
+  hi = 0.5f * group_max<L>(live ? hi : -kInf);
+  bad = group_sum<L>(live ? bad : 0.f);
   const T s = from_f32<T>(2.f * ((hi - lo) / 15.f));
   const float half = 0.5f * to_f32(s);
   uint32_t codes = 0;
   if (half > 0.f && bad == 0.f) {
+    // The quotient n / step by a reciprocal and one Newton step on the residual, which fma forms exactly: the
+    // correctly rounded quotient in three instructions. Small steps are scaled up first (exactly), so that the
+    // reciprocal and the residual stay normal numbers; the largest step, 2^124, has a normal reciprocal.
+    const float up = half < 0x1p-60f ? 0x1p80f : 1.f;
+    const float step = half * up, low = lo * up, inv = 1.f / step;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float c = __builtin_rintf((0.5f * x[e] - lo) / half);
-      codes |= (uint32_t)__builtin_fminf(__builtin_fmaxf(c, 0.f), 15.f) << (4 * e);
+      const float n = __builtin_fmaf(x[e], 0.5f * up, -low);
+      const float t = n * inv;
+      const float q = __builtin_amdgcn_fmed3f(__builtin_fmaf(__builtin_fmaf(-t, step, n), inv, t), 0.f, 15.f);
+      // 2^23 + 2^22 more: the sum's rounding is that of q to a whole number, ties to even, in its low bits
+      codes += (__float_as_uint(q + 12582912.f) - 0x4B400000u) << (4 * e);
     }
   }
   const T nan = from_f32<T>(__builtin_nanf(""));
@@ -78,11 +97,13 @@ __device__ __forceinline__ V8 dequantize_row8(uint32_t codes, uint32_t pair) {
   const float s = pair_scale<T>(pair), lo = pair_low<T>(pair);
   V8 y;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float v = __builtin_fmaf(s, (float)((codes >> (4 * e)) & 15u), lo);
-    if (v > kFiniteMax<T>) v = kFiniteMax<T>;
-    if (v < -kFiniteMax<T>) v = -kFiniteMax<T>;
-    y[e] = from_f32<T>(v);
+  for (int e = 0; e < 8; ++e) y[e] = from_f32<T>(__builtin_fmaf(s, (float)((codes >> (4 * e)) & 15u), lo));
+  if (__builtin_fmaf(15.f, s, lo) > kFiniteMax<T>) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = __builtin_fmaf(s, (float)((codes >> (4 * e)) & 15u), lo);
+      y[e] = from_f32<T>(v > kFiniteMax<T> ? kFiniteMax<T> : v);
+    }
   }
   return y;
 }

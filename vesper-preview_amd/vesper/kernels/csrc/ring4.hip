@@ -42,9 +42,15 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // ---- writing and reading ------------------------------------------------------------------------
-// L lanes a row of eight features each; a workgroup takes 256 / L tokens of one head, keys or values, so
-// the ring's side is contiguous and the tokens' side whole rows of dk elements. The heads of the same
-// tokens are consecutive workgroups of one XCD (short rows share their cache lines there).
+// L lanes a row of eight features each, key and value of a token by the same lanes; a workgroup takes 256 / L
+// tokens of one head, so the ring's side is contiguous and the tokens' side whole rows of dk elements. The heads
+// of the same tokens are consecutive workgroups of one XCD (short rows share their cache lines there). What is
+// left is the arithmetic a row (the slot's division by W and the indices), so a lane group takes both rows.
+// slot of a position >= 0: most fit 32 bits, where the division is a fraction of the 64-bit one
+__device__ __forceinline__ int slot_of(int64_t p, int W) {
+  return (uint64_t)p >> 32 == 0 ? (int)((uint32_t)p % (uint32_t)W) : (int)(p % W);
+}
+
 template <typename T, int L>
 __global__ __launch_bounds__(256) void quant_write_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                           const int64_t* __restrict__ pos,
@@ -53,30 +59,39 @@ __global__ __launch_bounds__(256) void quant_write_kernel(const T* __restrict__ 
                                                           int64_t* ring_pos, uint8_t* ring_valid, int B, int N, int HKV,
                                                           int dk, int W, int blocks) {
   constexpr int TB = 256 / L;
-  const int lg = xcd_logical_block(blockIdx.x, gridDim.x);
-  const int head2 = lg % (2 * HKV), rest = lg / (2 * HKV);
-  const int b = rest / blocks, tb = rest - b * blocks;
-  const int head = head2 >> 1;
-  const bool values = (head2 & 1) != 0;
-  const int part = threadIdx.x % L, t = tb * TB + (int)threadIdx.x / L;
+  const unsigned lg = (unsigned)xcd_logical_block(blockIdx.x, gridDim.x);
+  const unsigned head = lg % (unsigned)HKV, rest = lg / (unsigned)HKV;
+  const unsigned b = rest / (unsigned)blocks, tb = rest - b * (unsigned)blocks;
+  const unsigned part = threadIdx.x % L, t = threadIdx.x / L;
   const int len = lengths == nullptr ? N : (int)min(max(lengths[b], (int64_t)0), (int64_t)N);
-  const int i = max(len - W, 0) + t;  // the last W tokens of the row are the ones that stay
-  if (i >= len) return;               // whole rows of lanes leave together
-  const int64_t p = pos[(size_t)b * N + i];
-  if (p < 0) return;  // refused by the host wrapper
-  const int slot = (int)(p % W);
-  const bool live = 8 * part < dk;
-  float x[8];
+  const int i0 = max(len - W, 0) + (int)tb * TB;  // the last W tokens of the row are the ones that stay
+  if ((int)t >= len - i0) return;                 // whole rows of lanes leave together
+  const size_t token = (size_t)b * N + i0;        // the workgroup's first; lanes add 32-bit offsets
+  const int64_t p = pos[token + t];
+  const bool live = (int)(8 * part) < dk;
+  float xk[8], xv[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = 0.f;
-  if (live) load8_f32((values ? v : k) + (((size_t)b * N + i) * HKV + head) * dk + 8 * part, x);
-  uint32_t pair;
-  const uint32_t codes = quantize_row8<T, L>(x, live, pair);
-  const size_t row = ((size_t)b * HKV + head) * W + slot;
-  if (live) (values ? ring_v : ring_k)[row * (size_t)(dk / 8) + part] = codes;
+  for (int e = 0; e < 8; ++e) xk[e] = xv[e] = 0.f;
+  if (live) {
+    const size_t base = (token * HKV + head) * dk;
+    const unsigned at = t * (unsigned)(HKV * dk) + 8 * part;
+    load8_f32(k + base + at, xk);
+    load8_f32(v + base + at, xv);
+  }
+  if (p < 0) return;  // refused by the host wrapper
+  const unsigned slot = (unsigned)slot_of(p, W);
+  const size_t first = ((size_t)b * HKV + head) * W;  // the head's rows
+  uint32_t pk, pv;
+  const uint32_t ck = quantize_row8<T, L>(xk, live, pk), cv = quantize_row8<T, L>(xv, live, pv);
+  if (live) {
+    const unsigned at = slot * (unsigned)(dk / 8) + part;
+    (ring_k + first * (dk / 8))[at] = ck;
+    (ring_v + first * (dk / 8))[at] = cv;
+  }
   if (part == 0) {
-    (values ? v_scale : k_scale)[row] = pair;
-    if (head2 == 0) {
+    (k_scale + first)[slot] = pk;
+    (v_scale + first)[slot] = pv;
+    if (head == 0) {
       ring_pos[(size_t)b * W + slot] = p;
       ring_valid[(size_t)b * W + slot] = 1;
     }
@@ -95,28 +110,35 @@ __global__ __launch_bounds__(256) void quant_read_kernel(const uint32_t* __restr
                                                          int HKV, int dk, int W, int blocks) {
   typedef T V8 __attribute__((ext_vector_type(8)));
   constexpr int TB = 256 / L;
-  const int lg = xcd_logical_block(blockIdx.x, gridDim.x);
-  const int head2 = lg % (2 * HKV), rest = lg / (2 * HKV);
-  const int b = rest / blocks, tb = rest - b * blocks;
-  const int head = head2 >> 1;
-  const bool values = (head2 & 1) != 0;
-  const int part = threadIdx.x % L, i = tb * TB + (int)threadIdx.x / L;
-  if (i >= N) return;
-  const int64_t p = pos[(size_t)b * N + i];
-  const int slot = p < 0 ? 0 : (int)(p % W);
-  const size_t at = (size_t)b * W + slot;
-  const bool here = p >= 0 && ring_valid[at] != 0 && ring_pos[at] == p;
-  const size_t row = ((size_t)b * HKV + head) * W + slot;
-  if (8 * part < dk) {
-    V8 y;
+  const unsigned lg = (unsigned)xcd_logical_block(blockIdx.x, gridDim.x);
+  const unsigned head = lg % (unsigned)HKV, rest = lg / (unsigned)HKV;
+  const unsigned b = rest / (unsigned)blocks, tb = rest - b * (unsigned)blocks;
+  const unsigned part = threadIdx.x % L, t = threadIdx.x / L;
+  if ((int)t >= N - (int)tb * TB) return;
+  const size_t token = (size_t)b * N + tb * TB;  // the workgroup's first; lanes add 32-bit offsets
+  const int64_t p = pos[token + t];
+  const unsigned slot = p < 0 ? 0u : (unsigned)slot_of(p, W);
+  // the row's codes are loaded with the flag and position that say whether they count: one wait, not two
+  const uint8_t flag = (ring_valid + (size_t)b * W)[slot];
+  const int64_t held = (ring_pos + (size_t)b * W)[slot];
+  const size_t first = ((size_t)b * HKV + head) * W;  // the head's rows
+  const bool live = (int)(8 * part) < dk;
+  const unsigned piece = slot * (unsigned)(dk / 8) + (live ? part : 0u);
+  const uint32_t ck = (ring_k + first * (dk / 8))[piece], cv = (ring_v + first * (dk / 8))[piece];
+  const uint32_t pk = (k_scale + first)[slot], pv = (v_scale + first)[slot];
+  const bool here = p >= 0 && flag != 0 && held == p;
+  if (live) {
+    V8 yk = dequantize_row8<T, V8>(ck, pk), yv = dequantize_row8<T, V8>(cv, pv);
+    if (!here) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = from_f32<T>(0.f);
-    if (here)
-      y = dequantize_row8<T, V8>((values ? ring_v : ring_k)[row * (size_t)(dk / 8) + part],
-                                 (values ? v_scale : k_scale)[row]);
-    *reinterpret_cast<V8*>((values ? v : k) + (((size_t)b * N + i) * HKV + head) * dk + 8 * part) = y;
+      for (int e = 0; e < 8; ++e) yk[e] = yv[e] = from_f32<T>(0.f);
+    }
+    const size_t base = (token * HKV + head) * dk;
+    const unsigned to = t * (unsigned)(HKV * dk) + 8 * part;
+    *reinterpret_cast<V8*>(k + base + to) = yk;
+    *reinterpret_cast<V8*>(v + base + to) = yv;
   }
-  if (head2 == 0 && part == 0) found[(size_t)b * N + i] = here ? 1 : 0;
+  if (head == 0 && part == 0) found[token + t] = here ? 1 : 0;
 }
 
 // ---- attention ----------------------------------------------------------------------------------
@@ -201,14 +223,6 @@ __device__ __forceinline__ void load_dwords(__amdgpu_buffer_rsrc_t r, unsigned o
   }
 }
 
-__device__ __forceinline__ float max3(float x, float y, float z) {
-  float r = x;
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));  // without fmaxf's quieting of its inputs
-#endif
-  return r;
-}
-
 // The largest of x over the lanes l, l ^ 16, l ^ 32, l ^ 48 (a column of an MFMA result).
 __device__ __forceinline__ float max_over_rows(float x) {
   const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -243,7 +257,7 @@ __device__ __forceinline__ void write_tokens(const T* knew, const T* vnew, const
   const int b = (int)(head / a.HKV), kvh = (int)(head - (size_t)b * a.HKV);
   const int64_t p = a.pos[b];
   if (p < 0) return;
-  const int slot = (int)(p % a.W);
+  const int slot = slot_of(p, a.W);
   const bool live = 8 * part < a.dk;
   float x[8];
 #pragma unroll
@@ -334,7 +348,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
   if (t < last) fetch(t, even);
 
   const int64_t p = a.pos[b];
-  const int slot = p < 0 ? -1 : (int)(p % W);
+  const int slot = p < 0 ? -1 : slot_of(p, W);
   // the group's queries: column c holds head c % 8 (columns of heads past G are zero and never stored)
   const int hd = c & 7;
   const bool has = hd < G;
@@ -555,6 +569,7 @@ bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p)
 // The sizes every entry shares; 0 or an error.
 int quant_sizes(int B, int HKV, int D, int W, const char* who) {
   if (B < 0 || HKV < 1 || W < 1) return fail(ERR_ARG, "%s: bad sizes B=%d HKV=%d W=%d", who, B, HKV, W);
+  if (HKV > (1 << 14)) return fail(ERR_UNSUPPORTED, "%s: %d KV heads (at most 16384)", who, HKV);
   if (D < 8 || D > 256 || D % 8 != 0)
     return fail(ERR_UNSUPPORTED, "%s: head dimension %d (kernels: multiples of 8 up to 256)", who, D);
   if ((int64_t)(W + (int64_t)kTile) * (D / 2) >= ((int64_t)1 << 31))
@@ -590,7 +605,7 @@ int quant_write(const T* k, const T* v, const int64_t* pos, const int64_t* lengt
   if (!aligned(ring_k, 4) || !aligned(ring_v, 4) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
     return fail(ERR_ARG, "%s: the ring's tensors must be 4-byte aligned", who);
   const int tb = 256 / lanes_of(D), blocks = ((N < W ? N : W) + tb - 1) / tb;
-  const int64_t grid = (int64_t)B * blocks * 2 * HKV;
+  const int64_t grid = (int64_t)B * blocks * HKV;
   if (grid >= ((int64_t)1 << 31)) return fail(ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
   by_lanes(D, [&](auto lanes) {
     hipLaunchKernelGGL((quant_write_kernel<T, decltype(lanes)::value>), dim3((unsigned)grid), dim3(256), 0,
@@ -615,7 +630,7 @@ int quant_read(const void* ring_k, const void* ring_v, const void* k_scale, cons
   if (!aligned(ring_k, 4) || !aligned(ring_v, 4) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
     return fail(ERR_ARG, "%s: the ring's tensors must be 4-byte aligned", who);
   const int tb = 256 / lanes_of(D), blocks = (int)(((int64_t)N + tb - 1) / tb);
-  const int64_t grid = (int64_t)B * blocks * 2 * HKV;
+  const int64_t grid = (int64_t)B * blocks * HKV;
   if (grid >= ((int64_t)1 << 31)) return fail(ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
   by_lanes(D, [&](auto lanes) {
     hipLaunchKernelGGL((quant_read_kernel<T, decltype(lanes)::value>), dim3((unsigned)grid), dim3(256), 0,

@@ -32,6 +32,7 @@ from vesper.contracts import ContractError, Dims, check_shape, require
 from vesper.kernels import _lib
 from vesper.kernels.ring_attn import MAX_GROUP, MAX_HEAD_DIM, _aligned
 
+MAX_KV_HEADS = 16384  # a workgroup's tokens are addressed by 32-bit offsets
 _SUFFIX = {torch.bfloat16: "bf16", torch.float16: "f16"}
 
 
@@ -99,6 +100,8 @@ def _check_ring(cache: QuantRingKVCache, dims: Dims) -> torch.dtype:
         raise ContractError(f"cache.k_scale: dtype must be bfloat16 or float16, got {dtype}")
     if cache.window < 1:
         raise ContractError(f"the ring's window must be at least 1, got {cache.window}")
+    if dims["hkv"] > MAX_KV_HEADS:
+        raise ContractError(f"cache.k: {dims['hkv']} KV heads, the kernels take at most {MAX_KV_HEADS}")
     dk = 2 * dims["half"]
     if dims.setdefault("dk", dk) != dk:
         raise ContractError(f"cache.k: rows of {dims['half']} bytes hold {dk} features, the tokens have {dims['dk']}")
