@@ -35,55 +35,62 @@ __device__ __forceinline__ float pair_low(uint32_t pair) {
   return to_f32(__builtin_bit_cast(T, (uint16_t)(pair >> 16)));
 }
 
-// The least and the greatest of three, without fminf's and fmaxf's quieting of their inputs.
+// The least and the greatest of three (one instruction, gfx950's): NaN where one of them is NaN.
 __device__ __forceinline__ float min3(float x, float y, float z) {
   float r = x;
 #if defined(__HIP_DEVICE_COMPILE__)
-  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  asm("v_minimum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
 #endif
   return r;
 }
 __device__ __forceinline__ float max3(float x, float y, float z) {
   float r = x;
 #if defined(__HIP_DEVICE_COMPILE__)
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
 #endif
   return r;
 }
+struct MinNanOp {
+  __device__ __forceinline__ float operator()(float x, float y) const { return min3(x, y, y); }
+};
+struct MaxNanOp {
+  __device__ __forceinline__ float operator()(float x, float y) const { return max3(x, y, y); }
+};
 
-// Eight features of a row held by L adjacent lanes (lanes past the row's width are not live): the
-// lane's dword of codes, and the row's pair in every lane.
+// n / d correctly rounded, for finite n and normal d and 1 / d: a reciprocal within one unit and one Newton
+// step on the residual, which fma forms exactly.
+__device__ __forceinline__ float quotient(float n, float d, float reciprocal) {
+  const float t = n * reciprocal;
+  return __builtin_fmaf(__builtin_fmaf(-t, d, n), reciprocal, t);
+}
+
+// Eight features of a row held by L adjacent lanes (a lane past the row's width holds features of the row
+// again, which change nothing): the lane's dword of codes, and the row's pair in every lane.
 template <typename T, int L>
-__device__ __forceinline__ uint32_t quantize_row8(const float (&x)[8], bool live, uint32_t& pair) {
+__device__ __forceinline__ uint32_t quantize_row8(const float (&x)[8], uint32_t& pair) {
   float lo = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), min3(x[6], x[7], x[7]));
   float hi = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7]));
-  float bad = 0.f;  // NaN where the row holds a NaN or an infinity (which times 0 is one)
-#pragma unroll
-  for (int e = 0; e < 8; ++e) bad = __builtin_fmaf(x[e], 0.f, bad);
-  lo = 0.5f * -group_max<L>(live ? -lo : -kInf);
-  hi = 0.5f * group_max<L>(live ? hi : -kInf);
-  bad = group_sum<L>(live ? bad : 0.f);
-  const T s = from_f32<T>(2.f * ((hi - lo) / 15.f));
+  lo = 0.5f * group_reduce<L>(lo, MinNanOp{});
+  hi = 0.5f * group_reduce<L>(hi, MaxNanOp{});
+  const float range = hi - lo;  // finite for finite features; infinite or NaN with an infinity or a NaN
+  const bool fine = range < kInf;
+  const T s = from_f32<T>(2.f * quotient(range, 15.f, 1.f / 15.f));
   const float half = 0.5f * to_f32(s);
+  // Small steps are scaled up first (exactly), so that the reciprocal and the residual stay normal numbers;
+  // the largest step, 2^124, has a normal reciprocal.
+  const float up = half < 0x1p-60f ? 0x1p80f : 1.f;
+  const float step = half * up, low = lo * up, inv = half > 0.f ? __builtin_amdgcn_rcpf(step) : 0.f;
   uint32_t codes = 0;
-  if (half > 0.f && bad == 0.f) {
-    // The quotient n / step by a reciprocal and one Newton step on the residual, which fma forms exactly: the
-    // correctly rounded quotient in three instructions. Small steps are scaled up first (exactly), so that the
-    // reciprocal and the residual stay normal numbers; the largest step, 2^124, has a normal reciprocal.
-    const float up = half < 0x1p-60f ? 0x1p80f : 1.f;
-    const float step = half * up, low = lo * up, inv = 1.f / step;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float n = __builtin_fmaf(x[e], 0.5f * up, -low);
-      const float t = n * inv;
-      const float q = __builtin_amdgcn_fmed3f(__builtin_fmaf(__builtin_fmaf(-t, step, n), inv, t), 0.f, 15.f);
-      // 2^23 + 2^22 more: the sum's rounding is that of q to a whole number, ties to even, in its low bits
-      codes += (__float_as_uint(q + 12582912.f) - 0x4B400000u) << (4 * e);
-    }
+  for (int e = 0; e < 8; ++e) {
+    const float q = __builtin_fminf(quotient(__builtin_fmaf(x[e], 0.5f * up, -low), step, inv), 15.f);
+    // 2^23 + 2^22 more: the sum's rounding is that of q to a whole number, ties to even, in its low bits
+    codes += __float_as_uint(q + 12582912.f) << (4 * e);
   }
+  codes -= 0x4B400000u * 0x11111111u;  // the sum's exponent bits of all eight
   const T nan = from_f32<T>(__builtin_nanf(""));
-  pair = bad == 0.f ? pack_pair<T>(s, from_f32<T>(2.f * lo)) : pack_pair<T>(nan, nan);
-  return codes;
+  pair = fine ? pack_pair<T>(s, from_f32<T>(2.f * lo)) : pack_pair<T>(nan, nan);
+  return fine ? codes : 0u;
 }
 
 template <typename T> constexpr float kFiniteMax = 0.f;

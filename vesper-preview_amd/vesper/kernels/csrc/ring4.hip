@@ -67,32 +67,29 @@ __global__ __launch_bounds__(256) void quant_write_kernel(const T* __restrict__ 
   const int i0 = max(len - W, 0) + (int)tb * TB;  // the last W tokens of the row are the ones that stay
   if ((int)t >= len - i0) return;                 // whole rows of lanes leave together
   const size_t token = (size_t)b * N + i0;        // the workgroup's first; lanes add 32-bit offsets
-  const int64_t p = pos[token + t];
+  const int64_t p = pos[token];                   // positions go up by one: the first gives all
   const bool live = (int)(8 * part) < dk;
   float xk[8], xv[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) xk[e] = xv[e] = 0.f;
-  if (live) {
-    const size_t base = (token * HKV + head) * dk;
-    const unsigned at = t * (unsigned)(HKV * dk) + 8 * part;
-    load8_f32(k + base + at, xk);
-    load8_f32(v + base + at, xv);
-  }
+  const size_t base = (token * HKV + head) * dk;
+  const unsigned at = t * (unsigned)(HKV * dk) + (live ? 8 * part : 0u);
+  load8_f32(k + base + at, xk);
+  load8_f32(v + base + at, xv);
   if (p < 0) return;  // refused by the host wrapper
-  const unsigned slot = (unsigned)slot_of(p, W);
+  unsigned slot = (unsigned)slot_of(p, W) + t;  // t is below W, as tokens past it are not kept
+  if (slot >= (unsigned)W) slot -= (unsigned)W;
   const size_t first = ((size_t)b * HKV + head) * W;  // the head's rows
   uint32_t pk, pv;
-  const uint32_t ck = quantize_row8<T, L>(xk, live, pk), cv = quantize_row8<T, L>(xv, live, pv);
+  const uint32_t ck = quantize_row8<T, L>(xk, pk), cv = quantize_row8<T, L>(xv, pv);
   if (live) {
-    const unsigned at = slot * (unsigned)(dk / 8) + part;
-    (ring_k + first * (dk / 8))[at] = ck;
-    (ring_v + first * (dk / 8))[at] = cv;
+    const unsigned to = slot * (unsigned)(dk / 8) + part;
+    (ring_k + first * (dk / 8))[to] = ck;
+    (ring_v + first * (dk / 8))[to] = cv;
   }
   if (part == 0) {
     (k_scale + first)[slot] = pk;
     (v_scale + first)[slot] = pv;
     if (head == 0) {
-      ring_pos[(size_t)b * W + slot] = p;
+      ring_pos[(size_t)b * W + slot] = p + t;
       ring_valid[(size_t)b * W + slot] = 1;
     }
   }
@@ -223,12 +220,21 @@ __device__ __forceinline__ void load_dwords(__amdgpu_buffer_rsrc_t r, unsigned o
   }
 }
 
+// The greatest of three that are not NaN, without fmaxf's quieting of its inputs.
+__device__ __forceinline__ float top3(float x, float y, float z) {
+  float r = x;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+#endif
+  return r;
+}
+
 // The largest of x over the lanes l, l ^ 16, l ^ 32, l ^ 48 (a column of an MFMA result).
 __device__ __forceinline__ float max_over_rows(float x) {
   const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = max3(__uint_as_float(p[0]), __uint_as_float(p[1]), __uint_as_float(p[1]));
+  x = top3(__uint_as_float(p[0]), __uint_as_float(p[1]), __uint_as_float(p[1]));
   const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return max3(__uint_as_float(q[0]), __uint_as_float(q[1]), __uint_as_float(q[1]));
+  return top3(__uint_as_float(q[0]), __uint_as_float(q[1]), __uint_as_float(q[1]));
 }
 
 struct QuantAttnArgs {
@@ -260,11 +266,9 @@ __device__ __forceinline__ void write_tokens(const T* knew, const T* vnew, const
   const int slot = slot_of(p, a.W);
   const bool live = 8 * part < a.dk;
   float x[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = 0.f;
-  if (live) load8_f32((values ? vnew : knew) + head * a.dk + 8 * part, x);
+  load8_f32((values ? vnew : knew) + head * a.dk + (live ? 8 * part : 0), x);
   uint32_t pair;
-  const uint32_t codes = quantize_row8<T, L>(x, live, pair);
+  const uint32_t codes = quantize_row8<T, L>(x, pair);
   const size_t row = head * a.W + slot;
   if (live) (values ? a.ring_v : a.ring_k)[row * (size_t)(a.dk / 8) + part] = codes;
   if (part == 0) {
@@ -420,7 +424,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
         for (int i = 0; i < 8; ++i)
           if (((mine >> ((i & 3) + 16 * (i >> 2))) & 1u) == 0) sc[i] = -kInf;
       }
-      const float top = max_over_rows(max3(max3(sc[0], sc[1], sc[2]), max3(sc[3], sc[4], sc[5]), max3(sc[6], sc[7], sc[7])));
+      const float top = max_over_rows(top3(top3(sc[0], sc[1], sc[2]), top3(sc[3], sc[4], sc[5]), top3(sc[6], sc[7], sc[7])));
       if (__ballot(top > m + kRaise) != 0) {
         const float mn = __builtin_fmaxf(m, top);
         const float f = __builtin_amdgcn_exp2f(m - mn);

@@ -141,7 +141,8 @@ def quant_ring_write(k: Tensor, v: Tensor, pos: Tensor, cache: QuantRingKVCache,
 
     Args:
         k, v: ``[b, n, hkv, dk]`` rotated keys and values in the ring's dtype.
-        pos: ``[b, n]`` int64 nonnegative positions, going up by one along each row.
+        pos: ``[b, n]`` int64 nonnegative positions, going up by one along each row (the kernel reads some of
+            a row's and counts on from them).
         cache: the ring; a row's last ``window`` tokens replace what their slots hold.
         lengths: optional int32 or int64 ``[b]``, 0 to ``n``: row ``i`` writes its first ``lengths[i]`` tokens only (a
             padded batch); the others, and their positions, are not looked at.
