@@ -102,16 +102,20 @@ template <> constexpr float kFiniteMax<_Float16> = 65504.f;
 template <typename T, typename V8>
 __device__ __forceinline__ V8 dequantize_row8(uint32_t codes, uint32_t pair) {
   const float s = pair_scale<T>(pair), lo = pair_low<T>(pair);
-  V8 y;
+  const uint32_t even = codes & 0x0f0f0f0fu, odd = (codes >> 4) & 0x0f0f0f0fu;  // bytes: one instruction a float
+  float f[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = from_f32<T>(__builtin_fmaf(s, (float)((codes >> (4 * e)) & 15u), lo));
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __builtin_fmaf(s, (float)((even >> (8 * i)) & 255u), lo);
+    f[2 * i + 1] = __builtin_fmaf(s, (float)((odd >> (8 * i)) & 255u), lo);
+  }
   if (__builtin_fmaf(15.f, s, lo) > kFiniteMax<T>) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = __builtin_fmaf(s, (float)((codes >> (4 * e)) & 15u), lo);
-      y[e] = from_f32<T>(v > kFiniteMax<T> ? kFiniteMax<T> : v);
-    }
+    for (int e = 0; e < 8; ++e) f[e] = f[e] > kFiniteMax<T> ? kFiniteMax<T> : f[e];
   }
+  V8 y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = from_f32<T>(f[e]);
   return y;
 }
 

@@ -125,11 +125,9 @@ __global__ __launch_bounds__(256) void quant_read_kernel(const uint32_t* __restr
   const uint32_t pk = (k_scale + first)[slot], pv = (v_scale + first)[slot];
   const bool here = p >= 0 && flag != 0 && held == p;
   if (live) {
-    V8 yk = dequantize_row8<T, V8>(ck, pk), yv = dequantize_row8<T, V8>(cv, pv);
-    if (!here) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) yk[e] = yv[e] = from_f32<T>(0.f);
-    }
+    // a token that is not held: zeros, as codes and pairs of zero give
+    const V8 yk = dequantize_row8<T, V8>(here ? ck : 0u, here ? pk : 0u);
+    const V8 yv = dequantize_row8<T, V8>(here ? cv : 0u, here ? pv : 0u);
     const size_t base = (token * HKV + head) * dk;
     const unsigned to = t * (unsigned)(HKV * dk) + 8 * part;
     *reinterpret_cast<V8*>(k + base + to) = yk;
