@@ -95,6 +95,7 @@ __global__ __launch_bounds__(256) void quant_write_kernel(const T* __restrict__ 
   }
 }
 
+constexpr int kReadTokens = 2;  // tokens a lane group of the read takes
 template <typename T, int L>
 __global__ __launch_bounds__(256) void quant_read_kernel(const uint32_t* __restrict__ ring_k,
                                                          const uint32_t* __restrict__ ring_v,
@@ -106,34 +107,49 @@ __global__ __launch_bounds__(256) void quant_read_kernel(const uint32_t* __restr
                                                          T* __restrict__ v, uint8_t* __restrict__ found, int B, int N,
                                                          int HKV, int dk, int W, int blocks) {
   typedef T V8 __attribute__((ext_vector_type(8)));
-  constexpr int TB = 256 / L;
+  constexpr int TB = 256 / L, R = kReadTokens;
   const unsigned lg = (unsigned)xcd_logical_block(blockIdx.x, gridDim.x);
   const unsigned head = lg % (unsigned)HKV, rest = lg / (unsigned)HKV;
   const unsigned b = rest / (unsigned)blocks, tb = rest - b * (unsigned)blocks;
-  const unsigned part = threadIdx.x % L, t = threadIdx.x / L;
-  if ((int)t >= N - (int)tb * TB) return;
-  const size_t token = (size_t)b * N + tb * TB;  // the workgroup's first; lanes add 32-bit offsets
-  const int64_t p = pos[token + t];
-  const unsigned slot = p < 0 ? 0u : (unsigned)slot_of(p, W);
-  // the row's codes are loaded with the flag and position that say whether they count: one wait, not two
-  const uint8_t flag = (ring_valid + (size_t)b * W)[slot];
-  const int64_t held = (ring_pos + (size_t)b * W)[slot];
+  const unsigned part = threadIdx.x % L, t0 = threadIdx.x / L;
+  const size_t token = (size_t)b * N + tb * (R * TB);  // the workgroup's first; lanes add 32-bit offsets
+  const int left = N - (int)(tb * (R * TB));
   const size_t first = ((size_t)b * HKV + head) * W;  // the head's rows
   const bool live = (int)(8 * part) < dk;
-  const unsigned piece = slot * (unsigned)(dk / 8) + (live ? part : 0u);
-  const uint32_t ck = (ring_k + first * (dk / 8))[piece], cv = (ring_v + first * (dk / 8))[piece];
-  const uint32_t pk = (k_scale + first)[slot], pv = (v_scale + first)[slot];
-  const bool here = p >= 0 && flag != 0 && held == p;
-  if (live) {
-    // a token that is not held: zeros, as codes and pairs of zero give
-    const V8 yk = dequantize_row8<T, V8>(here ? ck : 0u, here ? pk : 0u);
-    const V8 yv = dequantize_row8<T, V8>(here ? cv : 0u, here ? pv : 0u);
-    const size_t base = (token * HKV + head) * dk;
-    const unsigned to = t * (unsigned)(HKV * dk) + 8 * part;
-    *reinterpret_cast<V8*>(k + base + to) = yk;
-    *reinterpret_cast<V8*>(v + base + to) = yv;
+  // R tokens a lane group, every load of all of them before any is used; a row's codes are loaded with the flag
+  // and position that say whether they count
+  int64_t p[R], held[R];
+  uint8_t flag[R];
+  uint32_t ck[R], cv[R], pk[R], pv[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) p[r] = pos[token + (unsigned)min((int)(t0 + r * TB), left - 1)];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const unsigned slot = p[r] < 0 ? 0u : (unsigned)slot_of(p[r], W);
+    flag[r] = (ring_valid + (size_t)b * W)[slot];
+    held[r] = (ring_pos + (size_t)b * W)[slot];
+    const unsigned piece = slot * (unsigned)(dk / 8) + (live ? part : 0u);
+    ck[r] = (ring_k + first * (dk / 8))[piece];
+    cv[r] = (ring_v + first * (dk / 8))[piece];
+    pk[r] = (k_scale + first)[slot];
+    pv[r] = (v_scale + first)[slot];
   }
-  if (head == 0 && part == 0) found[token + t] = here ? 1 : 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const unsigned t = t0 + r * TB;
+    if ((int)t >= left) break;
+    const bool here = p[r] >= 0 && flag[r] != 0 && held[r] == p[r];
+    if (live) {
+      // a token that is not held: zeros, as codes and pairs of zero give
+      const V8 yk = dequantize_row8<T, V8>(here ? ck[r] : 0u, here ? pk[r] : 0u);
+      const V8 yv = dequantize_row8<T, V8>(here ? cv[r] : 0u, here ? pv[r] : 0u);
+      const size_t base = (token * HKV + head) * dk;
+      const unsigned to = t * (unsigned)(HKV * dk) + 8 * part;
+      *reinterpret_cast<V8*>(k + base + to) = yk;
+      *reinterpret_cast<V8*>(v + base + to) = yv;
+    }
+    if (head == 0 && part == 0) found[token + t] = here ? 1 : 0;
+  }
 }
 
 // ---- attention ----------------------------------------------------------------------------------
@@ -631,7 +647,7 @@ int quant_read(const void* ring_k, const void* ring_v, const void* k_scale, cons
   if (!aligned(k, 16) || !aligned(v, 16)) return fail(ERR_ARG, "%s: k and v must be 16-byte aligned", who);
   if (!aligned(ring_k, 4) || !aligned(ring_v, 4) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
     return fail(ERR_ARG, "%s: the ring's tensors must be 4-byte aligned", who);
-  const int tb = 256 / lanes_of(D), blocks = (int)(((int64_t)N + tb - 1) / tb);
+  const int tb = kReadTokens * (256 / lanes_of(D)), blocks = (int)(((int64_t)N + tb - 1) / tb);
   const int64_t grid = (int64_t)B * blocks * HKV;
   if (grid >= ((int64_t)1 << 31)) return fail(ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
   by_lanes(D, [&](auto lanes) {
