@@ -220,7 +220,7 @@ def on_device(device: torch.device) -> AbstractContextManager[object]:
 
 def call(name: str, *args: object) -> None:
     """Call an entry point and turn a nonzero status into ``KernelLibraryError``."""
-    lib = library()
+    lib = _LIB if _LIB is not None else library()
     if lib.vsp_fault_bits():  # a fault of an earlier call: its results, and what used them, are invalid
         check_faults()
     status = getattr(lib, name)(*args)

@@ -19,6 +19,7 @@
 // all the tokens; its waves share the inputs, each reading whole 128-byte lines of 16 weight rows straight
 // into the MFMA operand's registers; the waves' int32 sums are joined through LDS.
 #include <type_traits>
+#include <cstdlib>
 
 #include "common.h"
 #include "vesper_kernels.h"
@@ -29,8 +30,6 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxBlocks = 4;
-constexpr int kBM = 256;  // tokens a workgroup of the tile kernel
-constexpr int kBN = 256;  // its output columns
 constexpr int kBK = 128;  // inputs a stage
 constexpr int kFewCols = 16;   // output columns a workgroup of the few-token kernel
 constexpr int kFewTokens = 64; // its most tokens
@@ -50,10 +49,14 @@ struct Args {
   int M, d, cols, sig_block;
 };
 
+// An output: the sum times both scales, through the logistic function where asked. That is formed with the
+// exponential and reciprocal instructions (each within a unit of float32): a thread has 64 to 128 outputs, and as
+// calls of the library's functions their code outgrew the instruction cache (32767 tokens of 768: 104 us with
+// it, 90 without a logistic block).
 template <typename T>
 __device__ __forceinline__ T finish(int sum, float scale, bool sig) {
   float y = (float)sum * scale;
-  if (sig) y = 1.f / (1.f + expf(-y));
+  if (sig) y = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * y));
   return from_f32<T>(y);
 }
 
@@ -70,72 +73,105 @@ __device__ __forceinline__ i32x4 load16(__amdgpu_buffer_rsrc_t r, unsigned off) 
   return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
 }
 
+// A resource over `rows` rows of d bytes from `base`, in scalar registers: its parts are the same in every lane, but
+// the compiler, which formed them from a division, would otherwise run a loop over the lanes for each load.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const int8_t* base, int rows, int d) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)p);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32));
+  const int bytes = __builtin_amdgcn_readfirstlane(rows * d);
+  return buffer_rsrc(reinterpret_cast<const int8_t*>((uint64_t)lo | ((uint64_t)hi << 32)), (unsigned)bytes);
+}
+
 constexpr unsigned kOutside = 0x80000000u;  // an offset past every resource's range (under 2 GiB)
 
-template <typename T>
-__global__ __launch_bounds__(512, 1) void project_int8_kernel(const Args a, const Blocks blk, int ctiles, int mtiles) {
-  __shared__ __align__(16) int8_t sZ0[kBM * kBK], sZ1[kBM * kBK];
-  __shared__ __align__(16) int8_t sW0[kBN * kBK], sW1[kBN * kBK];
+// WM x WN waves of 16 TM tokens x 16 TN columns each.
+template <typename T, int WM, int WN, int TM, int TN>
+__global__ __launch_bounds__(64 * WM * WN, 1) void project_int8_kernel(const Args a, const Blocks blk, int ctiles,
+                                                                      int mtiles, int band) {
+  constexpr int NW = WM * WN, BM = 16 * TM * WM, BN = 16 * TN * WN;
+  static_assert(BM == BN && BM % (8 * NW) == 0, "square tiles of whole load instructions");
+  // Two stages of the z rows and the weight rows, [rows][128 inputs] each: row r's 16-byte segment s at s ^
+  // 2 ((r >> 1) & 3), so that a fragment read (lanes 0-7 with 16-23: rows 0-7, two segments each) meets every
+  // bank once. Separate variables: the compiler tells the direct loads into one from the reads of the other.
+  __shared__ __align__(16) int8_t sZ0[BM * kBK], sZ1[BM * kBK];
+  __shared__ __align__(16) int8_t sW0[BN * kBK], sW1[BN * kBK];
 
+  // Workgroups of an XCD take runs of tiles, bands of `band` row tiles each, down a band's rows before the next
+  // column tile: those that run together share rows of z and columns of the weights in the XCD's L2.
   const int lg = xcd_logical_block(blockIdx.x, gridDim.x);
-  const int mt = lg / ctiles, ct = lg - mt * ctiles;
-  if (mt >= mtiles) return;  // the grid is padded to whole XCD rounds; whole workgroups leave
+  const int top = lg / (band * ctiles) * band, in_band = lg - top * ctiles, rows = min(band, mtiles - top);
+  if (rows <= 0) return;  // the grid is padded to whole XCD rounds; whole workgroups leave
+  const int ct = in_band / rows, mt = top + in_band - ct * rows;
+  if (ct >= ctiles) return;
   const int nb = block_of(blk, ct);
-  const int c0 = (ct - blk.start[nb]) * kBN;
+  const int c0 = (ct - blk.start[nb]) * BN;
   const int used = blk.used[nb], d = a.d;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, lq = l & 15, g = l >> 4;
-  const int wm = w & 3, wn = w >> 2;  // the wave's tokens 64 wm .. + 63 and columns 128 wn .. + 127
-  const bool live = c0 + 128 * wn < used;
+  const int wm = w % WM, wn = w / WM;  // the wave's tokens 16 TM wm .. and columns 16 TN wn ..
+  const bool live = c0 + 16 * TN * wn < used;
   const int stages = (d + kBK - 1) / kBK;
 
   // resources of the tile's own rows (under 256 x 16384 bytes): rows past the operands' ends read zeros
-  const int zrows = min(kBM, a.M - mt * kBM), wrows = min(kBN, a.cols - c0);
-  const __amdgpu_buffer_rsrc_t rz = buffer_rsrc(a.z + (size_t)mt * kBM * d, (unsigned)zrows * (unsigned)d);
-  const __amdgpu_buffer_rsrc_t rw = buffer_rsrc(a.wt + ((size_t)nb * a.cols + c0) * d, (unsigned)wrows * (unsigned)d);
+  const int zrows = min(BM, a.M - mt * BM), wrows = min(BN, a.cols - c0);
+  const __amdgpu_buffer_rsrc_t rz = rows_rsrc(a.z + (size_t)mt * BM * d, zrows, d);
+  const __amdgpu_buffer_rsrc_t rw = rows_rsrc(a.wt + ((size_t)nb * a.cols + c0) * d, wrows, d);
   auto kswz = [](int row) { return 2 * ((row >> 1) & 3); };
-  // direct loads: instruction j of wave w fills rows 8 (w + 8 j) .. + 7 of a stage, 128 bytes each; lane l brings
+  // direct loads: instruction j of wave w fills rows 8 (w + NW j) .. + 7 of a stage, 128 bytes each; lane l brings
   // row l / 8's logical segment (l % 8) ^ kswz(row)
+  constexpr int NL = BM / (8 * NW);
   const int lrow = l >> 3, lseg = (l & 7) ^ kswz(lrow);
-  unsigned off[4];  // the scalar offset holds the stage only: it stays below every resource's size
+  unsigned off[NL];  // the scalar offset holds the stage only: it stays below every resource's size
 #pragma unroll
-  for (int j = 0; j < 4; ++j) off[j] = (unsigned)(8 * w + 64 * j + lrow) * (unsigned)d + 16u * (unsigned)lseg;
+  for (int j = 0; j < NL; ++j) off[j] = (unsigned)(8 * (w + NW * j) + lrow) * (unsigned)d + 16u * (unsigned)lseg;
   auto issue = [&](int st, int8_t* dz, int8_t* dw) {
     // inputs past d (d is a multiple of 16, so whole segments) are zeros in z; the weights' are what follows
     const bool in = st * kBK + 16 * lseg < d;
     const unsigned so = (unsigned)(st * kBK);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      buffer_load_lds16(rz, dz + (w + 8 * j) * 1024, in ? off[j] : kOutside, so);
-      buffer_load_lds16(rw, dw + (w + 8 * j) * 1024, off[j], so);
+    for (int j = 0; j < NL; ++j) {
+      buffer_load_lds16(rz, dz + (w + NW * j) * 1024, in ? off[j] : kOutside, so);
+      buffer_load_lds16(rw, dw + (w + NW * j) * 1024, off[j], so);
     }
   };
 
-  i32x4 acc[8][4];
+  i32x4 acc[TN][TM];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < TN; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
+    for (int i = 0; i < TM; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
   auto compute = [&](const int8_t* sz, const int8_t* sw) {
     if (!live) return;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      i32x4 zf[4];
+      i32x4 zf[TM];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 64 * wm + 16 * i + lq;
+      for (int i = 0; i < TM; ++i) {
+        const int row = 16 * (TM * wm + i) + lq;
         zf[i] = *reinterpret_cast<const i32x4*>(sz + row * kBK + 16 * ((4 * s + g) ^ kswz(row)));
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int row = 128 * wn + 16 * j + lq;
+      for (int j = 0; j < TN; ++j) {
+        const int row = 16 * (TN * wn + j) + lq;
         const i32x4 f = *reinterpret_cast<const i32x4*>(sw + row * kBK + 16 * ((4 * s + g) ^ kswz(row)));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, zf[i], acc[j][i], 0, 0, 0);
+        for (int i = 0; i < TM; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, zf[i], acc[j][i], 0, 0, 0);
       }
     }
   };
 
   issue(0, sZ0, sW0);
+  // the scales of the lane's outputs (below), loaded behind the first stage: lane (lq, g) holds columns 16 j + 4 g + r
+  // of token 16 i + lq
+  const int m0 = mt * BM + 16 * TM * wm, cw = c0 + 16 * TN * wn;
+  const float* ws = a.w_scale + (size_t)nb * a.cols;
+  float zs[TM], bs[TN][4];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) zs[i] = a.z_scale[min(m0 + 16 * i + lq, a.M - 1)];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) bs[j][r] = ws[min(cw + 16 * j + 4 * g + r, used - 1)];
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
   for (int st = 0; st < stages; st += 2) {
@@ -152,43 +188,36 @@ __global__ __launch_bounds__(512, 1) void project_int8_kernel(const Args a, cons
   }
   if (!live) return;
 
-  // lane (lq, g) holds columns 16 j + 4 g + r of token 16 i + lq
-  const int m0 = mt * kBM + 64 * wm, cw = c0 + 128 * wn;
-  const float* ws = a.w_scale + (size_t)nb * a.cols;
-  float zs[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) zs[i] = a.z_scale[min(m0 + 16 * i + lq, a.M - 1)];
   T* out = static_cast<T*>(blk.out[nb]);
   if constexpr (sizeof(T) == 2) {
-    // through LDS (free once the last stage's barrier has passed), so that whole rows leave: the wave's
-    // 64 x 128 tile, row r's 16-byte segment s at s ^ (r & 15), then 16 lanes a row, four rows an instruction
+    // through LDS (free once the last stage's barrier has passed), so that whole rows leave: the wave's tile,
+    // row r's 16-byte segment s at s ^ (r % the row's segments), then as whole rows
     typedef T V4 __attribute__((ext_vector_type(4)));
     typedef T V8 __attribute__((ext_vector_type(8)));
-    int8_t* base = (w >> 1) == 0 ? sZ0 : (w >> 1) == 1 ? sZ1 : (w >> 1) == 2 ? sW0 : sW1;
-    T* stile = reinterpret_cast<T*>(base) + (w & 1) * 64 * 128;
+    constexpr int SEG = 2 * TN, TILE = 256 * TM * TN, PER = BM * kBK / (TILE * 2);  // PER waves' tiles a buffer
+    static_assert(PER >= 1 && 4 * PER >= NW, "the waves' tiles fit the stages");
+    int8_t* base = w / PER == 0 ? sZ0 : w / PER == 1 ? sZ1 : w / PER == 2 ? sW0 : sW1;
+    T* stile = reinterpret_cast<T*>(base) + (w % PER) * TILE;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < TN; ++j) {
       const int c = 16 * j + 4 * g;
-      float bs[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) bs[r] = ws[min(cw + c + r, used - 1)];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < TM; ++i) {
         const int row = 16 * i + lq;
         V4 y;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[r], nb == a.sig_block);
-        *reinterpret_cast<V4*>(stile + row * 128 + 8 * ((c >> 3) ^ (row & 15)) + (c & 7)) = y;
+        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[j][r], nb == a.sig_block);
+        *reinterpret_cast<V4*>(stile + row * (16 * TN) + 8 * ((c >> 3) ^ (row & (SEG - 1))) + (c & 7)) = y;
       }
     }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the tile is in LDS (only this wave reads it)
-    const int seg = l & 15, col = cw + 8 * seg;
+    const int seg = l % SEG, col = cw + 8 * seg;
     const bool whole = (used & 7) == 0;
 #pragma unroll
-    for (int it = 0; it < 16; ++it) {
-      const int row = 4 * it + (l >> 4), m = m0 + row;
+    for (int it = 0; it < 16 * TM * SEG / 64; ++it) {
+      const int row = (64 / SEG) * it + l / SEG, m = m0 + row;
       if (m >= a.M || col >= used) continue;
-      const V8 v = *reinterpret_cast<const V8*>(stile + row * 128 + 8 * (seg ^ (row & 15)));
+      const V8 v = *reinterpret_cast<const V8*>(stile + row * (16 * TN) + 8 * (seg ^ (row & (SEG - 1))));
       T* orow = out + (size_t)m * used + col;
       if (whole) {
         *reinterpret_cast<V8*>(orow) = v;
@@ -200,18 +229,15 @@ __global__ __launch_bounds__(512, 1) void project_int8_kernel(const Args a, cons
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < TN; ++j) {
       const int col = cw + 16 * j + 4 * g;
-      float bs[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) bs[r] = ws[min(col + r, used - 1)];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < TM; ++i) {
         const int m = m0 + 16 * i + lq;
         if (m >= a.M) continue;
         float y[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[r], nb == a.sig_block);
+        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[j][r], nb == a.sig_block);
         T* orow = out + (size_t)m * used + col;
         if ((used & 3) == 0 && col < used) {
           *reinterpret_cast<float4*>(orow) = make_float4(y[0], y[1], y[2], y[3]);
@@ -233,9 +259,9 @@ __global__ __launch_bounds__(64 * NW) void project_int8_few_kernel(const Args a,
   const int c0 = ((int)blockIdx.x - blk.start[nb]) * kFewCols;
   const int used = blk.used[nb], d = a.d;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, lq = l & 15, g = l >> 4;
-  const __amdgpu_buffer_rsrc_t rz = buffer_rsrc(a.z, (unsigned)a.M * (unsigned)d);
+  const __amdgpu_buffer_rsrc_t rz = rows_rsrc(a.z, a.M, d);
   const __amdgpu_buffer_rsrc_t rw =
-      buffer_rsrc(a.wt + ((size_t)nb * a.cols + c0) * d, (unsigned)min(kFewCols, a.cols - c0) * (unsigned)d);
+      rows_rsrc(a.wt + ((size_t)nb * a.cols + c0) * d, min(kFewCols, a.cols - c0), d);
   i32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = i32x4{0, 0, 0, 0};
@@ -281,7 +307,9 @@ int project_int8(const int8_t* z, const float* z_scale, const int8_t* wt, const 
   if (M < 0 || cols < 1) return fail(ERR_ARG, "%s: bad sizes M=%d cols=%d", who, M, cols);
   if (sigmoid_block < -1 || sigmoid_block >= nblk) return fail(ERR_ARG, "%s: sigmoid block %d", who, sigmoid_block);
   const bool few = M <= kFewTokens;
-  const int width = few ? kFewCols : kBN;
+  const int cfg = getenv("VSP_CFG") ? atoi(getenv("VSP_CFG")) : 0;
+  const int tile = cfg == 2 ? 128 : 256;
+  const int width = few ? kFewCols : tile;
   Blocks blk{};
   blk.nblk = nblk;
   int64_t tiles = 0;
@@ -301,13 +329,18 @@ int project_int8(const int8_t* z, const float* z_scale, const int8_t* wt, const 
   if (!z || !z_scale || !wt || !w_scale) return fail(ERR_ARG, "%s: null pointer", who);
   if ((reinterpret_cast<uintptr_t>(z) | reinterpret_cast<uintptr_t>(wt)) & 15)
     return fail(ERR_ARG, "%s: z and the weights must be 16-byte aligned", who);
-  const int mtiles = (int)(((int64_t)M + kBM - 1) / kBM);
+  const int mtiles = (int)(((int64_t)M + tile - 1) / tile);
   const int64_t n = few ? tiles : (tiles * mtiles + 7) / 8 * 8;  // whole rounds over the 8 XCDs
   if (n >= ((int64_t)1 << 31)) return fail(ERR_ARG, "%s: too many tiles", who);
   const Args a{z, z_scale, wt, w_scale, M, d, cols, sigmoid_block};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (!few) {
-    hipLaunchKernelGGL(project_int8_kernel<T>, dim3((unsigned)n), dim3(512), 0, s, a, blk, (int)tiles, mtiles);
+    auto run = [&](auto kern, int threads) {
+      hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(threads), 0, s, a, blk, (int)tiles, mtiles,
+                         getenv("VSP_BAND") ? atoi(getenv("VSP_BAND")) : 4);
+    };
+    if (cfg == 0) run(project_int8_kernel<T, 4, 2, 4, 8>, 512);
+    else run(project_int8_kernel<T, 2, 2, 4, 4>, 256);
     return check_launch(who);
   }
   auto go = [&](auto kern, int nw) { hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(64 * nw), 0, s, a, blk); };

@@ -247,11 +247,43 @@ def rms_norm_int8(x: Tensor, gain: Tensor | None = None, *, residual: Tensor | N
     Raises:
         ContractError: on a dtype, width or device outside that contract, or a tensor that needs a gradient.
     """
+    dtype, shape, device = x.dtype, x.shape, x.get_device()
+    rdtype = (torch.bfloat16 if dtype is torch.float32 else dtype) if residual is None else residual.dtype
+    suffix = _NORM_INT8.get((dtype, rdtype))
+    d = shape[-1] if shape else 0
+    # one test on the common path; the checks that name what is wrong run where it fails
+    if not (suffix is not None and device >= 0 and 8 <= d <= 16384 and d & 7 == 0 and not x.requires_grad
+            and (gain is None or (gain.shape == (d,) and gain.dtype is torch.float32 and gain.get_device() == device
+                                  and not gain.requires_grad))
+            and (residual is None or (residual.shape == shape and residual.get_device() == device
+                                      and not residual.requires_grad))):
+        _check_norm_int8(x, gain, residual, rdtype)
+    xc = _aligned(x)
+    gain = None if gain is None else _aligned(gain)
+    residual = None if residual is None else _aligned(residual)
+    if sum_out is not None:
+        if residual is None:
+            raise ContractError("sum_out needs a residual")
+        if (sum_out.shape != shape or sum_out.dtype is not dtype or sum_out.get_device() != device
+                or not sum_out.is_contiguous() or sum_out.data_ptr() % 16):
+            raise ContractError(f"sum_out: contiguous, aligned {dtype} {tuple(shape)} on {x.device}")
+        if x.numel() and sum_out.data_ptr() in (xc.data_ptr(), residual.data_ptr()):
+            raise ContractError("sum_out must not be x or the residual")
+    on = x.device
+    codes = torch.empty(shape, dtype=torch.int8, device=on)
+    scale = torch.empty(shape[:-1], dtype=torch.float32, device=on)
+    with _lib.on_device(on):
+        _lib.call(f"vsp_rms_norm_int8_{suffix}", xc.data_ptr(), _lib.ptr(residual), _lib.ptr(sum_out), _lib.ptr(gain),
+                  codes.data_ptr(), scale.data_ptr(), xc.numel() // d, d, _lib.stream_of(on))
+    return codes, scale
+
+
+def _check_norm_int8(x: Tensor, gain: Tensor | None, residual: Tensor | None, rdtype: torch.dtype) -> None:
+    """Raises for what ``rms_norm_int8`` does not take."""
     if x.device.type != "cuda":
         raise ContractError(f"the norm kernel runs on CUDA only, x is on {x.device}")
     if x.dim() < 1:
         raise ContractError("x: needs at least one axis")
-    rdtype = (torch.bfloat16 if x.dtype == torch.float32 else x.dtype) if residual is None else residual.dtype
     if (x.dtype, rdtype) not in _NORM_INT8:
         raise ContractError(f"x: dtype must be float32 (residual bfloat16 or float16), bfloat16 or float16 (residual the same), "
                             f"got {x.dtype} and {rdtype}")
@@ -259,30 +291,10 @@ def rms_norm_int8(x: Tensor, gain: Tensor | None = None, *, residual: Tensor | N
     if d < 8 or d > 16384 or d % 8:
         raise ContractError(f"x: last axis {d} is not a multiple of 8 in 8..16384")
     _refuse_grad("rms_norm_int8", x, gain, residual)
-    if gain is not None:
-        if gain.shape != (d,) or gain.dtype != torch.float32 or gain.device != x.device:
-            raise ContractError(f"gain: must be float32 [{d}] on {x.device}, got {tuple(gain.shape)} {gain.dtype}")
-        gain = _aligned(gain)
-    if residual is not None:
-        if residual.shape != x.shape or residual.device != x.device:
-            raise ContractError(f"residual: {tuple(x.shape)} on {x.device}, got {tuple(residual.shape)} on {residual.device}")
-        residual = _aligned(residual)
-    xc = _aligned(x)
-    if sum_out is not None:
-        if residual is None:
-            raise ContractError("sum_out needs a residual")
-        if (sum_out.shape != x.shape or sum_out.dtype != x.dtype or sum_out.device != x.device
-                or not sum_out.is_contiguous() or sum_out.data_ptr() % 16):
-            raise ContractError(f"sum_out: contiguous, aligned {x.dtype} {tuple(x.shape)} on {x.device}")
-        if x.numel() and sum_out.data_ptr() in (xc.data_ptr(), residual.data_ptr()):
-            raise ContractError("sum_out must not be x or the residual")
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    with _lib.on_device(x.device):
-        _lib.call(f"vsp_rms_norm_int8_{_NORM_INT8[x.dtype, rdtype]}", xc.data_ptr(), _lib.ptr(residual),
-                  _lib.ptr(sum_out), _lib.ptr(gain), codes.data_ptr(), scale.data_ptr(), xc.numel() // d, d,
-                  _lib.stream_of(x.device))
-    return codes, scale
+    if gain is not None and (gain.shape != (d,) or gain.dtype != torch.float32 or gain.device != x.device):
+        raise ContractError(f"gain: must be float32 [{d}] on {x.device}, got {tuple(gain.shape)} {gain.dtype}")
+    if residual is not None and (residual.shape != x.shape or residual.device != x.device):
+        raise ContractError(f"residual: {tuple(x.shape)} on {x.device}, got {tuple(residual.shape)} on {residual.device}")
 
 
 def quantize_weights(weights_t: Tensor) -> tuple[Tensor, Tensor]:
@@ -327,6 +339,32 @@ def projection_int8(z: Tensor, z_scale: Tensor, weights_q: Tensor, weights_scale
     Raises:
         ContractError: on shapes, dtypes or devices outside that contract, or a tensor that needs a gradient.
     """
+    p = len(used)
+    zshape, wshape, device, suffix = z.shape, weights_q.shape, z.get_device(), _INT8_SUFFIX.get(dtype)
+    # one test on the common path; the checks that name what is wrong run where it fails
+    if not (len(zshape) == 2 and len(wshape) == 3 and z.dtype is torch.int8 and weights_q.dtype is torch.int8
+            and wshape[2] == zshape[1] and wshape[0] == p and 1 <= p <= 4 and z_scale.shape == zshape[:1]
+            and weights_scale.shape == wshape[:2] and z_scale.dtype is torch.float32
+            and weights_scale.dtype is torch.float32 and device >= 0 and z_scale.get_device() == device
+            and weights_q.get_device() == device and weights_scale.get_device() == device
+            and min(used) >= 1 and max(used) <= wshape[1] and zshape[1] & 15 == 0 and 16 <= zshape[1] <= 16384
+            and suffix is not None and (sigmoid_block is None or 0 <= sigmoid_block < p)
+            and not (z_scale.requires_grad or weights_scale.requires_grad)):
+        _check_projection_int8(z, z_scale, weights_q, weights_scale, used, sigmoid_block, dtype)
+    m, d = zshape
+    zc, wc, zs, ws, on = _aligned(z), _aligned(weights_q), z_scale.contiguous(), weights_scale.contiguous(), z.device
+    outs = [torch.empty((m, u), dtype=dtype, device=on) for u in used]
+    ptrs = [o.data_ptr() for o in outs] + [0] * (4 - p)
+    widths = [*used] + [1] * (4 - p)
+    with _lib.on_device(on):
+        _lib.call(f"vsp_project_int8_{suffix}", zc.data_ptr(), zs.data_ptr(), wc.data_ptr(), ws.data_ptr(), p, wshape[1], d,
+                  m, *widths, *ptrs, -1 if sigmoid_block is None else sigmoid_block, _lib.stream_of(on))
+    return outs
+
+
+def _check_projection_int8(z: Tensor, z_scale: Tensor, weights_q: Tensor, weights_scale: Tensor, used: tuple[int, ...],
+                           sigmoid_block: int | None, dtype: torch.dtype) -> None:
+    """Raises for what ``projection_int8`` does not take."""
     if z.dim() != 2 or z.dtype != torch.int8 or z.device.type != "cuda":
         raise ContractError(f"z: int8 [M, d] on CUDA, got {tuple(z.shape)} {z.dtype} on {z.device}")
     m, d = z.shape
@@ -348,12 +386,3 @@ def projection_int8(z: Tensor, z_scale: Tensor, weights_q: Tensor, weights_scale
     if dtype not in _INT8_SUFFIX:
         raise ContractError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
     _refuse_grad("projection_int8", z_scale, weights_scale)
-    zc, wc, zs, ws = _aligned(z), _aligned(weights_q), z_scale.contiguous(), weights_scale.contiguous()
-    outs = [torch.empty(m, u, dtype=dtype, device=z.device) for u in used]
-    ptrs = [o.data_ptr() for o in outs] + [0] * (4 - p)
-    widths = list(used) + [1] * (4 - p)
-    with _lib.on_device(z.device):
-        _lib.call(f"vsp_project_int8_{_INT8_SUFFIX[dtype]}", zc.data_ptr(), zs.data_ptr(), wc.data_ptr(), ws.data_ptr(),
-                  p, cols, d, m, *widths, *ptrs, -1 if sigmoid_block is None else sigmoid_block,
-                  _lib.stream_of(z.device))
-    return outs

@@ -22,6 +22,7 @@ All are forward only.
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 
@@ -118,6 +119,28 @@ def _check_devices(cache: QuantRingKVCache, first: str, device: torch.device, *n
             raise ContractError(f"{name} is on {t.device}, {first} on {device}")
 
 
+def _ring_as_is(cache: QuantRingKVCache, b: int, hkv: int, dk: int, dtype: torch.dtype, device: int) -> bool:
+    """Whether every tensor of the ring is what the kernels take as it is: one test on the common path in place of
+    the checks that name what is wrong (a decode step's call spends more on those than its kernel runs)."""
+    w, k, v, ks, vs, pos, valid = cache.window, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.pos, cache.valid
+    codes, pairs, slots = (b, hkv, w, dk >> 1), (b, hkv, w, 2), (b, w)
+    return (k.shape == codes and v.shape == codes and ks.shape == pairs and vs.shape == pairs
+            and pos.shape == slots and valid.shape == slots
+            and k.dtype is torch.uint8 and v.dtype is torch.uint8 and ks.dtype is dtype and vs.dtype is dtype
+            and pos.dtype is torch.int64 and valid.dtype is torch.bool
+            and k.get_device() == device and v.get_device() == device and ks.get_device() == device
+            and vs.get_device() == device and pos.get_device() == device and valid.get_device() == device
+            and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
+            and pos.is_contiguous() and valid.is_contiguous()
+            and (k.data_ptr() | v.data_ptr() | ks.data_ptr() | vs.data_ptr()) & 3 == 0
+            and w >= 1 and dk & 7 == 0 and 8 <= dk <= MAX_HEAD_DIM and 1 <= hkv <= MAX_KV_HEADS)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(b: int, h: int, hkv: int, dk: int, w: int) -> int:
+    return int(_lib.library().vsp_quant_ring_attn_workspace_bytes(b, h, hkv, dk, w))
+
+
 def _writable(cache: QuantRingKVCache, inplace: bool) -> QuantRingKVCache:
     """The ring that a kernel writes: the cache's own tensors, or a contiguous copy."""
     if not inplace:
@@ -156,18 +179,23 @@ def quant_ring_write(k: Tensor, v: Tensor, pos: Tensor, cache: QuantRingKVCache,
     Raises:
         ContractError: on shapes, dtypes, devices or values outside that contract.
     """
-    dims: Dims = {}
-    check_shape("k", k, ("b", "n", "hkv", "dk"), dims)
-    check_shape("v", v, ("b", "n", "hkv", "dk"), dims, k.dtype)
-    check_shape("pos", pos, ("b", "n"), dims, torch.long)
-    dtype = _check_ring(cache, dims)
-    if k.dtype != dtype:
-        raise ContractError(f"k: dtype must be the ring's {dtype}, got {k.dtype}")
-    _check_devices(cache, "k", k.device, ("v", v), ("pos", pos))
-    _refuse_grad(k, v)
-    b, n, w = dims["b"], dims["n"], cache.window
+    shape, dtype, device, w = k.shape, k.dtype, k.get_device(), cache.window
+    as_is = (len(shape) == 4 and v.shape == shape and pos.shape == shape[:2] and v.dtype is dtype
+             and pos.dtype is torch.int64 and dtype in _SUFFIX and device >= 0 and v.get_device() == device
+             and pos.get_device() == device and not (k.requires_grad or v.requires_grad)
+             and _ring_as_is(cache, shape[0], shape[2], shape[3], dtype, device))
+    if not as_is:
+        dims: Dims = {}
+        check_shape("k", k, ("b", "n", "hkv", "dk"), dims)
+        check_shape("v", v, ("b", "n", "hkv", "dk"), dims, k.dtype)
+        check_shape("pos", pos, ("b", "n"), dims, torch.long)
+        if _check_ring(cache, dims) != dtype:
+            raise ContractError(f"k: dtype must be the ring's {cache.k_scale.dtype}, got {dtype}")
+        _check_devices(cache, "k", k.device, ("v", v), ("pos", pos))
+        _refuse_grad(k, v)
+    b, n, hkv, dk = shape
     if lengths is not None:
-        check_shape("lengths", lengths, ("b",), dims)
+        check_shape("lengths", lengths, (b,), {})
         if lengths.dtype not in (torch.int32, torch.long):
             raise ContractError(f"lengths: dtype must be int32 or int64, got {lengths.dtype}")
         if lengths.device != k.device:
@@ -180,16 +208,17 @@ def quant_ring_write(k: Tensor, v: Tensor, pos: Tensor, cache: QuantRingKVCache,
             first = (first | (lengths == 0)) & (lengths >= 0) & (lengths <= n)
         require((ok.all() & first.all()).reshape(1),
                 "quant_ring_write: positions must be nonnegative and consecutive, lengths in 0..n")
-    ring = _writable(cache, inplace)
+    ring = cache if inplace and as_is else _writable(cache, inplace)
     if b == 0 or n == 0:
         return ring
     if lengths is not None:
         lengths = lengths.long().contiguous()
-    k, v, pos = _aligned(k), _aligned(v), pos.contiguous()
-    with _lib.on_device(k.device):
+    k, v, pos, on = _aligned(k), _aligned(v), pos.contiguous(), k.device
+    with _lib.on_device(on):
         _lib.call(f"vsp_quant_ring_write_{_SUFFIX[dtype]}", k.data_ptr(), v.data_ptr(), pos.data_ptr(),
-                  _lib.ptr(lengths), *(t.data_ptr() for t in ring.tensors()), b, n, dims["hkv"], dims["dk"], w,
-                  _lib.stream_of(k.device))
+                  _lib.ptr(lengths), ring.k.data_ptr(), ring.v.data_ptr(), ring.k_scale.data_ptr(),
+                  ring.v_scale.data_ptr(), ring.pos.data_ptr(), ring.valid.data_ptr(), b, n, hkv, dk, w,
+                  _lib.stream_of(on))
     return ring
 
 
@@ -207,22 +236,28 @@ def quant_ring_read(cache: QuantRingKVCache, pos: Tensor) -> tuple[Tensor, Tenso
     Raises:
         ContractError: on shapes, dtypes or devices outside that contract.
     """
-    dims: Dims = {}
-    check_shape("pos", pos, ("b", "n"), dims, torch.long)
-    dtype = _check_ring(cache, dims)
-    _check_devices(cache, "pos", pos.device)
-    b, n, hkv, dk = dims["b"], dims["n"], dims["hkv"], dims["dk"]
-    k = torch.empty(b, n, hkv, dk, dtype=dtype, device=pos.device)
+    dtype, shape, device = cache.k_scale.dtype, cache.k.shape, pos.get_device()
+    held = cache
+    if not (len(shape) == 4 and pos.dim() == 2 and pos.shape[0] == shape[0] and pos.dtype is torch.int64 and dtype in _SUFFIX
+            and device >= 0 and _ring_as_is(cache, shape[0], shape[1], 2 * shape[3], dtype, device)):
+        dims: Dims = {}
+        check_shape("pos", pos, ("b", "n"), dims, torch.long)
+        _check_ring(cache, dims)
+        _check_devices(cache, "pos", pos.device)
+        parts = [t.contiguous() for t in cache.tensors()]
+        held = QuantRingKVCache(*(t if t.data_ptr() % 4 == 0 or t.dtype == torch.bool else t.clone() for t in parts),
+                                cache.window)
+    (b, n), hkv, dk, on = pos.shape, shape[1], 2 * shape[3], pos.device
+    k = torch.empty((b, n, hkv, dk), dtype=dtype, device=on)
     v = torch.empty_like(k)
-    found = torch.empty(b, n, dtype=torch.bool, device=pos.device)
+    found = torch.empty((b, n), dtype=torch.bool, device=on)
     if b == 0 or n == 0:
         return k, v, found
     pos = pos.contiguous()
-    held = [t.contiguous() for t in cache.tensors()]
-    held = [t if t.data_ptr() % 4 == 0 or t.dtype == torch.bool else t.clone() for t in held]
-    with _lib.on_device(pos.device):
-        _lib.call(f"vsp_quant_ring_read_{_SUFFIX[dtype]}", *(t.data_ptr() for t in held), pos.data_ptr(), k.data_ptr(),
-                  v.data_ptr(), found.data_ptr(), b, n, hkv, dk, cache.window, _lib.stream_of(pos.device))
+    with _lib.on_device(on):
+        _lib.call(f"vsp_quant_ring_read_{_SUFFIX[dtype]}", held.k.data_ptr(), held.v.data_ptr(), held.k_scale.data_ptr(),
+                  held.v_scale.data_ptr(), held.pos.data_ptr(), held.valid.data_ptr(), pos.data_ptr(), k.data_ptr(),
+                  v.data_ptr(), found.data_ptr(), b, n, hkv, dk, cache.window, _lib.stream_of(on))
     return k, v, found
 
 
@@ -253,36 +288,44 @@ def quant_ring_attention(q: Tensor, k: Tensor, v: Tensor, pos: Tensor, cache: Qu
     Raises:
         ContractError: on shapes, dtypes, devices or values outside that contract.
     """
-    dims: Dims = {"one": 1}
-    check_shape("q", q, ("b", "one", "h", "dk"), dims)
-    check_shape("k", k, ("b", "one", "hkv", "dk"), dims, q.dtype)
-    check_shape("v", v, ("b", "one", "hkv", "dk"), dims, q.dtype)
-    check_shape("pos", pos, ("b", "one"), dims, torch.long)
-    dtype = _check_ring(cache, dims)
-    if q.dtype != dtype:
-        raise ContractError(f"q: dtype must be the ring's {dtype}, got {q.dtype}")
-    _check_devices(cache, "q", q.device, ("k", k), ("v", v), ("pos", pos))
-    b, h, hkv, dk, w = dims["b"], dims["h"], dims["hkv"], dims["dk"], cache.window
+    shape, new, dtype, device, w = q.shape, k.shape, q.dtype, q.get_device(), cache.window
+    as_is = (len(shape) == 4 and len(new) == 4 and shape[1] == 1 and new[1] == 1 and new[0] == shape[0]
+             and new[3] == shape[3] and v.shape == new and pos.shape == shape[:2] and k.dtype is dtype
+             and v.dtype is dtype and pos.dtype is torch.int64 and dtype in _SUFFIX and device >= 0
+             and k.get_device() == device and v.get_device() == device and pos.get_device() == device
+             and not (q.requires_grad or k.requires_grad or v.requires_grad)
+             and _ring_as_is(cache, shape[0], new[2], shape[3], dtype, device))
+    if not as_is:
+        dims: Dims = {"one": 1}
+        check_shape("q", q, ("b", "one", "h", "dk"), dims)
+        check_shape("k", k, ("b", "one", "hkv", "dk"), dims, dtype)
+        check_shape("v", v, ("b", "one", "hkv", "dk"), dims, dtype)
+        check_shape("pos", pos, ("b", "one"), dims, torch.long)
+        if _check_ring(cache, dims) != dtype:
+            raise ContractError(f"q: dtype must be the ring's {cache.k_scale.dtype}, got {dtype}")
+        _check_devices(cache, "q", q.device, ("k", k), ("v", v), ("pos", pos))
+        _refuse_grad(q, k, v)
+    b, h, hkv, dk = shape[0], shape[2], new[2], shape[3]
     if hkv < 1 or h < 1 or h % hkv != 0 or h // hkv > MAX_GROUP:
         raise ContractError(f"{h} query heads over {hkv} KV heads: need a multiple, at most {MAX_GROUP} per KV head")
-    _refuse_grad(q, k, v)
     if check_positions and b > 0:
         require((pos >= 0).all().reshape(1), "quant_ring_attention: positions must be nonnegative")
     mask = None
     if active is not None:
-        check_shape("active", active, ("b",), dims, torch.bool)
+        check_shape("active", active, (b,), {}, torch.bool)
         if active.device != q.device:
             raise ContractError(f"active is on {active.device}, q on {q.device}")
         mask = active.contiguous()
-    ring = _writable(cache, inplace)
-    q, k, v, pos = _aligned(q), _aligned(k), _aligned(v), pos.contiguous()
+    ring = cache if inplace and as_is else _writable(cache, inplace)
+    q, k, v, pos, on = _aligned(q), _aligned(k), _aligned(v), pos.contiguous(), q.device
     o = torch.empty_like(q)
     if b == 0:
         return o, ring
-    nbytes = _lib.library().vsp_quant_ring_attn_workspace_bytes(b, h, hkv, dk, w)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    with _lib.on_device(q.device):
+    nbytes = _workspace_bytes(b, h, hkv, dk, w)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=on) if nbytes else None
+    with _lib.on_device(on):
         _lib.call(f"vsp_quant_ring_attn_{_SUFFIX[dtype]}", q.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(),
-                  *(t.data_ptr() for t in ring.tensors()), o.data_ptr(), _lib.ptr(mask), _lib.ptr(workspace), nbytes,
-                  b, h, hkv, dk, w, 1.0 / math.sqrt(dk), 1, _lib.stream_of(q.device))
+                  ring.k.data_ptr(), ring.v.data_ptr(), ring.k_scale.data_ptr(), ring.v_scale.data_ptr(),
+                  ring.pos.data_ptr(), ring.valid.data_ptr(), o.data_ptr(), _lib.ptr(mask), _lib.ptr(workspace), nbytes,
+                  b, h, hkv, dk, w, 1.0 / math.sqrt(dk), 1, _lib.stream_of(on))
     return o, ring
