@@ -11,15 +11,21 @@
 //
 // Two kernels, by the number of tokens:
 //
-// tile (many tokens): 256 tokens x 256 columns a workgroup, eight waves of 64 x 128, both operands through
-// LDS in double-buffered stages of 128 inputs (the 128-byte rows of the bf16 projection's stages, its
-// XOR swizzle and its block order), 16x16x64 int8 MFMA formed transposed (weight rows as the A operand).
+// tile (many tokens): 256 tokens x 256 columns a workgroup of eight waves of 64 x 128, both operands through LDS in
+// two stages of 128 inputs (whole cache lines a row), or, where that makes few workgroups, 128 x 128 in waves of
+// 64 x 32 and three stages. global_load_lds_dwordx4 moves eight rows of 128 bytes an instruction, each row's
+// 16-byte segments XOR-swizzled so that the fragment reads meet each bank once; 16x16x64 int8 MFMA formed
+// transposed (weight rows as the A operand); the second half's fragments are read during the first half's products.
+// 8192^3: 480 us (2.3 Pop/s; the chip's products clock down under them: the matrix units are busy 58 % of the
+// cycles), a library product of the same operands 547. 32767 x 768 to 2316 columns: 94 us, of which the loads into
+// LDS take 36 alone (503 MB, 14 TB/s), the products 25 and the outputs 29, with one workgroup a CU nearly one after
+// the other; 128 x 128 tiles, two workgroups a CU, need 57, 15 and 22: 98 us. Stages of 64 inputs, four deep, read
+// half cache lines: 117 us. Three stages of 256 x 128: 108 us.
 //
 // few (up to 64 tokens, a decode step): bound by reading the weights once. A workgroup takes 16 columns and
 // all the tokens; its waves share the inputs, each reading whole 128-byte lines of 16 weight rows straight
 // into the MFMA operand's registers; the waves' int32 sums are joined through LDS.
 #include <type_traits>
-#include <cstdlib>
 
 #include "common.h"
 #include "vesper_kernels.h"
@@ -31,6 +37,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxBlocks = 4;
 constexpr int kBK = 128;  // inputs a stage
+constexpr int kBand = 4;       // row tiles of a band (an XCD's workgroups go down its rows before the next column)
 constexpr int kFewCols = 16;   // output columns a workgroup of the few-token kernel
 constexpr int kFewTokens = 64; // its most tokens
 
@@ -85,17 +92,34 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const int8_t* base, 
 
 constexpr unsigned kOutside = 0x80000000u;  // an offset past every resource's range (under 2 GiB)
 
-// WM x WN waves of 16 TM tokens x 16 TN columns each.
-template <typename T, int WM, int WN, int TM, int TN>
+// The wave's loads but the N newest have arrived in LDS, its LDS reads have returned, and every wave is here.
+template <int N>
+__device__ __forceinline__ void arrive() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  // the wait as the builtin, which the compiler's own count of loads takes note of (behind inline assembly it would
+  // wait again, for all but the newest loads, before the first read of a stage)
+  static_assert(N < 64, "vmcnt has six bits");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | ((N >> 4) << 14));  // vmcnt(N), lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#endif
+}
+
+// WM x WN waves of 16 TM tokens x 16 TN columns each, S stages in LDS.
+template <typename T, int WM, int WN, int TM, int TN, int S>
 __global__ __launch_bounds__(64 * WM * WN, 1) void project_int8_kernel(const Args a, const Blocks blk, int ctiles,
                                                                       int mtiles, int band) {
+  constexpr int AHEAD = TN < 4 ? TN : 4;  // weight fragments read ahead of the products
   constexpr int NW = WM * WN, BM = 16 * TM * WM, BN = 16 * TN * WN;
   static_assert(BM == BN && BM % (8 * NW) == 0, "square tiles of whole load instructions");
-  // Two stages of the z rows and the weight rows, [rows][128 inputs] each: row r's 16-byte segment s at s ^
+  static_assert(S == 2 || S == 3, "two or three stages");
+  // Stages of the z rows and the weight rows, [rows][128 inputs] each: row r's 16-byte segment s at s ^
   // 2 ((r >> 1) & 3), so that a fragment read (lanes 0-7 with 16-23: rows 0-7, two segments each) meets every
-  // bank once. Separate variables: the compiler tells the direct loads into one from the reads of the other.
-  __shared__ __align__(16) int8_t sZ0[BM * kBK], sZ1[BM * kBK];
-  __shared__ __align__(16) int8_t sW0[BN * kBK], sW1[BN * kBK];
+  // bank once. Separate variables: the compiler tells the direct loads into one from the reads of the others.
+  __shared__ __align__(16) int8_t sZ0[BM * kBK], sZ1[BM * kBK], sZ2[S == 3 ? BM * kBK : 16];
+  __shared__ __align__(16) int8_t sW0[BN * kBK], sW1[BN * kBK], sW2[S == 3 ? BN * kBK : 16];
+  __shared__ __align__(16) float sScaleZ[BM], sScaleW[BN];
 
   // Workgroups of an XCD take runs of tiles, bands of `band` row tiles each, down a band's rows before the next
   // column tile: those that run together share rows of z and columns of the weights in the XCD's L2.
@@ -125,14 +149,13 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void project_int8_kernel(const Arg
 #pragma unroll
   for (int j = 0; j < NL; ++j) off[j] = (unsigned)(8 * (w + NW * j) + lrow) * (unsigned)d + 16u * (unsigned)lseg;
   auto issue = [&](int st, int8_t* dz, int8_t* dw) {
-    // inputs past d (d is a multiple of 16, so whole segments) are zeros in z; the weights' are what follows
+    // inputs past d (d is a multiple of 16, so whole segments), and whole stages past the last, are zeros
     const bool in = st * kBK + 16 * lseg < d;
-    const unsigned so = (unsigned)(st * kBK);
+    const unsigned so = (unsigned)(min(st, stages - 1) * kBK);
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      buffer_load_lds16(rz, dz + (w + NW * j) * 1024, in ? off[j] : kOutside, so);
-      buffer_load_lds16(rw, dw + (w + NW * j) * 1024, off[j], so);
-    }
+    for (int j = 0; j < NL; ++j) buffer_load_lds16(rz, dz + (w + NW * j) * 1024, in ? off[j] : kOutside, so);
+#pragma unroll
+    for (int j = 0; j < NL; ++j) buffer_load_lds16(rw, dw + (w + NW * j) * 1024, in ? off[j] : kOutside, so);
   };
 
   i32x4 acc[TN][TM];
@@ -140,8 +163,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void project_int8_kernel(const Arg
   for (int j = 0; j < TN; ++j)
 #pragma unroll
     for (int i = 0; i < TM; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
-  auto compute = [&](const int8_t* sz, const int8_t* sw) {
-    if (!live) return;
+  // A stage: the loads of the one S - 1 ahead, into the buffers that were read a stage ago (every wave has passed the
+  // barrier behind those reads); the products; then the next stage has to have arrived. Every stage issues the same
+  // number of loads (zeros past the last), so that the count of those still out, S - 2 stages', is the same too.
+  auto step = [&](const int8_t* sz, const int8_t* sw, int st, int8_t* dz, int8_t* dw) {
+    issue(st, dz, dw);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       i32x4 zf[TM];
@@ -158,55 +184,65 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void project_int8_kernel(const Arg
         for (int i = 0; i < TM; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, zf[i], acc[j][i], 0, 0, 0);
       }
     }
+    // the fragments of the second half are read while the first half's products run
+    constexpr int EACH = (TM + 2 * TN - AHEAD + TN - 1) / TN;
+    __builtin_amdgcn_sched_group_barrier(0x10, 2 * NL, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, TM + AHEAD, 0);
+#pragma unroll
+    for (int u = 0; u < 2 * TN; ++u) {
+      __builtin_amdgcn_sched_group_barrier(0x8, TM, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // the wait stays behind the products
+    arrive<2 * NL * (S - 2)>();
   };
 
   issue(0, sZ0, sW0);
-  // the scales of the lane's outputs (below), loaded behind the first stage: lane (lq, g) holds columns 16 j + 4 g + r
-  // of token 16 i + lq
-  const int m0 = mt * BM + 16 * TM * wm, cw = c0 + 16 * TN * wn;
-  const float* ws = a.w_scale + (size_t)nb * a.cols;
-  float zs[TM], bs[TN][4];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) zs[i] = a.z_scale[min(m0 + 16 * i + lq, a.M - 1)];
-#pragma unroll
-  for (int j = 0; j < TN; ++j)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) bs[j][r] = ws[min(cw + 16 * j + 4 * g + r, used - 1)];
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  __syncthreads();
-  for (int st = 0; st < stages; st += 2) {
-    if (st + 1 < stages) issue(st + 1, sZ1, sW1);
-    compute(sZ0, sW0);
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    __syncthreads();
-    if (st + 1 < stages) {
-      if (st + 2 < stages) issue(st + 2, sZ0, sW0);
-      compute(sZ1, sW1);
-      __builtin_amdgcn_s_waitcnt(0x0F70);
-      __syncthreads();
+  // the scales of the tile's tokens and columns, behind the first stage
+  for (int i = threadIdx.x; i < BM; i += 64 * NW) sScaleZ[i] = a.z_scale[min(mt * BM + i, a.M - 1)];
+  for (int i = threadIdx.x; i < BN; i += 64 * NW) sScaleW[i] = a.w_scale[(size_t)nb * a.cols + min(c0 + i, used - 1)];
+  if constexpr (S == 3) issue(1, sZ1, sW1);
+  arrive<2 * NL * (S - 2)>();
+  if constexpr (S == 2) {
+    for (int st = 0; st < stages; st += 2) {
+      step(sZ0, sW0, st + 1, sZ1, sW1);
+      if (st + 1 < stages) step(sZ1, sW1, st + 2, sZ0, sW0);
+    }
+  } else {
+    for (int st = 0; st < stages; st += 3) {
+      step(sZ0, sW0, st + 2, sZ2, sW2);
+      if (st + 1 < stages) step(sZ1, sW1, st + 3, sZ0, sW0);
+      if (st + 2 < stages) step(sZ2, sW2, st + 4, sZ1, sW1);
     }
   }
+  arrive<0>();  // the last loads (zeros) have landed before the buffers are used again
   if (!live) return;
 
+  // lane (lq, g) holds columns 16 j + 4 g + r of token 16 i + lq
+  const int m0 = mt * BM + 16 * TM * wm, cw = c0 + 16 * TN * wn;
   T* out = static_cast<T*>(blk.out[nb]);
+  float zs[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) zs[i] = sScaleZ[16 * (TM * wm + i) + lq];
   if constexpr (sizeof(T) == 2) {
-    // through LDS (free once the last stage's barrier has passed), so that whole rows leave: the wave's tile,
-    // row r's 16-byte segment s at s ^ (r % the row's segments), then as whole rows
+    // through LDS (free behind the last barrier), so that whole rows leave: the wave's tile, row r's 16-byte segment
+    // s at s ^ (r % the row's segments), then as whole rows
     typedef T V4 __attribute__((ext_vector_type(4)));
     typedef T V8 __attribute__((ext_vector_type(8)));
     constexpr int SEG = 2 * TN, TILE = 256 * TM * TN, PER = BM * kBK / (TILE * 2);  // PER waves' tiles a buffer
-    static_assert(PER >= 1 && 4 * PER >= NW, "the waves' tiles fit the stages");
+    static_assert(PER >= 1 && 4 * PER >= NW, "the waves' tiles fit two stages");
     int8_t* base = w / PER == 0 ? sZ0 : w / PER == 1 ? sZ1 : w / PER == 2 ? sW0 : sW1;
     T* stile = reinterpret_cast<T*>(base) + (w % PER) * TILE;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int c = 16 * j + 4 * g;
+      const f32x4 bs = *reinterpret_cast<const f32x4*>(sScaleW + 16 * TN * wn + c);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int row = 16 * i + lq;
         V4 y;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[j][r], nb == a.sig_block);
+        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[r], nb == a.sig_block);
         *reinterpret_cast<V4*>(stile + row * (16 * TN) + 8 * ((c >> 3) ^ (row & (SEG - 1))) + (c & 7)) = y;
       }
     }
@@ -231,13 +267,14 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void project_int8_kernel(const Arg
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int col = cw + 16 * j + 4 * g;
+      const f32x4 bs = *reinterpret_cast<const f32x4*>(sScaleW + 16 * TN * wn + 16 * j + 4 * g);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int m = m0 + 16 * i + lq;
         if (m >= a.M) continue;
         float y[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[j][r], nb == a.sig_block);
+        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[r], nb == a.sig_block);
         T* orow = out + (size_t)m * used + col;
         if ((used & 3) == 0 && col < used) {
           *reinterpret_cast<float4*>(orow) = make_float4(y[0], y[1], y[2], y[3]);
@@ -306,9 +343,11 @@ int project_int8(const int8_t* z, const float* z_scale, const int8_t* wt, const 
     return fail(ERR_ARG, "%s: width %d (a multiple of 16 in 16..16384)", who, d);
   if (M < 0 || cols < 1) return fail(ERR_ARG, "%s: bad sizes M=%d cols=%d", who, M, cols);
   if (sigmoid_block < -1 || sigmoid_block >= nblk) return fail(ERR_ARG, "%s: sigmoid block %d", who, sigmoid_block);
+  // the wide tile where the small one's workgroups would go around the 256 CUs more than twice
   const bool few = M <= kFewTokens;
-  const int cfg = getenv("VSP_CFG") ? atoi(getenv("VSP_CFG")) : 0;
-  const int tile = cfg == 2 ? 128 : 256;
+  int64_t small = 0;
+  for (int j = 0; j < nblk; ++j) small += ((int64_t)(used_in[j] > 0 ? used_in[j] : 0) + 127) / 128;
+  const int tile = small * (((int64_t)M + 127) / 128) > 512 ? 256 : 128;
   const int width = few ? kFewCols : tile;
   Blocks blk{};
   blk.nblk = nblk;
@@ -335,12 +374,11 @@ int project_int8(const int8_t* z, const float* z_scale, const int8_t* wt, const 
   const Args a{z, z_scale, wt, w_scale, M, d, cols, sigmoid_block};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (!few) {
-    auto run = [&](auto kern, int threads) {
-      hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(threads), 0, s, a, blk, (int)tiles, mtiles,
-                         getenv("VSP_BAND") ? atoi(getenv("VSP_BAND")) : 4);
+    auto run = [&](auto kern) {
+      hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(512), 0, s, a, blk, (int)tiles, mtiles, kBand);
     };
-    if (cfg == 0) run(project_int8_kernel<T, 4, 2, 4, 8>, 512);
-    else run(project_int8_kernel<T, 2, 2, 4, 4>, 256);
+    if (tile == 256) run(project_int8_kernel<T, 4, 2, 4, 8, 2>);
+    else run(project_int8_kernel<T, 2, 4, 4, 2, 3>);
     return check_launch(who);
   }
   auto go = [&](auto kern, int nw) { hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(64 * nw), 0, s, a, blk); };
