@@ -24,7 +24,11 @@
 //
 // few (up to 64 tokens, a decode step): bound by reading the weights once. A workgroup takes 16 columns and
 // all the tokens; its waves share the inputs, each reading whole 128-byte lines of 16 weight rows straight
-// into the MFMA operand's registers; the waves' int32 sums are joined through LDS.
+// into the MFMA operand's registers; the waves' int32 sums are joined through LDS. Past 16 tokens the tokens'
+// own reads count (from L2, by every workgroup): 32 columns a workgroup where there are enough (64 tokens, 8192 to
+// 8192: 40 us with 16 columns, 31 with 32; 64 x 512 to 1544: 4.0 and 4.7), and eight waves in place of four (64 x
+// 512: 4.5 -> 4.0; with up to 16 tokens four are as good or better: 16 x 8192 to 8192 17.0 us, 3.9 TB/s of
+// weights, against 17.8; two or four steps' loads in flight a wave gave nothing).
 #include <type_traits>
 
 #include "common.h"
@@ -38,7 +42,6 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr int kMaxBlocks = 4;
 constexpr int kBK = 128;  // inputs a stage
 constexpr int kBand = 4;       // row tiles of a band (an XCD's workgroups go down its rows before the next column)
-constexpr int kFewCols = 16;   // output columns a workgroup of the few-token kernel
 constexpr int kFewTokens = 64; // its most tokens
 
 struct Blocks {
@@ -288,44 +291,54 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void project_int8_kernel(const Arg
   }
 }
 
-// MT tiles of 16 tokens, NW waves sharing the inputs.
-template <typename T, int MT, int NW>
+// MT tiles of 16 tokens and NC of 16 columns, NW waves sharing the inputs.
+template <typename T, int MT, int NC, int NW>
 __global__ __launch_bounds__(64 * NW) void project_int8_few_kernel(const Args a, const Blocks blk) {
-  __shared__ int part[NW][MT][16][17];  // [token][column], a column more against bank conflicts
+  __shared__ int part[NW][MT][16][16 * NC + 1];  // [token][column], a column more against bank conflicts
   const int nb = block_of(blk, blockIdx.x);
-  const int c0 = ((int)blockIdx.x - blk.start[nb]) * kFewCols;
+  const int c0 = ((int)blockIdx.x - blk.start[nb]) * (16 * NC);
   const int used = blk.used[nb], d = a.d;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, lq = l & 15, g = l >> 4;
   const __amdgpu_buffer_rsrc_t rz = rows_rsrc(a.z, a.M, d);
   const __amdgpu_buffer_rsrc_t rw =
-      rows_rsrc(a.wt + ((size_t)nb * a.cols + c0) * d, min(kFewCols, a.cols - c0), d);
-  i32x4 acc[MT];
+      rows_rsrc(a.wt + ((size_t)nb * a.cols + c0) * d, min(16 * NC, a.cols - c0), d);
+  i32x4 acc[NC][MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = i32x4{0, 0, 0, 0};
-  // a step: 128 inputs of 16 weight rows, lane (lq, g) the 32 bytes at 32 g of row lq
-  const unsigned row = (unsigned)lq * (unsigned)d + 32u * (unsigned)g;
-  for (int k = 128 * w; k < d; k += 128 * NW) {
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[c][i] = i32x4{0, 0, 0, 0};
+  // a step: 128 inputs of 16 weight rows a tile, lane (lq, g) the 32 bytes at 32 g of row lq
+  const unsigned row = (unsigned)lq * (unsigned)d + 32u * (unsigned)g, tile = 16u * (unsigned)d;
+  for (int k0 = 128 * w; k0 < d; k0 += 128 * NW) {
+    i32x4 f[2][NC], zf[2][MT];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const unsigned o = (unsigned)k + 16u * h;
-      const i32x4 f = load16(rw, row + o);
-      const bool in = k + 32 * g + 16 * h < d;  // d is a multiple of 16
+      const int k = k0 + 16 * h;
+      const unsigned o = k + 32 * g < d ? row + (unsigned)k : kOutside;  // d is a multiple of 16
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const i32x4 zf = load16(rz, in ? (unsigned)(16 * i) * (unsigned)d + row + o : kOutside);
-        acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, zf, acc[i], 0, 0, 0);
-      }
+      for (int c = 0; c < NC; ++c) f[h][c] = load16(rw, o + tile * (unsigned)c);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) zf[h][i] = load16(rz, o + tile * (unsigned)i);
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          acc[c][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[h][c], zf[h][i], acc[c][i], 0, 0, 0);
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int c = 0; c < NC; ++c)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) part[w][i][lq][4 * g + r] = acc[i][r];
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) part[w][i][lq][16 * c + 4 * g + r] = acc[c][i][r];
   __syncthreads();
   const float* ws = a.w_scale + (size_t)nb * a.cols;
   T* out = static_cast<T*>(blk.out[nb]);
-  for (int i = threadIdx.x; i < 256 * MT; i += 64 * NW) {
-    const int c = i & 15, m = i >> 4;
+  for (int i = threadIdx.x; i < 256 * MT * NC; i += 64 * NW) {
+    const int c = i % (16 * NC), m = i / (16 * NC);
     if (m >= a.M || c0 + c >= used) continue;
     int sum = 0;
 #pragma unroll
@@ -348,7 +361,11 @@ int project_int8(const int8_t* z, const float* z_scale, const int8_t* wt, const 
   int64_t small = 0;
   for (int j = 0; j < nblk; ++j) small += ((int64_t)(used_in[j] > 0 ? used_in[j] : 0) + 127) / 128;
   const int tile = small * (((int64_t)M + 127) / 128) > 512 ? 256 : 128;
-  const int width = few ? kFewCols : tile;
+  // the few-token kernel's columns: 32 where 16 would make more than a workgroup a CU (each reads all the tokens)
+  int64_t narrow = 0;
+  for (int j = 0; j < nblk; ++j) narrow += ((int64_t)(used_in[j] > 0 ? used_in[j] : 0) + 15) / 16;
+  const int few_cols = M > 16 && narrow > 256 ? 32 : 16;
+  const int width = few ? few_cols : tile;
   Blocks blk{};
   blk.nblk = nblk;
   int64_t tiles = 0;
@@ -382,9 +399,9 @@ int project_int8(const int8_t* z, const float* z_scale, const int8_t* wt, const 
     return check_launch(who);
   }
   auto go = [&](auto kern, int nw) { hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(64 * nw), 0, s, a, blk); };
-  if (M <= 16) go(project_int8_few_kernel<T, 1, 4>, 4);
-  else if (M <= 32) go(project_int8_few_kernel<T, 2, 4>, 4);
-  else go(project_int8_few_kernel<T, 4, 4>, 4);
+  if (M <= 16) go(project_int8_few_kernel<T, 1, 1, 4>, 4);
+  else if (M <= 32) few_cols == 16 ? go(project_int8_few_kernel<T, 2, 1, 8>, 8) : go(project_int8_few_kernel<T, 2, 2, 8>, 8);
+  else few_cols == 16 ? go(project_int8_few_kernel<T, 4, 1, 8>, 8) : go(project_int8_few_kernel<T, 4, 2, 8>, 8);
   return check_launch(who);
 }
 
