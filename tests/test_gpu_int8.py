@@ -260,3 +260,33 @@ def test_a_product_past_32_bit_offsets():
     got = projection_int8(big, scales, w, ws, (24,), dtype=F32)[0]
     assert torch.equal(got[-200:], projection_int8(z, zs, w, ws, (24,), dtype=F32)[0])
     assert not bool(got[:-200].any())
+
+
+def test_refusals_on_the_gpu():
+    from vesper.contracts import ContractError
+    from vesper.kernels.norm import projection_int8, rms_norm_int8
+
+    x = torch.zeros(3, 64, device=GPU)
+    r = x.bfloat16()
+    out = torch.empty_like(x)
+    for args, match in ((dict(x=x[:, :12]), "axis 12"), (dict(x=x.double()), "dtype"), (dict(x=x, residual=x), "dtype"),
+                        (dict(x=r, residual=r.half()), "dtype"), (dict(x=x, residual=r[:2]), "residual"),
+                        (dict(x=x, residual=r.cpu()), "residual"), (dict(x=x, gain=torch.ones(32, device=GPU)), "gain"),
+                        (dict(x=x, gain=torch.ones(64)), "gain"), (dict(x=x, sum_out=out), "residual"),
+                        (dict(x=x, residual=r, sum_out=out.bfloat16()), "sum_out"), (dict(x=x, residual=r, sum_out=x), "must not be"),
+                        (dict(x=r, residual=r.clone(), sum_out=r), "must not be"),
+                        (dict(x=x.clone().requires_grad_()), "forward only")):
+        with pytest.raises(ContractError, match=match):
+            rms_norm_int8(**args)
+    with torch.no_grad():
+        rms_norm_int8(x, torch.ones(64, device=GPU, requires_grad=True))
+    z, zs, w, ws = (t.to(GPU) for t in _project_case(3, 64, (10, 10), seed=1))
+    good = dict(z=z, z_scale=zs, weights_q=w, weights_scale=ws, used=(10, 10))
+    for change, match in ((dict(z=z.short()), "int8"), (dict(z=z[:, :40]), "int8"), (dict(z_scale=zs[:2]), "z_scale"),
+                          (dict(z_scale=zs.half()), "z_scale"), (dict(weights_scale=ws[:1]), "weights_scale"),
+                          (dict(weights_scale=ws.cpu()), "on cpu"), (dict(used=(10, 11)), "widths"), (dict(used=(10, 0)), "widths"),
+                          (dict(used=(10,)), "widths"), (dict(sigmoid_block=2), "sigmoid_block"), (dict(dtype=torch.float64), "dtype")):
+        with pytest.raises(ContractError, match=match):
+            projection_int8(**{**good, **change})
+    with pytest.raises(ContractError, match="multiple of 16"):
+        projection_int8(z[:, :24], zs, w[..., :24], ws, (10, 10))

@@ -419,3 +419,93 @@ def test_the_last_row_of_a_cache_past_four_gibibytes():
     ref = _reference(q[-1:], kn[-1:], vn[-1:], torch.full((1, 1), 100 + n), small)
     assert bool(((o[-1:].cpu().double() - ref).abs() <= _bound(q, small, vn, ref, BF16)).all())
     assert int(ring.pos[-1].max()) == start + n and int(ring.valid.sum()) == n + b
+
+
+def test_one_score_far_below_the_others_and_none_above():
+    """The new token alone with a score of -1e33 (its weight is still 1), and beside a ring whose scores are 0."""
+    for w in (40, 5000):
+        ring = _ring(1, 1, 64, w, BF16)
+        q = torch.full((1, 1, 2, 64), -1e16, dtype=BF16)
+        k, v = torch.full((1, 1, 1, 64), 1e16, dtype=BF16), torch.randn(1, 1, 1, 64).to(BF16)
+        pos = torch.full((1, 1), 3 * w)
+        o, _ = _attend(q, k, v, pos, ring)
+        assert torch.equal(o.cpu(), v.repeat_interleave(2, dim=2))
+        zeros, values = torch.zeros(1, w, 1, 64, dtype=BF16), torch.randn(1, w, 1, 64).to(BF16)
+        ring = _write(zeros, values, pos - w + torch.arange(w), ring)
+        ref = _reference(q, k, v, pos, ring)
+        o, _ = _attend(q, k, v, pos, ring)
+        assert bool(((o.cpu().double() - ref).abs() <= _bound(torch.zeros(1, 1, 1, 64), ring, v, ref, BF16)).all())
+
+
+def test_rings_that_are_strided_are_copied_and_refused_in_place():
+    from vesper.contracts import ContractError
+    from vesper.kernels.ring_quant import QuantRingKVCache, quant_ring_read
+
+    q, k, v, pos, ring = _case(2, 48, 2, 2, 64, BF16, seed=17)
+    strided = QuantRingKVCache(*(torch.stack([t, t], -1)[..., 0] for t in ring.tensors()), ring.window)
+    want, ring_want = _attend(q, k, v, pos, ring)
+    o, out = _attend(q, k, v, pos, strided)
+    assert torch.equal(o, want)
+    for mine, theirs in zip(out.tensors(), ring_want.tensors()):
+        assert torch.equal(mine, theirs)
+    asked = pos.to(GPU) - 1 - torch.arange(10, device=GPU)
+    for a, b in zip(quant_ring_read(strided, asked), quant_ring_read(ring, asked)):
+        assert torch.equal(a, b)
+    for call in (lambda: _attend(q, k, v, pos, strided, inplace=True), lambda: _write(k, v, pos, strided, inplace=True)):
+        with pytest.raises(ContractError, match="contiguous"):
+            call()
+
+
+def test_refusals_on_the_gpu():
+    from vesper.contracts import ContractError
+    from vesper.kernels.ring_quant import QuantRingKVCache, quant_ring_attention, quant_ring_read, quant_ring_write
+
+    ring = _ring(2, 2, 16, 8, BF16)
+    x = torch.zeros(2, 3, 2, 16, dtype=BF16, device=GPU)
+    pos = torch.arange(3, device=GPU).expand(2, 3)
+    for bad, match in ((pos - 1, "nonnegative"), (pos * 2, "consecutive"), (pos.flip(1), "consecutive")):
+        with pytest.raises(ContractError, match=match):
+            quant_ring_write(x, x, bad, ring)
+    for lengths in ([-1, 2], [2, 4]):
+        with pytest.raises(ContractError, match="lengths"):
+            quant_ring_write(x, x, pos, ring, lengths=torch.tensor(lengths, device=GPU))
+    with pytest.raises(ContractError, match="lengths"):
+        quant_ring_write(x, x, pos, ring, lengths=torch.tensor([1, 2]))
+    with pytest.raises(ContractError, match="axis"):
+        quant_ring_write(x, x, pos, ring, lengths=torch.tensor([1, 2, 3], device=GPU))
+    with pytest.raises(ContractError, match="forward only"):
+        quant_ring_write(x.clone().requires_grad_(), x, pos, ring)
+    one, at = x[:, :1], pos[:, :1]
+    with pytest.raises(ContractError, match="forward only"):
+        quant_ring_attention(one.clone().requires_grad_(), one, one, at, ring)
+    with torch.no_grad():
+        quant_ring_attention(one.clone().requires_grad_(), one, one, at, ring)
+    with pytest.raises(ContractError, match="nonnegative"):
+        quant_ring_attention(one, one, one, at - 1, ring)
+    with pytest.raises(ContractError, match="at most 8"):
+        quant_ring_attention(one.repeat(1, 1, 9, 1), one, one, at, ring)
+    with pytest.raises(ContractError, match="need a multiple"):
+        quant_ring_attention(one[:, :, :1], one, one, at, ring)
+    with pytest.raises(ContractError, match="active"):
+        quant_ring_attention(one, one, one, at, ring, active=torch.ones(2, dtype=torch.bool))
+    with pytest.raises(ContractError, match="cache.pos is on cpu"):
+        quant_ring_attention(one, one, one, at, QuantRingKVCache(*ring.tensors()[:4], ring.pos.cpu(), ring.valid, 8))
+    learned = QuantRingKVCache(ring.k, ring.v, ring.k_scale.clone().requires_grad_(), *ring.tensors()[3:], 8)
+    with pytest.raises(ContractError, match="forward only"):
+        quant_ring_read(learned, pos)
+    assert not bool(ring.valid.any())  # nothing was written
+
+
+def test_calls_of_no_rows_and_no_tokens():
+    from vesper.kernels.ring_quant import quant_ring_attention, quant_ring_read, quant_ring_write
+
+    for b, n in ((0, 3), (2, 0)):
+        ring = _ring(b, 2, 16, 8, BF16)
+        x, pos = torch.zeros(b, n, 2, 16, dtype=BF16, device=GPU), torch.zeros(b, n, dtype=torch.long, device=GPU)
+        out = quant_ring_write(x, x, pos, ring)
+        assert out.k.shape == ring.k.shape and not bool(out.valid.any())
+        k, v, found = quant_ring_read(ring, pos)
+        assert k.shape == v.shape == (b, n, 2, 16) and found.shape == (b, n)
+    x = torch.zeros(0, 1, 2, 16, dtype=BF16, device=GPU)
+    o, _ = quant_ring_attention(x, x, x, torch.zeros(0, 1, dtype=torch.long, device=GPU), _ring(0, 2, 16, 8, BF16))
+    assert o.shape == (0, 1, 2, 16)

@@ -506,7 +506,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
       if (c < G) smerge[w][c][2 + (4 * g + r) * M + e] = x + low;
     }
   if (g == 0 && c < G) {
-    smerge[w][c][0] = m;
+    smerge[w][c][0] = lsum == 0.f ? -kInf : m;  // a wave that saw nothing has no say in the maximum
     smerge[w][c][1] = lsum;
   }
   __syncthreads();
@@ -514,17 +514,18 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
   const bool on = a.active == nullptr || a.active[b] != 0;
   for (int i = tid; i < G * dk; i += 64 * NW) {
     const int gi = i / dk, d = i - gi * dk;
-    float mx = split == 0 ? sfresh[gi] : -1e30f;
+    float mx = split == 0 ? sfresh[gi] : -kInf;
 #pragma unroll
     for (int u = 0; u < NW; ++u) mx = __builtin_fmaxf(mx, smerge[u][gi][0]);
+    const float from = mx == -kInf ? 0.f : mx;  // a split that saw nothing: weights of zero
     float ls = 0.f, num = 0.f;
     if (split == 0) {
-      ls = __builtin_amdgcn_exp2f(sfresh[gi] - mx);
+      ls = __builtin_amdgcn_exp2f(sfresh[gi] - from);
       num = ls * to_f32(vnew[head * dk + d]);
     }
 #pragma unroll
     for (int u = 0; u < NW; ++u) {
-      const float f = __builtin_amdgcn_exp2f(smerge[u][gi][0] - mx);
+      const float f = __builtin_amdgcn_exp2f(smerge[u][gi][0] - from);
       ls += smerge[u][gi][1] * f;
       num += smerge[u][gi][2 + d] * f;
     }
@@ -542,7 +543,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
   }
 }
 
-// The splits' softmax states of one query head joined: their weights first, one split a thread, then groups of
+// The splits' softmax states of one query head joined (the first holds the new token, so their maximum is one of a
+// score): their weights first, one split a thread, then groups of
 // dk threads take the splits in turn and the groups' sums are added in order.
 template <typename T>
 __global__ __launch_bounds__(1024) void quant_join_kernel(const float* __restrict__ partial, T* __restrict__ o,
@@ -553,7 +555,7 @@ __global__ __launch_bounds__(1024) void quant_join_kernel(const float* __restric
   const int pitch = 2 + dk;
   const float* part = partial + row * splits * (size_t)pitch;
   const int t = threadIdx.x, w = t >> 6, nw = blockDim.x >> 6;
-  const float m = t < splits ? part[(size_t)t * pitch] : -1e30f, l = t < splits ? part[(size_t)t * pitch + 1] : 0.f;
+  const float m = t < splits ? part[(size_t)t * pitch] : -kInf, l = t < splits ? part[(size_t)t * pitch + 1] : 0.f;
   float mx = group_max<64>(m);
   if ((t & 63) == 0) red[0][w] = mx;
   __syncthreads();

@@ -300,7 +300,8 @@ def _check_norm_int8(x: Tensor, gain: Tensor | None, residual: Tensor | None, rd
 def quantize_weights(weights_t: Tensor) -> tuple[Tensor, Tensor]:
     """A stacked projection weight ``[p, cols, d]`` (each block transposed, one output channel a row) as the
     operands of ``projection_int8``, made once: int8 ``[p, cols, d]`` and float32 scales ``[p, cols]``, each row
-    ``codes * scale`` with ``scale = max |w| / 127`` and ``codes = round(w / scale)`` (zeros for a row of zeros).
+    ``codes * scale`` with ``scale = max |w| / 127`` and ``codes = round(w / scale)`` (zeros for a row of zeros). Reads
+    a flag back from the device, so it does not run under a graph capture.
 
     Raises:
         ContractError: if ``weights_t`` is not a floating ``[p, cols, d]`` tensor of finite values.

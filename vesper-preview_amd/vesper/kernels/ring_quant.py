@@ -97,6 +97,7 @@ def _check_ring(cache: QuantRingKVCache, dims: Dims) -> torch.dtype:
     check_shape("cache.pos", cache.pos, ("b", "w"), dims, torch.long)
     check_shape("cache.valid", cache.valid, ("b", "w"), dims, torch.bool)
     dtype = cache.k_scale.dtype
+    _refuse_grad(cache.k_scale, cache.v_scale)
     if dtype not in _SUFFIX:
         raise ContractError(f"cache.k_scale: dtype must be bfloat16 or float16, got {dtype}")
     if cache.window < 1:
@@ -133,6 +134,7 @@ def _ring_as_is(cache: QuantRingKVCache, b: int, hkv: int, dk: int, dtype: torch
             and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
             and pos.is_contiguous() and valid.is_contiguous()
             and (k.data_ptr() | v.data_ptr() | ks.data_ptr() | vs.data_ptr()) & 3 == 0
+            and not (ks.requires_grad or vs.requires_grad)
             and w >= 1 and dk & 7 == 0 and 8 <= dk <= MAX_HEAD_DIM and 1 <= hkv <= MAX_KV_HEADS)
 
 
