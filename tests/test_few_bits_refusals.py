@@ -132,6 +132,8 @@ def test_the_c_entries_refuse_before_any_launch():
     assert write(one + 8, *[one] * 9, 1, 1, 1, 16, 4, None) != 0 and "16-byte" in err()
     assert write(one, one, one, None, one + 2, *[one] * 5, 1, 1, 1, 16, 4, None) != 0 and "4-byte" in err()
     assert write(*none8, 0, 1, 1, 16, 4, None) == 0 and write(*none8, 1, 0, 1, 16, 4, None) == 0
+    assert write(*[one] * 10, 1 << 24, 1, 1, 16, 4, None) != 0 and "16777216 workgroups" in err()
+    assert read(*[one] * 10, 1 << 24, 1, 1, 16, 4, None) != 0 and "16777216 workgroups" in err()
     assert read(*none8, 1, 1, 0, 16, 4, None) != 0 and "HKV=0" in err()
     assert read(*none8, 1, 1, 1, 16, 4, None) != 0 and "null" in err()
     assert read(*none8, 1, 0, 1, 16, 4, None) == 0
@@ -141,6 +143,7 @@ def test_the_c_entries_refuse_before_any_launch():
     assert call([None] * 13, 1, 1, 1, 264, 4) != 0 and "264" in err()
     assert call([None] * 13, 1, 1, 1, 16, 4) != 0 and "null" in err()
     assert call([None] * 13, 0, 1, 1, 16, 4) == 0
+    assert call([one] * 13, 1 << 24, 1, 1, 16, 4) != 0 and "workgroups" in err()
     need = lib.vsp_quant_ring_attn_workspace_bytes(1, 2, 1, 64, 4096)
     assert need > 0
     assert call([one] * 13, 1, 2, 1, 64, 4096, need - 1) != 0 and "workspace" in err()

@@ -110,6 +110,23 @@ def test_a_chunk_is_quantised_into_its_slots_and_read_back(b, n, w, hkv, dk, dty
             assert torch.equal(got[i].cpu(), ref)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_equal_features_of_every_size_have_a_scale_and_codes_of_zero(dtype):
+    top = torch.finfo(dtype).max
+    sizes = [0.0, 1e-7, 1.0, -3.0, 6e4] + ([1e-40, 1e13, -5e15, 1e30, top, -top] if dtype == BF16 else [top, -top])
+    x = torch.tensor(sizes, dtype=torch.float64).to(dtype)[None, :, None, None].expand(1, len(sizes), 2, 24)
+    ring = _write(x, x, torch.arange(len(sizes))[None], _ring(1, 2, 24, len(sizes), dtype))
+    for packed, pair in ((ring.k, ring.k_scale), (ring.v, ring.v_scale)):
+        assert not bool(packed.any()) and not bool(pair[..., 0].any())
+        assert torch.equal(pair[..., 1].cpu(), x[..., 0].transpose(1, 2))
+    q = x[:, :1].contiguous()
+    _, ring = _attend(q, q, q, torch.zeros(1, 1, dtype=torch.long), ring)
+    for size in sizes:
+        k = torch.full((1, 1, 2, 24), size, dtype=torch.float64).to(dtype)
+        _, out = _attend(q, k, k, torch.full((1, 1), 2 * len(sizes)), ring)
+        assert not bool(out.k[:, :, 0].any()) and not bool(out.v[:, :, 0].any())
+
+
 @pytest.mark.parametrize("inplace", [False, True])
 def test_a_padded_batch_writes_each_rows_own_tokens_and_nothing_else(inplace):
     b, n, w, hkv, dk = 5, 20, 12, 2, 32
@@ -432,6 +449,22 @@ def test_one_score_far_below_the_others_and_none_above():
         assert torch.equal(o.cpu(), v.repeat_interleave(2, dim=2))
         zeros, values = torch.zeros(1, w, 1, 64, dtype=BF16), torch.randn(1, w, 1, 64).to(BF16)
         ring = _write(zeros, values, pos - w + torch.arange(w), ring)
+        ref = _reference(q, k, v, pos, ring)
+        o, _ = _attend(q, k, v, pos, ring)
+        assert bool(((o.cpu().double() - ref).abs() <= _bound(torch.zeros(1, 1, 1, 64), ring, v, ref, BF16)).all())
+
+
+def test_scores_that_are_all_far_below_zero_keep_their_order():
+    """Scores of -2e32 in every slot but one, -4e31 there and -2e33 of the new token: that slot's value. Equal features
+    have a scale of 0, and gaps of 1e32 leave one weight, so the scores' rounding does not count."""
+    for w in (40, 5000):
+        pos = torch.full((1, 1), 3 * w)
+        keys = torch.full((1, w, 1, 64), 5e15, dtype=BF16)
+        keys[0, 2 * w // 3] = 1e15
+        values = torch.randn(1, w, 1, 64, generator=torch.Generator().manual_seed(w)).to(BF16)
+        ring = _write(keys, values, pos - w + torch.arange(w), _ring(1, 1, 64, w, BF16))
+        q = torch.full((1, 1, 2, 64), -5e15, dtype=BF16)
+        k, v = torch.full((1, 1, 1, 64), 5e16, dtype=BF16), torch.randn(1, 1, 1, 64).to(BF16)
         ref = _reference(q, k, v, pos, ring)
         o, _ = _attend(q, k, v, pos, ring)
         assert bool(((o.cpu().double() - ref).abs() <= _bound(torch.zeros(1, 1, 1, 64), ring, v, ref, BF16)).all())

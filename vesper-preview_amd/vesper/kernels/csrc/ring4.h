@@ -78,7 +78,8 @@ __device__ __forceinline__ uint32_t quantize_row8(const float (&x)[8], uint32_t&
   const float half = 0.5f * to_f32(s);
   // Small steps are scaled up first (exactly), so that the reciprocal and the residual stay normal numbers;
   // the largest step, 2^124, has a normal reciprocal.
-  const float up = half < 0x1p-60f ? 0x1p80f : 1.f;
+  // Not a step of 0, whose features may be of any size: it finds every quotient 0.
+  const float up = __float_as_uint(half) - 1u < __float_as_uint(0x1p-60f) - 1u ? 0x1p80f : 1.f;
   const float step = half * up, low = lo * up, inv = half > 0.f ? __builtin_amdgcn_rcpf(step) : 0.f;
   uint32_t codes = 0;
 #pragma unroll

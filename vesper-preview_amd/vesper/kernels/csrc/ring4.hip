@@ -24,6 +24,11 @@
 // the rest of it, rounded again, in the others, together 16 bits of it. Sums, maxima and weights are
 // float32; the running maximum is raised only when a tile's exceeds it by more than 8 (weights up to 2^8
 // are as exact), so the accumulators are rarely rescaled.
+//
+// Bound by HBM where the ring is long: 8 rows of 65536 slots, four heads of 128 (290 MB): 57.7 us, 5.0 TB/s, and 4.6
+// for the join. Short windows are a launch and a wave's chain of loads: 64 rows of 512 slots, 8 heads of 64: 9.4 us,
+// 4.8 with nothing to attend. Writing 7 ragged rows of 4097 tokens (8 heads of 64): 16 us, reading them back 16.5; a
+// bare copy of the write's pattern takes 10.4.
 #include <type_traits>
 
 #include "common.h"
@@ -36,6 +41,7 @@ namespace {
 constexpr int kQuantMaxGroup = 8;
 constexpr int kTile = 32;       // tokens a wave takes at a time
 constexpr int kMaxSplits = 256;  // workgroups that share a window (one thread each in the join)
+constexpr int64_t kMaxThreads = (int64_t)1 << 32;  // a launch has fewer
 constexpr float kRaise = 8.f;   // log2: how far a tile's maximum may exceed the running one
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -396,7 +402,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
     if (l < kQuantMaxGroup) sfresh[l] = fresh;
   }
 
-  float m = -1e30f, lsum = 0.f, low = 0.f;  // the running maximum, the lane's sums of P and of P m'
+  float m = -3.40282347e38f, lsum = 0.f, low = 0.f;  // the running maximum (finite: scores of -inf weigh 0), the lane's sums of P and of P m'
   f32x4 acc[M], bias = zero4();
 #pragma unroll
   for (int e = 0; e < M; ++e) acc[e] = zero4();
@@ -626,7 +632,7 @@ int quant_write(const T* k, const T* v, const int64_t* pos, const int64_t* lengt
     return fail(ERR_ARG, "%s: the ring's tensors must be 4-byte aligned", who);
   const int tb = 256 / lanes_of(D), blocks = ((N < W ? N : W) + tb - 1) / tb;
   const int64_t grid = (int64_t)B * blocks * HKV;
-  if (grid >= ((int64_t)1 << 31)) return fail(ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
+  if (grid >= kMaxThreads / 256) return fail(ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
   by_lanes(D, [&](auto lanes) {
     hipLaunchKernelGGL((quant_write_kernel<T, decltype(lanes)::value>), dim3((unsigned)grid), dim3(256), 0,
                        reinterpret_cast<hipStream_t>(stream), k, v, pos, lengths, static_cast<uint32_t*>(ring_k),
@@ -651,7 +657,7 @@ int quant_read(const void* ring_k, const void* ring_v, const void* k_scale, cons
     return fail(ERR_ARG, "%s: the ring's tensors must be 4-byte aligned", who);
   const int tb = kReadTokens * (256 / lanes_of(D)), blocks = (int)(((int64_t)N + tb - 1) / tb);
   const int64_t grid = (int64_t)B * blocks * HKV;
-  if (grid >= ((int64_t)1 << 31)) return fail(ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
+  if (grid >= kMaxThreads / 256) return fail(ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
   by_lanes(D, [&](auto lanes) {
     hipLaunchKernelGGL((quant_read_kernel<T, decltype(lanes)::value>), dim3((unsigned)grid), dim3(256), 0,
                        reinterpret_cast<hipStream_t>(stream), static_cast<const uint32_t*>(ring_k),
@@ -715,7 +721,7 @@ int quant_attn(const T* q, const T* knew, const T* vnew, const int64_t* pos, voi
     return fail(ERR_ARG, "%s: workspace of %zu bytes given, %zu needed", who, workspace ? ws_bytes : (size_t)0, need);
   const int threads = 64 * shape.waves, lanes = D <= 32 ? 4 : lanes_of(D);
   const int64_t grid = (int64_t)B * HKV * splits + (write ? ((int64_t)B * HKV * 2 * lanes + threads - 1) / threads : 0);
-  if (grid >= ((int64_t)1 << 31) || (int64_t)B * H >= ((int64_t)1 << 31))
+  if (grid >= kMaxThreads / threads || (int64_t)B * H >= ((int64_t)1 << 31))
     return fail(ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
   const QuantAttnArgs a{pos, static_cast<uint32_t*>(ring_k), static_cast<uint32_t*>(ring_v),
