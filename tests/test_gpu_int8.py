@@ -290,3 +290,33 @@ def test_refusals_on_the_gpu():
             projection_int8(**{**good, **change})
     with pytest.raises(ContractError, match="multiple of 16"):
         projection_int8(z[:, :24], zs, w[..., :24], ws, (10, 10))
+
+
+@pytest.mark.parametrize(("rows", "d"), [(2**26 + 5, 8), (2**22 + 3, 2056)])
+def test_more_rows_than_one_launch_takes(rows, d):
+    """Rows that repeat after 1000: each like the first of its kind, and those like a small call's."""
+    from vesper.kernels.norm import rms_norm_int8
+
+    few = torch.randn(1000, d, generator=torch.Generator().manual_seed(d)).to(torch.bfloat16).to(GPU)
+    x = few.repeat((rows + 999) // 1000, 1)[:rows]
+    codes, scale = rms_norm_int8(x)
+    want, want_scale = rms_norm_int8(few)
+    at = torch.arange(rows, device=GPU) % 1000
+    assert torch.equal(scale, want_scale[at])
+    for i in range(0, rows, 1000 * 2**10):
+        part = codes[i:i + 1000 * 2**10]
+        assert torch.equal(part, want[at[i:i + 1000 * 2**10]])
+
+
+def test_more_rows_than_32_bits_count_are_refused():
+    """Broadcast rows, so that nothing of that size is allocated."""
+    from vesper.contracts import ContractError
+    from vesper.kernels.norm import projection_int8, rms_norm_int8
+
+    rows = 2**31
+    with pytest.raises(ContractError, match="2147483647"):
+        rms_norm_int8(torch.ones(1, 8, dtype=torch.bfloat16, device=GPU).expand(rows, 8))
+    w = torch.ones(1, 8, 16, dtype=torch.int8, device=GPU)
+    with pytest.raises(ContractError, match="2147483647"):
+        projection_int8(torch.ones(1, 16, dtype=torch.int8, device=GPU).expand(rows, 16),
+                        torch.ones(1, device=GPU).expand(rows), w, torch.ones(1, 8, device=GPU), (8,))

@@ -211,6 +211,7 @@ def projection(z: Tensor, weights_t: Tensor, used: tuple[int, ...], *,
     return outs
 
 
+MAX_ROWS = 2**31 - 1  # of the 8-bit operators: their C entries count rows in 32 bits
 _INT8_SUFFIX = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
 # x and residual dtypes of rms_norm_int8
 _NORM_INT8 = {(torch.float32, torch.bfloat16): "f32_bf16", (torch.float32, torch.float16): "f32_f16",
@@ -252,7 +253,8 @@ def rms_norm_int8(x: Tensor, gain: Tensor | None = None, *, residual: Tensor | N
     suffix = _NORM_INT8.get((dtype, rdtype))
     d = shape[-1] if shape else 0
     # one test on the common path; the checks that name what is wrong run where it fails
-    if not (suffix is not None and device >= 0 and 8 <= d <= 16384 and d & 7 == 0 and not x.requires_grad
+    if not (suffix is not None and device >= 0 and 8 <= d <= 16384 and d & 7 == 0 and x.numel() <= MAX_ROWS * d
+            and not x.requires_grad
             and (gain is None or (gain.shape == (d,) and gain.dtype is torch.float32 and gain.get_device() == device
                                   and not gain.requires_grad))
             and (residual is None or (residual.shape == shape and residual.get_device() == device
@@ -290,6 +292,8 @@ def _check_norm_int8(x: Tensor, gain: Tensor | None, residual: Tensor | None, rd
     d = x.shape[-1]
     if d < 8 or d > 16384 or d % 8:
         raise ContractError(f"x: last axis {d} is not a multiple of 8 in 8..16384")
+    if x.numel() > MAX_ROWS * d:
+        raise ContractError(f"x: {x.numel() // d} rows, the kernel takes at most {MAX_ROWS}")
     _refuse_grad("rms_norm_int8", x, gain, residual)
     if gain is not None and (gain.shape != (d,) or gain.dtype != torch.float32 or gain.device != x.device):
         raise ContractError(f"gain: must be float32 [{d}] on {x.device}, got {tuple(gain.shape)} {gain.dtype}")
@@ -344,7 +348,7 @@ def projection_int8(z: Tensor, z_scale: Tensor, weights_q: Tensor, weights_scale
     zshape, wshape, device, suffix = z.shape, weights_q.shape, z.get_device(), _INT8_SUFFIX.get(dtype)
     # one test on the common path; the checks that name what is wrong run where it fails
     if not (len(zshape) == 2 and len(wshape) == 3 and z.dtype is torch.int8 and weights_q.dtype is torch.int8
-            and wshape[2] == zshape[1] and wshape[0] == p and 1 <= p <= 4 and z_scale.shape == zshape[:1]
+            and wshape[2] == zshape[1] and wshape[0] == p and 1 <= p <= 4 and zshape[0] <= MAX_ROWS and z_scale.shape == zshape[:1]
             and weights_scale.shape == wshape[:2] and z_scale.dtype is torch.float32
             and weights_scale.dtype is torch.float32 and device >= 0 and z_scale.get_device() == device
             and weights_q.get_device() == device and weights_scale.get_device() == device
@@ -380,6 +384,8 @@ def _check_projection_int8(z: Tensor, z_scale: Tensor, weights_q: Tensor, weight
             raise ContractError(f"{name} is on {t.device}, z on {z.device}")
     if len(used) != p or not 1 <= p <= 4 or any(not 1 <= u <= cols for u in used):
         raise ContractError(f"used: {p} widths in 1..{cols}, got {tuple(used)}")
+    if m > MAX_ROWS:
+        raise ContractError(f"z: {m} rows, the kernel takes at most {MAX_ROWS}")
     if d % 16 or not 16 <= d <= 16384:
         raise ContractError(f"z: width {d} is not a multiple of 16 in 16..16384")
     if sigmoid_block is not None and not 0 <= sigmoid_block < p:
