@@ -20,7 +20,9 @@
 // cycles), a library product of the same operands 547. 32767 x 768 to 2316 columns: 94 us, of which the loads into
 // LDS take 36 alone (503 MB, 14 TB/s), the products 25 and the outputs 29, with one workgroup a CU nearly one after
 // the other; 128 x 128 tiles, two workgroups a CU, need 57, 15 and 22: 98 us. Stages of 64 inputs, four deep, read
-// half cache lines: 117 us. Three stages of 256 x 128: 108 us.
+// half cache lines: 117 us. Three stages of 256 x 128: 108 us. A workgroup a CU that goes from tile to tile, loading the
+// next one's first stage under the last products: 95-107 us (stores and loads retire in one order, so its first wait
+// is for the stores too).
 //
 // few (up to 64 tokens, a decode step): bound by reading the weights once. A workgroup takes 16 columns and
 // all the tokens; its waves share the inputs, each reading whole 128-byte lines of 16 weight rows straight
