@@ -148,6 +148,14 @@ def test_the_projection_in_8_bits(m, d, used, dtype):
     _check_project(z, zs, w, ws, used, len(used) - 1 if len(used) > 1 else None, dtype)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize(("d", "sig"), [(16, 3), (272, None), (512, 0)])
+def test_more_tiles_than_one_round_of_workgroups(d, sig, dtype):
+    """67 x 6 tiles of 256 x 256: one, three and four stages, a last row tile of 104 tokens, ragged and narrow blocks."""
+    z, zs, w, ws = _project_case(17000, d, (300, 256, 265, 9), seed=d)
+    _check_project(z, zs, w, ws, (300, 256, 265, 9), sig, dtype)
+
+
 @pytest.mark.parametrize("m", [3, 40, 64, 65, 300])
 def test_the_largest_sums_are_exact(m):
     """Every product 127 * 127 (and its negative) over the widest row: 2.6e8, within int32."""

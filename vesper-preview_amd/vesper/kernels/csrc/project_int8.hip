@@ -11,18 +11,18 @@
 //
 // Two kernels, by the number of tokens:
 //
-// tile (many tokens): 256 tokens x 256 columns a workgroup of eight waves of 64 x 128, both operands through LDS in
-// two stages of 128 inputs (whole cache lines a row), or, where that makes few workgroups, 128 x 128 in waves of
-// 64 x 32 and three stages. global_load_lds_dwordx4 moves eight rows of 128 bytes an instruction, each row's
-// 16-byte segments XOR-swizzled so that the fragment reads meet each bank once; 16x16x64 int8 MFMA formed
-// transposed (weight rows as the A operand); the second half's fragments are read during the first half's products.
-// 8192^3: 480 us (2.3 Pop/s; the chip's products clock down under them: the matrix units are busy 58 % of the
-// cycles), a library product of the same operands 547. 32767 x 768 to 2316 columns: 94 us, of which the loads into
-// LDS take 36 alone (503 MB, 14 TB/s), the products 25 and the outputs 29, with one workgroup a CU nearly one after
-// the other; 128 x 128 tiles, two workgroups a CU, need 57, 15 and 22: 98 us. Stages of 64 inputs, four deep, read
-// half cache lines: 117 us. Three stages of 256 x 128: 108 us. A workgroup a CU that goes from tile to tile, loading the
-// next one's first stage under the last products: 95-107 us (stores and loads retire in one order, so its first wait
-// is for the stores too).
+// tile (many tokens): 256 tokens x 256 columns, eight waves of 64 x 128, both operands through LDS in two stages of
+// 128 inputs (whole cache lines a row), by a workgroup a CU that goes from tile to tile; or, where that makes few
+// workgroups, 128 x 128 in waves of 64 x 32 and three stages. global_load_lds_dwordx4 moves eight rows of 128 bytes an
+// instruction, each row's 16-byte segments XOR-swizzled so that the fragment reads meet each bank once; 16x16x64 int8
+// MFMA formed transposed (weight rows as the A operand); the second half's fragments are read during the first half's
+// products. 8192^3: 444 to 473 us among other work, 520 to 540 back to back (2.0 to 2.5 Pop/s; the clock falls under them:
+// the matrix units are busy 63 % of the cycles), a library product of the same operands 547. 32767 x 768 to 2316 columns: 72 us
+// (116 Gop, 1.6 Pop/s). One tile a workgroup needed 96: its first loads and its outputs stood alone, and the logistic
+// function, chosen an output at a time, ran for all of them (86 with that block's outputs apart; 78 from tile to
+// tile; 72 with the next tile's second stage loading under the outputs too). Stages of 64 inputs, four deep, read half
+// cache lines (117 when the present form took 94); three stages of 256 x 128: 108; outputs stored straight from the
+// accumulators, 32 bytes a row: 95 to 107.
 //
 // few (up to 64 tokens, a decode step): bound by reading the weights once. A workgroup takes 16 columns and
 // all the tokens; its waves share the inputs, each reading whole 128-byte lines of 16 weight rows straight
@@ -65,10 +65,10 @@ struct Args {
 // exponential and reciprocal instructions (each within a unit of float32): a thread has 64 to 128 outputs, and as
 // calls of the library's functions their code outgrew the instruction cache (32767 tokens of 768: 104 us with
 // it, 90 without a logistic block).
-template <typename T>
-__device__ __forceinline__ T finish(int sum, float scale, bool sig) {
+template <typename T, bool SIG>
+__device__ __forceinline__ T finish(int sum, float scale) {
   float y = (float)sum * scale;
-  if (sig) y = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * y));
+  if constexpr (SIG) y = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * y));
   return from_f32<T>(y);
 }
 
@@ -111,56 +111,295 @@ __device__ __forceinline__ void arrive() {
 #endif
 }
 
-// WM x WN waves of 16 TM tokens x 16 TN columns each, S stages in LDS.
-template <typename T, int WM, int WN, int TM, int TN, int S>
-__global__ __launch_bounds__(64 * WM * WN, 1) void project_int8_kernel(const Args a, const Blocks blk, int ctiles,
-                                                                      int mtiles, int band) {
-  constexpr int AHEAD = TN < 4 ? TN : 4;  // weight fragments read ahead of the products
-  constexpr int NW = WM * WN, BM = 16 * TM * WM, BN = 16 * TN * WN;
-  static_assert(BM == BN && BM % (8 * NW) == 0, "square tiles of whole load instructions");
-  static_assert(S == 2 || S == 3, "two or three stages");
-  // Stages of the z rows and the weight rows, [rows][128 inputs] each: row r's 16-byte segment s at s ^
-  // 2 ((r >> 1) & 3), so that a fragment read (lanes 0-7 with 16-23: rows 0-7, two segments each) meets every
-  // bank once. Separate variables: the compiler tells the direct loads into one from the reads of the others.
-  __shared__ __align__(16) int8_t sZ0[BM * kBK], sZ1[BM * kBK], sZ2[S == 3 ? BM * kBK : 16];
-  __shared__ __align__(16) int8_t sW0[BN * kBK], sW1[BN * kBK], sW2[S == 3 ? BN * kBK : 16];
-  __shared__ __align__(16) float sScaleZ[BM], sScaleW[BN];
-
-  // Workgroups of an XCD take runs of tiles, bands of `band` row tiles each, down a band's rows before the next
-  // column tile: those that run together share rows of z and columns of the weights in the XCD's L2.
-  const int lg = xcd_logical_block(blockIdx.x, gridDim.x);
-  const int top = lg / (band * ctiles) * band, in_band = lg - top * ctiles, rows = min(band, mtiles - top);
-  if (rows <= 0) return;  // the grid is padded to whole XCD rounds; whole workgroups leave
-  const int ct = in_band / rows, mt = top + in_band - ct * rows;
-  if (ct >= ctiles) return;
-  const int nb = block_of(blk, ct);
-  const int c0 = (ct - blk.start[nb]) * BN;
-  const int used = blk.used[nb], d = a.d;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, lq = l & 15, g = l >> 4;
-  const int wm = w % WM, wn = w / WM;  // the wave's tokens 16 TM wm .. and columns 16 TN wn ..
-  const bool live = c0 + 16 * TN * wn < used;
-  const int stages = (d + kBK - 1) / kBK;
-
-  // resources of the tile's own rows (under 256 x 16384 bytes): rows past the operands' ends read zeros
-  const int zrows = min(BM, a.M - mt * BM), wrows = min(BN, a.cols - c0);
-  const __amdgpu_buffer_rsrc_t rz = rows_rsrc(a.z + (size_t)mt * BM * d, zrows, d);
-  const __amdgpu_buffer_rsrc_t rw = rows_rsrc(a.wt + ((size_t)nb * a.cols + c0) * d, wrows, d);
-  auto kswz = [](int row) { return 2 * ((row >> 1) & 3); };
-  // direct loads: instruction j of wave w fills rows 8 (w + NW j) .. + 7 of a stage, 128 bytes each; lane l brings
-  // row l / 8's logical segment (l % 8) ^ kswz(row)
-  constexpr int NL = BM / (8 * NW);
-  const int lrow = l >> 3, lseg = (l & 7) ^ kswz(lrow);
-  unsigned off[NL];  // the scalar offset holds the stage only: it stays below every resource's size
+// A wave's tile of sums out: tokens m0 .. and columns c0 .. of block nb, with their scales, which lie in `lds` from
+// `zscale` and `wscale` on. Lane (lq, g) holds columns 16 j + 4 g + r of token 16 i + lq. Outputs of 16 bits go through
+// LDS (from `room` on, the wave's own), 16 tokens by 64 columns (or the tile's fewer) at a time, so that whole cache
+// lines leave; row r's 16-byte segment s is at s ^ (r % the row's segments). Returns how many stores the wave has made
+// for certain: kStores, or 0 where some had nothing to store.
+constexpr int kStores = 16;
+template <typename T, int TM, int TN>
+__device__ __forceinline__ int store_tile(const i32x4 (&acc)[TN][TM], const Args& a, const Blocks& blk, int nb, int m0,
+                                          int c0, int8_t* lds, int zscale, int wscale, int room) {
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  typedef T V8 __attribute__((ext_vector_type(8)));
+  int l = threadIdx.x & 63;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(l));  // formed anew for each tile: kept in registers over the products, addresses would spill
+#endif
+  const int lq = l & 15, g = l >> 4, used = blk.used[nb];
+  T* out = static_cast<T*>(blk.out[nb]);
+  auto put = [&](auto sig, auto all) {
+    constexpr bool SIG = decltype(sig)::value, full = decltype(all)::value;
+    if constexpr (sizeof(T) == 2) {
+      // TC column tiles a pass: 16-byte segments a row, rows an instruction
+      constexpr int TC = TN < 4 ? TN : 4, SEG = 2 * TC, EACH = 64 / SEG;
+      const int seg = l % SEG, r0 = l / SEG;
 #pragma unroll
-  for (int j = 0; j < NL; ++j) off[j] = (unsigned)(8 * (w + NW * j) + lrow) * (unsigned)d + 16u * (unsigned)lseg;
-  auto issue = [&](int st, int8_t* dz, int8_t* dw) {
-    // inputs past d (d is a multiple of 16, so whole segments), and whole stages past the last, are zeros
-    const bool in = st * kBK + 16 * lseg < d;
+      for (int i = 0; i < TM; ++i) {
+        const float zs = *reinterpret_cast<const float*>(lds + (zscale + 64 * i + 4 * lq));
+#pragma unroll
+        for (int j0 = 0; j0 < TN; j0 += TC) {
+#pragma unroll
+          for (int j = 0; j < TC; ++j) {
+            const int c = 16 * j + 4 * g;
+            const f32x4 bs = *reinterpret_cast<const f32x4*>(lds + (wscale + 64 * j0 + 4 * c));
+            V4 y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = finish<T, SIG>(acc[j0 + j][i][r], zs * bs[r]);
+            *reinterpret_cast<V4*>(lds + (room + 32 * TC * lq + 16 * ((c >> 3) ^ (lq & (SEG - 1))) + 2 * (c & 7))) = y;
+          }
+          __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the rows are in LDS
+#pragma unroll
+          for (int it = 0; it < 16 / EACH; ++it) {
+            const int r = EACH * it + r0, m = m0 + 16 * i + r, col = c0 + 16 * j0 + 8 * seg;
+            if (!full && (m >= a.M || col >= used)) continue;
+            const V8 v = *reinterpret_cast<const V8*>(lds + (room + 32 * TC * r + 16 * (seg ^ (r & (SEG - 1)))));
+            T* orow = out + (size_t)m * used + col;
+            if (full || (used & 7) == 0) {
+              *reinterpret_cast<V8*>(orow) = v;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (col + e < used) orow[e] = v[e];
+            }
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int m = m0 + 16 * i + lq;
+        if (m >= a.M) continue;
+        const float zs = *reinterpret_cast<const float*>(lds + (zscale + 64 * i + 4 * lq));
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int col = c0 + 16 * j + 4 * g;
+          const f32x4 bs = *reinterpret_cast<const f32x4*>(lds + (wscale + 64 * j + 16 * g));
+          float y[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[r] = finish<T, SIG>(acc[j][i][r], zs * bs[r]);
+          T* orow = out + (size_t)m * used + col;
+          if ((used & 3) == 0 && col < used) {
+            *reinterpret_cast<float4*>(orow) = make_float4(y[0], y[1], y[2], y[3]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (col + r < used) orow[r] = y[r];
+          }
+        }
+      }
+    }
+  };
+  // the logistic block's outputs apart: as a choice an output, its instructions run for all (32767 tokens of 768: 96 us
+  // and 86); and a whole tile without a test an output
+  if (nb == a.sig_block) {
+    put(std::true_type{}, std::false_type{});
+    return 0;
+  }
+  if ((used & 7) == 0 && m0 + 16 * TM <= a.M && c0 + 16 * TN <= used) {
+    put(std::false_type{}, std::true_type{});
+    return sizeof(T) == 2 ? kStores : 0;
+  }
+  put(std::false_type{}, std::false_type{});
+  return 0;
+}
+
+// The products of one stage of 128 inputs: TM x TN tiles from a wave's rows of both operands in LDS. Row r's 16-byte
+// segment s is at s ^ 2 ((r >> 1) & 3), so that a fragment read (lanes 0-7 with 16-23: rows 0-7, two segments each)
+// meets every bank once.
+__device__ __forceinline__ int swizzle(int row) { return 2 * ((row >> 1) & 3); }
+template <int TM, int TN>
+__device__ __forceinline__ void stage_products(const int8_t* sz, const int8_t* sw, int zrow, int wrow,
+                                               i32x4 (&acc)[TN][TM]) {
+  const int l = threadIdx.x & 63, lq = l & 15, g = l >> 4;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    i32x4 zf[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int row = zrow + 16 * i + lq;
+      zf[i] = *reinterpret_cast<const i32x4*>(sz + row * kBK + 16 * ((4 * s + g) ^ swizzle(row)));
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int row = wrow + 16 * j + lq;
+      const i32x4 f = *reinterpret_cast<const i32x4*>(sw + row * kBK + 16 * ((4 * s + g) ^ swizzle(row)));
+#pragma unroll
+      for (int i = 0; i < TM; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, zf[i], acc[j][i], 0, 0, 0);
+    }
+  }
+}
+// Their order, behind LOADS direct loads: the fragments of the second half are read while the first half's products
+// run, and the wait for the loads stays behind the products.
+template <int TM, int TN, int LOADS>
+__device__ __forceinline__ void stage_order() {
+  constexpr int AHEAD = TN < 4 ? TN : 4, EACH = (TM + 2 * TN - AHEAD + TN - 1) / TN;
+  if constexpr (LOADS > 0) __builtin_amdgcn_sched_group_barrier(0x10, LOADS, 0);
+  __builtin_amdgcn_sched_group_barrier(0x100, TM + AHEAD, 0);
+#pragma unroll
+  for (int u = 0; u < 2 * TN; ++u) {
+    __builtin_amdgcn_sched_group_barrier(0x8, TM, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Direct loads of stages into LDS: instruction j of wave w fills rows 8 (w + 8 j) .. + 7 of a stage, 128 bytes each;
+// lane l brings row l / 8's logical segment (l % 8) ^ swizzle(row).
+template <int NL>
+struct Loader {
+  unsigned off[NL];  // the scalar offset holds the stage only: it stays below every resource's size
+  int w, seg, d;
+  __device__ __forceinline__ Loader(int w_, int l, int d_) : w(w_), d(d_) {
+    const int row = l >> 3;
+    seg = (l & 7) ^ swizzle(row);
+#pragma unroll
+    for (int j = 0; j < NL; ++j) off[j] = (unsigned)(8 * (w + 8 * j) + row) * (unsigned)d + 16u * (unsigned)seg;
+  }
+  // inputs past d (a multiple of 16, so whole segments), and whole stages past the last, are zeros
+  __device__ __forceinline__ void rows(__amdgpu_buffer_rsrc_t r, int st, int stages, int8_t* to) const {
+    const bool in = st * kBK + 16 * seg < d;
     const unsigned so = (unsigned)(min(st, stages - 1) * kBK);
 #pragma unroll
-    for (int j = 0; j < NL; ++j) buffer_load_lds16(rz, dz + (w + NW * j) * 1024, in ? off[j] : kOutside, so);
+    for (int j = 0; j < NL; ++j) buffer_load_lds16(r, to + (w + 8 * j) * 1024, in ? off[j] : kOutside, so);
+  }
+};
+
+// A tile's place: its block, first row and first column; false past the last.
+struct Place {
+  int nb, m0, c0;
+};
+// Tiles are numbered in bands of kBand row tiles, down a band's rows before the next column tile: tiles of adjacent
+// numbers share rows of z and columns of the weights in an XCD's L2.
+template <int BM, int BN>
+__device__ __forceinline__ bool place_of(const Blocks& blk, int tile, int ctiles, int mtiles, Place& p) {
+  const int top = tile / (kBand * ctiles) * kBand, in_band = tile - top * ctiles, rows = min(kBand, mtiles - top);
+  if (rows <= 0) return false;
+  const int ct = in_band / rows;
+  if (ct >= ctiles) return false;
+  p.nb = block_of(blk, ct);
+  p.m0 = (top + in_band - ct * rows) * BM;
+  p.c0 = (ct - blk.start[p.nb]) * BN;
+  return true;
+}
+
+// Tiles of 256 x 256, eight waves of 64 tokens x 128 columns, a workgroup a CU that takes tiles until none is left: the
+// next tile's first two stages load under the last products and the outputs.
+template <typename T>
+__global__ __launch_bounds__(512, 1) void project_int8_kernel(const Args a, const Blocks blk, int ctiles, int mtiles,
+                                                             int tiles) {
+  constexpr int BM = 256, BN = 256, TM = 4, TN = 8, NL = 4;
+  // Two stages of [rows][128 inputs] of each operand, as separate variables: the compiler tells the direct loads into
+  // one from the reads of the other. It would wait for all of them at an access of a variable that none fills; so the
+  // scales ([tile's parity][tokens, columns]: one is written while the last tile's is read) and the waves' room for
+  // their outputs lie behind the first stage, whose loads have always arrived by then.
+  constexpr int kScale = BM * kBK, kRoom = sizeof(T) == 2 ? 2048 : 0;
+  __shared__ __align__(16) int8_t sZ0[kScale + 4096 + 8 * kRoom], sZ1[BM * kBK];
+  __shared__ __align__(16) int8_t sW0[BN * kBK], sW1[BN * kBK];
+
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
+  const int wm = w & 3, wn = w >> 2, d = a.d, stages = (d + kBK - 1) / kBK;
+  // XCD x (workgroups x, x + 8, ..) takes the x-th eighth of the tiles, its workgroups adjacent ones at a time; the
+  // grid is whole rounds over the 8 XCDs
+  const int xcd = blockIdx.x & 7, lane_wg = blockIdx.x >> 3, each = gridDim.x >> 3, share = (tiles + 7) >> 3;
+  int at = lane_wg;
+  Place p{}, next{};
+  auto place = [&](Place& q) {
+    const bool more = at < share && place_of<BM, BN>(blk, xcd * share + at, ctiles, mtiles, q);
+    at += each;
+    return more;
+  };
+  if (!place(p)) return;
+
+  const Loader<NL> load(w, l, d);
+  __amdgpu_buffer_rsrc_t rz, rw;  // of the rows of the tile being loaded: rows past the operands' ends read zeros
+  auto aim = [&](const Place& q, bool more) {
+    rz = rows_rsrc(a.z + (size_t)q.m0 * d, more ? min(BM, a.M - q.m0) : 0, d);
+    rw = rows_rsrc(a.wt + ((size_t)q.nb * a.cols + q.c0) * d, more ? min(BN, a.cols - q.c0) : 0, d);
+  };
+  auto issue = [&](int st, int8_t* dz, int8_t* dw) {
+    load.rows(rz, st, stages, dz);
+    load.rows(rw, st, stages, dw);
+  };
+  // a thread's one of the tile's 512 scales
+  const int si = threadIdx.x & 255;
+  auto scale = [&](const Place& q) {
+    return threadIdx.x < 256 ? a.z_scale[min(q.m0 + si, a.M - 1)]
+                             : a.w_scale[(size_t)q.nb * a.cols + min(q.c0 + si, blk.used[q.nb] - 1)];
+  };
+
+  aim(p, true);
+  issue(0, sZ0, sW0);
+  float sc = scale(p);
+  arrive<0>();
+  issue(1, sZ1, sW1);
+  int stores = 0;
+  for (int parity = 0;; parity ^= 1) {
+    *reinterpret_cast<float*>(sZ0 + (kScale + 2048 * parity + 4 * threadIdx.x)) = sc;
+    const bool more = place(next);
+    if (more) sc = scale(next);
+    i32x4 acc[TN][TM];
 #pragma unroll
-    for (int j = 0; j < NL; ++j) buffer_load_lds16(rw, dw + (w + NW * j) * 1024, in ? off[j] : kOutside, so);
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
+    // Pairs of stages (the second of the last pair may be all zeros), the first one's loads arrived and the second's on
+    // their way: the products of one, a barrier behind which the other has arrived and every wave is here, and the
+    // loads into the buffers that were just read.
+    int st = 0;
+    do {  // there is always one: the compiler then knows that the scale has arrived with them
+      stage_products<TM, TN>(sZ0, sW0, 64 * wm, 128 * wn, acc);
+      stage_order<TM, TN, 0>();
+      // the loads have arrived; the last tile's stores, issued behind them, may still be on their way (memory
+      // operations retire in the order of their issue): 72 us in place of 74 for 32767 tokens of 768
+      if (stores == kStores) arrive<kStores>();
+      else arrive<0>();
+      stores = 0;
+      const bool last = st + 2 >= stages;
+      if (last) aim(next, more);
+      issue(last ? 0 : st + 2, sZ0, sW0);
+      stage_products<TM, TN>(sZ1, sW1, 64 * wm, 128 * wn, acc);
+      stage_order<TM, TN, 2 * NL>();
+      arrive<0>();
+      issue(last ? 1 : st + 3, sZ1, sW1);
+      st += 2;
+    } while (st < stages);
+    __builtin_amdgcn_sched_barrier(0);  // the stores stay behind the loads
+    if (p.c0 + 128 * wn < blk.used[p.nb])
+      stores = store_tile<T, TM, TN>(acc, a, blk, p.nb, p.m0 + 64 * wm, p.c0 + 128 * wn, sZ0,
+                                     kScale + 2048 * parity + 256 * wm, kScale + 2048 * parity + 1024 + 512 * wn,
+                                     kScale + 4096 + kRoom * w);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!more) {
+      arrive<0>();  // the loads (zeros) have landed before the LDS is another workgroup's
+      return;
+    }
+    p = next;
+  }
+}
+
+// Tiles of 128 x 128, eight waves of 64 tokens x 32 columns, three stages in LDS: for the calls that have few tiles,
+// each of which then waits for most of its loads.
+template <typename T>
+__global__ __launch_bounds__(512, 1) void project_int8_small_kernel(const Args a, const Blocks blk, int ctiles,
+                                                                    int mtiles) {
+  constexpr int BM = 128, BN = 128, TM = 4, TN = 2, NL = 2;
+  constexpr int kScale = BM * kBK;  // the tokens' and the columns' scales behind the first stage
+  __shared__ __align__(16) int8_t sZ0[kScale + 1024], sZ1[BM * kBK], sZ2[BM * kBK];
+  __shared__ __align__(16) int8_t sW0[BN * kBK], sW1[BN * kBK], sW2[BN * kBK];
+
+  Place p{};  // the grid is padded to whole XCD rounds; whole workgroups leave
+  if (!place_of<BM, BN>(blk, xcd_logical_block(blockIdx.x, gridDim.x), ctiles, mtiles, p)) return;
+  const int used = blk.used[p.nb], d = a.d, stages = (d + kBK - 1) / kBK;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
+  const int wm = w & 1, wn = w >> 1;
+
+  const __amdgpu_buffer_rsrc_t rz = rows_rsrc(a.z + (size_t)p.m0 * d, min(BM, a.M - p.m0), d);
+  const __amdgpu_buffer_rsrc_t rw = rows_rsrc(a.wt + ((size_t)p.nb * a.cols + p.c0) * d, min(BN, a.cols - p.c0), d);
+  const Loader<NL> load(w, l, d);
+  auto issue = [&](int st, int8_t* dz, int8_t* dw) {
+    load.rows(rz, st, stages, dz);
+    load.rows(rw, st, stages, dw);
   };
 
   i32x4 acc[TN][TM];
@@ -168,129 +407,34 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void project_int8_kernel(const Arg
   for (int j = 0; j < TN; ++j)
 #pragma unroll
     for (int i = 0; i < TM; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
-  // A stage: the loads of the one S - 1 ahead, into the buffers that were read a stage ago (every wave has passed the
+  // A stage: the loads of the one two ahead, into the buffers that were read a stage ago (every wave has passed the
   // barrier behind those reads); the products; then the next stage has to have arrived. Every stage issues the same
-  // number of loads (zeros past the last), so that the count of those still out, S - 2 stages', is the same too.
+  // number of loads (zeros past the last), so that the count of those still out, one stage's, is the same too.
   auto step = [&](const int8_t* sz, const int8_t* sw, int st, int8_t* dz, int8_t* dw) {
     issue(st, dz, dw);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      i32x4 zf[TM];
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int row = 16 * (TM * wm + i) + lq;
-        zf[i] = *reinterpret_cast<const i32x4*>(sz + row * kBK + 16 * ((4 * s + g) ^ kswz(row)));
-      }
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int row = 16 * (TN * wn + j) + lq;
-        const i32x4 f = *reinterpret_cast<const i32x4*>(sw + row * kBK + 16 * ((4 * s + g) ^ kswz(row)));
-#pragma unroll
-        for (int i = 0; i < TM; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, zf[i], acc[j][i], 0, 0, 0);
-      }
-    }
-    // the fragments of the second half are read while the first half's products run
-    constexpr int EACH = (TM + 2 * TN - AHEAD + TN - 1) / TN;
-    __builtin_amdgcn_sched_group_barrier(0x10, 2 * NL, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, TM + AHEAD, 0);
-#pragma unroll
-    for (int u = 0; u < 2 * TN; ++u) {
-      __builtin_amdgcn_sched_group_barrier(0x8, TM, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);  // the wait stays behind the products
-    arrive<2 * NL * (S - 2)>();
+    stage_products<TM, TN>(sz, sw, 16 * TM * wm, 16 * TN * wn, acc);
+    stage_order<TM, TN, 2 * NL>();
+    arrive<2 * NL>();
   };
-
   issue(0, sZ0, sW0);
   // the scales of the tile's tokens and columns, behind the first stage
-  for (int i = threadIdx.x; i < BM; i += 64 * NW) sScaleZ[i] = a.z_scale[min(mt * BM + i, a.M - 1)];
-  for (int i = threadIdx.x; i < BN; i += 64 * NW) sScaleW[i] = a.w_scale[(size_t)nb * a.cols + min(c0 + i, used - 1)];
-  if constexpr (S == 3) issue(1, sZ1, sW1);
-  arrive<2 * NL * (S - 2)>();
-  if constexpr (S == 2) {
-    for (int st = 0; st < stages; st += 2) {
-      step(sZ0, sW0, st + 1, sZ1, sW1);
-      if (st + 1 < stages) step(sZ1, sW1, st + 2, sZ0, sW0);
-    }
-  } else {
-    for (int st = 0; st < stages; st += 3) {
-      step(sZ0, sW0, st + 2, sZ2, sW2);
-      if (st + 1 < stages) step(sZ1, sW1, st + 3, sZ0, sW0);
-      if (st + 2 < stages) step(sZ2, sW2, st + 4, sZ1, sW1);
-    }
+  if (threadIdx.x < 256) {
+    const int i = threadIdx.x & 127;
+    const float* from = threadIdx.x < 128 ? a.z_scale + min(p.m0 + i, a.M - 1)
+                                          : a.w_scale + ((size_t)p.nb * a.cols + min(p.c0 + i, used - 1));
+    *reinterpret_cast<float*>(sZ0 + (kScale + 4 * threadIdx.x)) = *from;
   }
-  arrive<0>();  // the last loads (zeros) have landed before the buffers are used again
-  if (!live) return;
-
-  // lane (lq, g) holds columns 16 j + 4 g + r of token 16 i + lq
-  const int m0 = mt * BM + 16 * TM * wm, cw = c0 + 16 * TN * wn;
-  T* out = static_cast<T*>(blk.out[nb]);
-  float zs[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) zs[i] = sScaleZ[16 * (TM * wm + i) + lq];
-  if constexpr (sizeof(T) == 2) {
-    // through LDS (free behind the last barrier), so that whole rows leave: the wave's tile, row r's 16-byte segment
-    // s at s ^ (r % the row's segments), then as whole rows
-    typedef T V4 __attribute__((ext_vector_type(4)));
-    typedef T V8 __attribute__((ext_vector_type(8)));
-    constexpr int SEG = 2 * TN, TILE = 256 * TM * TN, PER = BM * kBK / (TILE * 2);  // PER waves' tiles a buffer
-    static_assert(PER >= 1 && 4 * PER >= NW, "the waves' tiles fit two stages");
-    int8_t* base = w / PER == 0 ? sZ0 : w / PER == 1 ? sZ1 : w / PER == 2 ? sW0 : sW1;
-    T* stile = reinterpret_cast<T*>(base) + (w % PER) * TILE;
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int c = 16 * j + 4 * g;
-      const f32x4 bs = *reinterpret_cast<const f32x4*>(sScaleW + 16 * TN * wn + c);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int row = 16 * i + lq;
-        V4 y;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[r], nb == a.sig_block);
-        *reinterpret_cast<V4*>(stile + row * (16 * TN) + 8 * ((c >> 3) ^ (row & (SEG - 1))) + (c & 7)) = y;
-      }
-    }
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the tile is in LDS (only this wave reads it)
-    const int seg = l % SEG, col = cw + 8 * seg;
-    const bool whole = (used & 7) == 0;
-#pragma unroll
-    for (int it = 0; it < 16 * TM * SEG / 64; ++it) {
-      const int row = (64 / SEG) * it + l / SEG, m = m0 + row;
-      if (m >= a.M || col >= used) continue;
-      const V8 v = *reinterpret_cast<const V8*>(stile + row * (16 * TN) + 8 * (seg ^ (row & (SEG - 1))));
-      T* orow = out + (size_t)m * used + col;
-      if (whole) {
-        *reinterpret_cast<V8*>(orow) = v;
-      } else {
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (col + r < used) orow[r] = v[r];
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int col = cw + 16 * j + 4 * g;
-      const f32x4 bs = *reinterpret_cast<const f32x4*>(sScaleW + 16 * TN * wn + 16 * j + 4 * g);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int m = m0 + 16 * i + lq;
-        if (m >= a.M) continue;
-        float y[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = finish<T>(acc[j][i][r], zs[i] * bs[r], nb == a.sig_block);
-        T* orow = out + (size_t)m * used + col;
-        if ((used & 3) == 0 && col < used) {
-          *reinterpret_cast<float4*>(orow) = make_float4(y[0], y[1], y[2], y[3]);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (col + r < used) orow[r] = y[r];
-        }
-      }
-    }
+  issue(1, sZ1, sW1);
+  arrive<2 * NL>();
+  for (int st = 0; st < stages; st += 3) {
+    step(sZ0, sW0, st + 2, sZ2, sW2);
+    if (st + 1 < stages) step(sZ1, sW1, st + 3, sZ0, sW0);
+    if (st + 2 < stages) step(sZ2, sW2, st + 4, sZ1, sW1);
   }
+  arrive<0>();  // the last loads (zeros) have landed before the LDS is another workgroup's
+  if (p.c0 + 16 * TN * wn < used)
+    store_tile<T, TM, TN>(acc, a, blk, p.nb, p.m0 + 64 * wm, p.c0 + 32 * wn, sZ0, kScale + 256 * wm,
+                          kScale + 512 + 128 * wn, 1024 * w);
 }
 
 // MT tiles of 16 tokens and NC of 16 columns, NW waves sharing the inputs.
@@ -345,7 +489,8 @@ __global__ __launch_bounds__(64 * NW) void project_int8_few_kernel(const Args a,
     int sum = 0;
 #pragma unroll
     for (int u = 0; u < NW; ++u) sum += part[u][m >> 4][m & 15][c];
-    out[(size_t)m * used + c0 + c] = finish<T>(sum, a.z_scale[m] * ws[c0 + c], nb == a.sig_block);
+    const float scale = a.z_scale[m] * ws[c0 + c];
+    out[(size_t)m * used + c0 + c] = nb == a.sig_block ? finish<T, true>(sum, scale) : finish<T, false>(sum, scale);
   }
 }
 
@@ -393,11 +538,11 @@ int project_int8(const int8_t* z, const float* z_scale, const int8_t* wt, const 
   const Args a{z, z_scale, wt, w_scale, M, d, cols, sigmoid_block};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (!few) {
-    auto run = [&](auto kern) {
-      hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(512), 0, s, a, blk, (int)tiles, mtiles, kBand);
-    };
-    if (tile == 256) run(project_int8_kernel<T, 4, 2, 4, 8, 2>);
-    else run(project_int8_kernel<T, 2, 4, 4, 2, 3>);
+    if (tile == 256)
+      hipLaunchKernelGGL(project_int8_kernel<T>, dim3((unsigned)(n < 256 ? n : 256)), dim3(512), 0, s, a, blk,
+                         (int)tiles, mtiles, (int)(tiles * mtiles));
+    else
+      hipLaunchKernelGGL(project_int8_small_kernel<T>, dim3((unsigned)n), dim3(512), 0, s, a, blk, (int)tiles, mtiles);
     return check_launch(who);
   }
   auto go = [&](auto kern, int nw) { hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(64 * nw), 0, s, a, blk); };
