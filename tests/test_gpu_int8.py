@@ -149,6 +149,14 @@ def test_the_projection_in_8_bits(m, d, used, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize(("m", "used", "sig"), [(2500, (600, 250, 9), 1), (2049, (1200, 1024), None)])
+def test_tiles_of_128_columns(m, used, sig, dtype):
+    """Between the narrow tile (up to 256 of 128 x 64) and the wide one (over 512 of 128 x 128)."""
+    z, zs, w, ws = _project_case(m, 144, used, seed=m)
+    _check_project(z, zs, w, ws, used, sig, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize(("d", "sig"), [(16, 3), (272, None), (512, 0)])
 def test_more_tiles_than_one_round_of_workgroups(d, sig, dtype):
     """67 x 6 tiles of 256 x 256: one, three and four stages, a last row tile of 104 tokens, ragged and narrow blocks."""

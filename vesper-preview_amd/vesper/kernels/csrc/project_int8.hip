@@ -13,23 +13,23 @@
 //
 // tile (many tokens): 256 tokens x 256 columns, eight waves of 64 x 128, both operands through LDS in two stages of
 // 128 inputs (whole cache lines a row), by a workgroup a CU that goes from tile to tile; or, where that makes few
-// workgroups, 128 x 128 in waves of 64 x 32 and three stages. global_load_lds_dwordx4 moves eight rows of 128 bytes an
+// workgroups, 128 x 128 or 128 x 64 in waves of 64 x 32 and three stages. global_load_lds_dwordx4 moves eight rows of 128 bytes an
 // instruction, each row's 16-byte segments XOR-swizzled so that the fragment reads meet each bank once; 16x16x64 int8
 // MFMA formed transposed (weight rows as the A operand); the second half's fragments are read during the first half's
-// products. 8192^3: 444 to 473 us among other work, 520 to 540 back to back (2.0 to 2.5 Pop/s; the clock falls under them:
-// the matrix units are busy 63 % of the cycles), a library product of the same operands 547. 32767 x 768 to 2316 columns: 72 us
-// (116 Gop, 1.6 Pop/s). One tile a workgroup needed 96: its first loads and its outputs stood alone, and the logistic
-// function, chosen an output at a time, ran for all of them (86 with that block's outputs apart; 78 from tile to
-// tile; 72 with the next tile's second stage loading under the outputs too). Stages of 64 inputs, four deep, read half
-// cache lines (117 when the present form took 94); three stages of 256 x 128: 108; outputs stored straight from the
-// accumulators, 32 bytes a row: 95 to 107.
+// products. 8192^3: 444 to 473 us among other work, 520 to 540 back to back (2.0 to 2.5 Pop/s; the clock falls under
+// them: the matrix units are busy 63 % of the cycles), a library product of the same operands 547. 32767 x 768 to 2316
+// columns: 72 us (116 Gop, 1.6 Pop/s). One tile a workgroup needed 96: its first loads and its outputs stood alone, and
+// the logistic function, chosen an output at a time, ran for all of them (86 with that block's outputs apart; 78 from
+// tile to tile; 72 with the next tile's second stage loading under the outputs too). Stages of 64 inputs, four deep,
+// read half cache lines (117 when the present form took 94); three stages of 256 x 128: 108; outputs stored straight
+// from the accumulators, 32 bytes a row: 95 to 107.
 //
 // few (up to 64 tokens, a decode step): bound by reading the weights once. A workgroup takes 16 columns and
 // all the tokens; its waves share the inputs, each reading whole 128-byte lines of 16 weight rows straight
 // into the MFMA operand's registers; the waves' int32 sums are joined through LDS. Past 16 tokens the tokens'
 // own reads count (from L2, by every workgroup): 32 columns a workgroup where there are enough (64 tokens, 8192 to
-// 8192: 40 us with 16 columns, 31 with 32; 64 x 512 to 1544: 4.0 and 4.7), and eight waves in place of four (64 x
-// 512: 4.5 -> 4.0; with up to 16 tokens four are as good or better: 16 x 8192 to 8192 17.0 us, 3.9 TB/s of
+// 8192: 40 us with 16 columns, 31 with 32, now 26; 64 x 512 to 1544: 4.0 and 4.7), and eight waves in place of four
+// (64 x 512: 4.5 -> 4.0; with up to 16 tokens four are as good or better: 16 x 8192 to 8192 16.7 us, 4.0 TB/s of
 // weights, against 17.8; two or four steps' loads in flight a wave gave nothing).
 #include <type_traits>
 
@@ -244,9 +244,9 @@ __device__ __forceinline__ void stage_order() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// Direct loads of stages into LDS: instruction j of wave w fills rows 8 (w + 8 j) .. + 7 of a stage, 128 bytes each;
-// lane l brings row l / 8's logical segment (l % 8) ^ swizzle(row).
-template <int NL>
+// Direct loads of stages into LDS by NW waves: instruction j of wave w fills rows 8 (w + NW j) .. + 7 of a stage, 128
+// bytes each; lane l brings row l / 8's logical segment (l % 8) ^ swizzle(row).
+template <int NL, int NW>
 struct Loader {
   unsigned off[NL];  // the scalar offset holds the stage only: it stays below every resource's size
   int w, seg, d;
@@ -254,14 +254,16 @@ struct Loader {
     const int row = l >> 3;
     seg = (l & 7) ^ swizzle(row);
 #pragma unroll
-    for (int j = 0; j < NL; ++j) off[j] = (unsigned)(8 * (w + 8 * j) + row) * (unsigned)d + 16u * (unsigned)seg;
+    for (int j = 0; j < NL; ++j) off[j] = (unsigned)(8 * (w + NW * j) + row) * (unsigned)d + 16u * (unsigned)seg;
   }
   // inputs past d (a multiple of 16, so whole segments), and whole stages past the last, are zeros
+  template <int ROWS>
   __device__ __forceinline__ void rows(__amdgpu_buffer_rsrc_t r, int st, int stages, int8_t* to) const {
+    static_assert(ROWS % (8 * NW) == 0 && ROWS / (8 * NW) <= NL, "whole load instructions");
     const bool in = st * kBK + 16 * seg < d;
     const unsigned so = (unsigned)(min(st, stages - 1) * kBK);
 #pragma unroll
-    for (int j = 0; j < NL; ++j) buffer_load_lds16(r, to + (w + 8 * j) * 1024, in ? off[j] : kOutside, so);
+    for (int j = 0; j < ROWS / (8 * NW); ++j) buffer_load_lds16(r, to + (w + NW * j) * 1024, in ? off[j] : kOutside, so);
   }
 };
 
@@ -311,15 +313,15 @@ __global__ __launch_bounds__(512, 1) void project_int8_kernel(const Args a, cons
   };
   if (!place(p)) return;
 
-  const Loader<NL> load(w, l, d);
+  const Loader<NL, 8> load(w, l, d);
   __amdgpu_buffer_rsrc_t rz, rw;  // of the rows of the tile being loaded: rows past the operands' ends read zeros
   auto aim = [&](const Place& q, bool more) {
     rz = rows_rsrc(a.z + (size_t)q.m0 * d, more ? min(BM, a.M - q.m0) : 0, d);
     rw = rows_rsrc(a.wt + ((size_t)q.nb * a.cols + q.c0) * d, more ? min(BN, a.cols - q.c0) : 0, d);
   };
   auto issue = [&](int st, int8_t* dz, int8_t* dw) {
-    load.rows(rz, st, stages, dz);
-    load.rows(rw, st, stages, dw);
+    load.template rows<BM>(rz, st, stages, dz);
+    load.template rows<BN>(rw, st, stages, dw);
   };
   // a thread's one of the tile's 512 scales
   const int si = threadIdx.x & 255;
@@ -378,14 +380,16 @@ __global__ __launch_bounds__(512, 1) void project_int8_kernel(const Args a, cons
   }
 }
 
-// Tiles of 128 x 128, eight waves of 64 tokens x 32 columns, three stages in LDS: for the calls that have few tiles,
-// each of which then waits for most of its loads.
-template <typename T>
-__global__ __launch_bounds__(512, 1) void project_int8_small_kernel(const Args a, const Blocks blk, int ctiles,
-                                                                    int mtiles) {
-  constexpr int BM = 128, BN = 128, TM = 4, TN = 2, NL = 2;
+// Tiles of 128 x 32 WN, 2 WN waves of 64 tokens x 32 columns, three stages in LDS: for the calls that have few tiles,
+// each of which then waits for most of its loads. Bound by LDS (at 128 x 128 the fragments' reads take 768 cycles a stage
+// and the loads' writes 256, the products 512), so with few of them narrower tiles on more CUs are faster.
+template <typename T, int WN>
+__global__ __launch_bounds__(128 * WN, WN == 4 ? 1 : 2) void project_int8_small_kernel(const Args a, const Blocks blk,
+                                                                                     int ctiles, int mtiles) {
+  constexpr int NW = 2 * WN, BM = 128, BN = 32 * WN, TM = 4, TN = 2, NL = BM / (8 * NW);
+  constexpr int PER = NL + BN / (8 * NW);  // a wave's loads of a stage
   constexpr int kScale = BM * kBK;  // the tokens' and the columns' scales behind the first stage
-  __shared__ __align__(16) int8_t sZ0[kScale + 1024], sZ1[BM * kBK], sZ2[BM * kBK];
+  __shared__ __align__(16) int8_t sZ0[kScale + 4 * (BM + BN)], sZ1[BM * kBK], sZ2[BM * kBK];
   __shared__ __align__(16) int8_t sW0[BN * kBK], sW1[BN * kBK], sW2[BN * kBK];
 
   Place p{};  // the grid is padded to whole XCD rounds; whole workgroups leave
@@ -396,10 +400,10 @@ __global__ __launch_bounds__(512, 1) void project_int8_small_kernel(const Args a
 
   const __amdgpu_buffer_rsrc_t rz = rows_rsrc(a.z + (size_t)p.m0 * d, min(BM, a.M - p.m0), d);
   const __amdgpu_buffer_rsrc_t rw = rows_rsrc(a.wt + ((size_t)p.nb * a.cols + p.c0) * d, min(BN, a.cols - p.c0), d);
-  const Loader<NL> load(w, l, d);
+  const Loader<NL, NW> load(w, l, d);
   auto issue = [&](int st, int8_t* dz, int8_t* dw) {
-    load.rows(rz, st, stages, dz);
-    load.rows(rw, st, stages, dw);
+    load.template rows<BM>(rz, st, stages, dz);
+    load.template rows<BN>(rw, st, stages, dw);
   };
 
   i32x4 acc[TN][TM];
@@ -413,19 +417,19 @@ __global__ __launch_bounds__(512, 1) void project_int8_small_kernel(const Args a
   auto step = [&](const int8_t* sz, const int8_t* sw, int st, int8_t* dz, int8_t* dw) {
     issue(st, dz, dw);
     stage_products<TM, TN>(sz, sw, 16 * TM * wm, 16 * TN * wn, acc);
-    stage_order<TM, TN, 2 * NL>();
-    arrive<2 * NL>();
+    stage_order<TM, TN, PER>();
+    arrive<PER>();
   };
   issue(0, sZ0, sW0);
   // the scales of the tile's tokens and columns, behind the first stage
-  if (threadIdx.x < 256) {
-    const int i = threadIdx.x & 127;
-    const float* from = threadIdx.x < 128 ? a.z_scale + min(p.m0 + i, a.M - 1)
-                                          : a.w_scale + ((size_t)p.nb * a.cols + min(p.c0 + i, used - 1));
-    *reinterpret_cast<float*>(sZ0 + (kScale + 4 * threadIdx.x)) = *from;
+  if (threadIdx.x < BM + BN) {
+    const int i = threadIdx.x;
+    const float* from = i < BM ? a.z_scale + min(p.m0 + i, a.M - 1)
+                               : a.w_scale + ((size_t)p.nb * a.cols + min(p.c0 + i - BM, used - 1));
+    *reinterpret_cast<float*>(sZ0 + (kScale + 4 * i)) = *from;
   }
   issue(1, sZ1, sW1);
-  arrive<2 * NL>();
+  arrive<PER>();
   for (int st = 0; st < stages; st += 3) {
     step(sZ0, sW0, st + 2, sZ2, sW2);
     if (st + 1 < stages) step(sZ1, sW1, st + 3, sZ0, sW0);
@@ -454,13 +458,21 @@ __global__ __launch_bounds__(64 * NW) void project_int8_few_kernel(const Args a,
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[c][i] = i32x4{0, 0, 0, 0};
   // a step: 128 inputs of 16 weight rows a tile, lane (lq, g) the 32 bytes at 32 g of row lq
-  const unsigned row = (unsigned)lq * (unsigned)d + 32u * (unsigned)g, tile = 16u * (unsigned)d;
-  for (int k0 = 128 * w; k0 < d; k0 += 128 * NW) {
+  const unsigned row = (unsigned)lq * (unsigned)d + 16u * (unsigned)g, tile = 16u * (unsigned)d;
+  const int steps = (d + 127) / 128;
+  // Each workgroup begins at a step of its own (the sums are exact, so their order is free): from the first step on
+  // together, all of them read the same few lines of every row, which lie in few of the caches' and memory's channels
+  // (32 tokens, 8192 to 8192: 28 us together, 18.4 so; 64 tokens 29 and 26; 1 token, 4096 to 6144: 8.4 and 7.5).
+  int at = (w + (int)blockIdx.x) % steps;
+  for (int n = w; n < steps; n += NW) {
+    const int k0 = 128 * at;
+    at += NW;
+    if (at >= steps) at -= steps;
     i32x4 f[2][NC], zf[2][MT];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int k = k0 + 16 * h;
-      const unsigned o = k + 32 * g < d ? row + (unsigned)k : kOutside;  // d is a multiple of 16
+      const int k = k0 + 64 * h;
+      const unsigned o = k + 16 * g < d ? row + (unsigned)k : kOutside;  // d is a multiple of 16
 #pragma unroll
       for (int c = 0; c < NC; ++c) f[h][c] = load16(rw, o + tile * (unsigned)c);
 #pragma unroll
@@ -503,16 +515,22 @@ int project_int8(const int8_t* z, const float* z_scale, const int8_t* wt, const 
     return fail(ERR_ARG, "%s: width %d (a multiple of 16 in 16..16384)", who, d);
   if (M < 0 || cols < 1) return fail(ERR_ARG, "%s: bad sizes M=%d cols=%d", who, M, cols);
   if (sigmoid_block < -1 || sigmoid_block >= nblk) return fail(ERR_ARG, "%s: sigmoid block %d", who, sigmoid_block);
-  // the wide tile where the small one's workgroups would go around the 256 CUs more than twice
+  // the wide tile where the small one's workgroups would go around the 256 CUs more than twice, the narrow one where
+  // the narrow one's do not fill them once (128 x 8192 to 8192: 26.5 us, 128 columns 30.8; 256 x 4096 to 6144: 16.2 and
+  // 18.2; 1000 x 2048 to 2048: 10.7 and 11.8; but 512 x 8192 to 8192, 512 narrow ones: 41 and 37)
   const bool few = M <= kFewTokens;
-  int64_t small = 0;
-  for (int j = 0; j < nblk; ++j) small += ((int64_t)(used_in[j] > 0 ? used_in[j] : 0) + 127) / 128;
-  const int tile = small * (((int64_t)M + 127) / 128) > 512 ? 256 : 128;
+  int64_t small = 0, half = 0;
+  for (int j = 0; j < nblk; ++j) {
+    small += ((int64_t)(used_in[j] > 0 ? used_in[j] : 0) + 127) / 128;
+    half += ((int64_t)(used_in[j] > 0 ? used_in[j] : 0) + 63) / 64;
+  }
+  const int64_t mt = ((int64_t)M + 127) / 128;
+  const int tile = small * mt > 512 ? 256 : 128, tile_cols = tile == 256 ? 256 : half * mt <= 256 ? 64 : 128;
   // the few-token kernel's columns: 32 where 16 would make more than a workgroup a CU (each reads all the tokens)
   int64_t narrow = 0;
   for (int j = 0; j < nblk; ++j) narrow += ((int64_t)(used_in[j] > 0 ? used_in[j] : 0) + 15) / 16;
   const int few_cols = M > 16 && narrow > 256 ? 32 : 16;
-  const int width = few ? few_cols : tile;
+  const int width = few ? few_cols : tile_cols;
   Blocks blk{};
   blk.nblk = nblk;
   int64_t tiles = 0;
@@ -541,8 +559,10 @@ int project_int8(const int8_t* z, const float* z_scale, const int8_t* wt, const 
     if (tile == 256)
       hipLaunchKernelGGL(project_int8_kernel<T>, dim3((unsigned)(n < 256 ? n : 256)), dim3(512), 0, s, a, blk,
                          (int)tiles, mtiles, (int)(tiles * mtiles));
+    else if (tile_cols == 128)
+      hipLaunchKernelGGL((project_int8_small_kernel<T, 4>), dim3((unsigned)n), dim3(512), 0, s, a, blk, (int)tiles, mtiles);
     else
-      hipLaunchKernelGGL(project_int8_small_kernel<T>, dim3((unsigned)n), dim3(512), 0, s, a, blk, (int)tiles, mtiles);
+      hipLaunchKernelGGL((project_int8_small_kernel<T, 2>), dim3((unsigned)n), dim3(256), 0, s, a, blk, (int)tiles, mtiles);
     return check_launch(who);
   }
   auto go = [&](auto kern, int nw) { hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(64 * nw), 0, s, a, blk); };
