@@ -17,7 +17,7 @@
 // instruction, each row's 16-byte segments XOR-swizzled so that the fragment reads meet each bank once; 16x16x64 int8
 // MFMA formed transposed (weight rows as the A operand); the second half's fragments are read during the first half's
 // products. 8192^3: 444 to 473 us among other work, 520 to 540 back to back (2.0 to 2.5 Pop/s; the clock falls under
-// them: the matrix units are busy 63 % of the cycles), a library product of the same operands 547. 32767 x 768 to 2316
+// them: the matrix units are busy 69 % of the cycles), a library product of the same operands 547. 32767 x 768 to 2316
 // columns: 72 us (116 Gop, 1.6 Pop/s). One tile a workgroup needed 96: its first loads and its outputs stood alone, and
 // the logistic function, chosen an output at a time, ran for all of them (86 with that block's outputs apart; 78 from
 // tile to tile; 72 with the next tile's second stage loading under the outputs too). Stages of 64 inputs, four deep,
