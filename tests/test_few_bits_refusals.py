@@ -181,3 +181,43 @@ def test_the_oracles_quantiser_on_a_row_done_by_hand():
     packed = torch.tensor([[0x20, 0xF3]], dtype=torch.uint8)
     assert torch.equal(unpack_rows(packed), codes)
     assert ring_values(packed, torch.tensor([[1.0, -1.0]])).tolist() == [[-1, 1, 2, 14]]
+
+
+TOO_MANY = 2**32 + 8  # cut to 32 bits these are 8: sizes that every other check would take
+
+
+def _huge_ring(b, w, device="cpu"):
+    """A ring of ``b`` rows and ``w`` slots of one head of eight features, broadcast: nothing of that size is allocated."""
+    from vesper.kernels.ring_quant import QuantRingKVCache
+
+    one = lambda *shape, dtype: torch.zeros(1, dtype=dtype, device=device).expand(*shape)  # noqa: E731
+    return QuantRingKVCache(one(b, 1, w, 4, dtype=torch.uint8), one(b, 1, w, 4, dtype=torch.uint8), one(b, 1, w, 2, dtype=BF16),
+                            one(b, 1, w, 2, dtype=BF16), one(b, w, dtype=torch.long), one(b, w, dtype=torch.bool), w)
+
+
+@pytest.mark.parametrize(("b", "n", "w"), [(1, TOO_MANY, 4), (TOO_MANY, 1, 4), (1, 3, TOO_MANY), (2**31, 1, 4), (1, 2**31, 4)])
+def test_ring_sizes_past_32_bits_are_refused(b, n, w):
+    """The kernels count rows, tokens and slots in 32 bits: a size past them is refused, never cut."""
+    from vesper.contracts import ContractError
+    from vesper.kernels.ring_quant import quant_ring_attention, quant_ring_read, quant_ring_write
+
+    tokens, pos = torch.zeros(1, dtype=BF16).expand(b, n, 1, 8), torch.zeros(1, dtype=torch.long).expand(b, n)
+    ring = _huge_ring(b, w)
+    with pytest.raises(ContractError, match="at most 2147483647"):
+        quant_ring_write(tokens, tokens, pos, ring)
+    with pytest.raises(ContractError, match="at most 2147483647"):
+        quant_ring_read(ring, pos)
+    if n != 1 and w == 4:
+        return  # a step has one token a row
+    token = tokens[:, :1]
+    with pytest.raises(ContractError, match="at most 2147483647"):
+        quant_ring_attention(token, token, token, pos[:, :1], ring)
+
+
+def test_an_empty_ring_of_too_many_slots_is_refused():
+    from vesper.contracts import ContractError
+    from vesper.kernels.ring_quant import quant_ring_empty
+
+    for b, w in ((1, TOO_MANY), (TOO_MANY, 4)):
+        with pytest.raises(ContractError, match="at most 2147483647"):
+            quant_ring_empty(b, 1, 8, w, BF16, torch.device("meta"))

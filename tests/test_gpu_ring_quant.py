@@ -542,3 +542,18 @@ def test_calls_of_no_rows_and_no_tokens():
     x = torch.zeros(0, 1, 2, 16, dtype=BF16, device=GPU)
     o, _ = quant_ring_attention(x, x, x, torch.zeros(0, 1, dtype=torch.long, device=GPU), _ring(0, 2, 16, 8, BF16))
     assert o.shape == (0, 1, 2, 16)
+
+
+def test_token_counts_past_32_bits_are_refused():
+    """2^32 + 8 broadcast tokens, which cut to 32 bits would be 8, against a ring that the kernels take as it is."""
+    from vesper.contracts import ContractError
+    from vesper.kernels.ring_quant import quant_ring_read, quant_ring_write
+
+    n = 2**32 + 8
+    tokens, pos = torch.zeros(1, dtype=BF16, device=GPU).expand(1, n, 1, 8), torch.zeros(1, dtype=torch.long, device=GPU).expand(1, n)
+    ring = _ring(1, 1, 8, 4, BF16)
+    with pytest.raises(ContractError, match="at most 2147483647"):
+        quant_ring_write(tokens, tokens, pos, ring)
+    with pytest.raises(ContractError, match="at most 2147483647"):
+        quant_ring_read(ring, pos)
+    assert not bool(ring.valid.any())

@@ -34,6 +34,7 @@ from vesper.kernels import _lib
 from vesper.kernels.ring_attn import MAX_GROUP, MAX_HEAD_DIM, _aligned
 
 MAX_KV_HEADS = 16384  # a workgroup's tokens are addressed by 32-bit offsets
+MAX_COUNT = 2**31 - 1  # rows, tokens a row and slots: the C entries count each in 32 bits
 _SUFFIX = {torch.bfloat16: "bf16", torch.float16: "f16"}
 
 
@@ -63,10 +64,11 @@ def quant_ring_empty(b: int, hkv: int, dk: int, window: int, dtype: torch.dtype,
     the tokens (bfloat16 or float16).
 
     Raises:
-        ValueError: if ``window`` is below 1; ContractError: on a head width or dtype outside the contract.
+        ValueError: if ``window`` is below 1; ContractError: on a size, head width or dtype outside the contract.
     """
     if window < 1:
         raise ValueError(f"window must be at least 1, got {window}")
+    _check_counts({"b": b, "w": window})
     _check_width(dk)
     if dtype not in _SUFFIX:
         raise ContractError(f"the ring's dtype must be bfloat16 or float16, got {dtype}")
@@ -87,8 +89,14 @@ def _check_width(dk: int) -> None:
         raise ContractError(f"head dimension {dk}: the kernels take multiples of 8 up to {MAX_HEAD_DIM}")
 
 
+def _check_counts(dims: Dims) -> None:
+    for name, what in (("b", "rows"), ("n", "tokens a row"), ("w", "slots")):
+        if dims.get(name, 0) > MAX_COUNT:
+            raise ContractError(f"{dims[name]} {what}, the kernels take at most {MAX_COUNT}")
+
+
 def _check_ring(cache: QuantRingKVCache, dims: Dims) -> torch.dtype:
-    """The ring's shapes and dtypes under ``dims``; its tokens' dtype."""
+    """The ring's shapes, sizes and dtypes under ``dims``; its tokens' dtype."""
     dims["w"], dims["pair"] = cache.window, 2
     check_shape("cache.k", cache.k, ("b", "hkv", "w", "half"), dims, torch.uint8)
     check_shape("cache.v", cache.v, ("b", "hkv", "w", "half"), dims, torch.uint8)
@@ -96,6 +104,7 @@ def _check_ring(cache: QuantRingKVCache, dims: Dims) -> torch.dtype:
     check_shape("cache.v_scale", cache.v_scale, ("b", "hkv", "w", "pair"), dims, cache.k_scale.dtype)
     check_shape("cache.pos", cache.pos, ("b", "w"), dims, torch.long)
     check_shape("cache.valid", cache.valid, ("b", "w"), dims, torch.bool)
+    _check_counts(dims)
     dtype = cache.k_scale.dtype
     _refuse_grad(cache.k_scale, cache.v_scale)
     if dtype not in _SUFFIX:
@@ -135,7 +144,8 @@ def _ring_as_is(cache: QuantRingKVCache, b: int, hkv: int, dk: int, dtype: torch
             and pos.is_contiguous() and valid.is_contiguous()
             and (k.data_ptr() | v.data_ptr() | ks.data_ptr() | vs.data_ptr()) & 3 == 0
             and not (ks.requires_grad or vs.requires_grad)
-            and w >= 1 and dk & 7 == 0 and 8 <= dk <= MAX_HEAD_DIM and 1 <= hkv <= MAX_KV_HEADS)
+            and 1 <= w <= MAX_COUNT and b <= MAX_COUNT
+            and dk & 7 == 0 and 8 <= dk <= MAX_HEAD_DIM and 1 <= hkv <= MAX_KV_HEADS)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -182,7 +192,7 @@ def quant_ring_write(k: Tensor, v: Tensor, pos: Tensor, cache: QuantRingKVCache,
         ContractError: on shapes, dtypes, devices or values outside that contract.
     """
     shape, dtype, device, w = k.shape, k.dtype, k.get_device(), cache.window
-    as_is = (len(shape) == 4 and v.shape == shape and pos.shape == shape[:2] and v.dtype is dtype
+    as_is = (len(shape) == 4 and v.shape == shape and shape[1] <= MAX_COUNT and pos.shape == shape[:2] and v.dtype is dtype
              and pos.dtype is torch.int64 and dtype in _SUFFIX and device >= 0 and v.get_device() == device
              and pos.get_device() == device and not (k.requires_grad or v.requires_grad)
              and _ring_as_is(cache, shape[0], shape[2], shape[3], dtype, device))
@@ -240,8 +250,9 @@ def quant_ring_read(cache: QuantRingKVCache, pos: Tensor) -> tuple[Tensor, Tenso
     """
     dtype, shape, device = cache.k_scale.dtype, cache.k.shape, pos.get_device()
     held = cache
-    if not (len(shape) == 4 and pos.dim() == 2 and pos.shape[0] == shape[0] and pos.dtype is torch.int64 and dtype in _SUFFIX
-            and device >= 0 and _ring_as_is(cache, shape[0], shape[1], 2 * shape[3], dtype, device)):
+    if not (len(shape) == 4 and pos.dim() == 2 and pos.shape[0] == shape[0] and pos.shape[1] <= MAX_COUNT
+            and pos.dtype is torch.int64 and dtype in _SUFFIX and device >= 0
+            and _ring_as_is(cache, shape[0], shape[1], 2 * shape[3], dtype, device)):
         dims: Dims = {}
         check_shape("pos", pos, ("b", "n"), dims, torch.long)
         _check_ring(cache, dims)
