@@ -221,3 +221,14 @@ def test_an_empty_ring_of_too_many_slots_is_refused():
     for b, w in ((1, TOO_MANY), (TOO_MANY, 4)):
         with pytest.raises(ContractError, match="at most 2147483647"):
             quant_ring_empty(b, 1, 8, w, BF16, torch.device("meta"))
+
+
+def test_weights_of_too_many_columns_are_refused():
+    """A column count cut to 32 bits would put every block after the first in the wrong place."""
+    from vesper.contracts import ContractError
+    from vesper.kernels.norm import projection_int8
+
+    z, one = torch.zeros(2, 16, dtype=torch.int8), torch.ones(1)
+    w = torch.zeros(1, dtype=torch.int8).expand(2, TOO_MANY, 16)
+    with pytest.raises(ContractError, match="4294967304 columns, the kernel takes at most 2147483647"):
+        projection_int8(z, one.expand(2), w, one.expand(2, TOO_MANY), (8, 8))

@@ -211,7 +211,7 @@ def projection(z: Tensor, weights_t: Tensor, used: tuple[int, ...], *,
     return outs
 
 
-MAX_ROWS = 2**31 - 1  # of the 8-bit operators: their C entries count rows in 32 bits
+MAX_ROWS = 2**31 - 1  # of the 8-bit operators: their C entries count rows and a weight's columns in 32 bits
 _INT8_SUFFIX = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
 # x and residual dtypes of rms_norm_int8
 _NORM_INT8 = {(torch.float32, torch.bfloat16): "f32_bf16", (torch.float32, torch.float16): "f32_f16",
@@ -352,7 +352,7 @@ def projection_int8(z: Tensor, z_scale: Tensor, weights_q: Tensor, weights_scale
             and weights_scale.shape == wshape[:2] and z_scale.dtype is torch.float32
             and weights_scale.dtype is torch.float32 and device >= 0 and z_scale.get_device() == device
             and weights_q.get_device() == device and weights_scale.get_device() == device
-            and min(used) >= 1 and max(used) <= wshape[1] and zshape[1] & 15 == 0 and 16 <= zshape[1] <= 16384
+            and min(used) >= 1 and max(used) <= wshape[1] <= MAX_ROWS and zshape[1] & 15 == 0 and 16 <= zshape[1] <= 16384
             and suffix is not None and (sigmoid_block is None or 0 <= sigmoid_block < p)
             and not (z_scale.requires_grad or weights_scale.requires_grad)):
         _check_projection_int8(z, z_scale, weights_q, weights_scale, used, sigmoid_block, dtype)
@@ -370,6 +370,8 @@ def projection_int8(z: Tensor, z_scale: Tensor, weights_q: Tensor, weights_scale
 def _check_projection_int8(z: Tensor, z_scale: Tensor, weights_q: Tensor, weights_scale: Tensor, used: tuple[int, ...],
                            sigmoid_block: int | None, dtype: torch.dtype) -> None:
     """Raises for what ``projection_int8`` does not take."""
+    if weights_q.dim() == 3 and weights_q.shape[1] > MAX_ROWS:
+        raise ContractError(f"weights_q: {weights_q.shape[1]} columns, the kernel takes at most {MAX_ROWS}")
     if z.dim() != 2 or z.dtype != torch.int8 or z.device.type != "cuda":
         raise ContractError(f"z: int8 [M, d] on CUDA, got {tuple(z.shape)} {z.dtype} on {z.device}")
     m, d = z.shape
