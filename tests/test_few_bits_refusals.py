@@ -232,3 +232,13 @@ def test_weights_of_too_many_columns_are_refused():
     w = torch.zeros(1, dtype=torch.int8).expand(2, TOO_MANY, 16)
     with pytest.raises(ContractError, match="4294967304 columns, the kernel takes at most 2147483647"):
         projection_int8(z, one.expand(2), w, one.expand(2, TOO_MANY), (8, 8))
+
+
+def test_a_few_token_launch_of_2_to_the_32_threads_is_refused():
+    """2^28 columns in workgroups of 16 columns and 256 threads (one token), or of 32 and 512 (20 tokens): 2^32 threads."""
+    from vesper.kernels import _lib
+
+    lib, one = _lib.library(), 0x1000  # never read: the call is refused first
+    for m, groups in ((1, 1 << 24), (20, 1 << 23)):
+        status = lib.vsp_project_int8_bf16(one, one, one, one, 1, 1 << 28, 16, m, 1 << 28, 1, 1, 1, one, None, None, None, -1, None)
+        assert status == 2 and f"{groups} workgroups" in lib.vsp_last_error().decode()

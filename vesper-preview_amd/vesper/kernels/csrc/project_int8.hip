@@ -565,6 +565,8 @@ int project_int8(const int8_t* z, const float* z_scale, const int8_t* wt, const 
       hipLaunchKernelGGL((project_int8_small_kernel<T, 2>), dim3((unsigned)n), dim3(256), 0, s, a, blk, (int)tiles, mtiles);
     return check_launch(who);
   }
+  if (n >= ((int64_t)1 << 32) / (M <= 16 ? 256 : 512))  // a launch has less than 2^32 threads
+    return fail(ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)n);
   auto go = [&](auto kern, int nw) { hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(64 * nw), 0, s, a, blk); };
   if (M <= 16) go(project_int8_few_kernel<T, 1, 1, 4>, 4);
   else if (M <= 32) few_cols == 16 ? go(project_int8_few_kernel<T, 2, 1, 8>, 8) : go(project_int8_few_kernel<T, 2, 2, 8>, 8);
