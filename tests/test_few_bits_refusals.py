@@ -242,3 +242,49 @@ def test_a_few_token_launch_of_2_to_the_32_threads_is_refused():
     for m, groups in ((1, 1 << 24), (20, 1 << 23)):
         status = lib.vsp_project_int8_bf16(one, one, one, one, 1, 1 << 28, 16, m, 1 << 28, 1, 1, 1, one, None, None, None, -1, None)
         assert status == 2 and f"{groups} workgroups" in lib.vsp_last_error().decode()
+
+
+@pytest.mark.parametrize(("a", "b", "same"), [
+    ((0, 64), (0, 64), True), ((0, 64), (8, 72), True), ((8, 72), (0, 64), True), ((0, 64), (63, 64), True),
+    ((0, 64), (64, 128), False), ((64, 128), (0, 64), False), ((32, 32), (0, 64), False), ((0, 64), (32, 32), False),
+])
+def test_tensors_that_share_memory_in_part(a, b, same):
+    from vesper.kernels.norm import _overlap
+
+    buf = torch.zeros(128)
+    assert _overlap(buf[slice(*a)], buf[slice(*b)]) is same
+    assert _overlap(buf[slice(*a)], buf.view(BF16)[2 * b[0]:2 * b[1]]) is same
+
+
+class _Placed:
+    """A tensor as the norms' argument checks see one on a GPU (one that no machine has, so that no kernel is reached)."""
+
+    def __init__(self, t):
+        self.t = t
+
+    device = torch.device("cuda", 99)
+
+    def get_device(self):
+        return 99
+
+    def contiguous(self):
+        return self
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+def test_a_sum_that_overlaps_an_input_in_part_is_refused():
+    """One row's sum would overwrite what another row has yet to read."""
+    from vesper.contracts import ContractError
+    from vesper.kernels.norm import rms_norm_int8
+
+    n, d = 4, 64
+    buf, other = torch.zeros((n + 1) * d), torch.zeros(n, d, dtype=BF16)
+    x, late, gain = _Placed(buf[:n * d].view(n, d)), _Placed(buf[d:].view(n, d)), _Placed(buf[n * d:])
+    inside = _Placed(buf.view(BF16)[d:(n + 1) * d].view(n, d))
+    apart = _Placed(torch.zeros(n, d))
+    for kwargs in (dict(x=x, residual=_Placed(other), sum_out=late), dict(x=late, residual=_Placed(other), sum_out=x),
+                   dict(x=apart, residual=inside, sum_out=x), dict(x=apart, residual=_Placed(other), gain=gain, sum_out=late)):
+        with pytest.raises(ContractError, match="overlap"):
+            rms_norm_int8(**kwargs)

@@ -336,3 +336,24 @@ def test_more_rows_than_32_bits_count_are_refused():
     with pytest.raises(ContractError, match="2147483647"):
         projection_int8(torch.ones(1, 16, dtype=torch.int8, device=GPU).expand(rows, 16),
                         torch.ones(1, device=GPU).expand(rows), w, torch.ones(1, 8, device=GPU), (8,))
+
+
+def test_a_sum_that_overlaps_an_input_in_part_is_refused():
+    from vesper.contracts import ContractError
+    from vesper.kernels.norm import rms_norm_int8
+
+    n, d = 40, 64
+    buf, r = torch.randn((n + 1) * d, device=GPU), torch.randn(n, d, device=GPU).bfloat16()
+    x, late = buf[:n * d].view(n, d), buf[d:].view(n, d)
+    before = buf.clone()
+    for kwargs in (dict(x=x, residual=r, sum_out=late), dict(x=late, residual=r, sum_out=x),
+                   dict(x=x.clone(), residual=buf.view(BF16)[d:(n + 1) * d].view(n, d), sum_out=x),
+                   dict(x=x.clone(), residual=r, gain=buf[n * d:], sum_out=late)):
+        with pytest.raises(ContractError, match="overlap"):
+            rms_norm_int8(**kwargs)
+    assert torch.equal(buf, before)
+    # neighbours are taken, and so is a sum over an input that is read as a copy
+    pair = torch.randn(2, n, d, device=GPU)
+    want = pair[0] + r.float()
+    rms_norm_int8(pair[0], residual=r, sum_out=pair[1])
+    assert torch.equal(pair[1], want)

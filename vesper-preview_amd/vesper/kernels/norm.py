@@ -223,6 +223,13 @@ def _aligned(t: Tensor, nbytes: int = 16) -> Tensor:
     return t if t.data_ptr() % nbytes == 0 else t.clone()
 
 
+def _overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether two contiguous tensors share a byte."""
+    start_a, start_b = a.data_ptr(), b.data_ptr()
+    end_a, end_b = start_a + a.numel() * a.element_size(), start_b + b.numel() * b.element_size()
+    return max(start_a, start_b) < min(end_a, end_b)
+
+
 def _refuse_grad(name: str, *tensors: Tensor | None) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ContractError(f"{name} is forward only: call it under torch.no_grad()")
@@ -239,8 +246,9 @@ def rms_norm_int8(x: Tensor, gain: Tensor | None = None, *, residual: Tensor | N
         gain: optional float32 ``[d]`` (the norm's weight; ones when omitted).
         residual: optional tensor shaped like ``x``, bfloat16 or float16 with a float32 ``x`` and else of x's
             dtype: the norm is of the float32 sum ``x + residual``.
-        sum_out: with ``residual``, an optional contiguous tensor of x's shape and dtype (not ``x`` itself)
-            that receives the sum, rounded to that dtype.
+        sum_out: with ``residual``, an optional contiguous tensor of x's shape and dtype that receives the sum,
+            rounded to that dtype. It shares no memory with ``x``, ``residual`` or ``gain``: one row's sum is
+            written while others are still read.
 
     A row whose normalized values are all below ``2 ** -120`` has scale 0 and codes 0; a row with an infinity
     or a NaN has scale NaN and codes 0.
@@ -269,8 +277,8 @@ def rms_norm_int8(x: Tensor, gain: Tensor | None = None, *, residual: Tensor | N
         if (sum_out.shape != shape or sum_out.dtype is not dtype or sum_out.get_device() != device
                 or not sum_out.is_contiguous() or sum_out.data_ptr() % 16):
             raise ContractError(f"sum_out: contiguous, aligned {dtype} {tuple(shape)} on {x.device}")
-        if x.numel() and sum_out.data_ptr() in (xc.data_ptr(), residual.data_ptr()):
-            raise ContractError("sum_out must not be x or the residual")
+        if _overlap(sum_out, xc) or _overlap(sum_out, residual) or (gain is not None and _overlap(sum_out, gain)):
+            raise ContractError("sum_out must not be x, the residual or gain, nor overlap them")
     on = x.device
     codes = torch.empty(shape, dtype=torch.int8, device=on)
     scale = torch.empty(shape[:-1], dtype=torch.float32, device=on)
