@@ -413,7 +413,7 @@ int vsp_key_filter_backward_f32(const float* z, const float* history, const floa
 int vsp_rms_norm_bf16(const float* x, const float* gain, void* out, int rows, int d, void* stream);
 /* The same norm of s = x + residual (residual [rows, d] bf16, added in float32 as the column's
  * residual add does: vesper/column.py:779-796), with s also written to sum_out ([rows, d] float32,
- * or NULL; it must not overlap x): the add and the norm in one launch, bitwise the two launches'.
+ * or NULL; it must overlap none of the inputs): the add and the norm in one launch, bitwise the two launches'.
  * x, residual, sum_out, gain and out 16-byte aligned. */
 int vsp_add_rms_norm_bf16(const float* x, const void* residual, float* sum_out, const float* gain, void* out, int rows,
                           int d, void* stream);
@@ -421,7 +421,7 @@ int vsp_add_rms_norm_bf16(const float* x, const void* residual, float* sum_out, 
 /* The decode step's projection of that normalized stream, fused (the looped column's per-pass
  * projections, vesper/column.py:192-260 and vesper/attention.py:269-292, for a decode step of M
  * single-token rows): s = x + residual (float32; residual [M, d] bf16 or NULL) is written to
- * sum_out ([M, d] float32, or NULL; it must not overlap x), z = RMSNorm(s, gain) in bf16 exactly as
+ * sum_out ([M, d] float32, or NULL; it must overlap none of the inputs), z = RMSNorm(s, gain) in bf16 exactly as
  * vsp_rms_norm_bf16 computes it, and for each of the nblk (1..4) weight blocks
  * out_j = z W_j [:, :used_j] (bf16, [M, used_j] contiguous, fp32 accumulation), W_j [d, cols] the
  * block's weight passed transposed: weights_t [nblk, cols, d] bf16. Block sigmoid_block (or -1 for

@@ -68,3 +68,18 @@ def test_the_residual_add_inside_the_norm_equals_the_two_launches_bitwise(d, wit
     assert torch.equal(s, want_s)
     assert torch.equal(got, rms_norm_bf16(want_s, gain))
     assert torch.equal(rms_norm_bf16(x, gain, residual=r), got)  # without the sum written
+
+
+def test_a_sum_that_overlaps_an_input_in_part_is_refused():
+    from vesper.contracts import ContractError
+    from vesper.kernels.norm import rms_norm_bf16
+
+    n, d = 40, 64
+    buf, r = torch.randn((n + 1) * d, device=GPU), torch.randn(n, d, device=GPU).bfloat16()
+    x, late = buf[:n * d].view(n, d), buf[d:].view(n, d)
+    before = buf.clone()
+    for kwargs in (dict(x=x, residual=r, sum_out=late), dict(x=late, residual=r, sum_out=x),
+                   dict(x=x.clone(), residual=r, gain=buf[n * d:], sum_out=late)):
+        with pytest.raises(ContractError, match="overlap"):
+            rms_norm_bf16(**kwargs)
+    assert torch.equal(buf, before)

@@ -26,8 +26,8 @@ def rms_norm_bf16(x: Tensor, gain: Tensor | None = None, *, residual: Tensor | N
         residual: optional bfloat16 tensor shaped like ``x``: the norm is then of ``x + residual``
             (added in float32, the column's residual add), in the same launch
             (``vsp_add_rms_norm_bf16``), bitwise the add followed by the norm.
-        sum_out: with ``residual``, an optional contiguous float32 tensor shaped like ``x`` (not
-            ``x`` itself) that receives ``x + residual``.
+        sum_out: with ``residual``, an optional contiguous float32 tensor shaped like ``x`` that receives
+            ``x + residual``. It shares no memory with ``x``, ``residual`` or ``gain``.
 
     Raises:
         ContractError: on a dtype, width or device outside that contract.
@@ -68,8 +68,8 @@ def rms_norm_bf16(x: Tensor, gain: Tensor | None = None, *, residual: Tensor | N
         if (sum_out.shape != x.shape or sum_out.dtype != torch.float32 or sum_out.device != x.device
                 or not sum_out.is_contiguous() or sum_out.data_ptr() % 16):
             raise ContractError(f"sum_out: contiguous, aligned float32 {tuple(x.shape)} on {x.device}")
-        if sum_out.data_ptr() == xc.data_ptr():
-            raise ContractError("sum_out must not be x")
+        if _overlap(sum_out, xc) or _overlap(sum_out, rc) or (g is not None and _overlap(sum_out, g)):
+            raise ContractError("sum_out must not be x, the residual or gain, nor overlap them")
     with _lib.on_device(x.device):
         _lib.call("vsp_add_rms_norm_bf16", xc.data_ptr(), rc.data_ptr(), _lib.ptr(sum_out), _lib.ptr(g),
                   out.data_ptr(), rows, d, _lib.stream_of(x.device))
@@ -90,7 +90,7 @@ def decode_projection(x: Tensor, weights_t: Tensor, used: tuple[int, ...], *, re
         weights_t: bf16 ``[p, cols, d]``: the stacked ``[p, d, cols]`` weight, each block transposed.
         used: the columns kept of each of the ``p`` (1..4) blocks.
         residual: optional bf16 ``[M, d]`` added to ``x`` (the previous mixer's output).
-        sum_out: optional float32 ``[M, d]`` that receives ``s`` (not ``x`` itself).
+        sum_out: optional float32 ``[M, d]`` that receives ``s``. It shares no memory with the other operands.
         gain: optional float32 ``[d]`` (the norm's weight; ones when omitted).
         sigmoid_block: the block whose outputs pass through the logistic function (the write strength).
         rotary: ``(positions, inv_freq, dk, blocks)``: the blocks rotated as they are stored, as
@@ -122,8 +122,6 @@ def decode_projection(x: Tensor, weights_t: Tensor, used: tuple[int, ...], *, re
     if sum_out is not None:
         if sum_out.shape != (m, d) or sum_out.dtype != torch.float32 or not sum_out.is_contiguous():
             raise ContractError(f"sum_out: contiguous float32 [{m}, {d}], got {tuple(sum_out.shape)} {sum_out.dtype}")
-        if sum_out.data_ptr() == x.data_ptr():
-            raise ContractError("sum_out must not be x")
         tensors.append(("sum_out", sum_out))
     if gain is not None:
         if gain.shape != (d,) or gain.dtype != torch.float32:
@@ -152,6 +150,10 @@ def decode_projection(x: Tensor, weights_t: Tensor, used: tuple[int, ...], *, re
     for name, t in (("x", xc), ("weights_t", wc), ("residual", rc), ("sum_out", sum_out), ("gain", gc)):
         if t is not None and t.data_ptr() % 16:
             raise ContractError(f"{name} must be 16-byte aligned")
+    if sum_out is not None:
+        for name, t in (("x", xc), ("residual", rc), ("gain", gc), ("weights_t", wc)):
+            if t is not None and _overlap(sum_out, t):
+                raise ContractError(f"sum_out must not be x or another operand, nor overlap one: it overlaps {name}")
     outs = [torch.empty(m, u, dtype=torch.bfloat16, device=x.device) for u in used]
     ptrs = [o.data_ptr() for o in outs] + [0] * (4 - p)
     widths = list(used) + [1] * (4 - p)
@@ -225,9 +227,8 @@ def _aligned(t: Tensor, nbytes: int = 16) -> Tensor:
 
 def _overlap(a: Tensor, b: Tensor) -> bool:
     """Whether two contiguous tensors share a byte."""
-    start_a, start_b = a.data_ptr(), b.data_ptr()
-    end_a, end_b = start_a + a.numel() * a.element_size(), start_b + b.numel() * b.element_size()
-    return max(start_a, start_b) < min(end_a, end_b)
+    s, t = a.data_ptr(), b.data_ptr()
+    return s < t + b.nbytes and t < s + a.nbytes and a.numel() > 0 and b.numel() > 0
 
 
 def _refuse_grad(name: str, *tensors: Tensor | None) -> None:
