@@ -49,11 +49,11 @@ def rms_norm_bf16(x: Tensor, gain: Tensor | None = None, *, residual: Tensor | N
         g = gain.contiguous()
         if g.data_ptr() % 16:
             g = g.clone()
-    out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
     rows = xc.numel() // d
     if residual is None:
         if sum_out is not None:
             raise ContractError("sum_out needs a residual")
+        out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
         with _lib.on_device(x.device):
             _lib.call("vsp_rms_norm_bf16", xc.data_ptr(), _lib.ptr(g), out.data_ptr(), rows, d,
                       _lib.stream_of(x.device))
@@ -70,6 +70,7 @@ def rms_norm_bf16(x: Tensor, gain: Tensor | None = None, *, residual: Tensor | N
             raise ContractError(f"sum_out: contiguous, aligned float32 {tuple(x.shape)} on {x.device}")
         if _overlap(sum_out, xc) or _overlap(sum_out, rc) or (g is not None and _overlap(sum_out, g)):
             raise ContractError("sum_out must not be x, the residual or gain, nor overlap them")
+    out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
     with _lib.on_device(x.device):
         _lib.call("vsp_add_rms_norm_bf16", xc.data_ptr(), rc.data_ptr(), _lib.ptr(sum_out), _lib.ptr(g),
                   out.data_ptr(), rows, d, _lib.stream_of(x.device))
