@@ -115,8 +115,11 @@ __device__ __forceinline__ void arrive() {
 // `zscale` and `wscale` on. Lane (lq, g) holds columns 16 j + 4 g + r of token 16 i + lq. Outputs of 16 bits go through
 // LDS (from `room` on, the wave's own), 16 tokens by 64 columns (or the tile's fewer) at a time, so that whole cache
 // lines leave; row r's 16-byte segment s is at s ^ (r % the row's segments). Returns how many stores the wave has made
-// for certain: kStores, or 0 where some had nothing to store.
-constexpr int kStores = 16;
+// for certain: tile_stores, or 0 where some may have had nothing to store (or, in float32, are not counted).
+template <typename T, int TM, int TN>
+constexpr int tile_stores() {
+  return sizeof(T) == 2 ? TM * (TN * 16 * 16) / (64 * 8) : 0;  // 64 lanes of eight outputs a store
+}
 template <typename T, int TM, int TN>
 __device__ __forceinline__ int store_tile(const i32x4 (&acc)[TN][TM], const Args& a, const Blocks& blk, int nb, int m0,
                                           int c0, int8_t* lds, int zscale, int wscale, int room) {
@@ -133,6 +136,7 @@ __device__ __forceinline__ int store_tile(const i32x4 (&acc)[TN][TM], const Args
     if constexpr (sizeof(T) == 2) {
       // TC column tiles a pass: 16-byte segments a row, rows an instruction
       constexpr int TC = TN < 4 ? TN : 4, SEG = 2 * TC, EACH = 64 / SEG;
+      static_assert(TM * (TN / TC) * (16 / EACH) == tile_stores<T, TM, TN>(), "a store for each turn of the loops");
       const int seg = l % SEG, r0 = l / SEG;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
@@ -198,7 +202,7 @@ __device__ __forceinline__ int store_tile(const i32x4 (&acc)[TN][TM], const Args
   }
   if ((used & 7) == 0 && m0 + 16 * TM <= a.M && c0 + 16 * TN <= used) {
     put(std::false_type{}, std::true_type{});
-    return sizeof(T) == 2 ? kStores : 0;
+    return tile_stores<T, TM, TN>();
   }
   put(std::false_type{}, std::false_type{});
   return 0;
@@ -295,7 +299,7 @@ __global__ __launch_bounds__(512, 1) void project_int8_kernel(const Args a, cons
   // one from the reads of the other. It would wait for all of them at an access of a variable that none fills; so the
   // scales ([tile's parity][tokens, columns]: one is written while the last tile's is read) and the waves' room for
   // their outputs lie behind the first stage, whose loads have always arrived by then.
-  constexpr int kScale = BM * kBK, kRoom = sizeof(T) == 2 ? 2048 : 0;
+  constexpr int kScale = BM * kBK, kRoom = sizeof(T) == 2 ? 2048 : 0, kStores = tile_stores<T, TM, TN>();
   __shared__ __align__(16) int8_t sZ0[kScale + 4096 + 8 * kRoom], sZ1[BM * kBK];
   __shared__ __align__(16) int8_t sW0[BN * kBK], sW1[BN * kBK];
 
