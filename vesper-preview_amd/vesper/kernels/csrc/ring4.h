@@ -57,8 +57,10 @@ struct MaxNanOp {
   __device__ __forceinline__ float operator()(float x, float y) const { return max3(x, y, y); }
 };
 
-// n / d correctly rounded, for finite n and normal d and 1 / d: a reciprocal within one unit and one Newton
-// step on the residual, which fma forms exactly.
+// n / d correctly rounded for finite n and a normal d of at most 11 significant bits (15, or a scale rounded to bf16
+// or fp16) with a normal 1 / d: a reciprocal within one unit and one Newton step on the residual, which fma forms
+// exactly, are within 2^-46 of n / d before the last rounding, and no n / d lies within 2^-36 of the middle between two
+// floats (a middle has 25 bits; its product with d is never n's 24 and is a whole unit of it away).
 __device__ __forceinline__ float quotient(float n, float d, float reciprocal) {
   const float t = n * reciprocal;
   return __builtin_fmaf(__builtin_fmaf(-t, d, n), reciprocal, t);
