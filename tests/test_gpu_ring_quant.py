@@ -557,3 +557,20 @@ def test_token_counts_past_32_bits_are_refused():
     with pytest.raises(ContractError, match="at most 2147483647"):
         quant_ring_read(ring, pos)
     assert not bool(ring.valid.any())
+
+
+def test_the_most_tokens_a_row():
+    """2^31 - 1 tokens, of which the last four stay: the row's end is next to the largest int."""
+    n, w, dk = 2**31 - 1, 4, 8
+    if torch.cuda.mem_get_info()[0] < 80 * 2**30:
+        pytest.skip("needs 80 GiB of free GPU memory")
+    tokens, pos = torch.empty(1, n, 1, dk, dtype=BF16, device=GPU), torch.empty(1, n, dtype=torch.long, device=GPU)
+    last = torch.randn(1, w, 1, dk, generator=torch.Generator().manual_seed(30)).to(BF16)
+    tokens[:, -w:], pos[:, -w:] = last.to(GPU), torch.arange(n - w, n, device=GPU)
+    ring = _write(tokens, tokens, pos, _ring(1, 1, dk, w, BF16), check_positions=False)
+    want = _write(last, last, torch.arange(n - w, n)[None], _ring(1, 1, dk, w, BF16))
+    for mine, theirs in zip(ring.tensors(), want.tensors()):
+        assert torch.equal(mine, theirs)
+    assert int(ring.valid.sum()) == w
+    del tokens, pos
+    torch.cuda.empty_cache()

@@ -70,9 +70,9 @@ __global__ __launch_bounds__(256) void quant_write_kernel(const T* __restrict__ 
   const unsigned b = rest / (unsigned)blocks, tb = rest - b * (unsigned)blocks;
   const unsigned part = threadIdx.x % L, t = threadIdx.x / L;
   const int len = lengths == nullptr ? N : (int)min(max(lengths[b], (int64_t)0), (int64_t)N);
-  const int i0 = max(len - W, 0) + (int)tb * TB;  // the last W tokens of the row are the ones that stay
-  if ((int)t >= len - i0) return;                 // whole rows of lanes leave together
-  const size_t token = (size_t)b * N + i0;        // the workgroup's first; lanes add 32-bit offsets
+  const int kept = min(len, W), i0 = (int)tb * TB;  // the last W tokens of the row are the ones that stay
+  if ((int)t >= kept - i0) return;                  // whole rows of lanes leave together
+  const size_t token = (size_t)b * N + (len - kept) + i0;  // the workgroup's first; lanes add 32-bit offsets
   const int64_t p = pos[token];                   // positions go up by one: the first gives all
   const bool live = (int)(8 * part) < dk;
   float xk[8], xv[8];
