@@ -357,3 +357,36 @@ def test_a_sum_that_overlaps_an_input_in_part_is_refused():
     want = pair[0] + r.float()
     rms_norm_int8(pair[0], residual=r, sum_out=pair[1])
     assert torch.equal(pair[1], want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize(("m", "d", "used", "sig"), [
+    (17, 16, (4200,), None),
+    (17, 1040, (2500, 1700, 9), 2),
+    (31, 144, (4097, 33), 1),
+    (32, 512, (2064, 2064), 0),
+    (33, 144, (2500, 1700, 9), 2),
+    (48, 128, (4160, 1, 31, 16), 3),
+    (63, 2064, (4111,), 0),
+    (64, 512, (1500, 1500, 1500, 12), 3),
+])
+def test_few_tokens_against_many_columns(m, d, used, sig, dtype):
+    """17 to 64 tokens against more than 256 tiles of 16 columns: workgroups of 32 columns, the last ones ragged."""
+    assert sum((u + 15) // 16 for u in used) > 256
+    z, zs, w, ws = _project_case(m, d, used, seed=m + d)
+    _check_project(z, zs, w, ws, used, sig, dtype)
+
+
+@pytest.mark.parametrize("m", [20, 50])
+def test_few_tokens_against_many_wider_weights(m):
+    """Columns past the used ones do not reach the outputs."""
+    from vesper.kernels.norm import projection_int8
+
+    used = (2100, 2050)
+    z, zs, w, ws = _project_case(m, 144, used, seed=m, cols=2300)
+    _check_project(z, zs, w, ws, used, None, F16)
+    for j, u in enumerate(used):
+        w[j, u:], ws[j, u:] = 77, math.nan
+    want = projection_int8(z.to(GPU), zs.to(GPU), w[:, :2100].contiguous().to(GPU), ws[:, :2100].contiguous().to(GPU), used)
+    for a, b in zip(projection_int8(z.to(GPU), zs.to(GPU), w.to(GPU), ws.to(GPU), used), want):
+        assert torch.equal(a, b)
