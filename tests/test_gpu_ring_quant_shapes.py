@@ -200,3 +200,56 @@ def test_the_c_entry_without_a_write(b, w, hkv, dk):
     assert torch.equal(o, want)
     for mine, old in zip(ring.tensors(), before):
         assert torch.equal(mine, old)
+
+
+def _ring_of(k, v, w, dtype, after=0):
+    """A ring of tokens ``k, v [b, n, hkv, dk]`` at positions 0 .. n - 1, and the position behind them."""
+    from vesper.kernels.ring_quant import quant_ring_empty, quant_ring_write
+
+    b, n, hkv, dk = k.shape
+    k, v = k.to(dtype).to(GPU), v.to(dtype).to(GPU)
+    ring = quant_ring_write(k, v, torch.arange(n, device=GPU).expand(b, n), quant_ring_empty(b, hkv, dk, w, dtype, GPU))
+    return ring, torch.full((b, 1), n + after, device=GPU)
+
+
+EDGES = [(1, 40, 1, 64), (2, 520, 2, 72), (1, 5000, 2, 64), (32, 260, 8, 128), (8, 8300, 4, 72), (1, 9000, 1, 136)]
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("size", [2.0**60, 2.0**100, 2.0**116, 2.0**120, 2.0**127])
+@pytest.mark.parametrize(("b", "w", "hkv", "dk"), EDGES)
+def test_values_up_to_the_largest_bf16_are_averaged(b, w, hkv, dk, size):
+    """Every score 0, so that each weight is 1 and the sums are as many times the values as there are tokens."""
+    g = torch.Generator().manual_seed(w)
+    v = (2 * torch.rand(b, w, hkv, dk, generator=g, dtype=torch.float64) - 1) * size
+    ring, pos = _ring_of(torch.randn(b, w, hkv, dk, generator=g), v, w, BF16)
+    q = torch.zeros(b, 1, 2 * hkv, dk, dtype=BF16, device=GPU)
+    _check(q, v[:, :1].to(BF16).to(GPU), v[:, 1:2].to(BF16).to(GPU), pos, ring, BF16)
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("gap", [0.0, 3.0, 400.0, 2.0**27])
+@pytest.mark.parametrize("late", [False, True])
+@pytest.mark.parametrize(("b", "w", "hkv", "dk"), EDGES)
+def test_a_few_values_near_the_largest_among_small_ones(b, w, hkv, dk, late, gap):
+    """Seven tokens in a row of 2^126 among ones of about 1, their scores ``gap`` lower (from 400 on they weigh
+    nothing and the small ones are averaged as if alone), in the first tiles and in the last."""
+    g = torch.Generator().manual_seed(w + dk)
+    k, v = torch.zeros(b, w, hkv, dk), torch.randn(b, w, hkv, dk, generator=g, dtype=torch.float64)
+    at = slice(w - 9, w - 2) if late else slice(2, 9)
+    v[:, at] *= 2.0**126 / 4
+    k[:, at, :, 0] = -gap
+    ring, pos = _ring_of(k, v, w, BF16, after=1)
+    q = torch.zeros(b, 1, hkv, dk, dtype=BF16, device=GPU)
+    q[..., 0] = math.sqrt(dk)
+    new_k, new_v = torch.zeros(b, 1, hkv, dk, dtype=BF16, device=GPU), torch.randn(b, 1, hkv, dk, generator=g).to(BF16).to(GPU)
+    ref, (o, _) = _reference(q, new_k, new_v, pos, ring), _attend(q, new_k, new_v, pos, ring)
+    err = (o.double() - ref).abs()
+    if gap >= 400:  # the small rows' scales are below 1, whatever the large ones' are
+        small = ring.v_scale[..., 0].double()
+        sv = float(small[small < 2.0**60].max())
+        assert bool((err <= HALF_EPS[BF16] * ref.abs() + 143 * sv * 2.0**-16 + 2.0**-20).all()), float(err.max())
+    else:
+        assert bool((err <= _bound(q, ring, new_v, ref, BF16)).all()), float(err.max())

@@ -23,7 +23,8 @@
 // tile sixteen columns, so the columns hold each head twice: P s' rounded to bf16 in the first eight and
 // the rest of it, rounded again, in the others, together 16 bits of it. Sums, maxima and weights are
 // float32; the running maximum is raised only when a tile's exceeds it by more than 8 (weights up to 2^8
-// are as exact), so the accumulators are rarely rescaled.
+// are as exact), so the accumulators are rarely rescaled. It is also raised where the values are so large (past 2^72)
+// that the sums would overflow: the output then is finite as the values are, unless scores past 2^29 meet them.
 //
 // Bound by HBM where the ring is long: 8 rows of 65536 slots, four heads of 128 (290 MB): 57.7 us, 5.0 TB/s, and 4.6
 // for the join. Short windows are a launch and a wave's chain of loads: 64 rows of 512 slots, 8 heads of 64: 9.4 us,
@@ -43,6 +44,10 @@ constexpr int kTile = 32;       // tokens a wave takes at a time
 constexpr int kMaxSplits = 256;  // workgroups that share a window (one thread each in the join)
 constexpr int64_t kMaxThreads = (int64_t)1 << 32;  // a launch has fewer
 constexpr float kRaise = 8.f;   // log2: how far a tile's maximum may exceed the running one
+// Sums of weights up to 2^8 times 143 scales, over at most 2^29 slots, stay below 2^128 while no pair of the values
+// exceeds kLargePair. A wave that has met one that does keeps its running maximum kHeadroom (log2) above the scores, so
+// that its weights, of which only the ratios count, and its sums are 2^64 times smaller.
+constexpr float kLargePair = 0x1p72f, kHeadroom = 64.f;
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -403,6 +408,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
   }
 
   float m = -3.40282347e38f, lsum = 0.f, low = 0.f;  // the running maximum (finite: scores of -inf weigh 0), the lane's sums of P and of P m'
+  float room = 0.f;  // how far above the scores the running maximum is kept
   f32x4 acc[M], bias = zero4();
 #pragma unroll
   for (int e = 0; e < M; ++e) acc[e] = zero4();
@@ -422,6 +428,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
       float2 st;
       if (l < 32) st = make_float2(ps * a.scale_log2, (pl - C::kBias * ps) * a.scale_log2);
       else st = seen ? make_float2(ps, pl) : make_float2(0.f, 0.f);  // no NaN of an unseen slot meets a zero weight
+      if constexpr (std::is_same_v<T, __bf16>) {  // fp16's numbers are never that large
+        const float size = __builtin_fmaxf(__builtin_fabsf(st.x), __builtin_fabsf(st.y));
+        if (__ballot(size > kLargePair) >> 32 != 0) room = kHeadroom;
+      }
       __builtin_amdgcn_wave_barrier();
       stage[w][l >> 5][l & 31] = st;
       __builtin_amdgcn_wave_barrier();
@@ -445,8 +455,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
           if (((mine >> ((i & 3) + 16 * (i >> 2))) & 1u) == 0) sc[i] = -kInf;
       }
       const float top = max_over_rows(top3(top3(sc[0], sc[1], sc[2]), top3(sc[3], sc[4], sc[5]), top3(sc[6], sc[7], sc[7])));
-      if (__ballot(top > m + kRaise) != 0) {
-        const float mn = __builtin_fmaxf(m, top);
+      if (__ballot(top + room > m + kRaise) != 0) {
+        const float mn = __builtin_fmaxf(m, top + room);
         const float f = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         lsum *= f;
