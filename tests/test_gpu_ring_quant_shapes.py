@@ -253,3 +253,20 @@ def test_a_few_values_near_the_largest_among_small_ones(b, w, hkv, dk, late, gap
         assert bool((err <= HALF_EPS[BF16] * ref.abs() + 143 * sv * 2.0**-16 + 2.0**-20).all()), float(err.max())
     else:
         assert bool((err <= _bound(q, ring, new_v, ref, BF16)).all()), float(err.max())
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("size", [2.0**60, 2.0**116, 2.0**124, 2.0**127])
+@pytest.mark.parametrize(("b", "w", "hkv", "dk"), EDGES)
+def test_keys_up_to_the_largest_bf16_are_scored(b, w, hkv, dk, size):
+    """Queries as small as the keys are large, so that the scores are of the usual size; and queries of 0, whose scores
+    are 0 whatever the keys."""
+    g = torch.Generator().manual_seed(w)
+    k = (2 * torch.rand(b, w, hkv, dk, generator=g, dtype=torch.float64) - 1) * size
+    ring, pos = _ring_of(k, torch.randn(b, w, hkv, dk, generator=g), w, BF16)
+    new_v = torch.randn(b, 1, hkv, dk, generator=g).to(BF16).to(GPU)
+    small = torch.randn(b, 1, 2 * hkv, dk, generator=g, dtype=torch.float64)
+    small = (small.sign() * small.abs().clamp_min(0.5) / size * 2).to(BF16).to(GPU)  # no subnormal numbers
+    for q in (small, torch.zeros_like(small)):
+        _check(q, k[:, :1].to(BF16).to(GPU), new_v, pos, ring, BF16)

@@ -17,8 +17,9 @@
 // Both are MFMA products (16x16x32), scores formed transposed, S^T = K q^T, so that a lane holds one
 // query head's scores of eight tokens, which is the operand layout that O^T = V^T P^T takes: the softmax
 // weights go from one product to the next in registers. Codes become bf16 by setting the exponent of
-// 128 above the four bits (128 + c is exact in bf16), two codes an instruction; the 128 is taken out with
-// the sums (128 sum q, and a product with a row of 128s that gives 128 sum P s'). With fp16 queries the
+// 128 above the four bits (128 + c is exact in bf16), two codes an instruction; the 128 is taken out in
+// the sums (the scores' begin at -128 sum q, which with the scales applied would overflow for keys past 2^121; a product
+// with a row of 128s gives 128 sum P s'). With fp16 queries the
 // scores' codes are 1024 + c less 1024 in fp16, also exact. A group has at most eight query heads and the
 // tile sixteen columns, so the columns hold each head twice: P s' rounded to bf16 in the first eight and
 // the rest of it, rounded again, in the others, together 16 bits of it. Sums, maxima and weights are
@@ -402,6 +403,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
     }
   }
   qsum = sum_over_rows(qsum);
+  f32x4 unbias = zero4();  // where the scores' sums begin: they end as those of the codes alone
+  if constexpr (C::kBias != 0.f) unbias = f32x4{-C::kBias * qsum, -C::kBias * qsum, -C::kBias * qsum, -C::kBias * qsum};
   if (w == 0) {
     fresh = sum_over_rows(fresh) * a.scale_log2;
     if (l < kQuantMaxGroup) sfresh[l] = fresh;
@@ -426,7 +429,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
     if (mask != 0) {
       const float ps = pair_scale<T>(tile.pair), pl = pair_low<T>(tile.pair);
       float2 st;
-      if (l < 32) st = make_float2(ps * a.scale_log2, (pl - C::kBias * ps) * a.scale_log2);
+      if (l < 32) st = make_float2(ps * a.scale_log2, pl * a.scale_log2);
       else st = seen ? make_float2(ps, pl) : make_float2(0.f, 0.f);  // no NaN of an unseen slot meets a zero weight
       if constexpr (std::is_same_v<T, __bf16>) {  // fp16's numbers are never that large
         const float size = __builtin_fmaxf(__builtin_fabsf(st.x), __builtin_fabsf(st.y));
@@ -439,7 +442,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
       float sc[8];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        f32x4 d = zero4();
+        f32x4 d = unbias;
 #pragma unroll
         for (int s = 0; s < NS; ++s) d = C::mma(C::unpack(tile.k[u][s], kbits), qf[s], d);
 #pragma unroll
