@@ -519,7 +519,8 @@ int vsp_quant_ring_read_f16(const void* ring_k, const void* ring_v, const void* 
  * are not slot p % window, and over the new token k, v [B, HKV, D] itself (unquantised); o [B, H, D].
  * H / HKV at most 8. `active` uint8 [B] or NULL: an inactive row's output is 0. With write != 0 the token
  * is then quantised into slot p % window. Finite inputs whose scores are finite in float32 give a finite output, unless
- * queries pass 2^110 or scores past 2^29 meet values past 2^72. Where several workgroups share a window the workspace
+ * queries pass 2^110 or scores past 2^29 meet values past 2^72; one past the type's range by a scale's rounding is
+ * brought back to its largest number. Where several workgroups share a window the workspace
  * holds their softmax states (vsp_quant_ring_attn_workspace_bytes; no initial contents needed, not shared by calls that
  * may overlap in time). */
 size_t vsp_quant_ring_attn_workspace_bytes(int B, int H, int HKV, int D, int window);

@@ -270,3 +270,43 @@ def test_keys_up_to_the_largest_bf16_are_scored(b, w, hkv, dk, size):
     small = (small.sign() * small.abs().clamp_min(0.5) / size * 2).to(BF16).to(GPU)  # no subnormal numbers
     for q in (small, torch.zeros_like(small)):
         _check(q, k[:, :1].to(BF16).to(GPU), new_v, pos, ring, BF16)
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize(("b", "w", "hkv", "dk"), EDGES)
+def test_an_average_of_values_at_the_types_end_stays_in_the_type(b, w, hkv, dk, dtype):
+    """Rows from -top to top: the scale's rounding takes the last code past the type's range, and the output, an average
+    of numbers of the type, is brought back to its largest as the read brings back a value."""
+    from vesper.kernels.ring_quant import quant_ring_read
+
+    top = torch.finfo(dtype).max
+    row = torch.linspace(-1, 1, dk, dtype=torch.float64) * top
+    v = row.expand(b, w, hkv, dk).clone()
+    ring, pos = _ring_of(torch.randn(b, w, hkv, dk), v, w, dtype)
+    _, read, _ = quant_ring_read(ring, torch.zeros(b, 1, dtype=torch.long, device=GPU))
+    q, new_k = torch.zeros(b, 1, hkv, dk, dtype=dtype, device=GPU), torch.zeros(b, 1, hkv, dk, dtype=dtype, device=GPU)
+    for new_v in (read, read.flip(3)):  # the same values again, and others
+        ref = _reference(q, new_k, new_v, pos, ring).clamp(-top, top)
+        o, _ = _attend(q, new_k, new_v, pos, ring)
+        assert bool(torch.isfinite(o).all())
+        assert bool(((o.double() - ref).abs() <= _bound(q, ring, new_v, ref, dtype)).all())
+    new_v = read.clone()
+    new_v[..., 3] = math.inf  # an infinity is not brought back
+    o, _ = _attend(q, new_k, new_v, pos, ring)
+    assert bool((o[..., 3] == math.inf).all()) and bool(torch.isfinite(o[..., :3]).all())
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("w", [40, 5000])
+def test_a_lone_score_of_minus_infinity_is_nan(w):
+    """0 / 0 in the average: NaN, as a softmax over that score alone is."""
+    from vesper.kernels.ring_quant import quant_ring_empty
+
+    q, k = torch.ones(1, 1, 1, 64, dtype=BF16, device=GPU), torch.zeros(1, 1, 1, 64, dtype=BF16, device=GPU)
+    k[..., 5] = -math.inf
+    o, _ = _attend(q, k, torch.ones_like(k), torch.zeros(1, 1, dtype=torch.long, device=GPU),
+                   quant_ring_empty(1, 1, 64, w, BF16, GPU))
+    assert bool(o.isnan().all())

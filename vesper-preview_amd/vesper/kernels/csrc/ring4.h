@@ -100,6 +100,15 @@ template <typename T> constexpr float kFiniteMax = 0.f;
 template <> constexpr float kFiniteMax<__bf16> = 3.38953139e38f;
 template <> constexpr float kFiniteMax<_Float16> = 65504.f;
 
+// An average of numbers of T, formed as a / b: among them, so one that passes T's largest number, by the rounding of a
+// scale, is brought back to it; an infinity or a NaN in the sum is kept.
+template <typename T>
+__device__ __forceinline__ float average(float a, float b) {
+  const float x = a / b;
+  const bool past = __builtin_fabsf(a) < kInf && __builtin_fabsf(x) > kFiniteMax<T>;
+  return past ? __builtin_copysignf(kFiniteMax<T>, x) : x;
+}
+
 // A lane's eight features from its dword of codes. The top code may land past T's largest number by
 // the rounding of s: it is brought back to it.
 template <typename T, typename V8>

@@ -550,7 +550,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4 < 2 ? 2 : NW / 4) void quant_attn_k
     }
     const size_t row = (size_t)b * a.H + (size_t)kvh * G + gi;
     if (a.splits == 1) {
-      o[row * dk + d] = from_f32<T>(on ? num / ls : 0.f);
+      o[row * dk + d] = from_f32<T>(on ? average<T>(num, ls) : 0.f);
     } else {
       float* part = a.partial + (row * a.splits + split) * (size_t)(2 + dk);
       part[2 + d] = num;
@@ -597,7 +597,7 @@ __global__ __launch_bounds__(1024) void quant_join_kernel(const float* __restric
     for (int u = 0; u < nw; ++u) total += red[1][u];
     for (int u = 0; u < groups; ++u) sum += sums[u * dk + t];
     const bool on = active == nullptr || active[row / H] != 0;
-    o[row * dk + t] = from_f32<T>(on ? sum / total : 0.f);
+    o[row * dk + t] = from_f32<T>(on ? average<T>(sum, total) : 0.f);
   }
 }
 
