@@ -310,3 +310,36 @@ def test_a_lone_score_of_minus_infinity_is_nan(w):
     o, _ = _attend(q, k, torch.ones_like(k), torch.zeros(1, 1, dtype=torch.long, device=GPU),
                    quant_ring_empty(1, 1, 64, w, BF16, GPU))
     assert bool(o.isnan().all())
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_a_captured_write_and_read_replay_as_the_eager_ones():
+    """A padded batch, its positions and lengths checked in the graph, and a read of them: replays with other tokens,
+    positions and lengths, eager calls of the same shapes between them."""
+    from vesper.kernels.ring_quant import QuantRingKVCache, quant_ring_empty, quant_ring_read, quant_ring_write
+
+    b, n, w, hkv, dk = 3, 5000, 1200, 2, 40
+    g = torch.Generator(device=GPU).manual_seed(41)
+    k, v = _rows(g, b, n, hkv, dk, dtype=BF16), _rows(g, b, n, hkv, dk, dtype=BF16)
+    pos, lengths = torch.arange(n, device=GPU).expand(b, n).contiguous(), torch.tensor([n, 0, 700], device=GPU)
+    mine, check = quant_ring_empty(b, hkv, dk, w, BF16, GPU), quant_ring_empty(b, hkv, dk, w, BF16, GPU)
+    run = lambda ring: (quant_ring_write(k, v, pos, ring, lengths=lengths, inplace=True), quant_ring_read(ring, pos[:, ::7]))  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(QuantRingKVCache(*(t.clone() for t in mine.tensors()), w))
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, got = run(mine)
+    for t in range(4):
+        graph.replay()
+        _, want = run(check)
+        torch.cuda.synchronize()
+        for x, y in zip((*got, *mine.tensors()), (*want, *check.tensors())):
+            assert torch.equal(x, y)
+        pos.add_(lengths[:, None])
+        k.copy_(_rows(g, b, n, hkv, dk, dtype=BF16))
+        lengths.copy_(torch.tensor([17 * t, n - t, 1250], device=GPU))
