@@ -536,8 +536,8 @@ int vsp_quant_ring_attn_f16(const void* q, const void* k, const void* v, const i
 /* ---- projections in 8-bit integers ---------------------------------------------------------------
  * RMSNorm of the rows s = x + residual (float32; residual may be NULL) with gain (float32 [d] or NULL),
  * y = s / sqrt(mean(s^2) + 1e-6) * gain, as int8 codes [rows, d] and a float32 scale a row: scale = max |y| / 127,
- * code = round(y / scale) (both 0 where max |y| < 2^-120; scale NaN and codes 0 for a row with an infinity or
- * a NaN). sum_out (x's type, may be NULL) receives s and must not overlap x, the residual or gain. d a multiple of
+ * code = round(y / scale), in float32: a quotient within 1e-3 of the middle between two codes may become either (both
+ * 0 where max |y| < 2^-120; scale NaN and codes 0 for a row with an infinity or a NaN). sum_out (x's type, may be NULL) receives s and must not overlap x, the residual or gain. d a multiple of
  * 8 in 8..16384; x, residual, sum_out and gain 16-byte aligned, out 8-byte. The name says x's type and, where
  * it differs, the residual's. */
 int vsp_rms_norm_int8_f32_bf16(const void* x, const void* residual, void* sum_out, const float* gain, int8_t* out,

@@ -7,10 +7,12 @@
 // its largest magnitude floored at 1e-3. Rounding a row against its own largest value leaves every
 // element within half a step, a / 2. A row whose normalized values all stay below 2^-120 (zeros, or a
 // gain that small) is stored as zeros with a = 0; a row with an infinity or a NaN, in x, r or the gain's
-// product, has a = NaN and codes 0, so what is computed from it is NaN as from the bf16 norm.
+// product, has a = NaN and codes 0, so what is computed from it is NaN as from the bf16 norm. The quotients are
+// products with reciprocals (of the row's magnitude, its root and a), a few float32 roundings away from the exact
+// ones: one within 1e-3 of the middle between two codes may become either.
 //
 // Rows are held in registers between the reductions, so memory is touched once: bound by the bytes, 11
-// an element with a bf16 residual, the sum written and float32 x (32767 rows of 768: 52.5 us, 5.3 TB/s, a large
+// an element with a bf16 residual, the sum written and float32 x (32767 rows of 768: 50.7 us, 5.5 TB/s, a large
 // copy's rate; 64 rows of 512: 3.2 us). Up to 2048 wide a wave takes a row
 // (reductions by DPP and lane swaps, no barrier); wider rows take a workgroup.
 #include "common.h"

@@ -16,7 +16,7 @@
 // workgroups, 128 x 128 or 128 x 64 in waves of 64 x 32 and three stages. global_load_lds_dwordx4 moves eight rows of 128 bytes an
 // instruction, each row's 16-byte segments XOR-swizzled so that the fragment reads meet each bank once; 16x16x64 int8
 // MFMA formed transposed (weight rows as the A operand); the second half's fragments are read during the first half's
-// products. 8192^3: 444 to 473 us among other work, 520 to 540 back to back (2.0 to 2.5 Pop/s; the clock falls under
+// products. 8192^3: 412 to 473 us among other work, 520 to 540 back to back (2.0 to 2.7 Pop/s; the clock falls under
 // them: the matrix units are busy 69 % of the cycles), a library product of the same operands 547. 32767 x 768 to 2316
 // columns: 72 us (116 Gop, 1.6 Pop/s). One tile a workgroup needed 96: its first loads and its outputs stood alone, and
 // the logistic function, chosen an output at a time, ran for all of them (86 with that block's outputs apart; 78 from
@@ -62,7 +62,8 @@ struct Args {
 };
 
 // An output: the sum times both scales, through the logistic function where asked. That is formed with the
-// exponential and reciprocal instructions (each within a unit of float32): a thread has 64 to 128 outputs, and as
+// exponential and reciprocal instructions (each within a unit of float32; the exponent's own rounding moves a result
+// far below 1 by a relative |y| 2^-23, in float32 outputs too): a thread of the tiles has 32 or 128 outputs, and as
 // calls of the library's functions their code outgrew the instruction cache (32767 tokens of 768: 104 us with
 // it, 90 without a logistic block).
 template <typename T, bool SIG>

@@ -27,10 +27,10 @@
 // are as exact), so the accumulators are rarely rescaled. It is also raised where the values are so large (past 2^72)
 // that the sums would overflow: the output then is finite as the values are, unless scores past 2^29 meet them.
 //
-// Bound by HBM where the ring is long: 8 rows of 65536 slots, four heads of 128 (290 MB): 57.7 us, 5.0 TB/s, and 4.6
-// for the join. Short windows are a launch and a wave's chain of loads: 64 rows of 512 slots, 8 heads of 64: 9.4 us,
-// 4.8 with nothing to attend. Writing 7 ragged rows of 4097 tokens (8 heads of 64): 16 us, reading them back 16.5; a
-// bare copy of the write's pattern takes 10.4.
+// Bound by HBM where the ring is long: 8 rows of 65536 slots, four heads of 128 (290 MB): 58.5 us, 5.0 TB/s, and 4.7
+// for the join. Short windows are a launch and a wave's chain of loads: 64 rows of 512 slots, 8 heads of 64: 9.7 us,
+// 4.8 with nothing to attend. Writing 7 ragged rows of 4097 tokens (8 heads of 64): 16.8 us (14.0 at best), reading them
+// back 17.4 (16.3); a bare copy of the write's pattern takes 10.4.
 #include <type_traits>
 
 #include "common.h"

@@ -241,7 +241,8 @@ def rms_norm_int8(x: Tensor, gain: Tensor | None = None, *, residual: Tensor | N
                   sum_out: Tensor | None = None) -> tuple[Tensor, Tensor]:
     """``RMSNorm`` over the last axis of ``x [..., d]`` (plus ``residual``) in 8-bit integers, one scale a row:
     ``(codes int8 [..., d], scale float32 [...])`` with the norm ``y`` held as ``codes * scale``, ``scale = max
-    |y| / 127`` and ``codes = round(y / scale)``, in one launch (``vsp_rms_norm_int8_*``).
+    |y| / 127`` and ``codes = round(y / scale)``, in one launch (``vsp_rms_norm_int8_*``). The arithmetic is float32: a
+    quotient within 1e-3 of the middle between two codes may become either.
 
     Args:
         x: float32, bfloat16 or float16, its last axis ``d`` a multiple of 8 in 8..16384.
