@@ -390,3 +390,20 @@ def test_few_tokens_against_many_wider_weights(m):
     want = projection_int8(z.to(GPU), zs.to(GPU), w[:, :2100].contiguous().to(GPU), ws[:, :2100].contiguous().to(GPU), used)
     for a, b in zip(projection_int8(z.to(GPU), zs.to(GPU), w.to(GPU), ws.to(GPU), used), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_the_most_tokens(dtype):
+    """2^31 - 1 tokens: the last tile ends one row short of 2^31, and the rows of its last wave are the call's last."""
+    from vesper.kernels.norm import projection_int8
+
+    m, d, tail = 2**31 - 1, 16, 700
+    if torch.cuda.mem_get_info()[0] < 120 * 2**30:
+        pytest.skip("needs 120 GiB of free GPU memory")
+    z, zs, w, ws = (t.to(GPU) for t in _project_case(tail, d, (8,), seed=31))
+    big, scales = torch.empty(m, d, dtype=torch.int8, device=GPU), torch.empty(m, device=GPU)
+    big[-tail:], scales[-tail:] = z, zs
+    got = projection_int8(big, scales, w, ws, (8,), dtype=dtype)[0]
+    assert torch.equal(got[-tail:], projection_int8(z, zs, w, ws, (8,), dtype=dtype)[0])
+    del big, scales, got
+    torch.cuda.empty_cache()

@@ -201,7 +201,7 @@ __device__ __forceinline__ int store_tile(const i32x4 (&acc)[TN][TM], const Args
     put(std::true_type{}, std::false_type{});
     return 0;
   }
-  if ((used & 7) == 0 && m0 + 16 * TM <= a.M && c0 + 16 * TN <= used) {
+  if ((used & 7) == 0 && m0 <= a.M - 16 * TM && c0 <= used - 16 * TN) {  // (sums here could pass 2^31)
     put(std::false_type{}, std::true_type{});
     return tile_stores<T, TM, TN>();
   }
