@@ -343,3 +343,33 @@ def test_a_captured_write_and_read_replay_as_the_eager_ones():
         pos.add_(lengths[:, None])
         k.copy_(_rows(g, b, n, hkv, dk, dtype=BF16))
         lengths.copy_(torch.tensor([17 * t, n - t, 1250], device=GPU))
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_the_longest_window():
+    """2^29 - 64 slots of one head of eight (2 GiB of codes less a little; 4 GiB of positions), a chunk that wraps round
+    the end: as a small ring of the same tokens, written, read back and attended."""
+    from vesper.kernels.ring_quant import quant_ring_empty, quant_ring_read, quant_ring_write
+
+    w, n, dk = 2**29 - 64, 90, 8
+    if torch.cuda.mem_get_info()[0] < 40 * 2**30:
+        pytest.skip("needs 40 GiB of free GPU memory")
+    g = torch.Generator(device=GPU).manual_seed(50)
+    k, v = _rows(g, 1, n, 1, dk, dtype=BF16), _rows(g, 1, n, 1, dk, dtype=BF16)
+    start = 9 * w - 50
+    pos = start + torch.arange(n, device=GPU)[None]
+    ring = quant_ring_write(k, v, pos, quant_ring_empty(1, 1, dk, w, BF16, GPU), inplace=True)
+    small = quant_ring_write(k, v, pos - start, quant_ring_empty(1, 1, dk, 128, BF16, GPU))
+    for a, b in zip(quant_ring_read(ring, pos), quant_ring_read(small, pos - start)):
+        assert torch.equal(a, b)
+    assert int(ring.valid.sum()) == n and bool(ring.valid[0, -50:].all()) and bool(ring.valid[0, :n - 50].all())
+    q = torch.randn(1, 1, 4, dk, generator=g, device=GPU).to(BF16)
+    nk, nv = _rows(g, 1, 1, 1, dk, dtype=BF16), _rows(g, 1, 1, 1, dk, dtype=BF16)
+    at = pos[:, -1:] + 1
+    ref = _reference(q, nk, nv, at - start, small)
+    o, _ = _attend(q, nk, nv, at, ring, inplace=True)
+    assert bool(((o.double() - ref).abs() <= _bound(q, small, nv, ref, BF16)).all())
+    assert int(ring.pos[0, n - 50]) == int(at) and int(ring.valid.sum()) == n + 1
+    del ring
+    torch.cuda.empty_cache()
