@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define VSP_ABI_VERSION 23
+#define VSP_ABI_VERSION 24
 
 /* Status codes. */
 #define VSP_OK 0
@@ -563,6 +563,35 @@ int vsp_project_int8_f16(const int8_t* z, const float* z_scale, const int8_t* we
 int vsp_project_int8_f32(const int8_t* z, const float* z_scale, const int8_t* weights, const float* weights_scale,
                          int nblk, int cols, int d, int M, int used0, int used1, int used2, int used3, void* out0,
                          void* out1, void* out2, void* out3, int sigmoid_block, void* stream);
+
+/* ---- the gated delta rule ------------------------------------------------------------------------
+ * The delta rule with a decay of the state before each token, g float32 [B, N, H] its logarithm (at most 0;
+ * -inf forgets the state): H_t = e^g H_{t-1} + k_t u_t^T, u_t = beta_t (v_t - e^g H_{t-1}^T k_t), o_t = H_t^T q_t.
+ * q, k, v, o [B, N, H, D], beta [B, N, H] of the type the name ends in, the states float32 [B, H, D, D]. D a
+ * multiple of 8 in 8..256, N at most 2^30, at most 2^25 chunks of 64 tokens and 2^22 slices of 16 value columns over
+ * all heads. The workspace (vsp_gated_scan_workspace_bytes; no initial contents, not shared by calls that may
+ * overlap in time) holds each chunk's decays and triangular factors. `records` (vsp_gated_scan_records_bytes, or NULL)
+ * receives what the backward pass needs: each chunk's starting state and corrections in float32. q, k, v, o, the
+ * workspace and the records 16-byte aligned. No output overlaps an input. */
+size_t vsp_gated_scan_workspace_bytes(int B, int N, int H, int D, int fp32);
+size_t vsp_gated_scan_records_bytes(int B, int N, int H, int D);
+int vsp_gated_scan_bf16(const void* q, const void* k, const void* v, const void* beta, const float* g,
+                        const float* state_in, void* o, float* state_out, void* workspace, size_t workspace_bytes,
+                        void* records, size_t records_bytes, const uint8_t* active, int B, int N, int H, int D,
+                        void* stream);
+int vsp_gated_scan_f32(const void* q, const void* k, const void* v, const void* beta, const float* g,
+                       const float* state_in, void* o, float* state_out, void* workspace, size_t workspace_bytes,
+                       void* records, size_t records_bytes, const uint8_t* active, int B, int N, int H, int D,
+                       void* stream);
+
+/* One token per row: q, k, v, o [B, H, D], beta [B, H], g float32 [B, H], the states float32 [B, H, D, D];
+ * state_out may be state_in. D in 1..256, B * H under 2^20. `active` uint8 [B] or NULL. */
+int vsp_gated_step_bf16(const void* q, const void* k, const void* v, const void* beta, const float* g,
+                        const float* state_in, float* state_out, void* o, const uint8_t* active, int B, int H, int D,
+                        void* stream);
+int vsp_gated_step_f32(const void* q, const void* k, const void* v, const void* beta, const float* g,
+                       const float* state_in, float* state_out, void* o, const uint8_t* active, int B, int H, int D,
+                       void* stream);
 
 #ifdef __cplusplus
 }

@@ -19,7 +19,7 @@ import torch
 HERE = Path(__file__).resolve().parent
 LIBRARY_PATH = HERE / "libvesper_kernels.so"
 HEADER_PATH = HERE.parents[2] / "include" / "vesper_kernels.h"
-ABI_VERSION = 23
+ABI_VERSION = 24
 
 P = ctypes.c_void_p
 I = ctypes.c_int
@@ -103,6 +103,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "vsp_project_int8_bf16": (I, [P, P, P, P, I, I, I, I, I, I, I, I, P, P, P, P, I, P]),
     "vsp_project_int8_f16": (I, [P, P, P, P, I, I, I, I, I, I, I, I, P, P, P, P, I, P]),
     "vsp_project_int8_f32": (I, [P, P, P, P, I, I, I, I, I, I, I, I, P, P, P, P, I, P]),
+    "vsp_gated_scan_workspace_bytes": (Z, [I, I, I, I, I]),
+    "vsp_gated_scan_records_bytes": (Z, [I, I, I, I]),
+    "vsp_gated_scan_bf16": (I, [P, P, P, P, P, P, P, P, P, Z, P, Z, P, I, I, I, I, P]),
+    "vsp_gated_scan_f32": (I, [P, P, P, P, P, P, P, P, P, Z, P, Z, P, I, I, I, I, P]),
+    "vsp_gated_step_bf16": (I, [P, P, P, P, P, P, P, P, P, I, I, I, P]),
+    "vsp_gated_step_f32": (I, [P, P, P, P, P, P, P, P, P, I, I, I, P]),
     "vsp_key_filter_backward_workspace_bytes": (Z, [I, I, I, I]),
     "vsp_key_filter_backward_bf16": (I, [P, P, P, P, P, P, P, P, Z, I, I, I, I, I, P]),
     "vsp_key_filter_backward_f16": (I, [P, P, P, P, P, P, P, P, Z, I, I, I, I, I, P]),

@@ -1,0 +1,187 @@
+// What the gated delta rule's kernels share (gated_scan.hip, gated_backward.hip): matrix operands in
+// pieces, their way through LDS, the chunk's coefficients and factors in the workspace.
+//
+// The rule per head, state H [D, D] (key rows, value columns), log decay g_t:
+//   H_t = e^{g_t} H_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - e^{g_t} H_{t-1}^T k_t),  o_t = H_t^T q_t.
+// A chunk of C = 64 tokens with G_i = g_1 + .. + g_i, eps_i = e^{G_i}, E_ij = e^{G_i - G_j} (j <= i),
+// kap_j = e^{G_C - G_j}, gam = e^{G_C}, A_ij = beta_i E_ij k_i.k_j (j < i), T = (I + A)^-1,
+// P_ij = E_ij q_i.k_j:
+//   R_i = beta_i (v_i - eps_i H^T k_i),  Delta = T R,  O_i = eps_i H^T q_i + sum_j P_ij Delta_j,
+//   H' = gam H + sum_j kap_j k_j Delta_j^T.
+// Every exponent is at most zero where g is, so nothing overflows however far a state decays. The sums
+// G and their differences are in float64: behind a token that forgets (g of -inf counts as -1e4, whose
+// exponential is zero all the same) the sums are large and their differences are not.
+//
+// Precision: inputs in bf16 are exact MFMA operands. What the kernels compute in float32 and multiply
+// again (H, R, Delta, T, their gradients) goes into bf16 MFMA as the sum of kPieces bf16 numbers, each the
+// rounding of what the ones before it leave, and a product takes the pairs of pieces whose indices sum to
+// less than kPieces. Three pieces hold 24 bits, float32's own; six bf16 MFMAs (three where one operand is
+// an input) at 16 cycles a 16x16x32 tile each are 2.7 (5.3) times faster than float32 MFMA's 256 cycles.
+// With two pieces the states were off by 4e-6 of their norm and dg by 8e-6, with three by less than 1e-7
+// besides the accumulators' float32 rounding. Inputs in float32 go through float32 MFMA.
+#pragma once
+
+#include "common.h"
+
+namespace vsp {
+namespace gated {
+
+constexpr int kChunk = 64;
+constexpr int kPieces = 3;
+constexpr double kLeastDecay = -1e4;  // log decays below it: their exponentials are zero either way
+
+// ---- operands: 32 of a product's k a step; lane (c, g) = (l % 16, l / 16) holds row or column c, k 8 g .. 8 g + 7 ----
+template <typename T, int NP> struct Operand;
+template <int NP> struct Operand<__bf16, NP> { bf16x8 p[NP]; };
+template <int NP> struct Operand<float, NP> { f32x4 lo, hi; };
+
+// acc += A B over one step: the pairs of pieces of order below kPieces, the smallest first
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma(const Operand<__bf16, NA>& a, const Operand<__bf16, NB>& b, f32x4 acc) {
+#pragma unroll
+  for (int s = kPieces - 1; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i <= s; ++i)
+      if (i < NA && s - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i < NA ? i : 0], b.p[s - i < NB ? s - i : 0], acc, 0, 0, 0);
+  return acc;
+}
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma(const Operand<float, NA>& a, const Operand<float, NB>& b, f32x4 acc) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.lo[e], b.lo[e], acc, 0, 0, 0);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi[e], b.hi[e], acc, 0, 0, 0);
+  return acc;
+}
+
+// Four float32 values as N bf16 pieces, each the rounding of what is left.
+template <int N>
+__device__ __forceinline__ void split4(f32x4 x, bf16x4 (&out)[N]) {
+#pragma unroll
+  for (int p = 0; p < N; ++p)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      out[p][r] = (__bf16)x[r];
+      x[r] -= (float)out[p][r];
+    }
+}
+
+__device__ __forceinline__ int lane_col() { return threadIdx.x & 15; }
+__device__ __forceinline__ int lane_grp() { return (threadIdx.x & 63) >> 4; }
+
+// Eight elements of a row from k0 + 8 g (zeros where not `ok`); rows are 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ Operand<T, 1> load_row(const T* p, bool ok) {
+  Operand<T, 1> o;
+  if constexpr (sizeof(T) == 2) {
+    o.p[0] = ok ? *reinterpret_cast<const bf16x8*>(p) : bf16x8{};
+  } else {
+    o.lo = ok ? reinterpret_cast<const f32x4*>(p)[0] : zero4();
+    o.hi = ok ? reinterpret_cast<const f32x4*>(p)[1] : zero4();
+  }
+  return o;
+}
+
+// Column f0 + c of rows 32 s + 8 g .. + 7 of a row-major LDS tile [token][feature].
+template <typename T>
+__device__ __forceinline__ Operand<T, 1> load_columns(const T* tile, int pitch, int s, int f0) {
+  const int c = lane_col(), g = lane_grp();
+  Operand<T, 1> o;
+  if constexpr (sizeof(T) == 2) {
+    const T* p = tile + (32 * s + 8 * g + (c >> 2)) * pitch + f0 + 4 * (c & 3);
+    const bf16x4 a = read_tr16<bf16x4>(p), b = read_tr16<bf16x4>(p + 4 * pitch);
+    o.p[0] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  } else {
+    const T* p = tile + (32 * s + 8 * g) * pitch + f0 + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o.lo[e] = p[e * pitch];
+      o.hi[e] = p[(4 + e) * pitch];
+    }
+  }
+  return o;
+}
+
+// ---- operands on their way through LDS or memory: a step's pieces one after the other, a piece 16 bytes a lane --
+// (float32: the eight values in two planes of four). An accumulator tile (rows 16 t + 4 g + r, column c) is half of
+// step t / 2.
+template <typename T, int NP> struct Frags {
+  static constexpr int kStep = sizeof(T) == 2 ? NP * 512 : 512;  // elements of a step
+  __device__ __forceinline__ static void put(T* base, int t, f32x4 acc) {
+    const int c = lane_col(), g = lane_grp();
+    const int lane = (2 * (t & 1) + (g >> 1)) * 16 + c, half = g & 1;
+    T* step = base + (t >> 1) * kStep;
+    if constexpr (sizeof(T) == 2) {
+      bf16x4 x[NP];
+      split4<NP>(acc, x);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x4*>(step + (p * 64 + lane) * 8 + 4 * half) = x[p];
+    } else {
+      *reinterpret_cast<f32x4*>(step + (half * 64 + lane) * 4) = acc;
+    }
+  }
+  template <int N = NP> __device__ __forceinline__ static Operand<T, N> get(const T* base, int s) {
+    const int l = threadIdx.x & 63;
+    const T* step = base + s * kStep;
+    Operand<T, N> o;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int p = 0; p < N; ++p) o.p[p] = *reinterpret_cast<const bf16x8*>(step + (p * 64 + l) * 8);
+    } else {
+      o.lo = *reinterpret_cast<const f32x4*>(step + l * 4);
+      o.hi = *reinterpret_cast<const f32x4*>(step + (64 + l) * 4);
+    }
+    return o;
+  }
+};
+
+// The six operand steps that cover a lower triangle of 4 x 4 tiles. By rows i (the sums run over j <= i): steps
+// 0 .. i / 2; by columns j (over i >= j): steps j / 2 .. 1. The tiles of a step outside the triangle are zeros.
+constexpr int kTriSteps = 6;
+__host__ __device__ constexpr int row_step(int i, int s) { return i < 2 ? i : 2 * i - 2 + s; }
+__host__ __device__ constexpr int col_step(int j, int s) { return j < 2 ? 2 * j + s : j + 2; }
+
+// ---- the workspace of one chunk and head ----
+// coefficients: beta, eps, kap, 64 floats each
+constexpr int kCoef = 3 * kChunk;
+template <typename T, int NP> struct Factor {  // elements of a triangular factor
+  static constexpr int kElems = kTriSteps * Frags<T, NP>::kStep;
+};
+template <typename T> struct Pieces { static constexpr int kN = kPieces; };
+template <> struct Pieces<float> { static constexpr int kN = 1; };
+// pieces of H, Delta and P in the outputs' products: with one of P, heads of width 16 were off by 2.8e-3 (1.7e-3 is the
+// rounding of the outputs alone)
+template <typename T> struct OutPieces { static constexpr int kN = 2; };
+template <> struct OutPieces<float> { static constexpr int kN = 1; };
+
+// LDS writes before, LDS reads after, for the whole workgroup; loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <typename T>
+struct Dims {
+  int N, H, D, chunks;
+  // element offset of token t of head h in [B, N, H, D]
+  __device__ __forceinline__ size_t at(int b, int t, int h) const { return (((size_t)b * N + t) * H + h) * D; }
+};
+
+// ---- launchers shared between the translation units ----
+// The chunks' coefficients and the factors T and P, by rows (the forward's) or by columns (the backward's, P in
+// pieces too).
+template <typename T>
+int launch_prep(const T* q, const T* k, const T* beta, const float* g, float* coef, T* tf, T* pf, int B, int N, int H,
+                int D, bool columns, hipStream_t stream);
+
+int check_sizes(int B, int N, int H, int D, const char* who);
+
+// the records of a forward that a backward follows, float32: each chunk's starting state [value][feature], then its
+// Delta [value][token]
+inline size_t record_bytes(size_t total, int D) { return total * D * (D + kChunk) * sizeof(float); }
+inline int chunks_of(int N) { return (N + kChunk - 1) / kChunk; }
+inline int width_of(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+}  // namespace gated
+}  // namespace vsp

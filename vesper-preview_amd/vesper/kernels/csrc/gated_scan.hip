@@ -1,0 +1,573 @@
+// The gated delta rule's chunked scan on CDNA4 (gfx950); the mathematics and the operands are in gated.h.
+//
+//  * gated_prep_kernel: one wave a chunk and head, all of them at once: the decays' sums, the products of all
+//    pairs of the chunk's tokens (K K^T and K Q^T), the inverse T, and both factors written as MFMA operands.
+//  * gated_chain_kernel: a workgroup a head and 16 value columns walks the chunks. Value columns of the state
+//    evolve independently, so a head of width 64 is four chains. Four waves carry the chain, each one tile of 16
+//    tokens (R, Delta) and its share of the state's feature tiles in accumulators; between the three dependent
+//    products (K H, T R, K^T Delta) the tiles pass through LDS as operands in pieces. Four more waves bring the
+//    keys into LDS and form the outputs in the gaps.
+#include "gated.h"
+#include "vesper_kernels.h"
+
+namespace vsp {
+namespace gated {
+namespace {
+
+// --------------------------------------------------------------------------------------------
+// prep
+// --------------------------------------------------------------------------------------------
+constexpr int kPad = 20;                   // pitch of a 16 x 16 float32 tile in LDS
+constexpr int kTile = 16 * kPad + 4;       // tiles start on other banks
+constexpr int kPrepWaves = 4;
+
+struct PrepLds {
+  double sums[kChunk];
+  float beta[kChunk];
+  float a[4 * kTile];  // diagonal tiles of A
+  float x[4 * kTile];  // their inverses (I + A_bb)^-1
+};
+
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// C[16 x 16] += A B in float32: lane (c, g) holds A[c][4 g + r] and B[4 g + r][c], an accumulator's own layout.
+__device__ __forceinline__ f32x4 mm16f(f32x4 a, f32x4 b, f32x4 acc) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], acc, 0, 0, 0);
+  return acc;
+}
+
+// COLS: the factors by columns, with accumulator rows i and columns j; else by rows, transposed: rows j, columns i.
+// The off-diagonal tiles of T follow from the diagonal inverses X by T_ij = -X_i sum_k A_ik T_kj (k = j .. i - 1) or,
+// transposed, T_ij^T = -X_j^T sum_k A_kj^T T_ik^T (k = j + 1 .. i). In either form the tile A that multiplies is an
+// accumulator tile of the other form's layout, and what it multiplies is one of its own: no tile leaves registers.
+template <typename T, int DP, bool COLS>
+__global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ beta, const float* __restrict__ g,
+    float* __restrict__ coef, T* __restrict__ tf, T* __restrict__ pf, Dims<T> dims, int total) {
+  __shared__ PrepLds lds[kPrepWaves];
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, c = l & 15, grp = l >> 4;
+  const int id = blockIdx.x * kPrepWaves + wave;
+  if (id >= total) return;  // whole waves; no workgroup barrier below
+  PrepLds& s = lds[wave];
+  const int chunk = id % dims.chunks, bh = id / dims.chunks, h = bh % dims.H, b = bh / dims.H;
+  const int t0 = chunk * kChunk;
+  constexpr int KS = DP / 32;
+  constexpr int NT = Pieces<T>::kN, NPP = COLS ? NT : OutPieces<T>::kN;
+
+  // decays: lane l is token t0 + l; tokens behind the last decay nothing and write nothing
+  {
+    const int t = t0 + l;
+    const bool ok = t < dims.N;
+    const size_t at = ((size_t)b * dims.N + (ok ? t : t0)) * dims.H + h;
+    const float gl = g[at], bl = to_f32(beta[at]);
+    double sum = ok ? ((double)gl < kLeastDecay ? kLeastDecay : (double)gl) : 0.0;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const double up = __shfl_up(sum, off);
+      if (l >= off) sum += up;
+    }
+    const double all = __shfl(sum, 63);
+    const float be = ok ? bl : 0.f;
+    s.sums[l] = sum;
+    s.beta[l] = be;
+    float* co = coef + (size_t)id * kCoef;
+    co[l] = be;
+    co[kChunk + l] = expf((float)sum);
+    co[2 * kChunk + l] = expf((float)(all - sum));
+  }
+
+  // K K^T and Q K^T of the lower tiles, in both accumulator layouts where both are needed: `mult` multiplies (for
+  // COLS rows j, columns i; else rows i, columns j), the diagonal tiles serve both.
+  f32x4 mult[10], pp[10];
+#pragma unroll
+  for (int t = 0; t < 10; ++t) mult[t] = pp[t] = zero4();
+#pragma unroll
+  for (int st = 0; st < KS; ++st) {
+    Operand<T, 1> kf[4], qf[4];
+    const int f = 32 * st + 8 * grp;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = t0 + 16 * i + c;
+      const bool ok = t < dims.N && f < dims.D;
+      const size_t at = dims.at(b, ok ? t : t0, h) + (ok ? f : 0);
+      kf[i] = load_row(k + at, ok);
+      qf[i] = load_row(q + at, ok);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j <= i; ++j) {
+        const int t = i * (i + 1) / 2 + j;
+        mult[t] = COLS ? mma(kf[j], kf[i], mult[t]) : mma(kf[i], kf[j], mult[t]);
+        pp[t] = COLS ? mma(qf[i], kf[j], pp[t]) : mma(kf[j], qf[i], pp[t]);
+      }
+  }
+  wave_lds_sync();
+
+  // the decays between pairs, beta and the triangles
+  T* tout = tf + (size_t)id * Factor<T, NT>::kElems;
+  T* pout = pf + (size_t)id * Factor<T, NPP>::kElems;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j <= i; ++j) {
+      const int t = i * (i + 1) / 2 + j;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 4 * grp + r;
+        {
+          const int ii = 16 * i + (COLS ? c : row), jj = 16 * j + (COLS ? row : c);
+          const float e = jj < ii ? expf((float)(s.sums[ii] - s.sums[jj])) : 0.f;
+          mult[t][r] *= s.beta[ii] * e;
+        }
+        {
+          const int ii = 16 * i + (COLS ? row : c), jj = 16 * j + (COLS ? c : row);
+          pp[t][r] = jj <= ii ? pp[t][r] * expf((float)(s.sums[ii] - s.sums[jj])) : 0.f;
+        }
+      }
+      if (i == j) {  // A[ii][jj] of the diagonal tile, row-major
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int ii = COLS ? c : 4 * grp + r, jj = COLS ? 4 * grp + r : c;
+          s.a[i * kTile + ii * kPad + jj] = mult[t][r];
+        }
+      }
+      if constexpr (COLS) Frags<T, NPP>::put(pout + col_step(j, 0) * Frags<T, NPP>::kStep - (j < 2 ? 0 : Frags<T, NPP>::kStep), i, pp[t]);
+      else Frags<T, NPP>::put(pout + row_step(i, 0) * Frags<T, NPP>::kStep, j, pp[t]);
+    }
+  wave_lds_sync();
+
+  // X = (I + A_bb)^-1 by forward substitution: lane l solves column l % 16 of block l / 16, column by column
+  {
+    float x[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = r == c ? 1.f : 0.f;
+    const float* a = s.a + grp * kTile;
+#pragma unroll
+    for (int kk = 0; kk < 15; ++kk)
+#pragma unroll
+      for (int r = kk + 1; r < 16; ++r) x[r] = __builtin_fmaf(-a[r * kPad + kk], x[kk], x[r]);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s.x[grp * kTile + r * kPad + c] = x[r];
+  }
+  wave_lds_sync();
+
+  // T in this form's accumulator layout, and the diagonal inverses as multipliers
+  f32x4 tt[10], xm[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float* x = s.x + i * kTile;
+    const f32x4 along = *reinterpret_cast<const f32x4*>(x + c * kPad + 4 * grp);  // X[c][4 g + r]
+    f32x4 down;                                                                   // X[4 g + r][c]
+#pragma unroll
+    for (int r = 0; r < 4; ++r) down[r] = x[(4 * grp + r) * kPad + c];
+    tt[i * (i + 1) / 2 + i] = COLS ? down : along;
+    xm[i] = COLS ? along : down;
+  }
+#pragma unroll
+  for (int off = 1; off < 4; ++off)
+#pragma unroll
+    for (int j = 0; j + off < 4; ++j) {
+      const int i = j + off;
+      f32x4 m = zero4();
+      if constexpr (COLS) {
+#pragma unroll
+        for (int kk = j; kk < i; ++kk) m = mm16f(mult[i * (i + 1) / 2 + kk], tt[kk * (kk + 1) / 2 + j], m);
+        m = mm16f(xm[i], m, zero4());
+      } else {
+#pragma unroll
+        for (int kk = j + 1; kk <= i; ++kk) m = mm16f(mult[kk * (kk + 1) / 2 + j], tt[i * (i + 1) / 2 + kk], m);
+        m = mm16f(xm[j], m, zero4());
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) tt[i * (i + 1) / 2 + j][r] = -m[r];
+    }
+  // the factors as operands: by rows tile (i, j) is half j & 1 of row i's step j / 2, by columns half i & 1 of
+  // column j's step i / 2; the halves outside the triangle are zeros
+  using TF = Frags<T, NT>;
+  using PF = Frags<T, NPP>;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j <= i; ++j) {
+      if constexpr (COLS) TF::put(tout + col_step(j, 0) * TF::kStep - (j < 2 ? 0 : TF::kStep), i, tt[i * (i + 1) / 2 + j]);
+      else TF::put(tout + row_step(i, 0) * TF::kStep, j, tt[i * (i + 1) / 2 + j]);
+    }
+  if constexpr (COLS) {
+    TF::put(tout + col_step(1, 0) * TF::kStep, 0, zero4());
+    TF::put(tout + col_step(3, 0) * TF::kStep - TF::kStep, 2, zero4());
+    PF::put(pout + col_step(1, 0) * PF::kStep, 0, zero4());
+    PF::put(pout + col_step(3, 0) * PF::kStep - PF::kStep, 2, zero4());
+  } else {
+    TF::put(tout + row_step(0, 0) * TF::kStep, 1, zero4());
+    TF::put(tout + row_step(2, 0) * TF::kStep, 3, zero4());
+    PF::put(pout + row_step(0, 0) * PF::kStep, 1, zero4());
+    PF::put(pout + row_step(2, 0) * PF::kStep, 3, zero4());
+  }
+}
+
+// --------------------------------------------------------------------------------------------
+// chain
+// --------------------------------------------------------------------------------------------
+template <typename T, int DP> struct ChainShape {
+  static constexpr int KS = DP / 32;                     // operand steps over the features
+  static constexpr int TILES = DP / 16;                  // feature tiles
+  static constexpr int FT = TILES < 4 ? 1 : TILES / 4;   // of them a chain wave's, at most
+  static constexpr int PITCH = DP + (sizeof(T) == 2 ? 8 : 4);
+  static constexpr int NT = Pieces<T>::kN;
+  static constexpr int NO = OutPieces<T>::kN;
+  using F = Frags<T, NT>;
+  using FO = Frags<T, NO>;
+  struct Lds {
+    T keys[kChunk * PITCH];
+    T state[KS * F::kStep];
+    T r[2 * F::kStep];
+    T delta[2 * FO::kStep];
+    T kept[2 * F::kStep];
+  };
+};
+
+// What a chain wave reads of a chunk: its tokens' key rows, its rows of T, its tokens' values and coefficients.
+template <typename T, int DP> struct ChainIn {
+  Operand<T, 1> kf[ChainShape<T, DP>::KS];
+  Operand<T, Pieces<T>::kN> tf[2];
+  T v[4];
+  f32x4 beta, eps, kap;
+  float gam;
+};
+
+// What an output wave reads of a chunk: a quarter of the keys for LDS, its tokens' queries, its rows of P.
+template <typename T, int DP> struct OutIn {
+  static constexpr int LOADS = DP / 32;  // 8 elements a lane each: 64 x DP elements over 256 lanes
+  Operand<T, 1> keys[LOADS];
+  Operand<T, 1> qf[ChainShape<T, DP>::KS];
+  Operand<T, OutPieces<T>::kN> pf[2];
+  float eps;
+  uint8_t on;
+};
+
+template <typename T, int DP, bool RECORD>
+__global__ __launch_bounds__(512) void gated_chain_kernel(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const float* __restrict__ coef,
+    const T* __restrict__ tf, const T* __restrict__ pf, const float* __restrict__ s_in, T* __restrict__ o,
+    float* __restrict__ s_out, const uint8_t* __restrict__ active, float* __restrict__ rec_h, float* __restrict__ rec_d,
+    Dims<T> dims, int slices) {
+  using S = ChainShape<T, DP>;
+  using F = typename S::F;
+  using FO = typename S::FO;
+  constexpr int KS = S::KS, FT = S::FT, NT = S::NT, NO = S::NO;
+  __shared__ __attribute__((aligned(16))) typename S::Lds lds;
+
+  const int id = xcd_logical_block(blockIdx.x, gridDim.x);
+  const int sl = id % slices, bh = id / slices, h = bh % dims.H, b = bh / dims.H;
+  const int D = dims.D, nc = dims.chunks;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+  const int c = lane_col(), grp = lane_grp();
+  const int vcol = 16 * sl + c;
+  const size_t chunk0 = (size_t)bh * nc;
+
+  if (wave < 4) {
+    // ---- the chain ----
+    f32x4 hs[FT];
+    const float* sp = s_in + (size_t)bh * D * D;
+#pragma unroll
+    for (int i = 0; i < FT; ++i) {
+      const int ft = w + 4 * i;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int f = 16 * ft + 4 * grp + r;
+        hs[i][r] = f < D && vcol < D ? sp[(size_t)f * D + vcol] : 0.f;
+      }
+      if (ft < S::TILES) F::put(lds.state, ft, hs[i]);
+    }
+    auto load = [&](int ci, ChainIn<T, DP>& in) {
+      const int t0 = ci * kChunk;
+      const int t = t0 + 16 * w + c;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        const int f = 32 * st + 8 * grp;
+        const bool ok = t < dims.N && f < D;
+        in.kf[st] = load_row(k + dims.at(b, ok ? t : t0, h) + (ok ? f : 0), ok);
+      }
+      const T* tb = tf + (chunk0 + ci) * Factor<T, NT>::kElems + row_step(w, 0) * F::kStep;
+      in.tf[0] = F::get(tb, 0);
+      if (w >= 2) in.tf[1] = F::get(tb, 1);
+      const float* co = coef + (chunk0 + ci) * kCoef + 16 * w + 4 * grp;
+      in.beta = *reinterpret_cast<const f32x4*>(co);
+      in.eps = *reinterpret_cast<const f32x4*>(co + kChunk);
+      in.kap = *reinterpret_cast<const f32x4*>(co + 2 * kChunk);
+      in.gam = coef[(chunk0 + ci) * kCoef + 2 * kChunk - 1];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int tr = t0 + 16 * w + 4 * grp + r;
+        const bool ok = tr < dims.N && vcol < D;
+        const T x = v[dims.at(b, ok ? tr : t0, h) + (ok ? vcol : 0)];
+        in.v[r] = ok ? x : from_f32<T>(0.f);
+      }
+    };
+    auto step = [&](int ci, const ChainIn<T, DP>& in) {
+      if constexpr (RECORD) {
+        float* rh = rec_h + ((chunk0 + ci) * D + vcol) * D;
+#pragma unroll
+        for (int i = 0; i < FT; ++i) {
+          const int f = 16 * (w + 4 * i) + 4 * grp;
+          if (vcol < D && f < D) *reinterpret_cast<f32x4*>(rh + f) = hs[i];
+        }
+      }
+      // R = beta (V - eps K H)
+      f32x4 x = zero4();
+#pragma unroll
+      for (int st = 0; st < KS; ++st) x = mma(in.kf[st], F::get(lds.state, st), x);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = in.beta[r] * (to_f32(in.v[r]) - in.eps[r] * x[r]);
+      F::put(lds.r, w, x);
+      lds_barrier();
+      // Delta = T R
+      f32x4 dl = mma(in.tf[0], F::get(lds.r, 0), zero4());
+      if (w >= 2) dl = mma(in.tf[1], F::get(lds.r, 1), dl);
+      f32x4 kd;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) kd[r] = in.kap[r] * dl[r];
+      F::put(lds.kept, w, kd);
+      FO::put(lds.delta, w, dl);
+      if constexpr (RECORD)
+        if (vcol < D) *reinterpret_cast<f32x4*>(rec_d + ((chunk0 + ci) * D + vcol) * kChunk + 16 * w + 4 * grp) = dl;
+      lds_barrier();
+      // H' = gam H + K^T (kap Delta)
+      const Operand<T, NT> k0 = F::get(lds.kept, 0), k1 = F::get(lds.kept, 1);
+#pragma unroll
+      for (int i = 0; i < FT; ++i) {
+        const int ft = w + 4 * i;
+        if (ft < S::TILES) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) hs[i][r] *= in.gam;
+          hs[i] = mma(load_columns(lds.keys, S::PITCH, 0, 16 * ft), k0, hs[i]);
+          hs[i] = mma(load_columns(lds.keys, S::PITCH, 1, 16 * ft), k1, hs[i]);
+          F::put(lds.state, ft, hs[i]);
+        }
+      }
+      lds_barrier();
+    };
+    ChainIn<T, DP> a, bb;
+    load(0, a);
+    lds_barrier();
+    for (int ci = 0; ci < nc; ci += 2) {
+      if (ci + 1 < nc) load(ci + 1, bb);
+      step(ci, a);
+      if (ci + 1 < nc) {
+        if (ci + 2 < nc) load(ci + 2, a);
+        step(ci + 1, bb);
+      }
+    }
+    float* so = s_out + (size_t)bh * D * D;
+#pragma unroll
+    for (int i = 0; i < FT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int f = 16 * (w + 4 * i) + 4 * grp + r;
+        if (f < D && vcol < D) so[(size_t)f * D + vcol] = hs[i][r];
+      }
+  } else {
+    // ---- the keys into LDS, and the outputs: O^T tile of this wave's 16 tokens (rows values, columns tokens) ----
+    const int hl = threadIdx.x - 256;  // 0 .. 255
+    auto load = [&](int ci, OutIn<T, DP>& in) {
+      const int t0 = ci * kChunk;
+#pragma unroll
+      for (int i = 0; i < OutIn<T, DP>::LOADS; ++i) {
+        const int p = hl + 256 * i, row = p / (DP / 8), f = 8 * (p % (DP / 8));
+        const bool ok = t0 + row < dims.N && f < D;
+        in.keys[i] = load_row(k + dims.at(b, ok ? t0 + row : t0, h) + (ok ? f : 0), ok);
+      }
+      const int t = t0 + 16 * w + c;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        const int f = 32 * st + 8 * grp;
+        const bool ok = t < dims.N && f < D;
+        in.qf[st] = load_row(q + dims.at(b, ok ? t : t0, h) + (ok ? f : 0), ok);
+      }
+      using PF = FO;
+      const T* pb = pf + (chunk0 + ci) * Factor<T, NO>::kElems + row_step(w, 0) * PF::kStep;
+      in.pf[0] = PF::get(pb, 0);
+      if (w >= 2) in.pf[1] = PF::get(pb, 1);
+      in.eps = coef[(chunk0 + ci) * kCoef + kChunk + 16 * w + c];
+      in.on = active == nullptr || t >= dims.N ? 1 : active[(size_t)b * dims.N + t];
+    };
+    auto step = [&](int ci, const OutIn<T, DP>& in) {
+#pragma unroll
+      for (int i = 0; i < OutIn<T, DP>::LOADS; ++i) {
+        const int p = hl + 256 * i, row = p / (DP / 8), f = 8 * (p % (DP / 8));
+        T* at = lds.keys + row * S::PITCH + f;
+        if constexpr (sizeof(T) == 2) {
+          *reinterpret_cast<bf16x8*>(at) = in.keys[i].p[0];
+        } else {
+          reinterpret_cast<f32x4*>(at)[0] = in.keys[i].lo;
+          reinterpret_cast<f32x4*>(at)[1] = in.keys[i].hi;
+        }
+      }
+      f32x4 acc = zero4();
+#pragma unroll
+      for (int st = 0; st < KS; ++st) acc = mma(F::template get<NO>(lds.state, st), in.qf[st], acc);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] *= in.eps;
+      lds_barrier();
+      lds_barrier();
+      acc = mma(FO::get(lds.delta, 0), in.pf[0], acc);
+      if (w >= 2) acc = mma(FO::get(lds.delta, 1), in.pf[1], acc);
+      const int t = ci * kChunk + 16 * w + c, f = 16 * sl + 4 * grp;
+      if (t < dims.N && f < D) {
+        T* op = o + dims.at(b, t, h) + f;
+        if constexpr (sizeof(T) == 2) {
+          bf16x4 x;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = (__bf16)(in.on ? acc[r] : 0.f);
+          *reinterpret_cast<bf16x4*>(op) = x;
+        } else {
+          f32x4 x;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = in.on ? acc[r] : 0.f;
+          *reinterpret_cast<f32x4*>(op) = x;
+        }
+      }
+      lds_barrier();
+    };
+    OutIn<T, DP> a, bb;
+    load(0, a);
+    lds_barrier();
+    for (int ci = 0; ci < nc; ci += 2) {
+      if (ci + 1 < nc) load(ci + 1, bb);
+      step(ci, a);
+      if (ci + 1 < nc) {
+        if (ci + 2 < nc) load(ci + 2, a);
+        step(ci + 1, bb);
+      }
+    }
+  }
+}
+
+template <typename T, int DP>
+void launch_prep_width(const T* q, const T* k, const T* beta, const float* g, float* coef, T* tf, T* pf, Dims<T> dims,
+                       int total, bool columns, hipStream_t stream) {
+  const dim3 grid((unsigned)((total + kPrepWaves - 1) / kPrepWaves)), block(64 * kPrepWaves);
+  if (columns) hipLaunchKernelGGL((gated_prep_kernel<T, DP, true>), grid, block, 0, stream, q, k, beta, g, coef, tf, pf, dims, total);
+  else hipLaunchKernelGGL((gated_prep_kernel<T, DP, false>), grid, block, 0, stream, q, k, beta, g, coef, tf, pf, dims, total);
+}
+
+template <typename T, int DP>
+void launch_chain(const T* q, const T* k, const T* v, const float* coef, const T* tf, const T* pf, const float* s_in,
+                  T* o, float* s_out, const uint8_t* active, float* rec_h, float* rec_d, Dims<T> dims, int B,
+                  hipStream_t stream) {
+  const int slices = (dims.D + 15) / 16;
+  const dim3 grid((unsigned)(B * dims.H * slices)), block(512);
+  if (rec_h != nullptr)
+    hipLaunchKernelGGL((gated_chain_kernel<T, DP, true>), grid, block, 0, stream, q, k, v, coef, tf, pf, s_in, o, s_out, active,
+                       rec_h, rec_d, dims, slices);
+  else
+    hipLaunchKernelGGL((gated_chain_kernel<T, DP, false>), grid, block, 0, stream, q, k, v, coef, tf, pf, s_in, o, s_out, active,
+                       rec_h, rec_d, dims, slices);
+}
+
+size_t align16(size_t x) { return (x + 15) & ~(size_t)15; }
+
+// the forward's workspace: coefficients, T and P of every chunk and head
+template <typename T> size_t forward_bytes(size_t total) {
+  return align16(total * kCoef * sizeof(float)) + total * sizeof(T) * (Factor<T, Pieces<T>::kN>::kElems + Factor<T, OutPieces<T>::kN>::kElems);
+}
+
+template <typename T>
+int scan(const void* q_, const void* k_, const void* v_, const void* beta_, const float* g, const float* s_in, void* o_,
+         float* s_out, void* ws, size_t ws_bytes, float* records, size_t records_bytes, const uint8_t* active, int B,
+         int N, int H, int D, hipStream_t stream, const char* who) {
+  if (const int st = check_sizes(B, N, H, D, who); st != OK) return st;
+  if (B == 0 || N == 0) return fail(ERR_ARG, "%s: no tokens (B=%d N=%d)", who, B, N);
+  const size_t total = (size_t)B * H * chunks_of(N);
+  if (!q_ || !k_ || !v_ || !beta_ || !g || !s_in || !o_ || !s_out || !ws) return fail(ERR_ARG, "%s: null pointer", who);
+  if ((reinterpret_cast<uintptr_t>(q_) | reinterpret_cast<uintptr_t>(k_) | reinterpret_cast<uintptr_t>(v_) |
+       reinterpret_cast<uintptr_t>(o_) | reinterpret_cast<uintptr_t>(ws) | reinterpret_cast<uintptr_t>(records)) & 15)
+    return fail(ERR_ARG, "%s: q, k, v, o, the workspace and the records must be 16-byte aligned", who);
+  if (ws_bytes < forward_bytes<T>(total)) return fail(ERR_ARG, "%s: workspace of %zu bytes, needs %zu", who, ws_bytes, forward_bytes<T>(total));
+  if (records != nullptr && records_bytes < record_bytes(total, D))
+    return fail(ERR_ARG, "%s: records of %zu bytes, need %zu", who, records_bytes, record_bytes(total, D));
+  const T *q = static_cast<const T*>(q_), *k = static_cast<const T*>(k_), *v = static_cast<const T*>(v_);
+  const T* beta = static_cast<const T*>(beta_);
+  T* o = static_cast<T*>(o_);
+  float* coef = static_cast<float*>(ws);
+  T* tf = reinterpret_cast<T*>(static_cast<char*>(ws) + align16(total * kCoef * sizeof(float)));
+  T* pf = tf + total * Factor<T, Pieces<T>::kN>::kElems;
+  const Dims<T> dims{N, H, D, chunks_of(N)};
+  if (const int st = launch_prep<T>(q, k, beta, g, coef, tf, pf, B, N, H, D, false, stream); st != OK) return st;
+  float* rec_d = records == nullptr ? nullptr : records + total * D * D;
+  switch (width_of(D)) {
+    case 32: launch_chain<T, 32>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, dims, B, stream); break;
+    case 64: launch_chain<T, 64>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, dims, B, stream); break;
+    case 128: launch_chain<T, 128>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, dims, B, stream); break;
+    default: launch_chain<T, 256>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, dims, B, stream); break;
+  }
+  return check_launch(who);
+}
+
+}  // namespace
+
+template <typename T>
+int launch_prep(const T* q, const T* k, const T* beta, const float* g, float* coef, T* tf, T* pf, int B, int N, int H,
+                int D, bool columns, hipStream_t stream) {
+  const Dims<T> dims{N, H, D, chunks_of(N)};
+  const int total = B * H * dims.chunks;
+  switch (width_of(D)) {
+    case 32: launch_prep_width<T, 32>(q, k, beta, g, coef, tf, pf, dims, total, columns, stream); break;
+    case 64: launch_prep_width<T, 64>(q, k, beta, g, coef, tf, pf, dims, total, columns, stream); break;
+    case 128: launch_prep_width<T, 128>(q, k, beta, g, coef, tf, pf, dims, total, columns, stream); break;
+    default: launch_prep_width<T, 256>(q, k, beta, g, coef, tf, pf, dims, total, columns, stream); break;
+  }
+  return check_launch("the gated scan's factors");
+}
+template int launch_prep<__bf16>(const __bf16*, const __bf16*, const __bf16*, const float*, float*, __bf16*, __bf16*, int, int, int, int, bool, hipStream_t);
+template int launch_prep<float>(const float*, const float*, const float*, const float*, float*, float*, float*, int, int, int, int, bool, hipStream_t);
+
+int check_sizes(int B, int N, int H, int D, const char* who) {
+  if (B < 0 || N < 0 || H < 1) return fail(ERR_ARG, "%s: bad sizes B=%d N=%d H=%d", who, B, N, H);
+  if (D < 8 || D > 256 || D % 8 != 0) return fail(ERR_UNSUPPORTED, "%s: head dimension %d (multiples of 8 in 8..256)", who, D);
+  if (N > (1 << 30)) return fail(ERR_UNSUPPORTED, "%s: %d tokens a row (at most 2^30)", who, N);
+  // launches of fewer than 2^32 threads, counts in 32 bits: a wave a chunk and head, 512 threads a slice
+  if ((size_t)B * H * chunks_of(N) > (size_t)1 << 25 || (size_t)B * H * ((D + 15) / 16) > (size_t)1 << 22)
+    return fail(ERR_UNSUPPORTED, "%s: B=%d N=%d H=%d (at most 2^25 chunks of 64 tokens, 2^22 slices of 16 value columns)", who, B, N, H);
+  return OK;
+}
+
+}  // namespace gated
+}  // namespace vsp
+
+extern "C" size_t vsp_gated_scan_workspace_bytes(int B, int N, int H, int D, int fp32) {
+  using namespace vsp::gated;
+  if (B <= 0 || N <= 0 || H <= 0 || D <= 0) return 0;
+  const size_t total = (size_t)B * H * chunks_of(N);
+  return fp32 ? forward_bytes<float>(total) : forward_bytes<__bf16>(total);
+}
+
+extern "C" size_t vsp_gated_scan_records_bytes(int B, int N, int H, int D) {
+  using namespace vsp::gated;
+  if (B <= 0 || N <= 0 || H <= 0 || D <= 0) return 0;
+  return record_bytes((size_t)B * H * chunks_of(N), D);
+}
+
+extern "C" int vsp_gated_scan_bf16(const void* q, const void* k, const void* v, const void* beta, const float* g,
+                                   const float* state_in, void* o, float* state_out, void* workspace,
+                                   size_t workspace_bytes, void* records, size_t records_bytes, const uint8_t* active,
+                                   int B, int N, int H, int D, void* stream) {
+  return vsp::gated::scan<__bf16>(q, k, v, beta, g, state_in, o, state_out, workspace, workspace_bytes,
+                                  static_cast<float*>(records), records_bytes, active, B, N, H, D,
+                                  reinterpret_cast<hipStream_t>(stream), "vsp_gated_scan_bf16");
+}
+
+extern "C" int vsp_gated_scan_f32(const void* q, const void* k, const void* v, const void* beta, const float* g,
+                                  const float* state_in, void* o, float* state_out, void* workspace,
+                                  size_t workspace_bytes, void* records, size_t records_bytes, const uint8_t* active,
+                                  int B, int N, int H, int D, void* stream) {
+  return vsp::gated::scan<float>(q, k, v, beta, g, state_in, o, state_out, workspace, workspace_bytes,
+                                 static_cast<float*>(records), records_bytes, active, B, N, H, D,
+                                 reinterpret_cast<hipStream_t>(stream), "vsp_gated_scan_f32");
+}

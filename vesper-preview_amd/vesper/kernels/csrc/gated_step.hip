@@ -1,0 +1,171 @@
+// The gated delta rule's single-token step on CDNA4 (gfx950): the decode path of the gated scan.
+//
+// One token per (b, h): with a = e^g, H' = a H + k u^T, u = beta (v - a H^T k), o = H'^T q. One pass over H
+// gives both reads, H^T k and H^T q, and the write reuses its registers: o = a H^T q + (k . q) u. The state is
+// read once and written once, all that the step must move. Value columns are independent, so a head is cut
+// into blocks of COLS columns, a workgroup each: thread t holds V columns of the rows t / (COLS / V) + RG j, all of
+// its loads are issued before any arithmetic, and the column sums over the row groups reduce in a fixed order
+// (lane shuffles in a wave, LDS across waves).
+#include "common.h"
+#include "vesper_kernels.h"
+
+namespace vsp {
+namespace {
+
+constexpr int kStepThreads = 256;
+
+template <typename T, int DP, int COLS, int V>
+__global__ __launch_bounds__(kStepThreads) void gated_step_kernel(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ beta,
+    const float* __restrict__ g, const float* s_in, float* s_out, T* __restrict__ o, const uint8_t* __restrict__ active,
+    int H, int D, int blocks) {
+  // s_in and s_out may alias (an in-place step): each thread writes exactly the elements it read
+  constexpr int CPR = COLS / V, RG = kStepThreads / CPR, RPT = (DP + RG - 1) / RG, NW = kStepThreads / 64;
+  typedef float vec __attribute__((ext_vector_type(V)));
+  __shared__ float red[NW][3][COLS];
+  const int bh = blockIdx.x / blocks, block = blockIdx.x - bh * blocks;
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+  const int cb = t % CPR, rg = t / CPR, col = COLS * block + V * cb;
+  const bool col_ok = col < D;
+  const size_t base = (size_t)bh * D * D + (col_ok ? col : 0);
+
+  // the states stream (a decoder's outgrow the caches): nontemporal loads and stores
+  vec st[RPT];
+#pragma unroll
+  for (int j = 0; j < RPT; ++j) {
+    const int row = rg + RG * j;
+    const bool ok = col_ok && row < D;
+    const vec x = __builtin_nontemporal_load(reinterpret_cast<const vec*>(s_in + base + (size_t)(ok ? row : 0) * D));
+#pragma unroll
+    for (int e = 0; e < V; ++e) st[j][e] = ok ? x[e] : 0.f;
+  }
+  const size_t vec0 = (size_t)bh * D;
+  float kr[RPT], qr[RPT], vv[V];
+#pragma unroll
+  for (int j = 0; j < RPT; ++j) {
+    const int row = rg + RG * j;
+    const bool ok = row < D;
+    const float kx = to_f32(k[vec0 + (ok ? row : 0)]), qx = to_f32(q[vec0 + (ok ? row : 0)]);
+    kr[j] = ok ? kx : 0.f;
+    qr[j] = ok ? qx : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) vv[e] = to_f32(v[vec0 + (col_ok ? col + e : 0)]);
+  const float bt = to_f32(beta[bh]), a = expf(g[bh]);
+
+  // partial column sums of H^T k and H^T q over this thread's rows, and of k . q
+  float pk[V], pq[V], kq = 0.f;
+#pragma unroll
+  for (int e = 0; e < V; ++e) pk[e] = pq[e] = 0.f;
+#pragma unroll
+  for (int j = 0; j < RPT; ++j) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      pk[e] += st[j][e] * kr[j];
+      pq[e] += st[j][e] * qr[j];
+    }
+    kq += kr[j] * qr[j];
+  }
+#pragma unroll
+  for (int off = CPR; off < 64; off <<= 1) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      pk[e] += __shfl_xor(pk[e], off);
+      pq[e] += __shfl_xor(pq[e], off);
+    }
+    kq += __shfl_xor(kq, off);
+  }
+  if (lane < CPR) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      red[wv][0][V * cb + e] = pk[e];
+      red[wv][1][V * cb + e] = pq[e];
+    }
+    red[wv][2][V * cb] = kq;
+  }
+  __syncthreads();
+  kq = 0.f;
+#pragma unroll
+  for (int e = 0; e < V; ++e) pk[e] = pq[e] = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      pk[e] += red[w][0][V * cb + e];
+      pq[e] += red[w][1][V * cb + e];
+    }
+    kq += red[w][2][V * cb];
+  }
+  float u[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) u[e] = bt * (vv[e] - a * pk[e]);
+#pragma unroll
+  for (int j = 0; j < RPT; ++j) {
+    const int row = rg + RG * j;
+    if (!col_ok || row >= D) continue;
+    vec x;
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = a * st[j][e] + kr[j] * u[e];
+    __builtin_nontemporal_store(x, reinterpret_cast<vec*>(s_out + base + (size_t)row * D));
+  }
+  if (rg == 0 && col_ok) {
+    const bool on = active == nullptr || active[bh / H] != 0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[vec0 + col + e] = from_f32<T>(on ? a * pq[e] + kq * u[e] : 0.f);
+  }
+}
+
+template <typename T, int DP, int COLS, int V>
+void launch_gated_step(const T* q, const T* k, const T* v, const T* beta, const float* g, const float* s_in,
+                       float* s_out, T* o, const uint8_t* active, int B, int H, int D, hipStream_t stream) {
+  const int blocks = (D + COLS - 1) / COLS;
+  hipLaunchKernelGGL((gated_step_kernel<T, DP, COLS, V>), dim3((unsigned)(B * H * blocks)), dim3(kStepThreads), 0, stream, q,
+                     k, v, beta, g, s_in, s_out, o, active, H, D, blocks);
+}
+
+template <typename T>
+int gated_step(const void* q_, const void* k_, const void* v_, const void* beta_, const float* g, const float* s_in,
+               float* s_out, void* o_, const uint8_t* active, int B, int H, int D, hipStream_t stream, const char* who) {
+  if (B < 0 || H < 1) return fail(ERR_ARG, "%s: bad sizes B=%d H=%d", who, B, H);
+  if (D < 1 || D > 256) return fail(ERR_UNSUPPORTED, "%s: head dimension %d (1..256)", who, D);
+  // launches of fewer than 2^32 threads, at most 16 workgroups of 256 a head
+  if ((size_t)B * H >= (size_t)1 << 20) return fail(ERR_UNSUPPORTED, "%s: B=%d H=%d (fewer than 2^20 rows of heads)", who, B, H);
+  if (B == 0) return OK;
+  if (!q_ || !k_ || !v_ || !beta_ || !g || !s_in || !s_out || !o_) return fail(ERR_ARG, "%s: null pointer", who);
+  const T *q = static_cast<const T*>(q_), *k = static_cast<const T*>(k_), *v = static_cast<const T*>(v_);
+  const T* beta = static_cast<const T*>(beta_);
+  T* o = static_cast<T*>(o_);
+  const bool vec = D % 4 == 0 && ((reinterpret_cast<uintptr_t>(s_in) | reinterpret_cast<uintptr_t>(s_out)) & 15) == 0;
+#define VSP_STEP(DP, COLS, V) launch_gated_step<T, DP, COLS, V>(q, k, v, beta, g, s_in, s_out, o, active, B, H, D, stream)
+  if (!vec) {
+    if (D <= 64) VSP_STEP(64, 16, 1);
+    else VSP_STEP(256, 16, 1);
+  } else if (D <= 32) {
+    VSP_STEP(32, 32, 4);
+  } else if (D <= 64) {
+    VSP_STEP(64, 64, 4);
+  } else if (D <= 128) {
+    VSP_STEP(128, 64, 4);
+  } else {
+    VSP_STEP(256, 64, 4);
+  }
+#undef VSP_STEP
+  return check_launch(who);
+}
+
+}  // namespace
+}  // namespace vsp
+
+extern "C" int vsp_gated_step_bf16(const void* q, const void* k, const void* v, const void* beta, const float* g,
+                                   const float* state_in, float* state_out, void* o, const uint8_t* active, int B, int H,
+                                   int D, void* stream) {
+  return vsp::gated_step<__bf16>(q, k, v, beta, g, state_in, state_out, o, active, B, H, D,
+                                 reinterpret_cast<hipStream_t>(stream), "vsp_gated_step_bf16");
+}
+
+extern "C" int vsp_gated_step_f32(const void* q, const void* k, const void* v, const void* beta, const float* g,
+                                  const float* state_in, float* state_out, void* o, const uint8_t* active, int B, int H,
+                                  int D, void* stream) {
+  return vsp::gated_step<float>(q, k, v, beta, g, state_in, state_out, o, active, B, H, D,
+                                reinterpret_cast<hipStream_t>(stream), "vsp_gated_step_f32");
+}

@@ -1,0 +1,165 @@
+"""The gated delta rule on MI355X: the delta rule of ``delta_scan`` with a decay of the state before each token.
+
+Per head the state ``H [dk, dk]`` (key rows, value columns, float32) and per token the log decay ``g``:
+
+    ``H_t = e^{g_t} H_{t-1} + k_t u_t^T``, ``u_t = beta_t (v_t - e^{g_t} H_{t-1}^T k_t)``, ``o_t = H_t^T q_t``
+
+With ``g = 0`` it is the delta rule of ``delta_scan_fused`` (``vesper/recurrence.py:118-163``), whose layouts, checks
+and ``active`` mask these functions share: no query scaling, keys already normalised.
+
+- ``gated_delta_scan``: a block of tokens, chunked (``vsp_gated_scan_*``).
+- ``gated_delta_step``: one token per row, for decoding (``vsp_gated_step_*``), forward only.
+
+bfloat16 inputs run bf16 MFMA, with everything that is computed in float32 and multiplied again as the sum of three
+bf16 numbers (24 bits): the states and the decays' gradients come out as exact as float32 arithmetic gives them.
+float32 inputs run float32 MFMA.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from vesper.contracts import ContractError, Dims, check_shape
+from vesper.kernels import _lib
+from vesper.kernels.delta_scan import MAX_HEAD_DIM, STATE_DTYPE, _active_mask, _aligned, _refuse_grad
+
+GATE_DTYPE = torch.float32  # the log decays: sums of many of them decide what is left of a state
+INPUT_DTYPES = (torch.bfloat16, torch.float32)  # of q, k, v and beta, all alike
+_SUFFIX = {torch.bfloat16: "bf16", torch.float32: "f32"}
+
+
+def _check(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor, lead: tuple[str, ...]) -> Dims:
+    """Shapes, dtypes, devices and the width, with the error texts of ``delta_scan``'s checks."""
+    dtype = q.dtype
+    if dtype not in INPUT_DTYPES:
+        raise ContractError(f"q: dtype must be torch.bfloat16 or torch.float32, got {dtype}")
+    dims: Dims = {}
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        check_shape(name, t, (*lead, "dk"), dims, dtype)
+    check_shape("beta", beta, lead, dims, dtype)
+    check_shape("g", g, lead, dims, GATE_DTYPE)
+    check_shape("state", state, ("b", "h", "dk", "dk"), dims, STATE_DTYPE)
+    if q.device.type != "cuda":
+        raise ContractError(f"the fused scan runs on CUDA only, got q on {q.device}")
+    for name, t in (("k", k), ("v", v), ("beta", beta), ("g", g), ("state", state)):
+        if t.device != q.device:
+            raise ContractError(f"{name} is on {t.device}, q on {q.device}")
+    if not 1 <= dims["dk"] <= MAX_HEAD_DIM:
+        raise ContractError(f"head dimension {dims['dk']} exceeds the kernel's {MAX_HEAD_DIM}" if dims["dk"]
+                            else "head dimension 0: the kernel takes 1 and more")
+    return dims
+
+
+def _forward(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor, mask: Tensor | None,
+             records: Tensor | None) -> tuple[Tensor, Tensor]:
+    """The scan of contiguous, aligned tensors at a width that is a multiple of 8."""
+    b, n, h, dk = q.shape
+    o, s_out = torch.empty_like(q), torch.empty_like(state)
+    fp32 = q.dtype == torch.float32
+    ws_bytes = int(_lib.library().vsp_gated_scan_workspace_bytes(b, n, h, dk, int(fp32)))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    with _lib.on_device(q.device):
+        _lib.call(f"vsp_gated_scan_{_SUFFIX[q.dtype]}", q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(),
+                  g.data_ptr(), state.data_ptr(), o.data_ptr(), s_out.data_ptr(), ws.data_ptr(), ws_bytes,
+                  _lib.ptr(records), 0 if records is None else records.numel(), _lib.ptr(mask), b, n, h, dk,
+                  _lib.stream_of(q.device))
+    return o, s_out
+
+
+def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor, *,
+                     active: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """The gated delta rule over a block of ``n`` tokens (chunks of 64, float32 state).
+
+    Args:
+        q: the queries ``[b, n, h, dk]``, bfloat16 or float32, on the GPU; ``dk`` in 1..256.
+        k: the keys, same shape and dtype; the caller normalizes them (norm at most one).
+        v: the values, same shape and dtype.
+        beta: the write strengths ``[b, n, h]``, same dtype, each in [0, 1].
+        g: the log decays ``[b, n, h]``, float32, each at most 0; ``-inf`` forgets the state (the start of a
+            document in a packed row) and gives its log decay a gradient of 0.
+        state: the float32 state ``[b, h, dk, dk]`` the block starts from.
+        active: optional bool ``[b, n]``: a token marked False still decays and updates the state, but its output
+            row is zero.
+
+    Returns:
+        ``(o, state_n)``: the outputs ``[b, n, h, dk]`` in q's dtype and the float32 state after the block; for
+        ``n == 0`` the (empty) ``q`` tensor itself and the same ``state`` object.
+
+    Forward only. Widths that
+    are no multiple of 8 run zero-padded to the next, which changes no output. One token without autograd runs as
+    ``gated_delta_step``.
+
+    Raises:
+        ContractError: on a dtype, shape, device or width outside the contract, before any kernel runs.
+    """
+    dims = _check(q, k, v, beta, g, state, ("b", "n", "h"))
+    if active is not None:
+        check_shape("active", active, ("b", "n"), dims, torch.bool)
+    if dims["n"] == 0:
+        return q, state
+    mask = _active_mask(active, ("b", "n"), dims, q.device)
+    if q.numel() == 0:  # no rows or no heads
+        return torch.zeros_like(q), state.clone()
+    grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, beta, g, state))
+    dk = dims["dk"]
+    if dims["n"] == 1 and not grad:
+        first = (t[:, 0] for t in (q, k, v, beta, g))
+        o, after = gated_delta_step(*first, state.contiguous(), active=None if active is None else active[:, 0])
+        return o[:, None], after
+    pad = -dk % 8
+    if pad:
+        q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))
+        state = torch.nn.functional.pad(state, (0, pad, 0, pad))
+    if grad:
+        raise ContractError("gated_delta_scan is forward only: call it under torch.no_grad()")
+    else:
+        o, after = _forward(*(_aligned(t) for t in (q, k, v, beta, g, state)), mask, None)
+    return (o[..., :dk].contiguous(), after[..., :dk, :dk].contiguous()) if pad else (o, after)
+
+
+def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor, *,
+                     active: Tensor | None = None, out_state: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """One token per row through the gated delta rule, decayed, written, then read: ``(H'^T q, H')``.
+
+    Args:
+        q, k, v: ``[b, h, dk]`` float32 or bfloat16 (all three alike, ``beta [b, h]`` too), ``dk`` in 1..256.
+        g: the log decays ``[b, h]``, float32.
+        state: ``[b, h, dk, dk]`` float32, contiguous.
+        active: optional bool ``[b]``; an inactive row decays and writes the state and reads zero.
+        out_state: optional contiguous float32 tensor shaped like ``state`` that receives the new state; it may be
+            ``state`` itself (an in-place decode step), and overlaps it in no other way.
+
+    Returns:
+        ``(o [b, h, dk], state')`` with ``o`` in the inputs' dtype.
+
+    Raises:
+        ContractError: on a dtype, shape, device or width outside the contract, or inputs that require a gradient
+            while grad mode is on.
+    """
+    dims = _check(q, k, v, beta, g, state, ("b", "h"))
+    _refuse_grad(q, k, v, beta, g, state)
+    b, h, dk = q.shape
+    if not state.is_contiguous():
+        raise ContractError("state must be contiguous")
+    if out_state is None:
+        out_state = torch.empty_like(state)
+    else:
+        check_shape("out_state", out_state, ("b", "h", "dk", "dk"), dims, STATE_DTYPE)
+        if out_state.device != q.device or not out_state.is_contiguous():
+            raise ContractError("out_state must be a contiguous tensor on q's device")
+        apart = abs(out_state.data_ptr() - state.data_ptr())
+        if out_state.requires_grad and torch.is_grad_enabled():
+            raise ContractError("out_state must not require a gradient: the step writes it in place")
+        if 0 < apart < state.nbytes:
+            raise ContractError("out_state must be state itself or not overlap it")
+    q, k, v, beta, g = (t.contiguous() for t in (q, k, v, beta, g))
+    mask = _active_mask(active, ("b",), dims, q.device)
+    o = torch.empty_like(q)
+    if q.numel() == 0:
+        return o, out_state
+    with _lib.on_device(q.device):
+        _lib.call(f"vsp_gated_step_{_SUFFIX[q.dtype]}", q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(),
+                  g.data_ptr(), state.data_ptr(), out_state.data_ptr(), o.data_ptr(), _lib.ptr(mask), b, h, dk,
+                  _lib.stream_of(q.device))
+    return o, out_state
