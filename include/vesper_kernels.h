@@ -584,6 +584,22 @@ int vsp_gated_scan_f32(const void* q, const void* k, const void* v, const void* 
                        void* records, size_t records_bytes, const uint8_t* active, int B, int N, int H, int D,
                        void* stream);
 
+/* The scan's backward pass: d_o [B, N, H, D] and d_state (float32 [B, H, D, D], or NULL for zeros) are the gradients
+ * of o and state_out, `records` what the forward of the same inputs kept, `active` as it had it. Every gradient has its
+ * input's type and shape. The workspace as the forward's. q, k, v, d_o, dq, dk, dv, the workspace and the records
+ * 16-byte aligned. No output overlaps an input. */
+size_t vsp_gated_scan_backward_workspace_bytes(int B, int N, int H, int D, int fp32);
+int vsp_gated_scan_backward_bf16(const void* q, const void* k, const void* v, const void* beta, const float* g,
+                                 const void* records, size_t records_bytes, const void* d_o, const float* d_state,
+                                 const uint8_t* active, void* dq, void* dk, void* dv, void* dbeta, float* dg,
+                                 float* d_state_in, void* workspace, size_t workspace_bytes, int B, int N, int H, int D,
+                                 void* stream);
+int vsp_gated_scan_backward_f32(const void* q, const void* k, const void* v, const void* beta, const float* g,
+                                const void* records, size_t records_bytes, const void* d_o, const float* d_state,
+                                const uint8_t* active, void* dq, void* dk, void* dv, void* dbeta, float* dg,
+                                float* d_state_in, void* workspace, size_t workspace_bytes, int B, int N, int H, int D,
+                                void* stream);
+
 /* One token per row: q, k, v, o [B, H, D], beta [B, H], g float32 [B, H], the states float32 [B, H, D, D];
  * state_out may be state_in. D in 1..256, B * H under 2^20. `active` uint8 [B] or NULL. */
 int vsp_gated_step_bf16(const void* q, const void* k, const void* v, const void* beta, const float* g,

@@ -107,6 +107,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "vsp_gated_scan_records_bytes": (Z, [I, I, I, I]),
     "vsp_gated_scan_bf16": (I, [P, P, P, P, P, P, P, P, P, Z, P, Z, P, I, I, I, I, P]),
     "vsp_gated_scan_f32": (I, [P, P, P, P, P, P, P, P, P, Z, P, Z, P, I, I, I, I, P]),
+    "vsp_gated_scan_backward_workspace_bytes": (Z, [I, I, I, I, I]),
+    "vsp_gated_scan_backward_bf16": (I, [P, P, P, P, P, P, Z, P, P, P, P, P, P, P, P, P, P, Z, I, I, I, I, P]),
+    "vsp_gated_scan_backward_f32": (I, [P, P, P, P, P, P, Z, P, P, P, P, P, P, P, P, P, P, Z, I, I, I, I, P]),
     "vsp_gated_step_bf16": (I, [P, P, P, P, P, P, P, P, P, I, I, I, P]),
     "vsp_gated_step_f32": (I, [P, P, P, P, P, P, P, P, P, I, I, I, P]),
     "vsp_key_filter_backward_workspace_bytes": (Z, [I, I, I, I]),

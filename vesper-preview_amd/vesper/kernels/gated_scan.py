@@ -7,7 +7,7 @@ Per head the state ``H [dk, dk]`` (key rows, value columns, float32) and per tok
 With ``g = 0`` it is the delta rule of ``delta_scan_fused`` (``vesper/recurrence.py:118-163``), whose layouts, checks
 and ``active`` mask these functions share: no query scaling, keys already normalised.
 
-- ``gated_delta_scan``: a block of tokens, chunked (``vsp_gated_scan_*``).
+- ``gated_delta_scan``: a block of tokens, chunked, with its backward pass (``vsp_gated_scan_*``).
 - ``gated_delta_step``: one token per row, for decoding (``vsp_gated_step_*``), forward only.
 
 bfloat16 inputs run bf16 MFMA, with everything that is computed in float32 and multiplied again as the sum of three
@@ -17,8 +17,11 @@ float32 inputs run float32 MFMA.
 
 from __future__ import annotations
 
+from typing import Any
+
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from vesper.contracts import ContractError, Dims, check_shape
 from vesper.kernels import _lib
@@ -67,6 +70,39 @@ def _forward(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Te
     return o, s_out
 
 
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor,
+                mask: Tensor | None) -> tuple[Tensor, Tensor]:  # noqa: D102
+        q, k, v, beta, g, state = (_aligned(t.detach()) for t in (q, k, v, beta, g, state))
+        # each chunk's starting state and its Delta, for the backward
+        nrec = int(_lib.library().vsp_gated_scan_records_bytes(*q.shape))
+        records = torch.empty(nrec, dtype=torch.uint8, device=q.device)
+        o, s_out = _forward(q, k, v, beta, g, state, mask, records)
+        ctx.save_for_backward(q, k, v, beta, g, records, *(() if mask is None else (mask,)))
+        return o, s_out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, d_o: Tensor | None, d_state: Tensor | None) -> tuple[Tensor | None, ...]:  # noqa: D102
+        q, k, v, beta, g, records, *rest = ctx.saved_tensors
+        b, n, h, dk = q.shape
+        go = torch.zeros_like(q) if d_o is None else _aligned(d_o.to(q.dtype))
+        gs = None if d_state is None else _aligned(d_state.to(STATE_DTYPE))
+        dq, dk_, dv, db, dg = (torch.empty_like(t) for t in (q, k, v, beta, g))
+        d_state_in = torch.empty((b, h, dk, dk), dtype=STATE_DTYPE, device=q.device)
+        fp32 = q.dtype == torch.float32
+        ws_bytes = int(_lib.library().vsp_gated_scan_backward_workspace_bytes(b, n, h, dk, int(fp32)))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        with _lib.on_device(q.device):
+            _lib.call(f"vsp_gated_scan_backward_{_SUFFIX[q.dtype]}", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                      beta.data_ptr(), g.data_ptr(), records.data_ptr(), records.numel(), go.data_ptr(), _lib.ptr(gs),
+                      _lib.ptr(rest[0] if rest else None), dq.data_ptr(), dk_.data_ptr(), dv.data_ptr(), db.data_ptr(),
+                      dg.data_ptr(), d_state_in.data_ptr(), ws.data_ptr(), ws_bytes, b, n, h, dk, _lib.stream_of(q.device))
+        need = ctx.needs_input_grad
+        return (*(x if wanted else None for x, wanted in zip((dq, dk_, dv, db, dg, d_state_in), need)), None)
+
+
 def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor, *,
                      active: Tensor | None = None) -> tuple[Tensor, Tensor]:
     """The gated delta rule over a block of ``n`` tokens (chunks of 64, float32 state).
@@ -86,7 +122,8 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
         ``(o, state_n)``: the outputs ``[b, n, h, dk]`` in q's dtype and the float32 state after the block; for
         ``n == 0`` the (empty) ``q`` tensor itself and the same ``state`` object.
 
-    Forward only. Widths that
+    Under autograd the gradients of ``q, k, v, beta, g`` and ``state`` come from the backward kernels; the forward
+    then keeps each chunk's starting state and corrections, ``4 dk (dk + 64)`` bytes a chunk and head. Widths that
     are no multiple of 8 run zero-padded to the next, which changes no output. One token without autograd runs as
     ``gated_delta_step``.
 
@@ -112,7 +149,7 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
         q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))
         state = torch.nn.functional.pad(state, (0, pad, 0, pad))
     if grad:
-        raise ContractError("gated_delta_scan is forward only: call it under torch.no_grad()")
+        o, after = _GatedScan.apply(q, k, v, beta, g, state, mask)
     else:
         o, after = _forward(*(_aligned(t) for t in (q, k, v, beta, g, state)), mask, None)
     return (o[..., :dk].contiguous(), after[..., :dk, :dk].contiguous()) if pad else (o, after)
