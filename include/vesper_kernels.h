@@ -609,6 +609,25 @@ int vsp_gated_step_f32(const void* q, const void* k, const void* v, const void* 
                        const float* state_in, float* state_out, void* o, const uint8_t* active, int B, int H, int D,
                        void* stream);
 
+/* ---- layer norm ----------------------------------------------------------------------------------
+ * Rows s = x + residual (float32; residual may be NULL: then s = x and sum_out is not written), mu and var their
+ * mean and mean squared deviation: y = (s - mu) / sqrt(var + eps) * gain + bias (float32 [d]; bias may be NULL).
+ * sum_out receives s in x's type, stats (or NULL) mu and 1 / sqrt(var + eps) of each row, float32 [rows, 2].
+ * Types: 0 float32, 1 bfloat16, 2 float16; x float32 goes with any of the others, x of 16 bits with its own only.
+ * d 1..16384. Outputs overlap nothing. Memory of any alignment of its type; 16-byte aligned memory and a
+ * d that is a multiple of 8 run in 16-byte accesses. */
+int vsp_layer_norm(const void* x, const void* residual, const float* gain, const float* bias, void* sum_out, void* y,
+                   float* stats, int x_type, int residual_type, int y_type, int rows, int d, float eps, void* stream);
+
+/* Its backward pass from x and the residual (or, where x is float32, the sum and NULL) and the stats: dy, and dsum (the gradient of sum_out in x's type, or NULL),
+ * to dx (x's type), dresidual (the residual's type, the same values; or NULL), dgain and dbias (float32 [d], dbias may
+ * be NULL). The workspace holds partial sums over rows (no initial contents, not shared by calls that may overlap). */
+size_t vsp_layer_norm_backward_workspace_bytes(int rows, int d);
+int vsp_layer_norm_backward(const void* x, const void* residual, const float* gain, const float* stats, const void* dy,
+                            const void* dsum, void* dx, void* dresidual, float* dgain, float* dbias, void* workspace,
+                            size_t workspace_bytes, int x_type, int residual_type, int y_type, int rows, int d,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -112,6 +112,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "vsp_gated_scan_backward_f32": (I, [P, P, P, P, P, P, Z, P, P, P, P, P, P, P, P, P, P, Z, I, I, I, I, P]),
     "vsp_gated_step_bf16": (I, [P, P, P, P, P, P, P, P, P, I, I, I, P]),
     "vsp_gated_step_f32": (I, [P, P, P, P, P, P, P, P, P, I, I, I, P]),
+    "vsp_layer_norm": (I, [P, P, P, P, P, P, P, I, I, I, I, I, F, P]),
+    "vsp_layer_norm_backward_workspace_bytes": (Z, [I, I]),
+    "vsp_layer_norm_backward": (I, [P, P, P, P, P, P, P, P, P, P, P, Z, I, I, I, I, I, P]),
     "vsp_key_filter_backward_workspace_bytes": (Z, [I, I, I, I]),
     "vsp_key_filter_backward_bf16": (I, [P, P, P, P, P, P, P, P, Z, I, I, I, I, I, P]),
     "vsp_key_filter_backward_f16": (I, [P, P, P, P, P, P, P, P, Z, I, I, I, I, I, P]),

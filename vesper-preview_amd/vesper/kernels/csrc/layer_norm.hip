@@ -1,0 +1,395 @@
+// Layer norm on CDNA4 (gfx950), forward and backward, with the residual's addition in it.
+//
+// Forward, a row s = x + r of d values: y = (s - mu) / sqrt(var + eps) * gain + bias, mu the mean, var the mean of
+// (s - mu)^2; the sum s is written too (the residual stream), with mu and 1 / sqrt(var + eps) of each row for the
+// backward. Both passes take s in float32: a sum that is kept in 16 bits is formed again from x and r in the backward,
+// since the rounding of s would be off from its row's mu and rstd by up to the whole deviation of a narrow row (and
+// put 2e-3 on dgain).
+// Backward, xh = (s - mu) rstd, w = dy gain: ds = rstd (w - mean(w) - xh mean(w xh)) + dsum, which is dx and dr;
+// dgain = sum over rows of dy xh, dbias of dy.
+//
+// Both are bound by memory: a row is read once into registers (16-byte loads), the two sums a row needs are lane
+// reductions, and what is written is written once. Rows of up to 64 lanes' worth belong to a wave, wider ones to a
+// workgroup of four (or, past that, sixteen) waves. The sums over rows stay in registers: a workgroup takes rows
+// grid apart, each lane adds up the columns that it holds in every row, and leaves one partial row; a second kernel
+// adds the partial rows in order. No atomics: results repeat bit for bit.
+//
+// A row is scaled by a power of two (exact) that brings its largest deviation below 2^32 before it is squared, so
+// that var does not overflow; eps is scaled with it.
+#include <algorithm>
+#include <initializer_list>
+
+#include "common.h"
+#include "vesper_kernels.h"
+
+namespace vsp {
+namespace {
+
+// WAVES waves share a row; V elements a piece (8, or 1 for odd widths and unaligned memory); SEG pieces a lane.
+// Reduction over the waves of a row; `slot` alternates so that one barrier a reduction is enough.
+template <int WAVES, int N, typename Op>
+__device__ __forceinline__ void row_reduce(float (&x)[N], float (*red)[16][N], int slot, Op op) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = group_reduce<64>(x[i], op);
+  if constexpr (WAVES > 1) {
+    const int w = (threadIdx.x >> 6) % WAVES;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) red[slot][w][i] = x[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = red[slot][0][i];
+    for (int j = 1; j < WAVES; ++j)
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = op(x[i], red[slot][j][i]);
+  }
+}
+
+template <int V, typename T>
+__device__ __forceinline__ void load_piece(const T* p, float (&out)[V]) {
+  if constexpr (V == 8) load8_f32(p, out);
+  else out[0] = to_f32(p[0]);
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_piece(T* p, const float (&x)[V]) {
+  if constexpr (V == 8 && sizeof(T) == 2) {
+    typedef T V8 __attribute__((ext_vector_type(8)));
+    V8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = from_f32<T>(x[e]);
+    *reinterpret_cast<V8*>(p) = y;
+  } else if constexpr (V == 8) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    p[0] = from_f32<T>(x[0]);
+  }
+}
+
+template <int WAVES> struct NormShape {
+  static constexpr int NT = WAVES == 1 ? 256 : 64 * WAVES;
+  static constexpr int ROWS = NT / (64 * WAVES);  // rows a workgroup has in hand at once
+};
+
+template <typename TX, typename TR, typename TY, int WAVES, int V, int SEG>
+__global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_kernel(
+    const TX* __restrict__ x, const TR* __restrict__ res, const float* __restrict__ gain, const float* __restrict__ bias,
+    TX* __restrict__ sum_out, TY* __restrict__ y, float* __restrict__ stats, int rows, int d, float eps) {
+  __shared__ float red[4][16][1];
+  constexpr int LANES = 64 * WAVES;
+  const int t = threadIdx.x % LANES;
+  // whole waves, and whole workgroups where a barrier follows; the three slots are apart by two barriers
+  for (long row = (long)blockIdx.x * NormShape<WAVES>::ROWS + threadIdx.x / LANES; row < rows;
+       row += (long)gridDim.x * NormShape<WAVES>::ROWS) {
+    const size_t base = (size_t)row * d;
+    float v[SEG][V];
+    float sum[1] = {0.f};
+#pragma unroll
+    for (int j = 0; j < SEG; ++j) {
+      const int f = V * (t + LANES * j);
+      const bool ok = f < d;
+      load_piece<V>(x + base + (ok ? f : 0), v[j]);
+      if (res != nullptr) {
+        float r[V];
+        load_piece<V>(res + base + (ok ? f : 0), r);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[j][e] += r[e];
+        if (ok) store_piece<V>(sum_out + base + f, v[j]);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[0] += ok ? v[j][e] : 0.f;
+    }
+    row_reduce<WAVES, 1>(sum, red, 0, SumOp{});
+    const float mu = sum[0] / (float)d;
+    float peak[1] = {0.f};
+#pragma unroll
+    for (int j = 0; j < SEG; ++j) {
+      const bool ok = V * (t + LANES * j) < d;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[j][e] = ok ? v[j][e] - mu : 0.f;
+        peak[0] = __builtin_fmaxf(peak[0], fabsf(v[j][e]));
+      }
+    }
+    row_reduce<WAVES, 1>(peak, red, 1, MaxOp{});
+    float scale = 1.f;
+    if (peak[0] > 4294967296.f) scale = __builtin_ldexpf(1.f, 32 - __builtin_amdgcn_frexp_expf(peak[0]));
+    float sq[1] = {0.f};
+#pragma unroll
+    for (int j = 0; j < SEG; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[j][e] *= scale;
+        sq[0] += v[j][e] * v[j][e];
+      }
+    row_reduce<WAVES, 1>(sq, red, 2, SumOp{});
+    const float root = 1.f / __builtin_sqrtf(sq[0] / (float)d + eps * (scale * scale));
+    if (stats != nullptr && t == 0) {
+      stats[2 * (size_t)row] = mu;
+      stats[2 * (size_t)row + 1] = root * scale;
+    }
+#pragma unroll
+    for (int j = 0; j < SEG; ++j) {
+      const int f = V * (t + LANES * j);
+      if (f >= d) continue;
+      float gn[V], bs[V], out[V];
+      load_piece<V>(gain + f, gn);
+      if (bias != nullptr) load_piece<V>(bias + f, bs);
+#pragma unroll
+      for (int e = 0; e < V; ++e) out[e] = v[j][e] * root * gn[e] + (bias != nullptr ? bs[e] : 0.f);
+      store_piece<V>(y + base + f, out);
+    }
+  }
+}
+
+// res as in the forward, or null where x is the float32 sum itself. dres may be null (no residual, or of x's type:
+// then dx serves both). partial: [grid][2][d] sums of dy xh and dy.
+template <typename TX, typename TR, typename TY, int WAVES, int V, int SEG>
+__global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_backward_kernel(
+    const TX* __restrict__ x, const TR* __restrict__ res, const float* __restrict__ gain, const float* __restrict__ stats,
+    const TY* __restrict__ dy,
+    const TX* __restrict__ dsum, TX* __restrict__ dx, TR* __restrict__ dres, float* __restrict__ partial, int rows, int d) {
+  constexpr int LANES = 64 * WAVES, ROWS = NormShape<WAVES>::ROWS;
+  __shared__ float red[2][16][2];
+  __shared__ float cols[ROWS > 1 ? ROWS : 1][ROWS > 1 ? 64 * SEG * V : 1];
+  const int t = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+  float gn[SEG][V], dg[SEG][V], db[SEG][V];
+#pragma unroll
+  for (int j = 0; j < SEG; ++j) {
+    const int f = V * (t + LANES * j);
+    const bool ok = f < d;
+    load_piece<V>(gain + (ok ? f : 0), gn[j]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (!ok) gn[j][e] = 0.f;
+      dg[j][e] = db[j][e] = 0.f;
+    }
+  }
+  int slot = 0;
+  for (long row = (long)blockIdx.x * ROWS + sub; row < rows; row += (long)gridDim.x * ROWS) {
+    const size_t base = (size_t)row * d;
+    const float mu = stats[2 * (size_t)row], rstd = stats[2 * (size_t)row + 1];
+    float xh[SEG][V], w[SEG][V];
+    float sums[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < SEG; ++j) {
+      const int f = V * (t + LANES * j);
+      const bool ok = f < d;
+      load_piece<V>(x + base + (ok ? f : 0), xh[j]);
+      if (res != nullptr) {
+        float r[V];
+        load_piece<V>(res + base + (ok ? f : 0), r);
+#pragma unroll
+        for (int e = 0; e < V; ++e) xh[j][e] += r[e];
+      }
+      load_piece<V>(dy + base + (ok ? f : 0), w[j]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        xh[j][e] = ok ? (xh[j][e] - mu) * rstd : 0.f;
+        const float g0 = ok ? w[j][e] : 0.f;
+        db[j][e] += g0;
+        dg[j][e] += g0 * xh[j][e];
+        w[j][e] = g0 * gn[j][e];
+        sums[0] += w[j][e];
+        sums[1] += w[j][e] * xh[j][e];
+      }
+    }
+    row_reduce<WAVES, 2>(sums, red, slot, SumOp{});
+    slot ^= 1;
+    const float m0 = sums[0] / (float)d, m1 = sums[1] / (float)d;
+#pragma unroll
+    for (int j = 0; j < SEG; ++j) {
+      const int f = V * (t + LANES * j);
+      if (f >= d) continue;
+      float o[V], add[V];
+      if (dsum != nullptr) load_piece<V>(dsum + base + f, add);
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = rstd * (w[j][e] - m0 - xh[j][e] * m1) + (dsum != nullptr ? add[e] : 0.f);
+      store_piece<V>(dx + base + f, o);
+      if (dres != nullptr) store_piece<V>(dres + base + f, o);
+    }
+  }
+  float* out = partial + (size_t)blockIdx.x * 2 * d;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    if constexpr (ROWS > 1) {  // the workgroup's waves hold the same columns: their sums in order, through LDS
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < SEG; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) cols[sub][V * (t + LANES * j) + e] = half ? db[j][e] : dg[j][e];
+      __syncthreads();
+      for (int f = threadIdx.x; f < d; f += NormShape<WAVES>::NT) {
+        float x = cols[0][f];
+        for (int i = 1; i < ROWS; ++i) x += cols[i][f];
+        out[half * d + f] = x;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < SEG; ++j) {
+        const int f = V * (t + LANES * j);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (f + e < d) out[half * d + f + e] = half ? db[j][e] : dg[j][e];
+      }
+    }
+  }
+}
+
+// dgain and dbias: the column sums of the partial rows. A workgroup takes 64 columns (of the 2 d); its four waves
+// take every fourth partial row each, then the four sums are added in order.
+__global__ __launch_bounds__(256) void layer_norm_columns_kernel(const float* __restrict__ partial, float* __restrict__ dgain,
+                                                                float* __restrict__ dbias, int parts, int d) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  if (col < 2 * d) {
+    int p = w;
+    for (; p + 12 < parts; p += 16)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] += partial[(size_t)(p + 4 * i) * 2 * d + col];
+    for (int i = 0; p < parts; p += 4, ++i) a[i & 3] += partial[(size_t)p * 2 * d + col];
+  }
+  red[w][lane] = (a[0] + a[1]) + (a[2] + a[3]);
+  __syncthreads();
+  if (w == 0 && col < 2 * d) {
+    const float x = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+    if (col < d) dgain[col] = x;
+    else if (dbias != nullptr) dbias[col - d] = x;
+  }
+}
+
+// The widest row of a shape: WAVES * 64 lanes, SEG pieces of V.
+#define VSP_NORM_SHAPES(GO)                     \
+  if (vec) {                                    \
+    if (d <= 512) GO(1, 8, 1);                  \
+    else if (d <= 1024) GO(1, 8, 2);            \
+    else if (d <= 2048) GO(4, 8, 1);            \
+    else if (d <= 4096) GO(4, 8, 2);            \
+    else if (d <= 8192) GO(4, 8, 4);            \
+    else GO(16, 8, 2);                          \
+  } else {                                      \
+    if (d <= 256) GO(1, 1, 4);                  \
+    else if (d <= 2048) GO(4, 1, 8);            \
+    else GO(16, 1, 16);                         \
+  }
+
+bool aligned16(std::initializer_list<const void*> ps) {
+  uintptr_t x = 0;
+  for (const void* p : ps) x |= reinterpret_cast<uintptr_t>(p);
+  return (x & 15) == 0;
+}
+
+int norm_check(int rows, int d, const char* who) {
+  if (rows < 0 || d < 1 || d > 16384) return fail(ERR_ARG, "%s: rows %d, width %d (1..16384)", who, rows, d);
+  return OK;
+}
+
+template <typename TX, typename TR, typename TY>
+int norm_forward(const void* x_, const void* res_, const float* gain, const float* bias, void* sum_, void* y_, float* stats,
+                 int rows, int d, float eps, hipStream_t stream, const char* who) {
+  const TX* x = static_cast<const TX*>(x_);
+  const TR* res = static_cast<const TR*>(res_);
+  TX* sum = static_cast<TX*>(sum_);
+  TY* y = static_cast<TY*>(y_);
+  const bool vec = d % 8 == 0 && aligned16({x, res, gain, bias, sum, y});
+  // launches of fewer than 2^32 threads: past 2^20 workgroups each takes several rows
+#define VSP_GO(W, V, S)                                                                                              \
+  hipLaunchKernelGGL((layer_norm_kernel<TX, TR, TY, W, V, S>),                                                       \
+                     dim3((unsigned)std::min<long>(((long)rows + NormShape<W>::ROWS - 1) / NormShape<W>::ROWS, 1 << 20)), \
+                     dim3(NormShape<W>::NT), 0, stream, x, res, gain, bias, sum, y, stats, rows, d, eps)
+  VSP_NORM_SHAPES(VSP_GO)
+#undef VSP_GO
+  return check_launch(who);
+}
+
+// Workgroups of the backward, and so partial rows: enough to fill the card, each with several rows where there are
+// many.
+constexpr int kNormParts = 1024;
+int norm_parts(int rows, int d) {
+  const int at_once = d <= 1024 ? 4 : 1;
+  const int groups = rows / at_once + (rows % at_once != 0);
+  return groups < kNormParts ? groups : kNormParts;
+}
+
+template <typename TX, typename TR, typename TY>
+int norm_backward(const void* x_, const void* res_, const float* gain, const float* stats, const void* dy_, const void* dsum_, void* dx_,
+                  void* dres_, float* dgain, float* dbias, float* ws, int rows, int d, hipStream_t stream, const char* who) {
+  const TX *x = static_cast<const TX*>(x_), *dsum = static_cast<const TX*>(dsum_);
+  const TR* res = static_cast<const TR*>(res_);
+  const TY* dy = static_cast<const TY*>(dy_);
+  TX* dx = static_cast<TX*>(dx_);
+  TR* dres = static_cast<TR*>(dres_);
+  const bool vec = d % 8 == 0 && aligned16({x, res, gain, dy, dsum, dx, dres});
+  const int parts = norm_parts(rows, d);
+#define VSP_GO(W, V, S)                                                                                              \
+  hipLaunchKernelGGL((layer_norm_backward_kernel<TX, TR, TY, W, V, S>), dim3((unsigned)parts), dim3(NormShape<W>::NT), 0, \
+                     stream, x, res, gain, stats, dy, dsum, dx, dres, ws, rows, d)
+  VSP_NORM_SHAPES(VSP_GO)
+#undef VSP_GO
+  hipLaunchKernelGGL(layer_norm_columns_kernel, dim3((unsigned)((2 * d + 63) / 64)), dim3(256), 0, stream, ws, dgain, dbias, parts, d);
+  return check_launch(who);
+}
+
+// The types of x (and the sum), the residual and y. Codes: 0 float32, 1 bfloat16, 2 float16.
+template <typename F> int by_types(int tx, int tr, int ty, const char* who, F go) {
+  struct F32 { using T = float; };
+  struct B16 { using T = __bf16; };
+  struct H16 { using T = _Float16; };
+  if (tx == 1 && tr == 1 && ty == 1) return go(B16{}, B16{}, B16{});
+  if (tx == 2 && tr == 2 && ty == 2) return go(H16{}, H16{}, H16{});
+  if (tx == 0) switch (3 * tr + ty) {
+    case 0: return go(F32{}, F32{}, F32{});
+    case 1: return go(F32{}, F32{}, B16{});
+    case 2: return go(F32{}, F32{}, H16{});
+    case 3: return go(F32{}, B16{}, F32{});
+    case 4: return go(F32{}, B16{}, B16{});
+    case 5: return go(F32{}, B16{}, H16{});
+    case 6: return go(F32{}, H16{}, F32{});
+    case 7: return go(F32{}, H16{}, B16{});
+    case 8: return go(F32{}, H16{}, H16{});
+    default: break;
+  }
+  return fail(ERR_UNSUPPORTED, "%s: types %d, %d, %d of x, the residual and y", who, tx, tr, ty);
+}
+
+}  // namespace
+}  // namespace vsp
+
+extern "C" int vsp_layer_norm(const void* x, const void* residual, const float* gain, const float* bias, void* sum_out,
+                              void* y, float* stats, int x_type, int residual_type, int y_type, int rows, int d, float eps,
+                              void* stream) {
+  using namespace vsp;
+  const char* who = "vsp_layer_norm";
+  if (const int st = norm_check(rows, d, who); st != OK) return st;
+  if (rows == 0) return OK;
+  if (!x || !gain || !y || (residual && !sum_out)) return fail(ERR_ARG, "%s: null pointer", who);
+  return by_types(x_type, residual_type, y_type, who, [&](auto a, auto b, auto c) {
+    return norm_forward<typename decltype(a)::T, typename decltype(b)::T, typename decltype(c)::T>(
+        x, residual, gain, bias, sum_out, y, stats, rows, d, eps, reinterpret_cast<hipStream_t>(stream), who);
+  });
+}
+
+extern "C" size_t vsp_layer_norm_backward_workspace_bytes(int rows, int d) {
+  if (rows <= 0 || d <= 0) return 0;
+  return (size_t)vsp::norm_parts(rows, d) * 2 * d * sizeof(float);
+}
+
+extern "C" int vsp_layer_norm_backward(const void* x, const void* residual, const float* gain, const float* stats,
+                                       const void* dy, const void* dsum, void* dx, void* dresidual, float* dgain, float* dbias,
+                                       void* workspace, size_t workspace_bytes, int x_type, int residual_type, int y_type,
+                                       int rows, int d, void* stream) {
+  using namespace vsp;
+  const char* who = "vsp_layer_norm_backward";
+  if (const int st = norm_check(rows, d, who); st != OK) return st;
+  if (rows == 0) return fail(ERR_ARG, "%s: no rows", who);
+  if (!x || !gain || !stats || !dy || !dx || !dgain || !workspace) return fail(ERR_ARG, "%s: null pointer", who);
+  if (workspace_bytes < vsp_layer_norm_backward_workspace_bytes(rows, d))
+    return fail(ERR_ARG, "%s: workspace of %zu bytes, needs %zu", who, workspace_bytes, vsp_layer_norm_backward_workspace_bytes(rows, d));
+  return by_types(x_type, residual_type, y_type, who, [&](auto a, auto b, auto c) {
+    return norm_backward<typename decltype(a)::T, typename decltype(b)::T, typename decltype(c)::T>(
+        x, residual, gain, stats, dy, dsum, dx, dresidual, dgain, dbias, static_cast<float*>(workspace), rows, d,
+        reinterpret_cast<hipStream_t>(stream), who);
+  });
+}

@@ -74,6 +74,7 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor,
                 mask: Tensor | None) -> tuple[Tensor, Tensor]:  # noqa: D102
+        ctx.set_materialize_grads(False)
         q, k, v, beta, g, state = (_aligned(t.detach()) for t in (q, k, v, beta, g, state))
         # each chunk's starting state and its Delta, for the backward
         nrec = int(_lib.library().vsp_gated_scan_records_bytes(*q.shape))
