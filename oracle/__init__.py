@@ -9,7 +9,8 @@ the algorithms the HIP kernels of ``vesper`` must reproduce:
 - ``oracle.loop``: the looped column with per-token halting and copy-forward (reference
   ``vesper/loop.py``, ``vesper/column.py``);
 - ``oracle.keys``: the causal key filter and key normalization before the scan (reference
-  ``vesper/column.py``, ``vesper/kernels/keys.py``).
+  ``vesper/column.py``, ``vesper/kernels/keys.py``);
+- ``oracle.gated``: the gated delta rule and the layer norm (no counterpart in the reference).
 
 Only ``tests/``, ``__graft_entry__.smoke()`` and the CPU-baseline leg of ``bench.py`` may import
 this package, and only as the checker (or as the timed CPU baseline); the product path never
