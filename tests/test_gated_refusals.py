@@ -160,3 +160,39 @@ def test_workspace_sizes():
     assert lib.vsp_gated_scan_records_bytes(0, 130, 3, 64) == 0
     assert lib.vsp_layer_norm_backward_workspace_bytes(10, 768) == 3 * 2 * 768 * 4
     assert lib.vsp_layer_norm_backward_workspace_bytes(0, 768) == 0
+
+
+def test_a_sublayer_s_first_parameters_are_drawn_as_without_decay():
+    from vesper.column import RecurrentSublayer
+
+    plain = RecurrentSublayer(32, 4, key_conv=3, generator=torch.Generator().manual_seed(1))
+    gated = RecurrentSublayer(32, 4, key_conv=3, generator=torch.Generator().manual_seed(1), decay=True, norm=True)
+    shared = dict(gated.named_parameters())
+    for name, p in plain.named_parameters():
+        assert torch.equal(p, shared.pop(name)), name
+    assert set(shared) == {"w_decay", "decay_rate", "norm_gain", "norm_bias"}
+    x = torch.randn(2, 5, 32)
+    assert plain.decays(x) is None and plain.normalize(x) is x
+    g = gated.decays(x)
+    assert g.shape == (2, 5, 4) and g.dtype == F32 and bool((g < 0).all())
+    want = -torch.exp(gated.decay_rate) * torch.log1p(torch.exp(x @ gated.w_decay.t()))
+    assert torch.allclose(g, want, rtol=1e-5, atol=1e-7)
+    y = gated.normalize(x.to(BF16))
+    assert y.dtype == BF16 and float(y.detach().float().mean(-1).abs().max()) < 2.0**-8 * 4
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_reference_scan_with_decays(dtype):
+    from oracle.gated import gated_scan
+    from vesper.column import recurrent_scan
+
+    gen = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(2, 70, 3, 8, generator=gen).to(dtype) for _ in range(3))
+    k = torch.nn.functional.normalize(k.float(), dim=-1).to(dtype)
+    beta, g = torch.rand(2, 70, 3, generator=gen).to(dtype), -torch.rand(2, 70, 3, generator=gen)
+    state = torch.randn(2, 3, 8, 8, generator=gen)
+    o, after = recurrent_scan("reference", q, k, v, beta, state, g=g)
+    want, last = gated_scan(*(t.double() for t in (q, k, v, beta, g, state)))
+    assert o.dtype == dtype and after.dtype == F32
+    assert float((o.double() - want).norm() / want.norm()) < (2.0**-8 if dtype == BF16 else 1e-5)
+    assert float((after.double() - last).norm() / last.norm()) < 1e-5

@@ -16,6 +16,8 @@ driver written against the reference keeps its checks:
 - ``RecurrentSublayer``: the projections around the scan: ``project`` (``q``, the key input
   ``z``, ``v``, ``beta = sigmoid(W_beta x)``), ``keys`` (the causal key filter and
   ``normalize_keys``, ``recurrent_keys``), ``scan`` (the chosen scan and ``W_o``).
+  With ``decay`` its state forgets: ``decays`` gives each token's log decay a head and the scan is the gated delta rule
+  (``gated_delta_scan``); with ``norm`` it normalizes its input (``layer_norm``). Neither is in the reference.
 - ``recurrent_scan``: the scan part of ``RecurrentSublayer.scan`` (``column.py:291-326``).
 - ``recurrent_keys``: ``RecurrentSublayer.keys`` (``column.py:255-289``) on the key filter kernel.
 """
@@ -37,7 +39,9 @@ from vesper.kernels.delta_scan import (
     delta_scan_fused_fp32,
     fused_scan_available,
 )
-from vesper.recurrence import delta_scan_chunked
+from vesper.kernels.gated_scan import GATE_DTYPE, gated_delta_scan
+from vesper.kernels.layer_norm import layer_norm
+from vesper.recurrence import delta_scan_chunked, gated_delta_scan_chunked
 
 ScanImpl = Literal["reference", "fused", "fused-fp32"]
 SCAN_IMPLS: tuple[ScanImpl, ...] = ("reference", "fused", "fused-fp32")
@@ -126,13 +130,14 @@ def scan_of(model: nn.Module) -> ScanImpl:
 
 
 def recurrent_scan(impl: str, q: Tensor, k: Tensor, v: Tensor, beta: Tensor, state: Tensor, *,
-                   active: Tensor | None = None, block: int = 64) -> tuple[Tensor, Tensor]:
+                   active: Tensor | None = None, block: int = 64, g: Tensor | None = None) -> tuple[Tensor, Tensor]:
     """The scan of ``RecurrentSublayer.scan`` without its output projection: ``(o, state')``.
 
     ``q, k, v [b, n, h, dk]`` and ``beta [b, n, h]`` in the projections' dtype; ``state
     [b, h, dk, dk]``. The HIP scans take their input dtype with autocast off and return ``o`` in
     ``q``'s dtype and the state in float32; the reference scan runs in ``promote_types(dtype,
-    float32)`` (``column.py:316-325``) and returns its state in that dtype.
+    float32)`` (``column.py:316-325``) and returns its state in that dtype. With log decays ``g [b, n, h]`` (at most 0)
+    it is the gated delta rule, each implementation's own.
 
     Raises:
         ValueError: as ``check_scan``.
@@ -142,14 +147,20 @@ def recurrent_scan(impl: str, q: Tensor, k: Tensor, v: Tensor, beta: Tensor, sta
     if chosen == "reference":
         compute = torch.promote_types(q.dtype, torch.float32)
         with torch.autocast(device_type=q.device.type, enabled=False):
-            o, new_state = delta_scan_chunked(q.to(compute), k.to(compute), v.to(compute), beta.to(compute),
-                                              state.to(compute), block, active=active)
+            tokens = (q.to(compute), k.to(compute), v.to(compute), beta.to(compute))
+            if g is None:
+                o, new_state = delta_scan_chunked(*tokens, state.to(compute), block, active=active)
+            else:
+                o, new_state = gated_delta_scan_chunked(*tokens, g.to(compute), state.to(compute), block, active=active)
         return o.to(q.dtype), new_state
     kernel = delta_scan_fused if chosen == "fused" else delta_scan_fused_fp32
     dtype = FUSED_INPUT_DTYPES[chosen]
     with torch.autocast(device_type=q.device.type, enabled=False):
-        o, new_state = kernel(q.to(dtype), k.to(dtype), v.to(dtype), beta.to(dtype), state.to(STATE_DTYPE),
-                              active=active)
+        tokens = (q.to(dtype), k.to(dtype), v.to(dtype), beta.to(dtype))
+        if g is None:
+            o, new_state = kernel(*tokens, state.to(STATE_DTYPE), active=active)
+        else:
+            o, new_state = gated_delta_scan(*tokens, g.to(GATE_DTYPE), state.to(STATE_DTYPE), active=active)
     return o.to(q.dtype), new_state
 
 
@@ -159,10 +170,14 @@ class RecurrentSublayer(nn.Module):
     ``w_q, w_k, w_v, w_o`` of ``[d, d]`` and ``w_beta`` of ``[h, d]``, drawn ``N(0, 1/d)`` in that
     order, then the optional causal key filter ``conv_k [K, d]`` ~ ``U(-1/sqrt(K), 1/sqrt(K))``
     (``column.py:216-233``). ``scan_impl`` is module state (``set_scan``), never a parameter.
+
+    With ``decay`` the log decays are ``g = -e^rate softplus(W_decay x)``, ``w_decay [h, d]`` ~ ``N(0, 1/d)`` drawn after
+    the others and the rates ``e^decay_rate [h]`` from 1e-3 to 1 over the heads, so that some remember thousands of tokens
+    and some a few. With ``norm`` the input is normalized first (``norm_gain`` ones, ``norm_bias`` zeros ``[d]``).
     """
 
     def __init__(self, d: int, heads: int, key_conv: int = 0, block: int = 64,
-                 generator: torch.Generator | None = None) -> None:
+                 generator: torch.Generator | None = None, *, decay: bool = False, norm: bool = False) -> None:
         super().__init__()
         if d % heads != 0:
             raise ValueError(f"heads ({heads}) must divide d ({d})")
@@ -180,6 +195,36 @@ class RecurrentSublayer(nn.Module):
         if key_conv:
             bound = 1.0 / math.sqrt(key_conv)
             self.conv_k = nn.Parameter(torch.rand(key_conv, d, generator=generator) * (2 * bound) - bound)
+        self.w_decay: nn.Parameter | None = None
+        self.decay_rate: nn.Parameter | None = None
+        if decay:
+            self.w_decay = nn.Parameter(torch.randn(heads, d, generator=generator) * std)
+            self.decay_rate = nn.Parameter(torch.linspace(math.log(1e-3), 0.0, heads))
+        self.norm_gain: nn.Parameter | None = None
+        self.norm_bias: nn.Parameter | None = None
+        if norm:
+            self.norm_gain, self.norm_bias = nn.Parameter(torch.ones(d)), nn.Parameter(torch.zeros(d))
+
+    def normalize(self, x: Tensor) -> Tensor:
+        """The input's layer norm in its dtype (``x`` itself without ``norm``): the kernel where a HIP scan is chosen, plain
+        PyTorch for the "reference" scan."""
+        if self.norm_gain is None or self.norm_bias is None:
+            return x
+        if self.scan_impl == "reference":
+            compute = torch.promote_types(x.dtype, torch.float32)
+            return nn.functional.layer_norm(x.to(compute), x.shape[-1:], self.norm_gain.to(compute), self.norm_bias.to(compute)).to(x.dtype)
+        y = layer_norm(x, self.norm_gain.to(torch.float32), self.norm_bias.to(torch.float32))
+        assert isinstance(y, Tensor)
+        return y
+
+    def decays(self, x: Tensor) -> Tensor | None:
+        """The log decays ``[b, n, h]`` of ``x [b, n, d]``, in float32 or wider (None without ``decay``)."""
+        if self.w_decay is None or self.decay_rate is None:
+            return None
+        logits = nn.functional.linear(x, self.w_decay)
+        with torch.autocast(device_type=x.device.type, enabled=False):
+            wide = torch.promote_types(logits.dtype, torch.float32)
+            return -torch.exp(self.decay_rate.to(wide)) * nn.functional.softplus(logits.to(wide))
 
     def project(self, x: Tensor) -> tuple[Tensor, Tensor, Tensor, Tensor]:
         """``[b, n, d]`` to ``q [b, n, h, dk]`` (not normalized), the key input ``z [b, n, d]``,
@@ -194,16 +239,19 @@ class RecurrentSublayer(nn.Module):
         """Normalized keys and the next key history (``column.py:255-289``) on the key kernel."""
         return recurrent_keys(z, history, self.conv_k, self.heads)
 
-    def scan(self, q: Tensor, k: Tensor, v: Tensor, beta: Tensor, state: Tensor) -> tuple[Tensor, Tensor]:
+    def scan(self, q: Tensor, k: Tensor, v: Tensor, beta: Tensor, state: Tensor,
+             g: Tensor | None = None) -> tuple[Tensor, Tensor]:
         """The chosen scan and the output projection: ``(y [b, n, d], state')`` (``column.py:291-326``)."""
-        o, new_state = recurrent_scan(self.scan_impl, q, k, v, beta, state, block=self.block)
+        o, new_state = recurrent_scan(self.scan_impl, q, k, v, beta, state, block=self.block, g=g)
         return nn.functional.linear(o.flatten(2), self.w_o), new_state
 
     def forward(self, x: Tensor, state: Tensor, history: Tensor) -> tuple[Tensor, Tensor, Tensor]:
         """Project, make the keys, scan: ``(y, state', history')`` (``column.py:328-350``)."""
+        x = self.normalize(x)
         q, z, v, beta = self.project(x)
         k, history_next = self.keys(z, history)
-        y, state_next = self.scan(q, k, v, beta, state)
+        g = self.decays(x)
+        y, state_next = self.scan(q, k, v, beta, state, *(() if g is None else (g,)))
         return y, state_next, history_next
 
 
