@@ -26,6 +26,9 @@
 namespace vsp {
 namespace gated {
 
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
 constexpr int kChunk = 64;
 constexpr int kPieces = 3;
 constexpr double kLeastDecay = -1e4;  // log decays below it: their exponentials are zero either way
@@ -69,18 +72,53 @@ __device__ __forceinline__ void split4(f32x4 x, bf16x4 (&out)[N]) {
 __device__ __forceinline__ int lane_col() { return threadIdx.x & 15; }
 __device__ __forceinline__ int lane_grp() { return (threadIdx.x & 63) >> 4; }
 
-// Eight elements of a row from k0 + 8 g (zeros where not `ok`); rows are 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ Operand<T, 1> load_row(const T* p, bool ok) {
-  Operand<T, 1> o;
-  if constexpr (sizeof(T) == 2) {
-    o.p[0] = ok ? *reinterpret_cast<const bf16x8*>(p) : bf16x8{};
-  } else {
-    o.lo = ok ? reinterpret_cast<const f32x4*>(p)[0] : zero4();
-    o.hi = ok ? reinterpret_cast<const f32x4*>(p)[1] : zero4();
+// ---- one head's rows of a chunk in [B, N, H, D], through a buffer resource: rows past the sequence and features past D
+// read zeros and drop writes, so that no load is followed by a select (which would wait for it) and none is conditional
+// (a wait for an older load could not count the newer ones) ----
+constexpr unsigned kNowhere = 0x7ffffff0u;  // an offset past every range
+
+template <typename T> struct Rows {
+  __amdgpu_buffer_rsrc_t r;
+  unsigned pitch;  // bytes of a token's H heads
+  int D;
+  __device__ __forceinline__ unsigned at(int row, int f) const {
+    return f < D ? (unsigned)row * pitch + (unsigned)f * (unsigned)sizeof(T) : kNowhere;
   }
-  return o;
-}
+  // eight elements of a row, from feature f (a multiple of 8)
+  __device__ __forceinline__ Operand<T, 1> row(int row, int f) const {
+    const unsigned o = at(row, f);
+    Operand<T, 1> x;
+    if constexpr (sizeof(T) == 2) {
+      x.p[0] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0));
+    } else {
+      x.lo = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0));
+      x.hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o + 16, 0, 0));
+    }
+    return x;
+  }
+  __device__ __forceinline__ T one(int row, int f) const {
+    if constexpr (sizeof(T) == 2) {
+      return __builtin_bit_cast(T, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at(row, f), 0, 0));
+    } else {
+      return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, at(row, f), 0, 0));
+    }
+  }
+  __device__ __forceinline__ void put_one(int row, int f, T x) const {
+    if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, x), r, at(row, f), 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), r, at(row, f), 0, 0);
+  }
+  // four elements from feature f (a multiple of 4)
+  __device__ __forceinline__ void put_four(int row, int f, f32x4 x) const {
+    if constexpr (sizeof(T) == 2) {
+      bf16x4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = (__bf16)x[i];
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, y), r, at(row, f), 0, 0);
+    } else {
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), r, at(row, f), 0, 0);
+    }
+  }
+};
 
 // Column f0 + c of rows 32 s + 8 g .. + 7 of a row-major LDS tile [token][feature].
 template <typename T>
@@ -154,6 +192,20 @@ template <> struct Pieces<float> { static constexpr int kN = 1; };
 template <typename T> struct OutPieces { static constexpr int kN = 2; };
 template <> struct OutPieces<float> { static constexpr int kN = 1; };
 
+// A chunk's record of one value column a lane: float32 [D][rows], written four at a time; columns and rows past the
+// width are dropped.
+struct Record {
+  __amdgpu_buffer_rsrc_t r;
+  int rows, D;
+  __device__ __forceinline__ void put(int col, int row, f32x4 x) const {
+    const unsigned o = col < D && row < rows ? ((unsigned)col * rows + row) * 4u : kNowhere;
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), r, o, 0, 0);
+  }
+};
+__device__ __forceinline__ Record record(float* base, size_t chunk, int rows, int D) {
+  return {buffer_rsrc(base + chunk * rows * D, (unsigned)rows * D * 4u), rows, D};
+}
+
 // LDS writes before, LDS reads after, for the whole workgroup; loads from memory stay in flight.
 __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -166,6 +218,17 @@ struct Dims {
   int N, H, D, chunks;
   // element offset of token t of head h in [B, N, H, D]
   __device__ __forceinline__ size_t at(int b, int t, int h) const { return (((size_t)b * N + t) * H + h) * D; }
+  // the rows of head h from token t0 to the end of its chunk or of the sequence
+  __device__ __forceinline__ Rows<T> rows(const T* p, int b, int t0, int h) const {
+    const int count = N - t0 < kChunk ? N - t0 : kChunk;
+    const unsigned pitch = (unsigned)H * D * sizeof(T);
+    return {buffer_rsrc(p + at(b, t0, h), (count - 1) * pitch + (unsigned)(D * sizeof(T))), pitch, D};
+  }
+  // the bytes of a chunk's flags; without flags an empty range
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t flags(const uint8_t* p, int b, int t0) const {
+    const int count = N - t0 < kChunk ? N - t0 : kChunk;
+    return buffer_rsrc(p == nullptr ? p : p + (size_t)b * N + t0, p == nullptr ? 0u : (unsigned)count);
+  }
 };
 
 // ---- launchers shared between the translation units ----

@@ -64,7 +64,9 @@ template <typename T, int DP> struct BackTile {  // a quarter of a tile of keys 
 
 template <typename T, int DP> struct BackSide {  // what the other waves read of the next chunk, besides the queries
   Operand<T, Pieces<T>::kN> pf[2];
-  f32x4 d_o, eps;
+  f32x4 eps;
+  T d_o[4];
+  uint8_t on[4];
 };
 
 template <typename T, int DP>
@@ -100,16 +102,12 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
       if (ft < S::TILES) F::put(lds.state, ft, dh[i]);
     }
     auto load = [&](int ci, BackIn<T, DP>& in) {
-      const int t0 = ci * kChunk, t = t0 + 16 * w + c;
+      const Rows<T> krows = dims.rows(k, b, ci * kChunk, h);
 #pragma unroll
-      for (int st = 0; st < KS; ++st) {
-        const int f = 32 * st + 8 * grp;
-        const bool ok = t < dims.N && f < D;
-        in.kf[st] = load_row(k + dims.at(b, ok ? t : t0, h) + (ok ? f : 0), ok);
-      }
+      for (int st = 0; st < KS; ++st) in.kf[st] = krows.row(16 * w + c, 32 * st + 8 * grp);
       const T* tb = tf + (chunk0 + ci) * Factor<T, NT>::kElems + col_step(w, 0) * F::kStep;
       in.tf[0] = F::get(tb, 0);
-      if (w < 2) in.tf[1] = F::get(tb, 1);
+      in.tf[1] = F::get(tb, w < 2 ? 1 : 0);
       const float* co = coef + (chunk0 + ci) * kCoef + 16 * w + 4 * grp;
       in.beta = *reinterpret_cast<const f32x4*>(co);
       in.eps = *reinterpret_cast<const f32x4*>(co + kChunk);
@@ -117,12 +115,9 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
       in.gam = coef[(chunk0 + ci) * kCoef + 2 * kChunk - 1];
     };
     auto step = [&](int ci, const BackIn<T, DP>& in) {
-      float* rh = rec_dh + ((chunk0 + ci) * D + vcol) * D;
+      const Record rh = record(rec_dh, chunk0 + ci, D, D);
 #pragma unroll
-      for (int i = 0; i < FT; ++i) {
-        const int f = 16 * (w + 4 * i) + 4 * grp;
-        if (vcol < D && f < D) *reinterpret_cast<f32x4*>(rh + f) = dh[i];
-      }
+      for (int i = 0; i < FT; ++i) rh.put(vcol, 16 * (w + 4 * i) + 4 * grp, dh[i]);
       // dDelta = P^T dO + kap (K dH')
       f32x4 x = zero4();
 #pragma unroll
@@ -148,14 +143,10 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
 #pragma unroll
       for (int i = 0; i < FT; ++i)
         add[i] = w + 4 * i < S::TILES ? *reinterpret_cast<const f32x4*>(lds.qdo + ((w + 4 * i) * 64 + lane) * 4) : zero4();
-      if (vcol < D) {
-        *reinterpret_cast<f32x4*>(rec_dr + ((chunk0 + ci) * D + vcol) * kChunk + 16 * w + 4 * grp) = dr;
+      record(rec_dr, chunk0 + ci, kChunk, D).put(vcol, 16 * w + 4 * grp, dr);
+      const Rows<T> dvrows = dims.rows(dv, b, ci * kChunk, h);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int t = ci * kChunk + 16 * w + 4 * grp + r;
-          if (t < dims.N) dv[dims.at(b, t, h) + vcol] = from_f32<T>(in.beta[r] * dr[r]);
-        }
-      }
+      for (int r = 0; r < 4; ++r) dvrows.put_one(16 * w + 4 * grp + r, vcol, from_f32<T>(in.beta[r] * dr[r]));
       lds_barrier();
       // dH = gam dH' + Q^T (eps dO) - K^T (beta eps dR)
       const Operand<T, NT> y0 = F::get(lds.dread, 0), y1 = F::get(lds.dread, 1);
@@ -176,13 +167,12 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
     load(nc - 1, a);
     lds_barrier();
     lds_barrier();
-    for (int ci = nc - 1; ci >= 0; ci -= 2) {
-      if (ci >= 1) load(ci - 1, bb);
+    for (int ci = nc - 1; ci >= 0; ci -= 2) {  // past the first chunk it is loaded again, so that no load is conditional
+      load(ci >= 1 ? ci - 1 : 0, bb);
       step(ci, a);
-      if (ci >= 1) {
-        if (ci >= 2) load(ci - 2, a);
-        step(ci - 1, bb);
-      }
+      if (ci < 1) break;
+      load(ci >= 2 ? ci - 2 : 0, a);
+      step(ci - 1, bb);
     }
     float* so = d_state_in + (size_t)bh * D * D;
 #pragma unroll
@@ -197,11 +187,11 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
     //      Q^T (eps dO), each in one of the three spans between barriers ----
     const int hl = threadIdx.x - 256;
     auto load_tile = [&](const T* src, int ci, BackTile<T, DP>& in) {
+      const Rows<T> rows = dims.rows(src, b, ci * kChunk, h);
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) {
-        const int p = hl + 256 * i, row = p / (DP / 8), f = 8 * (p % (DP / 8)), t0 = ci * kChunk;
-        const bool ok = t0 + row < dims.N && f < D;
-        in.x[i] = load_row(src + dims.at(b, ok ? t0 + row : t0, h) + (ok ? f : 0), ok);
+        const int p = hl + 256 * i;
+        in.x[i] = rows.row(p / (DP / 8), 8 * (p % (DP / 8)));
       }
     };
     auto put_tile = [&](T* dst, const BackTile<T, DP>& in) {
@@ -220,22 +210,24 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
     auto load_side = [&](int ci, BackSide<T, DP>& in) {
       const T* pb = pf + (chunk0 + ci) * Factor<T, NT>::kElems + col_step(w, 0) * F::kStep;
       in.pf[0] = F::get(pb, 0);
-      if (w < 2) in.pf[1] = F::get(pb, 1);
+      in.pf[1] = F::get(pb, w < 2 ? 1 : 0);
       in.eps = *reinterpret_cast<const f32x4*>(coef + (chunk0 + ci) * kCoef + kChunk + 16 * w + 4 * grp);
-      const int t0 = ci * kChunk;
+      const Rows<T> rows = dims.rows(d_o, b, ci * kChunk, h);
+      const __amdgpu_buffer_rsrc_t flags = dims.flags(active, b, ci * kChunk);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int t = t0 + 16 * w + 4 * grp + r;
-        const bool ok = t < dims.N && vcol < D && (active == nullptr || active[(size_t)b * dims.N + t] != 0);
-        const float x = to_f32(d_o[dims.at(b, ok ? t : t0, h) + (ok ? vcol : 0)]);
-        in.d_o[r] = ok ? x : 0.f;
+        in.d_o[r] = rows.one(16 * w + 4 * grp + r, vcol);
+        in.on[r] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(flags, 16 * w + 4 * grp + r, 0, 0);
       }
     };
     auto put_side = [&](const BackSide<T, DP>& in) {
-      F1::put(lds.d_o, w, in.d_o);
-      f32x4 e;
+      f32x4 x, e;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) e[r] = in.eps[r] * in.d_o[r];
+      for (int r = 0; r < 4; ++r) {
+        x[r] = active == nullptr || in.on[r] ? to_f32(in.d_o[r]) : 0.f;
+        e[r] = in.eps[r] * x[r];
+      }
+      F1::put(lds.d_o, w, x);
       F::put(lds.edo, w, e);
     };
     auto form_z = [&](const BackSide<T, DP>& in) {
@@ -253,14 +245,11 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
         return load_columns(lds.queries, S::PITCH, s, f0);
       } else {
         Operand<T, 1> x;
-        const int f = f0 + c, t0 = ci * kChunk;
+        const Rows<T> rows = dims.rows(q, b, ci * kChunk, h);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int t = t0 + 32 * s + 8 * grp + e;
-          const bool ok = t < dims.N && f < D;
-          const float y = q[dims.at(b, ok ? t : t0, h) + (ok ? f : 0)];
-          if (e < 4) x.lo[e & 3] = ok ? y : 0.f;
-          else x.hi[e & 3] = ok ? y : 0.f;
+        for (int e = 0; e < 4; ++e) {
+          x.lo[e] = rows.one(32 * s + 8 * grp + e, f0 + c);
+          x.hi[e] = rows.one(32 * s + 8 * grp + 4 + e, f0 + c);
         }
         return x;
       }
@@ -287,26 +276,20 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
     lds_barrier();
     form_z(side);
     form_qdo(nc - 1);
-    if (nc > 1) {
-      if constexpr (S::kStageQ) load_tile(q, nc - 2, queries);
-      load_side(nc - 2, side);
-    }
+    if constexpr (S::kStageQ) load_tile(q, nc > 1 ? nc - 2 : 0, queries);
+    load_side(nc > 1 ? nc - 2 : 0, side);
     lds_barrier();
-    for (int ci = nc - 1; ci >= 0; --ci) {
+    for (int ci = nc - 1; ci >= 0; --ci) {  // past the first chunk it is formed again, so that nothing is conditional
       put_tile(lds.keys, keys);
-      if (ci >= 1) {
-        load_tile(k, ci - 1, keys);
-        if constexpr (S::kStageQ) put_tile(lds.queries, queries);
-        put_side(side);
-      }
+      load_tile(k, ci >= 1 ? ci - 1 : 0, keys);
+      if constexpr (S::kStageQ) put_tile(lds.queries, queries);
+      put_side(side);
       lds_barrier();
-      if (ci >= 1) form_z(side);
-      if (ci >= 2) {
-        if constexpr (S::kStageQ) load_tile(q, ci - 2, queries);
-        load_side(ci - 2, side);
-      }
+      form_z(side);
+      if constexpr (S::kStageQ) load_tile(q, ci >= 2 ? ci - 2 : 0, queries);
+      load_side(ci >= 2 ? ci - 2 : 0, side);
       lds_barrier();
-      if (ci >= 1) form_qdo(ci - 1);
+      form_qdo(ci >= 1 ? ci - 1 : 0);
       lds_barrier();
     }
   }
@@ -410,18 +393,6 @@ __device__ __forceinline__ f32x4 four(const T* p) {
   return x;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_four(T* p, f32x4 x) {
-  if constexpr (sizeof(T) == 2) {
-    bf16x4 y;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) y[r] = (__bf16)x[r];
-    *reinterpret_cast<bf16x4*>(p) = y;
-  } else {
-    *reinterpret_cast<f32x4*>(p) = x;
-  }
-}
-
 template <typename T, int DP> struct GradShape {
   static constexpr int TILES = DP / 16;
   static constexpr int NT = Pieces<T>::kN;
@@ -491,6 +462,14 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(
   for (int i = 0; i < 4; ++i) pt[i] = bt[i] = pr[i] = br[i] = zero4();
   float inner = 0.f, dot_v = 0.f;
   const int token = t0 + 16 * w + c;
+  const Rows<T> dorows = dims.rows(d_o, b, t0, h), vrows = dims.rows(v, b, t0, h);
+  bool on[4];  // of token 16 i + c
+  {
+    const __amdgpu_buffer_rsrc_t flags = dims.flags(active, b, t0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      on[i] = active == nullptr || (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(flags, 16 * i + c, 0, 0) != 0;
+  }
   for (int v0 = 0; v0 < D; v0 += 32) {
     if (v0 > 0) __syncthreads();
     constexpr int QUADS = DP / 4;
@@ -516,13 +495,8 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(
     Operand<T, 1> dof[4];
     const int vc = v0 + 8 * grp;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = t0 + 16 * i + c;
-      const bool ok = t < dims.N && vc < D && (active == nullptr || active[(size_t)b * dims.N + t] != 0);
-      dof[i] = load_row(d_o + dims.at(b, ok ? t : t0, h) + (ok ? vc : 0), ok);
-    }
-    const bool vok = token < dims.N && vc < D;
-    const Operand<T, 1> vf = load_row(v + dims.at(b, vok ? token : t0, h) + (vok ? vc : 0), vok);
+    for (int i = 0; i < 4; ++i) dof[i] = dorows.row(16 * i + c, on[i] ? vc : D);
+    const Operand<T, 1> vf = vrows.row(16 * w + c, vc);
     __syncthreads();
     const Operand<T, NT> del_w = lds.u.values.delta.columns(16 * w), dr_w = lds.u.values.dr.columns(16 * w);
     dot_v += operand_dot(dr_w, vf);
@@ -559,11 +533,11 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(
   // ---- the keys and queries, the decays between pairs, sums over the chunk's tokens ----
   {
     constexpr int PIECES = kChunk * (DP / 8);
+    const Rows<T> krows = dims.rows(k, b, t0, h), qrows = dims.rows(q, b, t0, h);
+#pragma unroll
     for (int p = threadIdx.x; p < PIECES; p += 256) {
       const int row = p / (DP / 8), f = 8 * (p % (DP / 8));
-      const bool ok = t0 + row < dims.N && f < D;
-      const size_t at = dims.at(b, ok ? t0 + row : t0, h) + (ok ? f : 0);
-      const Operand<T, 1> x = load_row(k + at, ok), y = load_row(q + at, ok);
+      const Operand<T, 1> x = krows.row(row, f), y = qrows.row(row, f);
       T *kd = lds.u.rows.keys + row * S::PITCH + f, *qd = lds.u.rows.queries + row * S::PITCH + f;
       if constexpr (sizeof(T) == 2) {
         *reinterpret_cast<bf16x8*>(kd) = x.p[0];
@@ -634,7 +608,7 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(
 
   // ---- out ----
   float dot_q = 0.f, dot_y = 0.f, dot_c = 0.f;
-  const size_t out = dims.at(b, token < dims.N ? token : t0, h);
+  const Rows<T> dqrows = dims.rows(dq, b, t0, h), dkrows = dims.rows(dk, b, t0, h);
 #pragma unroll
   for (int i = 0; i < TILES; ++i) {
     const int f = 16 * i + 4 * grp;
@@ -648,10 +622,8 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(
       dot_c += kx[r] * ac[i][r];
       x[r] = beta_own * y + ac[i][r];
     }
-    if (token < dims.N && f < D) {
-      store_four(dq + out + f, aq[i]);
-      store_four(dk + out + f, x);
-    }
+    dqrows.put_four(own, f, aq[i]);
+    dkrows.put_four(own, f, x);
   }
   dot_q = sum_over_rows(dot_q);
   dot_y = sum_over_rows(dot_y);

@@ -50,7 +50,7 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ beta, const float* __restrict__ g,
     float* __restrict__ coef, T* __restrict__ tf, T* __restrict__ pf, Dims<T> dims, int total) {
   __shared__ PrepLds lds[kPrepWaves];
-  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, c = l & 15, grp = l >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, c = l & 15, grp = l >> 4;
   const int id = blockIdx.x * kPrepWaves + wave;
   if (id >= total) return;  // whole waves; no workgroup barrier below
   PrepLds& s = lds[wave];
@@ -86,17 +86,14 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
   f32x4 mult[10], pp[10];
 #pragma unroll
   for (int t = 0; t < 10; ++t) mult[t] = pp[t] = zero4();
+  const Rows<T> krows = dims.rows(k, b, t0, h), qrows = dims.rows(q, b, t0, h);
 #pragma unroll
   for (int st = 0; st < KS; ++st) {
     Operand<T, 1> kf[4], qf[4];
-    const int f = 32 * st + 8 * grp;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int t = t0 + 16 * i + c;
-      const bool ok = t < dims.N && f < dims.D;
-      const size_t at = dims.at(b, ok ? t : t0, h) + (ok ? f : 0);
-      kf[i] = load_row(k + at, ok);
-      qf[i] = load_row(q + at, ok);
+      kf[i] = krows.row(16 * i + c, 32 * st + 8 * grp);
+      qf[i] = qrows.row(16 * i + c, 32 * st + 8 * grp);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -287,37 +284,25 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
     }
     auto load = [&](int ci, ChainIn<T, DP>& in) {
       const int t0 = ci * kChunk;
-      const int t = t0 + 16 * w + c;
+      const Rows<T> krows = dims.rows(k, b, t0, h), vrows = dims.rows(v, b, t0, h);
 #pragma unroll
-      for (int st = 0; st < KS; ++st) {
-        const int f = 32 * st + 8 * grp;
-        const bool ok = t < dims.N && f < D;
-        in.kf[st] = load_row(k + dims.at(b, ok ? t : t0, h) + (ok ? f : 0), ok);
-      }
+      for (int st = 0; st < KS; ++st) in.kf[st] = krows.row(16 * w + c, 32 * st + 8 * grp);
       const T* tb = tf + (chunk0 + ci) * Factor<T, NT>::kElems + row_step(w, 0) * F::kStep;
       in.tf[0] = F::get(tb, 0);
-      if (w >= 2) in.tf[1] = F::get(tb, 1);
+      in.tf[1] = F::get(tb, w >= 2 ? 1 : 0);
       const float* co = coef + (chunk0 + ci) * kCoef + 16 * w + 4 * grp;
       in.beta = *reinterpret_cast<const f32x4*>(co);
       in.eps = *reinterpret_cast<const f32x4*>(co + kChunk);
       in.kap = *reinterpret_cast<const f32x4*>(co + 2 * kChunk);
       in.gam = coef[(chunk0 + ci) * kCoef + 2 * kChunk - 1];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int tr = t0 + 16 * w + 4 * grp + r;
-        const bool ok = tr < dims.N && vcol < D;
-        const T x = v[dims.at(b, ok ? tr : t0, h) + (ok ? vcol : 0)];
-        in.v[r] = ok ? x : from_f32<T>(0.f);
-      }
+      for (int r = 0; r < 4; ++r) in.v[r] = vrows.one(16 * w + 4 * grp + r, vcol);
     };
     auto step = [&](int ci, const ChainIn<T, DP>& in) {
       if constexpr (RECORD) {
-        float* rh = rec_h + ((chunk0 + ci) * D + vcol) * D;
+        const Record rh = record(rec_h, chunk0 + ci, D, D);
 #pragma unroll
-        for (int i = 0; i < FT; ++i) {
-          const int f = 16 * (w + 4 * i) + 4 * grp;
-          if (vcol < D && f < D) *reinterpret_cast<f32x4*>(rh + f) = hs[i];
-        }
+        for (int i = 0; i < FT; ++i) rh.put(vcol, 16 * (w + 4 * i) + 4 * grp, hs[i]);
       }
       // R = beta (V - eps K H)
       f32x4 x = zero4();
@@ -335,8 +320,7 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
       for (int r = 0; r < 4; ++r) kd[r] = in.kap[r] * dl[r];
       F::put(lds.kept, w, kd);
       FO::put(lds.delta, w, dl);
-      if constexpr (RECORD)
-        if (vcol < D) *reinterpret_cast<f32x4*>(rec_d + ((chunk0 + ci) * D + vcol) * kChunk + 16 * w + 4 * grp) = dl;
+      if constexpr (RECORD) record(rec_d, chunk0 + ci, kChunk, D).put(vcol, 16 * w + 4 * grp, dl);
       lds_barrier();
       // H' = gam H + K^T (kap Delta)
       const Operand<T, NT> k0 = F::get(lds.kept, 0), k1 = F::get(lds.kept, 1);
@@ -356,13 +340,12 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
     ChainIn<T, DP> a, bb;
     load(0, a);
     lds_barrier();
-    for (int ci = 0; ci < nc; ci += 2) {
-      if (ci + 1 < nc) load(ci + 1, bb);
+    for (int ci = 0; ci < nc; ci += 2) {  // past the end the last chunk is loaded again, so that no load is conditional
+      load(ci + 1 < nc ? ci + 1 : ci, bb);
       step(ci, a);
-      if (ci + 1 < nc) {
-        if (ci + 2 < nc) load(ci + 2, a);
-        step(ci + 1, bb);
-      }
+      if (ci + 1 >= nc) break;
+      load(ci + 2 < nc ? ci + 2 : ci + 1, a);
+      step(ci + 1, bb);
     }
     float* so = s_out + (size_t)bh * D * D;
 #pragma unroll
@@ -377,25 +360,20 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
     const int hl = threadIdx.x - 256;  // 0 .. 255
     auto load = [&](int ci, OutIn<T, DP>& in) {
       const int t0 = ci * kChunk;
+      const Rows<T> krows = dims.rows(k, b, t0, h), qrows = dims.rows(q, b, t0, h);
 #pragma unroll
       for (int i = 0; i < OutIn<T, DP>::LOADS; ++i) {
-        const int p = hl + 256 * i, row = p / (DP / 8), f = 8 * (p % (DP / 8));
-        const bool ok = t0 + row < dims.N && f < D;
-        in.keys[i] = load_row(k + dims.at(b, ok ? t0 + row : t0, h) + (ok ? f : 0), ok);
+        const int p = hl + 256 * i;
+        in.keys[i] = krows.row(p / (DP / 8), 8 * (p % (DP / 8)));
       }
-      const int t = t0 + 16 * w + c;
 #pragma unroll
-      for (int st = 0; st < KS; ++st) {
-        const int f = 32 * st + 8 * grp;
-        const bool ok = t < dims.N && f < D;
-        in.qf[st] = load_row(q + dims.at(b, ok ? t : t0, h) + (ok ? f : 0), ok);
-      }
+      for (int st = 0; st < KS; ++st) in.qf[st] = qrows.row(16 * w + c, 32 * st + 8 * grp);
       using PF = FO;
       const T* pb = pf + (chunk0 + ci) * Factor<T, NO>::kElems + row_step(w, 0) * PF::kStep;
       in.pf[0] = PF::get(pb, 0);
-      if (w >= 2) in.pf[1] = PF::get(pb, 1);
+      in.pf[1] = PF::get(pb, w >= 2 ? 1 : 0);
       in.eps = coef[(chunk0 + ci) * kCoef + kChunk + 16 * w + c];
-      in.on = active == nullptr || t >= dims.N ? 1 : active[(size_t)b * dims.N + t];
+      in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, t0), 16 * w + c, 0, 0);
     };
     auto step = [&](int ci, const OutIn<T, DP>& in) {
 #pragma unroll
@@ -418,33 +396,20 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
       lds_barrier();
       acc = mma(FO::get(lds.delta, 0), in.pf[0], acc);
       if (w >= 2) acc = mma(FO::get(lds.delta, 1), in.pf[1], acc);
-      const int t = ci * kChunk + 16 * w + c, f = 16 * sl + 4 * grp;
-      if (t < dims.N && f < D) {
-        T* op = o + dims.at(b, t, h) + f;
-        if constexpr (sizeof(T) == 2) {
-          bf16x4 x;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = (__bf16)(in.on ? acc[r] : 0.f);
-          *reinterpret_cast<bf16x4*>(op) = x;
-        } else {
-          f32x4 x;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = in.on ? acc[r] : 0.f;
-          *reinterpret_cast<f32x4*>(op) = x;
-        }
-      }
+      for (int r = 0; r < 4; ++r) acc[r] = active == nullptr || in.on ? acc[r] : 0.f;
+      dims.rows(o, b, ci * kChunk, h).put_four(16 * w + c, 16 * sl + 4 * grp, acc);
       lds_barrier();
     };
     OutIn<T, DP> a, bb;
     load(0, a);
     lds_barrier();
-    for (int ci = 0; ci < nc; ci += 2) {
-      if (ci + 1 < nc) load(ci + 1, bb);
+    for (int ci = 0; ci < nc; ci += 2) {  // past the end the last chunk is loaded again, so that no load is conditional
+      load(ci + 1 < nc ? ci + 1 : ci, bb);
       step(ci, a);
-      if (ci + 1 < nc) {
-        if (ci + 2 < nc) load(ci + 2, a);
-        step(ci + 1, bb);
-      }
+      if (ci + 1 >= nc) break;
+      load(ci + 2 < nc ? ci + 2 : ci + 1, a);
+      step(ci + 1, bb);
     }
   }
 }
@@ -532,6 +497,8 @@ int check_sizes(int B, int N, int H, int D, const char* who) {
   if (B < 0 || N < 0 || H < 1) return fail(ERR_ARG, "%s: bad sizes B=%d N=%d H=%d", who, B, N, H);
   if (D < 8 || D > 256 || D % 8 != 0) return fail(ERR_UNSUPPORTED, "%s: head dimension %d (multiples of 8 in 8..256)", who, D);
   if (N > (1 << 30)) return fail(ERR_UNSUPPORTED, "%s: %d tokens a row (at most 2^30)", who, N);
+  // a chunk's rows are addressed by 32-bit offsets
+  if ((size_t)H * D > (size_t)1 << 22) return fail(ERR_UNSUPPORTED, "%s: tokens of %d x %d features (at most 2^22)", who, H, D);
   // launches of fewer than 2^32 threads, counts in 32 bits: a wave a chunk and head, 512 threads a slice
   if ((size_t)B * H * chunks_of(N) > (size_t)1 << 25 || (size_t)B * H * ((D + 15) / 16) > (size_t)1 << 22)
     return fail(ERR_UNSUPPORTED, "%s: B=%d N=%d H=%d (at most 2^25 chunks of 64 tokens, 2^22 slices of 16 value columns)", who, B, N, H);
