@@ -33,7 +33,9 @@ constexpr int kChunk = 64;
 constexpr int kPieces = 3;
 constexpr double kLeastDecay = -1e4;  // log decays below it: their exponentials are zero either way
 
-// ---- operands: 32 of a product's k a step; lane (c, g) = (l % 16, l / 16) holds row or column c, k 8 g .. 8 g + 7 ----
+// ---- operands: 32 of a product's k a step, eight a lane; lane (c, g) = (l % 16, l / 16) holds row or column c. Where
+// operands meet accumulators the k run in the order of a pair of accumulator tiles (rows 4 g + r of the first, then of the
+// second), so that a pair of tiles is the next product's operand as it lies in the registers; else k 8 g .. 8 g + 7 ----
 template <typename T, int NP> struct Operand;
 template <int NP> struct Operand<__bf16, NP> { bf16x8 p[NP]; };
 template <int NP> struct Operand<float, NP> { f32x4 lo, hi; };
@@ -57,16 +59,56 @@ __device__ __forceinline__ f32x4 mma(const Operand<float, NA>& a, const Operand<
   return acc;
 }
 
-// Four float32 values as N bf16 pieces, each the rounding of what is left.
-template <int N>
-__device__ __forceinline__ void split4(f32x4 x, bf16x4 (&out)[N]) {
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// Float32 values as NP bf16 pieces, each the rounding of what the ones before it leave; the difference (exact) takes one
+// instruction, the piece times -1 added.
+template <int NP, int N> __device__ __forceinline__ void split(float (&x)[N], __bf16 (&out)[NP][N]) {
+  // -1 in the low and in the high half, in registers: as a literal the second is float32's inline constant -1, which
+  // the instruction takes for a low half
+  unsigned low = 0xbf80u, high = 0xbf800000u;
+  asm("" : "+s"(low), "+s"(high));
+  const bf16x2 first = __builtin_bit_cast(bf16x2, low), second = __builtin_bit_cast(bf16x2, high);
 #pragma unroll
-  for (int p = 0; p < N; ++p)
+  for (int p = 0; p < NP; ++p)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      out[p][r] = (__bf16)x[r];
-      x[r] -= (float)out[p][r];
+    for (int e = 0; e < N; e += 2) {
+      const bf16x2 y = {(__bf16)x[e], (__bf16)x[e + 1]};
+      out[p][e] = y[0];
+      out[p][e + 1] = y[1];
+      if (p + 1 < NP) {
+        x[e] = __builtin_amdgcn_fdot2_f32_bf16(y, first, x[e], false);
+        x[e + 1] = __builtin_amdgcn_fdot2_f32_bf16(y, second, x[e + 1], false);
+      }
     }
+}
+template <int NP> __device__ __forceinline__ void split4(f32x4 v, bf16x4 (&out)[NP]) {
+  float x[4] = {v[0], v[1], v[2], v[3]};
+  __bf16 y[NP][4];
+  split<NP, 4>(x, y);
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[p][e] = y[p][e];
+}
+
+// A pair of accumulator tiles as the operand whose k run down their rows.
+template <typename T, int NP>
+__device__ __forceinline__ Operand<T, NP> paired(f32x4 a, f32x4 b) {
+  Operand<T, NP> o;
+  if constexpr (sizeof(T) == 2) {
+    float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    __bf16 y[NP][8];
+    split<NP, 8>(x, y);
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o.p[p][e] = y[p][e];
+  } else {
+    o.lo = a;
+    o.hi = b;
+  }
+  return o;
 }
 
 __device__ __forceinline__ int lane_col() { return threadIdx.x & 15; }
@@ -120,6 +162,79 @@ template <typename T> struct Rows {
   }
 };
 
+// ---- a chunk's rows in LDS as they come from memory, 16-byte pieces straight into LDS (no registers, no padding): a
+// row's pieces are permuted by bits of its number, so that the reads of a step of 16 rows (row operands) and the transposed
+// reads of 8 rows at a time (column operands) spread over the 64 banks ----
+template <typename T, int W> struct Tile {  // 64 rows of W elements
+  static constexpr int kPer = 16 / (int)sizeof(T);  // elements a piece
+  static constexpr int kRow = W / kPer;             // pieces a row: a power of two from 2 on
+  static constexpr int kElems = kChunk * W;
+  static constexpr int kInstr = kRow;               // wave instructions a tile: 64 pieces each
+  __device__ __forceinline__ static int permute(int row) {
+    if constexpr (kRow >= 16) return ((row >> 3) & 1) | ((row & 7) << 1);
+    else if constexpr (kRow == 8) return ((row >> 3) & 1) | (((row >> 1) & 3) << 1);
+    else if constexpr (kRow == 4) return ((row >> 3) & 1) | (((row >> 2) & 1) << 1);
+    else return 0;
+  }
+  __device__ __forceinline__ static int at(int row, int f) {
+    return row * W + (((f / kPer) ^ permute(row)) * kPer) + (f & (kPer - 1));
+  }
+  // instruction j of the tile: lane l brings piece 64 j + l of the rows' features from `first` on
+  __device__ __forceinline__ static void stage(T* tile, const Rows<T>& rows, int j, int first) {
+    const int l = threadIdx.x & 63, p = 64 * j + l, row = p / kRow;
+    buffer_load_lds16(rows.r, tile + 64 * kPer * j, rows.at(row, first + ((p & (kRow - 1)) ^ permute(row)) * kPer), 0);
+  }
+  // eight elements of a row from feature f (a multiple of 8)
+  __device__ __forceinline__ static Operand<T, 1> row(const T* tile, int row, int f) {
+    Operand<T, 1> x;
+    if constexpr (sizeof(T) == 2) {
+      x.p[0] = *reinterpret_cast<const bf16x8*>(tile + at(row, f));
+    } else {
+      x.lo = *reinterpret_cast<const f32x4*>(tile + at(row, f));
+      x.hi = *reinterpret_cast<const f32x4*>(tile + at(row, f + 4));
+    }
+    return x;
+  }
+  // rows 16 i + 4 g .. + 3 of column f0 + c: an accumulator tile's layout
+  __device__ __forceinline__ static f32x4 four(const T* tile, int i, int f0) {
+    const int c = lane_col(), r0 = 16 * i + 4 * lane_grp();
+    f32x4 x;
+    if constexpr (sizeof(T) == 2) {
+      const bf16x4 y = read_tr16<bf16x4>(tile + at(r0 + (c >> 2), f0 + 4 * (c & 3)));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = (float)y[r];
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = tile[at(r0 + r, f0 + c)];
+    }
+    return x;
+  }
+  // column f0 + c of the rows of step s, in the order of a pair of accumulator tiles
+  __device__ __forceinline__ static Operand<T, 1> columns(const T* tile, int s, int f0) {
+    const int c = lane_col(), r0 = 32 * s + 4 * lane_grp();
+    Operand<T, 1> x;
+    if constexpr (sizeof(T) == 2) {
+      const bf16x4 lo = read_tr16<bf16x4>(tile + at(r0 + (c >> 2), f0 + 4 * (c & 3)));
+      const bf16x4 hi = read_tr16<bf16x4>(tile + at(r0 + 16 + (c >> 2), f0 + 4 * (c & 3)));
+      x.p[0] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x.lo[e] = tile[at(r0 + e, f0 + c)];
+        x.hi[e] = tile[at(r0 + 16 + e, f0 + c)];
+      }
+    }
+    return x;
+  }
+};
+
+// The direct loads that this wave has issued are in LDS (and all else that it has loaded has arrived).
+__device__ __forceinline__ void direct_loads_done() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // Column f0 + c of rows 32 s + 8 g .. + 7 of a row-major LDS tile [token][feature].
 template <typename T>
 __device__ __forceinline__ Operand<T, 1> load_columns(const T* tile, int pitch, int s, int f0) {
@@ -140,14 +255,25 @@ __device__ __forceinline__ Operand<T, 1> load_columns(const T* tile, int pitch, 
   return o;
 }
 
-// ---- operands on their way through LDS or memory: a step's pieces one after the other, a piece 16 bytes a lane --
-// (float32: the eight values in two planes of four). An accumulator tile (rows 16 t + 4 g + r, column c) is half of
-// step t / 2.
+// ---- operands in LDS or memory: a step's pieces one after the other, a piece 16 bytes a lane (float32: the eight values in
+// two planes of four) ----
 template <typename T, int NP> struct Frags {
   static constexpr int kStep = sizeof(T) == 2 ? NP * 512 : 512;  // elements of a step
-  __device__ __forceinline__ static void put(T* base, int t, f32x4 acc) {
+  template <int N> __device__ __forceinline__ static void put(T* base, int s, const Operand<T, N>& o) {
+    const int l = threadIdx.x & 63;
+    T* step = base + s * kStep;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(step + (p * 64 + l) * 8) = o.p[p];
+    } else {
+      *reinterpret_cast<f32x4*>(step + l * 4) = o.lo;
+      *reinterpret_cast<f32x4*>(step + (64 + l) * 4) = o.hi;
+    }
+  }
+  // An accumulator tile as half of step t / 2: in the order of pairs of tiles, or (NATURAL) with k 8 g .. 8 g + 7 a lane.
+  template <bool NATURAL> __device__ __forceinline__ static void put_tile(T* base, int t, f32x4 acc) {
     const int c = lane_col(), g = lane_grp();
-    const int lane = (2 * (t & 1) + (g >> 1)) * 16 + c, half = g & 1;
+    const int lane = NATURAL ? (2 * (t & 1) + (g >> 1)) * 16 + c : 16 * g + c, half = NATURAL ? g & 1 : t & 1;
     T* step = base + (t >> 1) * kStep;
     if constexpr (sizeof(T) == 2) {
       bf16x4 x[NP];
@@ -158,6 +284,7 @@ template <typename T, int NP> struct Frags {
       *reinterpret_cast<f32x4*>(step + (half * 64 + lane) * 4) = acc;
     }
   }
+  // the first N pieces of a step
   template <int N = NP> __device__ __forceinline__ static Operand<T, N> get(const T* base, int s) {
     const int l = threadIdx.x & 63;
     const T* step = base + s * kStep;
@@ -171,6 +298,12 @@ template <typename T, int NP> struct Frags {
     }
     return o;
   }
+  // instruction j of `steps` steps straight into LDS: 1 KiB each
+  static constexpr int kStepInstr = kStep * (int)sizeof(T) / 1024;
+  __device__ __forceinline__ static void stage(T* dst, const T* src, int steps, int j) {
+    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(src, (unsigned)(steps * kStep * sizeof(T)));
+    buffer_load_lds16(r, dst + j * (1024 / (int)sizeof(T)), 16 * (threadIdx.x & 63) + 1024 * j, 0);
+  }
 };
 
 // The six operand steps that cover a lower triangle of 4 x 4 tiles. By rows i (the sums run over j <= i): steps
@@ -182,6 +315,10 @@ __host__ __device__ constexpr int col_step(int j, int s) { return j < 2 ? 2 * j 
 // ---- the workspace of one chunk and head ----
 // coefficients: beta, eps, kap, 64 floats each
 constexpr int kCoef = 3 * kChunk;
+__device__ __forceinline__ void stage_coef(float* dst, const float* coef) {
+  const __amdgpu_buffer_rsrc_t r = buffer_rsrc(coef, kCoef * sizeof(float));
+  if ((threadIdx.x & 63) < kCoef / 4) buffer_load_lds16(r, dst, 16 * (threadIdx.x & 63), 0);
+}
 template <typename T, int NP> struct Factor {  // elements of a triangular factor
   static constexpr int kElems = kTriSteps * Frags<T, NP>::kStep;
 };
@@ -206,11 +343,13 @@ __device__ __forceinline__ Record record(float* base, size_t chunk, int rows, in
   return {buffer_rsrc(base + chunk * rows * D, (unsigned)rows * D * 4u), rows, D};
 }
 
-// LDS writes before, LDS reads after, for the whole workgroup; loads from memory stay in flight.
+// LDS writes before, LDS reads after, for the whole workgroup; loads from memory stay in flight, direct loads into LDS
+// among them (a release fence would wait for those: direct_loads_done does, where they are due).
 __device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  asm volatile("" ::: "memory");
 }
 
 template <typename T>
@@ -218,12 +357,14 @@ struct Dims {
   int N, H, D, chunks;
   // element offset of token t of head h in [B, N, H, D]
   __device__ __forceinline__ size_t at(int b, int t, int h) const { return (((size_t)b * N + t) * H + h) * D; }
-  // the rows of head h from token t0 to the end of its chunk or of the sequence
-  __device__ __forceinline__ Rows<T> rows(const T* p, int b, int t0, int h) const {
-    const int count = N - t0 < kChunk ? N - t0 : kChunk;
+  // a head's rows of chunk ci, the first of them at `first`, to the end of the chunk or of the sequence
+  __device__ __forceinline__ Rows<T> rows_at(const T* first, int ci) const {
+    const int left = N - ci * kChunk, count = left < kChunk ? left : kChunk;
     const unsigned pitch = (unsigned)H * D * sizeof(T);
-    return {buffer_rsrc(p + at(b, t0, h), (count - 1) * pitch + (unsigned)(D * sizeof(T))), pitch, D};
+    return {buffer_rsrc(first, (count - 1) * pitch + (unsigned)(D * sizeof(T))), pitch, D};
   }
+  // the rows of head h from token t0, a chunk's first
+  __device__ __forceinline__ Rows<T> rows(const T* p, int b, int t0, int h) const { return rows_at(p + at(b, t0, h), t0 / kChunk); }
   // the bytes of a chunk's flags; without flags an empty range
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t flags(const uint8_t* p, int b, int t0) const {
     const int count = N - t0 < kChunk ? N - t0 : kChunk;

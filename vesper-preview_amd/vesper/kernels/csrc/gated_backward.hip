@@ -13,11 +13,13 @@
 //
 //  * gated_prep_kernel (gated_scan.hip) forms T and P again, as operands by columns.
 //  * gated_chain_backward_kernel walks the chunks from the last to the first like the forward's chain, a workgroup a
-//    head and 16 value columns: four waves carry dH through three dependent products, four more form P^T dO and
-//    Q^T (eps dO) of the chunk that comes next. It writes dV and keeps dH' and dR of each chunk, in float32.
+//    head and 16 value columns: four waves carry dH through three dependent products, four more bring everything into
+//    LDS ahead and form P^T dO and Q^T (eps dO) of the next chunk. It writes dV and keeps dH' and dR of each chunk.
 //  * gated_grad_kernel: a workgroup a chunk and head, all at once, for the rest: wave w holds dQ, Y and C of the
 //    16 tokens w, sums over the value columns 32 at a time from H, dH', Delta and dR in pieces in LDS, then over
 //    the chunk's tokens with accumulator tiles as operands.
+#include <type_traits>
+
 #include "gated.h"
 #include "vesper_kernels.h"
 
@@ -32,41 +34,36 @@ template <typename T, int DP> struct BackShape {
   static constexpr int KS = DP / 32;
   static constexpr int TILES = DP / 16;
   static constexpr int FT = TILES < 4 ? 1 : TILES / 4;
-  static constexpr int PITCH = DP + (sizeof(T) == 2 ? 8 : 4);
   static constexpr int NT = Pieces<T>::kN;
-  // float32 queries are read from memory by columns: both tiles of a head of width 256 would not fit the LDS
+  // float32 queries are read from memory by columns: the LDS has no room for them beside the rest
   static constexpr bool kStageQ = sizeof(T) == 2;
+  // chunks of keys and of queries in LDS at once: heads of width 256 have room for one of each, and wait for each
+  static constexpr int RING = DP > 128 ? 1 : 2;
   using F = Frags<T, NT>;
-  using F1 = Frags<T, 1>;
-  struct Lds {
-    T keys[kChunk * PITCH];
-    T queries[kStageQ ? kChunk * PITCH : 8];
-    T state[KS * F::kStep];   // dH
-    T ddelta[2 * F::kStep];
-    T dread[2 * F::kStep];    // -beta eps dR
-    T d_o[2 * F1::kStep];
-    T edo[2 * F::kStep];      // eps dO
-    float z[4 * 64 * 4];      // P^T dO, an accumulator tile after the other
-    float qdo[TILES * 64 * 4];  // Q^T (eps dO)
+  using Keys = Tile<T, DP>;
+  using Slice = Tile<T, 16>;
+  struct Stage {  // what comes from memory for the chain, besides T
+    T keys[Keys::kElems];
+    float coef[kCoef];
   };
+  struct Lds {
+    Stage ring[RING];
+    T queries[RING][kStageQ ? Keys::kElems : 8];
+    T d_o[Slice::kElems];        // of one chunk, as T: read into registers in a chunk's first span
+    T tf[kTriSteps * F::kStep];
+    T state[KS * F::kStep];      // dH
+    T ddelta[2 * F::kStep];
+    T dread[2 * F::kStep];       // -beta eps dR
+    float z[4 * 256];            // P^T dO, accumulator tiles one after the other
+    float qdo[TILES * 256];      // Q^T (eps dO)
+  };
+  static_assert(sizeof(Lds) <= 160 * 1024, "more than a CU's LDS");
 };
 
-template <typename T, int DP> struct BackIn {  // what a chain wave reads of a chunk
-  Operand<T, 1> kf[BackShape<T, DP>::KS];
-  Operand<T, Pieces<T>::kN> tf[2];
-  f32x4 beta, eps, kap;
-  float gam;
-};
-
-template <typename T, int DP> struct BackTile {  // a quarter of a tile of keys or queries
-  Operand<T, 1> x[DP / 32];
-};
-
-template <typename T, int DP> struct BackSide {  // what the other waves read of the next chunk, besides the queries
+template <typename T> struct BackIn {  // what the other waves keep of a chunk in registers
   Operand<T, Pieces<T>::kN> pf[2];
-  f32x4 eps;
-  T d_o[4];
-  uint8_t on[4];
+  f32x4 eps[4];
+  uint8_t on;  // of token l
 };
 
 template <typename T, int DP>
@@ -77,8 +74,9 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
     float* __restrict__ rec_dr, Dims<T> dims, int slices) {
   using S = BackShape<T, DP>;
   using F = typename S::F;
-  using F1 = typename S::F1;
-  constexpr int KS = S::KS, FT = S::FT, NT = S::NT;
+  using Keys = typename S::Keys;
+  using Slice = typename S::Slice;
+  constexpr int KS = S::KS, FT = S::FT, TILES = S::TILES, NT = S::NT, RING = S::RING;
   __shared__ __attribute__((aligned(16))) typename S::Lds lds;
 
   const int id = xcd_logical_block(blockIdx.x, gridDim.x);
@@ -86,10 +84,17 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
   const int D = dims.D, nc = dims.chunks;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
   const int c = lane_col(), grp = lane_grp(), lane = threadIdx.x & 63;
-  const int vcol = 16 * sl + c;
   const size_t chunk0 = (size_t)bh * nc;
 
+  // features past D and rows past the end are not brought: zeros, and what another chunk left there, times zeros
+  for (int i = threadIdx.x; i < (int)((sizeof(lds.ring) + sizeof(lds.queries) + sizeof(lds.d_o)) / 16); i += 512)
+    reinterpret_cast<f32x4*>(&lds)[i] = zero4();
+  lds_barrier();
+
   if (wave < 4) {
+    // ---- the chain: wave w has the 16 tokens w of dDelta and dR, and of dH's feature tiles each fourth ----
+    __builtin_amdgcn_s_setprio(3);
+    const int vcol = 16 * sl + c, own = 16 * w + 4 * grp;
     f32x4 dh[FT];
 #pragma unroll
     for (int i = 0; i < FT; ++i) {
@@ -99,80 +104,77 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
         const int f = 16 * ft + 4 * grp + r;
         dh[i][r] = d_state != nullptr && f < D && vcol < D ? d_state[((size_t)bh * D + f) * D + vcol] : 0.f;
       }
-      if (ft < S::TILES) F::put(lds.state, ft, dh[i]);
+      if (ft < TILES) F::template put_tile<true>(lds.state, ft, dh[i]);
     }
-    auto load = [&](int ci, BackIn<T, DP>& in) {
-      const Rows<T> krows = dims.rows(k, b, ci * kChunk, h);
+    lds_barrier();
+    lds_barrier();
+    lds_barrier();
+    for (int it = 0; it < nc; ++it) {
+      const int ci = nc - 1 - it;
+      const typename S::Stage& in = lds.ring[RING == 1 ? 0 : it & 1];
+      if constexpr (RING == 1) lds_barrier();
+      // dDelta = P^T dO + kap (K dH'); T's columns on the way
+      f32x4 x = zero4();
 #pragma unroll
-      for (int st = 0; st < KS; ++st) in.kf[st] = krows.row(16 * w + c, 32 * st + 8 * grp);
-      const T* tb = tf + (chunk0 + ci) * Factor<T, NT>::kElems + col_step(w, 0) * F::kStep;
-      in.tf[0] = F::get(tb, 0);
-      in.tf[1] = F::get(tb, w < 2 ? 1 : 0);
-      const float* co = coef + (chunk0 + ci) * kCoef + 16 * w + 4 * grp;
-      in.beta = *reinterpret_cast<const f32x4*>(co);
-      in.eps = *reinterpret_cast<const f32x4*>(co + kChunk);
-      in.kap = *reinterpret_cast<const f32x4*>(co + 2 * kChunk);
-      in.gam = coef[(chunk0 + ci) * kCoef + 2 * kChunk - 1];
-    };
-    auto step = [&](int ci, const BackIn<T, DP>& in) {
+      for (int s = 0; s < KS; ++s) x = mma(Keys::row(in.keys, 16 * w + c, 32 * s + 8 * grp), F::get(lds.state, s), x);
+      const f32x4 kap = *reinterpret_cast<const f32x4*>(in.coef + 2 * kChunk + own);
+      const f32x4 z = *reinterpret_cast<const f32x4*>(lds.z + 256 * w + 4 * lane);
+      const Operand<T, NT> t0 = F::get(lds.tf, col_step(w, 0)), t1 = F::get(lds.tf, col_step(w, w < 2 ? 1 : 0));
       const Record rh = record(rec_dh, chunk0 + ci, D, D);
 #pragma unroll
       for (int i = 0; i < FT; ++i) rh.put(vcol, 16 * (w + 4 * i) + 4 * grp, dh[i]);
-      // dDelta = P^T dO + kap (K dH')
-      f32x4 x = zero4();
 #pragma unroll
-      for (int st = 0; st < KS; ++st) x = mma(in.kf[st], F::get(lds.state, st), x);
-      const f32x4 z = *reinterpret_cast<const f32x4*>(lds.z + (w * 64 + lane) * 4);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = in.kap[r] * x[r] + z[r];
-      F::put(lds.ddelta, w, x);
+      for (int r = 0; r < 4; ++r) x[r] = kap[r] * x[r] + z[r];
+      F::template put_tile<false>(lds.ddelta, w, x);
       lds_barrier();
-      // dR = T^T dDelta
-      f32x4 dr;
-      if (w < 2) {
-        dr = mma(in.tf[0], F::get(lds.ddelta, 0), zero4());
-        dr = mma(in.tf[1], F::get(lds.ddelta, 1), dr);
-      } else {
-        dr = mma(in.tf[0], F::get(lds.ddelta, 1), zero4());
-      }
-      f32x4 y;
+      // dR = T^T dDelta; K^T and Q^T (eps dO) on the way
+      f32x4 dr = mma(t1, F::get(lds.ddelta, 1), zero4());
+      if (w < 2) dr = mma(t0, F::get(lds.ddelta, 0), dr);
+      const f32x4 beta = *reinterpret_cast<const f32x4*>(in.coef + own);
+      const f32x4 eps = *reinterpret_cast<const f32x4*>(in.coef + kChunk + own);
+      const float gam = in.coef[2 * kChunk - 1];
+      constexpr int AHEAD = FT < 2 ? FT : 2;  // feature tiles whose K^T waits in registers
+      Operand<T, 1> kc[AHEAD][2];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) y[r] = -(in.beta[r] * in.eps[r]) * dr[r];
-      F::put(lds.dread, w, y);
-      f32x4 add[FT];
+      for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) kc[i][s] = Keys::columns(in.keys, s, 16 * (TILES < 4 ? w & 1 : w + 4 * i));
 #pragma unroll
       for (int i = 0; i < FT; ++i)
-        add[i] = w + 4 * i < S::TILES ? *reinterpret_cast<const f32x4*>(lds.qdo + ((w + 4 * i) * 64 + lane) * 4) : zero4();
-      record(rec_dr, chunk0 + ci, kChunk, D).put(vcol, 16 * w + 4 * grp, dr);
+        if (w + 4 * i < TILES) {
+          const f32x4 add = *reinterpret_cast<const f32x4*>(lds.qdo + 256 * (w + 4 * i) + 4 * lane);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) dh[i][r] = gam * dh[i][r] + add[r];
+        }
+      f32x4 y, vx;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        vx[r] = beta[r] * dr[r];
+        y[r] = -(vx[r] * eps[r]);
+      }
+      F::template put_tile<false>(lds.dread, w, y);
+      record(rec_dr, chunk0 + ci, kChunk, D).put(vcol, own, dr);
       const Rows<T> dvrows = dims.rows(dv, b, ci * kChunk, h);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) dvrows.put_one(16 * w + 4 * grp + r, vcol, from_f32<T>(in.beta[r] * dr[r]));
+      for (int r = 0; r < 4; ++r) dvrows.put_one(own + r, vcol, from_f32<T>(vx[r]));
       lds_barrier();
       // dH = gam dH' + Q^T (eps dO) - K^T (beta eps dR)
       const Operand<T, NT> y0 = F::get(lds.dread, 0), y1 = F::get(lds.dread, 1);
 #pragma unroll
       for (int i = 0; i < FT; ++i) {
         const int ft = w + 4 * i;
-        if (ft < S::TILES) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) dh[i][r] = in.gam * dh[i][r] + add[i][r];
-          dh[i] = mma(load_columns(lds.keys, S::PITCH, 0, 16 * ft), y0, dh[i]);
-          dh[i] = mma(load_columns(lds.keys, S::PITCH, 1, 16 * ft), y1, dh[i]);
-          F::put(lds.state, ft, dh[i]);
+        if (ft < TILES) {
+          if (i >= AHEAD) {
+            dh[i] = mma(Keys::columns(in.keys, 0, 16 * ft), y0, dh[i]);
+            dh[i] = mma(Keys::columns(in.keys, 1, 16 * ft), y1, dh[i]);
+          } else {
+            dh[i] = mma(kc[i < AHEAD ? i : 0][0], y0, dh[i]);
+            dh[i] = mma(kc[i < AHEAD ? i : 0][1], y1, dh[i]);
+          }
+          F::template put_tile<true>(lds.state, ft, dh[i]);
         }
       }
       lds_barrier();
-    };
-    BackIn<T, DP> a, bb;
-    load(nc - 1, a);
-    lds_barrier();
-    lds_barrier();
-    for (int ci = nc - 1; ci >= 0; ci -= 2) {  // past the first chunk it is loaded again, so that no load is conditional
-      load(ci >= 1 ? ci - 1 : 0, bb);
-      step(ci, a);
-      if (ci < 1) break;
-      load(ci >= 2 ? ci - 2 : 0, a);
-      step(ci - 1, bb);
     }
     float* so = d_state_in + (size_t)bh * D * D;
 #pragma unroll
@@ -183,114 +185,144 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
         if (f < D && vcol < D) so[(size_t)f * D + vcol] = dh[i][r];
       }
   } else {
-    // ---- the keys of the chunk in hand into LDS; of the next chunk the queries, dO and eps dO, then P^T dO, then
-    //      Q^T (eps dO), each in one of the three spans between barriers ----
-    const int hl = threadIdx.x - 256;
-    auto load_tile = [&](const T* src, int ci, BackTile<T, DP>& in) {
-      const Rows<T> rows = dims.rows(src, b, ci * kChunk, h);
+    // ---- memory into LDS ahead, and of the next chunk P^T dO (the 16 tokens w) and Q^T (eps dO) (each fourth feature tile).
+    //      In a chunk's three spans: dO of the next chunk into registers; P^T dO; Q^T (eps dO). Chunk number it counts
+    //      from the last one back; past the first it stays, so that nothing is conditional ----
+    const size_t stride = (size_t)kChunk * dims.H * D;
+    const T *kp = k + dims.at(b, 0, h), *qp = q + dims.at(b, 0, h), *gp = d_o + dims.at(b, 0, h);
+    const T* tp = tf + chunk0 * Factor<T, NT>::kElems;
+    const T* pp = pf + chunk0 * Factor<T, NT>::kElems + col_step(w, 0) * F::kStep;
+    const float* cp = coef + chunk0 * kCoef;
+    auto chunk_of = [&](int it) { return it < nc ? nc - 1 - it : 0; };
+    auto stage = [&](int it) {
+      const int ci = chunk_of(it);
+      typename S::Stage& to = lds.ring[RING == 1 ? 0 : it & 1];
+      const Rows<T> rows = dims.rows_at(kp + ci * stride, ci);
 #pragma unroll
-      for (int i = 0; i < DP / 32; ++i) {
-        const int p = hl + 256 * i;
-        in.x[i] = rows.row(p / (DP / 8), 8 * (p % (DP / 8)));
+      for (int j = 0; j < Keys::kInstr / 4; ++j) Keys::stage(to.keys, rows, 4 * j + w, 0);
+      if (w == 3) stage_coef(to.coef, cp + (size_t)ci * kCoef);
+    };
+    // `slot` as a constant: the reads of one slot then do not wait for the loads into the other
+    auto stage_q = [&](int it, auto slot) {
+      if constexpr (S::kStageQ) {
+        const int ci = chunk_of(it);
+        const Rows<T> rows = dims.rows_at(qp + ci * stride, ci);
+#pragma unroll
+        for (int j = 0; j < Keys::kInstr / 4; ++j) Keys::stage(lds.queries[decltype(slot)::value], rows, 4 * j + w, 0);
       }
     };
-    auto put_tile = [&](T* dst, const BackTile<T, DP>& in) {
+    auto stage_t = [&](int it) {
+      const int ci = chunk_of(it);
+      constexpr int TI = kTriSteps * F::kStepInstr;
 #pragma unroll
-      for (int i = 0; i < DP / 32; ++i) {
-        const int p = hl + 256 * i, row = p / (DP / 8), f = 8 * (p % (DP / 8));
-        T* at = dst + row * S::PITCH + f;
-        if constexpr (sizeof(T) == 2) {
-          *reinterpret_cast<bf16x8*>(at) = in.x[i].p[0];
-        } else {
-          reinterpret_cast<f32x4*>(at)[0] = in.x[i].lo;
-          reinterpret_cast<f32x4*>(at)[1] = in.x[i].hi;
-        }
-      }
+      for (int j = 0; j < (TI + 3) / 4; ++j)
+        if (4 * j + w < TI) F::stage(lds.tf, tp + (size_t)ci * Factor<T, NT>::kElems, kTriSteps, 4 * j + w);
     };
-    auto load_side = [&](int ci, BackSide<T, DP>& in) {
-      const T* pb = pf + (chunk0 + ci) * Factor<T, NT>::kElems + col_step(w, 0) * F::kStep;
+    auto stage_do = [&](int it) {
+      const int ci = chunk_of(it);
+      if (w < Slice::kInstr) Slice::stage(lds.d_o, dims.rows_at(gp + ci * stride, ci), w, 16 * sl);
+    };
+    auto load = [&](int it, BackIn<T>& in) {
+      const int ci = chunk_of(it);
+      const T* pb = pp + (size_t)ci * Factor<T, NT>::kElems;
       in.pf[0] = F::get(pb, 0);
       in.pf[1] = F::get(pb, w < 2 ? 1 : 0);
-      in.eps = *reinterpret_cast<const f32x4*>(coef + (chunk0 + ci) * kCoef + kChunk + 16 * w + 4 * grp);
-      const Rows<T> rows = dims.rows(d_o, b, ci * kChunk, h);
-      const __amdgpu_buffer_rsrc_t flags = dims.flags(active, b, ci * kChunk);
+      const float* co = cp + (size_t)ci * kCoef + kChunk + 4 * grp;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        in.d_o[r] = rows.one(16 * w + 4 * grp + r, vcol);
-        in.on[r] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(flags, 16 * w + 4 * grp + r, 0, 0);
-      }
+      for (int i = 0; i < 4; ++i) in.eps[i] = *reinterpret_cast<const f32x4*>(co + 16 * i);
+      in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, ci * kChunk), lane, 0, 0);
     };
-    auto put_side = [&](const BackSide<T, DP>& in) {
-      f32x4 x, e;
+    f32x4 x[4];  // dO as accumulator tiles (rows tokens), zero where inactive
+    auto read_do = [&](const BackIn<T>& in) {
+      const uint64_t on = active == nullptr ? ~0ull : __builtin_amdgcn_ballot_w64(in.on != 0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[r] = active == nullptr || in.on[r] ? to_f32(in.d_o[r]) : 0.f;
-        e[r] = in.eps[r] * x[r];
-      }
-      F1::put(lds.d_o, w, x);
-      F::put(lds.edo, w, e);
-    };
-    auto form_z = [&](const BackSide<T, DP>& in) {
-      f32x4 z;
-      if (w < 2) {
-        z = mma(in.pf[0], F1::get(lds.d_o, 0), zero4());
-        z = mma(in.pf[1], F1::get(lds.d_o, 1), z);
-      } else {
-        z = mma(in.pf[0], F1::get(lds.d_o, 1), zero4());
-      }
-      *reinterpret_cast<f32x4*>(lds.z + (w * 64 + lane) * 4) = z;
-    };
-    auto query_columns = [&](int ci, int s, int f0) -> Operand<T, 1> {
-      if constexpr (S::kStageQ) {
-        return load_columns(lds.queries, S::PITCH, s, f0);
-      } else {
-        Operand<T, 1> x;
-        const Rows<T> rows = dims.rows(q, b, ci * kChunk, h);
+      for (int j = 0; j < 4; ++j) {
+        x[j] = Slice::four(lds.d_o, j, 0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x.lo[e] = rows.one(32 * s + 8 * grp + e, f0 + c);
-          x.hi[e] = rows.one(32 * s + 8 * grp + 4 + e, f0 + c);
-        }
-        return x;
+        for (int r = 0; r < 4; ++r) x[j][r] = (on >> (16 * j + 4 * grp + r)) & 1 ? x[j][r] : 0.f;
       }
     };
-    auto form_qdo = [&](int ci) {
-      const Operand<T, NT> e0 = F::get(lds.edo, 0), e1 = F::get(lds.edo, 1);
+    auto form_z = [&](const BackIn<T>& in) {
+      f32x4 z = mma(in.pf[1], paired<T, 1>(x[2], x[3]), zero4());
+      if (w < 2) z = mma(in.pf[0], paired<T, 1>(x[0], x[1]), z);
+      *reinterpret_cast<f32x4*>(lds.z + 256 * w + 4 * lane) = z;
+    };
+    auto form_qdo = [&](int it, auto slot, const BackIn<T>& in) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[j][r] *= in.eps[j][r];
+      const Operand<T, NT> e0 = paired<T, NT>(x[0], x[1]), e1 = paired<T, NT>(x[2], x[3]);
 #pragma unroll
       for (int i = 0; i < FT; ++i) {
         const int ft = w + 4 * i;
-        if (ft < S::TILES) {
-          f32x4 x = mma(query_columns(ci, 0, 16 * ft), e0, zero4());
-          x = mma(query_columns(ci, 1, 16 * ft), e1, x);
-          *reinterpret_cast<f32x4*>(lds.qdo + (ft * 64 + lane) * 4) = x;
+        if (ft < TILES) {
+          f32x4 y;
+          if constexpr (S::kStageQ) {
+            y = mma(Keys::columns(lds.queries[decltype(slot)::value], 0, 16 * ft), e0, zero4());
+            y = mma(Keys::columns(lds.queries[decltype(slot)::value], 1, 16 * ft), e1, y);
+          } else {
+            const int ci = chunk_of(it);
+            const Rows<T> rows = dims.rows_at(qp + ci * stride, ci);
+            Operand<T, 1> qc[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                qc[s].lo[e] = rows.one(32 * s + 4 * grp + e, 16 * ft + c);
+                qc[s].hi[e] = rows.one(32 * s + 16 + 4 * grp + e, 16 * ft + c);
+              }
+            y = mma(qc[0], e0, zero4());
+            y = mma(qc[1], e1, y);
+          }
+          *reinterpret_cast<f32x4*>(lds.qdo + 256 * ft + 4 * lane) = y;
         }
       }
     };
-    BackTile<T, DP> keys, queries;
-    BackSide<T, DP> side;
-    load_tile(k, nc - 1, keys);
-    if constexpr (S::kStageQ) load_tile(q, nc - 1, queries);
-    load_side(nc - 1, side);
-    if constexpr (S::kStageQ) put_tile(lds.queries, queries);
-    put_side(side);
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, RING - 1> odd{};
+    BackIn<T> in;
+    auto step = [&](int it, auto slot, auto other) {
+      if constexpr (RING == 1) {
+        stage(it);
+        stage_q(it + 1, slot);
+        direct_loads_done();
+        lds_barrier();
+        read_do(in);
+      } else {
+        read_do(in);
+        stage(it + 1);
+        stage_q(it + 2, slot);
+      }
+      lds_barrier();
+      form_z(in);
+      stage_t(it + 1);
+      stage_do(it + 2);
+      lds_barrier();
+      form_qdo(it + 1, other, in);
+      direct_loads_done();
+      load(it + 2, in);
+      lds_barrier();
+    };
+    if constexpr (RING > 1) stage(0);
+    stage_t(0);
+    stage_do(0);
+    stage_q(0, even);
+    load(0, in);
+    direct_loads_done();
     lds_barrier();
-    form_z(side);
-    form_qdo(nc - 1);
-    if constexpr (S::kStageQ) load_tile(q, nc > 1 ? nc - 2 : 0, queries);
-    load_side(nc > 1 ? nc - 2 : 0, side);
+    read_do(in);
+    form_z(in);
+    form_qdo(0, even, in);
     lds_barrier();
-    for (int ci = nc - 1; ci >= 0; --ci) {  // past the first chunk it is formed again, so that nothing is conditional
-      put_tile(lds.keys, keys);
-      load_tile(k, ci >= 1 ? ci - 1 : 0, keys);
-      if constexpr (S::kStageQ) put_tile(lds.queries, queries);
-      put_side(side);
-      lds_barrier();
-      form_z(side);
-      if constexpr (S::kStageQ) load_tile(q, ci >= 2 ? ci - 2 : 0, queries);
-      load_side(ci >= 2 ? ci - 2 : 0, side);
-      lds_barrier();
-      form_qdo(ci >= 1 ? ci - 1 : 0);
-      lds_barrier();
+    stage_do(1);
+    if constexpr (RING > 1) stage_q(1, odd);
+    load(1, in);
+    direct_loads_done();
+    lds_barrier();
+    for (int it = 0; it < nc; it += 2) {
+      step(it, even, odd);
+      if (it + 1 < nc) step(it + 1, odd, even);
     }
   }
 }
@@ -304,10 +336,10 @@ template <typename T, int NP, int ROWS, int PITCH> struct Planes {
   T x[NP * kPlane];
   __device__ __forceinline__ void put(int row, int col, f32x4 v) {
     if constexpr (sizeof(T) == 2) {
-      bf16x4 p[NP];
-      split4<NP>(v, p);
+      const Operand<T, NP> p = paired<T, NP>(v, zero4());
 #pragma unroll
-      for (int i = 0; i < NP; ++i) *reinterpret_cast<bf16x4*>(x + i * kPlane + row * PITCH + col) = p[i];
+      for (int i = 0; i < NP; ++i)
+        *reinterpret_cast<bf16x4*>(x + i * kPlane + row * PITCH + col) = __builtin_shufflevector(p.p[i], p.p[i], 0, 1, 2, 3);
     } else {
       *reinterpret_cast<f32x4*>(x + row * PITCH + col) = v;
     }
@@ -341,23 +373,6 @@ __device__ __forceinline__ Operand<T, 1> load_columns_paired(const T* tile, int 
       o.lo[e] = p[e * pitch];
       o.hi[e] = p[(16 + e) * pitch];
     }
-  }
-  return o;
-}
-
-// A pair of accumulator tiles as the operand whose k run down their rows.
-template <typename T, int NP>
-__device__ __forceinline__ Operand<T, NP> paired(f32x4 a, f32x4 b) {
-  Operand<T, NP> o;
-  if constexpr (sizeof(T) == 2) {
-    bf16x4 x[NP], y[NP];
-    split4<NP>(a, x);
-    split4<NP>(b, y);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) o.p[i] = __builtin_shufflevector(x[i], y[i], 0, 1, 2, 3, 4, 5, 6, 7);
-  } else {
-    o.lo = a;
-    o.hi = b;
   }
   return o;
 }

@@ -2,11 +2,11 @@
 //
 //  * gated_prep_kernel: one wave a chunk and head, all of them at once: the decays' sums, the products of all
 //    pairs of the chunk's tokens (K K^T and K Q^T), the inverse T, and both factors written as MFMA operands.
-//  * gated_chain_kernel: a workgroup a head and 16 value columns walks the chunks. Value columns of the state
-//    evolve independently, so a head of width 64 is four chains. Four waves carry the chain, each one tile of 16
-//    tokens (R, Delta) and its share of the state's feature tiles in accumulators; between the three dependent
-//    products (K H, T R, K^T Delta) the tiles pass through LDS as operands in pieces. Four more waves bring the
-//    keys into LDS and form the outputs in the gaps.
+//  * gated_chain_kernel: a workgroup a head and 16 value columns walks the chunks (value columns of the state evolve
+//    independently, so a head of width 64 is four chains). Four waves carry the chain, each one tile of 16 tokens
+//    (R, Delta) and its share of the state's feature tiles in accumulators; between the three dependent products
+//    (K H, T R, K^T Delta) the tiles pass through LDS as operands in pieces. Four more waves bring keys, values and
+//    T straight into LDS a chunk ahead and form the outputs in the gaps, so that the chain waits for no memory.
 #include "gated.h"
 #include "vesper_kernels.h"
 
@@ -39,6 +39,24 @@ __device__ __forceinline__ f32x4 mm16f(f32x4 a, f32x4 b, f32x4 acc) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], acc, 0, 0, 0);
   return acc;
+}
+
+// A lower triangle's ten accumulator tiles as the operands of gated.h's six steps; tiles outside the triangle are zeros.
+template <typename T, int NP, bool COLS>
+__device__ __forceinline__ void put_factor(T* out, const f32x4 (&x)[10]) {
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (COLS ? 2 * s + 1 < a : 2 * s > a) continue;
+      f32x4 half[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int o = 2 * s + e, i = COLS ? o : a, j = COLS ? a : o;
+        half[e] = j <= i ? x[j <= i ? i * (i + 1) / 2 + j : 0] : zero4();
+      }
+      Frags<T, NP>::put(out, COLS ? col_step(a, s - a / 2) : row_step(a, s), paired<T, NP>(half[0], half[1]));
+    }
 }
 
 // COLS: the factors by columns, with accumulator rows i and columns j; else by rows, transposed: rows j, columns i.
@@ -134,9 +152,8 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
           s.a[i * kTile + ii * kPad + jj] = mult[t][r];
         }
       }
-      if constexpr (COLS) Frags<T, NPP>::put(pout + col_step(j, 0) * Frags<T, NPP>::kStep - (j < 2 ? 0 : Frags<T, NPP>::kStep), i, pp[t]);
-      else Frags<T, NPP>::put(pout + row_step(i, 0) * Frags<T, NPP>::kStep, j, pp[t]);
     }
+  put_factor<T, NPP, COLS>(pout, pp);
   wave_lds_sync();
 
   // X = (I + A_bb)^-1 by forward substitution: lane l solves column l % 16 of block l / 16, column by column
@@ -184,65 +201,44 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
 #pragma unroll
       for (int r = 0; r < 4; ++r) tt[i * (i + 1) / 2 + j][r] = -m[r];
     }
-  // the factors as operands: by rows tile (i, j) is half j & 1 of row i's step j / 2, by columns half i & 1 of
-  // column j's step i / 2; the halves outside the triangle are zeros
-  using TF = Frags<T, NT>;
-  using PF = Frags<T, NPP>;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j <= i; ++j) {
-      if constexpr (COLS) TF::put(tout + col_step(j, 0) * TF::kStep - (j < 2 ? 0 : TF::kStep), i, tt[i * (i + 1) / 2 + j]);
-      else TF::put(tout + row_step(i, 0) * TF::kStep, j, tt[i * (i + 1) / 2 + j]);
-    }
-  if constexpr (COLS) {
-    TF::put(tout + col_step(1, 0) * TF::kStep, 0, zero4());
-    TF::put(tout + col_step(3, 0) * TF::kStep - TF::kStep, 2, zero4());
-    PF::put(pout + col_step(1, 0) * PF::kStep, 0, zero4());
-    PF::put(pout + col_step(3, 0) * PF::kStep - PF::kStep, 2, zero4());
-  } else {
-    TF::put(tout + row_step(0, 0) * TF::kStep, 1, zero4());
-    TF::put(tout + row_step(2, 0) * TF::kStep, 3, zero4());
-    PF::put(pout + row_step(0, 0) * PF::kStep, 1, zero4());
-    PF::put(pout + row_step(2, 0) * PF::kStep, 3, zero4());
-  }
+  put_factor<T, NT, COLS>(tout, tt);
 }
 
 // --------------------------------------------------------------------------------------------
 // chain
 // --------------------------------------------------------------------------------------------
 template <typename T, int DP> struct ChainShape {
-  static constexpr int KS = DP / 32;                     // operand steps over the features
-  static constexpr int TILES = DP / 16;                  // feature tiles
-  static constexpr int FT = TILES < 4 ? 1 : TILES / 4;   // of them a chain wave's, at most
-  static constexpr int PITCH = DP + (sizeof(T) == 2 ? 8 : 4);
+  static constexpr int KS = DP / 32;                    // operand steps over the features
+  static constexpr int TILES = DP / 16;                 // feature tiles
+  static constexpr int FT = TILES < 4 ? 1 : TILES / 4;  // of them a chain wave's, at most
   static constexpr int NT = Pieces<T>::kN;
   static constexpr int NO = OutPieces<T>::kN;
   using F = Frags<T, NT>;
   using FO = Frags<T, NO>;
+  using Keys = Tile<T, DP>;
+  using Slice = Tile<T, 16>;
+  struct Stage {  // what comes from memory for the chain, besides T
+    T keys[Keys::kElems];
+    T values[Slice::kElems];
+    float coef[kCoef];
+  };
+  // Chunks in LDS at once: the one in hand and the one whose loads are in flight. Float32 heads of width 256 have room
+  // for one, and wait for each.
+  static constexpr int RING = sizeof(T) == 4 && DP > 128 ? 1 : 2;
   struct Lds {
-    T keys[kChunk * PITCH];
+    Stage ring[RING];
+    T tf[kTriSteps * F::kStep];  // of one chunk: read into registers in its first span
     T state[KS * F::kStep];
     T r[2 * F::kStep];
-    T delta[2 * FO::kStep];
     T kept[2 * F::kStep];
+    float delta[4 * 256];  // accumulator tiles, one after the other
   };
+  static_assert(sizeof(Lds) <= 160 * 1024, "more than a CU's LDS");
 };
 
-// What a chain wave reads of a chunk: its tokens' key rows, its rows of T, its tokens' values and coefficients.
-template <typename T, int DP> struct ChainIn {
-  Operand<T, 1> kf[ChainShape<T, DP>::KS];
-  Operand<T, Pieces<T>::kN> tf[2];
-  T v[4];
-  f32x4 beta, eps, kap;
-  float gam;
-};
-
-// What an output wave reads of a chunk: a quarter of the keys for LDS, its tokens' queries, its rows of P.
+// What an output wave reads of a chunk: its tokens' queries, its rows of P.
 template <typename T, int DP> struct OutIn {
-  static constexpr int LOADS = DP / 32;  // 8 elements a lane each: 64 x DP elements over 256 lanes
-  Operand<T, 1> keys[LOADS];
-  Operand<T, 1> qf[ChainShape<T, DP>::KS];
+  Operand<T, 1> qf[DP / 32];
   Operand<T, OutPieces<T>::kN> pf[2];
   float eps;
   uint8_t on;
@@ -257,19 +253,26 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
   using S = ChainShape<T, DP>;
   using F = typename S::F;
   using FO = typename S::FO;
-  constexpr int KS = S::KS, FT = S::FT, NT = S::NT, NO = S::NO;
+  using Keys = typename S::Keys;
+  using Slice = typename S::Slice;
+  constexpr int KS = S::KS, FT = S::FT, TILES = S::TILES, NT = S::NT, NO = S::NO, RING = S::RING;
   __shared__ __attribute__((aligned(16))) typename S::Lds lds;
 
   const int id = xcd_logical_block(blockIdx.x, gridDim.x);
   const int sl = id % slices, bh = id / slices, h = bh % dims.H, b = bh / dims.H;
   const int D = dims.D, nc = dims.chunks;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
-  const int c = lane_col(), grp = lane_grp();
-  const int vcol = 16 * sl + c;
+  const int c = lane_col(), grp = lane_grp(), lane = threadIdx.x & 63;
   const size_t chunk0 = (size_t)bh * nc;
 
+  // features past D and rows past the end are not brought: zeros, and what an earlier chunk left there, times zeros
+  for (int i = threadIdx.x; i < (int)(sizeof(lds.ring) / 16); i += 512) reinterpret_cast<f32x4*>(lds.ring)[i] = zero4();
+  lds_barrier();
+
   if (wave < 4) {
-    // ---- the chain ----
+    // ---- the chain: wave w has the 16 tokens w of R and Delta, and of the state's feature tiles each fourth ----
+    __builtin_amdgcn_s_setprio(3);
+    const int vcol = 16 * sl + c, own = 16 * w + 4 * grp;
     f32x4 hs[FT];
     const float* sp = s_in + (size_t)bh * D * D;
 #pragma unroll
@@ -280,72 +283,68 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
         const int f = 16 * ft + 4 * grp + r;
         hs[i][r] = f < D && vcol < D ? sp[(size_t)f * D + vcol] : 0.f;
       }
-      if (ft < S::TILES) F::put(lds.state, ft, hs[i]);
+      if (ft < TILES) F::template put_tile<true>(lds.state, ft, hs[i]);
     }
-    auto load = [&](int ci, ChainIn<T, DP>& in) {
-      const int t0 = ci * kChunk;
-      const Rows<T> krows = dims.rows(k, b, t0, h), vrows = dims.rows(v, b, t0, h);
+    lds_barrier();
+    for (int ci = 0; ci < nc; ++ci) {
+      const typename S::Stage& in = lds.ring[RING == 1 ? 0 : ci & 1];
+      if constexpr (RING == 1) lds_barrier();
+      // R = beta (V - eps K H); T's rows on the way
+      f32x4 x = zero4();
 #pragma unroll
-      for (int st = 0; st < KS; ++st) in.kf[st] = krows.row(16 * w + c, 32 * st + 8 * grp);
-      const T* tb = tf + (chunk0 + ci) * Factor<T, NT>::kElems + row_step(w, 0) * F::kStep;
-      in.tf[0] = F::get(tb, 0);
-      in.tf[1] = F::get(tb, w >= 2 ? 1 : 0);
-      const float* co = coef + (chunk0 + ci) * kCoef + 16 * w + 4 * grp;
-      in.beta = *reinterpret_cast<const f32x4*>(co);
-      in.eps = *reinterpret_cast<const f32x4*>(co + kChunk);
-      in.kap = *reinterpret_cast<const f32x4*>(co + 2 * kChunk);
-      in.gam = coef[(chunk0 + ci) * kCoef + 2 * kChunk - 1];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) in.v[r] = vrows.one(16 * w + 4 * grp + r, vcol);
-    };
-    auto step = [&](int ci, const ChainIn<T, DP>& in) {
+      for (int s = 0; s < KS; ++s) x = mma(Keys::row(in.keys, 16 * w + c, 32 * s + 8 * grp), F::get(lds.state, s), x);
+      const f32x4 beta = *reinterpret_cast<const f32x4*>(in.coef + own);
+      const f32x4 eps = *reinterpret_cast<const f32x4*>(in.coef + kChunk + own);
+      const f32x4 vx = Slice::four(in.values, w, 0);
+      const Operand<T, NT> t0 = F::get(lds.tf, row_step(w, 0)), t1 = F::get(lds.tf, row_step(w, w >= 2 ? 1 : 0));
       if constexpr (RECORD) {
         const Record rh = record(rec_h, chunk0 + ci, D, D);
 #pragma unroll
         for (int i = 0; i < FT; ++i) rh.put(vcol, 16 * (w + 4 * i) + 4 * grp, hs[i]);
       }
-      // R = beta (V - eps K H)
-      f32x4 x = zero4();
 #pragma unroll
-      for (int st = 0; st < KS; ++st) x = mma(in.kf[st], F::get(lds.state, st), x);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = in.beta[r] * (to_f32(in.v[r]) - in.eps[r] * x[r]);
-      F::put(lds.r, w, x);
+      for (int r = 0; r < 4; ++r) x[r] = beta[r] * (vx[r] - eps[r] * x[r]);
+      F::template put_tile<false>(lds.r, w, x);
       lds_barrier();
-      // Delta = T R
-      f32x4 dl = mma(in.tf[0], F::get(lds.r, 0), zero4());
-      if (w >= 2) dl = mma(in.tf[1], F::get(lds.r, 1), dl);
+      // Delta = T R; K^T on the way
+      f32x4 dl = mma(t0, F::get(lds.r, 0), zero4());
+      if (w >= 2) dl = mma(t1, F::get(lds.r, 1), dl);
+      const f32x4 kap = *reinterpret_cast<const f32x4*>(in.coef + 2 * kChunk + own);
+      const float gam = in.coef[2 * kChunk - 1];
+      constexpr int AHEAD = FT < 2 ? FT : 2;  // feature tiles whose K^T waits in registers
+      Operand<T, 1> kc[AHEAD][2];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) kc[i][s] = Keys::columns(in.keys, s, 16 * (TILES < 4 ? w & 1 : w + 4 * i));
+#pragma unroll
+      for (int i = 0; i < FT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) hs[i][r] *= gam;
       f32x4 kd;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) kd[r] = in.kap[r] * dl[r];
-      F::put(lds.kept, w, kd);
-      FO::put(lds.delta, w, dl);
-      if constexpr (RECORD) record(rec_d, chunk0 + ci, kChunk, D).put(vcol, 16 * w + 4 * grp, dl);
+      for (int r = 0; r < 4; ++r) kd[r] = kap[r] * dl[r];
+      F::template put_tile<false>(lds.kept, w, kd);
+      *reinterpret_cast<f32x4*>(lds.delta + 256 * w + 4 * lane) = dl;
+      if constexpr (RECORD) record(rec_d, chunk0 + ci, kChunk, D).put(vcol, own, dl);
       lds_barrier();
       // H' = gam H + K^T (kap Delta)
       const Operand<T, NT> k0 = F::get(lds.kept, 0), k1 = F::get(lds.kept, 1);
 #pragma unroll
       for (int i = 0; i < FT; ++i) {
         const int ft = w + 4 * i;
-        if (ft < S::TILES) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) hs[i][r] *= in.gam;
-          hs[i] = mma(load_columns(lds.keys, S::PITCH, 0, 16 * ft), k0, hs[i]);
-          hs[i] = mma(load_columns(lds.keys, S::PITCH, 1, 16 * ft), k1, hs[i]);
-          F::put(lds.state, ft, hs[i]);
+        if (ft < TILES) {
+          if (i >= AHEAD) {
+            hs[i] = mma(Keys::columns(in.keys, 0, 16 * ft), k0, hs[i]);
+            hs[i] = mma(Keys::columns(in.keys, 1, 16 * ft), k1, hs[i]);
+          } else {
+            hs[i] = mma(kc[i < AHEAD ? i : 0][0], k0, hs[i]);
+            hs[i] = mma(kc[i < AHEAD ? i : 0][1], k1, hs[i]);
+          }
+          F::template put_tile<true>(lds.state, ft, hs[i]);
         }
       }
       lds_barrier();
-    };
-    ChainIn<T, DP> a, bb;
-    load(0, a);
-    lds_barrier();
-    for (int ci = 0; ci < nc; ci += 2) {  // past the end the last chunk is loaded again, so that no load is conditional
-      load(ci + 1 < nc ? ci + 1 : ci, bb);
-      step(ci, a);
-      if (ci + 1 >= nc) break;
-      load(ci + 2 < nc ? ci + 2 : ci + 1, a);
-      step(ci + 1, bb);
     }
     float* so = s_out + (size_t)bh * D * D;
 #pragma unroll
@@ -356,60 +355,75 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
         if (f < D && vcol < D) so[(size_t)f * D + vcol] = hs[i][r];
       }
   } else {
-    // ---- the keys into LDS, and the outputs: O^T tile of this wave's 16 tokens (rows values, columns tokens) ----
-    const int hl = threadIdx.x - 256;  // 0 .. 255
-    auto load = [&](int ci, OutIn<T, DP>& in) {
-      const int t0 = ci * kChunk;
-      const Rows<T> krows = dims.rows(k, b, t0, h), qrows = dims.rows(q, b, t0, h);
+    // ---- memory into LDS a chunk ahead, and the outputs: O^T tile of the 16 tokens w (rows values, columns tokens). In a
+    //      chunk's three spans: keys, values and coefficients of the next chunk and this wave's operands of it; T of the
+    //      next chunk (the chain has this one's in registers) and H^T Q^T; the rest ----
+    const size_t stride = (size_t)kChunk * dims.H * D;  // elements from a chunk's rows to the next one's
+    const T *kp = k + dims.at(b, 0, h), *vp = v + dims.at(b, 0, h), *qp = q + dims.at(b, 0, h);
+    const T* tp = tf + chunk0 * Factor<T, NT>::kElems;
+    const T* pp = pf + chunk0 * Factor<T, NO>::kElems + row_step(w, 0) * FO::kStep;
+    const float* cp = coef + chunk0 * kCoef;
+    auto stage = [&](int ci) {
+      typename S::Stage& to = lds.ring[RING == 1 ? 0 : ci & 1];
+      const Rows<T> krows = dims.rows_at(kp + ci * stride, ci), vrows = dims.rows_at(vp + ci * stride, ci);
 #pragma unroll
-      for (int i = 0; i < OutIn<T, DP>::LOADS; ++i) {
-        const int p = hl + 256 * i;
-        in.keys[i] = krows.row(p / (DP / 8), 8 * (p % (DP / 8)));
-      }
-#pragma unroll
-      for (int st = 0; st < KS; ++st) in.qf[st] = qrows.row(16 * w + c, 32 * st + 8 * grp);
-      using PF = FO;
-      const T* pb = pf + (chunk0 + ci) * Factor<T, NO>::kElems + row_step(w, 0) * PF::kStep;
-      in.pf[0] = PF::get(pb, 0);
-      in.pf[1] = PF::get(pb, w >= 2 ? 1 : 0);
-      in.eps = coef[(chunk0 + ci) * kCoef + kChunk + 16 * w + c];
-      in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, t0), 16 * w + c, 0, 0);
+      for (int j = 0; j < Keys::kInstr / 4; ++j) Keys::stage(to.keys, krows, 4 * j + w, 0);
+      if (w < Slice::kInstr) Slice::stage(to.values, vrows, w, 16 * sl);
+      if (w == 3) stage_coef(to.coef, cp + (size_t)ci * kCoef);
     };
-    auto step = [&](int ci, const OutIn<T, DP>& in) {
+    auto stage_t = [&](int ci) {
+      constexpr int TI = kTriSteps * F::kStepInstr;
 #pragma unroll
-      for (int i = 0; i < OutIn<T, DP>::LOADS; ++i) {
-        const int p = hl + 256 * i, row = p / (DP / 8), f = 8 * (p % (DP / 8));
-        T* at = lds.keys + row * S::PITCH + f;
-        if constexpr (sizeof(T) == 2) {
-          *reinterpret_cast<bf16x8*>(at) = in.keys[i].p[0];
-        } else {
-          reinterpret_cast<f32x4*>(at)[0] = in.keys[i].lo;
-          reinterpret_cast<f32x4*>(at)[1] = in.keys[i].hi;
-        }
+      for (int j = 0; j < (TI + 3) / 4; ++j)
+        if (4 * j + w < TI) F::stage(lds.tf, tp + (size_t)ci * Factor<T, NT>::kElems, kTriSteps, 4 * j + w);
+    };
+    auto load = [&](int ci, OutIn<T, DP>& in) {
+      const Rows<T> qrows = dims.rows_at(qp + ci * stride, ci);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) in.qf[s] = qrows.row(16 * w + c, 32 * s + 8 * grp);
+      const T* pb = pp + (size_t)ci * Factor<T, NO>::kElems;
+      in.pf[0] = FO::get(pb, 0);
+      in.pf[1] = FO::get(pb, w >= 2 ? 1 : 0);
+      in.eps = cp[(size_t)ci * kCoef + kChunk + 16 * w + c];
+      in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, ci * kChunk), 16 * w + c, 0, 0);
+    };
+    auto step = [&](int ci, const OutIn<T, DP>& in, OutIn<T, DP>& next) {
+      const int ni = ci + 1 < nc ? ci + 1 : ci;  // past the end the last chunk again, so that nothing is conditional
+      if constexpr (RING == 1) {
+        stage(ci);
+        direct_loads_done();
+        lds_barrier();
+      } else {
+        stage(ni);
       }
+      load(ni, next);
+      lds_barrier();
+      stage_t(ni);
       f32x4 acc = zero4();
 #pragma unroll
-      for (int st = 0; st < KS; ++st) acc = mma(F::template get<NO>(lds.state, st), in.qf[st], acc);
+      for (int s = 0; s < KS; ++s) acc = mma(F::template get<NO>(lds.state, s), in.qf[s], acc);
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[r] *= in.eps;
       lds_barrier();
-      lds_barrier();
-      acc = mma(FO::get(lds.delta, 0), in.pf[0], acc);
-      if (w >= 2) acc = mma(FO::get(lds.delta, 1), in.pf[1], acc);
+      const float* d = lds.delta + 4 * lane;
+      acc = mma(paired<T, NO>(*reinterpret_cast<const f32x4*>(d), *reinterpret_cast<const f32x4*>(d + 256)), in.pf[0], acc);
+      if (w >= 2)
+        acc = mma(paired<T, NO>(*reinterpret_cast<const f32x4*>(d + 512), *reinterpret_cast<const f32x4*>(d + 768)), in.pf[1], acc);
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[r] = active == nullptr || in.on ? acc[r] : 0.f;
+      direct_loads_done();
       dims.rows(o, b, ci * kChunk, h).put_four(16 * w + c, 16 * sl + 4 * grp, acc);
       lds_barrier();
     };
     OutIn<T, DP> a, bb;
+    if constexpr (RING > 1) stage(0);
+    stage_t(0);
     load(0, a);
+    direct_loads_done();
     lds_barrier();
-    for (int ci = 0; ci < nc; ci += 2) {  // past the end the last chunk is loaded again, so that no load is conditional
-      load(ci + 1 < nc ? ci + 1 : ci, bb);
-      step(ci, a);
-      if (ci + 1 >= nc) break;
-      load(ci + 2 < nc ? ci + 2 : ci + 1, a);
-      step(ci + 1, bb);
+    for (int ci = 0; ci < nc; ci += 2) {
+      step(ci, a, bb);
+      if (ci + 1 < nc) step(ci + 1, bb, a);
     }
   }
 }
