@@ -111,6 +111,16 @@ __device__ __forceinline__ Operand<T, NP> paired(f32x4 a, f32x4 b) {
   return o;
 }
 
+// A sum of log decays (in float64) times log2 e as two float32 numbers, and e to the difference of two sums: the first
+// parts' difference is rounded by half a step of itself, as a float32 exponent has to be.
+struct DecaySum { float hi, lo; };
+__device__ __forceinline__ DecaySum decay_sum(double sum) {
+  const double x = sum * 1.4426950408889634074;
+  const float hi = (float)x;
+  return {hi, (float)(x - (double)hi)};
+}
+__device__ __forceinline__ float decay(DecaySum a, DecaySum b) { return __builtin_amdgcn_exp2f((a.hi - b.hi) + (a.lo - b.lo)); }
+
 __device__ __forceinline__ int lane_col() { return threadIdx.x & 15; }
 __device__ __forceinline__ int lane_grp() { return (threadIdx.x & 63) >> 4; }
 
@@ -228,10 +238,11 @@ template <typename T, int W> struct Tile {  // 64 rows of W elements
   }
 };
 
-// The direct loads that this wave has issued are in LDS (and all else that it has loaded has arrived).
-__device__ __forceinline__ void direct_loads_done() {
+// All but the last LEFT of this wave's loads and stores are done: direct loads among them are in LDS.
+template <int LEFT = 0> __device__ __forceinline__ void direct_loads_done() {
+  static_assert(LEFT < 64);
   __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (LEFT & 15) | (LEFT >> 4) << 14);  // vmcnt
   __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -313,11 +324,10 @@ __host__ __device__ constexpr int row_step(int i, int s) { return i < 2 ? i : 2 
 __host__ __device__ constexpr int col_step(int j, int s) { return j < 2 ? 2 * j + s : j + 2; }
 
 // ---- the workspace of one chunk and head ----
-// coefficients: beta, eps, kap, 64 floats each
-constexpr int kCoef = 3 * kChunk;
+// coefficients: beta, eps, kap, 64 floats each; in LDS a direct load's 1 KiB (zeros behind them)
+constexpr int kCoef = 3 * kChunk, kCoefLds = 256;
 __device__ __forceinline__ void stage_coef(float* dst, const float* coef) {
-  const __amdgpu_buffer_rsrc_t r = buffer_rsrc(coef, kCoef * sizeof(float));
-  if ((threadIdx.x & 63) < kCoef / 4) buffer_load_lds16(r, dst, 16 * (threadIdx.x & 63), 0);
+  buffer_load_lds16(buffer_rsrc(coef, kCoef * sizeof(float)), dst, 16 * (threadIdx.x & 63), 0);
 }
 template <typename T, int NP> struct Factor {  // elements of a triangular factor
   static constexpr int kElems = kTriSteps * Frags<T, NP>::kStep;

@@ -44,7 +44,7 @@ template <typename T, int DP> struct BackShape {
   using Slice = Tile<T, 16>;
   struct Stage {  // what comes from memory for the chain, besides T
     T keys[Keys::kElems];
-    float coef[kCoef];
+    float coef[kCoefLds];
   };
   struct Lds {
     Stage ring[RING];
@@ -428,7 +428,7 @@ template <typename T, int DP> struct GradShape {
       Values values;
       Rows rows;
     } u;
-    double sums[kChunk];
+    DecaySum sums[kChunk];
     float beta[kChunk], eps[kChunk], kap[kChunk], dsum[kChunk];
     float part[4][2];  // each wave's share of <dH', H> and of the chunk end's other terms
   };
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(
       const double up = __shfl_up(sum, off);
       if (l >= off) sum += up;
     }
-    lds.sums[l] = sum;
+    lds.sums[l] = decay_sum(sum);
     const float* co = coef + (size_t)id * kCoef;
     lds.beta[l] = co[l];
     lds.eps[l] = co[kChunk + l];
@@ -567,19 +567,19 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(
   }
   const int own = 16 * w + c;
   const float beta_own = lds.beta[own], eps_own = lds.eps[own], kap_own = lds.kap[own];
-  const double sum_own = lds.sums[own];
+  const DecaySum sum_own = lds.sums[own];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = 16 * i + 4 * grp + r;
       if (i <= w) {  // row j, column i
-        const float e = row <= own ? expf((float)(sum_own - lds.sums[row])) : 0.f;
+        const float e = row <= own ? decay(sum_own, lds.sums[row]) : 0.f;
         pt[i][r] *= e;
         bt[i][r] *= row < own ? e : 0.f;
       }
       if (i >= w) {  // row i, column j
-        const float e = row >= own ? expf((float)(lds.sums[row] - sum_own)) : 0.f;
+        const float e = row >= own ? decay(lds.sums[row], sum_own) : 0.f;
         pr[i][r] *= e;
         br[i][r] *= row > own ? -lds.beta[row] * e : 0.f;
       }

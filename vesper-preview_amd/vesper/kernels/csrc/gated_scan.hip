@@ -1,12 +1,13 @@
 // The gated delta rule's chunked scan on CDNA4 (gfx950); the mathematics and the operands are in gated.h.
 //
-//  * gated_prep_kernel: one wave a chunk and head, all of them at once: the decays' sums, the products of all
-//    pairs of the chunk's tokens (K K^T and K Q^T), the inverse T, and both factors written as MFMA operands.
+//  * gated_prep_kernel: a wave a chunk and head, all of them at once: the decays' sums, the products of all
+//    pairs of the chunk's tokens (K K^T and Q K^T), the inverse T and W = P T, both written as MFMA operands.
 //  * gated_chain_kernel: a workgroup a head and 16 value columns walks the chunks (value columns of the state evolve
 //    independently, so a head of width 64 is four chains). Four waves carry the chain, each one tile of 16 tokens
 //    (R, Delta) and its share of the state's feature tiles in accumulators; between the three dependent products
-//    (K H, T R, K^T Delta) the tiles pass through LDS as operands in pieces. Four more waves bring keys, values and
-//    T straight into LDS a chunk ahead and form the outputs in the gaps, so that the chain waits for no memory.
+//    (K H, T R, K^T Delta) the tiles pass through LDS as operands in pieces. Four more waves bring keys and values
+//    straight into LDS two chunks ahead and form the outputs O = eps Q H + W R in the gaps, so that the chain waits
+//    for no memory.
 #include "gated.h"
 #include "vesper_kernels.h"
 
@@ -22,9 +23,9 @@ constexpr int kTile = 16 * kPad + 4;       // tiles start on other banks
 constexpr int kPrepWaves = 4;
 
 struct PrepLds {
-  double sums[kChunk];
-  float beta[kChunk];
-  float a[4 * kTile];  // diagonal tiles of A
+  DecaySum sums[kChunk];
+  float beta[kChunk];  // -beta
+  float a[4 * kTile];  // diagonal tiles of -A
   float x[4 * kTile];  // their inverses (I + A_bb)^-1
 };
 
@@ -41,30 +42,27 @@ __device__ __forceinline__ f32x4 mm16f(f32x4 a, f32x4 b, f32x4 acc) {
   return acc;
 }
 
-// A lower triangle's ten accumulator tiles as the operands of gated.h's six steps; tiles outside the triangle are zeros.
+// Row (COLS: column) a of a lower triangle of accumulator tiles, tile o at x[o], as its operands of gated.h's six steps;
+// tiles outside the triangle are zeros.
 template <typename T, int NP, bool COLS>
-__device__ __forceinline__ void put_factor(T* out, const f32x4 (&x)[10]) {
+__device__ __forceinline__ void put_line(T* out, int a, const f32x4 (&x)[4]) {
 #pragma unroll
-  for (int a = 0; a < 4; ++a)
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (COLS ? 2 * s + 1 < a : 2 * s > a) continue;
-      f32x4 half[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int o = 2 * s + e, i = COLS ? o : a, j = COLS ? a : o;
-        half[e] = j <= i ? x[j <= i ? i * (i + 1) / 2 + j : 0] : zero4();
-      }
-      Frags<T, NP>::put(out, COLS ? col_step(a, s - a / 2) : row_step(a, s), paired<T, NP>(half[0], half[1]));
-    }
+  for (int s = 0; s < 2; ++s) {
+    if (COLS ? 2 * s + 1 < a : 2 * s > a) continue;
+    const bool first = !COLS || 2 * s >= a, second = COLS || 2 * s + 1 <= a;
+    Frags<T, NP>::put(out, COLS ? col_step(a, s - a / 2) : row_step(a, s),
+                      paired<T, NP>(first ? x[2 * s] : zero4(), second ? x[2 * s + 1] : zero4()));
+  }
 }
 
-// COLS: the factors by columns, with accumulator rows i and columns j; else by rows, transposed: rows j, columns i.
-// The off-diagonal tiles of T follow from the diagonal inverses X by T_ij = -X_i sum_k A_ik T_kj (k = j .. i - 1) or,
-// transposed, T_ij^T = -X_j^T sum_k A_kj^T T_ik^T (k = j + 1 .. i). In either form the tile A that multiplies is an
-// accumulator tile of the other form's layout, and what it multiplies is one of its own: no tile leaves registers.
+// COLS, for the backward pass: the factors T and P by columns, with accumulator rows i and columns j. Else T and
+// W = P T by rows, transposed: rows j, columns i. With X the diagonal tiles' inverses (I + A_bb)^-1, tile by tile:
+//   T_ij = -X_i sum_k A_ik T_kj (k = j .. i - 1), or transposed T_ij^T = -X_j^T sum_k A_kj^T T_ik^T (k = j + 1 .. i);
+//   W_ij^T = X_j^T (P_ij^T - sum_k A_kj^T W_ik^T) (k = j + 1 .. i), from W (I + A) = P.
+// In either form the tile A that multiplies is an accumulator tile of the other form's layout, and what it multiplies is
+// one of its own: no tile leaves registers, and a line of T or W is written when it is done.
 template <typename T, int DP, bool COLS>
-__global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
+__global__ __launch_bounds__(64 * kPrepWaves, 2) void gated_prep_kernel(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ beta, const float* __restrict__ g,
     float* __restrict__ coef, T* __restrict__ tf, T* __restrict__ pf, Dims<T> dims, int total) {
   __shared__ PrepLds lds[kPrepWaves];
@@ -91,8 +89,8 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
     }
     const double all = __shfl(sum, 63);
     const float be = ok ? bl : 0.f;
-    s.sums[l] = sum;
-    s.beta[l] = be;
+    s.sums[l] = decay_sum(sum);
+    s.beta[l] = -be;
     float* co = coef + (size_t)id * kCoef;
     co[l] = be;
     co[kChunk + l] = expf((float)sum);
@@ -124,7 +122,7 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
   }
   wave_lds_sync();
 
-  // the decays between pairs, beta and the triangles
+  // the decays between pairs, -beta and the triangles
   T* tout = tf + (size_t)id * Factor<T, NT>::kElems;
   T* pout = pf + (size_t)id * Factor<T, NPP>::kElems;
 #pragma unroll
@@ -137,15 +135,15 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
         const int row = 4 * grp + r;
         {
           const int ii = 16 * i + (COLS ? c : row), jj = 16 * j + (COLS ? row : c);
-          const float e = jj < ii ? expf((float)(s.sums[ii] - s.sums[jj])) : 0.f;
-          mult[t][r] *= s.beta[ii] * e;
+          const float e = decay(s.sums[ii], s.sums[jj]);
+          mult[t][r] *= i > j || jj < ii ? s.beta[ii] * e : 0.f;
         }
         {
           const int ii = 16 * i + (COLS ? row : c), jj = 16 * j + (COLS ? c : row);
-          pp[t][r] = jj <= ii ? pp[t][r] * expf((float)(s.sums[ii] - s.sums[jj])) : 0.f;
+          pp[t][r] *= i > j || jj <= ii ? decay(s.sums[ii], s.sums[jj]) : 0.f;
         }
       }
-      if (i == j) {  // A[ii][jj] of the diagonal tile, row-major
+      if (i == j) {  // -A[ii][jj] of the diagonal tile, row-major
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int ii = COLS ? c : 4 * grp + r, jj = COLS ? 4 * grp + r : c;
@@ -153,7 +151,6 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
         }
       }
     }
-  put_factor<T, NPP, COLS>(pout, pp);
   wave_lds_sync();
 
   // X = (I + A_bb)^-1 by forward substitution: lane l solves column l % 16 of block l / 16, column by column
@@ -165,14 +162,14 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
 #pragma unroll
     for (int kk = 0; kk < 15; ++kk)
 #pragma unroll
-      for (int r = kk + 1; r < 16; ++r) x[r] = __builtin_fmaf(-a[r * kPad + kk], x[kk], x[r]);
+      for (int r = kk + 1; r < 16; ++r) x[r] = __builtin_fmaf(a[r * kPad + kk], x[kk], x[r]);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s.x[grp * kTile + r * kPad + c] = x[r];
   }
   wave_lds_sync();
 
-  // T in this form's accumulator layout, and the diagonal inverses as multipliers
-  f32x4 tt[10], xm[4];
+  // the diagonal inverses in this form's accumulator layout and as multipliers, then line by line
+  f32x4 xt[4], xm[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float* x = s.x + i * kTile;
@@ -180,28 +177,41 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gated_prep_kernel(
     f32x4 down;                                                                   // X[4 g + r][c]
 #pragma unroll
     for (int r = 0; r < 4; ++r) down[r] = x[(4 * grp + r) * kPad + c];
-    tt[i * (i + 1) / 2 + i] = COLS ? down : along;
+    xt[i] = COLS ? down : along;
     xm[i] = COLS ? along : down;
   }
 #pragma unroll
-  for (int off = 1; off < 4; ++off)
+  for (int a = 0; a < 4; ++a) {
+    f32x4 t[4], w[4];
 #pragma unroll
-    for (int j = 0; j + off < 4; ++j) {
-      const int i = j + off;
-      f32x4 m = zero4();
-      if constexpr (COLS) {
+    for (int i = 0; i < 4; ++i) t[i] = w[i] = zero4();
+    t[a] = xt[a];
+    if constexpr (COLS) {
 #pragma unroll
-        for (int kk = j; kk < i; ++kk) m = mm16f(mult[i * (i + 1) / 2 + kk], tt[kk * (kk + 1) / 2 + j], m);
-        m = mm16f(xm[i], m, zero4());
-      } else {
+      for (int i = a; i < 4; ++i) {
+        w[i] = pp[i * (i + 1) / 2 + a];
+        if (i == a) continue;
+        f32x4 m = zero4();
 #pragma unroll
-        for (int kk = j + 1; kk <= i; ++kk) m = mm16f(mult[kk * (kk + 1) / 2 + j], tt[i * (i + 1) / 2 + kk], m);
-        m = mm16f(xm[j], m, zero4());
+        for (int kk = a; kk < i; ++kk) m = mm16f(mult[i * (i + 1) / 2 + kk], t[kk], m);
+        t[i] = mm16f(xm[i], m, zero4());
       }
+    } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) tt[i * (i + 1) / 2 + j][r] = -m[r];
+      for (int j = a; j >= 0; --j) {
+        f32x4 m = zero4(), n = pp[a * (a + 1) / 2 + j];
+#pragma unroll
+        for (int kk = j + 1; kk <= a; ++kk) {
+          m = mm16f(mult[kk * (kk + 1) / 2 + j], t[kk], m);
+          n = mm16f(mult[kk * (kk + 1) / 2 + j], w[kk], n);
+        }
+        if (j < a) t[j] = mm16f(xm[j], m, zero4());
+        w[j] = mm16f(xm[j], n, zero4());
+      }
     }
-  put_factor<T, NT, COLS>(tout, tt);
+    put_line<T, NT, COLS>(tout, a, t);
+    put_line<T, NPP, COLS>(pout, a, w);
+  }
 }
 
 // --------------------------------------------------------------------------------------------
@@ -217,29 +227,35 @@ template <typename T, int DP> struct ChainShape {
   using FO = Frags<T, NO>;
   using Keys = Tile<T, DP>;
   using Slice = Tile<T, 16>;
-  struct Stage {  // what comes from memory for the chain, besides T
+  struct Stage {  // what comes from memory by LDS
     T keys[Keys::kElems];
     T values[Slice::kElems];
-    float coef[kCoef];
+    float coef[kCoefLds];
   };
-  // Chunks in LDS at once: the one in hand and the one whose loads are in flight. Float32 heads of width 256 have room
-  // for one, and wait for each.
-  static constexpr int RING = sizeof(T) == 4 && DP > 128 ? 1 : 2;
+  // How many chunks ahead of the one in hand the loads into LDS go: a chunk is shorter than the memory's latency, so two
+  // (with one, B1 T8191 H12 d64 took 10 us longer). Float32 heads of width 256 have room for the chunk in hand only, and
+  // wait for each.
+  static constexpr size_t kFixed = ((size_t)KS + 4) * F::kStep * sizeof(T), kLds = 160 * 1024;
+  static constexpr int LEAD = kFixed + 3 * sizeof(Stage) <= kLds ? 2 : 0;
+  static constexpr int RING = LEAD + 1;
   struct Lds {
     Stage ring[RING];
-    T tf[kTriSteps * F::kStep];  // of one chunk: read into registers in its first span
     T state[KS * F::kStep];
     T r[2 * F::kStep];
     T kept[2 * F::kStep];
-    float delta[4 * 256];  // accumulator tiles, one after the other
   };
-  static_assert(sizeof(Lds) <= 160 * 1024, "more than a CU's LDS");
+  static_assert(sizeof(Lds) <= kLds, "more than a CU's LDS");
+  // direct loads of one wave for a chunk: keys, a slice of values, coefficients (bf16: two waves each)
+  static constexpr int kLoads = Keys::kInstr / 4 + (sizeof(T) == 2 ? 1 : 2);
 };
 
-// What an output wave reads of a chunk: its tokens' queries, its rows of P.
+// What a chain wave reads of a chunk from memory: its tokens' rows of T.
+template <typename T> struct ChainIn { Operand<T, Pieces<T>::kN> t[2]; };
+
+// What an output wave reads of a chunk: its tokens' queries, its rows of W.
 template <typename T, int DP> struct OutIn {
   Operand<T, 1> qf[DP / 32];
-  Operand<T, OutPieces<T>::kN> pf[2];
+  Operand<T, OutPieces<T>::kN> wf[2];
   float eps;
   uint8_t on;
 };
@@ -255,14 +271,14 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
   using FO = typename S::FO;
   using Keys = typename S::Keys;
   using Slice = typename S::Slice;
-  constexpr int KS = S::KS, FT = S::FT, TILES = S::TILES, NT = S::NT, NO = S::NO, RING = S::RING;
+  constexpr int KS = S::KS, FT = S::FT, TILES = S::TILES, NT = S::NT, NO = S::NO, LEAD = S::LEAD, RING = S::RING;
   __shared__ __attribute__((aligned(16))) typename S::Lds lds;
 
   const int id = xcd_logical_block(blockIdx.x, gridDim.x);
   const int sl = id % slices, bh = id / slices, h = bh % dims.H, b = bh / dims.H;
   const int D = dims.D, nc = dims.chunks;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
-  const int c = lane_col(), grp = lane_grp(), lane = threadIdx.x & 63;
+  const int c = lane_col(), grp = lane_grp();
   const size_t chunk0 = (size_t)bh * nc;
 
   // features past D and rows past the end are not brought: zeros, and what an earlier chunk left there, times zeros
@@ -273,6 +289,14 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
     // ---- the chain: wave w has the 16 tokens w of R and Delta, and of the state's feature tiles each fourth ----
     __builtin_amdgcn_s_setprio(3);
     const int vcol = 16 * sl + c, own = 16 * w + 4 * grp;
+    const T* tp = tf + chunk0 * Factor<T, NT>::kElems + row_step(w, 0) * F::kStep;
+    auto load = [&](int ci, ChainIn<T>& to) {
+      const T* tc = tp + (size_t)(ci < nc ? ci : nc - 1) * Factor<T, NT>::kElems;
+      to.t[0] = F::get(tc, 0);
+      to.t[1] = F::get(tc, w >= 2 ? 1 : 0);  // always, so that no wait for a chunk's waits for the next one's too
+    };
+    ChainIn<T> ta, tb;
+    load(0, ta);
     f32x4 hs[FT];
     const float* sp = s_in + (size_t)bh * D * D;
 #pragma unroll
@@ -286,17 +310,29 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
       if (ft < TILES) F::template put_tile<true>(lds.state, ft, hs[i]);
     }
     lds_barrier();
-    for (int ci = 0; ci < nc; ++ci) {
-      const typename S::Stage& in = lds.ring[RING == 1 ? 0 : ci & 1];
-      if constexpr (RING == 1) lds_barrier();
-      // R = beta (V - eps K H); T's rows on the way
+    int slot = 0;
+    auto step = [&](int ci, const ChainIn<T>& tin, ChainIn<T>& next) {
+      const typename S::Stage& in = lds.ring[slot];
+      slot = slot + 1 < RING ? slot + 1 : 0;
+      if constexpr (LEAD == 0) lds_barrier();
+      // R = beta (V - eps K H)
       f32x4 x = zero4();
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x = mma(Keys::row(in.keys, 16 * w + c, 32 * s + 8 * grp), F::get(lds.state, s), x);
+      for (int s0 = 0; s0 < KS; s0 += 2) {
+        Operand<T, 1> kr[2];
+        Operand<T, NT> st[2];
+#pragma unroll
+        for (int s = 0; s < 2 && s0 + s < KS; ++s) {
+          kr[s] = Keys::row(in.keys, 16 * w + c, 32 * (s0 + s) + 8 * grp);
+          st[s] = F::get(lds.state, s0 + s);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // reads together, not one by one before its product
+#pragma unroll
+        for (int s = 0; s < 2 && s0 + s < KS; ++s) x = mma(kr[s], st[s], x);
+      }
       const f32x4 beta = *reinterpret_cast<const f32x4*>(in.coef + own);
       const f32x4 eps = *reinterpret_cast<const f32x4*>(in.coef + kChunk + own);
       const f32x4 vx = Slice::four(in.values, w, 0);
-      const Operand<T, NT> t0 = F::get(lds.tf, row_step(w, 0)), t1 = F::get(lds.tf, row_step(w, w >= 2 ? 1 : 0));
       if constexpr (RECORD) {
         const Record rh = record(rec_h, chunk0 + ci, D, D);
 #pragma unroll
@@ -306,9 +342,12 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
       for (int r = 0; r < 4; ++r) x[r] = beta[r] * (vx[r] - eps[r] * x[r]);
       F::template put_tile<false>(lds.r, w, x);
       lds_barrier();
-      // Delta = T R; K^T on the way
-      f32x4 dl = mma(t0, F::get(lds.r, 0), zero4());
-      if (w >= 2) dl = mma(t1, F::get(lds.r, 1), dl);
+      // Delta = T R; the next chunk's T and K^T on the way
+      const Operand<T, NT> r0 = F::get(lds.r, 0), r1 = F::get(lds.r, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      load(ci + 1, next);
+      f32x4 dl = mma(tin.t[0], r0, zero4());
+      if (w >= 2) dl = mma(tin.t[1], r1, dl);
       const f32x4 kap = *reinterpret_cast<const f32x4*>(in.coef + 2 * kChunk + own);
       const float gam = in.coef[2 * kChunk - 1];
       constexpr int AHEAD = FT < 2 ? FT : 2;  // feature tiles whose K^T waits in registers
@@ -325,11 +364,11 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
 #pragma unroll
       for (int r = 0; r < 4; ++r) kd[r] = kap[r] * dl[r];
       F::template put_tile<false>(lds.kept, w, kd);
-      *reinterpret_cast<f32x4*>(lds.delta + 256 * w + 4 * lane) = dl;
       if constexpr (RECORD) record(rec_d, chunk0 + ci, kChunk, D).put(vcol, own, dl);
       lds_barrier();
       // H' = gam H + K^T (kap Delta)
       const Operand<T, NT> k0 = F::get(lds.kept, 0), k1 = F::get(lds.kept, 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < FT; ++i) {
         const int ft = w + 4 * i;
@@ -345,6 +384,10 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
         }
       }
       lds_barrier();
+    };
+    for (int ci = 0; ci < nc; ci += 2) {
+      step(ci, ta, tb);
+      if (ci + 1 < nc) step(ci + 1, tb, ta);
     }
     float* so = s_out + (size_t)bh * D * D;
 #pragma unroll
@@ -355,69 +398,81 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
         if (f < D && vcol < D) so[(size_t)f * D + vcol] = hs[i][r];
       }
   } else {
-    // ---- memory into LDS a chunk ahead, and the outputs: O^T tile of the 16 tokens w (rows values, columns tokens). In a
-    //      chunk's three spans: keys, values and coefficients of the next chunk and this wave's operands of it; T of the
-    //      next chunk (the chain has this one's in registers) and H^T Q^T; the rest ----
+    // ---- memory into LDS ahead, and the outputs: O^T tile of the 16 tokens w (rows values, columns tokens). In a chunk's
+    //      three spans: H^T Q^T and this wave's operands of the next chunk; W R, while the chain loads its T; of the chunk
+    //      LEAD ahead keys, values and coefficients, and the outputs' store: the loads are spread, for a CU takes 64 bytes a
+    //      cycle and who issues waits for its turn. Every wave
+    //      issues kLoads direct loads a chunk, after its other loads and unconditionally, so that a wait can leave those of
+    //      one chunk in flight; past the end they bring the last chunk again ----
     const size_t stride = (size_t)kChunk * dims.H * D;  // elements from a chunk's rows to the next one's
     const T *kp = k + dims.at(b, 0, h), *vp = v + dims.at(b, 0, h), *qp = q + dims.at(b, 0, h);
-    const T* tp = tf + chunk0 * Factor<T, NT>::kElems;
+    T* op = o + dims.at(b, 0, h);
     const T* pp = pf + chunk0 * Factor<T, NO>::kElems + row_step(w, 0) * FO::kStep;
     const float* cp = coef + chunk0 * kCoef;
-    auto stage = [&](int ci) {
-      typename S::Stage& to = lds.ring[RING == 1 ? 0 : ci & 1];
+    auto within = [&](int ci) { return ci < nc ? ci : nc - 1; };
+    auto stage = [&](int ahead, int slot) {
+      const int ci = within(ahead);
+      typename S::Stage& to = lds.ring[slot];
       const Rows<T> krows = dims.rows_at(kp + ci * stride, ci), vrows = dims.rows_at(vp + ci * stride, ci);
+      const float* co = cp + (size_t)ci * kCoef;
 #pragma unroll
       for (int j = 0; j < Keys::kInstr / 4; ++j) Keys::stage(to.keys, krows, 4 * j + w, 0);
-      if (w < Slice::kInstr) Slice::stage(to.values, vrows, w, 16 * sl);
-      if (w == 3) stage_coef(to.coef, cp + (size_t)ci * kCoef);
+      if constexpr (Slice::kInstr == 4) {
+        Slice::stage(to.values, vrows, w, 16 * sl);
+        stage_coef(to.coef, co);
+      } else {
+        if (w < 2) Slice::stage(to.values, vrows, w, 16 * sl);
+        else stage_coef(to.coef, co);
+      }
     };
-    auto stage_t = [&](int ci) {
-      constexpr int TI = kTriSteps * F::kStepInstr;
-#pragma unroll
-      for (int j = 0; j < (TI + 3) / 4; ++j)
-        if (4 * j + w < TI) F::stage(lds.tf, tp + (size_t)ci * Factor<T, NT>::kElems, kTriSteps, 4 * j + w);
-    };
-    auto load = [&](int ci, OutIn<T, DP>& in) {
+    auto load = [&](int ahead, OutIn<T, DP>& in) {
+      const int ci = within(ahead);
       const Rows<T> qrows = dims.rows_at(qp + ci * stride, ci);
 #pragma unroll
       for (int s = 0; s < KS; ++s) in.qf[s] = qrows.row(16 * w + c, 32 * s + 8 * grp);
       const T* pb = pp + (size_t)ci * Factor<T, NO>::kElems;
-      in.pf[0] = FO::get(pb, 0);
-      in.pf[1] = FO::get(pb, w >= 2 ? 1 : 0);
+      in.wf[0] = FO::get(pb, 0);
+      in.wf[1] = FO::get(pb, w >= 2 ? 1 : 0);
       in.eps = cp[(size_t)ci * kCoef + kChunk + 16 * w + c];
       in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, ci * kChunk), 16 * w + c, 0, 0);
     };
+    int free = LEAD == 0 ? 0 : RING - 1;  // the slot of the chunk LEAD ahead
     auto step = [&](int ci, const OutIn<T, DP>& in, OutIn<T, DP>& next) {
-      const int ni = ci + 1 < nc ? ci + 1 : ci;  // past the end the last chunk again, so that nothing is conditional
-      if constexpr (RING == 1) {
-        stage(ci);
+      if constexpr (LEAD == 0) {
+        stage(ci, 0);
         direct_loads_done();
         lds_barrier();
-      } else {
-        stage(ni);
       }
-      load(ni, next);
-      lds_barrier();
-      stage_t(ni);
       f32x4 acc = zero4();
 #pragma unroll
-      for (int s = 0; s < KS; ++s) acc = mma(F::template get<NO>(lds.state, s), in.qf[s], acc);
+      for (int s0 = 0; s0 < KS; s0 += 2) {
+        Operand<T, NO> st[2];
+#pragma unroll
+        for (int s = 0; s < 2 && s0 + s < KS; ++s) st[s] = F::template get<NO>(lds.state, s0 + s);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < 2 && s0 + s < KS; ++s) acc = mma(st[s], in.qf[s0 + s], acc);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[r] *= in.eps;
+      load(ci + 1, next);
       lds_barrier();
-      const float* d = lds.delta + 4 * lane;
-      acc = mma(paired<T, NO>(*reinterpret_cast<const f32x4*>(d), *reinterpret_cast<const f32x4*>(d + 256)), in.pf[0], acc);
-      if (w >= 2)
-        acc = mma(paired<T, NO>(*reinterpret_cast<const f32x4*>(d + 512), *reinterpret_cast<const f32x4*>(d + 768)), in.pf[1], acc);
+      const Operand<T, NO> r0 = F::template get<NO>(lds.r, 0), r1 = F::template get<NO>(lds.r, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      acc = mma(r0, in.wf[0], acc);
+      if (w >= 2) acc = mma(r1, in.wf[1], acc);
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[r] = active == nullptr || in.on ? acc[r] : 0.f;
-      direct_loads_done();
-      dims.rows(o, b, ci * kChunk, h).put_four(16 * w + c, 16 * sl + 4 * grp, acc);
+      lds_barrier();
+      if constexpr (LEAD > 0) stage(ci + LEAD, free);
+      direct_loads_done<LEAD == 0 ? 0 : S::kLoads>();
+      dims.rows_at(op + ci * stride, ci).put_four(16 * w + c, 16 * sl + 4 * grp, acc);
+      free = free + 1 < RING ? free + 1 : 0;
       lds_barrier();
     };
     OutIn<T, DP> a, bb;
-    if constexpr (RING > 1) stage(0);
-    stage_t(0);
+#pragma unroll
+    for (int ci = 0; ci < LEAD; ++ci) stage(ci, ci);
     load(0, a);
     direct_loads_done();
     lds_barrier();
@@ -426,6 +481,7 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
       if (ci + 1 < nc) step(ci + 1, bb, a);
     }
   }
+  direct_loads_done();
 }
 
 template <typename T, int DP>
