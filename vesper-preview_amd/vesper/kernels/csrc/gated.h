@@ -324,8 +324,9 @@ __host__ __device__ constexpr int row_step(int i, int s) { return i < 2 ? i : 2 
 __host__ __device__ constexpr int col_step(int j, int s) { return j < 2 ? 2 * j + s : j + 2; }
 
 // ---- the workspace of one chunk and head ----
-// coefficients: beta, eps, kap, 64 floats each; in LDS a direct load's 1 KiB (zeros behind them)
-constexpr int kCoef = 3 * kChunk, kCoefLds = 256;
+// coefficients: beta, eps, kap, 64 floats each, and behind these both parts of the sums of the decays; of the first three
+// in LDS a direct load's 1 KiB (zeros behind them)
+constexpr int kCoef = 3 * kChunk, kCoefLds = 256, kCoefAll = 5 * kChunk;
 __device__ __forceinline__ void stage_coef(float* dst, const float* coef) {
   buffer_load_lds16(buffer_rsrc(coef, kCoef * sizeof(float)), dst, 16 * (threadIdx.x & 63), 0);
 }

@@ -192,7 +192,7 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
     const T *kp = k + dims.at(b, 0, h), *qp = q + dims.at(b, 0, h), *gp = d_o + dims.at(b, 0, h);
     const T* tp = tf + chunk0 * Factor<T, NT>::kElems;
     const T* pp = pf + chunk0 * Factor<T, NT>::kElems + col_step(w, 0) * F::kStep;
-    const float* cp = coef + chunk0 * kCoef;
+    const float* cp = coef + chunk0 * kCoefAll;
     auto chunk_of = [&](int it) { return it < nc ? nc - 1 - it : 0; };
     auto stage = [&](int it) {
       const int ci = chunk_of(it);
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
       const Rows<T> rows = dims.rows_at(kp + ci * stride, ci);
 #pragma unroll
       for (int j = 0; j < Keys::kInstr / 4; ++j) Keys::stage(to.keys, rows, 4 * j + w, 0);
-      if (w == 3) stage_coef(to.coef, cp + (size_t)ci * kCoef);
+      if (w == 3) stage_coef(to.coef, cp + (size_t)ci * kCoefAll);
     };
     // `slot` as a constant: the reads of one slot then do not wait for the loads into the other
     auto stage_q = [&](int it, auto slot) {
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
       const T* pb = pp + (size_t)ci * Factor<T, NT>::kElems;
       in.pf[0] = F::get(pb, 0);
       in.pf[1] = F::get(pb, w < 2 ? 1 : 0);
-      const float* co = cp + (size_t)ci * kCoef + kChunk + 4 * grp;
+      const float* co = cp + (size_t)ci * kCoefAll + kChunk + 4 * grp;
 #pragma unroll
       for (int i = 0; i < 4; ++i) in.eps[i] = *reinterpret_cast<const f32x4*>(co + 16 * i);
       in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, ci * kChunk), lane, 0, 0);
@@ -336,10 +336,10 @@ template <typename T, int NP, int ROWS, int PITCH> struct Planes {
   T x[NP * kPlane];
   __device__ __forceinline__ void put(int row, int col, f32x4 v) {
     if constexpr (sizeof(T) == 2) {
-      const Operand<T, NP> p = paired<T, NP>(v, zero4());
+      bf16x4 p[NP];
+      split4<NP>(v, p);
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
-        *reinterpret_cast<bf16x4*>(x + i * kPlane + row * PITCH + col) = __builtin_shufflevector(p.p[i], p.p[i], 0, 1, 2, 3);
+      for (int i = 0; i < NP; ++i) *reinterpret_cast<bf16x4*>(x + i * kPlane + row * PITCH + col) = p[i];
     } else {
       *reinterpret_cast<f32x4*>(x + row * PITCH + col) = v;
     }
@@ -413,6 +413,8 @@ template <typename T, int DP> struct GradShape {
   static constexpr int NT = Pieces<T>::kN;
   static constexpr int PAD = sizeof(T) == 2 ? 8 : 4;
   static constexpr int PITCH = DP + PAD;
+  static constexpr int QUADS = DP / 4;                      // float32 quads a row of the states' records
+  static constexpr int ITEMS = DP < 64 ? 1 : DP / 64;       // of 32 rows a thread's
   using States = Planes<T, NT, 32, DP + PAD>;
   using Tokens = Planes<T, NT, 32, kChunk + PAD>;
   struct Values {  // 32 value columns
@@ -427,246 +429,280 @@ template <typename T, int DP> struct GradShape {
     union {
       Values values;
       Rows rows;
+      f32x4 y[4][TILES][64];  // beta Y as accumulator tiles
     } u;
-    DecaySum sums[kChunk];
-    float beta[kChunk], eps[kChunk], kap[kChunk], dsum[kChunk];
-    float part[4][2];  // each wave's share of <dH', H> and of the chunk end's other terms
+    float coef[kCoefAll];
+    float dsum[2][kChunk];
+    float part[8][2];  // each wave's share of <dH', H> and of the chunk end's other terms
   };
 };
 
+// Waves 0 to 3 hold dQ and Y of the 16 tokens w, waves 4 to 7 C. What comes from memory for the next 32 value columns is in
+// flight while those in LDS are multiplied.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void gated_grad_kernel(
+__global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const float* __restrict__ g,
     const T* __restrict__ d_o, const float* __restrict__ coef, const float* __restrict__ rec_h,
     const float* __restrict__ rec_d, const float* __restrict__ rec_dh, const float* __restrict__ rec_dr,
     const uint8_t* __restrict__ active, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dbeta,
     float* __restrict__ dg, Dims<T> dims) {
   using S = GradShape<T, DP>;
-  constexpr int NT = S::NT, TILES = S::TILES;
+  constexpr int NT = S::NT, TILES = S::TILES, QUADS = S::QUADS, ITEMS = S::ITEMS;
   __shared__ __attribute__((aligned(16))) typename S::Lds lds;
   const int id = xcd_logical_block(blockIdx.x, gridDim.x);
   const int chunk = id % dims.chunks, bh = id / dims.chunks, h = bh % dims.H, b = bh / dims.H;
   const int D = dims.D, t0 = chunk * kChunk;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, c = l & 15, grp = l >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+  const int l = threadIdx.x & 63, c = l & 15, grp = l >> 4, own = 16 * w + c;
 
-  // the decays' sums, as the prep kernel forms them
-  float gl = 0.f;
-  if (w == 0) {
-    const bool ok = t0 + l < dims.N;
-    gl = g[((size_t)b * dims.N + (ok ? t0 + l : t0)) * dims.H + h];
-    double sum = ok ? ((double)gl < kLeastDecay ? kLeastDecay : (double)gl) : 0.0;
+  auto body = [&](auto kind) {
+    constexpr bool first = decltype(kind)::value;
+    // ---- sums over the value columns, 32 at a time ----
+    // first: dQ^T and Y^T (rows features, columns the wave's tokens); dP^T, B^T (rows j, columns the wave's tokens i >= j);
+    // else: C^T; dP, B (rows i, columns the wave's tokens j <= i)
+    f32x4 acc[TILES], ay[first ? TILES : 1], mp[4], mb[4];
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const double up = __shfl_up(sum, off);
-      if (l >= off) sum += up;
+    for (int i = 0; i < TILES; ++i) acc[i] = ay[first ? i : 0] = zero4();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mp[i] = mb[i] = zero4();
+    float inner = 0.f, dot_v = 0.f;
+    const unsigned state_bytes = (unsigned)D * D * 4u, token_bytes = (unsigned)D * kChunk * 4u;
+    const __amdgpu_buffer_rsrc_t rh = buffer_rsrc(rec_h + (size_t)id * D * D, state_bytes), rdh = buffer_rsrc(rec_dh + (size_t)id * D * D, state_bytes),
+                                 rd = buffer_rsrc(rec_d + (size_t)id * D * kChunk, token_bytes), rdr = buffer_rsrc(rec_dr + (size_t)id * D * kChunk, token_bytes);
+    const Rows<T> dorows = dims.rows(d_o, b, t0, h), vrows = dims.rows(v, b, t0, h);
+    bool on[first ? 1 : 4];  // of the own token; of token 16 i + c
+    {
+      const __amdgpu_buffer_rsrc_t flags = dims.flags(active, b, t0);
+#pragma unroll
+      for (int i = 0; i < (first ? 1 : 4); ++i)
+        on[i] = active == nullptr || (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(flags, first ? own : 16 * i + c, 0, 0) != 0;
     }
-    lds.sums[l] = decay_sum(sum);
-    const float* co = coef + (size_t)id * kCoef;
-    lds.beta[l] = co[l];
-    lds.eps[l] = co[kChunk + l];
-    lds.kap[l] = co[2 * kChunk + l];
-  }
+    if (threadIdx.x < kCoefAll / 4)
+      reinterpret_cast<f32x4*>(lds.coef)[threadIdx.x] = reinterpret_cast<const f32x4*>(coef + (size_t)id * kCoefAll)[threadIdx.x];
 
-  // ---- sums over the value columns, 32 at a time ----
-  f32x4 aq[TILES], ay[TILES], ac[TILES];  // dQ^T, Y^T, C^T: rows features, columns the wave's tokens
+    f32x4 xh[ITEMS], xdh[ITEMS], xd, xdr;  // records of the next value columns
+    auto load16 = [](__amdgpu_buffer_rsrc_t r, unsigned at) { return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0)); };
+    auto load = [&](int v0) {
 #pragma unroll
-  for (int i = 0; i < TILES; ++i) aq[i] = ay[i] = ac[i] = zero4();
-  // by rows j, columns the wave's tokens i: dP^T, B^T (j <= i); by rows i, columns the wave's tokens j: dP, B (i >= j)
-  f32x4 pt[4], bt[4], pr[4], br[4];
+      for (int n = 0; n < ITEMS; ++n) {
+        const int p = threadIdx.x + 512 * n, row = p / QUADS, f = 4 * (p % QUADS);
+        const unsigned at = row < 32 && f < D ? ((unsigned)(v0 + row) * D + f) * 4u : kNowhere;
+        xh[n] = load16(rh, at);
+        xdh[n] = load16(rdh, at);
+      }
+      const unsigned at = ((unsigned)v0 * kChunk + 4 * threadIdx.x) * 4u;
+      xd = load16(rd, at);
+      xdr = load16(rdr, at);
+    };
+    load(0);
+    for (int v0 = 0; v0 < D; v0 += 32) {
+      const int vc = v0 + 8 * grp;
+      Operand<T, 1> dof[4];  // dO of all tokens; first: dO and V of its own
+      if constexpr (first) {
+        dof[0] = dorows.row(own, on[0] ? vc : D);
+        dof[1] = vrows.row(own, vc);
+      } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) pt[i] = bt[i] = pr[i] = br[i] = zero4();
-  float inner = 0.f, dot_v = 0.f;
-  const int token = t0 + 16 * w + c;
-  const Rows<T> dorows = dims.rows(d_o, b, t0, h), vrows = dims.rows(v, b, t0, h);
-  bool on[4];  // of token 16 i + c
-  {
-    const __amdgpu_buffer_rsrc_t flags = dims.flags(active, b, t0);
+        for (int i = 0; i < 4; ++i) dof[i] = dorows.row(16 * i + c, on[first ? 0 : i] ? vc : D);
+      }
+#pragma unroll
+      for (int n = 0; n < ITEMS; ++n) {
+        const int p = threadIdx.x + 512 * n, row = p / QUADS, f = 4 * (p % QUADS);
+        inner += (xh[n][0] * xdh[n][0] + xh[n][1] * xdh[n][1]) + (xh[n][2] * xdh[n][2] + xh[n][3] * xdh[n][3]);
+        if (32 * QUADS >= 512 || row < 32) {
+          lds.u.values.h.put(row, f, xh[n]);
+          lds.u.values.dh.put(row, f, xdh[n]);
+        }
+      }
+      lds.u.values.delta.put(threadIdx.x / 16, 4 * (threadIdx.x % 16), xd);
+      lds.u.values.dr.put(threadIdx.x / 16, 4 * (threadIdx.x % 16), xdr);
+      lds_barrier();
+      load(v0 + 32);  // past the width: zeros
+      if constexpr (first) {
+        const Operand<T, NT> dr_w = lds.u.values.dr.columns(16 * w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i <= w) {
+            const Operand<T, NT> x = lds.u.values.delta.columns(16 * i);
+            mp[i] = mma(x, dof[0], mp[i]);
+            mb[i] = mma(x, dr_w, mb[i]);
+          }
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+          const Operand<T, NT> x = lds.u.values.h.columns(16 * i);
+          acc[i] = mma(x, dof[0], acc[i]);
+          ay[i] = mma(x, dr_w, ay[i]);
+        }
+        dot_v += operand_dot(dr_w, dof[1]);
+      } else {
+        const Operand<T, NT> del_w = lds.u.values.delta.columns(16 * w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i >= w) {
+            mp[i] = mma(dof[i], del_w, mp[i]);
+            mb[i] = mma(lds.u.values.dr.columns(16 * i), del_w, mb[i]);
+          }
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) acc[i] = mma(lds.u.values.dh.columns(16 * i), del_w, acc[i]);
+      }
+      lds_barrier();
+    }
+
+    // ---- the keys and queries, the decays between pairs, sums over the chunk's tokens ----
+    constexpr int PIECES = kChunk * (DP / 8), KQ = (PIECES + 511) / 512;
+    Operand<T, 1> kx[KQ], qx[KQ];
+    {
+      const Rows<T> krows = dims.rows(k, b, t0, h), qrows = dims.rows(q, b, t0, h);
+#pragma unroll
+      for (int n = 0; n < KQ; ++n) {
+        const int p = threadIdx.x + 512 * n, row = p / (DP / 8), f = 8 * (p % (DP / 8));
+        kx[n] = krows.row(row, row < kChunk ? f : D);
+        qx[n] = qrows.row(row, row < kChunk ? f : D);
+      }
+    }
+    auto sum_at = [&](int i) { return DecaySum{lds.coef[kCoef + i], lds.coef[kCoef + kChunk + i]}; };
+    const float beta_own = lds.coef[own];
+    const DecaySum sum_own = sum_at(own);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      on[i] = active == nullptr || (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(flags, 16 * i + c, 0, 0) != 0;
-  }
-  for (int v0 = 0; v0 < D; v0 += 32) {
-    if (v0 > 0) __syncthreads();
-    constexpr int QUADS = DP / 4;
-    for (int p = threadIdx.x; p < 32 * QUADS; p += 256) {
-      const int row = p / QUADS, f = 4 * (p % QUADS);
-      const bool ok = v0 + row < D && f < D;
-      const size_t at = ((size_t)id * D + (ok ? v0 + row : 0)) * D + (ok ? f : 0);
-      f32x4 x = *reinterpret_cast<const f32x4*>(rec_h + at), y = *reinterpret_cast<const f32x4*>(rec_dh + at);
-      if (!ok) x = y = zero4();
-      inner += (x[0] * y[0] + x[1] * y[1]) + (x[2] * y[2] + x[3] * y[3]);
-      lds.u.values.h.put(row, f, x);
-      lds.u.values.dh.put(row, f, y);
-    }
-    for (int p = threadIdx.x; p < 32 * (kChunk / 4); p += 256) {
-      const int row = p / (kChunk / 4), t = 4 * (p % (kChunk / 4));
-      const bool ok = v0 + row < D;
-      const size_t at = ((size_t)id * D + (ok ? v0 + row : 0)) * kChunk + t;
-      f32x4 x = *reinterpret_cast<const f32x4*>(rec_d + at), y = *reinterpret_cast<const f32x4*>(rec_dr + at);
-      if (!ok) x = y = zero4();
-      lds.u.values.delta.put(row, t, x);
-      lds.u.values.dr.put(row, t, y);
-    }
-    Operand<T, 1> dof[4];
-    const int vc = v0 + 8 * grp;
+      if (first ? i <= w : i >= w) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) dof[i] = dorows.row(16 * i + c, on[i] ? vc : D);
-    const Operand<T, 1> vf = vrows.row(16 * w + c, vc);
-    __syncthreads();
-    const Operand<T, NT> del_w = lds.u.values.delta.columns(16 * w), dr_w = lds.u.values.dr.columns(16 * w);
-    dot_v += operand_dot(dr_w, vf);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i <= w) {
-        const Operand<T, NT> x = lds.u.values.delta.columns(16 * i);
-        Operand<T, 1> own = dof[0];
-        if (w == 1) own = dof[1];
-        if (w == 2) own = dof[2];
-        if (w == 3) own = dof[3];
-        pt[i] = mma(x, own, pt[i]);
-        bt[i] = mma(x, dr_w, bt[i]);
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * i + 4 * grp + r;
+          const DecaySum sum = sum_at(row);
+          if constexpr (first) {  // row j, column i
+            const float e = row <= own ? decay(sum_own, sum) : 0.f;
+            mp[i][r] *= e;
+            mb[i][r] *= row < own ? e : 0.f;
+          } else {  // row i, column j
+            const float e = row >= own ? decay(sum, sum_own) : 0.f;
+            mp[i][r] *= e;
+            mb[i][r] *= row > own ? -lds.coef[row] * e : 0.f;
+          }
+        }
       }
-      if (i >= w) {
-        pr[i] = mma(dof[i], del_w, pr[i]);
-        br[i] = mma(lds.u.values.dr.columns(16 * i), del_w, br[i]);
+    const float scale = lds.coef[(first ? kChunk : 2 * kChunk) + own];  // eps, kap
+#pragma unroll
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        acc[i][r] *= scale;
+        if constexpr (first) ay[i][r] *= scale;
+      }
+#pragma unroll
+    for (int n = 0; n < KQ; ++n) {
+      const int p = threadIdx.x + 512 * n, row = p / (DP / 8), f = 8 * (p % (DP / 8));
+      if (PIECES % 512 == 0 || row < kChunk) {
+        T *kd = lds.u.rows.keys + row * S::PITCH + f, *qd = lds.u.rows.queries + row * S::PITCH + f;
+        if constexpr (sizeof(T) == 2) {
+          *reinterpret_cast<bf16x8*>(kd) = kx[n].p[0];
+          *reinterpret_cast<bf16x8*>(qd) = qx[n].p[0];
+        } else {
+          reinterpret_cast<f32x4*>(kd)[0] = kx[n].lo;
+          reinterpret_cast<f32x4*>(kd)[1] = kx[n].hi;
+          reinterpret_cast<f32x4*>(qd)[0] = qx[n].lo;
+          reinterpret_cast<f32x4*>(qd)[1] = qx[n].hi;
+        }
       }
     }
+    lds_barrier();
+    const T *keys_own = lds.u.rows.keys + own * S::PITCH + 4 * grp, *queries_own = lds.u.rows.queries + own * S::PITCH + 4 * grp;
+    float end = 0.f;  // sum_j kap_j k_j.(dH' Delta_j)
+    if constexpr (!first) {
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) {
+        const f32x4 kf = four(keys_own + 16 * i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) end += kf[r] * acc[i][r];
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (first ? 2 * s <= w : 2 * s + 1 >= w) {
+        const Operand<T, NT> x = paired<T, NT>(mp[2 * s], mp[2 * s + 1]), y = paired<T, NT>(mb[2 * s], mb[2 * s + 1]);
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+          const Operand<T, 1> kc = load_columns_paired(lds.u.rows.keys, S::PITCH, s, 16 * i);
+          if constexpr (first) {
+            acc[i] = mma(kc, x, acc[i]);
+            ay[i] = mma(kc, y, ay[i]);
+          } else {
+            acc[i] = mma(load_columns_paired(lds.u.rows.queries, S::PITCH, s, 16 * i), x, acc[i]);
+            acc[i] = mma(kc, y, acc[i]);
+          }
+        }
+      }
+
+    // ---- out ----
+    float dot_a = 0.f, dot_y = 0.f;  // q.dQ or k.C, and k.Y
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
-      const Operand<T, NT> x = lds.u.values.h.columns(16 * i);
-      Operand<T, 1> own = dof[0];
-      if (w == 1) own = dof[1];
-      if (w == 2) own = dof[2];
-      if (w == 3) own = dof[3];
-      aq[i] = mma(x, own, aq[i]);
-      ay[i] = mma(x, dr_w, ay[i]);
-      ac[i] = mma(lds.u.values.dh.columns(16 * i), del_w, ac[i]);
-    }
-  }
-  __syncthreads();
-
-  // ---- the keys and queries, the decays between pairs, sums over the chunk's tokens ----
-  {
-    constexpr int PIECES = kChunk * (DP / 8);
-    const Rows<T> krows = dims.rows(k, b, t0, h), qrows = dims.rows(q, b, t0, h);
+      const f32x4 kf = four(keys_own + 16 * i), af = first ? four(queries_own + 16 * i) : kf;
 #pragma unroll
-    for (int p = threadIdx.x; p < PIECES; p += 256) {
-      const int row = p / (DP / 8), f = 8 * (p % (DP / 8));
-      const Operand<T, 1> x = krows.row(row, f), y = qrows.row(row, f);
-      T *kd = lds.u.rows.keys + row * S::PITCH + f, *qd = lds.u.rows.queries + row * S::PITCH + f;
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<bf16x8*>(kd) = x.p[0];
-        *reinterpret_cast<bf16x8*>(qd) = y.p[0];
-      } else {
-        reinterpret_cast<f32x4*>(kd)[0] = x.lo;
-        reinterpret_cast<f32x4*>(kd)[1] = x.hi;
-        reinterpret_cast<f32x4*>(qd)[0] = y.lo;
-        reinterpret_cast<f32x4*>(qd)[1] = y.hi;
+      for (int r = 0; r < 4; ++r) {
+        dot_a += af[r] * acc[i][r];
+        if constexpr (first) dot_y -= kf[r] * ay[i][r];
       }
     }
-  }
-  const int own = 16 * w + c;
-  const float beta_own = lds.beta[own], eps_own = lds.eps[own], kap_own = lds.kap[own];
-  const DecaySum sum_own = lds.sums[own];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * i + 4 * grp + r;
-      if (i <= w) {  // row j, column i
-        const float e = row <= own ? decay(sum_own, lds.sums[row]) : 0.f;
-        pt[i][r] *= e;
-        bt[i][r] *= row < own ? e : 0.f;
+    dot_a = sum_over_rows(dot_a);
+    if constexpr (first) {
+      dot_y = sum_over_rows(dot_y);
+      dot_v = sum_over_rows(dot_v);
+      if (grp == 0) {
+        lds.dsum[0][own] = dot_a + beta_own * dot_y;
+        if (t0 + own < dims.N) dbeta[((size_t)b * dims.N + t0 + own) * dims.H + h] = from_f32<T>(dot_v + dot_y);
       }
-      if (i >= w) {  // row i, column j
-        const float e = row >= own ? decay(lds.sums[row], sum_own) : 0.f;
-        pr[i][r] *= e;
-        br[i][r] *= row > own ? -lds.beta[row] * e : 0.f;
-      }
+    } else if (grp == 0) {
+      lds.dsum[1][own] = dot_a;
     }
-#pragma unroll
-  for (int i = 0; i < TILES; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      aq[i][r] *= eps_own;
-      ay[i][r] *= eps_own;
-      ac[i][r] *= kap_own;
+    inner = group_sum<64>(inner);
+    end = group_sum<64>(end);
+    if (l == 0) {
+      lds.part[wave][0] = inner;
+      lds.part[wave][1] = end;
     }
-  __syncthreads();
-  float end = 0.f;  // sum_j kap_j k_j.(dH' Delta_j)
-#pragma unroll
-  for (int i = 0; i < TILES; ++i) {
-    const f32x4 kx = four(lds.u.rows.keys + own * S::PITCH + 16 * i + 4 * grp);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) end += kx[r] * ac[i][r];
-  }
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    if (2 * s <= w) {
-      const Operand<T, NT> x = paired<T, NT>(pt[2 * s], pt[2 * s + 1]), y = paired<T, NT>(bt[2 * s], bt[2 * s + 1]);
+    lds_barrier();
+    if constexpr (first) {  // dK = beta Y + C
 #pragma unroll
       for (int i = 0; i < TILES; ++i) {
-        const Operand<T, 1> kc = load_columns_paired(lds.u.rows.keys, S::PITCH, s, 16 * i);
-        aq[i] = mma(kc, x, aq[i]);
-        ay[i] = mma(kc, y, ay[i]);
+        f32x4 y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = -(beta_own * ay[i][r]);
+        lds.u.y[w][i][l] = y;
       }
     }
-    if (2 * s + 1 >= w) {
-      const Operand<T, NT> x = paired<T, NT>(pr[2 * s], pr[2 * s + 1]), y = paired<T, NT>(br[2 * s], br[2 * s + 1]);
+    lds_barrier();
+    const Rows<T> rows = dims.rows(first ? dq : dk, b, t0, h);
 #pragma unroll
-      for (int i = 0; i < TILES; ++i) {
-        ac[i] = mma(load_columns_paired(lds.u.rows.queries, S::PITCH, s, 16 * i), x, ac[i]);
-        ac[i] = mma(load_columns_paired(lds.u.rows.keys, S::PITCH, s, 16 * i), y, ac[i]);
+    for (int i = 0; i < TILES; ++i) {
+      if constexpr (!first) {
+        const f32x4 y = lds.u.y[w][i][l];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][r] += y[r];
       }
+      rows.put_four(own, 16 * i + 4 * grp, acc[i]);
     }
-  }
-
-  // ---- out ----
-  float dot_q = 0.f, dot_y = 0.f, dot_c = 0.f;
-  const Rows<T> dqrows = dims.rows(dq, b, t0, h), dkrows = dims.rows(dk, b, t0, h);
-#pragma unroll
-  for (int i = 0; i < TILES; ++i) {
-    const int f = 16 * i + 4 * grp;
-    const f32x4 kx = four(lds.u.rows.keys + own * S::PITCH + f), qx = four(lds.u.rows.queries + own * S::PITCH + f);
-    f32x4 x;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float y = -ay[i][r];
-      dot_q += qx[r] * aq[i][r];
-      dot_y += kx[r] * y;
-      dot_c += kx[r] * ac[i][r];
-      x[r] = beta_own * y + ac[i][r];
-    }
-    dqrows.put_four(own, f, aq[i]);
-    dkrows.put_four(own, f, x);
-  }
-  dot_q = sum_over_rows(dot_q);
-  dot_y = sum_over_rows(dot_y);
-  dot_c = sum_over_rows(dot_c);
-  dot_v = sum_over_rows(dot_v);
-  if (grp == 0) {
-    lds.dsum[own] = dot_q + beta_own * dot_y - dot_c;
-    if (token < dims.N) dbeta[((size_t)b * dims.N + token) * dims.H + h] = from_f32<T>(dot_v + dot_y);
-  }
-  inner = group_sum<64>(inner);
-  end = group_sum<64>(end);
-  if (l == 0) {
-    lds.part[w][0] = inner;
-    lds.part[w][1] = end;
-  }
-  __syncthreads();
-  if (w == 0) {
-    float x = lds.dsum[l];  // the sum over this token and those behind it
+  };
+  if (wave < 4) body(std::true_type{});
+  else body(std::false_type{});
+  if (wave == 0) {
+    const size_t at = ((size_t)b * dims.N + (t0 + l < dims.N ? t0 + l : t0)) * dims.H + h;
+    const float gl = g[at];
+    float x = lds.dsum[0][l] - lds.dsum[1][l];  // the sum over this token and those behind it
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const float down = __shfl_down(x, off);
       if (l + off < 64) x += down;
     }
-    const float hh = (lds.part[0][0] + lds.part[1][0]) + (lds.part[2][0] + lds.part[3][0]);
-    const float ee = (lds.part[0][1] + lds.part[1][1]) + (lds.part[2][1] + lds.part[3][1]);
-    x += lds.eps[kChunk - 1] * hh + ee;
+    float hh = 0.f, ee = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      hh += lds.part[i][0];
+      ee += lds.part[i][1];
+    }
+    x += lds.coef[2 * kChunk - 1] * hh + ee;
     // what forgets the state has no gradient
-    if (t0 + l < dims.N) dg[((size_t)b * dims.N + t0 + l) * dims.H + h] = (double)gl < kLeastDecay ? 0.f : x;
+    if (t0 + l < dims.N) dg[at] = (double)gl < kLeastDecay ? 0.f : x;
   }
 }
 
@@ -674,7 +710,7 @@ size_t align16(size_t x) { return (x + 15) & ~(size_t)15; }
 
 // coefficients, T and P by columns, then dH' and dR of every chunk and head
 template <typename T> size_t factor_bytes(size_t total) {
-  return align16(total * kCoef * sizeof(float)) + 2 * total * sizeof(T) * Factor<T, Pieces<T>::kN>::kElems;
+  return align16(total * kCoefAll * sizeof(float)) + 2 * total * sizeof(T) * Factor<T, Pieces<T>::kN>::kElems;
 }
 template <typename T> size_t backward_bytes(size_t total, int D) { return factor_bytes<T>(total) + record_bytes(total, D); }
 
@@ -686,7 +722,7 @@ void launch_back(const T* q, const T* k, const T* v, const float* g, const T* d_
   const int slices = (dims.D + 15) / 16;
   hipLaunchKernelGGL((gated_chain_backward_kernel<T, DP>), dim3((unsigned)(B * dims.H * slices)), dim3(512), 0, stream, q, k, d_o,
                      coef, tf, pf, d_state, dv, d_state_in, active, rec_dh, rec_dr, dims, slices);
-  hipLaunchKernelGGL((gated_grad_kernel<T, DP>), dim3((unsigned)(B * dims.H * dims.chunks)), dim3(256), 0, stream, q, k, v, g,
+  hipLaunchKernelGGL((gated_grad_kernel<T, DP>), dim3((unsigned)(B * dims.H * dims.chunks)), dim3(512), 0, stream, q, k, v, g,
                      d_o, coef, rec_h, rec_d, rec_dh, rec_dr, active, dq, dk, dbeta, dg, dims);
 }
 
@@ -712,7 +748,7 @@ int scan_backward(const void* q_, const void* k_, const void* v_, const void* be
   const T *beta = static_cast<const T*>(beta_), *d_o = static_cast<const T*>(d_o_);
   T *dq = static_cast<T*>(dq_), *dk = static_cast<T*>(dk_), *dv = static_cast<T*>(dv_), *dbeta = static_cast<T*>(dbeta_);
   float* coef = static_cast<float*>(ws);
-  T* tf = reinterpret_cast<T*>(static_cast<char*>(ws) + align16(total * kCoef * sizeof(float)));
+  T* tf = reinterpret_cast<T*>(static_cast<char*>(ws) + align16(total * kCoefAll * sizeof(float)));
   T* pf = tf + total * Factor<T, Pieces<T>::kN>::kElems;
   float* rec_dh = reinterpret_cast<float*>(static_cast<char*>(ws) + factor_bytes<T>(total));
   float* rec_dr = rec_dh + total * D * D;

@@ -89,12 +89,15 @@ __global__ __launch_bounds__(64 * kPrepWaves, 2) void gated_prep_kernel(
     }
     const double all = __shfl(sum, 63);
     const float be = ok ? bl : 0.f;
-    s.sums[l] = decay_sum(sum);
+    const DecaySum parts = decay_sum(sum);
+    s.sums[l] = parts;
     s.beta[l] = -be;
-    float* co = coef + (size_t)id * kCoef;
+    float* co = coef + (size_t)id * kCoefAll;
     co[l] = be;
     co[kChunk + l] = expf((float)sum);
     co[2 * kChunk + l] = expf((float)(all - sum));
+    co[kCoef + l] = parts.hi;
+    co[kCoef + kChunk + l] = parts.lo;
   }
 
   // K K^T and Q K^T of the lower tiles, in both accumulator layouts where both are needed: `mult` multiplies (for
@@ -408,13 +411,13 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
     const T *kp = k + dims.at(b, 0, h), *vp = v + dims.at(b, 0, h), *qp = q + dims.at(b, 0, h);
     T* op = o + dims.at(b, 0, h);
     const T* pp = pf + chunk0 * Factor<T, NO>::kElems + row_step(w, 0) * FO::kStep;
-    const float* cp = coef + chunk0 * kCoef;
+    const float* cp = coef + chunk0 * kCoefAll;
     auto within = [&](int ci) { return ci < nc ? ci : nc - 1; };
     auto stage = [&](int ahead, int slot) {
       const int ci = within(ahead);
       typename S::Stage& to = lds.ring[slot];
       const Rows<T> krows = dims.rows_at(kp + ci * stride, ci), vrows = dims.rows_at(vp + ci * stride, ci);
-      const float* co = cp + (size_t)ci * kCoef;
+      const float* co = cp + (size_t)ci * kCoefAll;
 #pragma unroll
       for (int j = 0; j < Keys::kInstr / 4; ++j) Keys::stage(to.keys, krows, 4 * j + w, 0);
       if constexpr (Slice::kInstr == 4) {
@@ -433,7 +436,7 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
       const T* pb = pp + (size_t)ci * Factor<T, NO>::kElems;
       in.wf[0] = FO::get(pb, 0);
       in.wf[1] = FO::get(pb, w >= 2 ? 1 : 0);
-      in.eps = cp[(size_t)ci * kCoef + kChunk + 16 * w + c];
+      in.eps = cp[(size_t)ci * kCoefAll + kChunk + 16 * w + c];
       in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, ci * kChunk), 16 * w + c, 0, 0);
     };
     int free = LEAD == 0 ? 0 : RING - 1;  // the slot of the chunk LEAD ahead
@@ -510,7 +513,7 @@ size_t align16(size_t x) { return (x + 15) & ~(size_t)15; }
 
 // the forward's workspace: coefficients, T and P of every chunk and head
 template <typename T> size_t forward_bytes(size_t total) {
-  return align16(total * kCoef * sizeof(float)) + total * sizeof(T) * (Factor<T, Pieces<T>::kN>::kElems + Factor<T, OutPieces<T>::kN>::kElems);
+  return align16(total * kCoefAll * sizeof(float)) + total * sizeof(T) * (Factor<T, Pieces<T>::kN>::kElems + Factor<T, OutPieces<T>::kN>::kElems);
 }
 
 template <typename T>
@@ -531,7 +534,7 @@ int scan(const void* q_, const void* k_, const void* v_, const void* beta_, cons
   const T* beta = static_cast<const T*>(beta_);
   T* o = static_cast<T*>(o_);
   float* coef = static_cast<float*>(ws);
-  T* tf = reinterpret_cast<T*>(static_cast<char*>(ws) + align16(total * kCoef * sizeof(float)));
+  T* tf = reinterpret_cast<T*>(static_cast<char*>(ws) + align16(total * kCoefAll * sizeof(float)));
   T* pf = tf + total * Factor<T, Pieces<T>::kN>::kElems;
   const Dims<T> dims{N, H, D, chunks_of(N)};
   if (const int st = launch_prep<T>(q, k, beta, g, coef, tf, pf, B, N, H, D, false, stream); st != OK) return st;
