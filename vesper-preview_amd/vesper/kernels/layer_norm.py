@@ -26,7 +26,7 @@ def _forward(x: Tensor, gain: Tensor, bias: Tensor | None, residual: Tensor | No
              stats: Tensor | None) -> tuple[Tensor, Tensor]:
     """``(y, sum)`` of contiguous tensors; without a residual the sum is ``x`` itself."""
     d = x.shape[-1]
-    y = torch.empty(x.shape, dtype=dtype, device=x.device)
+    y = torch.empty_like(x) if dtype is x.dtype else torch.empty_like(x, dtype=dtype)
     total = x if residual is None else torch.empty_like(x)
     with _lib.on_device(x.device):
         _lib.call("vsp_layer_norm", x.data_ptr(), _lib.ptr(residual), gain.data_ptr(), _lib.ptr(bias),
@@ -100,14 +100,15 @@ def layer_norm(x: Tensor, gain: Tensor, bias: Tensor | None = None, *, residual:
     """
     out = x.dtype if dtype is None else dtype
     d = _check(x, gain, bias, residual, eps, out)
-    inputs = (x, gain, bias, residual)
-    if x.numel() == 0 or not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)):
+    grad = torch.is_grad_enabled() and (x.requires_grad or gain.requires_grad or (bias is not None and bias.requires_grad)
+                                        or (residual is not None and residual.requires_grad))
+    if x.numel() == 0 or not grad:
         if x.numel() == 0:  # no rows: empty results that keep the graph
             total = x if residual is None else x + residual.to(x.dtype)
             y = (total * gain.sum()).to(out)
             return y if residual is None else (y, total)
-        x, gain, bias, residual = (None if t is None else t.contiguous() for t in inputs)
-        y, total = _forward(x, gain, bias, residual, eps, out, None)
+        y, total = _forward(x.contiguous(), gain.contiguous(), None if bias is None else bias.contiguous(),
+                            None if residual is None else residual.contiguous(), eps, out, None)
         return y if residual is None else (y, total)
     return _LayerNorm.apply(x, gain, bias, residual, eps, out)
 
