@@ -170,7 +170,7 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_backward_kern
   for (long row = (long)blockIdx.x * ROWS + sub; row < rows; row += (long)gridDim.x * ROWS) {
     const size_t base = (size_t)row * d;
     const float mu = stats[2 * (size_t)row], rstd = stats[2 * (size_t)row + 1];
-    float xh[SEG][V], w[SEG][V];
+    float xh[SEG][V], w[SEG][V], add[SEG][V];
     float sums[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < SEG; ++j) {
@@ -184,6 +184,7 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_backward_kern
         for (int e = 0; e < V; ++e) xh[j][e] += r[e];
       }
       load_piece<V>(dy + base + (ok ? f : 0), w[j]);
+      if (dsum != nullptr) load_piece<V>(dsum + base + (ok ? f : 0), add[j]);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         xh[j][e] = ok ? (xh[j][e] - mu) * rstd : 0.f;
@@ -202,10 +203,9 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_backward_kern
     for (int j = 0; j < SEG; ++j) {
       const int f = V * (t + LANES * j);
       if (f >= d) continue;
-      float o[V], add[V];
-      if (dsum != nullptr) load_piece<V>(dsum + base + f, add);
+      float o[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = rstd * (w[j][e] - m0 - xh[j][e] * m1) + (dsum != nullptr ? add[e] : 0.f);
+      for (int e = 0; e < V; ++e) o[e] = rstd * (w[j][e] - m0 - xh[j][e] * m1) + (dsum != nullptr ? add[j][e] : 0.f);
       store_piece<V>(dx + base + f, o);
       if (dres != nullptr) store_piece<V>(dres + base + f, o);
     }
@@ -237,24 +237,30 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_backward_kern
   }
 }
 
-// dgain and dbias: the column sums of the partial rows. A workgroup takes 64 columns (of the 2 d); its four waves
-// take every fourth partial row each, then the four sums are added in order.
-__global__ __launch_bounds__(256) void layer_norm_columns_kernel(const float* __restrict__ partial, float* __restrict__ dgain,
-                                                                float* __restrict__ dbias, int parts, int d) {
-  __shared__ float red[4][64];
+// dgain and dbias: the column sums of the partial rows. A workgroup takes 64 columns (of the 2 d); its sixteen waves take
+// every sixteenth partial row each, eight of them in flight, then the sixteen sums are added in order.
+constexpr int kColumnWaves = 16;
+__global__ __launch_bounds__(64 * kColumnWaves) void layer_norm_columns_kernel(const float* __restrict__ partial,
+                                                                              float* __restrict__ dgain,
+                                                                              float* __restrict__ dbias, int parts, int d) {
+  __shared__ float red[kColumnWaves][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
-  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  float a[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = 0.f;
   if (col < 2 * d) {
     int p = w;
-    for (; p + 12 < parts; p += 16)
+    for (; p + 7 * kColumnWaves < parts; p += 8 * kColumnWaves)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] += partial[(size_t)(p + 4 * i) * 2 * d + col];
-    for (int i = 0; p < parts; p += 4, ++i) a[i & 3] += partial[(size_t)p * 2 * d + col];
+      for (int i = 0; i < 8; ++i) a[i] += partial[(size_t)(p + i * kColumnWaves) * 2 * d + col];
+    for (; p < parts; p += kColumnWaves) a[0] += partial[(size_t)p * 2 * d + col];
   }
-  red[w][lane] = (a[0] + a[1]) + (a[2] + a[3]);
+  red[w][lane] = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
   __syncthreads();
   if (w == 0 && col < 2 * d) {
-    const float x = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+    float x = red[0][lane];
+#pragma unroll
+    for (int i = 1; i < kColumnWaves; ++i) x += red[i][lane];
     if (col < d) dgain[col] = x;
     else if (dbias != nullptr) dbias[col - d] = x;
   }
@@ -263,16 +269,16 @@ __global__ __launch_bounds__(256) void layer_norm_columns_kernel(const float* __
 // The widest row of a shape: WAVES * 64 lanes, SEG pieces of V.
 #define VSP_NORM_SHAPES(GO)                     \
   if (vec) {                                    \
-    if (d <= 512) GO(1, 8, 1);                  \
-    else if (d <= 1024) GO(1, 8, 2);            \
-    else if (d <= 2048) GO(4, 8, 1);            \
-    else if (d <= 4096) GO(4, 8, 2);            \
-    else if (d <= 8192) GO(4, 8, 4);            \
-    else GO(16, 8, 2);                          \
+    if (d <= 512) GO(1, 8, 1)                   \
+    else if (d <= 1024) GO(1, 8, 2)             \
+    else if (d <= 2048) GO(4, 8, 1)             \
+    else if (d <= 4096) GO(4, 8, 2)             \
+    else if (d <= 8192) GO(4, 8, 4)             \
+    else GO(16, 8, 2)                           \
   } else {                                      \
-    if (d <= 256) GO(1, 1, 4);                  \
-    else if (d <= 2048) GO(4, 1, 8);            \
-    else GO(16, 1, 16);                         \
+    if (d <= 256) GO(1, 1, 4)                   \
+    else if (d <= 2048) GO(4, 1, 8)             \
+    else GO(16, 1, 16)                          \
   }
 
 bool aligned16(std::initializer_list<const void*> ps) {
@@ -298,19 +304,26 @@ int norm_forward(const void* x_, const void* res_, const float* gain, const floa
 #define VSP_GO(W, V, S)                                                                                              \
   hipLaunchKernelGGL((layer_norm_kernel<TX, TR, TY, W, V, S>),                                                       \
                      dim3((unsigned)std::min<long>(((long)rows + NormShape<W>::ROWS - 1) / NormShape<W>::ROWS, 1 << 20)), \
-                     dim3(NormShape<W>::NT), 0, stream, x, res, gain, bias, sum, y, stats, rows, d, eps)
+                     dim3(NormShape<W>::NT), 0, stream, x, res, gain, bias, sum, y, stats, rows, d, eps);
   VSP_NORM_SHAPES(VSP_GO)
 #undef VSP_GO
   return check_launch(who);
 }
 
-// Workgroups of the backward, and so partial rows: enough to fill the card, each with several rows where there are
-// many.
-constexpr int kNormParts = 1024;
+// Workgroups of the backward, and so partial rows, at most; as many as the card holds at once are launched, each with
+// several rows where there are many: with 1024 of a kernel of which it holds 768, the last quarter ran alone (16384 x
+// 4096 in bf16: 195 us against 154).
+constexpr int kNormParts = 1024, kCus = 256;
 int norm_parts(int rows, int d) {
   const int at_once = d <= 1024 ? 4 : 1;
   const int groups = rows / at_once + (rows % at_once != 0);
   return groups < kNormParts ? groups : kNormParts;
+}
+
+int held_at_once(const void* kernel, int threads) {
+  int per_cu = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, 0) != hipSuccess || per_cu < 1) per_cu = 1;
+  return per_cu * kCus;
 }
 
 template <typename TX, typename TR, typename TY>
@@ -322,13 +335,17 @@ int norm_backward(const void* x_, const void* res_, const float* gain, const flo
   TX* dx = static_cast<TX*>(dx_);
   TR* dres = static_cast<TR*>(dres_);
   const bool vec = d % 8 == 0 && aligned16({x, res, gain, dy, dsum, dx, dres});
-  const int parts = norm_parts(rows, d);
+  int parts = norm_parts(rows, d);
 #define VSP_GO(W, V, S)                                                                                              \
-  hipLaunchKernelGGL((layer_norm_backward_kernel<TX, TR, TY, W, V, S>), dim3((unsigned)parts), dim3(NormShape<W>::NT), 0, \
-                     stream, x, res, gain, stats, dy, dsum, dx, dres, ws, rows, d)
+  {                                                                                                                  \
+    static const int held = held_at_once(reinterpret_cast<const void*>(layer_norm_backward_kernel<TX, TR, TY, W, V, S>), NormShape<W>::NT); \
+    parts = std::min(parts, held);                                                                                   \
+    hipLaunchKernelGGL((layer_norm_backward_kernel<TX, TR, TY, W, V, S>), dim3((unsigned)parts), dim3(NormShape<W>::NT), 0, \
+                       stream, x, res, gain, stats, dy, dsum, dx, dres, ws, rows, d);                                \
+  }
   VSP_NORM_SHAPES(VSP_GO)
 #undef VSP_GO
-  hipLaunchKernelGGL(layer_norm_columns_kernel, dim3((unsigned)((2 * d + 63) / 64)), dim3(256), 0, stream, ws, dgain, dbias, parts, d);
+  hipLaunchKernelGGL(layer_norm_columns_kernel, dim3((unsigned)((2 * d + 63) / 64)), dim3(64 * kColumnWaves), 0, stream, ws, dgain, dbias, parts, d);
   return check_launch(who);
 }
 
