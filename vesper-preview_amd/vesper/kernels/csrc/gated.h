@@ -155,9 +155,19 @@ template <typename T> struct Rows {
       return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, at(row, f), 0, 0));
     }
   }
-  __device__ __forceinline__ void put_one(int row, int f, T x) const {
-    if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, x), r, at(row, f), 0, 0);
-    else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), r, at(row, f), 0, 0);
+  // eight elements from feature f (a multiple of 8)
+  __device__ __forceinline__ void put_eight(int row, int f, const float (&x)[8]) const {
+    const unsigned o = at(row, f);
+    if constexpr (sizeof(T) == 2) {
+      bf16x8 y;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = (__bf16)x[i];
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, y), r, o, 0, 0);
+    } else {
+      const f32x4 lo = {x[0], x[1], x[2], x[3]}, hi = {x[4], x[5], x[6], x[7]};
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, lo), r, o, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, hi), r, o + 16, 0, 0);
+    }
   }
   // four elements from feature f (a multiple of 4)
   __device__ __forceinline__ void put_four(int row, int f, f32x4 x) const {

@@ -14,7 +14,7 @@
 //  * gated_prep_kernel (gated_scan.hip) forms T and P again, as operands by columns.
 //  * gated_chain_backward_kernel walks the chunks from the last to the first like the forward's chain, a workgroup a
 //    head and 16 value columns: four waves carry dH through three dependent products, four more bring everything into
-//    LDS ahead and form P^T dO and Q^T (eps dO) of the next chunk. It writes dV and keeps dH' and dR of each chunk.
+//    LDS ahead and form P^T dO and Q^T (eps dO) of the next chunk. It keeps dH' and dR of each chunk.
 //  * gated_grad_kernel: a workgroup a chunk and head, all at once, for the rest: wave w holds dQ, Y and C of the
 //    16 tokens w, sums over the value columns 32 at a time from H, dH', Delta and dR in pieces in LDS, then over
 //    the chunk's tokens with accumulator tiles as operands.
@@ -37,20 +37,17 @@ template <typename T, int DP> struct BackShape {
   static constexpr int NT = Pieces<T>::kN;
   // float32 queries are read from memory by columns: the LDS has no room for them beside the rest
   static constexpr bool kStageQ = sizeof(T) == 2;
-  // chunks of keys and of queries in LDS at once: heads of width 256 have room for one of each, and wait for each
-  static constexpr int RING = DP > 128 ? 1 : 2;
   using F = Frags<T, NT>;
   using Keys = Tile<T, DP>;
   using Slice = Tile<T, 16>;
-  struct Stage {  // what comes from memory for the chain, besides T
-    T keys[Keys::kElems];
-    float coef[kCoefLds];
-  };
+  // How many chunks ahead of the one in hand the loads of keys into LDS go; heads of width 256 have room for the chunk in
+  // hand only, and wait for each.
+  static constexpr int LEAD = DP > 128 ? 0 : 2, RING = LEAD + 1, QRING = LEAD == 0 ? 1 : 2;
   struct Lds {
-    Stage ring[RING];
-    T queries[RING][kStageQ ? Keys::kElems : 8];
-    T d_o[Slice::kElems];        // of one chunk, as T: read into registers in a chunk's first span
-    T tf[kTriSteps * F::kStep];
+    T keys[RING][Keys::kElems];
+    float coef[3][kCoefLds];
+    T queries[QRING][kStageQ ? Keys::kElems : 8];
+    T d_o[2][Slice::kElems];
     T state[KS * F::kStep];      // dH
     T ddelta[2 * F::kStep];
     T dread[2 * F::kStep];       // -beta eps dR
@@ -58,25 +55,29 @@ template <typename T, int DP> struct BackShape {
     float qdo[TILES * 256];      // Q^T (eps dO)
   };
   static_assert(sizeof(Lds) <= 160 * 1024, "more than a CU's LDS");
+  // direct loads of one wave for a chunk: queries, keys, a slice of dO and the coefficients (bf16: two waves each)
+  static constexpr int kLoads = (kStageQ ? 2 : 1) * Keys::kInstr / 4 + (sizeof(T) == 2 ? 1 : 2);
 };
+
+// What a chain wave reads of a chunk from memory: its tokens' columns of T.
+template <typename T> struct BackChainIn { Operand<T, Pieces<T>::kN> t[2]; };
 
 template <typename T> struct BackIn {  // what the other waves keep of a chunk in registers
   Operand<T, Pieces<T>::kN> pf[2];
-  f32x4 eps[4];
   uint8_t on;  // of token l
 };
 
 template <typename T, int DP>
 __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ d_o, const float* __restrict__ coef,
-    const T* __restrict__ tf, const T* __restrict__ pf, const float* __restrict__ d_state, T* __restrict__ dv,
+    const T* __restrict__ tf, const T* __restrict__ pf, const float* __restrict__ d_state,
     float* __restrict__ d_state_in, const uint8_t* __restrict__ active, float* __restrict__ rec_dh,
     float* __restrict__ rec_dr, Dims<T> dims, int slices) {
   using S = BackShape<T, DP>;
   using F = typename S::F;
   using Keys = typename S::Keys;
   using Slice = typename S::Slice;
-  constexpr int KS = S::KS, FT = S::FT, TILES = S::TILES, NT = S::NT, RING = S::RING;
+  constexpr int KS = S::KS, FT = S::FT, TILES = S::TILES, NT = S::NT, LEAD = S::LEAD, RING = S::RING, QRING = S::QRING;
   __shared__ __attribute__((aligned(16))) typename S::Lds lds;
 
   const int id = xcd_logical_block(blockIdx.x, gridDim.x);
@@ -87,7 +88,7 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
   const size_t chunk0 = (size_t)bh * nc;
 
   // features past D and rows past the end are not brought: zeros, and what another chunk left there, times zeros
-  for (int i = threadIdx.x; i < (int)((sizeof(lds.ring) + sizeof(lds.queries) + sizeof(lds.d_o)) / 16); i += 512)
+  for (int i = threadIdx.x; i < (int)((sizeof(lds.keys) + sizeof(lds.coef) + sizeof(lds.queries) + sizeof(lds.d_o)) / 16); i += 512)
     reinterpret_cast<f32x4*>(&lds)[i] = zero4();
   lds_barrier();
 
@@ -95,6 +96,7 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
     // ---- the chain: wave w has the 16 tokens w of dDelta and dR, and of dH's feature tiles each fourth ----
     __builtin_amdgcn_s_setprio(3);
     const int vcol = 16 * sl + c, own = 16 * w + 4 * grp;
+    const T* tp = tf + chunk0 * Factor<T, NT>::kElems;
     f32x4 dh[FT];
 #pragma unroll
     for (int i = 0; i < FT; ++i) {
@@ -109,17 +111,41 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
     lds_barrier();
     lds_barrier();
     lds_barrier();
-    for (int it = 0; it < nc; ++it) {
+    // BOTH: the wave's columns of T have two steps. The code twice, so that no load is conditional
+    auto run = [&](auto both) {
+    constexpr bool BOTH = decltype(both)::value;
+    auto load = [&](int it, BackChainIn<T>& to) {
+      const T* tc = tp + (size_t)(it < nc ? nc - 1 - it : 0) * Factor<T, NT>::kElems;
+      if constexpr (BOTH) to.t[0] = F::get(tc, col_step(w, 0));
+      to.t[1] = F::get(tc, col_step(w, 1));
+    };
+    BackChainIn<T> ta, tb;
+    load(0, ta);
+    int slot = 0, cslot = 0;
+    auto step = [&](int it, const BackChainIn<T>& tin, BackChainIn<T>& next) {
       const int ci = nc - 1 - it;
-      const typename S::Stage& in = lds.ring[RING == 1 ? 0 : it & 1];
-      if constexpr (RING == 1) lds_barrier();
-      // dDelta = P^T dO + kap (K dH'); T's columns on the way
+      const T* keys = lds.keys[slot];
+      const float* co = lds.coef[cslot];
+      slot = slot + 1 < RING ? slot + 1 : 0;
+      cslot = cslot + 1 < 3 ? cslot + 1 : 0;
+      if constexpr (LEAD == 0) lds_barrier();
+      // dDelta = P^T dO + kap (K dH')
       f32x4 x = zero4();
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x = mma(Keys::row(in.keys, 16 * w + c, 32 * s + 8 * grp), F::get(lds.state, s), x);
-      const f32x4 kap = *reinterpret_cast<const f32x4*>(in.coef + 2 * kChunk + own);
+      for (int s0 = 0; s0 < KS; s0 += 2) {
+        Operand<T, 1> kr[2];
+        Operand<T, NT> st[2];
+#pragma unroll
+        for (int s = 0; s < 2 && s0 + s < KS; ++s) {
+          kr[s] = Keys::row(keys, 16 * w + c, 32 * (s0 + s) + 8 * grp);
+          st[s] = F::get(lds.state, s0 + s);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // reads together, not one by one before its product
+#pragma unroll
+        for (int s = 0; s < 2 && s0 + s < KS; ++s) x = mma(kr[s], st[s], x);
+      }
+      const f32x4 kap = *reinterpret_cast<const f32x4*>(co + 2 * kChunk + own);
       const f32x4 z = *reinterpret_cast<const f32x4*>(lds.z + 256 * w + 4 * lane);
-      const Operand<T, NT> t0 = F::get(lds.tf, col_step(w, 0)), t1 = F::get(lds.tf, col_step(w, w < 2 ? 1 : 0));
       const Record rh = record(rec_dh, chunk0 + ci, D, D);
 #pragma unroll
       for (int i = 0; i < FT; ++i) rh.put(vcol, 16 * (w + 4 * i) + 4 * grp, dh[i]);
@@ -127,18 +153,23 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
       for (int r = 0; r < 4; ++r) x[r] = kap[r] * x[r] + z[r];
       F::template put_tile<false>(lds.ddelta, w, x);
       lds_barrier();
-      // dR = T^T dDelta; K^T and Q^T (eps dO) on the way
-      f32x4 dr = mma(t1, F::get(lds.ddelta, 1), zero4());
-      if (w < 2) dr = mma(t0, F::get(lds.ddelta, 0), dr);
-      const f32x4 beta = *reinterpret_cast<const f32x4*>(in.coef + own);
-      const f32x4 eps = *reinterpret_cast<const f32x4*>(in.coef + kChunk + own);
-      const float gam = in.coef[2 * kChunk - 1];
+      // dR = T^T dDelta; the next chunk's T, K^T and Q^T (eps dO) on the way
+      Operand<T, NT> d0;
+      if constexpr (BOTH) d0 = F::get(lds.ddelta, 0);
+      const Operand<T, NT> d1 = F::get(lds.ddelta, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      load(it + 1, next);
+      f32x4 dr = mma(tin.t[1], d1, zero4());
+      if constexpr (BOTH) dr = mma(tin.t[0], d0, dr);
+      const f32x4 beta = *reinterpret_cast<const f32x4*>(co + own);
+      const f32x4 eps = *reinterpret_cast<const f32x4*>(co + kChunk + own);
+      const float gam = co[2 * kChunk - 1];
       constexpr int AHEAD = FT < 2 ? FT : 2;  // feature tiles whose K^T waits in registers
       Operand<T, 1> kc[AHEAD][2];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) kc[i][s] = Keys::columns(in.keys, s, 16 * (TILES < 4 ? w & 1 : w + 4 * i));
+        for (int s = 0; s < 2; ++s) kc[i][s] = Keys::columns(keys, s, 16 * (TILES < 4 ? w & 1 : w + 4 * i));
 #pragma unroll
       for (int i = 0; i < FT; ++i)
         if (w + 4 * i < TILES) {
@@ -146,27 +177,22 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
 #pragma unroll
           for (int r = 0; r < 4; ++r) dh[i][r] = gam * dh[i][r] + add[r];
         }
-      f32x4 y, vx;
+      f32x4 y;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        vx[r] = beta[r] * dr[r];
-        y[r] = -(vx[r] * eps[r]);
-      }
+      for (int r = 0; r < 4; ++r) y[r] = -(beta[r] * dr[r] * eps[r]);
       F::template put_tile<false>(lds.dread, w, y);
       record(rec_dr, chunk0 + ci, kChunk, D).put(vcol, own, dr);
-      const Rows<T> dvrows = dims.rows(dv, b, ci * kChunk, h);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) dvrows.put_one(own + r, vcol, from_f32<T>(vx[r]));
       lds_barrier();
       // dH = gam dH' + Q^T (eps dO) - K^T (beta eps dR)
       const Operand<T, NT> y0 = F::get(lds.dread, 0), y1 = F::get(lds.dread, 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < FT; ++i) {
         const int ft = w + 4 * i;
         if (ft < TILES) {
           if (i >= AHEAD) {
-            dh[i] = mma(Keys::columns(in.keys, 0, 16 * ft), y0, dh[i]);
-            dh[i] = mma(Keys::columns(in.keys, 1, 16 * ft), y1, dh[i]);
+            dh[i] = mma(Keys::columns(keys, 0, 16 * ft), y0, dh[i]);
+            dh[i] = mma(Keys::columns(keys, 1, 16 * ft), y1, dh[i]);
           } else {
             dh[i] = mma(kc[i < AHEAD ? i : 0][0], y0, dh[i]);
             dh[i] = mma(kc[i < AHEAD ? i : 0][1], y1, dh[i]);
@@ -175,7 +201,14 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
         }
       }
       lds_barrier();
+    };
+    for (int it = 0; it < nc; it += 2) {
+      step(it, ta, tb);
+      if (it + 1 < nc) step(it + 1, tb, ta);
     }
+    };
+    if (w < 2) run(std::true_type{});
+    else run(std::false_type{});
     float* so = d_state_in + (size_t)bh * D * D;
 #pragma unroll
     for (int i = 0; i < FT; ++i)
@@ -186,21 +219,21 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
       }
   } else {
     // ---- memory into LDS ahead, and of the next chunk P^T dO (the 16 tokens w) and Q^T (eps dO) (each fourth feature tile).
-    //      In a chunk's three spans: dO of the next chunk into registers; P^T dO; Q^T (eps dO). Chunk number it counts
-    //      from the last one back; past the first it stays, so that nothing is conditional ----
+    //      Chunk number it counts from the last one back; past the first it stays, so that nothing is conditional. In
+    //      chunk it's three spans: dO of chunk it + 1 into registers, loads of the queries of it + 2 and the keys of
+    //      it + LEAD; P^T dO, loads of the coefficients of it + 2 and dO of it + 3; Q^T (eps dO), loads of this wave's
+    //      columns of P of it + 2. Every wave issues the same number of direct loads in the same order, so that the wait
+    //      for the last chunk's leaves this one's in flight; the loads are spread, for a CU takes 64 bytes a cycle ----
     const size_t stride = (size_t)kChunk * dims.H * D;
     const T *kp = k + dims.at(b, 0, h), *qp = q + dims.at(b, 0, h), *gp = d_o + dims.at(b, 0, h);
-    const T* tp = tf + chunk0 * Factor<T, NT>::kElems;
     const T* pp = pf + chunk0 * Factor<T, NT>::kElems + col_step(w, 0) * F::kStep;
     const float* cp = coef + chunk0 * kCoefAll;
     auto chunk_of = [&](int it) { return it < nc ? nc - 1 - it : 0; };
-    auto stage = [&](int it) {
+    auto stage = [&](int it, int slot) {
       const int ci = chunk_of(it);
-      typename S::Stage& to = lds.ring[RING == 1 ? 0 : it & 1];
       const Rows<T> rows = dims.rows_at(kp + ci * stride, ci);
 #pragma unroll
-      for (int j = 0; j < Keys::kInstr / 4; ++j) Keys::stage(to.keys, rows, 4 * j + w, 0);
-      if (w == 3) stage_coef(to.coef, cp + (size_t)ci * kCoefAll);
+      for (int j = 0; j < Keys::kInstr / 4; ++j) Keys::stage(lds.keys[slot], rows, 4 * j + w, 0);
     };
     // `slot` as a constant: the reads of one slot then do not wait for the loads into the other
     auto stage_q = [&](int it, auto slot) {
@@ -208,50 +241,53 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
         const int ci = chunk_of(it);
         const Rows<T> rows = dims.rows_at(qp + ci * stride, ci);
 #pragma unroll
-        for (int j = 0; j < Keys::kInstr / 4; ++j) Keys::stage(lds.queries[decltype(slot)::value], rows, 4 * j + w, 0);
+        for (int j = 0; j < Keys::kInstr / 4; ++j) Keys::stage(lds.queries[decltype(slot)::value % QRING], rows, 4 * j + w, 0);
       }
     };
-    auto stage_t = [&](int it) {
+    auto stage_do = [&](int it, auto slot, int coef_it, int coef_slot) {  // and the coefficients of chunk coef_it
       const int ci = chunk_of(it);
-      constexpr int TI = kTriSteps * F::kStepInstr;
-#pragma unroll
-      for (int j = 0; j < (TI + 3) / 4; ++j)
-        if (4 * j + w < TI) F::stage(lds.tf, tp + (size_t)ci * Factor<T, NT>::kElems, kTriSteps, 4 * j + w);
+      const Rows<T> rows = dims.rows_at(gp + ci * stride, ci);
+      T* to = lds.d_o[decltype(slot)::value];
+      const float* co = cp + (size_t)chunk_of(coef_it) * kCoefAll;
+      if constexpr (Slice::kInstr == 4) {
+        Slice::stage(to, rows, w, 16 * sl);
+        stage_coef(lds.coef[coef_slot], co);
+      } else {
+        if (w < 2) Slice::stage(to, rows, w, 16 * sl);
+        else stage_coef(lds.coef[coef_slot], co);
+      }
     };
-    auto stage_do = [&](int it) {
-      const int ci = chunk_of(it);
-      if (w < Slice::kInstr) Slice::stage(lds.d_o, dims.rows_at(gp + ci * stride, ci), w, 16 * sl);
-    };
+    auto run = [&](auto both) {  // as in the chain
+    constexpr bool BOTH = decltype(both)::value;
     auto load = [&](int it, BackIn<T>& in) {
       const int ci = chunk_of(it);
       const T* pb = pp + (size_t)ci * Factor<T, NT>::kElems;
-      in.pf[0] = F::get(pb, 0);
-      in.pf[1] = F::get(pb, w < 2 ? 1 : 0);
-      const float* co = cp + (size_t)ci * kCoefAll + kChunk + 4 * grp;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) in.eps[i] = *reinterpret_cast<const f32x4*>(co + 16 * i);
+      if constexpr (BOTH) in.pf[0] = F::get(pb, 0);
+      in.pf[1] = F::get(pb, BOTH ? 1 : 0);
       in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, ci * kChunk), lane, 0, 0);
     };
     f32x4 x[4];  // dO as accumulator tiles (rows tokens), zero where inactive
-    auto read_do = [&](const BackIn<T>& in) {
+    auto read_do = [&](const BackIn<T>& in, auto slot) {
       const uint64_t on = active == nullptr ? ~0ull : __builtin_amdgcn_ballot_w64(in.on != 0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        x[j] = Slice::four(lds.d_o, j, 0);
+        x[j] = Slice::four(lds.d_o[decltype(slot)::value], j, 0);
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[j][r] = (on >> (16 * j + 4 * grp + r)) & 1 ? x[j][r] : 0.f;
       }
     };
     auto form_z = [&](const BackIn<T>& in) {
       f32x4 z = mma(in.pf[1], paired<T, 1>(x[2], x[3]), zero4());
-      if (w < 2) z = mma(in.pf[0], paired<T, 1>(x[0], x[1]), z);
+      if constexpr (BOTH) z = mma(in.pf[0], paired<T, 1>(x[0], x[1]), z);
       *reinterpret_cast<f32x4*>(lds.z + 256 * w + 4 * lane) = z;
     };
-    auto form_qdo = [&](int it, auto slot, const BackIn<T>& in) {
+    auto form_qdo = [&](int it, auto slot, const float* co) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 eps = *reinterpret_cast<const f32x4*>(co + kChunk + 16 * j + 4 * grp);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[j][r] *= in.eps[j][r];
+        for (int r = 0; r < 4; ++r) x[j][r] *= eps[r];
+      }
       const Operand<T, NT> e0 = paired<T, NT>(x[0], x[1]), e1 = paired<T, NT>(x[2], x[3]);
 #pragma unroll
       for (int i = 0; i < FT; ++i) {
@@ -259,8 +295,8 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
         if (ft < TILES) {
           f32x4 y;
           if constexpr (S::kStageQ) {
-            y = mma(Keys::columns(lds.queries[decltype(slot)::value], 0, 16 * ft), e0, zero4());
-            y = mma(Keys::columns(lds.queries[decltype(slot)::value], 1, 16 * ft), e1, y);
+            y = mma(Keys::columns(lds.queries[decltype(slot)::value % QRING], 0, 16 * ft), e0, zero4());
+            y = mma(Keys::columns(lds.queries[decltype(slot)::value % QRING], 1, 16 * ft), e1, y);
           } else {
             const int ci = chunk_of(it);
             const Rows<T> rows = dims.rows_at(qp + ci * stride, ci);
@@ -280,51 +316,62 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
       }
     };
     constexpr std::integral_constant<int, 0> even{};
-    constexpr std::integral_constant<int, RING - 1> odd{};
+    constexpr std::integral_constant<int, 1> odd{};
     BackIn<T> in;
-    auto step = [&](int it, auto slot, auto other) {
-      if constexpr (RING == 1) {
-        stage(it);
-        stage_q(it + 1, slot);
+    int free = LEAD, c1 = 1, c2 = 2;  // the slots of the keys of chunk it + LEAD, of the coefficients of it + 1 and it + 2
+    auto step = [&](int it, auto mine, auto other) {  // `mine` is it's parity
+      if constexpr (LEAD == 0) {
+        stage(it, 0);
+        stage_q(it + 1, other);
+        stage_do(it + 2, mine, it + 2, c2);
         direct_loads_done();
         lds_barrier();
-        read_do(in);
-      } else {
-        read_do(in);
-        stage(it + 1);
-        stage_q(it + 2, slot);
+      }
+      read_do(in, other);
+      if constexpr (LEAD > 0) {
+        stage_q(it + 2, mine);
+        stage(it + LEAD, free);
       }
       lds_barrier();
+      if constexpr (LEAD > 0) stage_do(it + 3, other, it + 2, c2);
       form_z(in);
-      stage_t(it + 1);
-      stage_do(it + 2);
+      direct_loads_done<LEAD == 0 ? 0 : S::kLoads>();
       lds_barrier();
-      form_qdo(it + 1, other, in);
-      direct_loads_done();
       load(it + 2, in);
+      form_qdo(it + 1, other, lds.coef[c1]);
+      free = free + 1 < RING ? free + 1 : 0;
+      c1 = c2;
+      c2 = c2 + 1 < 3 ? c2 + 1 : 0;
       lds_barrier();
     };
-    if constexpr (RING > 1) stage(0);
-    stage_t(0);
-    stage_do(0);
+#pragma unroll
+    for (int it = 0; it < LEAD; ++it) stage(it, it);
     stage_q(0, even);
+    stage_do(0, even, 0, 0);
+    stage_do(1, odd, 1, 1);
     load(0, in);
     direct_loads_done();
     lds_barrier();
-    read_do(in);
+    read_do(in, even);
     form_z(in);
-    form_qdo(0, even, in);
-    lds_barrier();
-    stage_do(1);
-    if constexpr (RING > 1) stage_q(1, odd);
     load(1, in);
+    form_qdo(0, even, lds.coef[0]);
+    lds_barrier();
+    if constexpr (LEAD > 0) {
+      stage_q(1, odd);
+      stage_do(2, even, 1, 1);
+    }
     direct_loads_done();
     lds_barrier();
     for (int it = 0; it < nc; it += 2) {
       step(it, even, odd);
       if (it + 1 < nc) step(it + 1, odd, even);
     }
+    };
+    if (w < 2) run(std::true_type{});
+    else run(std::false_type{});
   }
+  direct_loads_done();
 }
 
 // --------------------------------------------------------------------------------------------
@@ -377,22 +424,18 @@ __device__ __forceinline__ Operand<T, 1> load_columns_paired(const T* tile, int 
   return o;
 }
 
-template <typename T, int NP>
-__device__ __forceinline__ float operand_dot(const Operand<T, NP>& a, const Operand<T, 1>& b) {
-  float s = 0.f;
-  if constexpr (sizeof(T) == 2) {
+// The pieces' sums.
+template <typename T, int NP> __device__ __forceinline__ void whole(const Operand<T, NP>& a, float (&x)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float x = (float)a.p[NP - 1][e];
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (sizeof(T) == 2) {
+      x[e] = (float)a.p[NP - 1][e];
 #pragma unroll
-      for (int i = NP - 2; i >= 0; --i) x += (float)a.p[i][e];
-      s += x * (float)b.p[0][e];
+      for (int i = NP - 2; i >= 0; --i) x[e] += (float)a.p[i][e];
+    } else {
+      x[e] = e < 4 ? a.lo[e & 3] : a.hi[e & 3];
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s += a.lo[e] * b.lo[e] + a.hi[e] * b.hi[e];
   }
-  return s;
 }
 
 template <typename T>
@@ -444,7 +487,7 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const float* __restrict__ g,
     const T* __restrict__ d_o, const float* __restrict__ coef, const float* __restrict__ rec_h,
     const float* __restrict__ rec_d, const float* __restrict__ rec_dh, const float* __restrict__ rec_dr,
-    const uint8_t* __restrict__ active, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dbeta,
+    const uint8_t* __restrict__ active, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv, T* __restrict__ dbeta,
     float* __restrict__ dg, Dims<T> dims) {
   using S = GradShape<T, DP>;
   constexpr int NT = S::NT, TILES = S::TILES, QUADS = S::QUADS, ITEMS = S::ITEMS;
@@ -495,6 +538,8 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
       xdr = load16(rdr, at);
     };
     load(0);
+    const float beta_own = coef[(size_t)id * kCoefAll + own];
+    const Rows<T> dvrows = dims.rows(dv, b, t0, h);
     for (int v0 = 0; v0 < D; v0 += 32) {
       const int vc = v0 + 8 * grp;
       Operand<T, 1> dof[4];  // dO of all tokens; first: dO and V of its own
@@ -533,7 +578,15 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
           acc[i] = mma(x, dof[0], acc[i]);
           ay[i] = mma(x, dr_w, ay[i]);
         }
-        dot_v += operand_dot(dr_w, dof[1]);
+        float dr8[8], v8[8];  // dV = beta dR
+        whole<T, NT>(dr_w, dr8);
+        whole<T, 1>(dof[1], v8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          dot_v += dr8[e] * v8[e];
+          dr8[e] *= beta_own;
+        }
+        dvrows.put_eight(own, vc, dr8);
       } else {
         const Operand<T, NT> del_w = lds.u.values.delta.columns(16 * w);
 #pragma unroll
@@ -561,7 +614,6 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
       }
     }
     auto sum_at = [&](int i) { return DecaySum{lds.coef[kCoef + i], lds.coef[kCoef + kChunk + i]}; };
-    const float beta_own = lds.coef[own];
     const DecaySum sum_own = sum_at(own);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -721,9 +773,9 @@ void launch_back(const T* q, const T* k, const T* v, const float* g, const T* d_
                  Dims<T> dims, int B, hipStream_t stream) {
   const int slices = (dims.D + 15) / 16;
   hipLaunchKernelGGL((gated_chain_backward_kernel<T, DP>), dim3((unsigned)(B * dims.H * slices)), dim3(512), 0, stream, q, k, d_o,
-                     coef, tf, pf, d_state, dv, d_state_in, active, rec_dh, rec_dr, dims, slices);
+                     coef, tf, pf, d_state, d_state_in, active, rec_dh, rec_dr, dims, slices);
   hipLaunchKernelGGL((gated_grad_kernel<T, DP>), dim3((unsigned)(B * dims.H * dims.chunks)), dim3(512), 0, stream, q, k, v, g,
-                     d_o, coef, rec_h, rec_d, rec_dh, rec_dr, active, dq, dk, dbeta, dg, dims);
+                     d_o, coef, rec_h, rec_d, rec_dh, rec_dr, active, dq, dk, dv, dbeta, dg, dims);
 }
 
 template <typename T>
