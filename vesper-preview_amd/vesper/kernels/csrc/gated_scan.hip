@@ -23,16 +23,35 @@ constexpr int kTile = 16 * kPad + 4;       // tiles start on other banks
 constexpr int kPrepWaves = 4;
 
 struct PrepLds {
-  DecaySum sums[kChunk];
-  float beta[kChunk];  // -beta
-  float a[4 * kTile];  // diagonal tiles of -A
-  float x[4 * kTile];  // their inverses (I + A_bb)^-1
+  float hi[kChunk], lo[kChunk];  // both parts of the decays' sums
+  float beta[kChunk];            // -beta
+  float a[4 * kTile];            // diagonal tiles of -A, column by column
+  float x[4 * kTile];            // their inverses (I + A_bb)^-1, row by row
 };
 
 __device__ __forceinline__ void wave_lds_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// x moved along the lanes by the pattern CTRL, in the rows of 16 lanes of ROWS; zero where nothing moves in.
+template <int CTRL, int ROWS> __device__ __forceinline__ double moved(double x) {
+  const u32x2_t y = __builtin_bit_cast(u32x2_t, x);
+  const u32x2_t z = {(unsigned)__builtin_amdgcn_update_dpp(0, (int)y[0], CTRL, ROWS, 0xf, false),
+                     (unsigned)__builtin_amdgcn_update_dpp(0, (int)y[1], CTRL, ROWS, 0xf, false)};
+  return __builtin_bit_cast(double, z);
+}
+// Sums of x over the lanes up to each one, moved in registers: through shuffles, by LDS, they
+// took 4000 cycles longer.
+__device__ __forceinline__ double sums_up_to(double x) {
+  x += moved<0x111, 0xf>(x);  // one, two, four and eight lanes up within 16
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  x += moved<0x142, 0xa>(x);  // lane 15 of 16 to the next 16, in the odd ones
+  x += moved<0x143, 0xc>(x);  // lane 31 to the upper half
+  return x;
 }
 
 // C[16 x 16] += A B in float32: lane (c, g) holds A[c][4 g + r] and B[4 g + r][c], an accumulator's own layout.
@@ -75,22 +94,33 @@ __global__ __launch_bounds__(64 * kPrepWaves, 2) void gated_prep_kernel(
   constexpr int KS = DP / 32;
   constexpr int NT = Pieces<T>::kN, NPP = COLS ? NT : OutPieces<T>::kN;
 
-  // decays: lane l is token t0 + l; tokens behind the last decay nothing and write nothing
-  {
-    const int t = t0 + l;
-    const bool ok = t < dims.N;
-    const size_t at = ((size_t)b * dims.N + (ok ? t : t0)) * dims.H + h;
-    const float gl = g[at], bl = to_f32(beta[at]);
-    double sum = ok ? ((double)gl < kLeastDecay ? kLeastDecay : (double)gl) : 0.0;
+  // the decays and the first rows are loaded together
+  const bool ok = t0 + l < dims.N;
+  const size_t at = ((size_t)b * dims.N + (ok ? t0 + l : t0)) * dims.H + h;
+  const float gl = g[at], bl = to_f32(beta[at]);
+  const Rows<T> krows = dims.rows(k, b, t0, h), qrows = dims.rows(q, b, t0, h);
+  struct In {
+    Operand<T, 1> k[4], q[4];
+  };
+  auto load = [&](int st, In& in) {
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const double up = __shfl_up(sum, off);
-      if (l >= off) sum += up;
+    for (int i = 0; i < 4; ++i) {
+      in.k[i] = krows.row(16 * i + c, 32 * st + 8 * grp);
+      in.q[i] = qrows.row(16 * i + c, 32 * st + 8 * grp);
     }
-    const double all = __shfl(sum, 63);
+  };
+  In in[2];
+  load(0, in[0]);
+  // lane l is token t0 + l; tokens behind the last decay nothing and write nothing
+  {
+    const double sum = sums_up_to(ok ? ((double)gl < kLeastDecay ? kLeastDecay : (double)gl) : 0.0);
+    const u32x2_t bits = __builtin_bit_cast(u32x2_t, sum);
+    const u32x2_t last = {(unsigned)__builtin_amdgcn_readlane((int)bits[0], 63), (unsigned)__builtin_amdgcn_readlane((int)bits[1], 63)};
+    const double all = __builtin_bit_cast(double, last);
     const float be = ok ? bl : 0.f;
     const DecaySum parts = decay_sum(sum);
-    s.sums[l] = parts;
+    s.hi[l] = parts.hi;
+    s.lo[l] = parts.lo;
     s.beta[l] = -be;
     float* co = coef + (size_t)id * kCoefAll;
     co[l] = be;
@@ -105,29 +135,36 @@ __global__ __launch_bounds__(64 * kPrepWaves, 2) void gated_prep_kernel(
   f32x4 mult[10], pp[10];
 #pragma unroll
   for (int t = 0; t < 10; ++t) mult[t] = pp[t] = zero4();
-  const Rows<T> krows = dims.rows(k, b, t0, h), qrows = dims.rows(q, b, t0, h);
 #pragma unroll
   for (int st = 0; st < KS; ++st) {
-    Operand<T, 1> kf[4], qf[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      kf[i] = krows.row(16 * i + c, 32 * st + 8 * grp);
-      qf[i] = qrows.row(16 * i + c, 32 * st + 8 * grp);
-    }
+    if (st + 1 < KS) load(st + 1, in[(st + 1) & 1]);
+    const In& now = in[st & 1];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j <= i; ++j) {
         const int t = i * (i + 1) / 2 + j;
-        mult[t] = COLS ? mma(kf[j], kf[i], mult[t]) : mma(kf[i], kf[j], mult[t]);
-        pp[t] = COLS ? mma(qf[i], kf[j], pp[t]) : mma(kf[j], qf[i], pp[t]);
+        mult[t] = COLS ? mma(now.k[j], now.k[i], mult[t]) : mma(now.k[i], now.k[j], mult[t]);
+        pp[t] = COLS ? mma(now.q[i], now.k[j], pp[t]) : mma(now.k[j], now.q[i], pp[t]);
       }
   }
   wave_lds_sync();
 
-  // the decays between pairs, -beta and the triangles
+  // the decays between pairs, -beta and the triangles; the sums are read at once, not each before its use
   T* tout = tf + (size_t)id * Factor<T, NT>::kElems;
   T* pout = pf + (size_t)id * Factor<T, NPP>::kElems;
+  f32x4 hi_row[4], lo_row[4], beta_row[4];  // of tokens 16 i + 4 g + r
+  DecaySum col[4];                          // of tokens 16 i + c
+  float beta_col[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    hi_row[i] = *reinterpret_cast<const f32x4*>(s.hi + 16 * i + 4 * grp);
+    lo_row[i] = *reinterpret_cast<const f32x4*>(s.lo + 16 * i + 4 * grp);
+    beta_row[i] = *reinterpret_cast<const f32x4*>(s.beta + 16 * i + 4 * grp);
+    col[i] = {s.hi[16 * i + c], s.lo[16 * i + c]};
+    beta_col[i] = s.beta[16 * i + c];
+  }
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -136,27 +173,25 @@ __global__ __launch_bounds__(64 * kPrepWaves, 2) void gated_prep_kernel(
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = 4 * grp + r;
-        {
-          const int ii = 16 * i + (COLS ? c : row), jj = 16 * j + (COLS ? row : c);
-          const float e = decay(s.sums[ii], s.sums[jj]);
-          mult[t][r] *= i > j || jj < ii ? s.beta[ii] * e : 0.f;
-        }
-        {
-          const int ii = 16 * i + (COLS ? row : c), jj = 16 * j + (COLS ? c : row);
-          pp[t][r] *= i > j || jj <= ii ? decay(s.sums[ii], s.sums[jj]) : 0.f;
-        }
+        const DecaySum row_i = {hi_row[i][r], lo_row[i][r]}, row_j = {hi_row[j][r], lo_row[j][r]};
+        // of mult: i by rows, j by columns (COLS: the other way round); of Q K^T: i by columns, j by rows (COLS: the other way)
+        const float em = (COLS ? beta_col[i] : beta_row[i][r]) * (COLS ? decay(col[i], row_j) : decay(row_i, col[j]));
+        mult[t][r] *= i > j || (COLS ? row < c : c < row) ? em : 0.f;
+        const float ep = COLS ? decay(row_i, col[j]) : decay(col[i], row_j);
+        pp[t][r] *= i > j || (COLS ? c <= row : row <= c) ? ep : 0.f;
       }
-      if (i == j) {  // -A[ii][jj] of the diagonal tile, row-major
+      if (i == j) {  // -A[ii][jj] of the diagonal tile at jj * kPad + ii
+        if constexpr (COLS) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int ii = COLS ? c : 4 * grp + r, jj = COLS ? 4 * grp + r : c;
-          s.a[i * kTile + ii * kPad + jj] = mult[t][r];
+          for (int r = 0; r < 4; ++r) s.a[i * kTile + (4 * grp + r) * kPad + c] = mult[t][r];
+        } else {
+          *reinterpret_cast<f32x4*>(s.a + i * kTile + c * kPad + 4 * grp) = mult[t];
         }
       }
     }
   wave_lds_sync();
 
-  // X = (I + A_bb)^-1 by forward substitution: lane l solves column l % 16 of block l / 16, column by column
+  // X = (I + A_bb)^-1 by forward substitution: lane l solves column l % 16 of block l / 16, column by column of A
   {
     float x[16];
 #pragma unroll
@@ -165,7 +200,12 @@ __global__ __launch_bounds__(64 * kPrepWaves, 2) void gated_prep_kernel(
 #pragma unroll
     for (int kk = 0; kk < 15; ++kk)
 #pragma unroll
-      for (int r = kk + 1; r < 16; ++r) x[r] = __builtin_fmaf(a[r * kPad + kk], x[kk], x[r]);
+      for (int f = (kk + 1) / 4; f < 4; ++f) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(a + kk * kPad + 4 * f);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (4 * f + r > kk) x[4 * f + r] = __builtin_fmaf(y[r], x[kk], x[4 * f + r]);
+      }
 #pragma unroll
     for (int r = 0; r < 16; ++r) s.x[grp * kTile + r * kPad + c] = x[r];
   }
