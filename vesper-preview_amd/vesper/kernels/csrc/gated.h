@@ -350,18 +350,16 @@ template <> struct Pieces<float> { static constexpr int kN = 1; };
 template <typename T> struct OutPieces { static constexpr int kN = 2; };
 template <> struct OutPieces<float> { static constexpr int kN = 1; };
 
-// A chunk's record of one value column a lane: float32 [D][rows], written four at a time; columns and rows past the
-// width are dropped.
+// A chunk's record of accumulator tiles, 1 KiB each as they lie in a wave's registers: a store of a wave is contiguous (by
+// columns of the matrix, 64 bytes at a time, the stores took as long as all else in the chain).
 struct Record {
   __amdgpu_buffer_rsrc_t r;
-  int rows, D;
-  __device__ __forceinline__ void put(int col, int row, f32x4 x) const {
-    const unsigned o = col < D && row < rows ? ((unsigned)col * rows + row) * 4u : kNowhere;
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), r, o, 0, 0);
+  __device__ __forceinline__ void put(int tile, f32x4 x) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), r, (64 * tile + (threadIdx.x & 63)) * 16, 0, 0);
   }
 };
-__device__ __forceinline__ Record record(float* base, size_t chunk, int rows, int D) {
-  return {buffer_rsrc(base + chunk * rows * D, (unsigned)rows * D * 4u), rows, D};
+__device__ __forceinline__ Record record(float* base, size_t chunk, int tiles) {
+  return {buffer_rsrc(base + chunk * tiles * 256, (unsigned)tiles * 1024u)};
 }
 
 // LDS writes before, LDS reads after, for the whole workgroup; loads from memory stay in flight, direct loads into LDS
@@ -402,9 +400,12 @@ int launch_prep(const T* q, const T* k, const T* beta, const float* g, float* co
 
 int check_sizes(int B, int N, int H, int D, const char* who);
 
-// the records of a forward that a backward follows, float32: each chunk's starting state [value][feature], then its
-// Delta [value][token]
-inline size_t record_bytes(size_t total, int D) { return total * D * (D + kChunk) * sizeof(float); }
+// the records of a forward that a backward follows, float32 accumulator tiles (rows features or tokens, columns values): of
+// each chunk its starting state, tile (value tile) * tiles + (feature tile); then of each its Delta, tile (value tile) * 4 +
+// (token tile)
+__host__ __device__ constexpr int tiles_of(int D) { return (D + 15) / 16; }
+__host__ __device__ inline size_t state_floats(size_t total, int D) { return total * tiles_of(D) * tiles_of(D) * 256; }
+inline size_t record_bytes(size_t total, int D) { return (state_floats(total, D) + total * tiles_of(D) * 4 * 256) * sizeof(float); }
 inline int chunks_of(int N) { return (N + kChunk - 1) / kChunk; }
 inline int width_of(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 

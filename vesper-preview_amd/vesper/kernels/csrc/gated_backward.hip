@@ -146,9 +146,10 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
       }
       const f32x4 kap = *reinterpret_cast<const f32x4*>(co + 2 * kChunk + own);
       const f32x4 z = *reinterpret_cast<const f32x4*>(lds.z + 256 * w + 4 * lane);
-      const Record rh = record(rec_dh, chunk0 + ci, D, D);
+      const Record rh = record(rec_dh, chunk0 + ci, slices * slices);
 #pragma unroll
-      for (int i = 0; i < FT; ++i) rh.put(vcol, 16 * (w + 4 * i) + 4 * grp, dh[i]);
+      for (int i = 0; i < FT; ++i)
+        if (w + 4 * i < slices) rh.put(sl * slices + w + 4 * i, dh[i]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] = kap[r] * x[r] + z[r];
       F::template put_tile<false>(lds.ddelta, w, x);
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
 #pragma unroll
       for (int r = 0; r < 4; ++r) y[r] = -(beta[r] * dr[r] * eps[r]);
       F::template put_tile<false>(lds.dread, w, y);
-      record(rec_dr, chunk0 + ci, kChunk, D).put(vcol, own, dr);
+      record(rec_dr, chunk0 + ci, 4 * slices).put(4 * sl + w, dr);
       lds_barrier();
       // dH = gam dH' + Q^T (eps dO) - K^T (beta eps dR)
       const Operand<T, NT> y0 = F::get(lds.dread, 0), y1 = F::get(lds.dread, 1);
@@ -456,8 +457,7 @@ template <typename T, int DP> struct GradShape {
   static constexpr int NT = Pieces<T>::kN;
   static constexpr int PAD = sizeof(T) == 2 ? 8 : 4;
   static constexpr int PITCH = DP + PAD;
-  static constexpr int QUADS = DP / 4;                      // float32 quads a row of the states' records
-  static constexpr int ITEMS = DP < 64 ? 1 : DP / 64;       // of 32 rows a thread's
+  static constexpr int ITEMS = TILES < 4 ? 1 : TILES / 4;  // tiles a wave's of the states' records of 32 columns
   using States = Planes<T, NT, 32, DP + PAD>;
   using Tokens = Planes<T, NT, 32, kChunk + PAD>;
   struct Values {  // 32 value columns
@@ -490,7 +490,7 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
     const uint8_t* __restrict__ active, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv, T* __restrict__ dbeta,
     float* __restrict__ dg, Dims<T> dims) {
   using S = GradShape<T, DP>;
-  constexpr int NT = S::NT, TILES = S::TILES, QUADS = S::QUADS, ITEMS = S::ITEMS;
+  constexpr int NT = S::NT, TILES = S::TILES, ITEMS = S::ITEMS;
   __shared__ __attribute__((aligned(16))) typename S::Lds lds;
   const int id = xcd_logical_block(blockIdx.x, gridDim.x);
   const int chunk = id % dims.chunks, bh = id / dims.chunks, h = bh % dims.H, b = bh / dims.H;
@@ -509,9 +509,10 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
 #pragma unroll
     for (int i = 0; i < 4; ++i) mp[i] = mb[i] = zero4();
     float inner = 0.f, dot_v = 0.f;
-    const unsigned state_bytes = (unsigned)D * D * 4u, token_bytes = (unsigned)D * kChunk * 4u;
-    const __amdgpu_buffer_rsrc_t rh = buffer_rsrc(rec_h + (size_t)id * D * D, state_bytes), rdh = buffer_rsrc(rec_dh + (size_t)id * D * D, state_bytes),
-                                 rd = buffer_rsrc(rec_d + (size_t)id * D * kChunk, token_bytes), rdr = buffer_rsrc(rec_dr + (size_t)id * D * kChunk, token_bytes);
+    const int tiles = tiles_of(D);
+    const unsigned state_bytes = (unsigned)(tiles * tiles) * 1024u, token_bytes = (unsigned)tiles * 4096u;
+    const __amdgpu_buffer_rsrc_t rh = buffer_rsrc(rec_h + state_floats(id, D), state_bytes), rdh = buffer_rsrc(rec_dh + state_floats(id, D), state_bytes),
+                                 rd = buffer_rsrc(rec_d + (size_t)id * tiles * 1024, token_bytes), rdr = buffer_rsrc(rec_dr + (size_t)id * tiles * 1024, token_bytes);
     const Rows<T> dorows = dims.rows(d_o, b, t0, h), vrows = dims.rows(v, b, t0, h);
     bool on[first ? 1 : 4];  // of the own token; of token 16 i + c
     {
@@ -528,12 +529,12 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
     auto load = [&](int v0) {
 #pragma unroll
       for (int n = 0; n < ITEMS; ++n) {
-        const int p = threadIdx.x + 512 * n, row = p / QUADS, f = 4 * (p % QUADS);
-        const unsigned at = row < 32 && f < D ? ((unsigned)(v0 + row) * D + f) * 4u : kNowhere;
+        const int tile = wave + 8 * n, ft = tile % TILES, half = tile / TILES;
+        const unsigned at = half < 2 && ft < tiles ? (unsigned)(64 * ((v0 / 16 + half) * tiles + ft) + l) * 16u : kNowhere;
         xh[n] = load16(rh, at);
         xdh[n] = load16(rdh, at);
       }
-      const unsigned at = ((unsigned)v0 * kChunk + 4 * threadIdx.x) * 4u;
+      const unsigned at = (unsigned)(64 * (4 * (v0 / 16) + wave) + l) * 16u;
       xd = load16(rd, at);
       xdr = load16(rdr, at);
     };
@@ -552,15 +553,15 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
       }
 #pragma unroll
       for (int n = 0; n < ITEMS; ++n) {
-        const int p = threadIdx.x + 512 * n, row = p / QUADS, f = 4 * (p % QUADS);
+        const int tile = wave + 8 * n, ft = tile % TILES, half = tile / TILES;
         inner += (xh[n][0] * xdh[n][0] + xh[n][1] * xdh[n][1]) + (xh[n][2] * xdh[n][2] + xh[n][3] * xdh[n][3]);
-        if (32 * QUADS >= 512 || row < 32) {
-          lds.u.values.h.put(row, f, xh[n]);
-          lds.u.values.dh.put(row, f, xdh[n]);
+        if (2 * TILES % 8 == 0 || half < 2) {
+          lds.u.values.h.put(16 * half + c, 16 * ft + 4 * grp, xh[n]);
+          lds.u.values.dh.put(16 * half + c, 16 * ft + 4 * grp, xdh[n]);
         }
       }
-      lds.u.values.delta.put(threadIdx.x / 16, 4 * (threadIdx.x % 16), xd);
-      lds.u.values.dr.put(threadIdx.x / 16, 4 * (threadIdx.x % 16), xdr);
+      lds.u.values.delta.put(16 * (wave / 4) + c, 16 * w + 4 * grp, xd);
+      lds.u.values.dr.put(16 * (wave / 4) + c, 16 * w + 4 * grp, xdr);
       lds_barrier();
       load(v0 + 32);  // past the width: zeros
       if constexpr (first) {
@@ -803,8 +804,8 @@ int scan_backward(const void* q_, const void* k_, const void* v_, const void* be
   T* tf = reinterpret_cast<T*>(static_cast<char*>(ws) + align16(total * kCoefAll * sizeof(float)));
   T* pf = tf + total * Factor<T, Pieces<T>::kN>::kElems;
   float* rec_dh = reinterpret_cast<float*>(static_cast<char*>(ws) + factor_bytes<T>(total));
-  float* rec_dr = rec_dh + total * D * D;
-  const float* rec_d = records + total * D * D;
+  float* rec_dr = rec_dh + state_floats(total, D);
+  const float* rec_d = records + state_floats(total, D);
   const Dims<T> dims{N, H, D, chunks_of(N)};
   if (const int st = launch_prep<T>(q, k, beta, g, coef, tf, pf, B, N, H, D, true, stream); st != OK) return st;
 #define VSP_BACK(DP) launch_back<T, DP>(q, k, v, g, d_o, d_state, active, records, rec_d, coef, tf, pf, rec_dh, rec_dr, dq, dk, \

@@ -377,9 +377,10 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
       const f32x4 eps = *reinterpret_cast<const f32x4*>(in.coef + kChunk + own);
       const f32x4 vx = Slice::four(in.values, w, 0);
       if constexpr (RECORD) {
-        const Record rh = record(rec_h, chunk0 + ci, D, D);
+        const Record rh = record(rec_h, chunk0 + ci, slices * slices);
 #pragma unroll
-        for (int i = 0; i < FT; ++i) rh.put(vcol, 16 * (w + 4 * i) + 4 * grp, hs[i]);
+        for (int i = 0; i < FT; ++i)
+          if (w + 4 * i < slices) rh.put(sl * slices + w + 4 * i, hs[i]);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] = beta[r] * (vx[r] - eps[r] * x[r]);
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
 #pragma unroll
       for (int r = 0; r < 4; ++r) kd[r] = kap[r] * dl[r];
       F::template put_tile<false>(lds.kept, w, kd);
-      if constexpr (RECORD) record(rec_d, chunk0 + ci, kChunk, D).put(vcol, own, dl);
+      if constexpr (RECORD) record(rec_d, chunk0 + ci, 4 * slices).put(4 * sl + w, dl);
       lds_barrier();
       // H' = gam H + K^T (kap Delta)
       const Operand<T, NT> k0 = F::get(lds.kept, 0), k1 = F::get(lds.kept, 1);
@@ -578,7 +579,7 @@ int scan(const void* q_, const void* k_, const void* v_, const void* beta_, cons
   T* pf = tf + total * Factor<T, Pieces<T>::kN>::kElems;
   const Dims<T> dims{N, H, D, chunks_of(N)};
   if (const int st = launch_prep<T>(q, k, beta, g, coef, tf, pf, B, N, H, D, false, stream); st != OK) return st;
-  float* rec_d = records == nullptr ? nullptr : records + total * D * D;
+  float* rec_d = records == nullptr ? nullptr : records + state_floats(total, D);
   switch (width_of(D)) {
     case 32: launch_chain<T, 32>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, dims, B, stream); break;
     case 64: launch_chain<T, 64>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, dims, B, stream); break;
