@@ -471,6 +471,7 @@ template <typename T, int DP> struct GradShape {
   struct Lds {
     union {
       Values values;
+      float pairs[2][kChunk][kChunk + 4];  // E dO.Delta (j <= i) and E dR.Delta (j < i), [i][j]
       Rows rows;
       f32x4 y[4][TILES][64];  // beta Y as accumulator tiles
     } u;
@@ -501,8 +502,8 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
   auto body = [&](auto kind) {
     constexpr bool first = decltype(kind)::value;
     // ---- sums over the value columns, 32 at a time ----
-    // first: dQ^T and Y^T (rows features, columns the wave's tokens); dP^T, B^T (rows j, columns the wave's tokens i >= j);
-    // else: C^T; dP, B (rows i, columns the wave's tokens j <= i)
+    // first: dQ^T and Y^T (rows features, columns the wave's tokens); else C^T, and dP and B (rows i, columns the wave's tokens
+    // j <= i), which the others get by LDS, transposed
     f32x4 acc[TILES], ay[first ? TILES : 1], mp[4], mb[4];
 #pragma unroll
     for (int i = 0; i < TILES; ++i) acc[i] = ay[first ? i : 0] = zero4();
@@ -567,13 +568,6 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
       if constexpr (first) {
         const Operand<T, NT> dr_w = lds.u.values.dr.columns(16 * w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i <= w) {
-            const Operand<T, NT> x = lds.u.values.delta.columns(16 * i);
-            mp[i] = mma(x, dof[0], mp[i]);
-            mb[i] = mma(x, dr_w, mb[i]);
-          }
-#pragma unroll
         for (int i = 0; i < TILES; ++i) {
           const Operand<T, NT> x = lds.u.values.h.columns(16 * i);
           acc[i] = mma(x, dof[0], acc[i]);
@@ -614,26 +608,26 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
         qx[n] = qrows.row(row, row < kChunk ? f : D);
       }
     }
-    auto sum_at = [&](int i) { return DecaySum{lds.coef[kCoef + i], lds.coef[kCoef + kChunk + i]}; };
-    const DecaySum sum_own = sum_at(own);
+    if constexpr (!first) {
+      const DecaySum sum_own = {lds.coef[kCoef + own], lds.coef[kCoef + kChunk + own]};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (first ? i <= w : i >= w) {
+      for (int i = 0; i < 4; ++i)
+        if (i >= w) {
+          const float* co = lds.coef + 16 * i + 4 * grp;
+          const f32x4 beta = *reinterpret_cast<const f32x4*>(co), hi = *reinterpret_cast<const f32x4*>(co + kCoef),
+                      lo = *reinterpret_cast<const f32x4*>(co + kCoef + kChunk);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * i + 4 * grp + r;
-          const DecaySum sum = sum_at(row);
-          if constexpr (first) {  // row j, column i
-            const float e = row <= own ? decay(sum_own, sum) : 0.f;
-            mp[i][r] *= e;
-            mb[i][r] *= row < own ? e : 0.f;
-          } else {  // row i, column j
-            const float e = row >= own ? decay(sum, sum_own) : 0.f;
-            mp[i][r] *= e;
-            mb[i][r] *= row > own ? -lds.coef[row] * e : 0.f;
+          for (int r = 0; r < 4; ++r) {
+            const int row = 16 * i + 4 * grp + r;
+            const float e = decay({hi[r], lo[r]}, sum_own);
+            mp[i][r] *= row >= own ? e : 0.f;
+            mb[i][r] *= row > own ? e : 0.f;
+            lds.u.pairs[0][row][own] = mp[i][r];
+            lds.u.pairs[1][row][own] = mb[i][r];
+            mb[i][r] *= -beta[r];
           }
         }
-      }
+    }
     const float scale = lds.coef[(first ? kChunk : 2 * kChunk) + own];  // eps, kap
 #pragma unroll
     for (int i = 0; i < TILES; ++i)
@@ -642,6 +636,16 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
         acc[i][r] *= scale;
         if constexpr (first) ay[i][r] *= scale;
       }
+    lds_barrier();
+    if constexpr (first) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i <= w) {
+          mp[i] = *reinterpret_cast<const f32x4*>(&lds.u.pairs[0][own][16 * i + 4 * grp]);
+          mb[i] = *reinterpret_cast<const f32x4*>(&lds.u.pairs[1][own][16 * i + 4 * grp]);
+        }
+    }
+    lds_barrier();
 #pragma unroll
     for (int n = 0; n < KQ; ++n) {
       const int p = threadIdx.x + 512 * n, row = p / (DP / 8), f = 8 * (p % (DP / 8));
