@@ -405,3 +405,59 @@ def test_offsets_past_32_bits():
         o, after = gated_delta_scan(q, k, v, beta, g, state)
         alone, last = gated_delta_scan(*(t[-1:] for t in (q, k, v, beta, g, state)))
     assert torch.equal(o[-1:], alone) and torch.equal(after[-1:], last)
+
+
+# few long rows: the sequence in segments, whose starting states are joined first
+LONG = [(1, 2100, 2, 64), (2, 2048, 1, 16), (1, 4095, 1, 64), (1, 2500, 1, 128), (1, 2049, 1, 200), (1, 2177, 3, 20)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", LONG, ids=str)
+@pytest.mark.parametrize("resets", [False, True])
+def test_long_rows_match_the_oracle(dtype, size, resets):
+    from vesper.kernels.gated_scan import gated_delta_scan
+
+    inputs = _inputs(*size, dtype, seed=sum(size), resets=resets)
+    active = (torch.rand(*size[:2], generator=torch.Generator().manual_seed(3)) < 0.8).to(GPU) if resets else None
+    with torch.no_grad():
+        o, after = gated_delta_scan(*inputs, active=active)
+    want, last = _oracle(inputs, active)
+    _close(o, want, what="o")
+    _close(after, last, what="state")
+    if active is not None:
+        assert not bool(o[~active].any())
+
+
+def test_long_rows_keep_a_nan_to_its_head_and_what_follows():
+    """Chunks before the one with the NaN, and the other head, are bit for bit as without it."""
+    from vesper.kernels.gated_scan import gated_delta_scan
+
+    inputs = _inputs(1, 2100, 2, 64, BF16, seed=9)
+    with torch.no_grad():
+        o, after = gated_delta_scan(*inputs)
+        inputs[2][0, 1000, 1, 5] = math.nan  # token 1000: chunk 15, the tokens 960 .. 1023
+        bad, bad_after = gated_delta_scan(*inputs)
+    assert torch.equal(bad[:, :960], o[:, :960]) and torch.equal(bad[:, :, 0], o[:, :, 0])
+    assert torch.equal(bad_after[:, 0], after[:, 0]) and bool(bad_after[0, 1].isnan().any())
+
+
+def test_long_rows_in_a_graph():
+    from vesper.kernels.gated_scan import gated_delta_scan
+
+    inputs = _inputs(1, 2100, 2, 64, BF16, seed=4)
+    side = torch.cuda.Stream()
+    with torch.no_grad(), torch.cuda.stream(side):
+        gated_delta_scan(*inputs)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            o, after = gated_delta_scan(*inputs)
+    torch.cuda.synchronize()
+    for seed in (5, 6, 7):
+        for t, x in zip(inputs, _inputs(1, 2100, 2, 64, BF16, seed=seed)):
+            t.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            want, last = gated_delta_scan(*inputs)
+        assert torch.equal(o, want) and torch.equal(after, last)

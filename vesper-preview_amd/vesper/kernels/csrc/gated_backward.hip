@@ -113,100 +113,100 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
     lds_barrier();
     // BOTH: the wave's columns of T have two steps. The code twice, so that no load is conditional
     auto run = [&](auto both) {
-    constexpr bool BOTH = decltype(both)::value;
-    auto load = [&](int it, BackChainIn<T>& to) {
-      const T* tc = tp + (size_t)(it < nc ? nc - 1 - it : 0) * Factor<T, NT>::kElems;
-      if constexpr (BOTH) to.t[0] = F::get(tc, col_step(w, 0));
-      to.t[1] = F::get(tc, col_step(w, 1));
-    };
-    BackChainIn<T> ta, tb;
-    load(0, ta);
-    int slot = 0, cslot = 0;
-    auto step = [&](int it, const BackChainIn<T>& tin, BackChainIn<T>& next) {
-      const int ci = nc - 1 - it;
-      const T* keys = lds.keys[slot];
-      const float* co = lds.coef[cslot];
-      slot = slot + 1 < RING ? slot + 1 : 0;
-      cslot = cslot + 1 < 3 ? cslot + 1 : 0;
-      if constexpr (LEAD == 0) lds_barrier();
-      // dDelta = P^T dO + kap (K dH')
-      f32x4 x = zero4();
+      constexpr bool BOTH = decltype(both)::value;
+      auto load = [&](int it, BackChainIn<T>& to) {
+        const T* tc = tp + (size_t)(it < nc ? nc - 1 - it : 0) * Factor<T, NT>::kElems;
+        if constexpr (BOTH) to.t[0] = F::get(tc, col_step(w, 0));
+        to.t[1] = F::get(tc, col_step(w, 1));
+      };
+      BackChainIn<T> ta, tb;
+      load(0, ta);
+      int slot = 0, cslot = 0;
+      auto step = [&](int it, const BackChainIn<T>& tin, BackChainIn<T>& next) {
+        const int ci = nc - 1 - it;
+        const T* keys = lds.keys[slot];
+        const float* co = lds.coef[cslot];
+        slot = slot + 1 < RING ? slot + 1 : 0;
+        cslot = cslot + 1 < 3 ? cslot + 1 : 0;
+        if constexpr (LEAD == 0) lds_barrier();
+        // dDelta = P^T dO + kap (K dH')
+        f32x4 x = zero4();
 #pragma unroll
-      for (int s0 = 0; s0 < KS; s0 += 2) {
-        Operand<T, 1> kr[2];
-        Operand<T, NT> st[2];
+        for (int s0 = 0; s0 < KS; s0 += 2) {
+          Operand<T, 1> kr[2];
+          Operand<T, NT> st[2];
 #pragma unroll
-        for (int s = 0; s < 2 && s0 + s < KS; ++s) {
-          kr[s] = Keys::row(keys, 16 * w + c, 32 * (s0 + s) + 8 * grp);
-          st[s] = F::get(lds.state, s0 + s);
-        }
-        __builtin_amdgcn_sched_barrier(0);  // reads together, not one by one before its product
-#pragma unroll
-        for (int s = 0; s < 2 && s0 + s < KS; ++s) x = mma(kr[s], st[s], x);
-      }
-      const f32x4 kap = *reinterpret_cast<const f32x4*>(co + 2 * kChunk + own);
-      const f32x4 z = *reinterpret_cast<const f32x4*>(lds.z + 256 * w + 4 * lane);
-      const Record rh = record(rec_dh, chunk0 + ci, slices * slices);
-#pragma unroll
-      for (int i = 0; i < FT; ++i)
-        if (w + 4 * i < slices) rh.put(sl * slices + w + 4 * i, dh[i]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = kap[r] * x[r] + z[r];
-      F::template put_tile<false>(lds.ddelta, w, x);
-      lds_barrier();
-      // dR = T^T dDelta; the next chunk's T, K^T and Q^T (eps dO) on the way
-      Operand<T, NT> d0;
-      if constexpr (BOTH) d0 = F::get(lds.ddelta, 0);
-      const Operand<T, NT> d1 = F::get(lds.ddelta, 1);
-      __builtin_amdgcn_sched_barrier(0);
-      load(it + 1, next);
-      f32x4 dr = mma(tin.t[1], d1, zero4());
-      if constexpr (BOTH) dr = mma(tin.t[0], d0, dr);
-      const f32x4 beta = *reinterpret_cast<const f32x4*>(co + own);
-      const f32x4 eps = *reinterpret_cast<const f32x4*>(co + kChunk + own);
-      const float gam = co[2 * kChunk - 1];
-      constexpr int AHEAD = FT < 2 ? FT : 2;  // feature tiles whose K^T waits in registers
-      Operand<T, 1> kc[AHEAD][2];
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) kc[i][s] = Keys::columns(keys, s, 16 * (TILES < 4 ? w & 1 : w + 4 * i));
-#pragma unroll
-      for (int i = 0; i < FT; ++i)
-        if (w + 4 * i < TILES) {
-          const f32x4 add = *reinterpret_cast<const f32x4*>(lds.qdo + 256 * (w + 4 * i) + 4 * lane);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) dh[i][r] = gam * dh[i][r] + add[r];
-        }
-      f32x4 y;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) y[r] = -(beta[r] * dr[r] * eps[r]);
-      F::template put_tile<false>(lds.dread, w, y);
-      record(rec_dr, chunk0 + ci, 4 * slices).put(4 * sl + w, dr);
-      lds_barrier();
-      // dH = gam dH' + Q^T (eps dO) - K^T (beta eps dR)
-      const Operand<T, NT> y0 = F::get(lds.dread, 0), y1 = F::get(lds.dread, 1);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < FT; ++i) {
-        const int ft = w + 4 * i;
-        if (ft < TILES) {
-          if (i >= AHEAD) {
-            dh[i] = mma(Keys::columns(keys, 0, 16 * ft), y0, dh[i]);
-            dh[i] = mma(Keys::columns(keys, 1, 16 * ft), y1, dh[i]);
-          } else {
-            dh[i] = mma(kc[i < AHEAD ? i : 0][0], y0, dh[i]);
-            dh[i] = mma(kc[i < AHEAD ? i : 0][1], y1, dh[i]);
+          for (int s = 0; s < 2 && s0 + s < KS; ++s) {
+            kr[s] = Keys::row(keys, 16 * w + c, 32 * (s0 + s) + 8 * grp);
+            st[s] = F::get(lds.state, s0 + s);
           }
-          F::template put_tile<true>(lds.state, ft, dh[i]);
+          __builtin_amdgcn_sched_barrier(0);  // reads together, not one by one before its product
+#pragma unroll
+          for (int s = 0; s < 2 && s0 + s < KS; ++s) x = mma(kr[s], st[s], x);
         }
+        const f32x4 kap = *reinterpret_cast<const f32x4*>(co + 2 * kChunk + own);
+        const f32x4 z = *reinterpret_cast<const f32x4*>(lds.z + 256 * w + 4 * lane);
+        const Record rh = record(rec_dh, chunk0 + ci, slices * slices);
+#pragma unroll
+        for (int i = 0; i < FT; ++i)
+          if (w + 4 * i < slices) rh.put(sl * slices + w + 4 * i, dh[i]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = kap[r] * x[r] + z[r];
+        F::template put_tile<false>(lds.ddelta, w, x);
+        lds_barrier();
+        // dR = T^T dDelta; the next chunk's T, K^T and Q^T (eps dO) on the way
+        Operand<T, NT> d0;
+        if constexpr (BOTH) d0 = F::get(lds.ddelta, 0);
+        const Operand<T, NT> d1 = F::get(lds.ddelta, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        load(it + 1, next);
+        f32x4 dr = mma(tin.t[1], d1, zero4());
+        if constexpr (BOTH) dr = mma(tin.t[0], d0, dr);
+        const f32x4 beta = *reinterpret_cast<const f32x4*>(co + own);
+        const f32x4 eps = *reinterpret_cast<const f32x4*>(co + kChunk + own);
+        const float gam = co[2 * kChunk - 1];
+        constexpr int AHEAD = FT < 2 ? FT : 2;  // feature tiles whose K^T waits in registers
+        Operand<T, 1> kc[AHEAD][2];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) kc[i][s] = Keys::columns(keys, s, 16 * (TILES < 4 ? w & 1 : w + 4 * i));
+#pragma unroll
+        for (int i = 0; i < FT; ++i)
+          if (w + 4 * i < TILES) {
+            const f32x4 add = *reinterpret_cast<const f32x4*>(lds.qdo + 256 * (w + 4 * i) + 4 * lane);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dh[i][r] = gam * dh[i][r] + add[r];
+          }
+        f32x4 y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = -(beta[r] * dr[r] * eps[r]);
+        F::template put_tile<false>(lds.dread, w, y);
+        record(rec_dr, chunk0 + ci, 4 * slices).put(4 * sl + w, dr);
+        lds_barrier();
+        // dH = gam dH' + Q^T (eps dO) - K^T (beta eps dR)
+        const Operand<T, NT> y0 = F::get(lds.dread, 0), y1 = F::get(lds.dread, 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FT; ++i) {
+          const int ft = w + 4 * i;
+          if (ft < TILES) {
+            if (i >= AHEAD) {
+              dh[i] = mma(Keys::columns(keys, 0, 16 * ft), y0, dh[i]);
+              dh[i] = mma(Keys::columns(keys, 1, 16 * ft), y1, dh[i]);
+            } else {
+              dh[i] = mma(kc[i < AHEAD ? i : 0][0], y0, dh[i]);
+              dh[i] = mma(kc[i < AHEAD ? i : 0][1], y1, dh[i]);
+            }
+            F::template put_tile<true>(lds.state, ft, dh[i]);
+          }
+        }
+        lds_barrier();
+      };
+      for (int it = 0; it < nc; it += 2) {
+        step(it, ta, tb);
+        if (it + 1 < nc) step(it + 1, tb, ta);
       }
-      lds_barrier();
-    };
-    for (int it = 0; it < nc; it += 2) {
-      step(it, ta, tb);
-      if (it + 1 < nc) step(it + 1, tb, ta);
-    }
     };
     if (w < 2) run(std::true_type{});
     else run(std::false_type{});
@@ -259,115 +259,115 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
       }
     };
     auto run = [&](auto both) {  // as in the chain
-    constexpr bool BOTH = decltype(both)::value;
-    auto load = [&](int it, BackIn<T>& in) {
-      const int ci = chunk_of(it);
-      const T* pb = pp + (size_t)ci * Factor<T, NT>::kElems;
-      if constexpr (BOTH) in.pf[0] = F::get(pb, 0);
-      in.pf[1] = F::get(pb, BOTH ? 1 : 0);
-      in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, ci * kChunk), lane, 0, 0);
-    };
-    f32x4 x[4];  // dO as accumulator tiles (rows tokens), zero where inactive
-    auto read_do = [&](const BackIn<T>& in, auto slot) {
-      const uint64_t on = active == nullptr ? ~0ull : __builtin_amdgcn_ballot_w64(in.on != 0);
+      constexpr bool BOTH = decltype(both)::value;
+      auto load = [&](int it, BackIn<T>& in) {
+        const int ci = chunk_of(it);
+        const T* pb = pp + (size_t)ci * Factor<T, NT>::kElems;
+        if constexpr (BOTH) in.pf[0] = F::get(pb, 0);
+        in.pf[1] = F::get(pb, BOTH ? 1 : 0);
+        in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, ci * kChunk), lane, 0, 0);
+      };
+      f32x4 x[4];  // dO as accumulator tiles (rows tokens), zero where inactive
+      auto read_do = [&](const BackIn<T>& in, auto slot) {
+        const uint64_t on = active == nullptr ? ~0ull : __builtin_amdgcn_ballot_w64(in.on != 0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[j] = Slice::four(lds.d_o[decltype(slot)::value], j, 0);
+        for (int j = 0; j < 4; ++j) {
+          x[j] = Slice::four(lds.d_o[decltype(slot)::value], j, 0);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[j][r] = (on >> (16 * j + 4 * grp + r)) & 1 ? x[j][r] : 0.f;
-      }
-    };
-    auto form_z = [&](const BackIn<T>& in) {
-      f32x4 z = mma(in.pf[1], paired<T, 1>(x[2], x[3]), zero4());
-      if constexpr (BOTH) z = mma(in.pf[0], paired<T, 1>(x[0], x[1]), z);
-      *reinterpret_cast<f32x4*>(lds.z + 256 * w + 4 * lane) = z;
-    };
-    auto form_qdo = [&](int it, auto slot, const float* co) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 eps = *reinterpret_cast<const f32x4*>(co + kChunk + 16 * j + 4 * grp);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[j][r] *= eps[r];
-      }
-      const Operand<T, NT> e0 = paired<T, NT>(x[0], x[1]), e1 = paired<T, NT>(x[2], x[3]);
-#pragma unroll
-      for (int i = 0; i < FT; ++i) {
-        const int ft = w + 4 * i;
-        if (ft < TILES) {
-          f32x4 y;
-          if constexpr (S::kStageQ) {
-            y = mma(Keys::columns(lds.queries[decltype(slot)::value % QRING], 0, 16 * ft), e0, zero4());
-            y = mma(Keys::columns(lds.queries[decltype(slot)::value % QRING], 1, 16 * ft), e1, y);
-          } else {
-            const int ci = chunk_of(it);
-            const Rows<T> rows = dims.rows_at(qp + ci * stride, ci);
-            Operand<T, 1> qc[2];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                qc[s].lo[e] = rows.one(32 * s + 4 * grp + e, 16 * ft + c);
-                qc[s].hi[e] = rows.one(32 * s + 16 + 4 * grp + e, 16 * ft + c);
-              }
-            y = mma(qc[0], e0, zero4());
-            y = mma(qc[1], e1, y);
-          }
-          *reinterpret_cast<f32x4*>(lds.qdo + 256 * ft + 4 * lane) = y;
+          for (int r = 0; r < 4; ++r) x[j][r] = (on >> (16 * j + 4 * grp + r)) & 1 ? x[j][r] : 0.f;
         }
-      }
-    };
-    constexpr std::integral_constant<int, 0> even{};
-    constexpr std::integral_constant<int, 1> odd{};
-    BackIn<T> in;
-    int free = LEAD, c1 = 1, c2 = 2;  // the slots of the keys of chunk it + LEAD, of the coefficients of it + 1 and it + 2
-    auto step = [&](int it, auto mine, auto other) {  // `mine` is it's parity
-      if constexpr (LEAD == 0) {
-        stage(it, 0);
-        stage_q(it + 1, other);
-        stage_do(it + 2, mine, it + 2, c2);
-        direct_loads_done();
-        lds_barrier();
-      }
-      read_do(in, other);
-      if constexpr (LEAD > 0) {
-        stage_q(it + 2, mine);
-        stage(it + LEAD, free);
-      }
-      lds_barrier();
-      if constexpr (LEAD > 0) stage_do(it + 3, other, it + 2, c2);
-      form_z(in);
-      direct_loads_done<LEAD == 0 ? 0 : S::kLoads>();
-      lds_barrier();
-      load(it + 2, in);
-      form_qdo(it + 1, other, lds.coef[c1]);
-      free = free + 1 < RING ? free + 1 : 0;
-      c1 = c2;
-      c2 = c2 + 1 < 3 ? c2 + 1 : 0;
-      lds_barrier();
-    };
+      };
+      auto form_z = [&](const BackIn<T>& in) {
+        f32x4 z = mma(in.pf[1], paired<T, 1>(x[2], x[3]), zero4());
+        if constexpr (BOTH) z = mma(in.pf[0], paired<T, 1>(x[0], x[1]), z);
+        *reinterpret_cast<f32x4*>(lds.z + 256 * w + 4 * lane) = z;
+      };
+      auto form_qdo = [&](int it, auto slot, const float* co) {
 #pragma unroll
-    for (int it = 0; it < LEAD; ++it) stage(it, it);
-    stage_q(0, even);
-    stage_do(0, even, 0, 0);
-    stage_do(1, odd, 1, 1);
-    load(0, in);
-    direct_loads_done();
-    lds_barrier();
-    read_do(in, even);
-    form_z(in);
-    load(1, in);
-    form_qdo(0, even, lds.coef[0]);
-    lds_barrier();
-    if constexpr (LEAD > 0) {
-      stage_q(1, odd);
-      stage_do(2, even, 1, 1);
-    }
-    direct_loads_done();
-    lds_barrier();
-    for (int it = 0; it < nc; it += 2) {
-      step(it, even, odd);
-      if (it + 1 < nc) step(it + 1, odd, even);
-    }
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 eps = *reinterpret_cast<const f32x4*>(co + kChunk + 16 * j + 4 * grp);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[j][r] *= eps[r];
+        }
+        const Operand<T, NT> e0 = paired<T, NT>(x[0], x[1]), e1 = paired<T, NT>(x[2], x[3]);
+#pragma unroll
+        for (int i = 0; i < FT; ++i) {
+          const int ft = w + 4 * i;
+          if (ft < TILES) {
+            f32x4 y;
+            if constexpr (S::kStageQ) {
+              y = mma(Keys::columns(lds.queries[decltype(slot)::value % QRING], 0, 16 * ft), e0, zero4());
+              y = mma(Keys::columns(lds.queries[decltype(slot)::value % QRING], 1, 16 * ft), e1, y);
+            } else {
+              const int ci = chunk_of(it);
+              const Rows<T> rows = dims.rows_at(qp + ci * stride, ci);
+              Operand<T, 1> qc[2];
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  qc[s].lo[e] = rows.one(32 * s + 4 * grp + e, 16 * ft + c);
+                  qc[s].hi[e] = rows.one(32 * s + 16 + 4 * grp + e, 16 * ft + c);
+                }
+              y = mma(qc[0], e0, zero4());
+              y = mma(qc[1], e1, y);
+            }
+            *reinterpret_cast<f32x4*>(lds.qdo + 256 * ft + 4 * lane) = y;
+          }
+        }
+      };
+      constexpr std::integral_constant<int, 0> even{};
+      constexpr std::integral_constant<int, 1> odd{};
+      BackIn<T> in;
+      int free = LEAD, c1 = 1, c2 = 2;  // the slots of the keys of chunk it + LEAD, of the coefficients of it + 1 and it + 2
+      auto step = [&](int it, auto mine, auto other) {  // `mine` is it's parity
+        if constexpr (LEAD == 0) {
+          stage(it, 0);
+          stage_q(it + 1, other);
+          stage_do(it + 2, mine, it + 2, c2);
+          direct_loads_done();
+          lds_barrier();
+        }
+        read_do(in, other);
+        if constexpr (LEAD > 0) {
+          stage_q(it + 2, mine);
+          stage(it + LEAD, free);
+        }
+        lds_barrier();
+        if constexpr (LEAD > 0) stage_do(it + 3, other, it + 2, c2);
+        form_z(in);
+        direct_loads_done<LEAD == 0 ? 0 : S::kLoads>();
+        lds_barrier();
+        load(it + 2, in);
+        form_qdo(it + 1, other, lds.coef[c1]);
+        free = free + 1 < RING ? free + 1 : 0;
+        c1 = c2;
+        c2 = c2 + 1 < 3 ? c2 + 1 : 0;
+        lds_barrier();
+      };
+#pragma unroll
+      for (int it = 0; it < LEAD; ++it) stage(it, it);
+      stage_q(0, even);
+      stage_do(0, even, 0, 0);
+      stage_do(1, odd, 1, 1);
+      load(0, in);
+      direct_loads_done();
+      lds_barrier();
+      read_do(in, even);
+      form_z(in);
+      load(1, in);
+      form_qdo(0, even, lds.coef[0]);
+      lds_barrier();
+      if constexpr (LEAD > 0) {
+        stage_q(1, odd);
+        stage_do(2, even, 1, 1);
+      }
+      direct_loads_done();
+      lds_barrier();
+      for (int it = 0; it < nc; it += 2) {
+        step(it, even, odd);
+        if (it + 1 < nc) step(it + 1, odd, even);
+      }
     };
     if (w < 2) run(std::true_type{});
     else run(std::false_type{});

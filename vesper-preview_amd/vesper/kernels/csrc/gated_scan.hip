@@ -303,12 +303,24 @@ template <typename T, int DP> struct OutIn {
   uint8_t on;
 };
 
-template <typename T, int DP, bool RECORD>
+// Few long rows leave most CUs without a chain: their sequence is walked in segments. What a segment makes of its starting
+// state is affine, H' = M H + U. A first launch walks all segments but the last from zero (its end is U) and, without
+// values, from the identity (M), gated_join_kernel carries the state from segment to segment, and a second launch walks
+// each from its start: three times the work, on all CUs. Whole and in segments, prep and all, in us (bf16): B1 T8191 H12 d64
+// 137 and 98, T4096 H2 d64 68 and 42, T4096 H16 d64 75 and 65, T2048 H8 d64 43 and 40, T4096 H2 d256 157 and 142.
+struct Segments {
+  int count, chunks;    // segments a row and head, chunks a segment
+  const float* states;  // the starting states of the second one and on, [B H][count - 1][D][D]
+  float* maps;          // U and M, [B H][count - 1][2][D][D]
+};
+enum Walk { kOutputs, kRecords, kMaps };  // outputs; outputs and records (of one segment); only the end state, into maps
+
+template <typename T, int DP, Walk WALK>
 __global__ __launch_bounds__(512) void gated_chain_kernel(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const float* __restrict__ coef,
     const T* __restrict__ tf, const T* __restrict__ pf, const float* __restrict__ s_in, T* __restrict__ o,
     float* __restrict__ s_out, const uint8_t* __restrict__ active, float* __restrict__ rec_h, float* __restrict__ rec_d,
-    Dims<T> dims, int slices) {
+    Dims<T> dims, int slices, Segments segs) {
   using S = ChainShape<T, DP>;
   using F = typename S::F;
   using FO = typename S::FO;
@@ -318,11 +330,14 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
   __shared__ __attribute__((aligned(16))) typename S::Lds lds;
 
   const int id = xcd_logical_block(blockIdx.x, gridDim.x);
-  const int sl = id % slices, bh = id / slices, h = bh % dims.H, b = bh / dims.H;
-  const int D = dims.D, nc = dims.chunks;
+  const int sl = id % slices, walks = WALK == kMaps ? 2 * (segs.count - 1) : segs.count, walk = id / slices % walks;
+  const int seg = WALK == kMaps ? walk / 2 : walk, bh = id / slices / walks, h = bh % dims.H, b = bh / dims.H;
+  const bool map = WALK == kMaps && walk % 2 == 1;  // M's columns
+  // the walk's chunks: nc from chunk `from` on
+  const int D = dims.D, from = seg * segs.chunks, nc = dims.chunks - from < segs.chunks ? dims.chunks - from : segs.chunks;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
   const int c = lane_col(), grp = lane_grp();
-  const size_t chunk0 = (size_t)bh * nc;
+  const size_t chunk0 = (size_t)bh * dims.chunks + from;
 
   // features past D and rows past the end are not brought: zeros, and what an earlier chunk left there, times zeros
   for (int i = threadIdx.x; i < (int)(sizeof(lds.ring) / 16); i += 512) reinterpret_cast<f32x4*>(lds.ring)[i] = zero4();
@@ -341,14 +356,15 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
     ChainIn<T> ta, tb;
     load(0, ta);
     f32x4 hs[FT];
-    const float* sp = s_in + (size_t)bh * D * D;
+    const float* sp = seg == 0 ? s_in + (size_t)bh * D * D : segs.states + ((size_t)bh * (segs.count - 1) + seg - 1) * D * D;
 #pragma unroll
     for (int i = 0; i < FT; ++i) {
       const int ft = w + 4 * i;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int f = 16 * ft + 4 * grp + r;
-        hs[i][r] = f < D && vcol < D ? sp[(size_t)f * D + vcol] : 0.f;
+        if constexpr (WALK == kMaps) hs[i][r] = map && f == vcol && f < D ? 1.f : 0.f;
+        else hs[i][r] = f < D && vcol < D ? sp[(size_t)f * D + vcol] : 0.f;
       }
       if (ft < TILES) F::template put_tile<true>(lds.state, ft, hs[i]);
     }
@@ -375,8 +391,8 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
       }
       const f32x4 beta = *reinterpret_cast<const f32x4*>(in.coef + own);
       const f32x4 eps = *reinterpret_cast<const f32x4*>(in.coef + kChunk + own);
-      const f32x4 vx = Slice::four(in.values, w, 0);
-      if constexpr (RECORD) {
+      const f32x4 vx = map ? zero4() : Slice::four(in.values, w, 0);
+      if constexpr (WALK == kRecords) {
         const Record rh = record(rec_h, chunk0 + ci, slices * slices);
 #pragma unroll
         for (int i = 0; i < FT; ++i)
@@ -408,7 +424,7 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
 #pragma unroll
       for (int r = 0; r < 4; ++r) kd[r] = kap[r] * dl[r];
       F::template put_tile<false>(lds.kept, w, kd);
-      if constexpr (RECORD) record(rec_d, chunk0 + ci, 4 * slices).put(4 * sl + w, dl);
+      if constexpr (WALK == kRecords) record(rec_d, chunk0 + ci, 4 * slices).put(4 * sl + w, dl);
       lds_barrier();
       // H' = gam H + K^T (kap Delta)
       const Operand<T, NT> k0 = F::get(lds.kept, 0), k1 = F::get(lds.kept, 1);
@@ -433,7 +449,8 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
       step(ci, ta, tb);
       if (ci + 1 < nc) step(ci + 1, tb, ta);
     }
-    float* so = s_out + (size_t)bh * D * D;
+    if (WALK != kMaps && seg + 1 < segs.count) return;  // the next segment's start is there already
+    float* so = WALK == kMaps ? segs.maps + (((size_t)bh * (segs.count - 1) + seg) * 2 + map) * D * D : s_out + (size_t)bh * D * D;
 #pragma unroll
     for (int i = 0; i < FT; ++i)
 #pragma unroll
@@ -449,15 +466,16 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
     //      issues kLoads direct loads a chunk, after its other loads and unconditionally, so that a wait can leave those of
     //      one chunk in flight; past the end they bring the last chunk again ----
     const size_t stride = (size_t)kChunk * dims.H * D;  // elements from a chunk's rows to the next one's
-    const T *kp = k + dims.at(b, 0, h), *vp = v + dims.at(b, 0, h), *qp = q + dims.at(b, 0, h);
-    T* op = o + dims.at(b, 0, h);
+    const size_t at = dims.at(b, from * kChunk, h);
+    const T *kp = k + at, *vp = v + at, *qp = q + at;
+    T* op = o + at;
     const T* pp = pf + chunk0 * Factor<T, NO>::kElems + row_step(w, 0) * FO::kStep;
     const float* cp = coef + chunk0 * kCoefAll;
     auto within = [&](int ci) { return ci < nc ? ci : nc - 1; };
     auto stage = [&](int ahead, int slot) {
       const int ci = within(ahead);
       typename S::Stage& to = lds.ring[slot];
-      const Rows<T> krows = dims.rows_at(kp + ci * stride, ci), vrows = dims.rows_at(vp + ci * stride, ci);
+      const Rows<T> krows = dims.rows_at(kp + ci * stride, from + ci), vrows = dims.rows_at(vp + ci * stride, from + ci);
       const float* co = cp + (size_t)ci * kCoefAll;
 #pragma unroll
       for (int j = 0; j < Keys::kInstr / 4; ++j) Keys::stage(to.keys, krows, 4 * j + w, 0);
@@ -471,14 +489,14 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
     };
     auto load = [&](int ahead, OutIn<T, DP>& in) {
       const int ci = within(ahead);
-      const Rows<T> qrows = dims.rows_at(qp + ci * stride, ci);
+      const Rows<T> qrows = dims.rows_at(qp + ci * stride, from + ci);
 #pragma unroll
       for (int s = 0; s < KS; ++s) in.qf[s] = qrows.row(16 * w + c, 32 * s + 8 * grp);
       const T* pb = pp + (size_t)ci * Factor<T, NO>::kElems;
       in.wf[0] = FO::get(pb, 0);
       in.wf[1] = FO::get(pb, w >= 2 ? 1 : 0);
       in.eps = cp[(size_t)ci * kCoefAll + kChunk + 16 * w + c];
-      in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, ci * kChunk), 16 * w + c, 0, 0);
+      in.on = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(dims.flags(active, b, (from + ci) * kChunk), 16 * w + c, 0, 0);
     };
     int free = LEAD == 0 ? 0 : RING - 1;  // the slot of the chunk LEAD ahead
     auto step = [&](int ci, const OutIn<T, DP>& in, OutIn<T, DP>& next) {
@@ -486,6 +504,15 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
         stage(ci, 0);
         direct_loads_done();
         lds_barrier();
+      }
+      if constexpr (WALK == kMaps) {
+        lds_barrier();
+        lds_barrier();
+        if constexpr (LEAD > 0) stage(ci + LEAD, free);
+        direct_loads_done<LEAD == 0 ? 0 : S::kLoads>();
+        free = free + 1 < RING ? free + 1 : 0;
+        lds_barrier();
+        return;
       }
       f32x4 acc = zero4();
 #pragma unroll
@@ -510,14 +537,14 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
       lds_barrier();
       if constexpr (LEAD > 0) stage(ci + LEAD, free);
       direct_loads_done<LEAD == 0 ? 0 : S::kLoads>();
-      dims.rows_at(op + ci * stride, ci).put_four(16 * w + c, 16 * sl + 4 * grp, acc);
+      dims.rows_at(op + ci * stride, from + ci).put_four(16 * w + c, 16 * sl + 4 * grp, acc);
       free = free + 1 < RING ? free + 1 : 0;
       lds_barrier();
     };
     OutIn<T, DP> a, bb;
 #pragma unroll
     for (int ci = 0; ci < LEAD; ++ci) stage(ci, ci);
-    load(0, a);
+    if constexpr (WALK != kMaps) load(0, a);
     direct_loads_done();
     lds_barrier();
     for (int ci = 0; ci < nc; ci += 2) {
@@ -526,6 +553,73 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
     }
   }
   direct_loads_done();
+}
+
+// The segments' starting states: H = M H + U, segment by segment, a workgroup a head and 16 value columns; wave w has the
+// feature tiles w, w + 4, ..
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ s_in, float* __restrict__ states, int D,
+                                                         int slices, Segments segs) {
+  using S = ChainShape<T, DP>;
+  using F = typename S::F;
+  constexpr int KS = S::KS, FT = S::FT, TILES = S::TILES, NT = S::NT;
+  __shared__ __attribute__((aligned(16))) T state[KS * F::kStep];
+  const int sl = blockIdx.x % slices, bh = blockIdx.x / slices, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane_col(), grp = lane_grp(), vcol = 16 * sl + c, joins = segs.count - 1;
+  const size_t size = (size_t)D * D;
+  auto read = [&](const float* p, int ft) {
+    f32x4 x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int f = 16 * ft + 4 * grp + r;
+      x[r] = f < D && vcol < D ? p[(size_t)f * D + vcol] : 0.f;
+    }
+    return x;
+  };
+  f32x4 hs[FT];
+#pragma unroll
+  for (int i = 0; i < FT; ++i) hs[i] = read(s_in + bh * size, w + 4 * i);
+  for (int s = 0; s < joins; ++s) {
+    const float* u = segs.maps + ((size_t)bh * joins + s) * 2 * size;
+    const Rows<float> m = {buffer_rsrc(u + size, (unsigned)(size * sizeof(float))), (unsigned)D * 4u, D};
+#pragma unroll
+    for (int i = 0; i < FT; ++i)
+      if (w + 4 * i < TILES) F::template put_tile<true>(state, w + 4 * i, hs[i]);
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < FT; ++i) hs[i] = read(u, w + 4 * i);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const Operand<T, NT> h = F::get(state, k);
+#pragma unroll
+      for (int i = 0; i < FT; ++i) {
+        const Operand<float, 1> x = m.row(16 * (w + 4 * i) + c, 32 * k + 8 * grp);
+        hs[i] = mma(paired<T, NT>(x.lo, x.hi), h, hs[i]);
+      }
+    }
+    float* to = states + ((size_t)bh * joins + s) * size;
+#pragma unroll
+    for (int i = 0; i < FT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int f = 16 * (w + 4 * i) + 4 * grp + r;
+        if (f < D && vcol < D) to[(size_t)f * D + vcol] = hs[i][r];
+      }
+    lds_barrier();
+  }
+}
+
+// Segments a row and head: what the CUs hold at once of either launch (heads of up to 64 two workgroups a CU, wider ones
+// one), 8 chunks each at least, 16 at most (joining them is serial), and no fewer than four.
+int segments_of(int B, int N, int H, int D) {
+  const size_t groups = (size_t)B * H * tiles_of(D);
+  const int chunks = chunks_of(N);
+  if (groups > 64) return 1;
+  const int most = chunks / 8 < 16 ? chunks / 8 : 16, walks = (int)(256 / groups), maps = 1 + (int)((D <= 64 ? 256 : 128) / groups);
+  const int fit = walks < maps ? walks : maps, count = fit < most ? fit : most;
+  if (count < 4) return 1;
+  const int each = (chunks + count - 1) / count;
+  return (chunks + each - 1) / each;
 }
 
 template <typename T, int DP>
@@ -538,23 +632,35 @@ void launch_prep_width(const T* q, const T* k, const T* beta, const float* g, fl
 
 template <typename T, int DP>
 void launch_chain(const T* q, const T* k, const T* v, const float* coef, const T* tf, const T* pf, const float* s_in,
-                  T* o, float* s_out, const uint8_t* active, float* rec_h, float* rec_d, Dims<T> dims, int B,
+                  T* o, float* s_out, const uint8_t* active, float* rec_h, float* rec_d, float* joined, Dims<T> dims, int B,
                   hipStream_t stream) {
-  const int slices = (dims.D + 15) / 16;
-  const dim3 grid((unsigned)(B * dims.H * slices)), block(512);
-  if (rec_h != nullptr)
-    hipLaunchKernelGGL((gated_chain_kernel<T, DP, true>), grid, block, 0, stream, q, k, v, coef, tf, pf, s_in, o, s_out, active,
-                       rec_h, rec_d, dims, slices);
-  else
-    hipLaunchKernelGGL((gated_chain_kernel<T, DP, false>), grid, block, 0, stream, q, k, v, coef, tf, pf, s_in, o, s_out, active,
-                       rec_h, rec_d, dims, slices);
+  const int slices = tiles_of(dims.D), heads = B * dims.H, count = rec_h != nullptr ? 1 : segments_of(B, dims.N, dims.H, dims.D);
+  const dim3 grid((unsigned)(heads * slices * count)), block(512);
+  const size_t floats = (size_t)heads * (count - 1) * dims.D * dims.D;
+  const Segments segs{count, (dims.chunks + count - 1) / count, joined, joined + floats};
+#define VSP_CHAIN(WALK, GRID)                                                                                                     \
+  hipLaunchKernelGGL((gated_chain_kernel<T, DP, WALK>), GRID, block, 0, stream, q, k, v, coef, tf, pf, s_in, o, s_out, active,    \
+                     rec_h, rec_d, dims, slices, segs)
+  if (rec_h != nullptr) {
+    VSP_CHAIN(kRecords, grid);
+    return;
+  }
+  if (count > 1) {
+    VSP_CHAIN(kMaps, dim3((unsigned)(heads * slices * 2 * (count - 1))));
+    hipLaunchKernelGGL((gated_join_kernel<T, DP>), dim3((unsigned)(heads * slices)), dim3(256), 0, stream, s_in, joined, dims.D, slices, segs);
+  }
+  VSP_CHAIN(kOutputs, grid);
+#undef VSP_CHAIN
 }
 
 size_t align16(size_t x) { return (x + 15) & ~(size_t)15; }
 
-// the forward's workspace: coefficients, T and P of every chunk and head
-template <typename T> size_t forward_bytes(size_t total) {
+// the forward's workspace: coefficients, T and W of every chunk and head, and the segments' states and maps
+template <typename T> size_t factor_bytes(size_t total) {
   return align16(total * kCoefAll * sizeof(float)) + total * sizeof(T) * (Factor<T, Pieces<T>::kN>::kElems + Factor<T, OutPieces<T>::kN>::kElems);
+}
+template <typename T> size_t forward_bytes(int B, int N, int H, int D) {
+  return factor_bytes<T>((size_t)B * H * chunks_of(N)) + (size_t)B * H * (segments_of(B, N, H, D) - 1) * 3 * D * D * sizeof(float);
 }
 
 template <typename T>
@@ -568,7 +674,8 @@ int scan(const void* q_, const void* k_, const void* v_, const void* beta_, cons
   if ((reinterpret_cast<uintptr_t>(q_) | reinterpret_cast<uintptr_t>(k_) | reinterpret_cast<uintptr_t>(v_) |
        reinterpret_cast<uintptr_t>(o_) | reinterpret_cast<uintptr_t>(ws) | reinterpret_cast<uintptr_t>(records)) & 15)
     return fail(ERR_ARG, "%s: q, k, v, o, the workspace and the records must be 16-byte aligned", who);
-  if (ws_bytes < forward_bytes<T>(total)) return fail(ERR_ARG, "%s: workspace of %zu bytes, needs %zu", who, ws_bytes, forward_bytes<T>(total));
+  if (ws_bytes < forward_bytes<T>(B, N, H, D))
+    return fail(ERR_ARG, "%s: workspace of %zu bytes, needs %zu", who, ws_bytes, forward_bytes<T>(B, N, H, D));
   if (records != nullptr && records_bytes < record_bytes(total, D))
     return fail(ERR_ARG, "%s: records of %zu bytes, need %zu", who, records_bytes, record_bytes(total, D));
   const T *q = static_cast<const T*>(q_), *k = static_cast<const T*>(k_), *v = static_cast<const T*>(v_);
@@ -579,12 +686,13 @@ int scan(const void* q_, const void* k_, const void* v_, const void* beta_, cons
   T* pf = tf + total * Factor<T, Pieces<T>::kN>::kElems;
   const Dims<T> dims{N, H, D, chunks_of(N)};
   if (const int st = launch_prep<T>(q, k, beta, g, coef, tf, pf, B, N, H, D, false, stream); st != OK) return st;
+  float* joined = reinterpret_cast<float*>(static_cast<char*>(ws) + factor_bytes<T>(total));
   float* rec_d = records == nullptr ? nullptr : records + state_floats(total, D);
   switch (width_of(D)) {
-    case 32: launch_chain<T, 32>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, dims, B, stream); break;
-    case 64: launch_chain<T, 64>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, dims, B, stream); break;
-    case 128: launch_chain<T, 128>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, dims, B, stream); break;
-    default: launch_chain<T, 256>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, dims, B, stream); break;
+    case 32: launch_chain<T, 32>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, joined, dims, B, stream); break;
+    case 64: launch_chain<T, 64>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, joined, dims, B, stream); break;
+    case 128: launch_chain<T, 128>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, joined, dims, B, stream); break;
+    default: launch_chain<T, 256>(q, k, v, coef, tf, pf, s_in, o, s_out, active, records, rec_d, joined, dims, B, stream); break;
   }
   return check_launch(who);
 }
@@ -625,8 +733,7 @@ int check_sizes(int B, int N, int H, int D, const char* who) {
 extern "C" size_t vsp_gated_scan_workspace_bytes(int B, int N, int H, int D, int fp32) {
   using namespace vsp::gated;
   if (B <= 0 || N <= 0 || H <= 0 || D <= 0) return 0;
-  const size_t total = (size_t)B * H * chunks_of(N);
-  return fp32 ? forward_bytes<float>(total) : forward_bytes<__bf16>(total);
+  return fp32 ? forward_bytes<float>(B, N, H, D) : forward_bytes<__bf16>(B, N, H, D);
 }
 
 extern "C" size_t vsp_gated_scan_records_bytes(int B, int N, int H, int D) {
