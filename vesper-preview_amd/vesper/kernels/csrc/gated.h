@@ -6,7 +6,7 @@
 // A chunk of C = 64 tokens with G_i = g_1 + .. + g_i, eps_i = e^{G_i}, E_ij = e^{G_i - G_j} (j <= i),
 // kap_j = e^{G_C - G_j}, gam = e^{G_C}, A_ij = beta_i E_ij k_i.k_j (j < i), T = (I + A)^-1,
 // P_ij = E_ij q_i.k_j:
-//   R_i = beta_i (v_i - eps_i H^T k_i),  Delta = T R,  O_i = eps_i H^T q_i + sum_j P_ij Delta_j,
+//   R_i = beta_i (v_i - eps_i H^T k_i),  Delta = T R,  O_i = eps_i H^T q_i + sum_j W_ij R_j with W = P T,
 //   H' = gam H + sum_j kap_j k_j Delta_j^T.
 // Every exponent is at most zero where g is, so nothing overflows however far a state decays. The sums
 // G and their differences are in float64: behind a token that forgets (g of -inf counts as -1e4, whose
@@ -276,7 +276,7 @@ __device__ __forceinline__ Operand<T, 1> load_columns(const T* tile, int pitch, 
   return o;
 }
 
-// ---- operands in LDS or memory: a step's pieces one after the other, a piece 16 bytes a lane (float32: the eight values in
+// ---- operands in LDS or in the workspace: a step's pieces one after the other, a piece 16 bytes a lane (float32: the eight values in
 // two planes of four) ----
 template <typename T, int NP> struct Frags {
   static constexpr int kStep = sizeof(T) == 2 ? NP * 512 : 512;  // elements of a step
@@ -319,12 +319,6 @@ template <typename T, int NP> struct Frags {
     }
     return o;
   }
-  // instruction j of `steps` steps straight into LDS: 1 KiB each
-  static constexpr int kStepInstr = kStep * (int)sizeof(T) / 1024;
-  __device__ __forceinline__ static void stage(T* dst, const T* src, int steps, int j) {
-    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(src, (unsigned)(steps * kStep * sizeof(T)));
-    buffer_load_lds16(r, dst + j * (1024 / (int)sizeof(T)), 16 * (threadIdx.x & 63) + 1024 * j, 0);
-  }
 };
 
 // The six operand steps that cover a lower triangle of 4 x 4 tiles. By rows i (the sums run over j <= i): steps
@@ -345,7 +339,7 @@ template <typename T, int NP> struct Factor {  // elements of a triangular facto
 };
 template <typename T> struct Pieces { static constexpr int kN = kPieces; };
 template <> struct Pieces<float> { static constexpr int kN = 1; };
-// pieces of H, Delta and P in the outputs' products: with one of P, heads of width 16 were off by 2.8e-3 (1.7e-3 is the
+// pieces of H, R and W in the outputs' products: with one, heads of width 16 were off by 2.8e-3 (1.7e-3 is the
 // rounding of the outputs alone)
 template <typename T> struct OutPieces { static constexpr int kN = 2; };
 template <> struct OutPieces<float> { static constexpr int kN = 1; };

@@ -74,6 +74,12 @@ __device__ __forceinline__ void put_line(T* out, int a, const f32x4 (&x)[4]) {
   }
 }
 
+// Bound by its own arithmetic and its latency, not by memory: of a wave's 20 to 27 thousand cycles alone on its SIMD the 80
+// decays a lane take 2500, the substitution 2700, the 144 float32 MFMAs of T and W and their splitting 7000, the loads and
+// the decays' sums 5000, and three waves a SIMD share them. B8 T4096 H8 d64 (160 MB in and out) 47 us, B1 T8191 H12 18, 64
+// chunks of float32 13. Tried: four waves a chunk, a line of T and W each, whose tiles of A passed by LDS (128 chunks 8 us
+// instead of 11, but 51 and 21 for the large ones: each wave inverts a diagonal tile, where one wave has all four in its 64
+// lanes); four waves a SIMD (61: the registers spill).
 // COLS, for the backward pass: the factors T and P by columns, with accumulator rows i and columns j. Else T and
 // W = P T by rows, transposed: rows j, columns i. With X the diagonal tiles' inverses (I + A_bb)^-1, tile by tile:
 //   T_ij = -X_i sum_k A_ik T_kj (k = j .. i - 1), or transposed T_ij^T = -X_j^T sum_k A_kj^T T_ik^T (k = j + 1 .. i);
@@ -303,6 +309,13 @@ template <typename T, int DP> struct OutIn {
   uint8_t on;
 };
 
+// A chunk is three dependent products and three barriers, about 2300 cycles: K H 800 (of it 120 the barrier), T R 850, K^T
+// Delta 500, in each the reads of the operands from LDS, the MFMAs of the pieces, and the split of the result into pieces. So
+// the time is the chunks' number times 0.9 us (B1 T8191 H12 d64, 48 workgroups) to 1.3 us (B8 T4096 H8 d64, 256 of them: 94 us;
+// the clock falls to 2.1 GHz, and one XCD is slower by a fifth). With records the writes bound it: B16 T1024 H12 d64 52 us
+// without and 96 with them (290 MB, past what the 256 MB cache behind the L2s holds). What brought it there, at B1: operands
+// in pieces through LDS between four waves instead of all in one wave's registers (208 us), direct loads into LDS (150), W
+// for the outputs, T into registers, two chunks ahead, loads spread over the spans, reads issued together (118).
 // Few long rows leave most CUs without a chain: their sequence is walked in segments. What a segment makes of its starting
 // state is affine, H' = M H + U. A first launch walks all segments but the last from zero (its end is U) and, without
 // values, from the identity (M), gated_join_kernel carries the state from segment to segment, and a second launch walks
@@ -462,9 +475,9 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
     // ---- memory into LDS ahead, and the outputs: O^T tile of the 16 tokens w (rows values, columns tokens). In a chunk's
     //      three spans: H^T Q^T and this wave's operands of the next chunk; W R, while the chain loads its T; of the chunk
     //      LEAD ahead keys, values and coefficients, and the outputs' store: the loads are spread, for a CU takes 64 bytes a
-    //      cycle and who issues waits for its turn. Every wave
-    //      issues kLoads direct loads a chunk, after its other loads and unconditionally, so that a wait can leave those of
-    //      one chunk in flight; past the end they bring the last chunk again ----
+    //      cycle and who issues waits for its turn. Every wave issues kLoads direct loads a chunk, after its other loads and
+    //      unconditionally, so that a wait can leave those of one chunk in flight; past the end they bring the last chunk
+    //      again ----
     const size_t stride = (size_t)kChunk * dims.H * D;  // elements from a chunk's rows to the next one's
     const size_t at = dims.at(b, from * kChunk, h);
     const T *kp = k + at, *vp = v + at, *qp = q + at;
@@ -556,7 +569,7 @@ __global__ __launch_bounds__(512) void gated_chain_kernel(
 }
 
 // The segments' starting states: H = M H + U, segment by segment, a workgroup a head and 16 value columns; wave w has the
-// feature tiles w, w + 4, ..
+// feature tiles w, w + 4, .. Serial: about 2 us a segment (the maps come from another XCD's L2).
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ s_in, float* __restrict__ states, int D,
                                                          int slices, Segments segs) {
