@@ -17,6 +17,7 @@ float32 inputs run float32 MFMA.
 
 from __future__ import annotations
 
+import functools
 from typing import Any
 
 import torch
@@ -31,6 +32,14 @@ GATE_DTYPE = torch.float32  # the log decays: sums of many of them decide what i
 INPUT_DTYPES = (torch.bfloat16, torch.float32)  # of q, k, v and beta, all alike
 _SUFFIX = {torch.bfloat16: "bf16", torch.float32: "f32"}
 _STEP = {dtype: f"vsp_gated_step_{suffix}" for dtype, suffix in _SUFFIX.items()}
+_SCAN = {dtype: f"vsp_gated_scan_{suffix}" for dtype, suffix in _SUFFIX.items()}
+_SCAN_BACKWARD = {dtype: f"vsp_gated_scan_backward_{suffix}" for dtype, suffix in _SUFFIX.items()}
+
+
+@functools.lru_cache(maxsize=256)
+def _bytes(what: str, *sizes: int) -> int:
+    """A size that the library gives for sizes: the workspaces' and the records'."""
+    return int(getattr(_lib.library(), f"vsp_gated_scan_{what}_bytes")(*sizes))
 
 
 def _check(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor, lead: tuple[str, ...]) -> Dims:
@@ -67,11 +76,10 @@ def _forward(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Te
     """The scan of contiguous, aligned tensors at a width that is a multiple of 8."""
     b, n, h, dk = q.shape
     o, s_out = torch.empty_like(q), torch.empty_like(state)
-    fp32 = q.dtype == torch.float32
-    ws_bytes = int(_lib.library().vsp_gated_scan_workspace_bytes(b, n, h, dk, int(fp32)))
+    ws_bytes = _bytes("workspace", b, n, h, dk, int(q.dtype == torch.float32))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     with _lib.on_device(q.device):
-        _lib.call(f"vsp_gated_scan_{_SUFFIX[q.dtype]}", q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(),
+        _lib.call(_SCAN[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(),
                   g.data_ptr(), state.data_ptr(), o.data_ptr(), s_out.data_ptr(), ws.data_ptr(), ws_bytes,
                   _lib.ptr(records), 0 if records is None else records.numel(), _lib.ptr(mask), b, n, h, dk,
                   _lib.stream_of(q.device))
@@ -83,33 +91,43 @@ class _GatedScan(torch.autograd.Function):
     def forward(ctx: Any, q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor,
                 mask: Tensor | None) -> tuple[Tensor, Tensor]:  # noqa: D102
         ctx.set_materialize_grads(False)
-        q, k, v, beta, g, state = (_aligned(t.detach()) for t in (q, k, v, beta, g, state))
+        q, k, v, beta, g, state = _aligned(q), _aligned(k), _aligned(v), _aligned(beta), _aligned(g), _aligned(state)
         # each chunk's starting state and its Delta, for the backward
-        nrec = int(_lib.library().vsp_gated_scan_records_bytes(*q.shape))
-        records = torch.empty(nrec, dtype=torch.uint8, device=q.device)
+        records = torch.empty(_bytes("records", *q.shape), dtype=torch.uint8, device=q.device)
         o, s_out = _forward(q, k, v, beta, g, state, mask, records)
-        ctx.save_for_backward(q, k, v, beta, g, records, *(() if mask is None else (mask,)))
+        if mask is None:
+            ctx.save_for_backward(q, k, v, beta, g, records)
+        else:
+            ctx.save_for_backward(q, k, v, beta, g, records, mask)
         return o, s_out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, d_o: Tensor | None, d_state: Tensor | None) -> tuple[Tensor | None, ...]:  # noqa: D102
-        q, k, v, beta, g, records, *rest = ctx.saved_tensors
-        b, n, h, dk = q.shape
-        go = torch.zeros_like(q) if d_o is None else _aligned(d_o.to(q.dtype))
-        gs = None if d_state is None else _aligned(d_state.to(STATE_DTYPE))
-        dq, dk_, dv, db, dg = (torch.empty_like(t) for t in (q, k, v, beta, g))
-        d_state_in = torch.empty((b, h, dk, dk), dtype=STATE_DTYPE, device=q.device)
-        fp32 = q.dtype == torch.float32
-        ws_bytes = int(_lib.library().vsp_gated_scan_backward_workspace_bytes(b, n, h, dk, int(fp32)))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-        with _lib.on_device(q.device):
-            _lib.call(f"vsp_gated_scan_backward_{_SUFFIX[q.dtype]}", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                      beta.data_ptr(), g.data_ptr(), records.data_ptr(), records.numel(), go.data_ptr(), _lib.ptr(gs),
-                      _lib.ptr(rest[0] if rest else None), dq.data_ptr(), dk_.data_ptr(), dv.data_ptr(), db.data_ptr(),
-                      dg.data_ptr(), d_state_in.data_ptr(), ws.data_ptr(), ws_bytes, b, n, h, dk, _lib.stream_of(q.device))
-        need = ctx.needs_input_grad
-        return (*(x if wanted else None for x, wanted in zip((dq, dk_, dv, db, dg, d_state_in), need)), None)
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, d_o, d_state)
+
+
+def _backward(ctx: Any, d_o: Tensor | None, d_state: Tensor | None) -> tuple[Tensor | None, ...]:
+    q, k, v, beta, g, records, *rest = ctx.saved_tensors
+    b, n, h, dk = q.shape
+    go = torch.zeros_like(q) if d_o is None else _aligned(d_o.to(q.dtype))
+    gs = None if d_state is None else _aligned(d_state.to(STATE_DTYPE))
+    dq, dk_, dv, db, dg = (torch.empty_like(q), torch.empty_like(k), torch.empty_like(v), torch.empty_like(beta),
+                           torch.empty_like(g))
+    d_state_in = torch.empty((b, h, dk, dk), dtype=STATE_DTYPE, device=q.device)
+    ws_bytes = _bytes("backward_workspace", b, n, h, dk, int(q.dtype == torch.float32))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    with _lib.on_device(q.device):
+        _lib.call(_SCAN_BACKWARD[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(), g.data_ptr(),
+                  records.data_ptr(), records.numel(), go.data_ptr(), _lib.ptr(gs), _lib.ptr(rest[0] if rest else None),
+                  dq.data_ptr(), dk_.data_ptr(), dv.data_ptr(), db.data_ptr(), dg.data_ptr(), d_state_in.data_ptr(),
+                  ws.data_ptr(), ws_bytes, b, n, h, dk, _lib.stream_of(q.device))
+    need = ctx.needs_input_grad
+    if all(need[:6]):
+        return dq, dk_, dv, db, dg, d_state_in, None
+    return (*(x if wanted else None for x, wanted in zip((dq, dk_, dv, db, dg, d_state_in), need)), None)
+
+
+_backward_once = once_differentiable(_backward)  # under create_graph: its results refuse a derivative
 
 
 def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor, *,
@@ -148,7 +166,8 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
     mask = _active_mask(active, ("b", "n"), dims, q.device)
     if q.numel() == 0:  # no rows or no heads
         return torch.zeros_like(q), state.clone()
-    grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, beta, g, state))
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or beta.requires_grad
+                                        or g.requires_grad or state.requires_grad)
     dk = dims["dk"]
     if dims["n"] == 1 and not grad:
         first = (t[:, 0] for t in (q, k, v, beta, g))

@@ -7,6 +7,7 @@ rows, then the sums over the rows).
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Any
 
@@ -20,6 +21,11 @@ from vesper.kernels import _lib
 MAX_WIDTH = 16384
 MAX_ROWS = 2**31 - 1  # the C entry counts rows in 32 bits
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(rows: int, d: int) -> int:
+    return int(_lib.library().vsp_layer_norm_backward_workspace_bytes(rows, d))
 
 
 def _forward(x: Tensor, gain: Tensor, bias: Tensor | None, residual: Tensor | None, eps: float, dtype: torch.dtype,
@@ -41,9 +47,9 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx: Any, x: Tensor, gain: Tensor, bias: Tensor | None, residual: Tensor | None, eps: float,
                 dtype: torch.dtype) -> Any:  # noqa: D102
         ctx.set_materialize_grads(False)
-        x, gain = x.detach().contiguous(), gain.detach().contiguous()
-        bias = None if bias is None else bias.detach().contiguous()
-        residual = None if residual is None else residual.detach().contiguous()
+        x, gain = x.contiguous(), gain.contiguous()
+        bias = None if bias is None else bias.contiguous()
+        residual = None if residual is None else residual.contiguous()
         stats = torch.empty((*x.shape[:-1], 2), dtype=torch.float32, device=x.device)
         y, total = _forward(x, gain, bias, residual, eps, dtype, stats)
         # a sum of 16 bits is formed again from x and the residual
@@ -54,26 +60,32 @@ class _LayerNorm(torch.autograd.Function):
         return y if residual is None else (y, total)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, dy: Tensor | None, dsum: Tensor | None = None) -> tuple[Tensor | None, ...]:  # noqa: D102
-        gain, stats, total, *rest = ctx.saved_tensors
-        d = gain.shape[0]
-        rows = total.numel() // d
-        dy = torch.zeros(total.shape, dtype=ctx.dtype, device=total.device) if dy is None else dy.contiguous()
-        dsum = None if dsum is None else dsum.contiguous()
-        dx, dgain, dbias = torch.empty_like(total), torch.empty_like(gain), torch.empty_like(gain)
-        other = ctx.residual is not None and ctx.residual != total.dtype
-        dres = torch.empty(total.shape, dtype=ctx.residual, device=total.device) if other else None
-        ws_bytes = int(_lib.library().vsp_layer_norm_backward_workspace_bytes(rows, d))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=total.device)
-        with _lib.on_device(total.device):
-            _lib.call("vsp_layer_norm_backward", total.data_ptr(), _lib.ptr(rest[0] if rest else None), gain.data_ptr(),
-                      stats.data_ptr(), dy.data_ptr(), _lib.ptr(dsum), dx.data_ptr(), _lib.ptr(dres), dgain.data_ptr(), dbias.data_ptr(), ws.data_ptr(),
-                      ws_bytes, _CODES[total.dtype], _CODES[ctx.residual or total.dtype], _CODES[ctx.dtype], rows, d,
-                      _lib.stream_of(total.device))
-        need = ctx.needs_input_grad
-        return (dx if need[0] else None, dgain if need[1] else None, dbias if need[2] else None,
-                (dres if other else dx) if need[3] else None, None, None)
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dy, dsum)
+
+
+def _backward(ctx: Any, dy: Tensor | None, dsum: Tensor | None) -> tuple[Tensor | None, ...]:
+    gain, stats, total, *rest = ctx.saved_tensors
+    d = gain.shape[0]
+    rows = total.numel() // d
+    dy = torch.zeros(total.shape, dtype=ctx.dtype, device=total.device) if dy is None else dy.contiguous()
+    dsum = None if dsum is None else dsum.contiguous()
+    dx, dgain, dbias = torch.empty_like(total), torch.empty_like(gain), torch.empty_like(gain)
+    other = ctx.residual is not None and ctx.residual != total.dtype
+    dres = torch.empty(total.shape, dtype=ctx.residual, device=total.device) if other else None
+    ws_bytes = _workspace_bytes(rows, d)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=total.device)
+    with _lib.on_device(total.device):
+        _lib.call("vsp_layer_norm_backward", total.data_ptr(), _lib.ptr(rest[0] if rest else None), gain.data_ptr(),
+                  stats.data_ptr(), dy.data_ptr(), _lib.ptr(dsum), dx.data_ptr(), _lib.ptr(dres), dgain.data_ptr(), dbias.data_ptr(), ws.data_ptr(),
+                  ws_bytes, _CODES[total.dtype], _CODES[ctx.residual or total.dtype], _CODES[ctx.dtype], rows, d,
+                  _lib.stream_of(total.device))
+    need = ctx.needs_input_grad
+    return (dx if need[0] else None, dgain if need[1] else None, dbias if need[2] else None,
+            (dres if other else dx) if need[3] else None, None, None)
+
+
+_backward_once = once_differentiable(_backward)  # under create_graph: its results refuse a derivative
 
 
 def layer_norm(x: Tensor, gain: Tensor, bias: Tensor | None = None, *, residual: Tensor | None = None,
