@@ -272,12 +272,14 @@ __global__ __launch_bounds__(512) void gated_chain_backward_kernel(
       };
       f32x4 x[4];  // dO as accumulator tiles (rows tokens), zero where inactive
       auto read_do = [&](const BackIn<T>& in, auto slot) {
-        const uint64_t on = active == nullptr ? ~0ull : __builtin_amdgcn_ballot_w64(in.on != 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[j] = Slice::four(lds.d_o[decltype(slot)::value], j, 0);
+        for (int j = 0; j < 4; ++j) x[j] = Slice::four(lds.d_o[decltype(slot)::value], j, 0);
+        if (active != nullptr) {
+          const uint64_t on = __builtin_amdgcn_ballot_w64(in.on != 0) >> (4 * grp);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[j][r] = (on >> (16 * j + 4 * grp + r)) & 1 ? x[j][r] : 0.f;
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[j][r] = (on >> (16 * j + r)) & 1 ? x[j][r] : 0.f;
         }
       };
       auto form_z = [&](const BackIn<T>& in) {
