@@ -428,6 +428,30 @@ def test_long_rows_match_the_oracle(dtype, size, resets):
         assert not bool(o[~active].any())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [(1, 2100, 2, 64), (1, 2048, 1, 24)], ids=str)
+def test_gradients_of_long_rows_match_the_oracle(dtype, size):
+    from vesper.kernels.gated_scan import gated_delta_scan
+
+    b, n, h, dk = size
+    inputs = _inputs(*size, dtype, seed=sum(size))
+    gen = torch.Generator().manual_seed(2)
+    do, ds = torch.randn(b, n, h, dk, generator=gen).to(GPU, dtype), torch.randn(b, h, dk, dk, generator=gen).to(GPU)
+    leaves = [t.requires_grad_() for t in inputs]
+    o, after = gated_delta_scan(*leaves)
+    got = torch.autograd.grad([o, after], leaves, [do, ds])
+    exact = [t.detach().cpu().double().requires_grad_() for t in inputs]
+    want_o, want_after = gated_scan(*exact)
+    want = torch.autograd.grad([want_o, want_after], exact, [do.cpu().double(), ds.cpu().double()])
+    _close(o, want_o, what="o")
+    _close(after, want_after, what="state")
+    for name, x, y in zip(NAMES, got, want):
+        _close(x, y, what=name)
+    with torch.no_grad():
+        plain, last = gated_delta_scan(*(t.detach() for t in inputs))
+    assert torch.equal(plain, o) and torch.equal(last, after)  # with and without records
+
+
 def test_long_rows_keep_a_nan_to_its_head_and_what_follows():
     """Chunks before the one with the NaN, and the other head, are bit for bit as without it."""
     from vesper.kernels.gated_scan import gated_delta_scan

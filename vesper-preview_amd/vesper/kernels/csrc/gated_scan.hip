@@ -326,7 +326,7 @@ struct Segments {
   const float* states;  // the starting states of the second one and on, [B H][count - 1][D][D]
   float* maps;          // U and M, [B H][count - 1][2][D][D]
 };
-enum Walk { kOutputs, kRecords, kMaps };  // outputs; outputs and records (of one segment); only the end state, into maps
+enum Walk { kOutputs, kRecords, kMaps };  // outputs; outputs and records; only the end state, into maps
 
 template <typename T, int DP, Walk WALK>
 __global__ __launch_bounds__(512) void gated_chain_kernel(
@@ -647,22 +647,19 @@ template <typename T, int DP>
 void launch_chain(const T* q, const T* k, const T* v, const float* coef, const T* tf, const T* pf, const float* s_in,
                   T* o, float* s_out, const uint8_t* active, float* rec_h, float* rec_d, float* joined, Dims<T> dims, int B,
                   hipStream_t stream) {
-  const int slices = tiles_of(dims.D), heads = B * dims.H, count = rec_h != nullptr ? 1 : segments_of(B, dims.N, dims.H, dims.D);
+  const int slices = tiles_of(dims.D), heads = B * dims.H, count = segments_of(B, dims.N, dims.H, dims.D);
   const dim3 grid((unsigned)(heads * slices * count)), block(512);
   const size_t floats = (size_t)heads * (count - 1) * dims.D * dims.D;
   const Segments segs{count, (dims.chunks + count - 1) / count, joined, joined + floats};
 #define VSP_CHAIN(WALK, GRID)                                                                                                     \
   hipLaunchKernelGGL((gated_chain_kernel<T, DP, WALK>), GRID, block, 0, stream, q, k, v, coef, tf, pf, s_in, o, s_out, active,    \
                      rec_h, rec_d, dims, slices, segs)
-  if (rec_h != nullptr) {
-    VSP_CHAIN(kRecords, grid);
-    return;
-  }
   if (count > 1) {
     VSP_CHAIN(kMaps, dim3((unsigned)(heads * slices * 2 * (count - 1))));
     hipLaunchKernelGGL((gated_join_kernel<T, DP>), dim3((unsigned)(heads * slices)), dim3(256), 0, stream, s_in, joined, dims.D, slices, segs);
   }
-  VSP_CHAIN(kOutputs, grid);
+  if (rec_h != nullptr) VSP_CHAIN(kRecords, grid);
+  else VSP_CHAIN(kOutputs, grid);
 #undef VSP_CHAIN
 }
 

@@ -152,7 +152,8 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
     Under autograd the gradients of ``q, k, v, beta, g`` and ``state`` come from the backward kernels; the forward
     then keeps each chunk's starting state and corrections, ``4 dk (dk + 64)`` bytes a chunk and head. Widths that
     are no multiple of 8 run zero-padded to the next, which changes no output. One token without autograd runs as
-    ``gated_delta_step``. A NaN or an infinity in a token reaches its head's outputs from the start of its chunk on (a
+    ``gated_delta_step``. The backward may be captured into a graph, as long as no eager graph of the same leaves is alive
+    (torch's accumulation into them would leave the capture). A NaN or an infinity in a token reaches its head's outputs from the start of its chunk on (a
     chunk's products are over all pairs of its tokens), not those of other heads and rows.
 
     Raises:
