@@ -616,7 +616,7 @@ int vsp_gated_step_f32(const void* q, const void* k, const void* v, const void* 
  * sum_out receives s in x's type, stats (or NULL) mu and 1 / sqrt(var + eps) of each row, float32 [rows, 2].
  * Types: 0 float32, 1 bfloat16, 2 float16; x float32 goes with any of the others, x of 16 bits with its own only.
  * d 1..16384. Outputs overlap nothing. Memory of any alignment of its type; 16-byte aligned memory and a
- * d that is a multiple of 8 run in 16-byte accesses. */
+ * d that is a multiple of 8 are the fast form. */
 int vsp_layer_norm(const void* x, const void* residual, const float* gain, const float* bias, void* sum_out, void* y,
                    float* stats, int x_type, int residual_type, int y_type, int rows, int d, float eps, void* stream);
 

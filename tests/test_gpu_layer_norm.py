@@ -267,3 +267,42 @@ def test_offsets_past_32_bits():
     small = layer_norm(tail, gain)
     assert torch.equal(y[-3:], small)
     assert torch.equal(dx[-3:], torch.autograd.grad(small, tail, tail.detach())[0])
+
+
+@pytest.mark.parametrize("types", [(F32, F32, F32), (F32, BF16, F16), (BF16, BF16, BF16)], ids=str)
+@pytest.mark.parametrize("size", [(3000, 513), (40, 1025), (700, 2047), (33, 4097), (9, 8191), (4, 8193), (2100, 12), (50, 5000)], ids=str)
+def test_odd_and_wide_rows(types, size):
+    test_norm_and_gradients_match_float64(types, size)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("d", [1, 9, 513, 2051])
+def test_rows_that_end_anywhere_write_no_neighbour(dtype, d):
+    """The library's entries with outputs one element into larger memory: what is before and behind them stays."""
+    from vesper.kernels import _lib
+
+    m, code = 5, {F32: 0, BF16: 1, F16: 2}[dtype]
+    t = _inputs(m, d, dtype, dtype, dtype, seed=d)
+
+    def guarded(like):
+        whole = torch.full((like.numel() + 40,), 7.0, dtype=like.dtype, device=GPU)
+        return whole, whole[1 : 1 + like.numel()]
+
+    outs = {n: guarded(t["x"]) for n in ("sum", "y", "dx")} | {n: guarded(t["gain"]) for n in ("dgain", "dbias")}
+    stats = torch.empty(m, 2, device=GPU)
+    stream = _lib.stream_of(GPU if GPU.index is not None else torch.device("cuda", torch.cuda.current_device()))
+    _lib.call("vsp_layer_norm", t["x"].data_ptr(), t["residual"].data_ptr(), t["gain"].data_ptr(), t["bias"].data_ptr(),
+              outs["sum"][1].data_ptr(), outs["y"][1].data_ptr(), stats.data_ptr(), code, code, code, m, d, 1e-2, stream)
+    nbytes = int(_lib.library().vsp_layer_norm_backward_workspace_bytes(m, d))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=GPU)
+    summed = dtype == F32  # float32 goes back from the sum
+    _lib.call("vsp_layer_norm_backward", (outs["sum"][1] if summed else t["x"]).data_ptr(), None if summed else t["residual"].data_ptr(),
+              t["gain"].data_ptr(), stats.data_ptr(), t["dy"].data_ptr(), t["ds"].data_ptr(), outs["dx"][1].data_ptr(), None,
+              outs["dgain"][1].data_ptr(), outs["dbias"][1].data_ptr(), ws.data_ptr(), nbytes, code, code, code, m, d, stream)
+    torch.cuda.synchronize()
+    want_y, want_s, want = _want(t, 1e-2)
+    for name, exact in (("sum", want_s), ("y", want_y), ("dx", want["x"]), ("dgain", want["gain"]), ("dbias", want["bias"])):
+        whole, inner = outs[name]
+        assert bool((whole[:1] == 7).all()) and bool((whole[1 + inner.numel() :] == 7).all()), name
+        if d > 1 or name in ("sum", "dbias"):
+            _close(inner.view(exact.shape), exact, name, _held(inner.dtype))

@@ -13,8 +13,9 @@
 // workgroup of four (or, past that, sixteen) waves. The sums over rows stay in registers: a workgroup takes rows
 // grid apart, each lane adds up the columns that it holds in every row, and leaves one partial row; a second kernel
 // adds the partial rows in order. No atomics: results repeat bit for bit. 16384 x 4096 in bf16 with the residual and the
-// sum's gradient: forward 100 us (537 MB, 5.4 TB/s), backward 154 (686 MB, 4.5 TB/s: each row waits for its two sums between
-// its loads and its stores) and 6 for the columns; 16383 x 768 in float32 30, 35 and 4.
+// sum's gradient: forward 100 us (537 MB, 5.4 TB/s), backward 140 (686 MB, 4.9 TB/s: each row waits for its two sums between
+// its loads and its stores) and 5 for the columns; 16383 x 768 in float32 30, 35 and 4; 30000 x 513 in bf16 48 and 73 (element by
+// element 116 and 173).
 //
 // A row is scaled by a power of two (exact) that brings its largest deviation below 2^32 before it is squared, so
 // that var does not overflow; eps is scaled with it.
@@ -27,7 +28,7 @@
 namespace vsp {
 namespace {
 
-// WAVES waves share a row; V elements a piece (8, or 1 for odd widths and unaligned memory); SEG pieces a lane.
+// WAVES waves share a row, SEG pieces of 8 elements a lane; EDGE for odd widths and unaligned memory.
 // Reduction over the waves of a row; `slot` alternates so that one barrier a reduction is enough.
 template <int WAVES, int N, typename Op>
 __device__ __forceinline__ void row_reduce(float (&x)[N], float (*red)[16][N], int slot, Op op) {
@@ -48,24 +49,41 @@ __device__ __forceinline__ void row_reduce(float (&x)[N], float (*red)[16][N], i
   }
 }
 
-template <int V, typename T>
-__device__ __forceinline__ void load_piece(const T* p, float (&out)[V]) {
-  if constexpr (V == 8) load8_f32(p, out);
-  else out[0] = to_f32(p[0]);
-}
-template <int V, typename T>
-__device__ __forceinline__ void store_piece(T* p, const float (&x)[V]) {
-  if constexpr (V == 8 && sizeof(T) == 2) {
-    typedef T V8 __attribute__((ext_vector_type(8)));
-    V8 y;
+// Eight elements of a row from f on. EDGE: rows of any width and alignment; a row's last piece goes element by element, the
+// others in 16 bytes at the type's alignment (which the memory path takes). Else the width is a multiple of 8 and all
+// memory 16-byte aligned, and a piece past the row reads its first one. What is past the row is masked by `inside`.
+template <bool EDGE> __device__ __forceinline__ bool inside(int f, int e, int d) { return EDGE ? f + e < d : f < d; }
+
+// as they come from memory, converted where they are used: 16-bit values take half of the registers
+template <typename T> struct Piece {
+  typedef T V8 __attribute__((ext_vector_type(8)));
+  typedef T V8u __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  V8 x;
+  template <bool EDGE> __device__ __forceinline__ void load(const T* row, int f, int d) {
+    if constexpr (!EDGE) {
+      x = *reinterpret_cast<const V8*>(row + (f < d ? f : 0));
+    } else if (f + 8 <= d) {
+      x = *reinterpret_cast<const V8u*>(row + f);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = from_f32<T>(x[e]);
-    *reinterpret_cast<V8*>(p) = y;
-  } else if constexpr (V == 8) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+      for (int e = 0; e < 8; ++e) x[e] = f + e < d ? row[f + e] : (T)0;
+    }
+  }
+  __device__ __forceinline__ float get(int e) const { return to_f32(x[e]); }
+};
+template <bool EDGE, typename T>
+__device__ __forceinline__ void store_piece(T* row, int f, int d, const float (&x)[8]) {
+  typename Piece<T>::V8 y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = from_f32<T>(x[e]);
+  if constexpr (!EDGE) {
+    *reinterpret_cast<typename Piece<T>::V8*>(row + f) = y;
+  } else if (f + 8 <= d) {
+    *reinterpret_cast<typename Piece<T>::V8u*>(row + f) = y;
   } else {
-    p[0] = from_f32<T>(x[0]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (f + e < d) row[f + e] = y[e];
   }
 }
 
@@ -74,7 +92,7 @@ template <int WAVES> struct NormShape {
   static constexpr int ROWS = NT / (64 * WAVES);  // rows a workgroup has in hand at once
 };
 
-template <typename TX, typename TR, typename TY, int WAVES, int V, int SEG>
+template <typename TX, typename TR, typename TY, int WAVES, int SEG, bool EDGE>
 __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_kernel(
     const TX* __restrict__ x, const TR* __restrict__ res, const float* __restrict__ gain, const float* __restrict__ bias,
     TX* __restrict__ sum_out, TY* __restrict__ y, float* __restrict__ stats, int rows, int d, float eps) {
@@ -85,32 +103,34 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_kernel(
   for (long row = (long)blockIdx.x * NormShape<WAVES>::ROWS + threadIdx.x / LANES; row < rows;
        row += (long)gridDim.x * NormShape<WAVES>::ROWS) {
     const size_t base = (size_t)row * d;
-    float v[SEG][V];
+    float v[SEG][8];
     float sum[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < SEG; ++j) {
-      const int f = V * (t + LANES * j);
-      const bool ok = f < d;
-      load_piece<V>(x + base + (ok ? f : 0), v[j]);
-      if (res != nullptr) {
-        float r[V];
-        load_piece<V>(res + base + (ok ? f : 0), r);
+      const int f = 8 * (t + LANES * j);
+      Piece<TX> xs;
+      xs.template load<EDGE>(x + base, f, d);
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[j][e] += r[e];
-        if (ok) store_piece<V>(sum_out + base + f, v[j]);
+      for (int e = 0; e < 8; ++e) v[j][e] = xs.get(e);
+      if (res != nullptr) {
+        Piece<TR> r;
+        r.template load<EDGE>(res + base, f, d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] += r.get(e);
+        if (f < d) store_piece<EDGE>(sum_out + base, f, d, v[j]);
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) sum[0] += ok ? v[j][e] : 0.f;
+      for (int e = 0; e < 8; ++e) sum[0] += inside<EDGE>(f, e, d) ? v[j][e] : 0.f;
     }
     row_reduce<WAVES, 1>(sum, red, 0, SumOp{});
     const float mu = sum[0] / (float)d;
     float peak[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < SEG; ++j) {
-      const bool ok = V * (t + LANES * j) < d;
+      const int f = 8 * (t + LANES * j);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        v[j][e] = ok ? v[j][e] - mu : 0.f;
+      for (int e = 0; e < 8; ++e) {
+        v[j][e] = inside<EDGE>(f, e, d) ? v[j][e] - mu : 0.f;
         peak[0] = __builtin_fmaxf(peak[0], fabsf(v[j][e]));
       }
     }
@@ -121,7 +141,7 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_kernel(
 #pragma unroll
     for (int j = 0; j < SEG; ++j)
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
+      for (int e = 0; e < 8; ++e) {
         v[j][e] *= scale;
         sq[0] += v[j][e] * v[j][e];
       }
@@ -133,69 +153,73 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_kernel(
     }
 #pragma unroll
     for (int j = 0; j < SEG; ++j) {
-      const int f = V * (t + LANES * j);
+      const int f = 8 * (t + LANES * j);
       if (f >= d) continue;
-      float gn[V], bs[V], out[V];
-      load_piece<V>(gain + f, gn);
-      if (bias != nullptr) load_piece<V>(bias + f, bs);
+      Piece<float> gn, bs;
+      gn.template load<EDGE>(gain, f, d);
+      if (bias != nullptr) bs.template load<EDGE>(bias, f, d);
+      float out[8];
 #pragma unroll
-      for (int e = 0; e < V; ++e) out[e] = v[j][e] * root * gn[e] + (bias != nullptr ? bs[e] : 0.f);
-      store_piece<V>(y + base + f, out);
+      for (int e = 0; e < 8; ++e) out[e] = v[j][e] * root * gn.get(e) + (bias != nullptr ? bs.get(e) : 0.f);
+      store_piece<EDGE>(y + base, f, d, out);
     }
   }
 }
 
 // res as in the forward, or null where x is the float32 sum itself. dres may be null (no residual, or of x's type:
 // then dx serves both). partial: [grid][2][d] sums of dy xh and dy.
-template <typename TX, typename TR, typename TY, int WAVES, int V, int SEG>
+template <typename TX, typename TR, typename TY, int WAVES, int SEG, bool EDGE>
 __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_backward_kernel(
     const TX* __restrict__ x, const TR* __restrict__ res, const float* __restrict__ gain, const float* __restrict__ stats,
     const TY* __restrict__ dy,
     const TX* __restrict__ dsum, TX* __restrict__ dx, TR* __restrict__ dres, float* __restrict__ partial, int rows, int d) {
   constexpr int LANES = 64 * WAVES, ROWS = NormShape<WAVES>::ROWS;
+  // Sixteen waves of two pieces have 128 registers each: the sum's gradient is loaded at the end, the gain at each use.
+  constexpr bool TIGHT = WAVES == 16 && SEG > 1;
   __shared__ float red[2][16][2];
-  __shared__ float cols[ROWS > 1 ? ROWS : 1][ROWS > 1 ? 64 * SEG * V : 1];
+  __shared__ float cols[ROWS > 1 ? ROWS : 1][ROWS > 1 ? 64 * SEG * 8 : 1];
   const int t = threadIdx.x % LANES, sub = threadIdx.x / LANES;
-  float gn[SEG][V], dg[SEG][V], db[SEG][V];
+  Piece<float> gn[SEG];
+  float dg[SEG][8], db[SEG][8];
 #pragma unroll
   for (int j = 0; j < SEG; ++j) {
-    const int f = V * (t + LANES * j);
-    const bool ok = f < d;
-    load_piece<V>(gain + (ok ? f : 0), gn[j]);
+    if (!TIGHT) gn[j].template load<EDGE>(gain, 8 * (t + LANES * j), d);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      if (!ok) gn[j][e] = 0.f;
-      dg[j][e] = db[j][e] = 0.f;
-    }
+    for (int e = 0; e < 8; ++e) dg[j][e] = db[j][e] = 0.f;
   }
   int slot = 0;
   for (long row = (long)blockIdx.x * ROWS + sub; row < rows; row += (long)gridDim.x * ROWS) {
     const size_t base = (size_t)row * d;
     const float mu = stats[2 * (size_t)row], rstd = stats[2 * (size_t)row + 1];
-    float xh[SEG][V], w[SEG][V], add[SEG][V];
+    float xh[SEG][8];
+    Piece<TY> g[SEG];
+    Piece<TX> add[SEG];
     float sums[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < SEG; ++j) {
-      const int f = V * (t + LANES * j);
-      const bool ok = f < d;
-      load_piece<V>(x + base + (ok ? f : 0), xh[j]);
+      const int f = 8 * (t + LANES * j);
+      Piece<TX> xs;
+      xs.template load<EDGE>(x + base, f, d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) xh[j][e] = xs.get(e);
       if (res != nullptr) {
-        float r[V];
-        load_piece<V>(res + base + (ok ? f : 0), r);
+        Piece<TR> r;
+        r.template load<EDGE>(res + base, f, d);
 #pragma unroll
-        for (int e = 0; e < V; ++e) xh[j][e] += r[e];
+        for (int e = 0; e < 8; ++e) xh[j][e] += r.get(e);
       }
-      load_piece<V>(dy + base + (ok ? f : 0), w[j]);
-      if (dsum != nullptr) load_piece<V>(dsum + base + (ok ? f : 0), add[j]);
+      g[j].template load<EDGE>(dy + base, f, d);
+      if (TIGHT) gn[j].template load<EDGE>(gain, f, d);
+      if (!TIGHT && dsum != nullptr) add[j].template load<EDGE>(dsum + base, f, d);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
+      for (int e = 0; e < 8; ++e) {
+        const bool ok = inside<EDGE>(f, e, d);
         xh[j][e] = ok ? (xh[j][e] - mu) * rstd : 0.f;
-        const float g0 = ok ? w[j][e] : 0.f;
+        const float g0 = ok ? g[j].get(e) : 0.f, w = ok ? g0 * gn[j].get(e) : 0.f;
         db[j][e] += g0;
         dg[j][e] += g0 * xh[j][e];
-        w[j][e] = g0 * gn[j][e];
-        sums[0] += w[j][e];
-        sums[1] += w[j][e] * xh[j][e];
+        sums[0] += w;
+        sums[1] += w * xh[j][e];
       }
     }
     row_reduce<WAVES, 2>(sums, red, slot, SumOp{});
@@ -203,13 +227,15 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_backward_kern
     const float m0 = sums[0] / (float)d, m1 = sums[1] / (float)d;
 #pragma unroll
     for (int j = 0; j < SEG; ++j) {
-      const int f = V * (t + LANES * j);
+      const int f = 8 * (t + LANES * j);
       if (f >= d) continue;
-      float o[V];
+      float o[8];
+      if (TIGHT) gn[j].template load<EDGE>(gain, f, d);
+      if (TIGHT && dsum != nullptr) add[j].template load<EDGE>(dsum + base, f, d);
 #pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = rstd * (w[j][e] - m0 - xh[j][e] * m1) + (dsum != nullptr ? add[j][e] : 0.f);
-      store_piece<V>(dx + base + f, o);
-      if (dres != nullptr) store_piece<V>(dres + base + f, o);
+      for (int e = 0; e < 8; ++e) o[e] = rstd * (g[j].get(e) * gn[j].get(e) - m0 - xh[j][e] * m1) + (dsum != nullptr ? add[j].get(e) : 0.f);
+      store_piece<EDGE>(dx + base, f, d, o);
+      if (dres != nullptr) store_piece<EDGE>(dres + base, f, d, o);
     }
   }
   float* out = partial + (size_t)blockIdx.x * 2 * d;
@@ -220,7 +246,7 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_backward_kern
 #pragma unroll
       for (int j = 0; j < SEG; ++j)
 #pragma unroll
-        for (int e = 0; e < V; ++e) cols[sub][V * (t + LANES * j) + e] = half ? db[j][e] : dg[j][e];
+        for (int e = 0; e < 8; ++e) cols[sub][8 * (t + LANES * j) + e] = half ? db[j][e] : dg[j][e];
       __syncthreads();
       for (int f = threadIdx.x; f < d; f += NormShape<WAVES>::NT) {
         float x = cols[0][f];
@@ -230,9 +256,9 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_backward_kern
     } else {
 #pragma unroll
       for (int j = 0; j < SEG; ++j) {
-        const int f = V * (t + LANES * j);
+        const int f = 8 * (t + LANES * j);
 #pragma unroll
-        for (int e = 0; e < V; ++e)
+        for (int e = 0; e < 8; ++e)
           if (f + e < d) out[half * d + f + e] = half ? db[j][e] : dg[j][e];
       }
     }
@@ -268,19 +294,21 @@ __global__ __launch_bounds__(64 * kColumnWaves) void layer_norm_columns_kernel(c
   }
 }
 
-// The widest row of a shape: WAVES * 64 lanes, SEG pieces of V.
-#define VSP_NORM_SHAPES(GO)                     \
+// The widest row of a shape: WAVES * 64 lanes, SEG pieces of 8. W4 and W8 are the shapes of rows of up to 4096 and 8192. Rows
+// of odd widths take one piece a lane where they can: with two, their element-wise ends take all registers.
+#define VSP_NORM_SHAPES(GO, W4, W8)             \
   if (vec) {                                    \
-    if (d <= 512) GO(1, 8, 1)                   \
-    else if (d <= 1024) GO(1, 8, 2)             \
-    else if (d <= 2048) GO(4, 8, 1)             \
-    else if (d <= 4096) GO(4, 8, 2)             \
-    else if (d <= 8192) GO(4, 8, 4)             \
-    else GO(16, 8, 2)                           \
+    if (d <= 512) GO(1, 1, false)               \
+    else if (d <= 1024) GO(1, 2, false)         \
+    else if (d <= 2048) GO(4, 1, false)         \
+    else if (d <= 4096) W4(GO)                  \
+    else if (d <= 8192) W8(GO)                  \
+    else GO(16, 2, false)                       \
   } else {                                      \
-    if (d <= 256) GO(1, 1, 4)                   \
-    else if (d <= 2048) GO(4, 1, 8)             \
-    else GO(16, 1, 16)                          \
+    if (d <= 512) GO(1, 1, true)                \
+    else if (d <= 2048) GO(4, 1, true)          \
+    else if (d <= 8192) GO(16, 1, true)         \
+    else GO(16, 2, true)                        \
   }
 
 bool aligned16(std::initializer_list<const void*> ps) {
@@ -303,11 +331,15 @@ int norm_forward(const void* x_, const void* res_, const float* gain, const floa
   TY* y = static_cast<TY*>(y_);
   const bool vec = d % 8 == 0 && aligned16({x, res, gain, bias, sum, y});
   // launches of fewer than 2^32 threads: past 2^20 workgroups each takes several rows
-#define VSP_GO(W, V, S)                                                                                              \
-  hipLaunchKernelGGL((layer_norm_kernel<TX, TR, TY, W, V, S>),                                                       \
+#define VSP_GO(W, S, EDGE)                                                                                              \
+  hipLaunchKernelGGL((layer_norm_kernel<TX, TR, TY, W, S, EDGE>),                                                       \
                      dim3((unsigned)std::min<long>(((long)rows + NormShape<W>::ROWS - 1) / NormShape<W>::ROWS, 1 << 20)), \
                      dim3(NormShape<W>::NT), 0, stream, x, res, gain, bias, sum, y, stats, rows, d, eps);
-  VSP_NORM_SHAPES(VSP_GO)
+#define VSP_W4(GO) GO(4, 2, false)
+#define VSP_W8(GO) GO(4, 4, false)
+  VSP_NORM_SHAPES(VSP_GO, VSP_W4, VSP_W8)
+#undef VSP_W4
+#undef VSP_W8
 #undef VSP_GO
   return check_launch(who);
 }
@@ -338,14 +370,19 @@ int norm_backward(const void* x_, const void* res_, const float* gain, const flo
   TR* dres = static_cast<TR*>(dres_);
   const bool vec = d % 8 == 0 && aligned16({x, res, gain, dy, dsum, dx, dres});
   int parts = norm_parts(rows, d);
-#define VSP_GO(W, V, S)                                                                                              \
+#define VSP_GO(W, S, EDGE)                                                                                              \
   {                                                                                                                  \
-    static const int held = held_at_once(reinterpret_cast<const void*>(layer_norm_backward_kernel<TX, TR, TY, W, V, S>), NormShape<W>::NT); \
+    static const int held = held_at_once(reinterpret_cast<const void*>(layer_norm_backward_kernel<TX, TR, TY, W, S, EDGE>), NormShape<W>::NT); \
     parts = std::min(parts, held);                                                                                   \
-    hipLaunchKernelGGL((layer_norm_backward_kernel<TX, TR, TY, W, V, S>), dim3((unsigned)parts), dim3(NormShape<W>::NT), 0, \
+    hipLaunchKernelGGL((layer_norm_backward_kernel<TX, TR, TY, W, S, EDGE>), dim3((unsigned)parts), dim3(NormShape<W>::NT), 0, \
                        stream, x, res, gain, stats, dy, dsum, dx, dres, ws, rows, d);                                \
   }
-  VSP_NORM_SHAPES(VSP_GO)
+// one piece a lane: four waves of four pieces have room for one workgroup a CU (4096 x 8192 in bf16: 123 us against 82)
+#define VSP_W4(GO) GO(8, 1, false)
+#define VSP_W8(GO) GO(16, 1, false)
+  VSP_NORM_SHAPES(VSP_GO, VSP_W4, VSP_W8)
+#undef VSP_W4
+#undef VSP_W8
 #undef VSP_GO
   hipLaunchKernelGGL(layer_norm_columns_kernel, dim3((unsigned)((2 * d + 63) / 64)), dim3(64 * kColumnWaves), 0, stream, ws, dgain, dbias, parts, d);
   return check_launch(who);
