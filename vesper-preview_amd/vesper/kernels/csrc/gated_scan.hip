@@ -1,7 +1,8 @@
 // The gated delta rule's chunked scan on CDNA4 (gfx950); the mathematics and the operands are in gated.h.
 //
-//  * gated_prep_kernel: a wave a chunk and head, all of them at once: the decays' sums, the products of all
-//    pairs of the chunk's tokens (K K^T and Q K^T), the inverse T and W = P T, both written as MFMA operands.
+//  * gated_prep_kernel: a wave a chunk and head (for few chunks gated_prep_lines_kernel: four), all of them at once:
+//    the decays' sums, the products of all pairs of the chunk's tokens (K K^T and Q K^T), the inverse T and W = P T,
+//    both written as MFMA operands.
 //  * gated_chain_kernel: a workgroup a head and 16 value columns walks the chunks (value columns of the state evolve
 //    independently, so a head of width 64 is four chains). Four waves carry the chain, each one tile of 16 tokens
 //    (R, Delta) and its share of the state's feature tiles in accumulators; between the three dependent products
@@ -21,6 +22,7 @@ namespace {
 constexpr int kPad = 20;                   // pitch of a 16 x 16 float32 tile in LDS
 constexpr int kTile = 16 * kPad + 4;       // tiles start on other banks
 constexpr int kPrepWaves = 4;
+constexpr int kLineChunks = 256;  // up to a workgroup a CU, prep by lines
 
 struct PrepLds {
   float hi[kChunk], lo[kChunk];  // both parts of the decays' sums
@@ -77,9 +79,8 @@ __device__ __forceinline__ void put_line(T* out, int a, const f32x4 (&x)[4]) {
 // Bound by its own arithmetic and its latency, not by memory: of a wave's 20 to 27 thousand cycles alone on its SIMD the 80
 // decays a lane take 2500, the substitution 2700, the 144 float32 MFMAs of T and W and their splitting 7000, the loads and
 // the decays' sums 5000, and three waves a SIMD share them. B8 T4096 H8 d64 (160 MB in and out) 47 us, B1 T8191 H12 18, 64
-// chunks of float32 13. Tried: four waves a chunk, a line of T and W each, whose tiles of A passed by LDS (128 chunks 8 us
-// instead of 11, but 51 and 21 for the large ones: each wave inverts a diagonal tile, where one wave has all four in its 64
-// lanes); four waves a SIMD (61: the registers spill).
+// chunks of float32 13 (by lines, below, 8; but 51 and 21 for the large ones: each wave inverts a diagonal tile, where one
+// wave has all four in its 64 lanes). Tried: four waves a SIMD (61: the registers spill).
 // COLS, for the backward pass: the factors T and P by columns, with accumulator rows i and columns j. Else T and
 // W = P T by rows, transposed: rows j, columns i. With X the diagonal tiles' inverses (I + A_bb)^-1, tile by tile:
 //   T_ij = -X_i sum_k A_ik T_kj (k = j .. i - 1), or transposed T_ij^T = -X_j^T sum_k A_kj^T T_ik^T (k = j + 1 .. i);
@@ -261,6 +262,199 @@ __global__ __launch_bounds__(64 * kPrepWaves, 2) void gated_prep_kernel(
     put_line<T, NT, COLS>(tout, a, t);
     put_line<T, NPP, COLS>(pout, a, w);
   }
+}
+
+struct LinesLds {
+  float hi[kChunk], lo[kChunk];  // both parts of the decays' sums
+  float beta[kChunk];            // -beta
+  f32x4 mult[6][64];    // -A's tiles below the diagonal, (i, j) at i (i - 1) / 2 + j, as they lie in registers
+  float a[4 * kTile];   // the diagonal ones, column by column
+  float x[4 * kTile];   // their inverses (I + A_bb)^-1, row by row
+};
+
+// The same by a workgroup of four waves a chunk and head, for few chunks: a wave has a line (row or column a), its tiles of
+// K K^T and Q K^T, its diagonal tile's inverse and its tiles of T and W; the tiles of A and the inverses pass by LDS. Its
+// results are the other's bit for bit. Calls of the scan with one and the other for 64, 128, 256, 512 and 1024 chunks of one a
+// row, in us: float32 14 and 19, 17 and 21, 24 and 30, 38 and 42, 70 and 66; bf16 12 and 14, 14 and 17, 20 and 23, 32.5 and
+// 32.6, 52 and 49.
+template <typename T, int DP, bool COLS>
+__global__ __launch_bounds__(256) void gated_prep_lines_kernel(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ beta, const float* __restrict__ g,
+    float* __restrict__ coef, T* __restrict__ tf, T* __restrict__ pf, Dims<T> dims) {
+  __shared__ __attribute__((aligned(16))) LinesLds s;
+  const int id = blockIdx.x, l = threadIdx.x & 63, c = l & 15, grp = l >> 4;
+  // the lines are of different lengths: the waves of a SIMD shall not all have the same one
+  const int a = __builtin_amdgcn_readfirstlane(((threadIdx.x >> 6) + id) & 3);
+  const int chunk = id % dims.chunks, bh = id / dims.chunks, h = bh % dims.H, b = bh / dims.H;
+  const int t0 = chunk * kChunk;
+  constexpr int KS = DP / 32;
+  constexpr int NT = Pieces<T>::kN, NPP = COLS ? NT : OutPieces<T>::kN;
+
+  // the line's tiles (tile o of the other index): of K K^T as what multiplies (COLS: rows j, columns i; else rows i,
+  // columns j), of Q K^T as what is multiplied; tiles outside the triangle: the diagonal one's rows again, not used
+  f32x4 mult[4], pp[4];
+#pragma unroll
+  for (int o = 0; o < 4; ++o) mult[o] = pp[o] = zero4();
+  const Rows<T> krows = dims.rows(k, b, t0, h), qrows = dims.rows(q, b, t0, h);
+  struct In {
+    Operand<T, 1> ka, qa, kf[4], qf[COLS ? 4 : 1];
+  };
+  auto load = [&](int st, In& in) {
+    const int f = 32 * st + 8 * grp;
+    in.ka = krows.row(16 * a + c, f);
+    if constexpr (!COLS) in.qa = qrows.row(16 * a + c, f);
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+      const int row = 16 * (COLS ? (o < a ? a : o) : (o < a ? o : a)) + c;
+      in.kf[o] = krows.row(row, f);
+      if constexpr (COLS) in.qf[o] = qrows.row(row, f);
+    }
+  };
+  auto multiply = [&](const In& in) {
+#pragma unroll
+    for (int o = 0; o < 4; ++o)
+      if (COLS ? o >= a : o <= a) {
+        mult[o] = mma(in.ka, in.kf[o], mult[o]);
+        pp[o] = COLS ? mma(in.qf[COLS ? o : 0], in.ka, pp[o]) : mma(in.kf[o], in.qa, pp[o]);
+      }
+  };
+  // the decays, by the wave with the shortest line: lane l is token t0 + l; tokens behind the last decay nothing and write
+  // nothing
+  const bool sums = a == (COLS ? 3 : 0), ok = t0 + l < dims.N;
+  float gl = 0.f, bl = 0.f;
+  if (sums) {
+    const size_t at = ((size_t)b * dims.N + (ok ? t0 + l : t0)) * dims.H + h;
+    gl = g[at];
+    bl = to_f32(beta[at]);
+  }
+  constexpr int AHEAD = KS < 2 || sizeof(T) == 4 ? 1 : 2;  // steps whose loads are in flight while the decays are summed
+  In in[AHEAD];
+#pragma unroll
+  for (int st = 0; st < AHEAD; ++st) load(st, in[st]);
+  double sum = 0.0;
+  if (sums) {
+    if (!ok) bl = 0.f;
+    sum = sums_up_to(ok ? ((double)gl < kLeastDecay ? kLeastDecay : (double)gl) : 0.0);
+    const DecaySum parts = decay_sum(sum);
+    s.hi[l] = parts.hi;
+    s.lo[l] = parts.lo;
+    s.beta[l] = -bl;
+  }
+#pragma unroll
+  for (int st = 0; st < AHEAD; ++st) multiply(in[st]);
+#pragma unroll
+  for (int st = AHEAD; st < KS; ++st) {
+    load(st, in[0]);
+    multiply(in[0]);
+  }
+  lds_barrier();
+  if (sums) {
+    const double all = __shfl(sum, 63);
+    const DecaySum parts = decay_sum(sum);
+    float* co = coef + (size_t)id * kCoefAll;
+    co[l] = bl;
+    co[kChunk + l] = expf((float)sum);
+    co[2 * kChunk + l] = expf((float)(all - sum));
+    co[kCoef + l] = parts.hi;
+    co[kCoef + kChunk + l] = parts.lo;
+  }
+
+  // the decays between pairs, -beta and the triangles; the sums are read at once, not each before its use
+  const f32x4 hi_own = *reinterpret_cast<const f32x4*>(s.hi + 16 * a + 4 * grp), lo_own = *reinterpret_cast<const f32x4*>(s.lo + 16 * a + 4 * grp);
+  const f32x4 beta_own = *reinterpret_cast<const f32x4*>(s.beta + 16 * a + 4 * grp);
+  const DecaySum col_own = {s.hi[16 * a + c], s.lo[16 * a + c]};
+  f32x4 hi_row[4], lo_row[4];
+  DecaySum col[4];
+  float beta_col[4];
+#pragma unroll
+  for (int o = 0; o < 4; ++o) {
+    hi_row[o] = *reinterpret_cast<const f32x4*>(s.hi + 16 * o + 4 * grp);
+    lo_row[o] = *reinterpret_cast<const f32x4*>(s.lo + 16 * o + 4 * grp);
+    col[o] = {s.hi[16 * o + c], s.lo[16 * o + c]};
+    beta_col[o] = s.beta[16 * o + c];
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int o = 0; o < 4; ++o)
+    if (COLS ? o >= a : o <= a) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 4 * grp + r;
+        const DecaySum mine = {hi_own[r], lo_own[r]}, other = {hi_row[o][r], lo_row[o][r]};
+        // of mult: i the own rows (COLS: columns of tile o), j the columns of tile o (COLS: the own rows)
+        const float em = (COLS ? beta_col[o] : beta_own[r]) * (COLS ? decay(col[o], mine) : decay(mine, col[o]));
+        mult[o][r] *= o != a || (COLS ? row < c : c < row) ? em : 0.f;
+        // of Q K^T: i the own columns (COLS: rows of tile o), j the rows of tile o (COLS: the own columns)
+        const float ep = COLS ? decay(other, col_own) : decay(col_own, other);
+        pp[o][r] *= o != a || (COLS ? c <= row : row <= c) ? ep : 0.f;
+      }
+      if (o == a) {
+        if constexpr (COLS) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s.a[a * kTile + (4 * grp + r) * kPad + c] = mult[o][r];
+        } else {
+          *reinterpret_cast<f32x4*>(s.a + a * kTile + c * kPad + 4 * grp) = mult[o];
+        }
+      } else {
+        s.mult[COLS ? o * (o - 1) / 2 + a : a * (a - 1) / 2 + o][l] = mult[o];
+      }
+    }
+  wave_lds_sync();
+
+  // X = (I + A_aa)^-1 by forward substitution: each lane solves column l % 16, column by column of A
+  {
+    float x[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = r == c ? 1.f : 0.f;
+    const float* t = s.a + a * kTile;
+#pragma unroll
+    for (int kk = 0; kk < 15; ++kk)
+#pragma unroll
+      for (int q4 = (kk + 1) / 4; q4 < 4; ++q4) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(t + kk * kPad + 4 * q4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (4 * q4 + r > kk) x[4 * q4 + r] = __builtin_fmaf(y[r], x[kk], x[4 * q4 + r]);
+      }
+    if (grp == 0) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s.x[a * kTile + r * kPad + c] = x[r];
+    }
+  }
+  lds_barrier();
+
+  // the line, tile by tile from the diagonal on
+  f32x4 t[4], w[4];
+#pragma unroll
+  for (int o = 0; o < 4; ++o) t[o] = w[o] = zero4();
+#pragma unroll
+  for (int step = 0; step < 4; ++step) {
+    const int o = COLS ? step : 3 - step;
+    if (COLS ? o < a : o > a) continue;
+    const float* x = s.x + o * kTile;
+    const f32x4 along = *reinterpret_cast<const f32x4*>(x + c * kPad + 4 * grp);  // X[c][4 g + r]
+    f32x4 down;                                                                   // X[4 g + r][c]
+#pragma unroll
+    for (int r = 0; r < 4; ++r) down[r] = x[(4 * grp + r) * kPad + c];
+    f32x4 m = zero4();
+    if constexpr (COLS) w[o] = pp[o];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      if constexpr (COLS) {
+        if (kk < o && kk >= a) m = mm16f(s.mult[o * (o - 1) / 2 + (kk < o ? kk : 0)][l], t[kk], m);
+      } else {
+        if (kk > o && kk <= a) {
+          const f32x4 y = s.mult[kk * (kk - 1) / 2 + (kk > o ? o : 0)][l];
+          m = mm16f(y, t[kk], m);
+          pp[o] = mm16f(y, w[kk], pp[o]);
+        }
+      }
+    }
+    t[o] = o == a ? (COLS ? down : along) : mm16f(COLS ? along : down, m, zero4());
+    if constexpr (!COLS) w[o] = mm16f(down, pp[o], zero4());
+  }
+  put_line<T, NT, COLS>(tf + (size_t)id * Factor<T, NT>::kElems, a, t);
+  put_line<T, NPP, COLS>(pf + (size_t)id * Factor<T, NPP>::kElems, a, w);
 }
 
 // --------------------------------------------------------------------------------------------
@@ -638,6 +832,12 @@ int segments_of(int B, int N, int H, int D) {
 template <typename T, int DP>
 void launch_prep_width(const T* q, const T* k, const T* beta, const float* g, float* coef, T* tf, T* pf, Dims<T> dims,
                        int total, bool columns, hipStream_t stream) {
+  if (total <= kLineChunks) {
+    const dim3 grid((unsigned)total), block(256);
+    if (columns) hipLaunchKernelGGL((gated_prep_lines_kernel<T, DP, true>), grid, block, 0, stream, q, k, beta, g, coef, tf, pf, dims);
+    else hipLaunchKernelGGL((gated_prep_lines_kernel<T, DP, false>), grid, block, 0, stream, q, k, beta, g, coef, tf, pf, dims);
+    return;
+  }
   const dim3 grid((unsigned)((total + kPrepWaves - 1) / kPrepWaves)), block(64 * kPrepWaves);
   if (columns) hipLaunchKernelGGL((gated_prep_kernel<T, DP, true>), grid, block, 0, stream, q, k, beta, g, coef, tf, pf, dims, total);
   else hipLaunchKernelGGL((gated_prep_kernel<T, DP, false>), grid, block, 0, stream, q, k, beta, g, coef, tf, pf, dims, total);
