@@ -205,7 +205,8 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
             while grad mode is on.
     """
     dims = _check(q, k, v, beta, g, state, ("b", "h"))
-    _refuse_grad(q, k, v, beta, g, state)
+    if torch.is_grad_enabled():
+        _refuse_grad(q, k, v, beta, g, state)
     b, h, dk = q.shape
     if not state.is_contiguous():
         raise ContractError("state must be contiguous")
@@ -221,12 +222,10 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
         if 0 < apart < state.nbytes:
             raise ContractError("out_state must be state itself or not overlap it")
     q, k, v, beta, g = q.contiguous(), k.contiguous(), v.contiguous(), beta.contiguous(), g.contiguous()
-    mask = _active_mask(active, ("b",), dims, q.device)
+    mask = None if active is None else _active_mask(active, ("b",), dims, q.device)
     o = torch.empty_like(q)
-    if q.numel() == 0:
+    if b == 0 or h == 0:
         return o, out_state
-    with _lib.on_device(q.device):
-        _lib.call(_STEP[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(),
-                  g.data_ptr(), state.data_ptr(), out_state.data_ptr(), o.data_ptr(), _lib.ptr(mask), b, h, dk,
-                  _lib.stream_of(q.device))
+    _lib.launch(q.device, _STEP[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(), g.data_ptr(),
+                state.data_ptr(), out_state.data_ptr(), o.data_ptr(), None if mask is None else mask.data_ptr(), b, h, dk)
     return o, out_state

@@ -34,11 +34,11 @@ def _forward(x: Tensor, gain: Tensor, bias: Tensor | None, residual: Tensor | No
     d = x.shape[-1]
     y = torch.empty_like(x) if dtype is x.dtype else torch.empty_like(x, dtype=dtype)
     total = x if residual is None else torch.empty_like(x)
-    with _lib.on_device(x.device):
-        _lib.call("vsp_layer_norm", x.data_ptr(), _lib.ptr(residual), gain.data_ptr(), _lib.ptr(bias),
-                  None if residual is None else total.data_ptr(), y.data_ptr(), _lib.ptr(stats), _CODES[x.dtype],
-                  _CODES[x.dtype if residual is None else residual.dtype], _CODES[dtype], x.numel() // d, d, eps,
-                  _lib.stream_of(x.device))
+    code = _CODES[x.dtype]
+    _lib.launch(x.device, "vsp_layer_norm", x.data_ptr(), None if residual is None else residual.data_ptr(), gain.data_ptr(),
+                None if bias is None else bias.data_ptr(), None if residual is None else total.data_ptr(), y.data_ptr(),
+                None if stats is None else stats.data_ptr(), code, code if residual is None else _CODES[residual.dtype],
+                _CODES[dtype], x.numel() // d, d, eps)
     return y, total
 
 
