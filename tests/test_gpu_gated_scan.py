@@ -485,3 +485,41 @@ def test_long_rows_in_a_graph():
         with torch.no_grad():
             want, last = gated_delta_scan(*inputs)
         assert torch.equal(o, want) and torch.equal(after, last)
+
+
+# more chunks and heads than CUs: the other form of the chunks' factors
+MANY = [(20, 200, 4, 64), (9, 70, 15, 32), (33, 130, 3, 16), (17, 65, 8, 128), (1, 70, 131, 136), (5, 64, 60, 8), (2, 5, 130, 256)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", MANY, ids=str)
+@pytest.mark.parametrize("resets", [False, True])
+def test_many_chunks_match_the_oracle(dtype, size, resets):
+    test_scan_matches_the_oracle(dtype, size, resets)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [(20, 200, 4, 64), (33, 130, 3, 16), (17, 65, 8, 72), (9, 70, 15, 24)], ids=str)
+@pytest.mark.parametrize("masked", [False, True])
+def test_gradients_of_many_chunks_match_the_oracle(dtype, size, masked):
+    test_gradients_match_the_oracle(dtype, size, masked)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dk", [32, 64, 128, 256])
+def test_a_row_among_many_is_the_row_alone(dtype, dk):
+    """Rows of a large batch (a wave a chunk in the first kernel) bit for bit as alone (four waves a chunk), gradients too."""
+    from vesper.kernels.gated_scan import gated_delta_scan
+
+    b, n, h = 90, 130, 1
+    inputs = _inputs(b, n, h, dk, dtype, seed=dk, resets=True)
+    do = torch.randn(b, n, h, dk, device=GPU, generator=torch.Generator(GPU).manual_seed(1)).to(dtype)
+    leaves = [t.detach().requires_grad_() for t in inputs]
+    o, after = gated_delta_scan(*leaves)
+    grads = torch.autograd.grad([o, after], leaves, [do, torch.ones_like(after)])
+    for row in (0, 41, 89):
+        alone = [t[row : row + 1].detach().clone().requires_grad_() for t in inputs]
+        o1, after1 = gated_delta_scan(*alone)
+        grads1 = torch.autograd.grad([o1, after1], alone, [do[row : row + 1].clone(), torch.ones_like(after1)])
+        for name, x, y in zip(("o", "state", *NAMES), (o, after, *grads), (o1, after1, *grads1)):
+            assert torch.equal(x[row : row + 1], y), (name, row)
