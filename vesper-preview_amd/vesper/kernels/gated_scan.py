@@ -78,11 +78,10 @@ def _forward(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Te
     o, s_out = torch.empty_like(q), torch.empty_like(state)
     ws_bytes = _bytes("workspace", b, n, h, dk, int(q.dtype == torch.float32))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-    with _lib.on_device(q.device):
-        _lib.call(_SCAN[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(),
-                  g.data_ptr(), state.data_ptr(), o.data_ptr(), s_out.data_ptr(), ws.data_ptr(), ws_bytes,
-                  _lib.ptr(records), 0 if records is None else records.numel(), _lib.ptr(mask), b, n, h, dk,
-                  _lib.stream_of(q.device))
+    _lib.launch(q.device, _SCAN[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(), g.data_ptr(),
+                state.data_ptr(), o.data_ptr(), s_out.data_ptr(), ws.data_ptr(), ws_bytes,
+                None if records is None else records.data_ptr(), 0 if records is None else records.numel(),
+                None if mask is None else mask.data_ptr(), b, n, h, dk)
     return o, s_out
 
 
@@ -116,11 +115,10 @@ def _backward(ctx: Any, d_o: Tensor | None, d_state: Tensor | None) -> tuple[Ten
     d_state_in = torch.empty((b, h, dk, dk), dtype=STATE_DTYPE, device=q.device)
     ws_bytes = _bytes("backward_workspace", b, n, h, dk, int(q.dtype == torch.float32))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-    with _lib.on_device(q.device):
-        _lib.call(_SCAN_BACKWARD[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(), g.data_ptr(),
-                  records.data_ptr(), records.numel(), go.data_ptr(), _lib.ptr(gs), _lib.ptr(rest[0] if rest else None),
-                  dq.data_ptr(), dk_.data_ptr(), dv.data_ptr(), db.data_ptr(), dg.data_ptr(), d_state_in.data_ptr(),
-                  ws.data_ptr(), ws_bytes, b, n, h, dk, _lib.stream_of(q.device))
+    _lib.launch(q.device, _SCAN_BACKWARD[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(), g.data_ptr(),
+                records.data_ptr(), records.numel(), go.data_ptr(), None if gs is None else gs.data_ptr(),
+                rest[0].data_ptr() if rest else None, dq.data_ptr(), dk_.data_ptr(), dv.data_ptr(), db.data_ptr(),
+                dg.data_ptr(), d_state_in.data_ptr(), ws.data_ptr(), ws_bytes, b, n, h, dk)
     need = ctx.needs_input_grad
     if all(need[:6]):
         return dq, dk_, dv, db, dg, d_state_in, None
@@ -164,8 +162,8 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
         check_shape("active", active, ("b", "n"), dims, torch.bool)
     if dims["n"] == 0:
         return q, state
-    mask = _active_mask(active, ("b", "n"), dims, q.device)
-    if q.numel() == 0:  # no rows or no heads
+    mask = None if active is None else _active_mask(active, ("b", "n"), dims, q.device)
+    if dims["b"] == 0 or dims["h"] == 0:
         return torch.zeros_like(q), state.clone()
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or beta.requires_grad
                                         or g.requires_grad or state.requires_grad)
@@ -181,7 +179,7 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
     if grad:
         o, after = _GatedScan.apply(q, k, v, beta, g, state, mask)
     else:
-        o, after = _forward(*(_aligned(t) for t in (q, k, v, beta, g, state)), mask, None)
+        o, after = _forward(_aligned(q), _aligned(k), _aligned(v), _aligned(beta), _aligned(g), _aligned(state), mask, None)
     return (o[..., :dk].contiguous(), after[..., :dk, :dk].contiguous()) if pad else (o, after)
 
 
