@@ -514,7 +514,7 @@ template <typename T, int DP> struct OutIn {
 // state is affine, H' = M H + U. A first launch walks all segments but the last from zero (its end is U) and, without
 // values, from the identity (M), gated_join_kernel carries the state from segment to segment, and a second launch walks
 // each from its start: three times the work, on all CUs. Whole and in segments, prep and all, in us (bf16): B1 T8191 H12 d64
-// 137 and 98, T4096 H2 d64 68 and 42, T4096 H16 d64 75 and 65, T2048 H8 d64 43 and 40, T4096 H2 d256 157 and 142.
+// 137 and 87, T4096 H2 d64 68 and 42, T4096 H16 d64 75 and 65, T2048 H8 d64 43 and 40, T4096 H2 d256 157 and 142.
 struct Segments {
   int count, chunks;    // segments a row and head, chunks a segment
   const float* states;  // the starting states of the second one and on, [B H][count - 1][D][D]
