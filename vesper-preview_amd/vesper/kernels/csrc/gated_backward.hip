@@ -6,10 +6,12 @@
 // With dP_ij = E_ij dO_i.Delta_j (j <= i) and B_ij = E_ij dR_i.Delta_j (j < i):
 //   dQ_i = eps_i H dO_i + sum_j dP_ij k_j,    Y_i = -(eps_i H dR_i + sum_j B_ij k_j),
 //   C_j = kap_j dH' Delta_j + sum_i dP_ij q_i - sum_i beta_i B_ij k_i,
-//   dK_i = beta_i Y_i + C_i,   dbeta_i = dR_i.v_i + k_i.Y_i,
-//   dG_i = q_i.dQ_i + beta_i k_i.Y_i - k_i.C_i,  and for the chunk's last sum also
-//   gam <dH', H> + sum_j kap_j k_j.(dH' Delta_j);   dg_t = sum of dG_i over the chunk's i >= t.
-// (Every exponent is a difference of sums: its derivative adds to the later sum what it takes from the earlier one.)
+//   dK_i = beta_i Y_i + C_i,   dbeta_i = dR_i.v_i + k_i.Y_i.
+// A token's decay is in every exponent that reaches over it, and its gradient is the sum of their terms:
+//   dg_t = sum_{i >= t} eps_i (q_i.(H dO_i) - beta_i k_i.(H dR_i)) + sum_{j < t <= i} (dP_ij q_i.k_j - beta_i B_ij k_i.k_j)
+//        + sum_{j < t} kap_j k_j.(dH' Delta_j) + gam <dH', H>.
+// Every term has e^{g_t} in it. The sums G_i's own gradients, summed over i >= t, are the same number as the
+// difference of terms that have not: behind decays of e^-10 and less their rounding was all that was left of it.
 //
 //  * gated_prep_kernel (gated_scan.hip) forms T and P again, as operands by columns.
 //  * gated_chain_backward_kernel walks the chunks from the last to the first like the forward's chain, a workgroup a
@@ -457,6 +459,18 @@ __device__ __forceinline__ f32x4 four(const T* p) {
   return x;
 }
 
+template <typename T>
+__device__ __forceinline__ Operand<T, 1> eight(const T* p) {
+  Operand<T, 1> x;
+  if constexpr (sizeof(T) == 2) {
+    x.p[0] = *reinterpret_cast<const bf16x8*>(p);
+  } else {
+    x.lo = reinterpret_cast<const f32x4*>(p)[0];
+    x.hi = reinterpret_cast<const f32x4*>(p)[1];
+  }
+  return x;
+}
+
 template <typename T, int DP> struct GradShape {
   static constexpr int TILES = DP / 16;
   static constexpr int NT = Pieces<T>::kN;
@@ -481,14 +495,16 @@ template <typename T, int DP> struct GradShape {
       f32x4 y[4][TILES][64];  // beta Y as accumulator tiles
     } u;
     float coef[kCoefAll];
-    float dsum[2][kChunk];
-    float part[8][2];  // each wave's share of <dH', H> and of the chunk end's other terms
+    float ends[2][kChunk];          // of dg: each token's terms with the chunk's start, and with its end
+    float across[4][kChunk];        // of dg: the terms of the pairs around token t whose first is of tile w, [w][t]
+    float part[8];                  // each wave's share of <dH', H>
   };
 };
 
-// Bound by memory: 122 KB a chunk and head of width 64 (half of it the four records), B16 T1024 H12 d64 106 us for 375 MB (3.5
-// TB/s), B2 T1500 H8 d128 37 us for 160 MB. With four waves for all it was 227 us (286 registers, one workgroup a CU), with
-// eight 127, with the pairs' products formed once and no register spilled 106.
+// Bound by memory: 122 KB a chunk and head of width 64 (half of it the four records), B16 T1024 H12 d64 113 us for 375 MB (3.3
+// TB/s), B2 T1500 H8 d128 39 us for 160 MB. With four waves for all it was 227 us (286 registers, one workgroup a CU), with
+// eight 127, with the pairs' products formed once and no register spilled 107; the decays' gradients by the terms around
+// each token, with Q K^T and K K^T of the lower tiles once more, take 6 of the 113 (2.5 of the 39).
 // Waves 0 to 3 hold dQ and Y of the 16 tokens w, waves 4 to 7 C. What comes from memory for the next 32 value columns is in
 // flight while those in LDS are multiplied.
 template <typename T, int DP>
@@ -672,14 +688,49 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
     }
     lds_barrier();
     const T *keys_own = lds.u.rows.keys + own * S::PITCH + 4 * grp, *queries_own = lds.u.rows.queries + own * S::PITCH + 4 * grp;
-    float end = 0.f;  // sum_j kap_j k_j.(dH' Delta_j)
-    if constexpr (!first) {
+    float end = 0.f;  // eps_i (q_i.(H dO_i) - beta_i k_i.(H dR_i)), or kap_j k_j.(dH' Delta_j)
 #pragma unroll
-      for (int i = 0; i < TILES; ++i) {
-        const f32x4 kf = four(keys_own + 16 * i);
+    for (int i = 0; i < TILES; ++i) {
+      const f32x4 kf = four(keys_own + 16 * i), qf = first ? four(queries_own + 16 * i) : kf;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) end += kf[r] * acc[i][r];
+      for (int r = 0; r < 4; ++r) {
+        end += qf[r] * acc[i][r];
+        if constexpr (first) end -= beta_own * (kf[r] * ay[i][r]);
       }
+    }
+    end = sum_over_rows(end);
+    if (grp == 0) lds.ends[first ? 0 : 1][own] = end;
+    if constexpr (!first) {
+      // the pairs' terms, rows i, columns j: down each column the sums over i >= t, then over the columns j < t
+      float below = 0.f;  // of the tiles below
+#pragma unroll
+      for (int i = 3; i >= 0; --i)
+        if (i >= w) {
+          f32x4 qk = zero4(), kk = zero4();
+#pragma unroll
+          for (int s = 0; s < DP / 32; ++s) {
+            const int f = 32 * s + 8 * grp;
+            const Operand<T, 1> kj = eight(lds.u.rows.keys + own * S::PITCH + f);
+            qk = mma(eight(lds.u.rows.queries + (16 * i + c) * S::PITCH + f), kj, qk);
+            kk = mma(eight(lds.u.rows.keys + (16 * i + c) * S::PITCH + f), kj, kk);
+          }
+          f32x4 x;
+#pragma unroll
+          for (int r = 3; r >= 0; --r) {
+            x[r] = mp[i][r] * qk[r] + mb[i][r] * kk[r];
+            if (r < 3) x[r] += x[r + 1];
+          }
+          // x[0] of the rows' groups behind this one
+          const auto p16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[0]), __float_as_uint(x[0]), false, false);
+          const float odd = __uint_as_float(p16[1]), both = __uint_as_float(p16[0]) + odd;
+          const auto p32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(both), __float_as_uint(both), false, false);
+          const float upper = __uint_as_float(p32[1]);
+          const float behind = ((grp & 1) == 0 ? odd : 0.f) + (grp < 2 ? upper : 0.f) + below;
+          below += __uint_as_float(p32[0]) + upper;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = group_sum<16>(i > w || 4 * grp + r > c ? x[r] + behind : 0.f);
+          if (c == 0) *reinterpret_cast<f32x4*>(&lds.across[w][16 * i + 4 * grp]) = x;
+        }
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -699,33 +750,20 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
       }
 
     // ---- out ----
-    float dot_a = 0.f, dot_y = 0.f;  // q.dQ or k.C, and k.Y
-#pragma unroll
-    for (int i = 0; i < TILES; ++i) {
-      const f32x4 kf = four(keys_own + 16 * i), af = first ? four(queries_own + 16 * i) : kf;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        dot_a += af[r] * acc[i][r];
-        if constexpr (first) dot_y -= kf[r] * ay[i][r];
-      }
-    }
-    dot_a = sum_over_rows(dot_a);
     if constexpr (first) {
+      float dot_y = 0.f;  // k.Y
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) {
+        const f32x4 kf = four(keys_own + 16 * i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dot_y -= kf[r] * ay[i][r];
+      }
       dot_y = sum_over_rows(dot_y);
       dot_v = sum_over_rows(dot_v);
-      if (grp == 0) {
-        lds.dsum[0][own] = dot_a + beta_own * dot_y;
-        if (t0 + own < dims.N) dbeta[((size_t)b * dims.N + t0 + own) * dims.H + h] = from_f32<T>(dot_v + dot_y);
-      }
-    } else if (grp == 0) {
-      lds.dsum[1][own] = dot_a;
+      if (grp == 0 && t0 + own < dims.N) dbeta[((size_t)b * dims.N + t0 + own) * dims.H + h] = from_f32<T>(dot_v + dot_y);
     }
     inner = group_sum<64>(inner);
-    end = group_sum<64>(end);
-    if (l == 0) {
-      lds.part[wave][0] = inner;
-      lds.part[wave][1] = end;
-    }
+    if (l == 0) lds.part[wave] = inner;
     lds_barrier();
     if constexpr (first) {  // dK = beta Y + C
 #pragma unroll
@@ -753,19 +791,20 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void gated_grad_kernel(
   if (wave == 0) {
     const size_t at = ((size_t)b * dims.N + (t0 + l < dims.N ? t0 + l : t0)) * dims.H + h;
     const float gl = g[at];
-    float x = lds.dsum[0][l] - lds.dsum[1][l];  // the sum over this token and those behind it
+    float from = lds.ends[0][l], to = l > 0 ? lds.ends[1][l - 1] : 0.f;  // the sums from this token on, and before it
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const float down = __shfl_down(x, off);
-      if (l + off < 64) x += down;
+      const float down = __shfl_down(from, off), up = __shfl_up(to, off);
+      if (l + off < 64) from += down;
+      if (l >= off) to += up;
     }
-    float hh = 0.f, ee = 0.f;
+    float x = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      hh += lds.part[i][0];
-      ee += lds.part[i][1];
-    }
-    x += lds.coef[2 * kChunk - 1] * hh + ee;
+    for (int i = 0; i < 8; ++i) x += lds.part[i];
+    x = lds.coef[2 * kChunk - 1] * x + from + to;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (16 * i <= l) x += lds.across[i][l];
     // what forgets the state has no gradient
     if (t0 + l < dims.N) dg[at] = (double)gl < kLeastDecay ? 0.f : x;
   }
