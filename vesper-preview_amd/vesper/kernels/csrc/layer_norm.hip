@@ -17,8 +17,9 @@
 // its loads and its stores) and 5 for the columns; 16383 x 768 in float32 30, 35 and 4; 30000 x 513 in bf16 48 and 73 (element by
 // element 116 and 173).
 //
-// A row is scaled by a power of two (exact) that brings its largest deviation below 2^32 before it is squared, so
-// that var does not overflow; eps is scaled with it.
+// A row whose sum passes float32 is summed again in parts of 2^-ceil(log2 d) of its values. A row is scaled by a power of
+// two (exact) that brings its largest deviation below 2^32 before it is squared, so that var does not overflow; eps is
+// scaled with it.
 #include <algorithm>
 #include <initializer_list>
 
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_kernel(
   __shared__ float red[4][16][1];
   constexpr int LANES = 64 * WAVES;
   const int t = threadIdx.x % LANES;
-  // whole waves, and whole workgroups where a barrier follows; the three slots are apart by two barriers
+  // whole waves, and whole workgroups where a barrier follows; between two uses of a slot are two barriers at least
   for (long row = (long)blockIdx.x * NormShape<WAVES>::ROWS + threadIdx.x / LANES; row < rows;
        row += (long)gridDim.x * NormShape<WAVES>::ROWS) {
     const size_t base = (size_t)row * d;
@@ -123,7 +124,17 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_kernel(
       for (int e = 0; e < 8; ++e) sum[0] += inside<EDGE>(f, e, d) ? v[j][e] : 0.f;
     }
     row_reduce<WAVES, 1>(sum, red, 0, SumOp{});
-    const float mu = sum[0] / (float)d;
+    float mu = sum[0] / (float)d;
+    if (!(fabsf(sum[0]) <= 3.40282347e38f)) {  // the same for all of the row's lanes: its sum overflowed (or a value is none)
+      const float part = __builtin_ldexpf(1.f, d > 1 ? __builtin_clz((unsigned)(d - 1)) - 32 : 0);
+      float again[1] = {0.f};
+#pragma unroll
+      for (int j = 0; j < SEG; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) again[0] += inside<EDGE>(8 * (t + LANES * j), e, d) ? v[j][e] * part : 0.f;
+      row_reduce<WAVES, 1>(again, red, 3, SumOp{});
+      mu = again[0] / ((float)d * part);
+    }
     float peak[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < SEG; ++j) {

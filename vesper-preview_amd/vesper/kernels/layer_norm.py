@@ -106,7 +106,8 @@ def layer_norm(x: Tensor, gain: Tensor, bias: Tensor | None = None, *, residual:
 
     Under autograd the gradients of ``x``, ``residual``, ``gain`` and ``bias`` (each in its input's dtype) come from the
     backward kernels, from the float32 sum; they may be captured into a graph, as long as no eager graph of the same leaves
-    is alive (torch's accumulation into them would leave the capture). Finite rows below ``2 ** 126`` give finite norms.
+    is alive (torch's accumulation into them would leave the capture). Rows of sums ``s`` below ``2 ** 126`` give finite
+    norms, however large their own sum is.
 
     Raises:
         ContractError: on a dtype, width, shape or device outside that contract, before any kernel runs.
