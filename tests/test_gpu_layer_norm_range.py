@@ -81,6 +81,30 @@ def test_sums_with_a_residual_that_pass_float32(d):
     _check(x.to(BF16), r.to(BF16), BF16, 1e-5, 1.5e-4)
 
 
+@pytest.mark.parametrize("types", [(F32, F32), (F32, BF16), (BF16, BF16)], ids=str)
+@pytest.mark.parametrize("eps", [0.0, 2.0**-140])
+@pytest.mark.parametrize("d", [2, 8, 513, 1024, 4096, 16384])
+def test_rows_of_small_deviations_without_an_eps(types, eps, d):
+    """Squares below float32 beside an eps of nothing: deviations of 2^-80 and 2^-110, and plain and large rows between."""
+    x = torch.randn(5, d, generator=torch.Generator().manual_seed(d))
+    x[:, ::2] += 1  # two values that differ
+    for row, scale in ((0, 2.0**-80), (1, 2.0**-110), (3, 2.0**80), (4, 2.0**-40)):
+        x[row] *= scale
+    _check(x.to(types[0]), None, types[1], eps, 2e-5)
+
+
+def test_the_smallest_rows_and_rows_without_deviations():
+    from vesper.kernels.layer_norm import layer_norm
+
+    x = torch.zeros(4, 256)
+    x[0, ::2], x[1, ::2], x[2, ::2] = 2.0**-126, 2.0**-145, 1.0
+    y = layer_norm(x.to(GPU), torch.ones(256, device=GPU), eps=0.0).cpu()
+    want = torch.ones(256).index_fill(0, torch.arange(1, 256, 2), -1.0)  # exact: powers of two throughout
+    assert torch.equal(y[:3], want.expand(3, 256)) and bool(y[3].isnan().all())
+    small = layer_norm(x.to(GPU), torch.ones(256, device=GPU), eps=1e-5).cpu()
+    assert float(small[1].abs().max()) < 2.0**-130 and not bool(small[3].any())
+
+
 def test_a_row_of_infinities_or_nan_stays_one():
     from vesper.kernels.layer_norm import layer_norm
 

@@ -19,7 +19,8 @@
 //
 // A row whose sum passes float32 is summed again in parts of 2^-ceil(log2 d) of its values. A row is scaled by a power of
 // two (exact) that brings its largest deviation below 2^32 before it is squared, so that var does not overflow; eps is
-// scaled with it.
+// scaled with it. So is, up, a row of small deviations where eps is next to nothing (below 2^-100), so that the squares
+// do not vanish; beside a larger eps what is lost of them does not count.
 #include <algorithm>
 #include <initializer_list>
 
@@ -147,7 +148,10 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_kernel(
     }
     row_reduce<WAVES, 1>(peak, red, 1, MaxOp{});
     float scale = 1.f;
-    if (peak[0] > 4294967296.f) scale = __builtin_ldexpf(1.f, 32 - __builtin_amdgcn_frexp_expf(peak[0]));
+    if (peak[0] > 4294967296.f || (eps < 0x1p-100f && peak[0] < 0x1p-32f && peak[0] > 0.f)) {
+      const int up = 32 - __builtin_amdgcn_frexp_expf(peak[0]);
+      scale = __builtin_ldexpf(1.f, up < 100 ? up : 100);
+    }
     float sq[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < SEG; ++j)
@@ -157,7 +161,7 @@ __global__ __launch_bounds__(NormShape<WAVES>::NT) void layer_norm_kernel(
         sq[0] += v[j][e] * v[j][e];
       }
     row_reduce<WAVES, 1>(sq, red, 2, SumOp{});
-    const float root = 1.f / __builtin_sqrtf(sq[0] / (float)d + eps * (scale * scale));
+    const float root = 1.f / __builtin_sqrtf(sq[0] / (float)d + eps * scale * scale);
     if (stats != nullptr && t == 0) {
       stats[2 * (size_t)row] = mu;
       stats[2 * (size_t)row + 1] = root * scale;

@@ -98,7 +98,8 @@ def layer_norm(x: Tensor, gain: Tensor, bias: Tensor | None = None, *, residual:
         gain: float32 ``[d]``.
         bias: optional float32 ``[d]``.
         residual: optional tensor shaped like ``x``: of x's dtype, or with a float32 ``x`` of any of the three.
-        eps: added to the variance; finite, not negative.
+        eps: added to the variance; finite, not negative. With 0 a row without deviations is NaN (0 / 0), and gradients are
+            finite from deviations of ``2 ** -120`` on.
         dtype: the norm's dtype, with a float32 ``x`` any of the three (by default x's).
 
     Returns:
