@@ -114,3 +114,26 @@ def test_a_row_of_infinities_or_nan_stays_one():
     y = layer_norm(x.to(GPU), torch.ones(700, device=GPU))
     assert bool(y[1].isnan().any()) and bool(y[2].isnan().all())
     assert torch.equal(y[0], clean[0]) and torch.equal(y[3], clean[3])
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (F32, BF16), (BF16, BF16)], ids=str)
+@pytest.mark.parametrize("d", [8, 264, 768, 2048, 8192])
+def test_memory_at_16_but_not_32_bytes_gives_the_same_bits(types, d):
+    from vesper.kernels.layer_norm import layer_norm
+
+    def moved(t):
+        buf = torch.empty(t.numel() + 32, dtype=t.dtype, device=GPU)
+        first = next(i for i in range(32) if (buf.data_ptr() + i * t.element_size()) % 32 == 16)
+        return buf[first : first + t.numel()].view(t.shape).copy_(t)
+
+    gen = torch.Generator().manual_seed(d)
+    t = [torch.randn(33, d, generator=gen).to(GPU, types[0]), torch.rand(d, generator=gen).to(GPU), torch.rand(d, generator=gen).to(GPU),
+         torch.randn(33, d, generator=gen).to(GPU, types[0])]
+    dy, ds = torch.randn(33, d, generator=gen).to(GPU, types[1]), torch.randn(33, d, generator=gen).to(GPU, types[0])
+    results = []
+    for change in (lambda v: v, moved):
+        leaves = [change(v).detach().requires_grad_() for v in t]
+        y, s = layer_norm(*leaves[:3], residual=leaves[3], dtype=types[1])
+        results.append([y, s, *torch.autograd.grad([y, s], leaves, [change(dy), change(ds)])])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)

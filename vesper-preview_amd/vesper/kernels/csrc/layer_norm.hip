@@ -58,7 +58,7 @@ template <bool EDGE> __device__ __forceinline__ bool inside(int f, int e, int d)
 
 // as they come from memory, converted where they are used: 16-bit values take half of the registers
 template <typename T> struct Piece {
-  typedef T V8 __attribute__((ext_vector_type(8)));
+  typedef T V8 __attribute__((ext_vector_type(8), aligned(16)));  // as the launcher checks it (eight floats of their own: 32)
   typedef T V8u __attribute__((ext_vector_type(8), aligned(sizeof(T))));
   V8 x;
   template <bool EDGE> __device__ __forceinline__ void load(const T* row, int f, int d) {
