@@ -120,7 +120,7 @@ def layer_norm(x: Tensor, gain: Tensor, bias: Tensor | None = None, *, residual:
     if x.numel() == 0 or not grad:
         if x.numel() == 0:  # no rows: empty results that keep the graph
             total = x if residual is None else x + residual.to(x.dtype)
-            y = (total * gain.sum()).to(out)
+            y = (total * gain if bias is None else total * gain + bias).to(out)
             return y if residual is None else (y, total)
         y, total = _forward(x.contiguous(), gain.contiguous(), None if bias is None else bias.contiguous(),
                             None if residual is None else residual.contiguous(), eps, out, None)
