@@ -33,3 +33,22 @@ def test_the_norm_of_no_rows_has_every_gradient(types, lead):
     assert only.requires_grad and not bool(torch.autograd.grad(only.sum(), bias)[0].any())
     with torch.no_grad():
         assert not layer_norm(x, gain, bias, dtype=types[2]).requires_grad
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize(("b", "n", "h", "dk"), [(0, 5, 2, 16), (2, 5, 0, 16), (0, 1, 2, 12), (0, 3, 0, 1)])
+def test_the_scan_of_an_empty_batch_has_every_gradient(dtype, b, n, h, dk):
+    from vesper.kernels.gated_scan import gated_delta_scan
+
+    leaves = [*(_leaf(b, n, h, dk, dtype=dtype) for _ in range(3)), _leaf(b, n, h, dtype=dtype), _leaf(b, n, h), _leaf(b, h, dk, dk)]
+    o, after = gated_delta_scan(*leaves, active=_on(torch.ones(b, n, dtype=torch.bool)))
+    assert o.shape == leaves[0].shape and o.dtype == dtype and after.shape == leaves[5].shape and after.dtype == F32
+    for result in (o, after):
+        grads = torch.autograd.grad(result.sum(), leaves, retain_graph=True)
+        for leaf, grad in zip(leaves, grads):
+            assert grad.shape == leaf.shape and grad.dtype == leaf.dtype
+    only = gated_delta_scan(*(t.detach() for t in leaves[:4]), leaves[4], leaves[5].detach())  # the decays alone
+    assert all(t.requires_grad for t in only)
+    with torch.no_grad():
+        o, after = gated_delta_scan(*leaves)
+    assert not o.requires_grad and not after.requires_grad and after is not leaves[5]

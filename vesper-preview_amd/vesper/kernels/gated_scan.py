@@ -163,8 +163,9 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
     if dims["n"] == 0:
         return q, state
     mask = None if active is None else _active_mask(active, ("b", "n"), dims, q.device)
-    if dims["b"] == 0 or dims["h"] == 0:
-        return torch.zeros_like(q), state.clone()
+    if dims["b"] == 0 or dims["h"] == 0:  # empty results that keep the graph
+        o = q + k + v + (beta + g.to(q.dtype))[..., None] + state.sum().to(q.dtype)
+        return o, state + o.sum().to(STATE_DTYPE)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or beta.requires_grad
                                         or g.requires_grad or state.requires_grad)
     dk = dims["dk"]
