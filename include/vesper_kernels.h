@@ -568,8 +568,8 @@ int vsp_project_int8_f32(const int8_t* z, const float* z_scale, const int8_t* we
  * The delta rule with a decay of the state before each token, g float32 [B, N, H] its logarithm (at most 0;
  * -inf forgets the state): H_t = e^g H_{t-1} + k_t u_t^T, u_t = beta_t (v_t - e^g H_{t-1}^T k_t), o_t = H_t^T q_t.
  * q, k, v, o [B, N, H, D], beta [B, N, H] of the type the name ends in, the states float32 [B, H, D, D]. D a
- * multiple of 8 in 8..256, H * D at most 2^22, N at most 2^30, at most 2^25 chunks of 64 tokens and 2^22 slices of 16 value columns over
- * all heads. The workspace (vsp_gated_scan_workspace_bytes; no initial contents, not shared by calls that may
+ * multiple of 8 in 8..256, H * D at most 2^22, N at most 2^30, at most 2^25 chunks of 64 tokens (with records, and in
+ * the backward: fewer than 2^23) and 2^22 slices of 16 value columns over all heads. The workspace (vsp_gated_scan_workspace_bytes; no initial contents, not shared by calls that may
  * overlap in time) holds each chunk's decays and triangular factors, and for few long rows the states and maps of their
  * segments. `records` (vsp_gated_scan_records_bytes, or NULL)
  * receives what the backward pass needs: each chunk's starting state and corrections in float32. q, k, v, o, the

@@ -392,7 +392,8 @@ template <typename T>
 int launch_prep(const T* q, const T* k, const T* beta, const float* g, float* coef, T* tf, T* pf, int B, int N, int H,
                 int D, bool columns, hipStream_t stream);
 
-int check_sizes(int B, int N, int H, int D, const char* who);
+// `kept`: a forward that keeps records, or the backward, whose last kernel has 512 threads a chunk.
+int check_sizes(int B, int N, int H, int D, bool kept, const char* who);
 
 // the records of a forward that a backward follows, float32 accumulator tiles (rows features or tokens, columns values): of
 // each chunk its starting state, tile (value tile) * tiles + (feature tile); then of each its Delta, tile (value tile) * 4 +

@@ -835,7 +835,7 @@ int scan_backward(const void* q_, const void* k_, const void* v_, const void* be
                   const float* records, size_t records_bytes, const void* d_o_, const float* d_state,
                   const uint8_t* active, void* dq_, void* dk_, void* dv_, void* dbeta_, float* dg, float* d_state_in,
                   void* ws, size_t ws_bytes, int B, int N, int H, int D, hipStream_t stream, const char* who) {
-  if (const int st = check_sizes(B, N, H, D, who); st != OK) return st;
+  if (const int st = check_sizes(B, N, H, D, true, who); st != OK) return st;
   if (B == 0 || N == 0) return fail(ERR_ARG, "%s: no tokens (B=%d N=%d)", who, B, N);
   const size_t total = (size_t)B * H * chunks_of(N);
   if (!q_ || !k_ || !v_ || !beta_ || !g || !records || !d_o_ || !dq_ || !dk_ || !dv_ || !dbeta_ || !dg || !d_state_in || !ws)

@@ -877,7 +877,7 @@ template <typename T>
 int scan(const void* q_, const void* k_, const void* v_, const void* beta_, const float* g, const float* s_in, void* o_,
          float* s_out, void* ws, size_t ws_bytes, float* records, size_t records_bytes, const uint8_t* active, int B,
          int N, int H, int D, hipStream_t stream, const char* who) {
-  if (const int st = check_sizes(B, N, H, D, who); st != OK) return st;
+  if (const int st = check_sizes(B, N, H, D, records != nullptr, who); st != OK) return st;
   if (B == 0 || N == 0) return fail(ERR_ARG, "%s: no tokens (B=%d N=%d)", who, B, N);
   const size_t total = (size_t)B * H * chunks_of(N);
   if (!q_ || !k_ || !v_ || !beta_ || !g || !s_in || !o_ || !s_out || !ws) return fail(ERR_ARG, "%s: null pointer", who);
@@ -925,15 +925,18 @@ int launch_prep(const T* q, const T* k, const T* beta, const float* g, float* co
 template int launch_prep<__bf16>(const __bf16*, const __bf16*, const __bf16*, const float*, float*, __bf16*, __bf16*, int, int, int, int, bool, hipStream_t);
 template int launch_prep<float>(const float*, const float*, const float*, const float*, float*, float*, float*, int, int, int, int, bool, hipStream_t);
 
-int check_sizes(int B, int N, int H, int D, const char* who) {
+int check_sizes(int B, int N, int H, int D, bool kept, const char* who) {
   if (B < 0 || N < 0 || H < 1) return fail(ERR_ARG, "%s: bad sizes B=%d N=%d H=%d", who, B, N, H);
   if (D < 8 || D > 256 || D % 8 != 0) return fail(ERR_UNSUPPORTED, "%s: head dimension %d (multiples of 8 in 8..256)", who, D);
   if (N > (1 << 30)) return fail(ERR_UNSUPPORTED, "%s: %d tokens a row (at most 2^30)", who, N);
   // a chunk's rows are addressed by 32-bit offsets
   if ((size_t)H * D > (size_t)1 << 22) return fail(ERR_UNSUPPORTED, "%s: tokens of %d x %d features (at most 2^22)", who, H, D);
-  // launches of fewer than 2^32 threads, counts in 32 bits: a wave a chunk and head, 512 threads a slice
+  // launches of fewer than 2^32 threads, counts in 32 bits: a wave a chunk and head, 512 threads a slice; of the backward
+  // 512 a chunk and head
   if ((size_t)B * H * chunks_of(N) > (size_t)1 << 25 || (size_t)B * H * ((D + 15) / 16) > (size_t)1 << 22)
     return fail(ERR_UNSUPPORTED, "%s: B=%d N=%d H=%d (at most 2^25 chunks of 64 tokens, 2^22 slices of 16 value columns)", who, B, N, H);
+  if (kept && (size_t)B * H * chunks_of(N) >= (size_t)1 << 23)
+    return fail(ERR_UNSUPPORTED, "%s: B=%d N=%d H=%d (fewer than 2^23 chunks of 64 tokens with records)", who, B, N, H);
   return OK;
 }
 

@@ -30,6 +30,11 @@ from vesper.kernels.delta_scan import MAX_HEAD_DIM, STATE_DTYPE, _active_mask, _
 
 GATE_DTYPE = torch.float32  # the log decays: sums of many of them decide what is left of a state
 INPUT_DTYPES = (torch.bfloat16, torch.float32)  # of q, k, v and beta, all alike
+MAX_TOKENS = 2**30  # of a row
+MAX_FEATURES = 2**22  # of a token's heads, a head's rounded up to a multiple of 8
+MAX_CHUNKS = 2**25  # of 64 tokens, over all rows and heads
+MAX_KEPT_CHUNKS = 2**23 - 1  # where the backward follows: 512 threads each
+MAX_SLICES = 2**22  # of 16 value columns, over all rows and heads
 _SUFFIX = {torch.bfloat16: "bf16", torch.float32: "f32"}
 _STEP = {dtype: f"vsp_gated_step_{suffix}" for dtype, suffix in _SUFFIX.items()}
 _SCAN = {dtype: f"vsp_gated_scan_{suffix}" for dtype, suffix in _SUFFIX.items()}
@@ -69,6 +74,23 @@ def _check(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tens
         raise ContractError(f"head dimension {dims['dk']} exceeds the kernel's {MAX_HEAD_DIM}" if dims["dk"]
                             else "head dimension 0: the kernel takes 1 and more")
     return dims
+
+
+def _check_sizes(b: int, n: int, h: int, dk: int, grad: bool) -> None:
+    """Raises for sizes past the kernels' launches and offsets (what the C entries count in 32 bits among them)."""
+    chunks, slices = b * h * -(-n // 64), b * h * -(-dk // 16)
+    if (n <= MAX_TOKENS and h * dk <= MAX_FEATURES - 7 * h and chunks <= (MAX_KEPT_CHUNKS if grad else MAX_CHUNKS)
+            and slices <= MAX_SLICES):
+        return
+    if n > MAX_TOKENS:
+        raise ContractError(f"q: {n} tokens a row, the kernels take at most 2**30")
+    if h * (dk + -dk % 8) > MAX_FEATURES:
+        raise ContractError(f"q: {h} heads of {dk + -dk % 8} features a token, the kernels take at most 2**22 features")
+    if chunks > MAX_CHUNKS or (grad and chunks > MAX_KEPT_CHUNKS):
+        most = "2**23 - 1 under autograd" if grad else "2**25"
+        raise ContractError(f"q: {chunks} chunks of 64 tokens over all rows and heads, the kernels take at most {most}")
+    if slices > MAX_SLICES:
+        raise ContractError(f"q: {slices} slices of 16 value columns over all rows and heads, the kernels take at most 2**22")
 
 
 def _forward(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor, mask: Tensor | None,
@@ -154,8 +176,11 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
     (torch's accumulation into them would leave the capture). A NaN or an infinity in a token reaches its head's outputs from the start of its chunk on (a
     chunk's products are over all pairs of its tokens), not those of other heads and rows.
 
+    At most ``2**30`` tokens a row, ``2**22`` features a token (a head's rounded up to a multiple of 8), ``2**25`` chunks of 64
+    tokens (``2**23 - 1`` under autograd) and ``2**22`` slices of 16 value columns over all rows and heads.
+
     Raises:
-        ContractError: on a dtype, shape, device or width outside the contract, before any kernel runs.
+        ContractError: on a dtype, shape, device, width or size outside the contract, before any kernel runs.
     """
     dims = _check(q, k, v, beta, g, state, ("b", "n", "h"))
     if active is not None:
@@ -173,6 +198,7 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
         first = (t[:, 0] for t in (q, k, v, beta, g))
         o, after = gated_delta_step(*first, state.contiguous(), active=None if active is None else active[:, 0])
         return o[:, None], after
+    _check_sizes(dims["b"], dims["n"], dims["h"], dk, grad)
     pad = -dk % 8
     if pad:
         q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))
