@@ -61,7 +61,7 @@ def test_a_scan_that_keeps_records_takes_fewer_chunks(reached):
     assert not reached
 
 
-@pytest.mark.parametrize("size", [(1, 2**30, 1, 256, True), (1, 64, 2**19, 1, False), (1, 64, 2**14, 256, False), (2**25 // 8, 512, 1, 8, False),
+@pytest.mark.parametrize("size", [(1, 2**30, 1, 256, False), (1, 2**29 - 64, 1, 256, True), (1, 64, 2**19, 1, False), (1, 64, 2**14, 256, False), (2**25 // 8, 512, 1, 8, False),
                                   (2**22, 64, 1, 16, True), (2**23 - 1, 64, 1, 16, True)], ids=str)
 def test_the_limits_themselves_are_taken(size):
     from vesper.contracts import ContractError
