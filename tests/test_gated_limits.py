@@ -87,3 +87,40 @@ def test_the_c_entries_refuse_as_many_chunks():
     assert "null" in lib.vsp_last_error().decode()
     assert lib.vsp_gated_scan_backward_bf16(*[None] * 6, 0, *[None] * 10, 0, 2**12, 2**17 - 64, 1, 8, None) != 0
     assert "null" in lib.vsp_last_error().decode()
+
+
+def test_a_step_of_more_heads_than_a_launch_takes_runs_in_parts(reached):
+    """2^20 heads and more, by the step and by a scan of one token: rows of fewer than 2^20 heads a launch, in order."""
+    from vesper.kernels.gated_scan import gated_delta_scan, gated_delta_step
+
+    b, h, dk = 2**17 + 3, 8, 1
+    lead = [torch.zeros(b, h, dk, dtype=BF16).as_subclass(_Wide) for _ in range(3)]
+    beta, g = torch.zeros(b, h, dtype=BF16).as_subclass(_Wide), torch.zeros(b, h).as_subclass(_Wide)
+    state = torch.zeros(b, h, dk, dk).as_subclass(_Wide)
+    active = torch.ones(b, dtype=torch.bool).as_subclass(_Wide)
+    with torch.no_grad():
+        o, after = gated_delta_step(*lead, beta, g, state, active=active, out_state=state)
+        assert o.shape == (b, h, dk) and after is state
+        gated_delta_scan(*(t[:, None] for t in lead), beta[:, None], g[:, None], state)
+    assert len(reached) == 4 and {name for name, _ in reached} == {"vsp_gated_step_bf16"}
+    for calls in (reached[:2], reached[2:]):
+        first = 0
+        for _, args in calls:
+            rows, heads, width = args[-3:]
+            assert rows * heads < 2**20 and (heads, width) == (h, dk)
+            for at, t in zip(args, (*lead, beta, g, state)):
+                assert at == t.data_ptr() + first * t[:1].nbytes
+            first += rows
+        assert first == b
+    first = reached[0][1][-3]
+    for before, behind, t in zip(reached[0][1][6:9], reached[1][1][6:9], (state, o, active)):
+        assert before == t.data_ptr() and behind == t.data_ptr() + first * t[:1].nbytes
+
+
+def test_a_step_of_more_heads_a_row_is_refused(reached):
+    from vesper.contracts import ContractError
+    from vesper.kernels.gated_scan import gated_delta_step
+
+    with pytest.raises(ContractError, match="heads"):
+        gated_delta_step(*_args(1, None, 2**20, 1))
+    assert not reached

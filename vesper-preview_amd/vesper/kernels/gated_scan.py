@@ -35,6 +35,7 @@ MAX_FEATURES = 2**22  # of a token's heads, a head's rounded up to a multiple of
 MAX_CHUNKS = 2**25  # of 64 tokens, over all rows and heads
 MAX_KEPT_CHUNKS = 2**23 - 1  # where the backward follows: 512 threads each
 MAX_SLICES = 2**22  # of 16 value columns, over all rows and heads
+MAX_STEP_HEADS = 2**20 - 1  # rows times heads of one launch of the step
 _SUFFIX = {torch.bfloat16: "bf16", torch.float32: "f32"}
 _STEP = {dtype: f"vsp_gated_step_{suffix}" for dtype, suffix in _SUFFIX.items()}
 _SCAN = {dtype: f"vsp_gated_scan_{suffix}" for dtype, suffix in _SUFFIX.items()}
@@ -215,7 +216,8 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
     """One token per row through the gated delta rule, decayed, written, then read: ``(H'^T q, H')``.
 
     Args:
-        q, k, v: ``[b, h, dk]`` float32 or bfloat16 (all three alike, ``beta [b, h]`` too), ``dk`` in 1..256.
+        q, k, v: ``[b, h, dk]`` float32 or bfloat16 (all three alike, ``beta [b, h]`` too), ``dk`` in 1..256, ``h`` under
+            ``2**20`` (rows of as many heads in all run in one launch, more in several).
         g: the log decays ``[b, h]``, float32.
         state: ``[b, h, dk, dk]`` float32, contiguous.
         active: optional bool ``[b]``; an inactive row decays and writes the state and reads zero.
@@ -233,6 +235,8 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
     if torch.is_grad_enabled():
         _refuse_grad(q, k, v, beta, g, state)
     b, h, dk = q.shape
+    if h > MAX_STEP_HEADS:
+        raise ContractError(f"q: {h} heads, the step takes at most 2**20 - 1")
     if not state.is_contiguous():
         raise ContractError("state must be contiguous")
     if out_state is None:
@@ -251,6 +255,19 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
     o = torch.empty_like(q)
     if b == 0 or h == 0:
         return o, out_state
+    if b * h <= MAX_STEP_HEADS:
+        _launch_step(q, k, v, beta, g, state, out_state, o, mask)
+        return o, out_state
+    rows = MAX_STEP_HEADS // h
+    for i in range(0, b, rows):
+        part = slice(i, i + rows)
+        _launch_step(q[part], k[part], v[part], beta[part], g[part], state[part], out_state[part], o[part],
+                     None if mask is None else mask[part])
+    return o, out_state
+
+
+def _launch_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor, out_state: Tensor, o: Tensor,
+                 mask: Tensor | None) -> None:
+    b, h, dk = q.shape
     _lib.launch(q.device, _STEP[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(), g.data_ptr(),
                 state.data_ptr(), out_state.data_ptr(), o.data_ptr(), None if mask is None else mask.data_ptr(), b, h, dk)
-    return o, out_state
