@@ -124,3 +124,33 @@ def test_a_step_of_more_heads_a_row_is_refused(reached):
     with pytest.raises(ContractError, match="heads"):
         gated_delta_step(*_args(1, None, 2**20, 1))
     assert not reached
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_a_new_state_over_another_input_is_refused(reached, which):
+    """Tokens within or at the ends of out_state's memory; right before and right behind it they are taken."""
+    from vesper.contracts import ContractError
+    from vesper.kernels.gated_scan import gated_delta_step
+
+    b, h, dk = 2, 3, 4
+    sizes = [b * h * dk] * 3 + [b * h] * 2
+    shapes = [(b, h, dk)] * 3 + [(b, h)] * 2
+    buf = torch.zeros(1000)
+    held = buf[300 : 300 + b * h * dk * dk]
+    out = held.view(b, h, dk, dk).as_subclass(_Wide)
+    tokens = [torch.zeros(s).as_subclass(_Wide) for s in shapes]
+    size = sizes[which]
+
+    def call(at, **more):
+        args = list(tokens)
+        args[which] = buf[at : at + size].view(shapes[which]).as_subclass(_Wide)
+        return gated_delta_step(*args, **more)
+
+    for state in (out, torch.zeros(b, h, dk, dk).as_subclass(_Wide)):
+        for at in (300 - size + 1, 300, 310, 300 + held.numel() - 1):
+            with pytest.raises(ContractError, match="overlap"):
+                call(at, state=state, out_state=out)
+        for at in (300 - size, 300 + held.numel()):
+            call(at, state=state, out_state=out)
+    call(310, state=out)  # read only
+    assert len(reached) == 5

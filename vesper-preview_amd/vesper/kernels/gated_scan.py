@@ -222,7 +222,7 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
         state: ``[b, h, dk, dk]`` float32, contiguous.
         active: optional bool ``[b]``; an inactive row decays and writes the state and reads zero.
         out_state: optional contiguous float32 tensor shaped like ``state`` that receives the new state; it may be
-            ``state`` itself (an in-place decode step), and overlaps it in no other way.
+            ``state`` itself (an in-place decode step), and overlaps it and the other inputs in no other way.
 
     Returns:
         ``(o [b, h, dk], state')`` with ``o`` in the inputs' dtype.
@@ -239,6 +239,7 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
         raise ContractError(f"q: {h} heads, the step takes at most 2**20 - 1")
     if not state.is_contiguous():
         raise ContractError("state must be contiguous")
+    given = out_state is not None
     if out_state is None:
         out_state = torch.empty_like(state)
     else:
@@ -251,6 +252,13 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
         if 0 < apart < state.nbytes:
             raise ContractError("out_state must be state itself or not overlap it")
     q, k, v, beta, g = q.contiguous(), k.contiguous(), v.contiguous(), beta.contiguous(), g.contiguous()
+    if given and b * h:  # other workgroups would still read what one has written
+        first, row = out_state.data_ptr(), b * h * q.element_size()
+        behind = first + 4 * b * h * dk * dk
+        for t, size in ((q, row * dk), (k, row * dk), (v, row * dk), (beta, row), (g, 4 * b * h)):
+            at = t.data_ptr()
+            if at < behind and first < at + size:
+                raise ContractError("out_state must not overlap q, k, v, beta or g")
     mask = None if active is None else _active_mask(active, ("b",), dims, q.device)
     o = torch.empty_like(q)
     if b == 0 or h == 0:
