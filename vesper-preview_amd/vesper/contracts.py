@@ -8,6 +8,7 @@ dtype mismatch says "dtype"), so callers and tests written against the reference
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 Dims = dict[str, int]
 DimSpec = tuple
@@ -42,6 +43,20 @@ def _refuse_shape(name: str, shape: tuple[int, ...], spec: DimSpec, dims: Dims) 
                 raise ContractError(f"{name}: axis {axis} must be {want}, got {got} (shape {shape})")
         elif dims[want] != got:
             raise ContractError(f"{name}: axis {axis} '{want}' is {got}, but '{want}' = {dims[want]} elsewhere")
+
+
+def refuse_tangents(*tensors: torch.Tensor | None) -> None:
+    """Refuses inputs with a tangent, for kernels without a forward-mode derivative: they read memory, where no tangent is, and
+    the result would have none.
+
+    Raises:
+        ContractError: on a tensor with a tangent at the current forward-mode level.
+    """
+    if forward_ad._current_level < 0:  # noqa: SLF001
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ContractError("the kernel has no forward-mode derivative: an input has a tangent")
 
 
 def require(condition: torch.Tensor, message: str) -> None:

@@ -34,7 +34,7 @@ from typing import Any
 import torch
 from torch import Tensor
 
-from vesper.contracts import ContractError, Dims, check_shape
+from vesper.contracts import ContractError, Dims, check_shape, refuse_tangents
 from vesper.kernels import _lib
 
 MAX_HEAD_DIM = 256  # delta_scan.py:41 in the reference; the HIP kernels take any width up to it
@@ -79,6 +79,7 @@ def _checked_length(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, state: Tensor
             raise ContractError(f"{name} is on {tensor.device}, q on {q.device}")
     if dims["dk"] > MAX_HEAD_DIM:
         raise ContractError(f"head dimension {dims['dk']} exceeds the kernel's {MAX_HEAD_DIM}")
+    refuse_tangents(q, k, v, beta, state)
     return dims["n"]
 
 
@@ -206,6 +207,7 @@ def _autograd_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, state: Tensor,
     mask = _active_mask(active, ("b", "n"), {"b": b, "n": n}, q.device)
     if carried is not None:
         carried = _checked_carried(carried, k, v, beta, active)
+        refuse_tangents(*carried)
     grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, beta, state, *(carried or ())))
     if grad and carried is not None and active is not None:
         # under autograd the merge is explicit, so the gradient reaches the carried tensors
@@ -306,6 +308,7 @@ def delta_scan_step_fused(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, state: 
     if dims["dk"] > MAX_HEAD_DIM:
         raise ContractError(f"head dimension {dims['dk']} exceeds the kernel's {MAX_HEAD_DIM}")
     _refuse_grad(q, k, v, beta, state)
+    refuse_tangents(q, k, v, beta, state)
     b, h, dk = q.shape
     q, k, v, beta = (t.contiguous() for t in (q, k, v, beta))
     if not state.is_contiguous():

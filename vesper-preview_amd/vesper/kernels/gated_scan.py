@@ -24,7 +24,7 @@ import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
-from vesper.contracts import ContractError, Dims, check_shape
+from vesper.contracts import ContractError, Dims, check_shape, refuse_tangents
 from vesper.kernels import _lib
 from vesper.kernels.delta_scan import MAX_HEAD_DIM, STATE_DTYPE, _active_mask, _aligned, _refuse_grad
 
@@ -181,9 +181,11 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
     tokens (``2**23 - 1`` under autograd) and ``2**22`` slices of 16 value columns over all rows and heads.
 
     Raises:
-        ContractError: on a dtype, shape, device, width or size outside the contract, before any kernel runs.
+        ContractError: on a dtype, shape, device, width or size outside the contract or a forward-mode tangent, before any
+            kernel runs.
     """
     dims = _check(q, k, v, beta, g, state, ("b", "n", "h"))
+    refuse_tangents(q, k, v, beta, g, state)
     if active is not None:
         check_shape("active", active, ("b", "n"), dims, torch.bool)
     if dims["n"] == 0:
@@ -232,6 +234,7 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
             while grad mode is on.
     """
     dims = _check(q, k, v, beta, g, state, ("b", "h"))
+    refuse_tangents(q, k, v, beta, g, state)
     if torch.is_grad_enabled():
         _refuse_grad(q, k, v, beta, g, state)
     b, h, dk = q.shape

@@ -15,7 +15,7 @@ import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
-from vesper.contracts import ContractError
+from vesper.contracts import ContractError, refuse_tangents
 from vesper.kernels import _lib
 
 MAX_WIDTH = 16384
@@ -111,10 +111,12 @@ def layer_norm(x: Tensor, gain: Tensor, bias: Tensor | None = None, *, residual:
     norms, however large their own sum is.
 
     Raises:
-        ContractError: on a dtype, width, shape or device outside that contract, before any kernel runs.
+        ContractError: on a dtype, width, shape or device outside that contract or a forward-mode tangent, before any kernel
+            runs.
     """
     out = x.dtype if dtype is None else dtype
     d = _check(x, gain, bias, residual, eps, out)
+    refuse_tangents(x, gain, bias, residual)
     grad = torch.is_grad_enabled() and (x.requires_grad or gain.requires_grad or (bias is not None and bias.requires_grad)
                                         or (residual is not None and residual.requires_grad))
     if x.numel() == 0 or not grad:
