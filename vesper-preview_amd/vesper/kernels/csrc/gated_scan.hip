@@ -22,7 +22,8 @@ namespace {
 constexpr int kPad = 20;                   // pitch of a 16 x 16 float32 tile in LDS
 constexpr int kTile = 16 * kPad + 4;       // tiles start on other banks
 constexpr int kPrepWaves = 4;
-constexpr int kLineChunks = 256;  // up to a workgroup a CU, prep by lines
+// Up to so many chunks prep by lines: a workgroup a CU, in float32, whose products are longer, two.
+template <typename T> constexpr int kLineChunks = sizeof(T) == 2 ? 256 : 512;
 
 struct PrepLds {
   float hi[kChunk], lo[kChunk];  // both parts of the decays' sums
@@ -832,7 +833,7 @@ int segments_of(int B, int N, int H, int D) {
 template <typename T, int DP>
 void launch_prep_width(const T* q, const T* k, const T* beta, const float* g, float* coef, T* tf, T* pf, Dims<T> dims,
                        int total, bool columns, hipStream_t stream) {
-  if (total <= kLineChunks) {
+  if (total <= kLineChunks<T>) {
     const dim3 grid((unsigned)total), block(256);
     if (columns) hipLaunchKernelGGL((gated_prep_lines_kernel<T, DP, true>), grid, block, 0, stream, q, k, beta, g, coef, tf, pf, dims);
     else hipLaunchKernelGGL((gated_prep_lines_kernel<T, DP, false>), grid, block, 0, stream, q, k, beta, g, coef, tf, pf, dims);
