@@ -137,3 +137,27 @@ def test_memory_at_16_but_not_32_bytes_gives_the_same_bits(types, d):
         results.append([y, s, *torch.autograd.grad([y, s], leaves, [change(dy), change(ds)])])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16)], ids=str)
+@pytest.mark.parametrize("size", [(300000, 64), (40000, 513), (20001, 1024), (9000, 4096)], ids=str)
+def test_sums_over_many_rows(types, size):
+    """The gain's and the bias's gradients of many rows. At most 1024 workgroups, at least one a CU, 256, add up their rows in
+    order (four rows at once up to 1024 wide): 300000 / 1024 = 293 rows, 4 waves, then the partial rows, sixteen waves of 64:
+    8 in order in each of 8 sums, 3 joins, 16 in order. 324 roundings of 2^-24 are 2e-5 of the magnitudes summed, and each
+    row's own values are off by 1e-5: 3e-5."""
+    from vesper.kernels.layer_norm import layer_norm
+
+    m, d = size
+    gen = torch.Generator(GPU).manual_seed(d)
+    x, dy = (torch.randn(m, d, device=GPU, generator=gen).to(t) for t in types)
+    gain, bias = torch.rand(d, device=GPU, generator=gen).requires_grad_(), torch.zeros(d, device=GPU, requires_grad=True)
+    dgain, dbias = torch.autograd.grad(layer_norm(x, gain, bias, dtype=types[1]), [gain, bias], dy)
+    want = [torch.zeros(d, dtype=torch.float64) for _ in range(4)]
+    for part in range(0, m, 10000):
+        xs, gs = x[part : part + 10000].cpu().double(), dy[part : part + 10000].cpu().double()
+        xh = (xs - xs.mean(-1, keepdim=True)) / torch.sqrt(xs.var(-1, correction=0, keepdim=True) + 1e-5)
+        for total, term in zip(want, (gs * xh, gs, (gs * xh).abs(), gs.abs())):
+            total += term.sum(0)
+    assert float((dgain.cpu().double() - want[0]).norm()) <= 3e-5 * float(want[2].norm())
+    assert float((dbias.cpu().double() - want[1]).norm()) <= 2e-5 * float(want[3].norm())
