@@ -22,6 +22,7 @@ from typing import Any
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from vesper.contracts import ContractError, Dims, check_shape, refuse_tangents
@@ -185,7 +186,8 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
             kernel runs.
     """
     dims = _check(q, k, v, beta, g, state, ("b", "n", "h"))
-    refuse_tangents(q, k, v, beta, g, state)
+    if forward_ad._current_level >= 0:  # noqa: SLF001
+        refuse_tangents(q, k, v, beta, g, state)
     if active is not None:
         check_shape("active", active, ("b", "n"), dims, torch.bool)
     if dims["n"] == 0:
@@ -234,7 +236,8 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
             while grad mode is on.
     """
     dims = _check(q, k, v, beta, g, state, ("b", "h"))
-    refuse_tangents(q, k, v, beta, g, state)
+    if forward_ad._current_level >= 0:  # noqa: SLF001
+        refuse_tangents(q, k, v, beta, g, state)
     if torch.is_grad_enabled():
         _refuse_grad(q, k, v, beta, g, state)
     b, h, dk = q.shape
@@ -245,40 +248,33 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
     given = out_state is not None
     if out_state is None:
         out_state = torch.empty_like(state)
-    else:
+    elif out_state is not state:
         check_shape("out_state", out_state, ("b", "h", "dk", "dk"), dims, STATE_DTYPE)
         if out_state.device != q.device or not out_state.is_contiguous():
             raise ContractError("out_state must be a contiguous tensor on q's device")
-        apart = abs(out_state.data_ptr() - state.data_ptr())
         if out_state.requires_grad and torch.is_grad_enabled():
             raise ContractError("out_state must not require a gradient: the step writes it in place")
-        if 0 < apart < state.nbytes:
+        if 0 < abs(out_state.data_ptr() - state.data_ptr()) < state.nbytes:
             raise ContractError("out_state must be state itself or not overlap it")
     q, k, v, beta, g = q.contiguous(), k.contiguous(), v.contiguous(), beta.contiguous(), g.contiguous()
-    if given and b * h:  # other workgroups would still read what one has written
-        first, row = out_state.data_ptr(), b * h * q.element_size()
-        behind = first + 4 * b * h * dk * dk
-        for t, size in ((q, row * dk), (k, row * dk), (v, row * dk), (beta, row), (g, 4 * b * h)):
-            at = t.data_ptr()
-            if at < behind and first < at + size:
-                raise ContractError("out_state must not overlap q, k, v, beta or g")
     mask = None if active is None else _active_mask(active, ("b",), dims, q.device)
     o = torch.empty_like(q)
     if b == 0 or h == 0:
         return o, out_state
+    qp, kp, vp, bp, gp, to = q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(), g.data_ptr(), out_state.data_ptr()
+    if given:  # a workgroup would write what others are yet to read
+        strength = (2 if q.dtype is torch.bfloat16 else 4) * b * h  # bytes of beta; of q, k and v dk times as many
+        behind, token = to + 4 * b * h * dk * dk, strength * dk
+        if ((qp < behind and to < qp + token) or (kp < behind and to < kp + token) or (vp < behind and to < vp + token)
+                or (bp < behind and to < bp + strength) or (gp < behind and to < gp + 4 * b * h)):
+            raise ContractError("out_state must not overlap q, k, v, beta or g")
     if b * h <= MAX_STEP_HEADS:
-        _launch_step(q, k, v, beta, g, state, out_state, o, mask)
+        _lib.launch(q.device, _STEP[q.dtype], qp, kp, vp, bp, gp, state.data_ptr(), to, o.data_ptr(),
+                    None if mask is None else mask.data_ptr(), b, h, dk)
         return o, out_state
     rows = MAX_STEP_HEADS // h
     for i in range(0, b, rows):
-        part = slice(i, i + rows)
-        _launch_step(q[part], k[part], v[part], beta[part], g[part], state[part], out_state[part], o[part],
-                     None if mask is None else mask[part])
+        part = [t[i : i + rows] for t in (q, k, v, beta, g, state, out_state, o, *(() if mask is None else (mask,)))]
+        _lib.launch(q.device, _STEP[q.dtype], *(t.data_ptr() for t in part), *(() if mask is not None else (None,)),
+                    part[0].shape[0], h, dk)
     return o, out_state
-
-
-def _launch_step(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, state: Tensor, out_state: Tensor, o: Tensor,
-                 mask: Tensor | None) -> None:
-    b, h, dk = q.shape
-    _lib.launch(q.device, _STEP[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), beta.data_ptr(), g.data_ptr(),
-                state.data_ptr(), out_state.data_ptr(), o.data_ptr(), None if mask is None else mask.data_ptr(), b, h, dk)

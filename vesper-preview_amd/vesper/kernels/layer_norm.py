@@ -13,6 +13,7 @@ from typing import Any
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from vesper.contracts import ContractError, refuse_tangents
@@ -116,7 +117,8 @@ def layer_norm(x: Tensor, gain: Tensor, bias: Tensor | None = None, *, residual:
     """
     out = x.dtype if dtype is None else dtype
     d = _check(x, gain, bias, residual, eps, out)
-    refuse_tangents(x, gain, bias, residual)
+    if forward_ad._current_level >= 0:  # noqa: SLF001
+        refuse_tangents(x, gain, bias, residual)
     grad = torch.is_grad_enabled() and (x.requires_grad or gain.requires_grad or (bias is not None and bias.requires_grad)
                                         or (residual is not None and residual.requires_grad))
     if x.numel() == 0 or not grad:
