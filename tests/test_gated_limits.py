@@ -74,6 +74,14 @@ def test_the_limits_themselves_are_taken(size):
         _check_sizes(*size)
 
 
+def test_the_records_are_of_whole_tiles():
+    from vesper.kernels import _lib
+
+    lib = _lib.library()
+    for dk, wide in ((8, 16), (16, 16), (24, 32), (40, 48), (136, 144), (256, 256)):
+        assert lib.vsp_gated_scan_records_bytes(3, 70, 5, dk) == 3 * 5 * 2 * 4 * wide * (wide + 64)
+
+
 def test_the_c_entries_refuse_as_many_chunks():
     from vesper.kernels import _lib
 

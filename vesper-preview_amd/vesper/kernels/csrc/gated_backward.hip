@@ -504,7 +504,8 @@ template <typename T, int DP> struct GradShape {
 // Bound by memory: 122 KB a chunk and head of width 64 (half of it the four records), B16 T1024 H12 d64 113 us for 375 MB (3.3
 // TB/s), B2 T1500 H8 d128 39 us for 160 MB. With four waves for all it was 227 us (286 registers, one workgroup a CU), with
 // eight 127, with the pairs' products formed once and no register spilled 107; the decays' gradients by the terms around
-// each token, with Q K^T and K K^T of the lower tiles once more, take 6 of the 113 (2.5 of the 39).
+// each token, with Q K^T and K K^T of the lower tiles once more, take 6 of the 113 (2.5 of the 39, and 2 of the 10.7 of B32 T88
+// H2 d16 in float32).
 // Waves 0 to 3 hold dQ and Y of the 16 tokens w, waves 4 to 7 C. What comes from memory for the next 32 value columns is in
 // flight while those in LDS are multiplied.
 template <typename T, int DP>

@@ -506,8 +506,8 @@ template <typename T, int DP> struct OutIn {
 
 // A chunk is three dependent products and three barriers, about 2300 cycles: K H 800 (of it 120 the barrier), T R 850, K^T
 // Delta 500, in each the reads of the operands from LDS, the MFMAs of the pieces, and the split of the result into pieces. So
-// the time is the chunks' number times 0.9 us (B1 T8191 H12 d64, 48 workgroups) to 1.3 us (B8 T4096 H8 d64, 256 of them: 94 us;
-// the clock falls to 2.1 GHz, and one XCD is slower by a fifth). With records the writes bound it: B16 T1024 H12 d64 52 us
+// the time is the chunks' number times 0.9 us (B1 T8191 H12 d64, 48 workgroups) to 1.5 us (B8 T4096 H8 d64, 256 of them: 94 us
+// for 64; the clock falls to 2.1 GHz, and one XCD is slower by a fifth). With records the writes bound it: B16 T1024 H12 d64 52 us
 // without and 96 with them (290 MB, past what the 256 MB cache behind the L2s holds). What brought it there, at B1: operands
 // in pieces through LDS between four waves instead of all in one wave's registers (208 us), direct loads into LDS (150), W
 // for the outputs, T into registers, two chunks ahead, loads spread over the spans, reads issued together (118).

@@ -11,7 +11,8 @@ and ``active`` mask these functions share: no query scaling, keys already normal
 - ``gated_delta_step``: one token per row, for decoding (``vsp_gated_step_*``), forward only.
 
 bfloat16 inputs run bf16 MFMA, with everything that is computed in float32 and multiplied again as the sum of three
-bf16 numbers (24 bits): the states and the decays' gradients come out as exact as float32 arithmetic gives them.
+bf16 numbers (24 bits; in the outputs' products two): the states and the decays' gradients come out as exact as float32 sums
+give them, the latter behind strong decays too (every term of a decay's gradient carries that decay).
 float32 inputs run float32 MFMA.
 """
 
@@ -172,7 +173,8 @@ def gated_delta_scan(q: Tensor, k: Tensor, v: Tensor, beta: Tensor, g: Tensor, s
         ``n == 0`` the (empty) ``q`` tensor itself and the same ``state`` object.
 
     Under autograd the gradients of ``q, k, v, beta, g`` and ``state`` come from the backward kernels; the forward
-    then keeps each chunk's starting state and corrections, ``4 dk (dk + 64)`` bytes a chunk and head. Widths that
+    then keeps each chunk's starting state and corrections, ``4 w (w + 64)`` bytes a chunk and head, ``w`` being ``dk`` rounded
+    up to a multiple of 16. Widths that
     are no multiple of 8 run zero-padded to the next, which changes no output. One token without autograd runs as
     ``gated_delta_step``. The backward may be captured into a graph, as long as no eager graph of the same leaves is alive
     (torch's accumulation into them would leave the capture). A NaN or an infinity in a token reaches its head's outputs from the start of its chunk on (a
